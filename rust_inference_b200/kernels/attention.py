@@ -13,6 +13,8 @@
   the plain form of the score
   anything else                  the generic kernel (`attention_generic`): any head size, any
                                  dtype, float32 arithmetic
+  a cache in 8 bits              the pages that a step looks at are read back into scratch in the run dtype, which the
+                                 kernels above then take (`_over_quantized`)
 
 Besides causality a mixer may limit a query's keys to the last `window` keys or to the query's own
 chunk of positions.  The tensor-core kernels take either as one signed span (`csrc/common.cuh:
@@ -22,10 +24,11 @@ from __future__ import annotations
 
 import functools
 import os
+from typing import NamedTuple
 
 import torch
 
-from . import ops
+from . import ops, quantized_cache
 
 
 @functools.lru_cache(maxsize=None)
@@ -129,7 +132,12 @@ def attention(qkv, cache_layer, out, ctx, *, n_heads, n_kv_heads, head_dim, scal
     both limits at once are the generic kernel's.
     `softcap`, `keep_first`, `sink`, `dist`, `gate`: a cap on the scores, first positions that stay visible beyond
     the window, a term without key in the softmax's denominator, a bias by distance and a gate per head on the
-    result (see `ops.attention_generic`)."""
+    result (see `ops.attention_generic`).  cache_layer: a layer in the run dtype, or one in 8 bits
+    (`quantized_cache.QuantizedPages`)."""
+    if quantized_cache.is_quantized(cache_layer):
+        return _over_quantized(qkv, cache_layer, out, ctx, n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, scale=scale,
+                               window=window, chunk=chunk, v_head_dim=v_head_dim, out_scale=out_scale, softcap=softcap,
+                               keep_first=keep_first, sink=sink, dist=dist, gate=gate)
     q_ld = qkv.shape[1]
     same_sizes = v_head_dim is None or v_head_dim == head_dim
     plain = not (softcap or keep_first or sink is not None or dist is not None or gate is not None)
@@ -222,6 +230,37 @@ def attention(qkv, cache_layer, out, ctx, *, n_heads, n_kv_heads, head_dim, scal
         head_dim=head_dim, page_size=ctx.page_size, scale=scale, window=window, chunk=chunk or 0,
         v_head_dim=v_head_dim, out_scale=out_scale, softcap=softcap, keep_first=keep_first, sink=sink, dist=dist,
         gate=gate)
+
+
+# Rows (new tokens times query heads per kv head) of a sequence up to which a bfloat16 step reads the codes themselves
+QUANTIZED_ROWS = 64
+
+
+def _over_quantized(qkv, layer, out, ctx, *, window, chunk, keep_first, **forms):
+    """`attention` over a cache in 8 bits."""
+    plain = not (forms["softcap"] or keep_first or any(forms[n] is not None for n in ("sink", "dist", "gate"))) and not (window and chunk)
+    heads, kv, hd = forms["n_heads"], forms["n_kv_heads"], forms["head_dim"]
+    if (plain and quantized_cache.attention_supports(qkv.dtype, hd, forms["v_head_dim"])
+            and (qkv.dtype == torch.float32 or ctx.max_new * (heads // kv) <= QUANTIZED_ROWS)):
+        floats, ints = quantized_cache.attention_workspace(qkv.shape[0], heads, kv, hd, ctx.max_new)
+        return quantized_cache.attention(
+            qkv, layer, out, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens, n_heads=heads, n_kv_heads=kv, head_dim=hd,
+            max_new=ctx.max_new, scale=forms["scale"], part=ctx.buffer("quantized_part", (floats,), torch.float32),
+            arrived=ctx.zeroed_buffer("quantized_arrived", (ints,), torch.int32), span=window if window else -int(chunk or 0),
+            out_scale=forms["out_scale"])
+    k = ctx.buffer("readback_k", layer.k.shape, qkv.dtype)
+    v = ctx.buffer("readback_v", layer.v.shape, qkv.dtype)
+    # (a captured step may run with longer sequences than it was captured with)
+    longest = ctx.page_table.shape[1] * ctx.page_size if ctx.all_single else ctx.max_len
+    quantized_cache.read(layer, k, v, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.seq_len, max_len=longest,
+                         seen_span=0 if keep_first else (window if window else -int(chunk or 0)))
+    return attention(qkv, _Pages(k, v), out, ctx, window=window, chunk=chunk, keep_first=keep_first, **forms)
+
+
+class _Pages(NamedTuple):
+    """Keys and values in the run dtype, as the kernels take them."""
+    k: torch.Tensor
+    v: torch.Tensor
 
 
 class FormedHeads:

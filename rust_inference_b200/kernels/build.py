@@ -42,6 +42,9 @@ MODULES = {
     "parallel_streams": "parallel_streams.cu",
     "state_scan": "state_scan.cu",
     "short_conv": "short_conv.cu",
+    "quantized_cache": "quantized_cache.cu",
+    "attention_quantized": "attention_quantized.cu",
+    "token_logprobs": "token_logprobs.cu",
     "wait_probe": "wait_probe.cu",
     "host_runtime": "host_runtime.cpp",
 }

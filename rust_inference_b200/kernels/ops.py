@@ -10,12 +10,14 @@ import ctypes
 from ctypes import c_int, c_float, c_void_p, c_longlong, c_ulonglong
 
 import math
+from typing import NamedTuple
 
 import torch
 
 from .build import load
 
 RI_F32, RI_BF16 = 0, 1
+TOKEN_LOGPROBS_MOST = 64     # alternatives per row of `token_logprobs`
 _DTYPE_CODE = {torch.float32: RI_F32, torch.bfloat16: RI_BF16}
 
 
@@ -641,6 +643,32 @@ def sample(logits: torch.Tensor, out: torch.Tensor, *, temperature: float, top_k
           c_ulonglong(seed & 0xFFFFFFFFFFFFFFFF), _p(row_stream), _p(row_counter), c_int(counter_offset),
           c_void_p(mirror.data_ptr() if mirror is not None else 0), _p(newest), _p(seed_dev), _stream())
     return out
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor              # float32 [R]
+    entropy: torch.Tensor              # float32 [R], in nats
+    top_ids: torch.Tensor | None       # int32 [R, top], likeliest first
+    top_logprobs: torch.Tensor | None  # float32 [R, top]
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0) -> TokenLogprobs:
+    """ln softmax(logits[r])[targets[r]], the entropy of softmax(logits[r]) and, with top > 0, the row's likeliest tokens with
+    their log probabilities.  logits: float32 or bfloat16 [R, V], rows any distance apart; targets: int32 [R] (an id outside the
+    vocabulary, as -1: log probability NaN).  Logits of minus infinity are tokens that cannot come; a row with a NaN, plus
+    infinity or nothing else has no distribution, and its results are NaN.  Equal logits rank by their id."""
+    _need_cuda(logits, targets)
+    _need(logits.dim() == 2 and logits.dtype in _DTYPE_CODE and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1),
+          "token_logprobs: logits must be float32 or bfloat16 [rows, vocabulary] with neighbours side by side")
+    rows, vocab = logits.shape
+    _need(targets.dtype == torch.int32 and targets.is_contiguous() and targets.numel() == rows, "token_logprobs: targets must be int32 [rows]")
+    _need(0 <= top <= min(vocab, TOKEN_LOGPROBS_MOST), f"token_logprobs: 0 to {TOKEN_LOGPROBS_MOST} alternatives, at most the vocabulary")
+    logprob, entropy = torch.empty(2, rows, dtype=torch.float32, device=logits.device)
+    ids = torch.empty(rows, top, dtype=torch.int32, device=logits.device) if top else None
+    best = torch.empty(rows, top, dtype=torch.float32, device=logits.device) if top else None
+    _call("token_logprobs", "ri_token_logprobs", _p(logits), c_int(dtype_code(logits.dtype)), c_longlong(logits.stride(0)), c_int(rows),
+          c_int(vocab), _p(targets), c_int(top), _p(logprob), _p(entropy), _p(ids), _p(best), _stream())
+    return TokenLogprobs(logprob, entropy, ids, best)
 
 
 def cast(src: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

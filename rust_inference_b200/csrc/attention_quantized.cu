@@ -161,8 +161,8 @@ template <> __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16*
 __device__ __forceinline__ float merge_weight(float m, float top) { return exp2f(m - (top == -INFINITY ? 0.f : top)); }
 __device__ __forceinline__ float unit_ratio(float s, float most) { return s == most ? 1.f : s / most; }      // (both 0: 1; s NaN never is the unit)
 
-constexpr int ring_bytes(int hd) { return WARPS * STAGES * (2 * BLOCK * hd + 16); }
-constexpr int smem_bytes(int hd, int rows_cap) { return ring_bytes(hd) + WARPS * rows_cap * (hd + 4) * 4 + WARPS * ROWS * 16; }
+template <int HD> constexpr int RING_BYTES = WARPS * STAGES * (2 * BLOCK * HD + 16);
+template <int HD> int smem_bytes(int rows_cap) { return RING_BYTES<HD> + WARPS * rows_cap * (HD + 4) * 4 + WARPS * ROWS * 16; }
 
 template <int HD, typename T, int TERMS>
 __global__ void __launch_bounds__(THREADS)
@@ -170,7 +170,6 @@ attn_quantized_kernel(const Args a) {
     constexpr int KS = HD / 16;                  // steps of a score's contraction
     constexpr int NT = HD / 8;                   // column tiles of the result
     constexpr int TILE = BLOCK * HD;             // bytes of 16 keys
-    constexpr int RING = ring_bytes(HD);
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int sums[THREADS + 1];
     __shared__ int found[2];
@@ -271,7 +270,7 @@ attn_quantized_kernel(const Args a) {
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) fetch();
 
-    float* so = reinterpret_cast<float*>(smem + RING);                       // [WARPS][rows_cap][HD + 4]
+    float* so = reinterpret_cast<float*>(smem + RING_BYTES<HD>);                       // [WARPS][rows_cap][HD + 4]
     float4* sml = reinterpret_cast<float4*>(so + WARPS * a.rows_cap * (HD + 4));       // [WARPS][ROWS]
     int slot = 0;
     for (int u = u0; u < u1;) {
@@ -557,8 +556,8 @@ template <int HD, typename T, int TERMS>
 int launch(const Args& a, int blocks, cudaStream_t stream) {
     static PerDeviceOnce once;
     auto kernel = attn_quantized_kernel<HD, T, TERMS>;
-    if (raise_dynamic_smem(kernel, smem_bytes(HD, ROWS), once, "attention_quantized")) return 1;
-    return check_launch(launch_dependent(kernel, dim3((unsigned)blocks), dim3(THREADS), (size_t)smem_bytes(HD, a.rows_cap), stream, a),
+    if (raise_dynamic_smem(kernel, smem_bytes<HD>(ROWS), once, "attention_quantized")) return 1;
+    return check_launch(launch_dependent(kernel, dim3((unsigned)blocks), dim3(THREADS), (size_t)smem_bytes<HD>(a.rows_cap), stream, a),
                         "attention_quantized");
 }
 

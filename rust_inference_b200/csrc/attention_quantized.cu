@@ -1,28 +1,35 @@
 // Attention over a cache in 8 bits (quantized_cache.cu) for steps of few query rows: single tokens, drafted tokens, short
-// continuations; head sizes 64 and 128.  It reads codes and scales as they lie in the cache, each once per 16 query rows.
+// continuations; head sizes 64 and 128.  It reads codes and scales as they lie in the cache, each once per tile of query rows.
 //
 // The mathematics.  With key codes c_j of scale s_j, value codes d_j of scale t_j, both the same for the 16 positions of a block:
 //   score_j = scale s_j (q . c_j),  out = sum_j w_j t_j d_j / sum_j w_j,  w_j = 2^(score_j log2 e - m)
-// over the keys 0..pos of the token's slot within its span (common.cuh: first_visible_key).  Codes are whole numbers up to 127, so
-// as float16 numbers they are exact, and the products run on the tensor cores (m16n8k16, float32 sums) without a rounding of keys
-// or values:
-//   - a row of q is brought to [2^14, 2^15) by a power of two and cut into one float16 number per channel, for float32
-//     queries into two (the second holds what the first left over).  A bfloat16 number has 8 significant bits, float16 has 11:
-//     the first one is exact, down to 2^-28 of the row's largest number;
-//   - a weight times 2^14 times t_j over the largest t so far of the warp is at most 2^14: as float16 it is rounded to
-//     2^-12 relative (two numbers for float32: 2^-23), whatever its size down to 2^-28 of the largest.  The sums run
-//     in units of that t; when a larger one comes, they are brought to it as they are to a new maximum.
+// over the keys 0..pos of the token's slot within its span (common.cuh: first_visible_key).  Codes enter the tensor cores' products
+// exactly, so that keys and values are rounded nowhere:
+//   - scores are sums of whole numbers (m16n8k32, int8): a row of q is brought to +-127 256 and rounded to whole numbers of
+//     two signed bytes, q = 256 d1 + d0 (float32: +-127 65536, three bytes), 2^-16 (2^-24) of the row's largest
+//     number; codes times bytes add up in 32 bits without a rounding.  The codes are operands as they lie in memory;
+//   - results are sums of weights in float16 (m16n8k16, float32 sums; for float32 two float16 numbers each, the second what
+//     the first left over) times codes.  A weight times t_j over the largest t so far of the warp is rounded to 2^-12 (2^-23)
+//     relative, down to 2^-20 of the largest; the sums run in units of that t, and when a larger one comes, they are brought to
+//     it as they are to a new maximum.  A code c becomes float16 by its bits: 1024 + 128 + c has the byte c + 128 as its low one.
+//     With one number per weight the products are taken of 1152 + c, one byte permutation for two codes, and a product of the same
+//     weights with -1152 follows each of them (float32 sums of that size are off by 2^-23 1152 = 1.4e-4 of a code); with two numbers
+//     1152 is taken off the codes.
 //
-// The work.  A unit is one page (64 keys) of one kv head for a tile of 16 rows (row = token * n_rep + head of the kv head).  The
-// units of a step, sequence by sequence, are cut into equal runs, one per thread block: however unequal the sequences are, all
-// blocks have the same to read.  A block's four warps take 16 keys of each page each, every warp with a ring of its own that
-// cp.async fills (no barrier inside a run).  An item (sequence, kv head, tile) that lies in one block is finished there; one that
-// spreads over several is written as partial sums, and the block that arrives last (a counter per item) adds them up in the
-// order of the blocks, so that the result does not depend on who was last.
+// The products are taken with codes as the rows of the MMA, 16 keys (scores) or 16 channels (result), and the query rows as its
+// columns, 8 at a time: a code is made a float16 number once for all rows, and the usual 4 to 8 query heads of a kv head fill the
+// columns, where they left half of 16 rows empty.
 //
-// Fragments come straight from 16-byte reads of shared memory, because the order of a contraction's terms is free: lane (g, t) of
-// a product holds of key g the channels t HD/4 .. + HD/4, of its four keys (2t, 2t + 1, 2t + 8, 2t + 9) the channels g HD/8 ..
-// + HD/8, and of the result's row g the channels t HD/4 .. + HD/4 again.
+// The work.  A unit is one page (64 keys) of one kv head for a tile of 8 or 16 rows (row = token * n_rep + head of the kv head).
+// The units of a step, sequence by sequence, are cut into equal runs, one per thread block: however unequal the sequences are,
+// all blocks have the same to read.  A block's four warps take half of one of two pages each at a time, every warp with a ring of its
+// own that cp.async fills (no barrier inside a run).  An item (sequence, kv head, tile) that lies in one block is finished there;
+// one that spreads over several is written as partial sums, which the blocks that arrive last (a counter per eight parts) add up
+// in the order of the blocks, so that the result does not depend on who was last.
+//
+// Fragments come straight from 16-byte reads of shared memory, because the order of a contraction's terms, and which channel is which
+// row of a product, are free: lane (g, t) holds of the keys g and g + 8 the channels t HD/4 .. + HD/4, of its four keys (2t,
+// 2t + 1, 2t + 8, 2t + 9) the channels g HD/8 .. + HD/8, and of the result's rows 2t and 2t + 1 those channels again.
 #include "common.cuh"
 
 #include <cuda_fp16.h>
@@ -31,8 +38,19 @@ using namespace ri;
 
 namespace {
 
-constexpr int PAGE = 64, BLOCK = 16, WARPS = 4, THREADS = 32 * WARPS, ROWS = 16, STAGES = 4;
-constexpr float BIAS = 14.f;                     // weights are formed times 2^14
+constexpr int PAGE = 64, BLOCK = 16, WARPS = 4, THREADS = 32 * WARPS;
+constexpr int STEP = 2 * BLOCK;                  // keys that a warp takes at a time
+constexpr int MOST_BLOCKS = 5;                   // thread blocks per SM, at most
+// What an item costs a block beside its pages (queries fetched, warps joined, the result written), in pages
+constexpr int SETUP = 2;
+// ... and what a block has at least
+constexpr int LEAST = 1;
+// Parts of an item are added up eight at a time: a block that arrives last of eight adds theirs and goes on with seven others
+constexpr int GROUP = 8;
+// Weights are formed times 2^6 against a reference that follows the row's maximum only when that is 2^8 times ahead: they stay below
+// 2^14, which float16 holds, and sums are brought to a new reference a few times per row instead of at most steps.
+constexpr float BIAS = 6.f, AHEAD = 8.f;
+constexpr float LOWEST = -1.7e38f;               // the reference of a row without keys
 
 struct Args {
     const void* q;
@@ -49,7 +67,8 @@ struct Args {
     float out_scale;
     float* part;                                 // [2 * blocks][rows_cap][HD]
     float4* stat;                                // [2 * blocks][rows_cap]: maximum, sum, unit of the sums
-    int* arrived;                                // per item, zero between calls
+    int* arrived;                                // [4][2 * blocks] (8^4 parts are more than there are blocks), zero between calls
+    int places;                                  // 2 * blocks
     int rows_cap;                                // rows of a tile that any item fills
 };
 
@@ -58,33 +77,37 @@ struct Item {
     int seq, head, tile;                         // kv head, tile of rows
     int low, end;                                // its pages
     int first_tok, start, n_rows, tiles;
+    int first_key, last_pos;                     // the keys that any row of the sequence sees
+    const int* table;                            // its pages' numbers
 };
 
-__device__ __forceinline__ int pages_of(const Args& a, int start, int n_tok, int& low) {
-    low = first_visible_key(start, a.span) / PAGE;
-    return n_tok > 0 ? (start + n_tok - 1) / PAGE + 1 - low : 0;
+__device__ __forceinline__ int units_of(const Args& a, int seq, int rows) {
+    const int n = a.cu_seqlens[seq + 1] - a.cu_seqlens[seq], start = a.seq_start[seq];
+    return n > 0 ? ((start + n - 1) / PAGE + 1 - first_visible_key(start, a.span) / PAGE + SETUP) * a.n_kv * ((n * a.n_rep + rows - 1) / rows) : 0;
 }
-__device__ __forceinline__ int units_of(const Args& a, int seq) {
-    const int n = a.cu_seqlens[seq + 1] - a.cu_seqlens[seq];
-    int low;
-    return pages_of(a, a.seq_start[seq], n, low) * a.n_kv * ((n * a.n_rep + ROWS - 1) / ROWS);
-}
-__device__ __forceinline__ void enter(const Args& a, int seq, Item& it) {
+__device__ __forceinline__ void enter(const Args& a, int seq, int rows, Item& it) {
     it.seq = seq;
     it.first_tok = a.cu_seqlens[seq];
     const int n = a.cu_seqlens[seq + 1] - it.first_tok;
     it.start = a.seq_start[seq];
     it.n_rows = n * a.n_rep;
-    it.tiles = (it.n_rows + ROWS - 1) / ROWS;
-    it.end = pages_of(a, it.start, n, it.low) + it.low;
+    it.tiles = (it.n_rows + rows - 1) / rows;
+    it.first_key = first_visible_key(it.start, a.span);
+    it.last_pos = it.start + n - 1;
+    it.low = it.first_key / PAGE;
+    it.end = n > 0 ? it.last_pos / PAGE + 1 : it.low;
+    int slot = a.seq_slot[seq];
+    // checked build: a slot outside is recorded, slot 0 read in its place
+    if (!RI_IN_LIMIT(slot, RI_LIMIT_SLOTS, RI_CHECK_SLOT)) slot = 0;
+    it.table = a.page_table + (size_t)slot * a.max_pages;
 }
 // the item after this one (there is one)
-__device__ __forceinline__ void next_item(const Args& a, Item& it) {
+__device__ __forceinline__ void next_item(const Args& a, int rows, Item& it) {
     if (++it.tile < it.tiles) return;
     it.tile = 0;
     if (++it.head < a.n_kv) return;
     it.head = 0;
-    do enter(a, it.seq + 1, it); while (it.n_rows == 0);
+    do enter(a, it.seq + 1, rows, it); while (it.n_rows == 0);
 }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -99,9 +122,10 @@ template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("c
 // Sixteen-byte pieces lie in lines of 128 bytes; piece p of line l at p ^ swizzle(l), so that the reads below meet no bank twice.
 template <int HD> __device__ __forceinline__ int swizzle(int line) { return HD == 128 ? line & 7 : (line & 3) << 1; }
 
-// two codes (bytes `pick` of w, offset by 128) as float16 numbers: 1024 + code + 128 by its bits, less 1152
+// Two codes (bytes `pick` of w, offset by 128) as float16 numbers: 1024 + 128 + code by its bits, and the code itself
+__device__ __forceinline__ uint32_t offset_halves(uint32_t w, uint32_t pick) { return __byte_perm(w, 0x64646464u, pick); }
 __device__ __forceinline__ uint32_t halves(uint32_t w, uint32_t pick) {
-    const uint32_t u = __byte_perm(w, 0x64646464u, pick);
+    const uint32_t u = offset_halves(w, pick);
     const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&v);
 }
@@ -110,7 +134,25 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+// an 8 x 8 matrix of 16-bit numbers, two neighbours of a row per lane, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t w;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(w) : "r"(v));
+    return w;
+}
+// 2^x by the hardware's instruction: 2 units in the last place
+__device__ __forceinline__ float two_to(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
+// the same of whole numbers, 32 terms
+__device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -158,29 +200,37 @@ template <> __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16*
 }
 
 // What several partial results of a row are weighted with: maxima m, sums l, units s of their values
-__device__ __forceinline__ float merge_weight(float m, float top) { return exp2f(m - (top == -INFINITY ? 0.f : top)); }
+__device__ __forceinline__ float merge_weight(float m, float top) { return two_to(m - top); }
 __device__ __forceinline__ float unit_ratio(float s, float most) { return s == most ? 1.f : s / most; }      // (both 0: 1; s NaN never is the unit)
 
-template <int HD> constexpr int RING_BYTES = WARPS * STAGES * (2 * BLOCK * HD + 16);
-template <int HD> int smem_bytes(int rows_cap) { return RING_BYTES<HD> + WARPS * rows_cap * (HD + 4) * 4 + WARPS * ROWS * 16; }
+template <int HD> constexpr int OWN_BYTES = 2 * STEP * HD + 16;         // a warp's keys, values, two scales of each
+// ... and what it sums up: in the place of its last values (8 rows), or beside them
+template <int HD, int NQ> constexpr int PART_BYTES = NQ == 1 ? 0 : 8 * NQ * HD * 4;
+template <int HD, int NQ> constexpr int SMEM_BYTES = WARPS * (OWN_BYTES<HD> + PART_BYTES<HD, NQ> + 8 * NQ * 16);
 
-template <int HD, typename T, int TERMS>
-__global__ void __launch_bounds__(THREADS)
+// NQ: tiles of 8 query rows; TERMS: float16 numbers per weight, TERMS + 1 bytes per query channel
+template <int HD, typename T, int TERMS, int NQ>
+__global__ void __launch_bounds__(THREADS, TERMS * NQ == 1 ? 4 : 2)
 attn_quantized_kernel(const Args a) {
-    constexpr int KS = HD / 16;                  // steps of a score's contraction
-    constexpr int NT = HD / 8;                   // column tiles of the result
+    constexpr int ROWS = 8 * NQ;
+    constexpr int KS = HD / 16;                  // four-channel pieces of a key per lane
+    constexpr int DIGITS = TERMS + 1;
+    constexpr int CT = HD / 16;                  // tiles of 16 channels of the result
     constexpr int TILE = BLOCK * HD;             // bytes of 16 keys
+    constexpr int OWN = OWN_BYTES<HD>, PART = PART_BYTES<HD, NQ>;
+    static_assert(PART > 0 || ROWS * HD * 4 <= 2 * TILE, "a warp's sums fit where its values were");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int sums[THREADS + 1];
     __shared__ int found[2];
     __shared__ int last_here;
+    __shared__ float4 sgroup[GROUP][ROWS];       // statistics of parts that are added up
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     let_next_kernel_start();
 
-    // ---- this block's run of units ----
+    // ---- this block's run of units (lengths, slots and pages are fixed before the step) ----
     const int per = (a.n_seqs + THREADS - 1) / THREADS;
     int mine = 0;
-    for (int s = tid * per; s < min((tid + 1) * per, a.n_seqs); ++s) mine += units_of(a, s);
+    for (int s = tid * per; s < min((tid + 1) * per, a.n_seqs); ++s) mine += units_of(a, s, ROWS);
     sums[tid + 1] = mine;
     if (tid == 0) sums[0] = 0;
     __syncthreads();
@@ -199,284 +249,355 @@ attn_quantized_kernel(const Args a) {
         for (int i = 0; i < 4; ++i) sums[4 * lane + 1 + i] = v[i] + before;
     }
     __syncthreads();
-    const long long total = sums[THREADS];
-    const int blocks = (int)min((long long)gridDim.x, total), me = blockIdx.x;
+    const int total = sums[THREADS], blocks = min((int)gridDim.x, (total + LEAST - 1) / LEAST), me = blockIdx.x;
     if (me >= blocks) {
         wait_for_previous_kernels();             // (who waits for this kernel waits for those before it too)
         return;
     }
-    const int u0 = (int)(total * me / blocks), u1 = (int)(total * (me + 1) / blocks);
+    auto run_start = [&](int b) { return (int)((long long)total * b / blocks); };
+    const int u0 = run_start(me), u1 = run_start(me + 1);
     if (sums[tid] <= u0 && u0 < sums[tid + 1]) {
         int at = sums[tid], s = tid * per;
-        for (int n; at + (n = units_of(a, s)) <= u0; ++s) at += n;
+        for (int n; at + (n = units_of(a, s, ROWS)) <= u0; ++s) at += n;
         found[0] = s;
         found[1] = at;
     }
     __syncthreads();
     Item it;
-    enter(a, found[0], it);
-    int page;
+    enter(a, found[0], ROWS, it);
+    int page, u;                                 // the next page, and its place among the units
     {
-        const int within = u0 - found[1], n = it.end - it.low;
-        page = it.low + within % n;
+        const int within = u0 - found[1], n = it.end - it.low + SETUP, at = within % n;
         it.tile = within / n % it.tiles;
         it.head = within / n / it.tiles;
+        page = it.low + max(at - SETUP, 0);
+        u = u0 + max(SETUP - at, 0);
     }
-    wait_for_previous_kernels();
+    if (u >= u1) {
+        wait_for_previous_kernels();
+        return;
+    }
 
-    // ---- the ring ----
-    unsigned char* ring = smem + warp * STAGES * (2 * TILE + 16);
-    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    // ---- half a page at a time: keys are on their way while values are worked on, values while scores are ----
+    unsigned char* kt = smem + warp * OWN;
+    unsigned char* vt = kt + 2 * TILE;
+    const float* scales = reinterpret_cast<const float*>(kt + 4 * TILE);
+    const uint32_t k_to = (uint32_t)__cvta_generic_to_shared(kt);
+    // where this lane's pieces go (those of odd runs of 32: 4 pieces further on in the swizzle), and where it reads: keys g and
+    // g + 8, pieces 2t and 2t + 1 (64 channels: piece t); keys 2t and 2t + 1 (and 8 on), piece g (64 channels: half of piece g / 2)
+    const int put = ((lane >> 3) * 8 + ((lane & 7) ^ swizzle<HD>(lane >> 3))) * 16, put_odd = put ^ (HD == 128 ? 64 : 0);
+    const int k_at = HD == 128 ? (g * 8 + ((2 * t) ^ g)) * 16 : ((g >> 1) * 8 + (((g & 1) * 4 + t) ^ swizzle<HD>(g >> 1))) * 16;
+    const int v_at = HD == 128 ? (2 * t * 8 + (g ^ (2 * t))) * 16 : (t * 8 + ((g >> 1) ^ swizzle<HD>(t))) * 16 + (g & 1) * 8;
+    const int v_at_1 = HD == 128 ? ((2 * t + 1) * 8 + (g ^ (2 * t + 1))) * 16 : (t * 8 + ((4 + (g >> 1)) ^ swizzle<HD>(t))) * 16 + (g & 1) * 8;
+    const int my_page = warp >> 1, my_half = (warp & 1) * STEP;
     Item ahead = it;
-    int ahead_page = page, ahead_u = u0, ahead_slot = 0;
+    // (ahead_u: where the item's pages would begin, also if an earlier block has its first ones)
+    int ahead_u = u - (page - it.low), ahead_page = page, ahead_stop = min(it.end, page + (u1 - u));
     auto number_of = [&](const Item& i, int p) {
-        const int slot = a.seq_slot[i.seq];
-        // checked build: a slot or a page index outside is recorded, page 0 read in its place
-        if (!RI_IN_LIMIT(slot, RI_LIMIT_SLOTS, RI_CHECK_SLOT) || !RI_IN_RANGE(p, a.max_pages, RI_CHECK_PAGE_INDEX)) return 0;
-        return a.page_table[(size_t)slot * a.max_pages + p];
+        if (p >= i.end || !RI_IN_RANGE(p, a.max_pages, RI_CHECK_PAGE_INDEX)) return 0;     // checked build: recorded, page 0 read in its place
+        return i.table[p];
     };
-    int ahead_number = number_of(ahead, ahead_page);
-    auto fetch = [&]() {
-        if (ahead_u < u1) {
-            const int base = ahead_page * PAGE + warp * BLOCK;
-            // 16 keys that no row of the sequence sees are left out
-            if (base <= ahead.start + (ahead.n_rows - 1) / a.n_rep && base + BLOCK > first_visible_key(ahead.start, a.span)) {
+    int ahead_number = number_of(ahead, ahead_page + my_page);
+    size_t v_tile = 0;                           // where the values lie that belong to the keys fetched last
+    bool v_there = false;
+    wait_for_previous_kernels();
+    auto fetch_keys = [&]() {
+        v_there = false;
+        if (ahead_page < ahead_stop) {
+            const int base = (ahead_page + my_page) * PAGE + my_half;
+            // half a page that no row of the sequence sees is left out
+            if (ahead_page + my_page < ahead_stop && base <= ahead.last_pos && base + STEP > ahead.first_key) {
                 int number = ahead_number;
-                if (!RI_IN_LIMIT(number, RI_LIMIT_PAGES, RI_CHECK_PAGE)) number = 0;    // checked build: recorded, read from a page that exists
-                const size_t tile = (size_t)number * a.n_kv + ahead.head;
-                const int8_t* k = a.kc + (tile * PAGE + warp * BLOCK) * HD;
-                const int8_t* v = a.vc + (tile * PAGE + warp * BLOCK) * HD;
-                const uint32_t to = ring_at + ahead_slot * (2 * TILE + 16);
+                if (!RI_IN_LIMIT(number, RI_LIMIT_PAGES, RI_CHECK_PAGE)) number = 0;
+                v_there = true;
+                v_tile = (size_t)number * a.n_kv + ahead.head;
+                const int8_t* k = a.kc + (v_tile * PAGE + my_half) * HD + lane * 16;
 #pragma unroll
-                for (int i = 0; i < HD / 32; ++i) {
-                    const int piece = i * 32 + lane, line = piece >> 3;
-                    const uint32_t at = to + (line * 8 + ((piece & 7) ^ swizzle<HD>(line))) * 16;
-                    copy16(at, k + piece * 16);
-                    copy16(at + TILE, v + piece * 16);
-                }
-                if (lane < 2) copy4(to + 2 * TILE + 4 * lane, (lane ? a.vs : a.ks) + tile * (PAGE / BLOCK) + warp);
+                for (int i = 0; i < HD / 16; ++i) copy16(k_to + (i & 1 ? put_odd : put) + i * 512, k + i * 512);
+                if (lane < 2) copy4(k_to + 4 * TILE + 4 * lane, a.ks + v_tile * (PAGE / BLOCK) + my_half / BLOCK + lane);
             }
-            if (++ahead_u < u1) {
-                if (++ahead_page == ahead.end) {
-                    next_item(a, ahead);
-                    ahead_page = ahead.low;
-                }
-                ahead_number = number_of(ahead, ahead_page);
+            ahead_page += 2;
+            if (ahead_page >= ahead_stop && ahead_stop == ahead.end && (ahead_u += SETUP + ahead.end - ahead.low) < u1) {
+                next_item(a, ROWS, ahead);
+                ahead_page = ahead.low;
+                ahead_stop = min(ahead.end, ahead.low + (u1 - ahead_u));
             }
-            ahead_slot = ahead_slot + 1 == STAGES ? 0 : ahead_slot + 1;
+            if (ahead_page < ahead_stop) ahead_number = number_of(ahead, ahead_page + my_page);
         }
         copies_commit();
     };
+    auto fetch_values = [&]() {
+        if (v_there) {
+            const int8_t* v = a.vc + (v_tile * PAGE + my_half) * HD + lane * 16;
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) fetch();
+            for (int i = 0; i < HD / 16; ++i) copy16(k_to + 2 * TILE + (i & 1 ? put_odd : put) + i * 512, v + i * 512);
+            if (lane < 2) copy4(k_to + 4 * TILE + 8 + 4 * lane, a.vs + v_tile * (PAGE / BLOCK) + my_half / BLOCK + lane);
+        }
+        copies_commit();
+    };
+    fetch_keys();
 
-    float* so = reinterpret_cast<float*>(smem + RING_BYTES<HD>);                       // [WARPS][rows_cap][HD + 4]
-    float4* sml = reinterpret_cast<float4*>(so + WARPS * a.rows_cap * (HD + 4));       // [WARPS][ROWS]
-    int slot = 0;
-    for (int u = u0; u < u1;) {
+    // a warp's sums [WARPS][ROWS][HD] and their rows' statistics [WARPS][ROWS]
+    auto part_at = [&](int w) { return reinterpret_cast<float*>(smem + (PART ? WARPS * OWN + w * PART : w * OWN + 2 * TILE)); };
+    float4* sml = reinterpret_cast<float4*>(smem + WARPS * (OWN + PART));
+    while (true) {
         // ---- an item's part in this block: pages page .. stop - 1 ----
         const int stop = min(it.end, page + (u1 - u));
         const int row0 = it.tile * ROWS, here = min(ROWS, it.n_rows - row0);
         const bool whole = page == it.low && stop == it.end;
-        const int item_u0 = u - (page - it.low), item_n = it.end - it.low;
+        const int item_u = u - (page - it.low), item_n = it.end - it.low;        // the item's pages among the units
 
-        // queries: rows g and g + 8 of the tile, as float16 numbers
-        uint32_t qa[TERMS][KS][4];
-        float unit[2];                           // what a score's sum is multiplied by (without the keys' scale)
-        int pos[2], low[2];
+        // queries: bytes of row 8 n + g of the tile
+        uint32_t qd[DIGITS][NQ][KS];
+        // ... and of the rows 8 n + 2t + r, whose scores this lane has: what a sum of products is multiplied by (without the keys'
+        // scale), position and first visible key
+        float unit[NQ][2];
+        int pos[NQ][2], low[NQ][2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = row0 + g + 8 * r;
+        for (int n = 0; n < NQ; ++n) {
+            const int row = row0 + 8 * n + g;
             const bool there = row < it.n_rows;
-            pos[r] = there ? it.start + row / a.n_rep : -1;
-            low[r] = there ? first_visible_key(pos[r], a.span) : 0;
-            float x[KS][4], top = 0.f;
             const T* src = reinterpret_cast<const T*>(a.q) + (size_t)(it.first_tok + (there ? row / a.n_rep : 0)) * a.q_ld +
                            (size_t)(it.head * a.n_rep + (there ? row % a.n_rep : 0)) * HD + t * (HD / 4);
+            float x[KS][4], top = 0.f;
+            bool fine = true;
 #pragma unroll
-            for (int i = 0; i < KS; ++i) load4<T>(src + 4 * i, a.q_vec, x[i]);
+            for (int i = 0; i < KS; ++i) {
+                load4<T>(src + 4 * i, a.q_vec, x[i]);
+                if (!there) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;       // its scores stay 0, its result is not written
+            }
 #pragma unroll
             for (int i = 0; i < KS; ++i)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) top = fmaxf(top, fabsf(x[i][c]));
+                for (int c = 0; c < 4; ++c) {
+                    top = fmaxf(top, fabsf(x[i][c]));
+                    fine &= fabsf(x[i][c]) < INFINITY;
+                }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // the power of two that brings the largest number to [2^14, 2^15); numbers below 2^-112 are brought less far
-            const int e = max((int)(__float_as_uint(top) >> 23) - 127, -112);
-            const float up = __uint_as_float((uint32_t)(127 + 14 - min(e, 127)) << 23), down = __uint_as_float((uint32_t)max(127 - 14 + e, 1) << 23);
-            unit[r] = down * (a.scale * 1.4426950408889634f);
+            constexpr float MOST = TERMS == 1 ? 127.f * 256.f : 127.f * 65536.f;
+            constexpr int HALF = TERMS == 1 ? 0x8080 : 0x808080;               // makes the bytes of a number its signed digits
+            const float size = fmaxf(top, 7.9e-31f), up = MOST / size;         // (a row below 2^-100 is 0)
+            // a row with an infinity or a NaN has no scores
+            float down = size * (1.f / MOST) * (a.scale * 1.4426950408889634f);
+            fine = (__ballot_sync(0xffffffffu, fine) >> (lane & 28) & 15u) == 15u;
+            if (!fine) down = __int_as_float(0x7fffffff);
 #pragma unroll
-            for (int i = 0; i < KS; ++i)
+            for (int i = 0; i < KS; ++i) {
+                uint32_t d[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float y0 = x[i][2 * h] * up, y1 = x[i][2 * h + 1] * up;
-                    const uint32_t first = pack(y0, y1);
-                    qa[0][i][2 * h + r] = first;
-                    if (TERMS == 2) {
-                        const float2 f = unpack(first);
-                        qa[TERMS - 1][i][2 * h + r] = pack(y0 - f.x, y1 - f.y);
-                    }
-                }
+                for (int c = 0; c < 4; ++c) d[c] = (uint32_t)(__float2int_rn(x[i][c] * up) + HALF) ^ HALF;
+                const uint32_t lo01 = __byte_perm(d[0], d[1], 0x5140), lo23 = __byte_perm(d[2], d[3], 0x5140);
+                qd[0][n][i] = __byte_perm(lo01, lo23, 0x5410);
+                qd[1][n][i] = __byte_perm(lo01, lo23, 0x7632);
+                if (DIGITS == 3) qd[DIGITS - 1][n][i] = __byte_perm(__byte_perm(d[0], d[1], 0x0062), __byte_perm(d[2], d[3], 0x0062), 0x5410);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int mine = row0 + 8 * n + 2 * t + r;
+                unit[n][r] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + r));
+                pos[n][r] = mine < it.n_rows ? it.start + mine / a.n_rep : -1;
+                low[n][r] = mine < it.n_rows ? first_visible_key(pos[n][r], a.span) : 0;
+            }
         }
 
-        float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, most = 0.f, inverse = 0.f;
+        float o[NQ][CT][4], m[NQ][2], l[NQ][2], most = 0.f, inverse = 0.f;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        for (int n = 0; n < NQ; ++n) {
+            m[n][0] = m[n][1] = LOWEST;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < CT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+        }
         const int last_pos = it.start + (row0 + here - 1) / a.n_rep;
         const int first_pos = it.start + row0 / a.n_rep, first_key = first_visible_key(first_pos, a.span);
         const int last_low = first_visible_key(last_pos, a.span);
 
-        for (; page < stop; ++page, ++u) {
-            __syncwarp();                        // every lane has read what the next copies overwrite
-            fetch();
-            copies_wait<STAGES - 1>();
-            __syncwarp();
-            const unsigned char* kt = ring + slot * (2 * TILE + 16);
-            const unsigned char* vt = kt + TILE;
-            const float* scales = reinterpret_cast<const float*>(kt + 2 * TILE);
-            slot = slot + 1 == STAGES ? 0 : slot + 1;
-            const int base = page * PAGE + warp * BLOCK;
-            if (base > last_pos || base + BLOCK <= first_key) continue;
+        u += stop - page;
+        for (; page < stop; page += 2) {
+            __syncwarp();                        // every lane has read the values that the next ones overwrite
+            fetch_values();
+            copies_wait<1>();
+            __syncwarp();                        // the keys are there
+            const int base = (page + my_page) * PAGE + my_half;
+            if (page + my_page >= stop || base > last_pos || base + STEP <= first_key) {
+                fetch_keys();
+                copies_wait<1>();                // values that nobody wants have landed before the next ones are sent for
+                continue;
+            }
 
-            // scores of 16 rows and 16 keys
-            float s[2][4];
+            // scores of the keys g (s[..][0], [1]) and g + 8 ([2], [3]) of two blocks for the rows 2t and 2t + 1
+            float s[2][NQ][4];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-                uint32_t w[KS];
-                const int key = 8 * j + g;
+                uint32_t w[2][KS];
 #pragma unroll
-                for (int i = 0; i < KS / 4; ++i) {
-                    const int line = HD == 128 ? key : key >> 1, piece = HD == 128 ? 2 * t + i : (key & 1) * 4 + t;
-                    *reinterpret_cast<uint4*>(w + 4 * i) = *reinterpret_cast<const uint4*>(kt + (line * 8 + (piece ^ swizzle<HD>(line))) * 16);
-                }
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < KS; ++i) {
-                    const uint32_t c = w[i] ^ 0x80808080u;
-                    const uint32_t b0 = halves(c, 0x4140), b1 = halves(c, 0x4342);
+                    for (int i = 0; i < KS / 4; ++i)
+                        *reinterpret_cast<uint4*>(w[h] + 4 * i) = *reinterpret_cast<const uint4*>(kt + (i ? k_at ^ 16 : k_at) + h * (TILE / 2) + j * TILE);
+                const float k_scale = scales[j];
 #pragma unroll
-                    for (int x = 0; x < TERMS; ++x) mma(s[j], qa[x][i], b0, b1);
-                }
-            }
-            const float k_scale = scales[0], v_scale = scales[1];
-            const bool edge = base + BLOCK - 1 > first_pos || base < last_low || here < ROWS;
-            float alpha[2];
-            bool moved = false;
+                for (int n = 0; n < NQ; ++n) {
+                    int c[DIGITS][4];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float f = k_scale * unit[r];
-                float top = -INFINITY;
+                    for (int d = 0; d < DIGITS; ++d) c[d][0] = c[d][1] = c[d][2] = c[d][3] = 0;
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                    for (int i = 0; i < KS; i += 2)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int key = base + 8 * j + 2 * t + c;
-                        float& v = s[j][2 * r + c];
-                        v *= f;
-                        if (edge && !(key <= pos[r] && key >= low[r])) v = -INFINITY;
-                        top = fmaxf(top, v);
+                        for (int d = 0; d < DIGITS; ++d) mma_s8(c[d], w[0][i], w[1][i], w[0][i + 1], w[1][i + 1], qd[d][n][i], qd[d][n][i + 1]);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        float v = (float)(c[1][x] * 256 + c[0][x]);
+                        if (DIGITS == 3) v = fmaf((float)c[DIGITS - 1][x], 65536.f, v);
+                        s[j][n][x] = v * (k_scale * unit[n][x & 1]);
                     }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float m_new = fmaxf(m[r], top), ref = m_new == -INFINITY ? 0.f : m_new;
-                alpha[r] = exp2f(m[r] - ref);
-                moved |= m_new != m[r];
-                m[r] = m_new;
-                float sum = 0.f;
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float& v = s[j][2 * r + c];
-                        v = exp2f(v - (ref - BIAS));
-                        sum += v;
-                    }
-                l[r] = l[r] * alpha[r] + sum;
-            }
-            if (v_scale > most) {                // a larger unit for the sums (of this warp: all lanes alike)
-                const float f = most * (1.f / v_scale);
-                alpha[0] *= f;
-                alpha[1] *= f;
-                moved = true;
-                most = v_scale;
-                inverse = 1.f / v_scale;
-            }
-            if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    o[i][0] *= alpha[0];
-                    o[i][1] *= alpha[0];
-                    o[i][2] *= alpha[1];
-                    o[i][3] *= alpha[1];
                 }
             }
-            // weights in units of `most`, as one or two float16 numbers
-            const float ratio = v_scale == most ? 1.f : v_scale * inverse;
-            uint32_t pa[TERMS][4];
+            const bool edge = base + STEP - 1 > first_pos || base < last_low;
+            __syncwarp();                        // every lane has read the keys
+            fetch_keys();
+            if (edge) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int key = base + 16 * j + 8 * (x >> 1) + g;
+                            if (!(key <= pos[n][x & 1] && key >= low[n][x & 1])) s[j][n][x] = -INFINITY;
+                        }
+            }
+            // whether the rows' references are far behind
+            bool ahead_of[NQ];
+            float top[NQ][2];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                ahead_of[n] = false;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    float y0 = s[j][2 * r] * ratio, y1 = s[j][2 * r + 1] * ratio;
-                    if (edge) {                  // an unseen key's weight is 0 also beside a scale that is no number
-                        const int key = base + 8 * j + 2 * t;
-                        if (!(key <= pos[r] && key >= low[r])) y0 = 0.f;
-                        if (!(key + 1 <= pos[r] && key + 1 >= low[r])) y1 = 0.f;
-                    }
-                    const uint32_t first = pack(y0, y1);
-                    pa[0][2 * j + r] = first;
-                    if (TERMS == 2) {
-                        const float2 f = unpack(first);
-                        pa[TERMS - 1][2 * j + r] = pack(y0 - f.x, y1 - f.y);
-                    }
-                }
-            // values: four keys of this lane, four channels at a time
-            uint32_t w[4][HD / 32];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int key = 2 * t + (k & 1) + (k >> 1) * 8;
-                if (HD == 128) {
-                    *reinterpret_cast<uint4*>(w[k]) = *reinterpret_cast<const uint4*>(vt + (key * 8 + (g ^ swizzle<HD>(key))) * 16);
-                } else {
-                    const int line = key >> 1, piece = (key & 1) * 4 + (g >> 1);
-                    *reinterpret_cast<uint2*>(w[k]) =
-                        *reinterpret_cast<const uint2*>(vt + (line * 8 + (piece ^ swizzle<HD>(line))) * 16 + (g & 1) * 8);
+                    top[n][r] = fmaxf(fmaxf(s[0][n][r], s[0][n][2 + r]), fmaxf(s[1][n][r], s[1][n][2 + r]));
+                    ahead_of[n] |= top[n][r] > m[n][r] + AHEAD;
                 }
             }
+            copies_wait<1>();
+            __syncwarp();                        // the values are there
+            // a larger unit for the sums (of this warp: all lanes alike); a block that no row sees has no say
+            const float v0 = edge && !(base <= last_pos && base + BLOCK > first_key) ? 0.f : scales[2];
+            const float v1 = edge && !(base + BLOCK <= last_pos && base + STEP > first_key) ? 0.f : scales[3];
+            float shrink = 1.f;
+            if (fmaxf(v0, v1) > most) {
+                const float higher = fmaxf(v0, v1);
+                inverse = 1.f / higher;
+                shrink = most * inverse;
+                most = higher;
+            }
+            const float ratio[2] = {v0 == most ? 1.f : v0 * inverse, v1 == most ? 1.f : v1 * inverse};
+            uint32_t pb[2][TERMS][NQ][2];
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) {
+            for (int n = 0; n < NQ; ++n) {
+                if (__any_sync(0xffffffffu, ahead_of[n] || shrink != 1.f)) {
+                    float alpha[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t pick = h ? 0x7362 : 0x5140;
-                    const uint32_t x = __byte_perm(w[0][i], w[1][i], pick) ^ 0x80808080u, y = __byte_perm(w[2][i], w[3][i], pick) ^ 0x80808080u;
+                    for (int r = 0; r < 2; ++r) {
+                        float& most_of = top[n][r];
+                        most_of = fmaxf(most_of, __shfl_xor_sync(0xffffffffu, most_of, 4));
+                        most_of = fmaxf(most_of, __shfl_xor_sync(0xffffffffu, most_of, 8));
+                        most_of = fmaxf(most_of, __shfl_xor_sync(0xffffffffu, most_of, 16));
+                        const float m_new = fmaxf(m[n][r], most_of);
+                        alpha[r] = two_to(m[n][r] - m_new);
+                        m[n][r] = m_new;
+                        l[n][r] *= alpha[r];
+                        alpha[r] *= shrink;
+                    }
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const uint32_t b0 = halves(x, c ? 0x4342 : 0x4140), b1 = halves(y, c ? 0x4342 : 0x4140);
+                    for (int i = 0; i < CT; ++i) {
+                        o[n][i][0] *= alpha[0];
+                        o[n][i][1] *= alpha[1];
+                        o[n][i][2] *= alpha[0];
+                        o[n][i][3] *= alpha[1];
+                    }
+                }
 #pragma unroll
-                        for (int n = 0; n < TERMS; ++n) mma(o[4 * i + 2 * h + c], pa[n], b0, b1);
+                for (int j = 0; j < 2; ++j) {
+                    float y[4];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float ref = m[n][r] - BIAS, p0 = two_to(s[j][n][r] - ref), p1 = two_to(s[j][n][2 + r] - ref);
+                        l[n][r] += p0 + p1;
+                        y[r] = p0 * ratio[j];    // weights in units of `most`
+                        y[2 + r] = p1 * ratio[j];
+                    }
+                    if (edge) {                  // an unseen key's weight is 0 also beside a scale that is no number
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int key = base + 16 * j + 8 * (x >> 1) + g;
+                            if (!(key <= pos[n][x & 1] && key >= low[n][x & 1])) y[x] = 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t first = pack(y[2 * h], y[2 * h + 1]);
+                        pb[j][0][n][h] = transposed(first);
+                        if (TERMS == 2) {
+                            const float2 f = unpack(first);
+                            pb[j][TERMS - 1][n][h] = transposed(pack(y[2 * h] - f.x, y[2 * h + 1] - f.y));
+                        }
+                    }
+                }
+            }
+            // values: four keys of this lane in each block, four channels at a time
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t w[4][HD / 32];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const unsigned char* at = vt + (k & 1 ? v_at_1 : v_at) + (k >> 1) * (TILE / 2) + j * TILE;
+                    if (HD == 128) *reinterpret_cast<uint4*>(w[k]) = *reinterpret_cast<const uint4*>(at);
+                    else *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(at);
+                }
+#pragma unroll
+                for (int i = 0; i < CT; ++i) {
+                    const uint32_t pick = i & 1 ? 0x7362 : 0x5140;
+                    const uint32_t x = __byte_perm(w[0][i / 2], w[1][i / 2], pick) ^ 0x80808080u, y = __byte_perm(w[2][i / 2], w[3][i / 2], pick) ^ 0x80808080u;
+                    if (TERMS == 1) {
+                        const uint32_t v[4] = {offset_halves(x, 0x4140), offset_halves(x, 0x4342), offset_halves(y, 0x4140), offset_halves(y, 0x4342)};
+                        const uint32_t less[4] = {0xe480e480u, 0xe480e480u, 0xe480e480u, 0xe480e480u};       // -1152
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n) {
+                            mma(o[n][i], v, pb[j][0][n][0], pb[j][0][n][1]);
+                            mma(o[n][i], less, pb[j][0][n][0], pb[j][0][n][1]);
+                        }
+                    } else {
+                        const uint32_t v[4] = {halves(x, 0x4140), halves(x, 0x4342), halves(y, 0x4140), halves(y, 0x4342)};
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                            for (int k = 0; k < TERMS; ++k) mma(o[n][i], v, pb[j][k][n][0], pb[j][k][n][1]);
                     }
                 }
             }
         }
 
         // ---- the four warps' parts together ----
+        __syncwarp();
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            const int row = g + 8 * r;
-            if (t == 0) sml[warp * ROWS + row] = make_float4(m[r], l[r], most, 0.f);
-            if (row < here) {
-                // columns 2t and 2t + 1 of the tiles are the channels (2t) HD/8 + i and (2t + 1) HD/8 + i
-                float* to = so + (warp * a.rows_cap + row) * (HD + 4) + t * (HD / 4);
+        for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                for (int i = 0; i < NT; i += 4) {
-                    *reinterpret_cast<float4*>(to + i) = make_float4(o[i][2 * r], o[i + 1][2 * r], o[i + 2][2 * r], o[i + 3][2 * r]);
-                    *reinterpret_cast<float4*>(to + NT + i) =
-                        make_float4(o[i][2 * r + 1], o[i + 1][2 * r + 1], o[i + 2][2 * r + 1], o[i + 3][2 * r + 1]);
+            for (int r = 0; r < 2; ++r) {
+                float sum = l[n][r];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const int row = 8 * n + 2 * t + r;
+                if (g == 0) sml[warp * ROWS + row] = make_float4(m[n][r], sum, most, 0.f);
+                if (row < here) {
+                    float* to = part_at(warp) + row * HD + g * (HD / 8);
+#pragma unroll
+                    for (int i = 0; i < CT; i += 2)
+                        *reinterpret_cast<float4*>(to + 2 * i) = make_float4(o[n][i][r], o[n][i][2 + r], o[n][i + 1][r], o[n][i + 1][2 + r]);
                 }
             }
-        }
         __syncthreads();
         auto write = [&](int row, int d, float4 v, float sum, float s) {
             const float inv = 1.f / sum, f = s * a.out_scale;
@@ -485,11 +606,14 @@ attn_quantized_kernel(const Args a) {
             store4<T>(reinterpret_cast<T*>(a.out) + (size_t)(it.first_tok + row / a.n_rep) * a.out_ld +
                       (size_t)(it.head * a.n_rep + row % a.n_rep) * HD + d, a.out_vec, v);
         };
-        const int first_block = (int)(((item_u0 + 1ll) * blocks - 1) / total), last_block = (int)(((long long)(item_u0 + item_n) * blocks - 1) / total);
-        auto part_of = [&](int b) { return (size_t)(2 * b + (b == first_block && (int)(total * b / blocks) < item_u0 ? 1 : 0)) * a.rows_cap; };
+        auto block_of = [&](int x) { return (int)(((x + 1ll) * blocks - 1) / total); };
+        const int first_block = block_of(item_u), parts = block_of(item_u + item_n - 1) - first_block + 1;
+        // a block has two places: for an item whose pages began before its run (or with it), and for one whose began inside
+        const int first_place = 2 * first_block + (run_start(first_block) < item_u ? 1 : 0);
+        auto place_of = [&](int part) { return part == 0 ? first_place : 2 * (first_block + part); };
         for (int i = tid; i < here * (HD / 4); i += THREADS) {
             const int row = i / (HD / 4), d = i % (HD / 4) * 4;
-            float top = -INFINITY, s = 0.f, sum = 0.f;
+            float top = LOWEST, s = 0.f, sum = 0.f;
             float4 st[WARPS], v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
@@ -500,83 +624,135 @@ attn_quantized_kernel(const Args a) {
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
                 const float f = merge_weight(st[w].x, top), x = f * unit_ratio(st[w].z, s);
-                const float4 p = *reinterpret_cast<const float4*>(so + (w * a.rows_cap + row) * (HD + 4) + d);
+                const float4 p = *reinterpret_cast<const float4*>(part_at(w) + row * HD + d);
                 sum = fmaf(st[w].y, f, sum);
                 v = make_float4(fmaf(p.x, x, v.x), fmaf(p.y, x, v.y), fmaf(p.z, x, v.z), fmaf(p.w, x, v.w));
             }
             if (whole) {
                 write(row, d, v, sum, s);
             } else {
-                const size_t at = part_of(me) + row;
+                const size_t at = (size_t)place_of(me - first_block) * a.rows_cap + row;
                 *reinterpret_cast<float4*>(a.part + at * HD + d) = v;
                 if (d == 0) a.stat[at] = make_float4(top, sum, s, 0.f);
             }
         }
         if (!whole) {
-            __threadfence();
-            __syncthreads();
-            int* arrived = a.arrived + ((size_t)it.first_tok * a.n_rep + it.tile) * a.n_kv + it.head;
-            if (tid == 0) last_here = atomicAdd(arrived, 1) == last_block - first_block;
-            __syncthreads();
-            if (last_here) {
+            int n = parts, index = me - first_block, stride = 1;       // parts of this level, this block's among them, how far apart they lie
+            for (int level = 0;; ++level) {
+                const int lead = index / GROUP * GROUP, members = min(GROUP, n - lead);
                 __threadfence();
-                if (tid == 0) *arrived = 0;
-                for (int i = tid; i < here * (HD / 4); i += THREADS) {
-                    const int row = i / (HD / 4), d = i % (HD / 4) * 4;
-                    float top = -INFINITY, s = 0.f, sum = 0.f;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int b = first_block; b <= last_block; ++b) {
-                        const float4 st = __ldcg(a.stat + part_of(b) + row);
-                        top = fmaxf(top, st.x);
-                        s = fmaxf(s, st.z);
-                    }
-                    for (int b = first_block; b <= last_block; ++b) {
-                        const size_t at = part_of(b) + row;
-                        const float4 st = __ldcg(a.stat + at), p = __ldcg(reinterpret_cast<const float4*>(a.part + at * HD + d));
-                        const float f = merge_weight(st.x, top), x = f * unit_ratio(st.z, s);
-                        sum = fmaf(st.y, f, sum);
-                        v = make_float4(fmaf(p.x, x, v.x), fmaf(p.y, x, v.y), fmaf(p.z, x, v.z), fmaf(p.w, x, v.w));
-                    }
-                    write(row, d, v, sum, s);
+                __syncthreads();
+                int* arrived = a.arrived + level * a.places + place_of(lead * stride);
+                if (tid == 0) {
+                    last_here = atomicAdd(arrived, 1) == members - 1;
+                    if (last_here) *arrived = 0;
                 }
+                __syncthreads();
+                if (!last_here) break;
+                __threadfence();
+                const bool done = n <= GROUP;
+                // the parts' statistics, one per thread; what each part is weighted with, and the row's own
+                if (tid < GROUP * ROWS) {
+                    const int x = tid / ROWS, row = tid % ROWS;
+                    float4 st = make_float4(LOWEST, 0.f, 0.f, 0.f);
+                    if (x < members && row < here) st = __ldcg(a.stat + (size_t)place_of((lead + x) * stride) * a.rows_cap + row);
+                    sgroup[x][row] = st;
+                }
+                __syncthreads();
+                if (tid < here) {
+                    float top = LOWEST, s = 0.f, sum = 0.f;
+                    for (int x = 0; x < members; ++x) top = fmaxf(top, sgroup[x][tid].x), s = fmaxf(s, sgroup[x][tid].z);
+                    for (int x = 0; x < members; ++x) {
+                        const float f = merge_weight(sgroup[x][tid].x, top);
+                        sum = fmaf(sgroup[x][tid].y, f, sum);
+                        sgroup[x][tid].w = f * unit_ratio(sgroup[x][tid].z, s);
+                    }
+                    sml[tid] = make_float4(top, sum, s, 0.f);
+                }
+                __syncthreads();
+                constexpr int TWO = 2;           // places that a thread reads together
+                for (int i0 = tid; i0 < here * (HD / 4); i0 += TWO * THREADS) {
+                    float4 p[TWO][GROUP];
+#pragma unroll
+                    for (int z = 0; z < TWO; ++z) {
+                        const int i = i0 + z * THREADS, row = i / (HD / 4), d = i % (HD / 4) * 4;
+#pragma unroll
+                        for (int x = 0; x < GROUP; ++x) {
+                            p[z][x] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (x < members && row < here)
+                                p[z][x] = __ldcg(reinterpret_cast<const float4*>(a.part + ((size_t)place_of((lead + x) * stride) * a.rows_cap + row) * HD + d));
+                        }
+                    }
+#pragma unroll
+                    for (int z = 0; z < TWO; ++z) {
+                        const int i = i0 + z * THREADS, row = i / (HD / 4), d = i % (HD / 4) * 4;
+                        if (row >= here) continue;
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int x = 0; x < GROUP; ++x) {
+                            const float w = x < members ? sgroup[x][row].w : 0.f;
+                            v = make_float4(fmaf(p[z][x].x, w, v.x), fmaf(p[z][x].y, w, v.y), fmaf(p[z][x].z, w, v.z), fmaf(p[z][x].w, w, v.w));
+                        }
+                        if (done) write(row, d, v, sml[row].y, sml[row].z);
+                        // in the place of the first (its channels are this thread's; its statistics have been read)
+                        else *reinterpret_cast<float4*>(a.part + ((size_t)place_of(lead * stride) * a.rows_cap + row) * HD + d) = v;
+                    }
+                }
+                if (done) break;
+                if (tid < here) a.stat[(size_t)place_of(lead * stride) * a.rows_cap + tid] = sml[tid];
+                n = (n + GROUP - 1) / GROUP;
+                index = lead / GROUP;
+                stride *= GROUP;
             }
         }
+        if (stop != it.end || (u += SETUP) >= u1) break;
         __syncthreads();                         // the warps' parts have been read
-        if (u < u1) {
-            next_item(a, it);
-            page = it.low;
-        }
+        next_item(a, ROWS, it);
+        page = it.low;
     }
     copies_wait<0>();
 }
 
-int rows_cap(int n_rep, int max_new) { return n_rep * max_new < ROWS ? n_rep * max_new : ROWS; }
-
-template <int HD, typename T, int TERMS>
-int launch(const Args& a, int blocks, cudaStream_t stream) {
+template <int HD, typename T, int TERMS, int NQ>
+int launch(Args a, long long part_floats, cudaStream_t stream) {
     static PerDeviceOnce once;
-    auto kernel = attn_quantized_kernel<HD, T, TERMS>;
-    if (raise_dynamic_smem(kernel, smem_bytes<HD>(ROWS), once, "attention_quantized")) return 1;
-    return check_launch(launch_dependent(kernel, dim3((unsigned)blocks), dim3(THREADS), (size_t)smem_bytes<HD>(a.rows_cap), stream, a),
-                        "attention_quantized");
+    static std::atomic<int> resident[64];
+    auto kernel = attn_quantized_kernel<HD, T, TERMS, NQ>;
+    constexpr int smem = SMEM_BYTES<HD, NQ>;
+    if (raise_dynamic_smem(kernel, smem, once, "attention_quantized")) return 1;
+    // as many blocks as the device holds at once (asked once per device)
+    int dev = 0, per_sm = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64) per_sm = resident[dev].load(std::memory_order_relaxed);
+    if (per_sm == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, THREADS, smem) != cudaSuccess || per_sm <= 0) per_sm = 1;
+        if (per_sm > MOST_BLOCKS) per_sm = MOST_BLOCKS;
+        if (dev >= 0 && dev < 64) resident[dev].store(per_sm, std::memory_order_relaxed);
+    }
+    const int blocks = per_sm * sm_count();
+    if (part_floats < 2ll * blocks * a.rows_cap * (HD + 4)) return fail("attention_quantized: scratch of %lld numbers is too small", part_floats);
+    a.places = 2 * blocks;
+    a.stat = reinterpret_cast<float4*>(a.part);
+    a.part += (size_t)2 * blocks * a.rows_cap * 4;
+    return check_launch(launch_dependent(kernel, dim3((unsigned)blocks), dim3(THREADS), (size_t)smem, stream, a), "attention_quantized");
 }
 
 }  // namespace
 
-// Thread blocks of a step: two per SM
-RI_API int ri_attention_quantized_blocks() { return 2 * sm_count(); }
+// Thread blocks of a step, at most
+RI_API int ri_attention_quantized_blocks() { return MOST_BLOCKS * sm_count(); }
 
-// part: float32 [2 * blocks * min(16, n_rep * max_new) * (hd + 4)]; arrived: int32 [tokens * heads], zero, and left so.
+// part: float32 [2 * blocks * min(16, n_rep * max_new) * (hd + 4)]; arrived: int32 [4 * 2 * blocks], zero, and left so.
 RI_API int ri_attention_quantized(const void* q, int dtype, int q_ld, const int8_t* kc, const int8_t* vc, const float* ks, const float* vs,
                                   const int* page_table, int max_pages, const int* seq_slot, const int* seq_start, const int* cu_seqlens,
                                   void* out, int out_ld, int n_seqs, int max_new, int n_heads, int n_kv, int hd, float scale, int span,
-                                  float out_scale, float* part, int* arrived, int blocks, cudaStream_t stream) {
+                                  float out_scale, float* part, long long part_floats, int* arrived, cudaStream_t stream) {
     if (n_seqs <= 0 || max_new <= 0) return 0;
     if (hd != 64 && hd != 128) return fail("attention_quantized: heads of %d channels (64 or 128 wanted)", hd);
     if (n_kv <= 0 || n_heads % n_kv) return fail("attention_quantized: %d heads over %d kv heads", n_heads, n_kv);
     if ((uintptr_t)kc % 16 || (uintptr_t)vc % 16 || (uintptr_t)part % 16) return fail("attention_quantized: codes and scratch must lie on 16-byte boundaries");
     const long long rows = (long long)max_new * (n_heads / n_kv);
-    if ((long long)n_seqs * max_pages * n_kv * ((rows + ROWS - 1) / ROWS) > 0x7fffffff || rows > 0x7fffffff)
+    if ((long long)n_seqs * (max_pages + SETUP) * n_kv * ((rows + 7) / 8) > 0x7fffffff || rows > 0x7fffffff)
         return fail("attention_quantized: %d sequences of %d new tokens are too many", n_seqs, max_new);
     Args a = {};
     const int item = dtype == RI_F32 ? 4 : 2;
@@ -595,12 +771,16 @@ RI_API int ri_attention_quantized(const void* q, int dtype, int q_ld, const int8
     a.scale = scale;
     a.span = span;
     a.out_scale = out_scale;
-    a.rows_cap = rows_cap(a.n_rep, max_new);
-    a.stat = reinterpret_cast<float4*>(part);
-    a.part = part + (size_t)2 * blocks * a.rows_cap * 4;
+    a.part = part;
     a.arrived = arrived;
-    if (dtype == RI_F32) return hd == 64 ? launch<64, float, 2>(a, blocks, stream) : launch<128, float, 2>(a, blocks, stream);
-    if (dtype == RI_BF16) return hd == 64 ? launch<64, __nv_bfloat16, 1>(a, blocks, stream) : launch<128, __nv_bfloat16, 1>(a, blocks, stream);
+    // tiles of 8 rows where the step has no more, else of 16
+    const int nq = rows <= 8 ? 1 : 2;
+    a.rows_cap = (int)(rows < 8 * nq ? rows : 8 * nq);
+    if (dtype == RI_F32 && nq == 1) return hd == 64 ? launch<64, float, 2, 1>(a, part_floats, stream) : launch<128, float, 2, 1>(a, part_floats, stream);
+    if (dtype == RI_F32) return hd == 64 ? launch<64, float, 2, 2>(a, part_floats, stream) : launch<128, float, 2, 2>(a, part_floats, stream);
+    if (dtype == RI_BF16 && nq == 1)
+        return hd == 64 ? launch<64, __nv_bfloat16, 1, 1>(a, part_floats, stream) : launch<128, __nv_bfloat16, 1, 1>(a, part_floats, stream);
+    if (dtype == RI_BF16) return hd == 64 ? launch<64, __nv_bfloat16, 1, 2>(a, part_floats, stream) : launch<128, __nv_bfloat16, 1, 2>(a, part_floats, stream);
     return fail("attention_quantized: unknown dtype %d", dtype);
 }
 

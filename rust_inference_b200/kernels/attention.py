@@ -242,7 +242,7 @@ def _over_quantized(qkv, layer, out, ctx, *, window, chunk, keep_first, **forms)
     heads, kv, hd = forms["n_heads"], forms["n_kv_heads"], forms["head_dim"]
     if (plain and quantized_cache.attention_supports(qkv.dtype, hd, forms["v_head_dim"])
             and (qkv.dtype == torch.float32 or ctx.max_new * (heads // kv) <= QUANTIZED_ROWS)):
-        floats, ints = quantized_cache.attention_workspace(qkv.shape[0], heads, kv, hd, ctx.max_new)
+        floats, ints = quantized_cache.attention_workspace(heads, kv, hd, ctx.max_new)
         return quantized_cache.attention(
             qkv, layer, out, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens, n_heads=heads, n_kv_heads=kv, head_dim=hd,
             max_new=ctx.max_new, scale=forms["scale"], part=ctx.buffer("quantized_part", (floats,), torch.float32),

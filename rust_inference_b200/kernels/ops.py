@@ -657,16 +657,18 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0)
     their log probabilities.  logits: float32 or bfloat16 [R, V], rows any distance apart; targets: int32 [R] (an id outside the
     vocabulary, as -1: log probability NaN).  Logits of minus infinity are tokens that cannot come; a row with a NaN, plus
     infinity or nothing else has no distribution, and its results are NaN.  Equal logits rank by their id."""
-    _need_cuda(logits, targets)
-    _need(logits.dim() == 2 and logits.dtype in _DTYPE_CODE and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1),
-          "token_logprobs: logits must be float32 or bfloat16 [rows, vocabulary] with neighbours side by side")
+    _need(logits.is_cuda and targets.is_cuda and logits.dim() == 2 and logits.dtype in _DTYPE_CODE and logits.shape[1] > 0
+          and (logits.stride(1) == 1 or logits.shape[1] == 1), "token_logprobs: logits must be float32 or bfloat16 [rows, vocabulary] on the "
+          "device, neighbours side by side")
     rows, vocab = logits.shape
     _need(targets.dtype == torch.int32 and targets.is_contiguous() and targets.numel() == rows, "token_logprobs: targets must be int32 [rows]")
-    _need(0 <= top <= min(vocab, TOKEN_LOGPROBS_MOST), f"token_logprobs: 0 to {TOKEN_LOGPROBS_MOST} alternatives, at most the vocabulary")
-    logprob, entropy = torch.empty(2, rows, dtype=torch.float32, device=logits.device)
-    ids = torch.empty(rows, top, dtype=torch.int32, device=logits.device) if top else None
-    best = torch.empty(rows, top, dtype=torch.float32, device=logits.device) if top else None
-    _call("token_logprobs", "ri_token_logprobs", _p(logits), c_int(dtype_code(logits.dtype)), c_longlong(logits.stride(0)), c_int(rows),
+    _need(0 <= top <= min(vocab, TOKEN_LOGPROBS_MOST), "token_logprobs: too many alternatives, or fewer than none")
+    logprob, entropy = torch.empty((2, rows), dtype=torch.float32, device=logits.device).unbind()
+    ids = best = None
+    if top:
+        ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+        best = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
+    _call("token_logprobs", "ri_token_logprobs", _p(logits), c_int(_DTYPE_CODE[logits.dtype]), c_longlong(logits.stride(0)), c_int(rows),
           c_int(vocab), _p(targets), c_int(top), _p(logprob), _p(entropy), _p(ids), _p(best), _stream())
     return TokenLogprobs(logprob, entropy, ids, best)
 

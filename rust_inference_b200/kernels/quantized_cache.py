@@ -13,26 +13,51 @@ positions of a page and kv head, [pages, kv heads, 64 / BLOCK], keys and values 
 from __future__ import annotations
 
 import functools
-from ctypes import c_float, c_int
-from dataclasses import dataclass
+from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
 
 from .build import load
-from .ops import _call, _need, _need_cuda, _p, _stream, dtype_code
+from .ops import KernelError, _call, _stream, dtype_code
 
 PAGE_SIZE, BLOCK = 64, 16
 
+# The entry points' arguments, one letter each, told to ctypes once: plain numbers then go through without an object for each.
+_KINDS = {"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float}
+_SIGNATURES = {
+    ("quantized_cache", "ri_quantized_write"): "piipipipppipppppppiiiiiiiip",
+    ("quantized_cache", "ri_quantized_read"): "ppppppipippppiiiiiiip",
+    ("attention_quantized", "ri_attention_quantized"): "piipppppipppp" "iiiiiififplpp",
+}
 
-@dataclass
+
+@functools.lru_cache(maxsize=None)
+def _prepare(module: str, fn: str) -> None:
+    getattr(load(module), fn).argtypes = [_KINDS[k] for k in _SIGNATURES[module, fn]]
+
+
 class QuantizedPages:
     """One layer: k, v int8 [pages, kv heads, 64, head size] (values may have a head size of their own), k_scale, v_scale
-    float32 [pages, kv heads, 4]."""
-    k: torch.Tensor
-    v: torch.Tensor
-    k_scale: torch.Tensor
-    v_scale: torch.Tensor
-    request: object = None
+    float32 [pages, kv heads, 4], contiguous and on one device.  The tensors are looked at here, once, and stay the layer's."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "request", "sizes", "pointers", "aligned", "device")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, request=None):
+        for t in (k, v, k_scale, v_scale):
+            if not t.is_cuda or t.device != k.device:
+                raise KernelError("a quantized layer's tensors lie on one CUDA device; this library has no CPU path")
+        if not (k.dtype == torch.int8 and v.dtype == torch.int8 and k.is_contiguous() and v.is_contiguous() and k.dim() == 4
+                and v.dim() == 4 and k.shape[2] == PAGE_SIZE and v.shape[:3] == k.shape[:3]):
+            raise KernelError(f"a quantized layer's codes are contiguous int8 [pages, kv heads, {PAGE_SIZE}, head size]")
+        scales = (k.shape[0], k.shape[1], PAGE_SIZE // BLOCK)
+        for t in (k_scale, v_scale):
+            if not (t.dtype == torch.float32 and t.is_contiguous() and tuple(t.shape) == scales):
+                raise KernelError(f"a quantized layer's scales are contiguous float32 {list(scales)}")
+        self.k, self.v, self.k_scale, self.v_scale, self.request = k, v, k_scale, v_scale, request
+        self.sizes = (k.shape[1], k.shape[3], v.shape[3])           # kv heads, head size, value head size
+        self.pointers = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        self.aligned = self.pointers[0] % 16 == 0 and self.pointers[1] % 16 == 0
+        self.device = k.device
 
 
 def empty_layer(n_pages: int, n_kv_heads: int, head_dim: int, v_head_dim: int | None = None, device="cuda") -> QuantizedPages:
@@ -46,20 +71,16 @@ def is_quantized(layer) -> bool:
     return isinstance(layer, QuantizedPages)
 
 
-def _need_layer(layer: QuantizedPages, n_kv_heads: int, head_dim: int, v_head_dim: int, what: str) -> None:
-    k, v = layer.k, layer.v
-    _need_cuda(k, v, layer.k_scale, layer.v_scale)
-    _need(k.dtype == torch.int8 and v.dtype == torch.int8 and k.is_contiguous() and v.is_contiguous() and k.dim() == 4 and v.dim() == 4
-          and k.shape[1:] == (n_kv_heads, PAGE_SIZE, head_dim) and v.shape[1:] == (n_kv_heads, PAGE_SIZE, v_head_dim)
-          and k.shape[0] == v.shape[0], f"{what}: codes must be contiguous int8 [pages, {n_kv_heads}, {PAGE_SIZE}, head size]")
-    scales = (k.shape[0], n_kv_heads, PAGE_SIZE // BLOCK)
-    for t in (layer.k_scale, layer.v_scale):
-        _need(t.dtype == torch.float32 and t.is_contiguous() and tuple(t.shape) == scales, f"{what}: scales must be float32 {list(scales)}")
+def _index(what: str, t: torch.Tensor, least: int) -> int:
+    """The address of an index array of at least so many entries."""
+    if t.dtype != torch.int32 or not t.is_cuda or t.numel() < least or not t.is_contiguous():
+        raise KernelError(f"{what}: index arrays are contiguous int32 on the device, {least} entries or more here")
+    return t.data_ptr()
 
 
-def _need_int32(what: str, *tensors) -> None:
-    for t in tensors:
-        _need(t is None or (t.dtype == torch.int32 and t.is_contiguous()), f"{what}: index arrays must be contiguous int32")
+def _need(good: bool, what: str, message: str) -> None:
+    if not good:
+        raise KernelError(f"{what}: {message}")
 
 
 def write(src: torch.Tensor, q_out: torch.Tensor | None, cos, sin, layer: QuantizedPages, page_table: torch.Tensor, seq_slot, seq_start,
@@ -74,23 +95,25 @@ def write(src: torch.Tensor, q_out: torch.Tensor | None, cos, sin, layer: Quanti
     what = "quantized_cache.write"
     v_hd = head_dim if v_head_dim is None else int(v_head_dim)
     rot = head_dim if rot_dims is None else int(rot_dims)
-    _need_cuda(src, q_out, cos, sin, page_table, seq_slot, seq_start, cu_seqlens, bias)
-    _need_layer(layer, n_kv_heads, head_dim, v_hd, what)
-    _need_int32(what, page_table, seq_slot, seq_start, cu_seqlens)
-    n_seqs = seq_slot.numel()
-    cols = (n_heads + n_kv_heads) * head_dim + n_kv_heads * v_hd
-    _need(src.dim() == 2 and src.is_contiguous() and src.shape[1] >= cols, f"{what}: a contiguous [tokens, {cols} or more] is wanted")
-    _need(seq_start.numel() >= n_seqs and cu_seqlens.numel() > n_seqs, f"{what}: one start per sequence and one offset more")
-    _need(q_out is None or (q_out.is_contiguous() and q_out.shape == (src.shape[0], n_heads * head_dim)
-                            and (q_out.dtype == src.dtype or src.dtype == torch.float32)), f"{what}: q_out must be [tokens, heads * head size]")
-    _need(rot == 0 or (cos.dtype == sin.dtype == torch.float32 and cos.shape[1] == rot // 2 and sin.shape == cos.shape
-                       and cos.is_contiguous() and sin.is_contiguous()), f"{what}: tables must be float32 [positions, rotated channels / 2]")
-    _need(bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() >= cols), f"{what}: bias must be float32 [columns]")
-    _call("quantized_cache", "ri_quantized_write", _p(src), c_int(dtype_code(src.dtype)), c_int(src.shape[1]), _p(bias),
-          c_int(1 if clear else 0), _p(q_out), c_int(dtype_code(src.dtype if q_out is None else q_out.dtype)), _p(cos), _p(sin),
-          _p(page_table), c_int(page_table.shape[1]), _p(seq_slot), _p(seq_start), _p(cu_seqlens), _p(layer.k), _p(layer.v),
-          _p(layer.k_scale), _p(layer.v_scale), c_int(n_seqs), c_int(max_new), c_int(n_heads), c_int(n_kv_heads), c_int(head_dim),
-          c_int(v_hd), c_int(rot), c_int(style), _stream())
+    n_seqs, cols = seq_slot.numel(), (n_heads + n_kv_heads) * head_dim + n_kv_heads * v_hd
+    _need(layer.sizes == (n_kv_heads, head_dim, v_hd), what, f"the layer has {layer.sizes[0]} kv heads of {layer.sizes[1:]} channels")
+    _need(src.is_cuda and src.dim() == 2 and src.is_contiguous() and src.shape[1] >= cols, what, "a contiguous [tokens, q | k | v columns] on the device is wanted")
+    _need(q_out is None or (q_out.is_cuda and q_out.is_contiguous() and q_out.shape == (src.shape[0], n_heads * head_dim)
+                            and (q_out.dtype == src.dtype or src.dtype == torch.float32)), what, "q_out must be [tokens, heads * head size]")
+    if rot:
+        _need(cos.is_cuda and sin.is_cuda and cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.dim() == 2
+              and cos.shape[1] * 2 == rot and sin.shape == cos.shape and cos.is_contiguous() and sin.is_contiguous(),
+              what, "tables must be float32 [positions, rotated channels / 2]")
+    _need(bias is None or (bias.is_cuda and bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() >= cols), what,
+          "bias must be float32 [columns]")
+    _need(page_table.dim() == 2, what, "the page table must be int32 [slots, pages]")
+    _prepare("quantized_cache", "ri_quantized_write")
+    k, v, ks, vs = layer.pointers
+    _call("quantized_cache", "ri_quantized_write", src.data_ptr(), dtype_code(src.dtype), src.shape[1], None if bias is None else bias.data_ptr(),
+          1 if clear else 0, None if q_out is None else q_out.data_ptr(), dtype_code(src.dtype if q_out is None else q_out.dtype),
+          cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, _index(what, page_table, 1), page_table.shape[1],
+          _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs), _index(what, cu_seqlens, n_seqs + 1), k, v, ks, vs, n_seqs,
+          max_new, n_heads, n_kv_heads, head_dim, v_hd, rot, style, _stream())
 
 
 def read(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, page_table: torch.Tensor, seq_slot, seq_first, seq_len, *,
@@ -101,36 +124,30 @@ def read(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, page_t
     longer.  seen_span: reading begins at the first key that a query at position seq_first[b] sees, of all keys (0), the last so many
     (> 0) or its own block of -span positions (< 0)."""
     what = "quantized_cache.read"
-    n_kv, hd, v_hd = layer.k.shape[1], layer.k.shape[3], layer.v.shape[3]
-    _need_cuda(k_out, v_out, page_table, seq_slot, seq_first, seq_len, cu_rows)
-    _need_layer(layer, n_kv, hd, v_hd, what)
-    _need_int32(what, page_table, seq_slot, seq_first, seq_len, cu_rows)
+    n_kv, hd, v_hd = layer.sizes
     n_seqs = seq_slot.numel()
-    _need(seq_first.numel() >= n_seqs and seq_len.numel() >= n_seqs and (cu_rows is None or cu_rows.numel() >= n_seqs),
-          f"{what}: one entry per sequence")
-    _need(k_out.dtype == v_out.dtype and k_out.is_contiguous() and v_out.is_contiguous(), f"{what}: outputs of one dtype, contiguous")
+    _need(k_out.is_cuda and v_out.is_cuda and k_out.dtype == v_out.dtype and k_out.is_contiguous() and v_out.is_contiguous(), what,
+          "outputs of one dtype, contiguous, on the device")
     if cu_rows is None:
-        _need(k_out.shape == layer.k.shape and v_out.shape == layer.v.shape, f"{what}: without cu_rows the outputs have the cache's shape")
+        _need(k_out.shape == layer.k.shape and v_out.shape == layer.v.shape, what, "without cu_rows the outputs have the cache's shape")
     else:
-        _need(k_out.dim() == 3 and k_out.shape[1:] == (n_kv, hd) and v_out.shape == (k_out.shape[0], n_kv, v_hd),
-              f"{what}: with cu_rows the outputs are [rows, kv heads, head size]")
-    _call("quantized_cache", "ri_quantized_read", _p(layer.k), _p(layer.v), _p(layer.k_scale), _p(layer.v_scale), _p(k_out), _p(v_out),
-          c_int(dtype_code(k_out.dtype)), _p(page_table), c_int(page_table.shape[1]), _p(seq_slot), _p(seq_first), _p(seq_len),
-          _p(cu_rows), c_int(n_seqs), c_int(max_len), c_int(n_kv), c_int(hd), c_int(v_hd),
-          c_int(0 if seen_span is None else 1), c_int(seen_span or 0), _stream())
+        _need(k_out.dim() == 3 and k_out.shape[1:] == (n_kv, hd) and v_out.shape == (k_out.shape[0], n_kv, v_hd), what,
+              "with cu_rows the outputs are [rows, kv heads, head size]")
+    _need(page_table.dim() == 2, what, "the page table must be int32 [slots, pages]")
+    _prepare("quantized_cache", "ri_quantized_read")
+    k, v, ks, vs = layer.pointers
+    _call("quantized_cache", "ri_quantized_read", k, v, ks, vs, k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype),
+          _index(what, page_table, 1), page_table.shape[1], _index(what, seq_slot, n_seqs), _index(what, seq_first, n_seqs),
+          _index(what, seq_len, n_seqs), None if cu_rows is None else _index(what, cu_rows, n_seqs), n_seqs, max_len, n_kv, hd, v_hd,
+          0 if seen_span is None else 1, seen_span or 0, _stream())
     return k_out, v_out
 
 
 @functools.lru_cache(maxsize=None)
-def _attention_blocks(device: int) -> int:
-    return int(load("attention_quantized").ri_attention_quantized_blocks())
-
-
-def attention_workspace(n_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int, max_new: int) -> tuple:
-    """(float32 numbers of scratch, int32 counters) that `attention` wants for a step of n_tokens; the counters are zero when it
-    begins, and when it ends."""
-    cap = min(16, max_new * (n_heads // n_kv_heads))
-    return 2 * _attention_blocks(torch.cuda.current_device()) * cap * (head_dim + 4), n_tokens * n_heads
+def attention_workspace(n_heads: int, n_kv_heads: int, head_dim: int, max_new: int) -> tuple:
+    """(float32 numbers of scratch, int32 counters) that `attention` wants; the counters are zero when it begins, and when it ends."""
+    blocks = int(load("attention_quantized").ri_attention_quantized_blocks())
+    return 2 * blocks * min(16, max_new * (n_heads // n_kv_heads)) * (head_dim + 4), 4 * 2 * blocks
 
 
 def attention_supports(dtype: torch.dtype, head_dim: int, v_head_dim: int | None) -> bool:
@@ -145,18 +162,18 @@ def attention(q: torch.Tensor, layer: QuantizedPages, out: torch.Tensor, page_ta
     steps of few tokens per sequence, and for float32.  q: rows whose leading n_heads * head_dim columns are the queries, rotated;
     span: > 0 the last so many keys, < 0 the keys of the query's own block of -span positions; part, arrived: `attention_workspace`."""
     what = "quantized_cache.attention"
-    _need_cuda(q, out, page_table, seq_slot, seq_start, cu_seqlens, part, arrived)
-    _need_layer(layer, n_kv_heads, head_dim, head_dim, what)
-    _need_int32(what, page_table, seq_slot, seq_start, cu_seqlens, arrived)
-    n_seqs = seq_slot.numel()
-    _need(q.dtype == out.dtype and attention_supports(q.dtype, head_dim, None) and q.dim() == 2 and out.dim() == 2 and q.stride(1) == 1
-          and out.stride(1) == 1 and q.shape[0] == out.shape[0] and min(q.shape[1], out.shape[1]) >= n_heads * head_dim,
-          f"{what}: queries and result must be float32 or bfloat16 [tokens, heads * 64 or 128]")
-    _need(n_heads % n_kv_heads == 0 and seq_start.numel() >= n_seqs and cu_seqlens.numel() > n_seqs, f"{what}: heads, or entries per sequence")
-    floats, ints = attention_workspace(q.shape[0], n_heads, n_kv_heads, head_dim, max_new)
-    _need(part.dtype == torch.float32 and part.is_contiguous() and part.numel() >= floats and arrived.numel() >= ints, f"{what}: scratch too small")
-    _call("attention_quantized", "ri_attention_quantized", _p(q), c_int(dtype_code(q.dtype)), c_int(q.stride(0)), _p(layer.k), _p(layer.v),
-          _p(layer.k_scale), _p(layer.v_scale), _p(page_table), c_int(page_table.shape[1]), _p(seq_slot), _p(seq_start), _p(cu_seqlens),
-          _p(out), c_int(out.stride(0)), c_int(n_seqs), c_int(max_new), c_int(n_heads), c_int(n_kv_heads), c_int(head_dim), c_float(scale),
-          c_int(span), c_float(out_scale), _p(part), _p(arrived), c_int(_attention_blocks(torch.cuda.current_device())), _stream())
+    n_seqs, width = seq_slot.numel(), n_heads * head_dim
+    _need(layer.sizes == (n_kv_heads, head_dim, head_dim) and layer.aligned, what, f"the layer has {layer.sizes[0]} kv heads of {layer.sizes[1:]} channels, or is not aligned")
+    _need(q.is_cuda and out.is_cuda and q.dtype == out.dtype and attention_supports(q.dtype, head_dim, None) and q.dim() == 2
+          and out.dim() == 2 and q.stride(1) == 1 and out.stride(1) == 1 and q.shape[0] == out.shape[0] and q.shape[1] >= width
+          and out.shape[1] >= width and n_heads % n_kv_heads == 0 and page_table.dim() == 2, what,
+          "queries and result must be float32 or bfloat16 [tokens, heads * 64 or 128] on the device")
+    floats, ints = attention_workspace(n_heads, n_kv_heads, head_dim, max_new)
+    _need(part.is_cuda and part.dtype == torch.float32 and part.is_contiguous() and part.numel() >= floats, what, "scratch too small")
+    _prepare("attention_quantized", "ri_attention_quantized")
+    k, v, ks, vs = layer.pointers
+    _call("attention_quantized", "ri_attention_quantized", q.data_ptr(), dtype_code(q.dtype), q.stride(0), k, v, ks, vs,
+          _index(what, page_table, 1), page_table.shape[1], _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs),
+          _index(what, cu_seqlens, n_seqs + 1), out.data_ptr(), out.stride(0), n_seqs, max_new, n_heads, n_kv_heads, head_dim, scale, span,
+          out_scale, part.data_ptr(), part.numel(), _index(what, arrived, ints), _stream())
     return out

@@ -347,13 +347,16 @@ def test_refusals():
     bad = [dict(src=rows[:, :-1]), dict(src=rows[:, :7 * 64].contiguous()), dict(src=rows.half()), dict(q_out=q.float()),
            dict(c=cos.double()), dict(c=cos[:, :31].contiguous()), dict(table=step.page_table.long()), dict(start=step.seq_start.cpu()),
            dict(head_dim=32), dict(n_kv_heads=1), dict(style=2), dict(bias=torch.zeros(8 * 64, device=DEV, dtype=torch.bfloat16)),
-           dict(rot_dims=63, c=cos[:, :31].contiguous(), s=sin[:, :31].contiguous()), dict(src=rows.cpu()),
-           dict(layer=qc.QuantizedPages(step.layer.k.float(), step.layer.v, step.layer.k_scale, step.layer.v_scale)),
-           dict(layer=qc.QuantizedPages(step.layer.k, step.layer.v, step.layer.k_scale[:, :, :2].contiguous(), step.layer.v_scale)),
-           dict(layer=qc.QuantizedPages(step.layer.k, step.layer.v, step.layer.k_scale, step.layer.v_scale.double()))]
+           dict(rot_dims=63, c=cos[:, :31].contiguous(), s=sin[:, :31].contiguous()), dict(src=rows.cpu())]
     for case in bad:
         with pytest.raises(KernelError):
             write(**case)
+    n = step.layer                              # layers of another make are refused when they are put together
+    for tensors in [(n.k.float(), n.v, n.k_scale, n.v_scale), (n.k, n.v, n.k_scale[:, :, :2].contiguous(), n.v_scale),
+                    (n.k, n.v, n.k_scale, n.v_scale.double()), (n.k.cpu(), n.v, n.k_scale, n.v_scale), (n.k, n.v[:1], n.k_scale, n.v_scale),
+                    (n.k[:, :, ::2], n.v[:, :, ::2], n.k_scale, n.v_scale), (n.k.transpose(1, 2), n.v, n.k_scale, n.v_scale)]:
+        with pytest.raises(KernelError):
+            qc.QuantizedPages(*tensors)
     k = torch.zeros(4, 2, 64, device=DEV)
     call = dict(max_len=4, cu_rows=step.cu_seqlens)
     qc.read(step.layer, k, k.clone(), step.page_table, step.seq_slot, step.seq_start, step.seq_len, **call)

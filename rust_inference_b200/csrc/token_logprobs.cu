@@ -6,92 +6,356 @@
 // nothing but minus infinity, has no distribution: all of its results are NaN.  The likeliest tokens are the largest logits in
 // descending order, ties in the order of the ids (NaN before all).  A target outside the vocabulary (-1: none) has the log
 // probability NaN.
-#include "common.cuh"
+//
+// One pass over the row: every thread keeps the maximum of its elements, sixteen bytes at a time, and z and t against a reference
+// that moves up with it (m -> m': z' = z a, t' = a (t + z (m - m')), a = exp(m - m')); all of it is float32.
+//
+// The likeliest `top` tokens without a second pass: four neighbouring threads are a group.  With tau the top-th largest of
+// the groups' maxima, at least `top` elements are tau or more, and all of those lie in groups whose maximum is.  Those are about
+// `top` groups of 1/128 of a block's part of the row; only they are read again, out of the L2 cache, and the few elements above
+// tau, with those equal to it, are put in order by counting.  (Where blocks share a row, tau is taken from 128 maxima too, each of
+// as many groups as there are blocks.)
+//
+// A row belongs to one block of 512 threads, or, where the rows would leave SMs idle, to a cluster of 2, 4 or 8, which exchange
+// their sums, maxima and candidates through distributed shared memory.  What bounds many rows is memory.
+#include "cluster.cuh"
+
+#include <float.h>
 
 using namespace ri;
 
 namespace {
 
-constexpr int THREADS = 1024;
+constexpr int THREADS = 512, WARPS = THREADS / 32, GROUP = 4, GROUPS = THREADS / GROUP, MOST_TOP = 64, MOST_BLOCKS = 8;
+constexpr int ROOM = 1024;                       // elements above tau, and equal to it, that a block's lists hold
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-// The order of the alternatives as one number: larger logits first, the lower id among equals (0 and -0 are equal)
-__device__ __forceinline__ unsigned long long rank_key(float x, int id) {
-    unsigned u = __float_as_uint(x + 0.f);
-    u = x != x ? 0xffffffffu : ((u & 0x80000000u) ? ~u : u | 0x80000000u);
-    return ((unsigned long long)u << 32) | (unsigned)~id;
+struct Sums { float m, z, t; };                  // t in units of log2
+
+__device__ __forceinline__ float two_to(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void raise(Sums& s, float m) {
+    const float d = (s.m - m) * LOG2E, a = two_to(d);
+    s.t = a * fmaf(s.z, fmaxf(d, -1000.f), s.t);
+    s.z *= a;
+    s.m = m;
+}
+__device__ __forceinline__ Sums joined(Sums a, Sums b) {
+    const float m = fmaxf(a.m, b.m);
+    raise(a, m);
+    raise(b, m);
+    a.z += b.z;
+    a.t += b.t;
+    return a;
+}
+__device__ __forceinline__ void add(Sums& s, float x) {                // s.m is x or more
+    const float d = (x - s.m) * LOG2E, e = two_to(d);
+    s.z += e;
+    s.t = fmaf(e, fmaxf(d, -1000.f), s.t);       // (banned: e = 0; a NaN stays one through e)
 }
 
-__device__ __forceinline__ unsigned long long block_max64(unsigned long long v, unsigned long long* scratch) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long w = __shfl_xor_sync(0xffffffffu, v, o);
-        v = w > v ? w : v;
+// sixteen bytes that an earlier kernel writes (see load_written), not kept in L1
+__device__ __forceinline__ uint4 load16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float load1(const float* p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float load1(const __nv_bfloat16* p) {
+    unsigned short v;
+    asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
+    return __uint_as_float((uint32_t)v << 16);
+}
+template <typename T> struct Piece;              // sixteen bytes of logits
+template <> struct Piece<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void open(const uint4& v, float* f) {
+        f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
     }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        v = threadIdx.x < (blockDim.x >> 5) ? scratch[threadIdx.x] : 0ull;
+};
+template <> struct Piece<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void open(const uint4& v, float* f) { unpack8(v, f); }
+};
+
+// Larger logits first: whole numbers in their order (0 and -0 are equal, NaN before all)
+__device__ __forceinline__ unsigned order(float x) {
+    const unsigned u = __float_as_uint(x + 0.f);
+    return x != x ? 0xffffffffu : ((u & 0x80000000u) ? ~u : u | 0x80000000u);
+}
+
+__device__ __forceinline__ const void* peer(const void* own, int rank) {           // a place in a peer's shared memory
+    uint64_t there;
+    asm volatile("mapa.u64 %0, %1, %2;" : "=l"(there) : "l"(own), "r"(rank));
+    return reinterpret_cast<const void*>(there);
+}
+
+struct Lists {
+    unsigned long long found[WARPS];
+    Sums sums[WARPS];
+    Sums block;                                  // of this block's part of the row
+    unsigned most[GROUPS];                       // the groups' maxima, in their order
+    unsigned every[GROUPS];                      // those of all the row's blocks, as many of them together as there are blocks
+    int votes[WARPS];
+    unsigned tau;
+    int above_n, equal_n, groups_n;
+    unsigned above_x[ROOM];
+    int above_id[ROOM], equal_id[ROOM], group[GROUPS];
+};
+
+// The whole row, ordered by x and id, from the largest on, by one block and one pass per token: where the lists do not hold what is
+// above tau (rows whose large logits lie in a few of the groups).
+template <typename T>
+__device__ void one_by_one(const T* x, int vocab, int top, float m, float log_z, int* ids, float* best, unsigned long long* scratch) {
+    unsigned long long last = ~0ull;
+    for (int k = 0; k < top; ++k) {
+        unsigned long long found = 0ull;
+        for (int i = threadIdx.x; i < vocab; i += THREADS) {
+            const unsigned long long key = ((unsigned long long)order(load1(x + i)) << 32) | (unsigned)~i;
+            if ((k == 0 || key < last) && key > found) found = key;
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long w = __shfl_xor_sync(0xffffffffu, v, o);
-            v = w > v ? w : v;
+            const unsigned long long w = __shfl_xor_sync(0xffffffffu, found, o);
+            found = w > found ? w : found;
         }
-        if (threadIdx.x == 0) scratch[32] = v;
+        __syncthreads();
+        if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = found;
+        __syncthreads();
+        last = 0ull;
+        for (int w = 0; w < WARPS; ++w) last = scratch[w] > last ? scratch[w] : last;
+        if (threadIdx.x == 0) {
+            const int id = (int)~(unsigned)last;
+            ids[k] = id;
+            best[k] = load1(x + id) - m - log_z;
+        }
     }
-    __syncthreads();
-    return scratch[32];
 }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
-logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int* __restrict__ targets, int top, float* __restrict__ logprob,
-                float* __restrict__ entropy, int* __restrict__ top_ids, float* __restrict__ top_logprobs) {
-    __shared__ float scratch[33];
-    __shared__ unsigned long long scratch64[33];
+__global__ void __launch_bounds__(THREADS, 3)
+logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, int top, float* __restrict__ logprob, float* __restrict__ entropy,
+                int* __restrict__ top_ids, float* __restrict__ top_logprobs, int blocks) {
+    constexpr int N = Piece<T>::N, AT_ONCE = 4;
+    __shared__ Lists s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = blocks > 1 ? (int)cluster_rank() : 0, row = blockIdx.x / blocks;
     let_next_kernel_start();
-    wait_for_previous_kernels();
-    const int row = blockIdx.x;
     const T* x = logits + (size_t)row * ld;
-    float m = -INFINITY;
-    bool bad = false;
-    for (int i = threadIdx.x; i < vocab; i += THREADS) {
-        const float v = to_f32<T>(x[i]);
-        bad |= v != v;
-        m = fmaxf(m, v);
+    // this block's part of the row, cut at 16-byte boundaries of memory: a head of single elements, pieces, a tail
+    const int skew = (int)(((16 - (uintptr_t)x % 16) % 16) / sizeof(T));              // elements before the first boundary
+    const int first = min(skew, vocab), pieces = (vocab - first) / N;
+    const int p0 = (int)((long long)pieces * rank / blocks), p1 = (int)((long long)pieces * (rank + 1) / blocks);
+    const int singles = rank == 0 ? vocab - pieces * N : 0;                            // head and tail, the first block's
+    auto single = [&](int i) { return i < first ? i : i + pieces * N; };               // the i-th of them
+    const T* body = x + first;
+    if (tid == 0) s.above_n = s.equal_n = s.groups_n = 0;
+    wait_for_previous_kernels();
+
+    Sums mine = {-FLT_MAX, 0.f, 0.f};            // (a finite reference: minus infinity less it is minus infinity)
+    float most = -INFINITY;
+    for (int p = p0 + tid; p < p1; p += AT_ONCE * THREADS) {
+        uint4 v[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+            if (p + k * THREADS < p1) v[k] = load16(body + (size_t)(p + k * THREADS) * N);
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            if (p + k * THREADS >= p1) break;
+            float f[N], higher = -INFINITY;
+            Piece<T>::open(v[k], f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) higher = fmaxf(higher, f[i]);
+            most = fmaxf(most, higher);
+            if (higher > mine.m) raise(mine, higher);
+#pragma unroll
+            for (int i = 0; i < N; ++i) add(mine, f[i]);
+        }
     }
-    m = block_max(m, scratch);
-    bad = __syncthreads_or(bad);
-    float z = 0.f, t = 0.f;
-    for (int i = threadIdx.x; i < vocab; i += THREADS) {
-        const float d = fmaxf(to_f32<T>(x[i]) - m, -1000.f), e = expf(d);      // (banned: e = 0, and e d too)
-        z += e;
-        t = fmaf(e, d, t);
+    for (int i = tid; i < singles; i += THREADS) {
+        const float f = load1(x + single(i));
+        most = fmaxf(most, f);
+        if (f > mine.m) raise(mine, f);
+        add(mine, f);
     }
-    z = block_sum(z, scratch);
-    t = block_sum(t, scratch);
-    const float nan = __int_as_float(0x7fffffff);
-    bad |= !(fabsf(m) < INFINITY);
-    const float lz = bad ? nan : logf(z);
-    if (threadIdx.x == 0) {
+    unsigned key = order(most);
+    if (mine.z != mine.z) {                      // a NaN (or an infinity less itself): maxima leave NaN out, the order does not
+        for (int p = p0 + tid; p < p1; p += THREADS)
+            for (int i = 0; i < N; ++i) key = max(key, order(load1(body + (size_t)p * N + i)));
+        for (int i = tid; i < singles; i += THREADS) key = max(key, order(load1(x + single(i))));
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        if (o < GROUP) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+        const Sums other = {__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.z, o), __shfl_xor_sync(0xffffffffu, mine.t, o)};
+        mine = joined(mine, other);
+    }
+    if (lane == 0) s.sums[warp] = mine;
+    if (tid % GROUP == 0) s.most[tid / GROUP] = key;
+    __syncthreads();
+    if (tid < 32) {
+        Sums all = tid < WARPS ? s.sums[tid] : Sums{-FLT_MAX, 0.f, 0.f};
+#pragma unroll
+        for (int o = 1; o < WARPS; o <<= 1) {
+            const Sums other = {__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.z, o), __shfl_xor_sync(0xffffffffu, all.t, o)};
+            all = joined(all, other);
+        }
+        if (tid == 0) s.block = all;
+    }
+    if (blocks > 1) cluster_sync();
+    else __syncthreads();
+    Sums all = s.block;
+    if (blocks > 1) {
+        all = {-FLT_MAX, 0.f, 0.f};
+        for (int b = 0; b < blocks; ++b) all = joined(all, *reinterpret_cast<const Sums*>(peer(&s.block, b)));
+    }
+    // no distribution: an infinite maximum, a NaN among the sums, nothing but banned tokens
+    const bool none = !(all.m < INFINITY) || !(all.z > 0.f);
+    const float log_z = none ? __int_as_float(0x7fffffff) : logf(all.z);
+    if (rank == 0 && tid == 0) {
         const int id = targets[row];
-        logprob[row] = id >= 0 && id < vocab ? to_f32<T>(x[id]) - m - lz : nan;
-        entropy[row] = lz - t / z;
+        logprob[row] = id >= 0 && id < vocab ? load1(x + id) - all.m - log_z : __int_as_float(0x7fffffff);
+        entropy[row] = log_z - all.t * LN2 / all.z;
     }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < top; ++k) {
-        unsigned long long best = 0ull;
-        for (int i = threadIdx.x; i < vocab; i += THREADS) {
-            const unsigned long long key = rank_key(to_f32<T>(x[i]), i);
-            if ((k == 0 || key < last) && key > best) best = key;
+    if (top == 0) {
+        if (blocks > 1) cluster_sync();          // a peer may still be reading this block's sums
+        return;
+    }
+
+    // ---- tau: the top-th largest of the groups' maxima ----
+    if (tid < GROUPS) {
+        const int per = GROUPS / blocks, at = tid % per * blocks;
+        unsigned largest = s.most[tid];
+        if (blocks > 1) {
+            const unsigned* theirs = reinterpret_cast<const unsigned*>(peer(s.most + at, tid / per));
+            largest = 0;
+            for (int i = 0; i < blocks; ++i) largest = max(largest, theirs[i]);
         }
-        last = block_max64(best, scratch64);
-        if (threadIdx.x == 0) {
-            const int id = (int)~(unsigned)last;
-            top_ids[(size_t)row * top + k] = id;
-            top_logprobs[(size_t)row * top + k] = to_f32<T>(x[id]) - m - lz;
+        s.every[tid] = largest;
+    }
+    __syncthreads();
+    {                                            // a maximum's place: how many are larger, or as large and earlier (four threads for each)
+        const int k = tid / 4, quarter = tid % 4 * (GROUPS / 4);
+        const unsigned mine = s.every[k];
+        int before = 0;
+#pragma unroll 8
+        for (int i = 0; i < GROUPS / 4; ++i) {
+            const int o = quarter + (i + 8 * (tid % 4)) % (GROUPS / 4);        // (the four in different banks)
+            before += s.every[o] > mine || (s.every[o] == mine && o < k);
+        }
+        before += __shfl_xor_sync(0xffffffffu, before, 1);
+        before += __shfl_xor_sync(0xffffffffu, before, 2);
+        if (tid % 4 == 0 && before == top - 1) s.tau = mine;
+    }
+    __syncthreads();
+    const unsigned tau = s.tau;
+
+    // ---- what is above it, and equal to it, in the groups that have any ----
+    if (tid < GROUPS && s.most[tid] >= tau) s.group[atomicAdd(&s.groups_n, 1)] = tid;
+    __syncthreads();
+    auto look = [&](float f, int id) {
+        const unsigned u = order(f);
+        if (u < tau) return;
+        if (u > tau) {
+            const int at = atomicAdd(&s.above_n, 1);
+            if (at < ROOM) s.above_x[at] = u, s.above_id[at] = id;
+        } else {
+            const int at = atomicAdd(&s.equal_n, 1);
+            if (at < ROOM) s.equal_id[at] = id;
+        }
+    };
+    constexpr int RUN = GROUP * N;               // neighbouring elements of a group
+    for (int i = warp; i < s.groups_n; i += WARPS) {
+        const int g = s.group[i];
+        // 32 / RUN runs at a time, one element per lane
+        const int turn = lane / RUN, within = lane % RUN;
+        for (int p = p0 + g * GROUP + turn * THREADS; p < p1; p += 8 * (32 / RUN) * THREADS) {
+            float f[8];
+            bool there[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int piece = p + k * (32 / RUN) * THREADS + within / N;
+                there[k] = piece < p1;
+                if (there[k]) f[k] = load1(body + (size_t)piece * N + within % N);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int piece = p + k * (32 / RUN) * THREADS + within / N;
+                if (there[k]) look(f[k], first + piece * N + within % N);
+            }
         }
     }
+    for (int i = tid; i < singles; i += THREADS) look(load1(x + single(i)), single(i));
+    if (blocks > 1) cluster_sync();
+    else __syncthreads();
+
+    if (rank == 0) {
+        // ---- the first block brings the lists together and puts them in order ----
+        int above = s.above_n, equal = s.equal_n;
+        bool held = above <= ROOM;               // all that is above; of the equal ones as many as are wanted
+        bool ties = equal <= ROOM;
+        const int own_above = min(above, ROOM), own_equal = min(equal, ROOM);
+        int at_above = own_above, at_equal = own_equal;
+        for (int b = 1; b < blocks; ++b) {
+            const Lists& other = *reinterpret_cast<const Lists*>(peer(&s, b));
+            const int na = other.above_n, ne = other.equal_n;
+            above += na;
+            equal += ne;
+            held = held && at_above + na <= ROOM;
+            ties = ties && at_equal + ne <= ROOM;
+            if (held)
+                for (int i = tid; i < na; i += THREADS) s.above_x[at_above + i] = other.above_x[i], s.above_id[at_above + i] = other.above_id[i];
+            if (ties)
+                for (int i = tid; i < ne; i += THREADS) s.equal_id[at_equal + i] = other.equal_id[i];
+            at_above += na;
+            at_equal += ne;
+        }
+        __syncthreads();
+        int* ids = top_ids + (size_t)row * top;
+        float* best = top_logprobs + (size_t)row * top;
+        auto value = [&](int id) { return load1(x + id) - all.m - log_z; };
+        if (!held) {
+            one_by_one<T>(x, vocab, top, all.m, log_z, ids, best, s.found);
+        } else {
+            for (int i = tid; i < above; i += THREADS) {
+                const unsigned u = s.above_x[i];
+                const int id = s.above_id[i];
+                int place = 0;
+                for (int o = 0; o < above; ++o) place += s.above_x[o] > u || (s.above_x[o] == u && s.above_id[o] < id);
+                if (place < top) ids[place] = id, best[place] = value(id);
+            }
+            if (above < top && ties) {
+                for (int i = tid; i < equal; i += THREADS) {
+                    const int id = s.equal_id[i];
+                    int place = above;
+                    for (int o = 0; o < equal; ++o) place += s.equal_id[o] < id;
+                    if (place < top) ids[place] = id, best[place] = value(id);
+                }
+            } else if (above < top) {            // more of them than the list holds (banned tokens, for one): the lowest ids, in their order
+                for (int from = 0, place = above; place < top && from < vocab; from += THREADS) {
+                    const bool is = from + tid < vocab && order(load1(x + from + tid)) == tau;
+                    const unsigned votes = __ballot_sync(0xffffffffu, is);
+                    __syncthreads();
+                    if (lane == 0) s.votes[warp] = __popc(votes);
+                    __syncthreads();
+                    int at = place + __popc(votes & ((1u << lane) - 1u));
+                    for (int w = 0; w < WARPS; ++w) {
+                        if (w < warp) at += s.votes[w];
+                        place += s.votes[w];
+                    }
+                    if (is && at < top) ids[at] = from + tid, best[at] = value(from + tid);
+                }
+            }
+        }
+    }
+    if (blocks > 1) cluster_sync();              // the first block may still be reading the others' lists
 }
 
 }  // namespace
@@ -100,10 +364,14 @@ logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int
 RI_API int ri_token_logprobs(const void* logits, int dtype, long long ld, int rows, int vocab, const int* targets, int top, float* logprob,
                              float* entropy, int* top_ids, float* top_logprobs, cudaStream_t stream) {
     if (rows <= 0) return 0;
-    if (vocab <= 0 || top < 0 || top > vocab) return fail("token_logprobs: %d alternatives of %d tokens", top, vocab);
+    if (vocab <= 0 || top < 0 || top > vocab || top > MOST_TOP) return fail("token_logprobs: %d alternatives of %d tokens", top, vocab);
+    // as many blocks per row as the SMs hold together (three each), and no more than have 512 pieces of a row each
+    int blocks = 1;
+    while (blocks < MOST_BLOCKS && (long long)rows * blocks * 2 <= 3ll * sm_count() && vocab / (dtype == RI_F32 ? 4 : 8) >= 2 * blocks * THREADS) blocks *= 2;
+    if ((long long)rows * blocks > 0x7fffffff) return fail("token_logprobs: %d rows are too many", rows);
     auto launch = [&](auto kernel, auto* x) {
-        return check_launch(launch_dependent(kernel, dim3((unsigned)rows), dim3(THREADS), 0, stream, x, ld, vocab, targets, top, logprob,
-                                             entropy, top_ids, top_logprobs), "token_logprobs");
+        return launch_cluster("token_logprobs", kernel, dim3((unsigned)(rows * blocks)), THREADS, 0, blocks, stream, x, ld, vocab, targets, top,
+                              logprob, entropy, top_ids, top_logprobs, blocks);
     };
     if (dtype == RI_F32) return launch(logprobs_kernel<float>, (const float*)logits);
     if (dtype == RI_BF16) return launch(logprobs_kernel<__nv_bfloat16>, (const __nv_bfloat16*)logits);

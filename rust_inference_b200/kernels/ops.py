@@ -668,8 +668,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0)
     if top:
         ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
         best = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-    _call("token_logprobs", "ri_token_logprobs", _p(logits), c_int(_DTYPE_CODE[logits.dtype]), c_longlong(logits.stride(0)), c_int(rows),
-          c_int(vocab), _p(targets), c_int(top), _p(logprob), _p(entropy), _p(ids), _p(best), _stream())
+    _call("token_logprobs", "ri_token_logprobs", _p(logits), _DTYPE_CODE[logits.dtype], c_longlong(logits.stride(0)), rows, vocab, _p(targets),
+          top, _p(logprob), _p(entropy), _p(ids), _p(best), _stream())
     return TokenLogprobs(logprob, entropy, ids, best)
 
 

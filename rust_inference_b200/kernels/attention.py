@@ -134,7 +134,13 @@ def attention(qkv, cache_layer, out, ctx, *, n_heads, n_kv_heads, head_dim, scal
     the window, a term without key in the softmax's denominator, a bias by distance and a gate per head on the
     result (see `ops.attention_generic`).  cache_layer: a layer in the run dtype, or one in 8 bits
     (`quantized_cache.QuantizedPages`)."""
-    if quantized_cache.is_quantized(cache_layer):
+    if type(cache_layer) is quantized_cache.QuantizedPages:
+        # steps of few rows (and all in float32) read the codes themselves
+        if ((qkv.dtype is torch.float32 or ctx.max_new * (n_heads // n_kv_heads) <= QUANTIZED_ROWS) and not (window and chunk)
+                and (head_dim == 64 or head_dim == 128) and (v_head_dim is None or v_head_dim == head_dim)
+                and not (softcap or keep_first or sink is not None or dist is not None or gate is not None)):
+            return quantized_cache.attend_step(qkv, cache_layer, out, quantized_cache.step_of(ctx, n_heads, n_kv_heads, head_dim), scale,
+                                               window if window else -int(chunk or 0), out_scale)
         return _over_quantized(qkv, cache_layer, out, ctx, n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, scale=scale,
                                window=window, chunk=chunk, v_head_dim=v_head_dim, out_scale=out_scale, softcap=softcap,
                                keep_first=keep_first, sink=sink, dist=dist, gate=gate)
@@ -237,17 +243,7 @@ QUANTIZED_ROWS = 64
 
 
 def _over_quantized(qkv, layer, out, ctx, *, window, chunk, keep_first, **forms):
-    """`attention` over a cache in 8 bits."""
-    plain = not (forms["softcap"] or keep_first or any(forms[n] is not None for n in ("sink", "dist", "gate"))) and not (window and chunk)
-    heads, kv, hd = forms["n_heads"], forms["n_kv_heads"], forms["head_dim"]
-    if (plain and quantized_cache.attention_supports(qkv.dtype, hd, forms["v_head_dim"])
-            and (qkv.dtype == torch.float32 or ctx.max_new * (heads // kv) <= QUANTIZED_ROWS)):
-        floats, ints = quantized_cache.attention_workspace(heads, kv, hd, ctx.max_new)
-        return quantized_cache.attention(
-            qkv, layer, out, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens, n_heads=heads, n_kv_heads=kv, head_dim=hd,
-            max_new=ctx.max_new, scale=forms["scale"], part=ctx.buffer("quantized_part", (floats,), torch.float32),
-            arrived=ctx.zeroed_buffer("quantized_arrived", (ints,), torch.int32), span=window if window else -int(chunk or 0),
-            out_scale=forms["out_scale"])
+    """`attention` over a cache in 8 bits by way of the run dtype."""
     k = ctx.buffer("readback_k", layer.k.shape, qkv.dtype)
     v = ctx.buffer("readback_v", layer.v.shape, qkv.dtype)
     # (a captured step may run with longer sequences than it was captured with)

@@ -7,6 +7,7 @@ a missing compiler or a library that does not load is an error, never a detour.
 from __future__ import annotations
 
 import ctypes
+import functools
 from ctypes import c_int, c_float, c_void_p, c_longlong, c_ulonglong
 
 import math
@@ -657,20 +658,28 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0)
     their log probabilities.  logits: float32 or bfloat16 [R, V], rows any distance apart; targets: int32 [R] (an id outside the
     vocabulary, as -1: log probability NaN).  Logits of minus infinity are tokens that cannot come; a row with a NaN, plus
     infinity or nothing else has no distribution, and its results are NaN.  Equal logits rank by their id."""
-    _need(logits.is_cuda and targets.is_cuda and logits.dim() == 2 and logits.dtype in _DTYPE_CODE and logits.shape[1] > 0
-          and (logits.stride(1) == 1 or logits.shape[1] == 1), "token_logprobs: logits must be float32 or bfloat16 [rows, vocabulary] on the "
-          "device, neighbours side by side")
+    code = _DTYPE_CODE.get(logits.dtype)
+    if not (code is not None and logits.is_cuda and targets.is_cuda and logits.dim() == 2 and targets.dtype is torch.int32
+            and targets.is_contiguous()):
+        raise KernelError("token_logprobs: logits must be float32 or bfloat16 [rows, vocabulary], targets int32 [rows], both on the device")
     rows, vocab = logits.shape
-    _need(targets.dtype == torch.int32 and targets.is_contiguous() and targets.numel() == rows, "token_logprobs: targets must be int32 [rows]")
-    _need(0 <= top <= min(vocab, TOKEN_LOGPROBS_MOST), "token_logprobs: too many alternatives, or fewer than none")
-    logprob, entropy = torch.empty((2, rows), dtype=torch.float32, device=logits.device).unbind()
+    ld, step = logits.stride()
+    if targets.numel() != rows or vocab == 0 or (step != 1 and vocab != 1) or not 0 <= top <= min(vocab, TOKEN_LOGPROBS_MOST):
+        raise KernelError(f"token_logprobs: {rows} rows of {vocab} logits side by side, a target each, and 0 to {TOKEN_LOGPROBS_MOST} alternatives")
+    floats = logits if code == RI_F32 else logits.new_empty(0, dtype=torch.float32)
+    logprob, entropy = floats.new_empty(rows), floats.new_empty(rows)
     ids = best = None
     if top:
-        ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-        best = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-    _call("token_logprobs", "ri_token_logprobs", _p(logits), _DTYPE_CODE[logits.dtype], c_longlong(logits.stride(0)), rows, vocab, _p(targets),
-          top, _p(logprob), _p(entropy), _p(ids), _p(best), _stream())
+        ids, best = targets.new_empty(rows, top), floats.new_empty(rows, top)
+    _prepare_logprobs()
+    _call("token_logprobs", "ri_token_logprobs", logits.data_ptr(), code, ld, rows, vocab, targets.data_ptr(), top, logprob.data_ptr(),
+          entropy.data_ptr(), ids.data_ptr() if top else None, best.data_ptr() if top else None, _stream())
     return TokenLogprobs(logprob, entropy, ids, best)
+
+
+@functools.lru_cache(maxsize=None)
+def _prepare_logprobs() -> None:
+    load("token_logprobs").ri_token_logprobs.argtypes = [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int] + [c_void_p] * 5
 
 
 def cast(src: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

@@ -68,12 +68,12 @@ def empty_layer(n_pages: int, n_kv_heads: int, head_dim: int, v_head_dim: int | 
 
 
 def is_quantized(layer) -> bool:
-    return isinstance(layer, QuantizedPages)
+    return type(layer) is QuantizedPages
 
 
 def _index(what: str, t: torch.Tensor, least: int) -> int:
     """The address of an index array of at least so many entries."""
-    if t.dtype != torch.int32 or not t.is_cuda or t.numel() < least or not t.is_contiguous():
+    if t.dtype is not torch.int32 or not t.is_cuda or t.numel() < least or not t.is_contiguous():
         raise KernelError(f"{what}: index arrays are contiguous int32 on the device, {least} entries or more here")
     return t.data_ptr()
 
@@ -96,21 +96,25 @@ def write(src: torch.Tensor, q_out: torch.Tensor | None, cos, sin, layer: Quanti
     v_hd = head_dim if v_head_dim is None else int(v_head_dim)
     rot = head_dim if rot_dims is None else int(rot_dims)
     n_seqs, cols = seq_slot.numel(), (n_heads + n_kv_heads) * head_dim + n_kv_heads * v_hd
-    _need(layer.sizes == (n_kv_heads, head_dim, v_hd), what, f"the layer has {layer.sizes[0]} kv heads of {layer.sizes[1:]} channels")
-    _need(src.is_cuda and src.dim() == 2 and src.is_contiguous() and src.shape[1] >= cols, what, "a contiguous [tokens, q | k | v columns] on the device is wanted")
-    _need(q_out is None or (q_out.is_cuda and q_out.is_contiguous() and q_out.shape == (src.shape[0], n_heads * head_dim)
-                            and (q_out.dtype == src.dtype or src.dtype == torch.float32)), what, "q_out must be [tokens, heads * head size]")
-    if rot:
-        _need(cos.is_cuda and sin.is_cuda and cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.dim() == 2
-              and cos.shape[1] * 2 == rot and sin.shape == cos.shape and cos.is_contiguous() and sin.is_contiguous(),
-              what, "tables must be float32 [positions, rotated channels / 2]")
-    _need(bias is None or (bias.is_cuda and bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() >= cols), what,
-          "bias must be float32 [columns]")
-    _need(page_table.dim() == 2, what, "the page table must be int32 [slots, pages]")
+    if layer.sizes != (n_kv_heads, head_dim, v_hd):
+        raise KernelError(f"{what}: the layer has {layer.sizes[0]} kv heads of {layer.sizes[1:]} channels")
+    dtype = src.dtype
+    if not (src.is_cuda and src.dim() == 2 and src.is_contiguous() and src.shape[1] >= cols):
+        raise KernelError(f"{what}: a contiguous [tokens, q | k | v columns] on the device is wanted")
+    if q_out is not None and not (q_out.is_cuda and q_out.is_contiguous() and q_out.shape == (src.shape[0], n_heads * head_dim)
+                                  and (q_out.dtype is dtype or dtype is torch.float32)):
+        raise KernelError(f"{what}: q_out must be [tokens, heads * head size]")
+    if rot and not (cos.is_cuda and sin.is_cuda and cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.dim() == 2
+                    and cos.shape[1] * 2 == rot and sin.shape == cos.shape and cos.is_contiguous() and sin.is_contiguous()):
+        raise KernelError(f"{what}: tables must be float32 [positions, rotated channels / 2]")
+    if bias is not None and not (bias.is_cuda and bias.dtype is torch.float32 and bias.is_contiguous() and bias.numel() >= cols):
+        raise KernelError(f"{what}: bias must be float32 [columns]")
+    if page_table.dim() != 2:
+        raise KernelError(f"{what}: the page table must be int32 [slots, pages]")
     _prepare("quantized_cache", "ri_quantized_write")
     k, v, ks, vs = layer.pointers
-    _call("quantized_cache", "ri_quantized_write", src.data_ptr(), dtype_code(src.dtype), src.shape[1], None if bias is None else bias.data_ptr(),
-          1 if clear else 0, None if q_out is None else q_out.data_ptr(), dtype_code(src.dtype if q_out is None else q_out.dtype),
+    _call("quantized_cache", "ri_quantized_write", src.data_ptr(), dtype_code(dtype), src.shape[1], None if bias is None else bias.data_ptr(),
+          1 if clear else 0, None if q_out is None else q_out.data_ptr(), dtype_code(dtype if q_out is None else q_out.dtype),
           cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, _index(what, page_table, 1), page_table.shape[1],
           _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs), _index(what, cu_seqlens, n_seqs + 1), k, v, ks, vs, n_seqs,
           max_new, n_heads, n_kv_heads, head_dim, v_hd, rot, style, _stream())
@@ -126,14 +130,14 @@ def read(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, page_t
     what = "quantized_cache.read"
     n_kv, hd, v_hd = layer.sizes
     n_seqs = seq_slot.numel()
-    _need(k_out.is_cuda and v_out.is_cuda and k_out.dtype == v_out.dtype and k_out.is_contiguous() and v_out.is_contiguous(), what,
-          "outputs of one dtype, contiguous, on the device")
+    if not (k_out.is_cuda and v_out.is_cuda and k_out.dtype is v_out.dtype and k_out.is_contiguous() and v_out.is_contiguous()
+            and page_table.dim() == 2):
+        raise KernelError(f"{what}: outputs of one dtype, contiguous, on the device, and an int32 [slots, pages] table")
     if cu_rows is None:
-        _need(k_out.shape == layer.k.shape and v_out.shape == layer.v.shape, what, "without cu_rows the outputs have the cache's shape")
-    else:
-        _need(k_out.dim() == 3 and k_out.shape[1:] == (n_kv, hd) and v_out.shape == (k_out.shape[0], n_kv, v_hd), what,
-              "with cu_rows the outputs are [rows, kv heads, head size]")
-    _need(page_table.dim() == 2, what, "the page table must be int32 [slots, pages]")
+        if k_out.shape != layer.k.shape or v_out.shape != layer.v.shape:
+            raise KernelError(f"{what}: without cu_rows the outputs have the cache's shape")
+    elif not (k_out.dim() == 3 and k_out.shape[1:] == (n_kv, hd) and v_out.shape == (k_out.shape[0], n_kv, v_hd)):
+        raise KernelError(f"{what}: with cu_rows the outputs are [rows, kv heads, head size]")
     _prepare("quantized_cache", "ri_quantized_read")
     k, v, ks, vs = layer.pointers
     _call("quantized_cache", "ri_quantized_read", k, v, ks, vs, k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype),
@@ -161,19 +165,59 @@ def attention(q: torch.Tensor, layer: QuantizedPages, out: torch.Tensor, page_ta
     """Attention of every token of the step over its slot's cached keys, straight from the codes (csrc/attention_quantized.cu): for
     steps of few tokens per sequence, and for float32.  q: rows whose leading n_heads * head_dim columns are the queries, rotated;
     span: > 0 the last so many keys, < 0 the keys of the query's own block of -span positions; part, arrived: `attention_workspace`."""
-    what = "quantized_cache.attention"
-    n_seqs, width = seq_slot.numel(), n_heads * head_dim
-    _need(layer.sizes == (n_kv_heads, head_dim, head_dim) and layer.aligned, what, f"the layer has {layer.sizes[0]} kv heads of {layer.sizes[1:]} channels, or is not aligned")
-    _need(q.is_cuda and out.is_cuda and q.dtype == out.dtype and attention_supports(q.dtype, head_dim, None) and q.dim() == 2
-          and out.dim() == 2 and q.stride(1) == 1 and out.stride(1) == 1 and q.shape[0] == out.shape[0] and q.shape[1] >= width
-          and out.shape[1] >= width and n_heads % n_kv_heads == 0 and page_table.dim() == 2, what,
-          "queries and result must be float32 or bfloat16 [tokens, heads * 64 or 128] on the device")
-    floats, ints = attention_workspace(n_heads, n_kv_heads, head_dim, max_new)
-    _need(part.is_cuda and part.dtype == torch.float32 and part.is_contiguous() and part.numel() >= floats, what, "scratch too small")
-    _prepare("attention_quantized", "ri_attention_quantized")
+    step = _Step(page_table, seq_slot, seq_start, cu_seqlens, n_heads, n_kv_heads, head_dim, max_new, part, arrived)
+    return attend_step(q, layer, out, step, scale, span, out_scale)
+
+
+class _Step:
+    """What the calls of a step have in common: its arrays' addresses and sizes, looked at once."""
+
+    __slots__ = ("n_heads", "n_kv_heads", "head_dim", "sizes", "table", "max_pages", "slot", "start", "cu", "n_seqs", "max_new", "part",
+                 "part_size", "arrived", "kept")
+
+    def __init__(self, page_table, seq_slot, seq_start, cu_seqlens, n_heads, n_kv_heads, head_dim, max_new, part, arrived):
+        what = "quantized_cache.attention"
+        _need(n_kv_heads > 0 and n_heads % n_kv_heads == 0 and attention_supports(torch.float32, head_dim, None) and page_table.dim() == 2, what,
+              f"{n_heads} heads of {head_dim} over {n_kv_heads}, or a page table that is not [slots, pages]")
+        floats, ints = attention_workspace(n_heads, n_kv_heads, head_dim, max_new)
+        _need(part.is_cuda and part.dtype == torch.float32 and part.is_contiguous() and part.numel() >= floats, what, "scratch too small")
+        self.n_heads, self.n_kv_heads, self.head_dim, self.max_new = n_heads, n_kv_heads, head_dim, max_new
+        self.sizes = (n_kv_heads, head_dim, head_dim)
+        self.n_seqs = seq_slot.numel()
+        self.table, self.max_pages = _index(what, page_table, 1), page_table.shape[1]
+        self.slot, self.start = _index(what, seq_slot, self.n_seqs), _index(what, seq_start, self.n_seqs)
+        self.cu = _index(what, cu_seqlens, self.n_seqs + 1)
+        self.part, self.part_size, self.arrived = part.data_ptr(), part.numel(), _index(what, arrived, ints)
+        self.kept = (page_table, seq_slot, seq_start, cu_seqlens, part, arrived)     # whose addresses these are
+        _prepare("attention_quantized", "ri_attention_quantized")
+
+
+def step_of(ctx, n_heads: int, n_kv_heads: int, head_dim: int) -> _Step:
+    """`attention`'s view of a step (`engine.context.StepContext`), made by the first layer that asks."""
+    key = ("quantized", n_heads, n_kv_heads, head_dim)
+    step = ctx.extras.get(key)
+    if step is None:
+        floats, ints = attention_workspace(n_heads, n_kv_heads, head_dim, ctx.max_new)
+        step = ctx.extras[key] = _Step(ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens, n_heads, n_kv_heads, head_dim, ctx.max_new,
+                                       ctx.buffer("quantized_part", (floats,), torch.float32),
+                                       ctx.zeroed_buffer("quantized_arrived", (ints,), torch.int32))
+    return step
+
+
+def attend_step(q, layer, out, step, scale, span, out_scale):
+    """`attention` for a step that has been looked at."""
+    dtype, width = q.dtype, step.n_heads * step.head_dim
+    if not (layer.sizes == step.sizes and layer.aligned and out.dtype is dtype and (dtype is torch.bfloat16 or dtype is torch.float32)
+            and q.is_cuda and out.is_cuda and q.dim() == 2 and out.dim() == 2):
+        raise KernelError("quantized_cache.attention: queries and result must be float32 or bfloat16 [tokens, heads * head size] on the "
+                          f"device, the layer {step.n_kv_heads} kv heads of {step.head_dim}")
+    q_ld, q_step = q.stride()
+    out_ld, out_step = out.stride()
+    (rows, q_width), out_shape = q.shape, out.shape
+    if q_step != 1 or out_step != 1 or q_width < width or out_shape[0] != rows or out_shape[1] < width:
+        raise KernelError("quantized_cache.attention: rows of queries and result hold all heads side by side")
     k, v, ks, vs = layer.pointers
-    _call("attention_quantized", "ri_attention_quantized", q.data_ptr(), dtype_code(q.dtype), q.stride(0), k, v, ks, vs,
-          _index(what, page_table, 1), page_table.shape[1], _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs),
-          _index(what, cu_seqlens, n_seqs + 1), out.data_ptr(), out.stride(0), n_seqs, max_new, n_heads, n_kv_heads, head_dim, scale, span,
-          out_scale, part.data_ptr(), part.numel(), _index(what, arrived, ints), _stream())
+    _call("attention_quantized", "ri_attention_quantized", q.data_ptr(), 0 if dtype is torch.float32 else 1, q_ld, k, v, ks, vs, step.table,
+          step.max_pages, step.slot, step.start, step.cu, out.data_ptr(), out_ld, step.n_seqs, step.max_new, step.n_heads, step.n_kv_heads,
+          step.head_dim, scale, span, out_scale, step.part, step.part_size, step.arrived, _stream())
     return out

@@ -25,6 +25,8 @@ namespace {
 constexpr int PAGE = 64, BLOCK = 16, PER_PAGE = PAGE / BLOCK;
 constexpr int THREADS = 128;
 
+bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+
 struct Written {                 // where a projection's columns go
     void* src;                   // [tokens][ld]: q heads, k heads, v heads
     int ld;
@@ -37,15 +39,46 @@ struct Written {                 // where a projection's columns go
     int8_t *kc, *vc;
     float *ks, *vs;
     int n_heads, n_kv, hd, v_hd, rot, style;
-    int runs;                    // blocks of positions per sequence, at most
+    int n_seqs, runs;            // blocks of positions per sequence, at most; 0: counted through, sequence by sequence
 };
+
+// a pair of channels turned, every product and sum rounded once
+__device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
+    const float x0 = a, x1 = b;
+    a = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, s));
+    b = __fadd_rn(__fmul_rn(x0, s), __fmul_rn(x1, c));
+}
 
 // A position block of a step: rows lo..hi-1 of the sequence's positions base..base+15
 struct Run { int seq, base, lo, hi, row0; };
+__device__ __forceinline__ int runs_of(int start, int n) { return n > 0 ? (start + n - 1) / BLOCK - start / BLOCK + 1 : 0; }
 __device__ __forceinline__ bool run_of(const Written& w, int i, Run& r) {
-    r.seq = i / w.runs;
+    r.seq = w.runs ? i / w.runs : w.n_seqs;
+    int nth = w.runs ? i % w.runs : i;
+    if (w.runs == 0) {                              // a lane per sequence
+        const int lane = threadIdx.x & 31;
+        for (int s0 = 0; s0 < w.n_seqs; s0 += 32) {
+            const int s = s0 + lane;
+            const int mine = s < w.n_seqs ? runs_of(w.seq_start[s], w.cu_seqlens[s + 1] - w.cu_seqlens[s]) : 0;
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int before = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += before;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, upto > nth);
+            if (past) {
+                const int at = __ffs(past) - 1;
+                r.seq = s0 + at;
+                nth -= __shfl_sync(0xffffffffu, upto - mine, at);
+                break;
+            }
+            nth -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (r.seq == w.n_seqs) return false;
+    }
     const int first = w.cu_seqlens[r.seq], n = w.cu_seqlens[r.seq + 1] - first, start = w.seq_start[r.seq];
-    r.base = (start / BLOCK + i % w.runs) * BLOCK;
+    r.base = (start / BLOCK + nth) * BLOCK;
     r.lo = max(r.base, start);
     r.hi = min(r.base + BLOCK, start + n);
     r.row0 = first + r.lo - start;
@@ -82,8 +115,7 @@ __global__ void __launch_bounds__(THREADS) write_any_kernel(Written w) {
         y1 = x1;
         if (turned) {
             const float c = w.cos_t[(size_t)(r.lo + row) * half + i], s = w.sin_t[(size_t)(r.lo + row) * half + i];
-            y0 = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, s));
-            y1 = __fadd_rn(__fmul_rn(x0, s), __fmul_rn(x1, c));
+            rotate(y0, y1, c, s);
         }
     };
     auto cleared = [&](int row, int d0, int d1) {
@@ -141,8 +173,199 @@ __global__ void __launch_bounds__(THREADS) write_any_kernel(Written w) {
     if (threadIdx.x == 0) *scale = s;
 }
 
-// Reading back: a block of threads takes a page of one kv head, keys and values, sixteen codes per thread and turn.  What
-// bounds it is memory.
+// Heads of 64 or 128 whose channels are all rotated, or none, on 16-byte boundaries: two warps take eight rows each of a position
+// block of one head (four heads to a block of threads, which read the same angles), each lane four pairs of channels of every second
+// or fourth row; keys and values stay in registers between their maximum and their codes.  Angles are read before the wait for the
+// kernel before.  What bounds a prompt is memory, what bounds a step of single tokens is the latency of its few loads.
+// How a lane's pairs lie in a head: (i, i + HD/2), or (2i, 2i + 1) for i = 4 lane' .. + 4; unrotated heads as the second.
+template <typename T> struct Four;                 // four neighbouring numbers as they lie in memory
+template <> struct Four<float> {
+    float4 v;
+    __device__ __forceinline__ void get(const float* p) { v = load_written(p); }
+    __device__ __forceinline__ void open(float* f) const { f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w; }
+};
+template <> struct Four<__nv_bfloat16> {
+    uint32_t x, y;
+    __device__ __forceinline__ void get(const __nv_bfloat16* p) { asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "l"(p) : "memory"); }
+    __device__ __forceinline__ void open(float* f) const {
+        f[0] = __uint_as_float(x << 16), f[1] = __uint_as_float(x & 0xffff0000u);
+        f[2] = __uint_as_float(y << 16), f[3] = __uint_as_float(y & 0xffff0000u);
+    }
+};
+template <typename T> __device__ __forceinline__ void put4(T* p, const float* f);
+template <> __device__ __forceinline__ void put4<float>(float* p, const float* f) { *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(f); }
+template <> __device__ __forceinline__ void put4<__nv_bfloat16>(__nv_bfloat16* p, const float* f) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+    uint2 v;
+    v.x = *reinterpret_cast<const uint32_t*>(&a), v.y = *reinterpret_cast<const uint32_t*>(&b);
+    *reinterpret_cast<uint2*>(p) = v;
+}
+__device__ __forceinline__ uint32_t four_codes(const float* f, float inverse) {
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v |= (uint32_t)(__float2int_rn(f[i] * inverse) & 255) << (8 * i);
+    return v;
+}
+__device__ __forceinline__ uint32_t rounded_again(uint32_t codes, float factor) {
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v |= (uint32_t)(__float2int_rn((float)(int8_t)(codes >> (8 * i)) * factor) & 255) << (8 * i);
+    return v;
+}
+
+constexpr int HEADS = 4, HALF = BLOCK / 2;          // heads of a block of threads; rows of a warp
+
+template <typename TS, typename TQ, int HD>
+__global__ void __launch_bounds__(64 * HEADS, 4) write_kernel(Written w, int kv_blocks, int q_each) {
+    constexpr int LANES = HD / 8, STRIDE = 32 / LANES, TURNS = HALF / STRIDE;      // lanes per row, rows per turn, turns
+    __shared__ float most[2 * HEADS];
+    __shared__ __align__(16) float angles[2][BLOCK][HD / 2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES, sub = lane / LANES;
+    let_next_kernel_start();
+    Run r;
+    const bool some = run_of(w, blockIdx.x, r);
+    // the first blocks: k heads, v heads; then q heads
+    const bool kv = (int)blockIdx.y < kv_blocks;
+    const int part = kv ? (int)blockIdx.y * HEADS + (warp >> 1) : ((int)blockIdx.y - kv_blocks) * HEADS * q_each + (warp >> 1);
+    const bool is_k = kv && part < w.n_kv;
+    const int head = kv && !is_k ? part - w.n_kv : part;
+    const bool here = some && part < (kv ? 2 * w.n_kv : w.n_heads);
+    int col = !kv ? head * HD : (is_k ? w.n_heads + head : w.n_heads + w.n_kv + head) * HD;
+    const bool turned = (is_k || !kv) && w.rot != 0, apart = turned && w.style == 0;
+    const int d0 = apart ? 4 * l : 8 * l, d1 = d0 + (apart ? HD / 2 : 4);          // this lane's channels: four from d0, four from d1
+    const int lo = r.lo - r.base, hi = r.hi - r.base, row0 = (warp & 1) * HALF + sub;      // the block's new rows; this lane's first row
+    auto mine = [&](int turn) { return row0 + turn * STRIDE >= lo && row0 + turn * STRIDE < hi; };
+    // the rows' angles (cosines, then sines), once for the block's heads
+    if (some && w.rot != 0) {
+        const size_t at = (size_t)(r.base + lo) * (HD / 2);
+        for (int i = threadIdx.x; i < (hi - lo) * (HD / 8); i += 64 * HEADS) {
+            reinterpret_cast<float4*>(angles[0][lo])[i] = reinterpret_cast<const float4*>(w.cos_t + at)[i];
+            reinterpret_cast<float4*>(angles[1][lo])[i] = reinterpret_cast<const float4*>(w.sin_t + at)[i];
+        }
+    }
+    bool there = false;
+    int page = 0;
+    if (kv && here) {
+        const int slot = w.seq_slot[r.seq];
+        // checked build: a slot, a page index or a page outside is recorded and nothing is written
+        there = RI_IN_LIMIT(slot, RI_LIMIT_SLOTS, RI_CHECK_SLOT) && RI_IN_RANGE(r.base / PAGE, w.max_pages, RI_CHECK_PAGE_INDEX);
+        if (there) page = w.page_table[(size_t)slot * w.max_pages + r.base / PAGE];
+        there = there && RI_IN_LIMIT(page, RI_LIMIT_PAGES, RI_CHECK_PAGE);
+    }
+    wait_for_previous_kernels();
+    if (!some) return;
+    TS* src = reinterpret_cast<TS*>(w.src) + ((ptrdiff_t)r.row0 - lo + row0) * w.ld + col;     // this lane's row of turn 0 (looked at from row lo on)
+
+    Four<TS> raw[TURNS][2];
+    auto get = [&](const TS* from) {
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k)
+            if (mine(k)) {
+                raw[k][0].get(from + (ptrdiff_t)k * STRIDE * w.ld + d0);
+                raw[k][1].get(from + (ptrdiff_t)k * STRIDE * w.ld + d1);
+            }
+    };
+    if (here) get(src);
+    __syncthreads();                                // the angles are there
+    auto finish = [&](int k, float* y) {            // bias, rotation, zeros behind
+        raw[k][0].open(y);
+        raw[k][1].open(y + 4);
+        if (w.clear) {
+            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+            TS* at = src + (ptrdiff_t)k * STRIDE * w.ld;
+            put4<TS>(at + d0, zero);
+            put4<TS>(at + d1, zero);
+        }
+        if (w.bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] += w.bias[col + d0 + i], y[4 + i] += w.bias[col + d1 + i];
+        }
+        if (!turned) return;
+        __align__(16) float c[4], s[4];
+        *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(&angles[0][row0 + k * STRIDE][4 * l]);
+        *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(&angles[1][row0 + k * STRIDE][4 * l]);
+        if (apart) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rotate(y[i], y[4 + i], c[i], s[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rotate(y[2 * i], y[2 * i + 1], c[i], s[i]);
+        }
+    };
+    if (!kv) {
+        // as many q heads as the launch gives a warp, four apart: the same rows and angles
+        TQ* q = reinterpret_cast<TQ*>(w.q_out) + ((ptrdiff_t)r.row0 - lo + row0) * w.n_heads * HD + head * HD;
+        for (int n = 0; n < q_each && part + n * HEADS < w.n_heads; ++n) {
+#pragma unroll
+            for (int k = 0; k < TURNS; ++k)
+                if (mine(k)) {
+                    float y[8];
+                    finish(k, y);
+                    TQ* at = q + (ptrdiff_t)k * STRIDE * w.n_heads * HD;
+                    put4<TQ>(at + d0, y);
+                    put4<TQ>(at + d1, y + 4);
+                }
+            src += HEADS * HD;
+            col += HEADS * HD;
+            if (n + 1 < q_each && part + (n + 1) * HEADS < w.n_heads) get(src);
+            q += HEADS * HD;
+        }
+        return;
+    }
+    float y[TURNS][8];
+    if (here) {
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k)
+            if (mine(k)) finish(k, y[k]);
+    }
+    // the largest value, over the two warps of the rows' block; an infinity where one is no number
+    float a = 0.f;
+    bool fine = true;
+    if (here) {
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k)
+            if (mine(k)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    a = fmaxf(a, fabsf(y[k][i]));
+                    fine &= fabsf(y[k][i]) <= FLT_MAX;
+                }
+            }
+    }
+    a = warp_max(a);
+    if (!__all_sync(0xffffffffu, fine)) a = INFINITY;
+    if (lane == 0) most[warp] = a;
+    const size_t tile = (size_t)page * w.n_kv + head;
+    int8_t* codes = (is_k ? w.kc : w.vc) + (tile * PAGE + r.base % PAGE) * HD;
+    float* scale = (is_k ? w.ks : w.vs) + tile * PER_PAGE + r.base % PAGE / BLOCK;
+    const float had = there && lo > 0 ? *scale : 0.f;
+    __syncthreads();                                // both warps' maxima are there, and both have read the old scale
+    if (!there) return;
+    a = fmaxf(a, most[warp ^ 1]);
+    float s = a * (1.f / 127.f);
+    s = fmaxf(s < FLT_MIN ? 0.f : s, had);
+    if (!(a <= FLT_MAX) || had != had) s = __int_as_float(0x7fffffff);
+    const float inverse = s > 0.f ? 1.f / s : 0.f;
+    if (s > had && lo > 0) {
+        for (int k = 0, row = row0; k < TURNS && row < lo; ++k, row += STRIDE) {
+            uint32_t* at = reinterpret_cast<uint32_t*>(codes + row * HD);
+            at[d0 / 4] = rounded_again(at[d0 / 4], had * inverse);
+            at[d1 / 4] = rounded_again(at[d1 / 4], had * inverse);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < TURNS; ++k) {
+        if (!mine(k)) continue;
+        uint32_t* at = reinterpret_cast<uint32_t*>(codes + (row0 + k * STRIDE) * HD);
+        at[d0 / 4] = four_codes(y[k], inverse);
+        at[d1 / 4] = four_codes(y[k] + 4, inverse);
+    }
+    if (lane == 0 && warp % 2 == 0) *scale = s;
+}
+
+// Reading back: a block of threads takes a page of one kv head, keys and values, as many codes per thread and turn as make sixteen
+// bytes of values (a warp then writes whole sectors).  What bounds it is memory.
+constexpr int READERS = 256;
 struct Read {
     const int8_t *kc, *vc;
     const float *ks, *vs;
@@ -152,49 +375,47 @@ struct Read {
     int seen, span;                                                    // seen: from the first key that position seq_first sees (span)
 };
 
-template <typename T> __device__ __forceinline__ void put16(T* to, const float* v);
-template <> __device__ __forceinline__ void put16<float>(float* to, const float* v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(to)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-}
-template <> __device__ __forceinline__ void put16<__nv_bfloat16>(__nv_bfloat16* to, const float* v) {
-    reinterpret_cast<uint4*>(to)[0] = pack8(v);
-    reinterpret_cast<uint4*>(to)[1] = pack8(v + 8);
-}
-
 template <typename T, bool VEC>
 __device__ __forceinline__ void read_tile(const Read& r, const int8_t* codes, const float* scales, T* out, int size, int head, int page,
                                           int base, int first, int len, int seq) {
     const size_t tile = (size_t)page * r.n_kv + head;
     codes += tile * PAGE * size;
     scales += tile * PER_PAGE;
-    const int step = VEC ? 16 : 1;
-    for (int e = threadIdx.x * step; e < PAGE * size; e += blockDim.x * step) {
-        const int row = e / size, d = e % size, pos = base + row;
-        T* to;
-        if (r.cu_rows != nullptr) {
-            if (pos < first || pos >= len) continue;
-            to = out + ((size_t)(r.cu_rows[seq] + pos - first) * r.n_kv + head) * size + d;
-        } else {
-            to = out + tile * PAGE * size + e;
-        }
-        const float s = scales[row / BLOCK];
-        const bool there = pos >= first && pos < len;    // the rest of a page reads as zeros
-        if (VEC) {
-            const int4 c = *reinterpret_cast<const int4*>(codes + e);
-            __align__(16) float v[16];
-            const int8_t* b = reinterpret_cast<const int8_t*>(&c);
+    constexpr int PER = VEC ? 16 / sizeof(T) : 1, AT_ONCE = VEC ? 4 : 1;             // codes that make sixteen bytes of values; pieces at once
+    for (int e0 = threadIdx.x * PER; e0 < PAGE * size; e0 += AT_ONCE * READERS * PER) {
+        uint2 c[AT_ONCE];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = there ? s * (float)b[i] : 0.f;
-            put16<T>(to, v);
-        } else {
-            *to = from_f32<T>(there ? s * (float)codes[e] : 0.f);
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int e = e0 + k * READERS * PER;
+            if (e >= PAGE * size) break;
+            if (PER == 8) c[k] = *reinterpret_cast<const uint2*>(codes + e);
+            else if (PER == 4) c[k].x = *reinterpret_cast<const uint32_t*>(codes + e);
+            else c[k].x = (uint8_t)codes[e];
+        }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int e = e0 + k * READERS * PER;
+            if (e >= PAGE * size) break;
+            const int row = e / size, d = e % size, pos = base + row;
+            T* to = out + tile * PAGE * size + e;
+            if (r.cu_rows != nullptr) {
+                if (pos < first || pos >= len) continue;
+                to = out + ((size_t)(r.cu_rows[seq] + pos - first) * r.n_kv + head) * size + d;
+            }
+            const float s = scales[row / BLOCK];
+            const bool there = pos >= first && pos < len;    // the rest of a page reads as zeros
+            __align__(16) float v[8];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[i] = there ? s * (float)(int8_t)((i < 4 ? c[k].x : c[k].y) >> (8 * (i & 3))) : 0.f;
+            if (PER == 8) *reinterpret_cast<uint4*>(to) = pack8(v);
+            else if (PER == 4) *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(v);
+            else *to = from_f32<T>(v[0]);
         }
     }
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) read_kernel(Read r) {
+__global__ void __launch_bounds__(READERS) read_kernel(Read r) {
     let_next_kernel_start();
     const int seq = blockIdx.x / r.pages, head = blockIdx.y;
     const int first = r.seen ? first_visible_key(r.seq_first[seq], r.span) : r.seq_first[seq], len = r.seq_len[seq];
@@ -209,27 +430,46 @@ __global__ void __launch_bounds__(256) read_kernel(Read r) {
     read_tile<T, VEC>(r, r.vc, r.vs, reinterpret_cast<T*>(r.v_out), r.v_hd, head, page, base, first, len, seq);
 }
 
-bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
-
 }  // namespace
 
 // src [tokens, ld] of src_dtype holds q heads, k heads, v heads (plus bias where one is given); queries, rotated, go to q_out
 // [tokens, n_heads * hd] of q_dtype, keys and values into the cache.  `rot` channels of q and k are rotated (0: none), style 0:
-// pairs (i, i + rot / 2), style 1: pairs (2i, 2i + 1).  max_new: the most tokens that a sequence brings.  clear: src is left zeroed.
+// pairs (i, i + rot / 2), style 1: pairs (2i, 2i + 1).  n_tokens: rows of src; max_new: the most tokens that a sequence brings.  clear: src is left zeroed.
 RI_API int ri_quantized_write(void* src, int src_dtype, int ld, const float* bias, int clear, void* q_out, int q_dtype, const float* cos_t,
                               const float* sin_t, const int* page_table, int max_pages, const int* seq_slot, const int* seq_start,
-                              const int* cu_seqlens, int8_t* kc, int8_t* vc, float* ks, float* vs, int n_seqs, int max_new, int n_heads,
+                              const int* cu_seqlens, int8_t* kc, int8_t* vc, float* ks, float* vs, int n_tokens, int n_seqs, int max_new, int n_heads,
                               int n_kv, int hd, int v_hd, int rot, int style, cudaStream_t stream) {
     if (n_seqs <= 0 || max_new <= 0) return 0;
     if (hd <= 0 || v_hd <= 0 || hd % 2 || v_hd % 2) return fail("quantized_write: heads of %d and %d channels (even numbers wanted)", hd, v_hd);
     if (rot < 0 || rot % 2 || rot > hd) return fail("quantized_write: %d rotated channels of a head of %d", rot, hd);
     if (style != 0 && style != 1) return fail("quantized_write: unknown style %d", style);
     if (n_heads + 2 * n_kv > 65535) return fail("quantized_write: %d heads are too many", n_heads + 2 * n_kv);
-    const int runs = (max_new + 2 * BLOCK - 2) / BLOCK;
-    if ((long long)runs * n_seqs > 0x7fffffff) return fail("quantized_write: %d sequences of %d tokens are too many", n_seqs, max_new);
+    // blocks of positions: so many per sequence, or, where most sequences bring far fewer tokens than the longest, counted through
+    const long long each = (max_new + 2 * BLOCK - 2) / BLOCK, counted = n_tokens / BLOCK + 2ll * n_seqs;
+    const bool direct = each * n_seqs <= counted;
+    if ((direct ? each * n_seqs : counted) > 0x7fffffff) return fail("quantized_write: %d sequences of %d tokens are too many", n_seqs, max_new);
+    const int runs = (int)(direct ? each * n_seqs : counted);
     const Written w = {src, ld, bias, clear, q_out, cos_t, sin_t, page_table, seq_slot, seq_start, cu_seqlens, max_pages, kc, vc, ks, vs,
-                       n_heads, n_kv, hd, v_hd, rot, style, runs};
-    const dim3 grid((unsigned)(runs * n_seqs), (unsigned)(2 * n_kv + (q_out ? n_heads : 0)));
+                       n_heads, n_kv, hd, v_hd, rot, style, n_seqs, direct ? (int)each : 0};
+    const int heads = 2 * n_kv + (q_out ? n_heads : 0);
+    const int item = src_dtype == RI_F32 ? 4 : 2;
+    if ((hd == 64 || hd == 128) && v_hd == hd && (rot == 0 || rot == hd) && ld * item % 16 == 0 && aligned16(src) && aligned16(q_out) &&
+        aligned16(cos_t) && aligned16(sin_t) && aligned16(kc) && aligned16(vc)) {
+        // a warp takes one q head where the step would leave SMs idle otherwise, four of the same rows in a longer one (its address
+        // arithmetic and the angles' reads are then a quarter)
+        const int kv_blocks = (2 * n_kv + HEADS - 1) / HEADS;
+        const int q_each = (long long)runs * ((n_heads + HEADS - 1) / HEADS) > 8ll * sm_count() ? 4 : 1;
+        const int q_blocks = q_out ? (n_heads + HEADS * q_each - 1) / (HEADS * q_each) : 0;
+        const dim3 grid((unsigned)runs, (unsigned)(kv_blocks + q_blocks));
+        auto launch = [&](auto kernel) {
+            return check_launch(launch_dependent(kernel, grid, dim3(64 * HEADS), 0, stream, w, kv_blocks, q_each), "quantized_write");
+        };
+        using B = __nv_bfloat16;
+        if (src_dtype == RI_F32 && q_dtype == RI_F32) return hd == 64 ? launch(write_kernel<float, float, 64>) : launch(write_kernel<float, float, 128>);
+        if (src_dtype == RI_F32 && q_dtype == RI_BF16) return hd == 64 ? launch(write_kernel<float, B, 64>) : launch(write_kernel<float, B, 128>);
+        if (src_dtype == RI_BF16 && q_dtype == RI_BF16) return hd == 64 ? launch(write_kernel<B, B, 64>) : launch(write_kernel<B, B, 128>);
+    }
+    const dim3 grid((unsigned)runs, (unsigned)heads);
     auto launch = [&](auto kernel) { return check_launch(launch_dependent(kernel, grid, dim3(THREADS), 0, stream, w), "quantized_write"); };
     if (src_dtype == RI_F32 && q_dtype == RI_F32) return launch(write_any_kernel<float, float>);
     if (src_dtype == RI_F32 && q_dtype == RI_BF16) return launch(write_any_kernel<float, __nv_bfloat16>);
@@ -249,8 +489,8 @@ RI_API int ri_quantized_read(const int8_t* kc, const int8_t* vc, const float* ks
     if ((long long)pages * n_seqs > 0x7fffffff) return fail("quantized_read: %d sequences of %d positions are too many", n_seqs, max_len);
     const Read r = {kc, vc, ks, vs, k_out, v_out, page_table, seq_slot, seq_first, seq_len, cu_rows, max_pages, n_kv, hd, v_hd, pages, seen, span};
     const dim3 grid((unsigned)(pages * n_seqs), (unsigned)n_kv);
-    const bool vec = hd % 16 == 0 && v_hd % 16 == 0 && aligned16(kc) && aligned16(vc) && aligned16(k_out) && aligned16(v_out);
-    auto launch = [&](auto kernel) { return check_launch(launch_dependent(kernel, grid, dim3(256), 0, stream, r), "quantized_read"); };
+    const bool vec = hd % 8 == 0 && v_hd % 8 == 0 && aligned16(kc) && aligned16(vc) && aligned16(k_out) && aligned16(v_out);
+    auto launch = [&](auto kernel) { return check_launch(launch_dependent(kernel, grid, dim3(READERS), 0, stream, r), "quantized_read"); };
     if (dtype == RI_F32) return vec ? launch(read_kernel<float, true>) : launch(read_kernel<float, false>);
     if (dtype == RI_BF16) return vec ? launch(read_kernel<__nv_bfloat16, true>) : launch(read_kernel<__nv_bfloat16, false>);
     return fail("quantized_read: unknown dtype %d", dtype);

@@ -25,7 +25,7 @@ PAGE_SIZE, BLOCK = 64, 16
 # The entry points' arguments, one letter each, told to ctypes once: plain numbers then go through without an object for each.
 _KINDS = {"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float}
 _SIGNATURES = {
-    ("quantized_cache", "ri_quantized_write"): "piipipipppipppppppiiiiiiiip",
+    ("quantized_cache", "ri_quantized_write"): "piipipipppipppppppiiiiiiiiip",
     ("quantized_cache", "ri_quantized_read"): "ppppppipippppiiiiiiip",
     ("attention_quantized", "ri_attention_quantized"): "piipppppipppp" "iiiiiififplpp",
 }
@@ -116,8 +116,8 @@ def write(src: torch.Tensor, q_out: torch.Tensor | None, cos, sin, layer: Quanti
     _call("quantized_cache", "ri_quantized_write", src.data_ptr(), dtype_code(dtype), src.shape[1], None if bias is None else bias.data_ptr(),
           1 if clear else 0, None if q_out is None else q_out.data_ptr(), dtype_code(dtype if q_out is None else q_out.dtype),
           cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, _index(what, page_table, 1), page_table.shape[1],
-          _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs), _index(what, cu_seqlens, n_seqs + 1), k, v, ks, vs, n_seqs,
-          max_new, n_heads, n_kv_heads, head_dim, v_hd, rot, style, _stream())
+          _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs), _index(what, cu_seqlens, n_seqs + 1), k, v, ks, vs,
+          src.shape[0], n_seqs, max_new, n_heads, n_kv_heads, head_dim, v_hd, rot, style, _stream())
 
 
 def read(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, page_table: torch.Tensor, seq_slot, seq_first, seq_len, *,

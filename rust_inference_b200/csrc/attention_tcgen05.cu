@@ -39,9 +39,19 @@
 // bfloat16 terms (map_low: the second ones), which leaves one CTA on an SM (128 KiB).  A head's
 // result is multiplied by the sigmoid of the token's gate, if there are gates, before it is rounded.
 //
+// Over a cache in 8 bits (template HALF): keys and values lie in scratch pages as float16 numbers, the values of a sequence's kv head
+// over a power of two of their own (factors [sequences][2][kv heads]; quantized_cache.cu: widen_kernel), so that a code times its
+// scale has 11 significant bits, not 8.  A row's query is brought to [2^14, 2^15) by a power of two and made float16 in place, where
+// the copy put it, by the thread that has the row's softmax (a bfloat16 number is exact in float16 down to 2^-28 of the row's
+// largest); the powers go into the scale of the row's scores and into the factor on its result.  P is float16 too, times 2^6:
+// up to 2^14 between two moves of the maximum, 2^-12 of a weight down to 2^-20 of the largest.  (2,048 tokens of 28 heads of 128 over
+// 4, results against 64 bits: 4.1e-3 of their size by way of bfloat16 pages, 1.7e-3 this way, which is bfloat16's own rounding.)
+//
 // All mbarrier waits are bounded; on a timeout the kernel records a code in the host-visible
 // status word and winds down.
 #include "tcgen05_common.cuh"
+
+#include <cuda_fp16.h>
 
 using namespace ri;
 using namespace ri::tc;
@@ -92,8 +102,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
+__device__ __forceinline__ uint32_t pack2_half(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+
 // VD: the size of a value head; one below 64 takes a tile of 64 columns that the copy fills up with zeros, and so does the product
-template <int HD, int VD, bool FORMS, int LATENT = 0>
+template <int HD, int VD, bool FORMS, int LATENT = 0, bool HALF = false>
 __global__ void __launch_bounds__(THREADS, 2)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const int* __restrict__ page_table, int max_pages,
@@ -102,7 +117,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                        float out_scale, __nv_bfloat16* __restrict__ out, int out_ld, uint32_t smem_bytes, int* status,
                        float cap_log2, float scale_over_cap, int keep_first, const float* __restrict__ sink,
                        const __grid_constant__ CUtensorMap map_shared, const __grid_constant__ CUtensorMap map_low, const __nv_bfloat16* gate,
-                       int gate_ld) {
+                       int gate_ld, const float* factors) {
     constexpr int ATOMS = HD / 64;                       // 64-wide (128-byte) column tiles per row of head_dim
     constexpr int Q_BYTES = ATOMS * BM * 128;            // [atom][128 queries][64]
     constexpr int K_BYTES = ATOMS * BN * 128;            // one buffer: [atom][64 keys][64]
@@ -112,8 +127,9 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     constexpr int V_BUFS = LATENT ? 1 : 2;
     constexpr int S_COL = 0, O_COL = 2 * BN;             // two score buffers, then the output accumulator
     constexpr int TMEM_COLS = 256;
-    constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-    constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(V_ATOMS * 64 >> 3) << 17) |
+    constexpr uint32_t TYPES = HALF ? 0u : (1u << 7) | (1u << 10);      // both operands float16, or both bfloat16
+    constexpr uint32_t IDESC_S = (1u << 4) | TYPES | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+    constexpr uint32_t IDESC_PV = (1u << 4) | TYPES | (1u << 16) | ((uint32_t)(V_ATOMS * 64 >> 3) << 17) |
                                   ((uint32_t)(BM >> 4) << 24);
 
     // Everything lives in dynamic shared memory: the tiles (1024-byte aligned for the 128-byte swizzle) and,
@@ -123,6 +139,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     extern __shared__ uint8_t smem_raw[];
     struct Sync {
         uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full, pv_done;
+        uint64_t q_half;
         uint32_t tmem_base_slot;
         volatile int abort_flag;
     };
@@ -168,6 +185,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         mbar_init(smem_u32(&s_full[1]), 1);
         mbar_init(smem_u32(&p_full), 4);          // one arrival per softmax warp
         mbar_init(smem_u32(&pv_done), 1);
+        if constexpr (HALF) mbar_init(smem_u32(&sy.q_half), 4);      // one arrival per softmax warp
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -251,7 +269,9 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         // ---------------- MMA issuer ----------------
         {                                                        // the whole warp goes through, one lane issues
             const uint32_t leader = elect_one();
-            bool ok = mbar_wait_warp(smem_u32(&q_full), 0);
+            bool ok;
+            if constexpr (HALF) ok = mbar_wait_warp(smem_u32(&sy.q_half), 0);
+            else ok = mbar_wait_warp(smem_u32(&q_full), 0);
             if (!ok) { if (lane == 0) report(status, ST_ATTN_MMA); abort_flag = 1; }
             // The descriptors are built once, and a page's MMAs add constants to their address field (shared memory
             // ends below 256 KiB, so the 14-bit field never carries).
@@ -308,7 +328,43 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const uint32_t trow = tmem_base + ((uint32_t)lane_base << 16);
         float m_used = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int j = 0; j < n_pages; ++j) {
+        float row_scale = scale_log2;
+        if constexpr (HALF) {
+            // the row's queries as float16 numbers, sixteen bytes at a time, each eight rows' in different banks
+            wait_for_previous_kernels();                      // the factors come from the kernel before
+            if (!mbar_wait(smem_u32(&q_full), 0) || abort_flag) {
+                if (lane == 0) { report(status, ST_ATTN_SOFTMAX); abort_flag = 1; }
+                ok = false;
+            }
+            if (ok) {
+                uint4* const mine = reinterpret_cast<uint4*>(smem_raw + (q_smem - raw)) + r * 8;
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < ATOMS * 8; ++i) {
+                    float x[8];
+                    unpack8(mine[(i / 8) * BM * 8 + ((i + r) & 7)], x);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) top = fmaxf(top, fabsf(x[c]));
+                }
+                const int e = max((int)(__float_as_uint(top) >> 23) - 127, -112);
+                const float up = __uint_as_float((uint32_t)(127 + 14 - min(e, 127)) << 23);
+                row_scale = scale_log2 * (factors[(size_t)(2 * b) * n_kv_heads + kvh] * __uint_as_float((uint32_t)max(127 - 14 + e, 1) << 23));
+#pragma unroll
+                for (int i = 0; i < ATOMS * 8; ++i) {
+                    uint4& at = mine[(i / 8) * BM * 8 + ((i + r) & 7)];
+                    float x[8];
+                    unpack8(at, x);
+                    uint4 v;
+                    v.x = pack2_half(x[0] * up, x[1] * up), v.y = pack2_half(x[2] * up, x[3] * up);
+                    v.z = pack2_half(x[4] * up, x[5] * up), v.w = pack2_half(x[6] * up, x[7] * up);
+                    at = v;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the products read them through the other proxy
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sy.q_half));
+        }
+        for (int j = 0; j < n_pages && ok; ++j) {
             if (!mbar_wait(smem_u32(&s_full[j & 1]), (uint32_t)((j >> 1) & 1)) || abort_flag) {
                 if (lane == 0) { report(status, ST_ATTN_SOFTMAX); abort_flag = 1; }
                 ok = false;
@@ -329,7 +385,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     sv[c] = __float_as_uint(cap_log2 * (1.f - __fdividef(2.f, 1.f + e)));
                 }
             }
-            const float eff_scale = (FORMS && cap_log2 > 0.f) ? 1.f : scale_log2;
+            const float eff_scale = (FORMS && cap_log2 > 0.f) ? 1.f : row_scale;
             // The maximum is taken over the raw scores (the scale is positive), and scale and maximum
             // are folded into one multiply-add per score: p = 2^(s * scale_log2 - m).
             float mx_raw = -INFINITY;
@@ -355,7 +411,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const bool move = mx > m_used + (float)RESCALE_LOG2;
             const float m_new = move ? mx : m_used;
             const float alpha = (!move) ? 1.f : ((m_used == -INFINITY) ? 0.f : fast_exp2(m_used - m_new));
-            const float neg_mref = (m_new == -INFINITY) ? 0.f : -m_new;   // nothing visible yet: every p is 0
+            const float neg_mref = (m_new == -INFINITY) ? 0.f : (HALF ? 6.f : 0.f) - m_new;   // nothing visible yet: every p is 0
             // the exponentials do not need the previous P V product; everything after this does
             // two scores at a time through the packed float32 pipe (one FMA and one ADD per pair)
             const float2 scale2 = make_float2(eff_scale, eff_scale), shift2 = make_float2(neg_mref, neg_mref);
@@ -366,7 +422,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 const float2 e = __ffma2_rn(make_float2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), scale2, shift2);
                 const float2 p = make_float2(fast_exp2(e.x), fast_exp2(e.y));
                 sum2 = __fadd2_rn(sum2, p);
-                pk[c >> 1] = pack2(p.x, p.y);
+                pk[c >> 1] = HALF ? pack2_half(p.x, p.y) : pack2(p.x, p.y);
             }
             const float sum = sum2.x + sum2.y;
             if (j > 0) {
@@ -429,6 +485,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             // FORMS: a sink joins the row's sum as one more term exp(sink_h) without a value (2^x may overflow to infinity when
             // the sink outweighs every score: the result is then 0, as it should be)
             float inv = out_scale / ((FORMS && sink != nullptr) ? l + fast_exp2(fmaf(sink[h], 1.4426950408889634f, -m_used)) : l);
+            if (HALF) inv *= factors[(size_t)(2 * b + 1) * n_kv_heads + kvh];
             if (LATENT && gate != nullptr && r < rows)
                 inv = inv / (1.f + expf(-__bfloat162float(gate[(size_t)(tok0 + q0 + r) * gate_ld + h])));
             __nv_bfloat16* dst = out + (size_t)(tok0 + q0 + r) * out_ld + (size_t)h * VD;
@@ -462,18 +519,18 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     }
 }
 
-template <int HD, int VD, bool FORMS, int LATENT = 0>
+template <int HD, int VD, bool FORMS, int LATENT = 0, bool HALF = false>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const int* page_table, int max_pages,
            const int* seq_slot, const int* seq_start, const int* cu_seqlens, int n_seqs, int max_new, int n_heads,
            int n_kv_heads, float scale, int window, float out_scale, void* out, int out_ld, int* status, cudaStream_t stream,
            float softcap = 0.f, int keep_first = 0, const float* sink = nullptr, const CUtensorMap* shared = nullptr,
-           const CUtensorMap* low = nullptr, const void* gate = nullptr, int gate_ld = 0) {
+           const CUtensorMap* low = nullptr, const void* gate = nullptr, int gate_ld = 0, const float* factors = nullptr) {
     constexpr int ATOMS = HD / 64;
     // Q, two K and two V pages, P, the barriers; with head_dim 128 no room for alignment padding is left if
     // two CTAs are to share an SM (the kernel refuses, with a status code, a shared window that needs any)
     constexpr int TILES = ATOMS * BM * 128 + (2 * ATOMS + (LATENT == 1 ? 1 : 2) * ((VD + 63) / 64)) * BN * 128;
     constexpr int SMEM = TILES + (HD >= 128 && VD >= 128 ? 256 : 1024 + 256);
-    auto kernel = attn_prefill_tc_kernel<HD, VD, FORMS, LATENT>;
+    auto kernel = attn_prefill_tc_kernel<HD, VD, FORMS, LATENT, HALF>;
     static PerDeviceOnce configured;       // per device: the attribute belongs to a device's copy of the kernel
     if (int rc = raise_dynamic_smem(kernel, SMEM, configured, "attention_tcgen05")) return rc;
     // blocks are handed out x fastest: every head and sequence of the longest query tiles first, the short
@@ -485,7 +542,7 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
                                      out_scale, (__nv_bfloat16*)out, out_ld, (uint32_t)SMEM, status,
                                      softcap * 1.4426950408889634f, softcap > 0.f ? scale / softcap : 0.f, keep_first, sink, shared != nullptr ? *shared : mk,
                                      low != nullptr ? *low : mk,
-                                     (const __nv_bfloat16*)gate, gate_ld);
+                                     (const __nv_bfloat16*)gate, gate_ld, factors);
     return check_launch(e, "attention_tcgen05");
 }
 
@@ -528,6 +585,28 @@ RI_API int ri_attention_tcgen05_prefill(const void* map_q, const void* map_k, co
     RI_LAUNCH(64, 32); RI_LAUNCH(64, 64); RI_LAUNCH(64, 128); RI_LAUNCH(128, 32); RI_LAUNCH(128, 64); RI_LAUNCH(128, 128);
 #undef RI_LAUNCH
     return fail("attention_tcgen05: no kernel for heads of %d with values of %d", hd, v_hd);
+}
+
+// The same over pages of float16 numbers (`HALF` above): factors float32 [n_seqs][2][n_kv_heads], what the keys and the values of a
+// sequence's kv head are to be multiplied by.  Queries and result are bfloat16; values have the keys' head size.
+RI_API int ri_attention_tcgen05_prefill_half(const void* map_q, const void* map_k, const void* map_v, const int* page_table, int max_pages,
+                                             const int* seq_slot, const int* seq_start, const int* cu_seqlens, void* out, int out_ld,
+                                             int n_seqs, int max_new, int n_heads, int n_kv_heads, int hd, int page_size, float scale,
+                                             int window, float out_scale, const float* factors, int* status, cudaStream_t stream) {
+    if (n_seqs <= 0 || max_new <= 0) return 0;
+    if (!ri_attention_tcgen05_supports(hd, hd, page_size, n_heads, n_kv_heads, 8, out_ld))
+        return fail("attention_tcgen05: head_dim %d, pages of %d, %d heads over %d kv heads, out rows of %d are not supported",
+                    hd, page_size, n_heads, n_kv_heads, out_ld);
+    if ((uintptr_t)out % 16) return fail("attention_tcgen05: out is not 16-byte aligned");
+    if (n_heads > 65535 || n_seqs > 65535) return fail("attention_tcgen05: %d heads / %d sequences exceed the grid limit", n_heads, n_seqs);
+    const CUtensorMap& mq = *reinterpret_cast<const CUtensorMap*>(map_q);
+    const CUtensorMap& mk = *reinterpret_cast<const CUtensorMap*>(map_k);
+    const CUtensorMap& mv = *reinterpret_cast<const CUtensorMap*>(map_v);
+#define RI_LAUNCH(H) if (hd == H) return launch<H, H, false, 0, true>(mq, mk, mv, page_table, max_pages, seq_slot, seq_start, cu_seqlens, n_seqs, max_new, \
+        n_heads, n_kv_heads, scale, window, out_scale, out, out_ld, status, stream, 0.f, 0, nullptr, nullptr, nullptr, nullptr, 0, factors)
+    RI_LAUNCH(64); RI_LAUNCH(128);
+#undef RI_LAUNCH
+    return fail("attention_tcgen05: no kernel for heads of %d", hd);
 }
 
 // The same with capped scores (softcap > 0: s <- softcap tanh(s scale / softcap)) and, with a window (> 0 only: the last

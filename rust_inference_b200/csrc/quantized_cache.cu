@@ -16,6 +16,7 @@
 // scale each time.
 #include "common.cuh"
 
+#include <cuda_fp16.h>
 #include <float.h>
 
 using namespace ri;
@@ -430,7 +431,108 @@ __global__ void __launch_bounds__(READERS) read_kernel(Read r) {
     read_tile<T, VEC>(r, r.vc, r.vs, reinterpret_cast<T*>(r.v_out), r.v_hd, head, page, base, first, len, seq);
 }
 
+// A cache's pages for the prompts' attention (attention_tcgen05.cu): as float16 numbers over a power of two of their own per
+// sequence and kv head, the one that brings the largest scale of the blocks that are read to [2^7, 2^8).  A block of threads takes
+// a page of one kv head and finds that scale for itself (four numbers a page).  What a sequence does not see, before its first
+// seen block and behind its end, is 0.  A block that is no number is that in its keys, whose scores a row that does not see them
+// leaves out, and 0 in its values, which every row's sum runs over.
+struct Widen {
+    const int8_t *kc, *vc;
+    const float *ks, *vs;
+    __half *k_out, *v_out;
+    float* factors;              // [sequences][2][kv heads]
+    const int *page_table, *seq_slot, *seq_start, *seq_len;
+    int max_pages, n_kv, pages, span;
+};
+constexpr int WIDENERS = 256;
+
+__device__ __forceinline__ float power_above(float scale) {            // 2^e with scale / 2^e in [2^7, 2^8); 1 for no scale
+    const int e = (int)(__float_as_uint(scale) >> 23) - 127 - 7;
+    return scale > 0.f ? __uint_as_float((uint32_t)(127 + max(e, -126)) << 23) : 1.f;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(WIDENERS) widen_kernel(Widen w) {
+    __shared__ float scratch[33];
+    __shared__ float scales[2][PER_PAGE];
+    let_next_kernel_start();
+    const int seq = blockIdx.x / w.pages, head = blockIdx.y, tid = threadIdx.x;
+    const int start = w.seq_start[seq], len = w.seq_len[seq];
+    const int first = first_visible_key(start, w.span) / BLOCK, last = (len - 1) / BLOCK;      // blocks that are seen
+    const int index = first / PER_PAGE + (int)(blockIdx.x % w.pages), end = last / PER_PAGE + 1;
+    const int slot = w.seq_slot[seq];
+    wait_for_previous_kernels();
+    if (len <= start || index >= end) return;
+    if (!RI_BLOCK_IN_LIMIT(slot, RI_LIMIT_SLOTS, RI_CHECK_SLOT) || !RI_BLOCK_IN_RANGE(end - 1, w.max_pages, RI_CHECK_PAGE_INDEX)) return;
+    const int* pages = w.page_table + (size_t)slot * w.max_pages;
+    const int page = pages[index];
+    if (!RI_BLOCK_IN_LIMIT(page, RI_LIMIT_PAGES, RI_CHECK_PAGE)) return;
+    const size_t tile = (size_t)page * w.n_kv + head;
+    constexpr int TURNS = PAGE * HD / 8 / WIDENERS;
+    uint2 k[TURNS], v[TURNS];
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+        k[i] = reinterpret_cast<const uint2*>(w.kc + tile * PAGE * HD)[tid + i * WIDENERS];
+        v[i] = reinterpret_cast<const uint2*>(w.vc + tile * PAGE * HD)[tid + i * WIDENERS];
+    }
+    float k_top = 0.f, v_top = 0.f;                 // (fmaxf leaves out what is no number)
+    for (int b = first + tid; b <= last; b += WIDENERS) {
+        const int p = pages[b / PER_PAGE];
+        if (!RI_IN_LIMIT(p, RI_LIMIT_PAGES, RI_CHECK_PAGE)) continue;
+        const size_t at = ((size_t)p * w.n_kv + head) * PER_PAGE + b % PER_PAGE;
+        k_top = fmaxf(k_top, w.ks[at]);
+        v_top = fmaxf(v_top, w.vs[at]);
+    }
+    const float k_unit = power_above(block_max(k_top, scratch)), v_unit = power_above(block_max(v_top, scratch));
+    if (tid < PER_PAGE) {
+        const int b = index * PER_PAGE + tid;
+        const bool seen = b >= first && b <= last;
+        const float ks = seen ? w.ks[tile * PER_PAGE + tid] : 0.f, vs = seen ? w.vs[tile * PER_PAGE + tid] : 0.f;
+        scales[0][tid] = vs != vs ? vs : ks / k_unit;
+        scales[1][tid] = vs != vs ? 0.f : vs / v_unit;
+    }
+    if (index == first / PER_PAGE && tid == 0) {
+        w.factors[(size_t)(2 * seq) * w.n_kv + head] = k_unit;
+        w.factors[(size_t)(2 * seq + 1) * w.n_kv + head] = v_unit;
+    }
+    __syncthreads();
+    auto widened = [&](const uint2& c, float s, bool there) {
+        uint4 o;
+        __half2* h = reinterpret_cast<__half2*>(&o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t two = (i < 2 ? c.x : c.y) >> (16 * (i & 1));
+            h[i] = there ? __floats2half2_rn(s * (float)(int8_t)two, s * (float)(int8_t)(two >> 8)) : __floats2half2_rn(0.f, 0.f);
+        }
+        return o;
+    };
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+        const int e = tid + i * WIDENERS, row = e / (HD / 8);
+        const bool there = index * PAGE + row < len;
+        reinterpret_cast<uint4*>(w.k_out + tile * PAGE * HD)[e] = widened(k[i], scales[0][row / BLOCK], there);
+        reinterpret_cast<uint4*>(w.v_out + tile * PAGE * HD)[e] = widened(v[i], scales[1][row / BLOCK], there);
+    }
+}
+
 }  // namespace
+
+// The pages that a step's queries see (all keys, or a span of them: first_visible_key) as float16 numbers, of the cache's shape, and
+// float32 factors [n_seqs][2][n_kv] that keys and values are to be multiplied by.  Heads of 64 or 128; max_len: no sequence is longer.
+RI_API int ri_quantized_widen(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, void* k_out, void* v_out, float* factors,
+                              const int* page_table, int max_pages, const int* seq_slot, const int* seq_start, const int* seq_len,
+                              int n_seqs, int max_len, int n_kv, int hd, int span, cudaStream_t stream) {
+    if (n_seqs <= 0 || max_len <= 0) return 0;
+    if (hd != 64 && hd != 128) return fail("quantized_widen: heads of %d channels (64 or 128 wanted)", hd);
+    if (n_kv > 65535) return fail("quantized_widen: %d kv heads are too many", n_kv);
+    if (!aligned16(kc) || !aligned16(vc) || !aligned16(k_out) || !aligned16(v_out)) return fail("quantized_widen: pages must lie on 16-byte boundaries");
+    const int pages = (max_len + PAGE - 1) / PAGE;
+    if ((long long)pages * n_seqs > 0x7fffffff) return fail("quantized_widen: %d sequences of %d positions are too many", n_seqs, max_len);
+    const Widen w = {kc, vc, ks, vs, (__half*)k_out, (__half*)v_out, factors, page_table, seq_slot, seq_start, seq_len, max_pages, n_kv, pages, span};
+    const dim3 grid((unsigned)(pages * n_seqs), (unsigned)n_kv);
+    auto launch = [&](auto kernel) { return check_launch(launch_dependent(kernel, grid, dim3(WIDENERS), 0, stream, w), "quantized_widen"); };
+    return hd == 64 ? launch(widen_kernel<64>) : launch(widen_kernel<128>);
+}
 
 // src [tokens, ld] of src_dtype holds q heads, k heads, v heads (plus bias where one is given); queries, rotated, go to q_out
 // [tokens, n_heads * hd] of q_dtype, keys and values into the cache.  `rot` channels of q and k are rotated (0: none), style 0:

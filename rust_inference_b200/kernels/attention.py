@@ -243,7 +243,21 @@ QUANTIZED_ROWS = 64
 
 
 def _over_quantized(qkv, layer, out, ctx, *, window, chunk, keep_first, **forms):
-    """`attention` over a cache in 8 bits by way of the run dtype."""
+    """`attention` over a cache in 8 bits by way of scratch pages: float16 numbers for bfloat16 prompts with the plain form of the
+    score, else the run dtype for the kernels that a cache in it has."""
+    heads, kv, hd = forms["n_heads"], forms["n_kv_heads"], forms["head_dim"]
+    plain = not (forms["softcap"] or keep_first or any(forms[n] is not None for n in ("sink", "dist", "gate"))) and not (window and chunk)
+    if plain and qkv.dtype == torch.bfloat16 and layer.sizes == (kv, hd, hd) and layer.aligned and _PREFILL != "mma":
+        from . import attention_tc
+        if attention_tc.supports(hd, ctx.page_size, heads, kv, qkv.shape[1], out.shape[1]):
+            span = window if window else -int(chunk or 0)
+            k = ctx.buffer("widened_k", layer.k.shape, torch.float16)
+            v = ctx.buffer("widened_v", layer.v.shape, torch.float16)
+            factors = ctx.buffer("widened_factors", (ctx.n_seqs, 2, kv), torch.float32)
+            quantized_cache.widen(layer, k, v, factors, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.seq_len, max_len=ctx.max_len, span=span)
+            return attention_tc.prefill_half(qkv, k, v, factors, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens, out,
+                                             n_seqs=ctx.n_seqs, max_new=ctx.max_new, n_heads=heads, n_kv_heads=kv, head_dim=hd,
+                                             page_size=ctx.page_size, scale=forms["scale"], window=span, out_scale=forms["out_scale"])
     k = ctx.buffer("readback_k", layer.k.shape, qkv.dtype)
     v = ctx.buffer("readback_v", layer.v.shape, qkv.dtype)
     # (a captured step may run with longer sequences than it was captured with)

@@ -81,6 +81,27 @@ def prefill(qkv: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, page_
     return out
 
 
+def prefill_half(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, factors: torch.Tensor, page_table, seq_slot, seq_start, cu_seqlens,
+                 out: torch.Tensor, *, n_seqs: int, max_new: int, n_heads: int, n_kv_heads: int, head_dim: int, page_size: int, scale: float,
+                 window: int = 0, out_scale: float = 1.0) -> torch.Tensor:
+    """`prefill` over pages of float16 numbers that are to be multiplied by a factor per sequence and kv head
+    (`quantized_cache.widen`); q and out are bfloat16."""
+    _need_cuda(q, k, v, factors, page_table, seq_slot, seq_start, cu_seqlens, out)
+    _need(q.dtype == torch.bfloat16 and k.dtype == v.dtype == torch.float16 and out.dtype == torch.bfloat16 and q.is_contiguous()
+          and k.is_contiguous() and v.is_contiguous() and out.is_contiguous() and v.shape == k.shape and out.shape[1] >= n_heads * head_dim
+          and tuple(k.shape[1:]) == (n_kv_heads, page_size, head_dim), "attention_tcgen05: bfloat16 queries over float16 pages")
+    _need(factors.dtype == torch.float32 and factors.numel() >= 2 * n_seqs * n_kv_heads, "attention_tcgen05: factors")
+    rows = k.shape[0] * k.shape[1] * k.shape[2]
+    mq = _map(0, q, q.shape[0], q.shape[1], q.shape[1])
+    mk, mv = _map(1, k, rows, head_dim, head_dim), _map(1, v, rows, head_dim, head_dim)
+    st = status_word()
+    _call("attention_tcgen05", "ri_attention_tcgen05_prefill_half", c_void_p(mq.data_ptr()), c_void_p(mk.data_ptr()), c_void_p(mv.data_ptr()),
+          _p(page_table), c_int(page_table.shape[1]), _p(seq_slot), _p(seq_start), _p(cu_seqlens), _p(out), c_int(out.shape[1]), c_int(n_seqs),
+          c_int(max_new), c_int(n_heads), c_int(n_kv_heads), c_int(head_dim), c_int(page_size), c_float(scale), c_int(window),
+          c_float(out_scale), _p(factors), c_void_p(st.data_ptr()), _stream())
+    return out
+
+
 EXPANDED_SIZES = (128, 64, 128)      # a head's own key channels, the key channels shared by all heads, value channels
 
 

@@ -27,6 +27,7 @@ _KINDS = {"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float}
 _SIGNATURES = {
     ("quantized_cache", "ri_quantized_write"): "piipipipppipppppppiiiiiiiiip",
     ("quantized_cache", "ri_quantized_read"): "ppppppipippppiiiiiiip",
+    ("quantized_cache", "ri_quantized_widen"): "ppppppppipppiiiiip",
     ("attention_quantized", "ri_attention_quantized"): "piipppppipppp" "iiiiiififplpp",
 }
 
@@ -145,6 +146,27 @@ def read(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, page_t
           _index(what, seq_len, n_seqs), None if cu_rows is None else _index(what, cu_rows, n_seqs), n_seqs, max_len, n_kv, hd, v_hd,
           0 if seen_span is None else 1, seen_span or 0, _stream())
     return k_out, v_out
+
+
+def widen(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, factors: torch.Tensor, page_table: torch.Tensor, seq_slot,
+          seq_start, seq_len, *, max_len: int, span: int = 0) -> None:
+    """The pages that a step's queries see as float16 numbers for `attention_tc.prefill_half`: k_out, v_out float16 of the cache's
+    shape, and factors float32 [sequences, 2, kv heads] that keys and values are to be multiplied by.  What is outside a sequence's
+    seen blocks is 0; a block that is no number is that in its keys."""
+    what = "quantized_cache.widen"
+    n_kv, hd, v_hd = layer.sizes
+    n_seqs = seq_slot.numel()
+    _need(layer.aligned and v_hd == hd and hd in (64, 128), what, "heads of 64 or 128 channels, keys and values alike")
+    _need(k_out.is_cuda and v_out.is_cuda and k_out.dtype == v_out.dtype == torch.float16 and k_out.is_contiguous() and v_out.is_contiguous()
+          and k_out.shape == layer.k.shape and v_out.shape == layer.v.shape, what, "outputs must be float16 of the cache's shape")
+    _need(factors.is_cuda and factors.dtype == torch.float32 and factors.is_contiguous() and factors.numel() >= 2 * n_seqs * n_kv, what,
+          "factors must be float32 [sequences, 2, kv heads]")
+    _need(page_table.dim() == 2, what, "the page table must be int32 [slots, pages]")
+    _prepare("quantized_cache", "ri_quantized_widen")
+    k, v, ks, vs = layer.pointers
+    _call("quantized_cache", "ri_quantized_widen", k, v, ks, vs, k_out.data_ptr(), v_out.data_ptr(), factors.data_ptr(),
+          _index(what, page_table, 1), page_table.shape[1], _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs),
+          _index(what, seq_len, n_seqs), n_seqs, max_len, n_kv, hd, span, _stream())
 
 
 @functools.lru_cache(maxsize=None)

@@ -309,6 +309,40 @@ def test_attention_past_what_it_does_not_see(hd, dtype):
     assert out[:3].isfinite().all() and out[3].isnan().all()
 
 
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prompts_past_what_they_do_not_see(hd, dtype, window):
+    """The same for prompts of many rows: who does not see a marked block is as without it, and who does is no number."""
+    from rust_inference_b200.kernels import attention
+    runs = [(0, 130), (37, 90), (0, 50)]
+    step = Step(runs, 2, hd)
+    step.arrays([(s + n, 0) for s, n in runs])
+    step.fill()
+    step.arrays(runs)
+    q = torch.randn(step.n_tokens, 8 * hd, device=DEV).to(dtype)
+    call = dict(n_heads=8, n_kv_heads=2, head_dim=hd, scale=0.1, window=window)
+    want = torch.empty_like(q)
+    attention.attention(q, step.layer, want, step.context(dtype), **call)
+    assert want.isfinite().all()
+    step.layer.k_scale[step.pages(0)[1].item(), 0, 0] = math.nan         # sequence 0: positions 64..79 of kv head 0
+    step.layer.v_scale[step.pages(1)[1].item(), 1, 1] = math.nan         # sequence 1: positions 80..95 of kv head 1
+    step.layer.v_scale[step.pages(2)[0].item(), :, 3] = math.nan         # sequence 2: its last block
+    got = torch.empty_like(q)
+    attention.attention(q, step.layer, got, step.context(dtype), **call)
+    bad = torch.zeros(step.n_tokens, 8, dtype=torch.bool)
+    for b, head, low, high in ((0, 0, 64, 80), (1, 1, 80, 96), (2, 0, 48, 64), (2, 1, 48, 64)):
+        start, n = runs[b]
+        for t in range(n):
+            pos = start + t
+            first = max(0, pos - window + 1) if window else 0
+            if pos >= low and first < high:
+                bad[step.cu[b] + t, 4 * head:4 * head + 4] = True
+    got, want = got.view(-1, 8, hd).cpu(), want.view(-1, 8, hd).cpu()
+    assert got[bad].isnan().all()
+    assert torch.equal(got[~bad], want[~bad]) or (got[~bad].float() - want[~bad].float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+
+
 def test_attention_of_large_and_small_queries_and_scales():
     """Queries, keys and values far from one: the float32 result stays as near as the sums allow."""
     from rust_inference_b200.kernels import attention

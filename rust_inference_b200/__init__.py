@@ -17,7 +17,7 @@ from .config.registry import (config_from_dict, load_config, register_architectu
                               registered_architectures)
 from .sampling.params import SamplerConfig
 
-__all__ = ["Model", "SamplerConfig", "GenerationResult", "DenseDecoderConfig", "ConfigError",
+__all__ = ["Model", "SamplerConfig", "GenerationResult", "TokenScores", "DenseDecoderConfig", "ConfigError",
            "config_from_dict", "load_config", "register_architecture", "registered_architectures",
            "write_random_model"]
 
@@ -27,6 +27,9 @@ def __getattr__(name):
     if name == "Model":
         from .api import Model
         return Model
+    if name == "TokenScores":
+        from .api import TokenScores
+        return TokenScores
     if name == "GenerationResult":
         from .engine.generate import GenerationResult
         return GenerationResult

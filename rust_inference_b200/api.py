@@ -1,10 +1,28 @@
 """The Python entry point: load a model folder, generate from token ids."""
 from __future__ import annotations
 
+import math
+from dataclasses import dataclass
+
 from .engine.engine import Engine, resolve_max_seq_len
 from .engine.generate import GenerationResult, Generator
 from .sampling.params import SamplerConfig
 from .sampling.sampler import Sampler
+
+
+SCORE_LOGITS = 1 << 26             # logits that `Model.score` holds at a time
+
+
+@dataclass
+class TokenScores:
+    logprobs: list                 # of every token but the first, given those before it (nats)
+    entropies: list                # of the distributions they were drawn from
+    top: list | None               # per token: [(id, log probability)], likeliest first
+
+    @property
+    def perplexity(self) -> float:
+        """e to the mean of the negative log probabilities."""
+        return math.exp(-sum(self.logprobs) / len(self.logprobs))
 
 
 class Model:
@@ -17,27 +35,30 @@ class Model:
 
     @classmethod
     def load(cls, path: str, max_seq_len: int | None = None, *, dtype: str = "bfloat16",
-             device: str = "cuda", max_tokens_in_cache: int | None = None, n_slots: int | None = None) -> "Model":
+             device: str = "cuda", max_tokens_in_cache: int | None = None, n_slots: int | None = None,
+             cache_dtype: str | None = None) -> "Model":
         """path: a folder with config.json and model.safetensors (or shards with an index).
         max_seq_len overrides the model's context length, as `--max-seq-len` does in the
         reference (model.rs:142-144): it caps the cache and the rotary table.
         max_tokens_in_cache: positions all live sequences may hold together (default: 8 sequences
-        of max_seq_len, at most 65,536 positions)."""
+        of max_seq_len, at most 65,536 positions).
+        cache_dtype: "int8" keeps keys and values in 8 bits (see `Engine`); default: in `dtype`."""
         from .config.registry import load_spec
         seq = resolve_max_seq_len(max_seq_len, load_spec(path)[1].max_positions)
         if max_tokens_in_cache is None:
             max_tokens_in_cache = min(8 * seq, max(seq, 65536))
         return cls(Engine.from_pretrained(path, dtype=dtype, device=device, max_tokens=max_tokens_in_cache,
-                                          max_seq_len=seq, n_slots=n_slots))
+                                          max_seq_len=seq, n_slots=n_slots, cache_dtype=cache_dtype))
 
     @classmethod
     def random(cls, config, *, seed: int = 0, std: float = 0.02, norm_std: float = 0.0, dtype: str = "bfloat16",
                device: str = "cuda", max_seq_len: int | None = None, max_tokens_in_cache: int = 65536,
-               n_slots: int | None = None) -> "Model":
+               n_slots: int | None = None, cache_dtype: str | None = None) -> "Model":
         """A model with random weights made on the device from a typed config and a seed: matrices and
         biases N(0, std), norm weights 1 + N(0, norm_std)."""
         return cls(Engine.from_random(config, seed=seed, std=std, norm_std=norm_std, dtype=dtype, device=device,
-                                      max_tokens=max_tokens_in_cache, max_seq_len=max_seq_len, n_slots=n_slots))
+                                      max_tokens=max_tokens_in_cache, max_seq_len=max_seq_len, n_slots=n_slots,
+                                      cache_dtype=cache_dtype))
 
     def memory(self) -> dict:
         """Bytes the model holds on the device and what a decode step has to read of them: the weights
@@ -57,9 +78,12 @@ class Model:
             for req in flat(entry):
                 if req is not None and hasattr(req, "n_kv_heads"):
                     values = 0 if getattr(req, "values_in_keys", False) else (req.v_head_dim or req.head_dim)
-                    per_position += req.n_kv_heads * (req.head_dim + values) * item
+                    if eng.cache.kv_dtype is None:
+                        per_position += req.n_kv_heads * (req.head_dim + values) * item
+                    else:                        # a byte per number, and a block's two scales shared by its positions
+                        per_position += req.n_kv_heads * (req.head_dim + values + 2 * 4 / 16)
         return {"weight_bytes": eng.model.weight_bytes(), "weight_bytes_per_step": eng.model.weight_bytes(False),
-                "cache_bytes": eng.cache.bytes(), "cache_bytes_per_position": per_position}
+                "cache_bytes": eng.cache.bytes(), "cache_bytes_per_position": int(per_position)}
 
     def state_dict(self) -> dict:
         """name -> tensor for every tensor of the model, under the weight file's names, as held on the
@@ -99,6 +123,41 @@ class Model:
         if probe is not None:
             layer_stats.extend(probe.stats[0])
         return out
+
+    def score(self, tokens, top: int = 0) -> "TokenScores":
+        """How likely the model finds a text: for every token but the first its log probability given those before it, the
+        entropy of the distribution it was drawn from and, with top > 0, that distribution's likeliest tokens
+        (`ops.token_logprobs`).  The text runs in pieces whose logits fit in a quarter of a gigabyte, against the cache as the
+        engine keeps it, so that the scores of a cache in 8 bits can be compared with those of another.  `tokens`: one list of
+        at least two token ids; the sequence's slot is given back afterwards."""
+        import torch
+        from .kernels import ops
+        tokens = [int(t) for t in tokens]
+        if len(tokens) < 2:
+            raise ValueError("score: a text of at least two tokens")
+        eng = self.engine
+        vocab = eng.model.spec.vocab_size
+        if not 0 <= tokens[-1] < vocab:
+            raise ValueError(f"score: a token id outside [0, {vocab}): {tokens[-1]}")
+        piece = max(1, SCORE_LOGITS // vocab)
+        parts = []
+        slot = eng.alloc_slot()
+        try:
+            for at in range(0, len(tokens) - 1, piece):
+                end = min(at + piece, len(tokens) - 1)
+                logits = eng.step([slot], [tokens[at:end]], "all", borrow=True)
+                targets = torch.tensor(tokens[at + 1:end + 1], dtype=torch.int32).to(logits.device)
+                with torch.cuda.device(eng.device):
+                    parts.append(ops.token_logprobs(logits, targets, top=top))
+        finally:
+            eng.free_slot(slot)
+        logprobs, entropies = (torch.cat([p[i] for p in parts]).tolist() for i in range(2))
+        eng.check_device_status()
+        likeliest = None
+        if top:
+            ids, best = (torch.cat([p[i] for p in parts]).tolist() for i in (2, 3))
+            likeliest = [list(zip(i, b)) for i, b in zip(ids, best)]
+        return TokenScores(logprobs, entropies, likeliest)
 
     def generate(self, prompts, max_tokens: int = 512, sampler_config: SamplerConfig | None = None,
                  stop_ids=None, max_batch: int | None = None, record_step_times: bool = False) -> list:

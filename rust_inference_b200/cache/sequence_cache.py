@@ -12,6 +12,9 @@ form a *group* with storage of its own:
                values are the leading channels of its keys (one row per position that serves as
                both, as attention over a shared latent keeps it): then there is no V, and the
                layer's `v` is its `k`.
+               With `kv_dtype` int8 a group holds 8-bit codes and their scales instead (`kernels.quantized_cache`): K, V as above
+               but int8, and per page and kv head one float32 scale for every 16 positions of each.  Layers whose request
+               does not say that it can be held so are refused.
   state group  [layers in group, slots, *shape]: state of fixed size per sequence, zeroed
                when the slot is handed out (a recurrent mixer's matrix state, for one).
 
@@ -27,7 +30,7 @@ reference's per-layer `[max_seq_len, kv_dim]` pair with one length counter
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import numpy as np
 import torch
@@ -44,6 +47,7 @@ class KVRequest:
     window: int | None = None      # None: the layer reads all keys
     v_head_dim: int | None = None  # None: values have the keys' head size
     values_in_keys: bool = False   # the values are the first v_head_dim channels of the keys: no storage of their own
+    quantizable: bool = field(default=False, compare=False)    # the layer writes and reads a cache in 8 bits if it is given one
 
 
 @dataclass(frozen=True)
@@ -73,10 +77,14 @@ class CompositeLayer:
 
 class SequenceCache:
     def __init__(self, requests: list, *, max_tokens: int, max_seq_len: int, dtype: torch.dtype,
-                 device, n_slots: int | None = None, page_size: int = PAGE_SIZE):
-        """requests[i] is what cache layer i needs (KVRequest, StateRequest or None).
+                 device, n_slots: int | None = None, page_size: int = PAGE_SIZE, kv_dtype: torch.dtype | None = None):
+        """requests[i] is what cache layer i needs (KVRequest, StateRequest or None).  `kv_dtype`: None, keys and values in the run
+        dtype, or torch.int8.
         `max_tokens` is the number of positions all live sequences may hold together, each
         sequence's count rounded up to a whole page."""
+        if kv_dtype not in (None, torch.int8):
+            raise ValueError(f"cache: keys and values are kept in the run dtype or as int8, not {kv_dtype}")
+        self.kv_dtype = kv_dtype
         self.device = torch.device(device)
         self.dtype = dtype
         self.page_size = page_size
@@ -109,6 +117,8 @@ class SequenceCache:
                 for m, sub in enumerate(req):
                     enlist(sub, path + (m,))
             elif req is not None:
+                if kv_dtype is not None and isinstance(req, KVRequest) and not req.quantizable:
+                    raise CacheError(f"cache layer {path[0]}: keys and values of this kind are not kept in 8 bits ({req})")
                 members.setdefault(req, []).append(path)
 
         def composites(req, path):
@@ -135,6 +145,18 @@ class SequenceCache:
         for req, users in members.items():
             if isinstance(req, KVRequest):
                 shape = (len(users), n_pages, req.n_kv_heads, page_size, req.head_dim)
+                if kv_dtype is not None:
+                    from ..kernels import quantized_cache
+                    if page_size != quantized_cache.PAGE_SIZE:
+                        raise ValueError(f"cache: pages of {page_size} positions are not kept in 8 bits")
+                    v_shape = shape[:-1] + (req.v_head_dim or req.head_dim,)
+                    s_shape = shape[:3] + (page_size // quantized_cache.BLOCK,)
+                    k, v = (torch.zeros(sh, dtype=kv_dtype, device=self.device) for sh in (shape, v_shape))
+                    ks, vs = (torch.zeros(s_shape, dtype=torch.float32, device=self.device) for _ in range(2))
+                    self.groups[req] = (k, v, ks, vs)
+                    for j, path in enumerate(users):
+                        place(path, quantized_cache.QuantizedPages(k[j], v[j], ks[j], vs[j], req))
+                    continue
                 k = torch.zeros(shape, dtype=dtype, device=self.device)
                 if req.values_in_keys:
                     if (req.v_head_dim or req.head_dim) > req.head_dim:

@@ -18,6 +18,10 @@ Added for a library that takes token ids and may run without a checkpoint:
   --bench                                   after generating, one JSON line on standard error: steps, prompt and
                                             generated tokens, seconds, tokens per second, bytes copied, the model's
                                             bytes on the device
+  --cache-dtype int8                        keys and values in 8 bits instead of the run dtype
+  --score K                                 instead of generating: for every token of a prompt but the first one line with its
+                                            id, its log probability, the entropy of its distribution and the K likeliest
+                                            tokens; per prompt the perplexity on standard error
   --dump-layer-stats                        min / max / mean / first values of the hidden vector at position 0
                                             after every layer, as debug builds of the reference print them
                                             (transformer.rs:80-96)
@@ -51,6 +55,8 @@ Options:
   --max-seq-len      Override max sequence length
   --stop-ids         Stop token ids (default: the model's eos ids)
   --dtype            bfloat16 (default) or float32
+  --cache-dtype      same (default: as --dtype) or int8: keys and values in 8 bits
+  --score            Score the prompts instead of generating; the number of alternatives to print per token
   --slots            Sequences live at once (default: as many as the cache holds)
   --print-logits-topk  Print the K largest logits after each prompt
   --dump-layer-stats Print per-layer statistics of the hidden state at position 0
@@ -76,7 +82,7 @@ def parse_args(argv: list) -> dict:
     a = {"model": None, "prompts": [], "max_tokens": 512, "temperature": 0.8, "top_k": 40, "top_p": 0.95,
          "repetition_penalty": 1.1, "seed": 12345, "max_seq_len": None, "stop_ids": None,
          "dtype": "bfloat16", "help": False, "random_config": None, "weights_seed": 0, "random_prompts": None,
-         "slots": None, "logits_topk": 0, "layer_stats": False, "bench": False}
+         "slots": None, "cache_dtype": None, "score": None, "logits_topk": 0, "layer_stats": False, "bench": False}
     i = 0
 
     def value(flag):
@@ -126,6 +132,14 @@ def parse_args(argv: list) -> dict:
             a["dtype"] = value("--dtype")
             if a["dtype"] not in ("bfloat16", "float32", "bf16", "fp32"):
                 raise CliError(f"Invalid --dtype: {a['dtype']!r}")
+        elif arg == "--cache-dtype":
+            a["cache_dtype"] = value("--cache-dtype")
+            if a["cache_dtype"] not in ("same", "int8"):
+                raise CliError(f"Invalid --cache-dtype: {a['cache_dtype']!r}")
+        elif arg == "--score":
+            a["score"] = number("--score", int)
+            if not 0 <= a["score"] <= 64:
+                raise CliError("Invalid --score: 0 to 64 alternatives")
         elif arg == "--random-config":
             a["random_config"] = value("--random-config")
         elif arg == "--weights-seed":
@@ -192,9 +206,9 @@ def main(argv=None) -> int:
             with open(a["random_config"], encoding="utf-8") as f:
                 config = config_from_dict(json.load(f))
             model = Model.random(config, seed=a["weights_seed"], dtype=a["dtype"], max_seq_len=a["max_seq_len"],
-                                 n_slots=a["slots"])
+                                 n_slots=a["slots"], cache_dtype=a["cache_dtype"])
         else:
-            model = Model.load(a["model"], a["max_seq_len"], dtype=a["dtype"], n_slots=a["slots"])
+            model = Model.load(a["model"], a["max_seq_len"], dtype=a["dtype"], n_slots=a["slots"], cache_dtype=a["cache_dtype"])
     except Exception as e:                          # main.rs:257-263
         print(f"Failed to load model: {e}", file=sys.stderr)
         return 1
@@ -219,6 +233,17 @@ def main(argv=None) -> int:
                 print(f"prompt {i}: top logits " + " ".join(f"{int(t)}:{float(v):.4f}" for v, t in
                                                              zip(top.values.tolist(), top.indices.tolist())),
                       file=sys.stderr)
+    if a["score"] is not None:
+        for i, p in enumerate(prompts):
+            if len(p) < 2:
+                print(f"prompt {i}: nothing to score in a single token", file=sys.stderr)
+                continue
+            found = model.score(p, top=min(a["score"], vocab))
+            for n, token in enumerate(p[1:]):
+                others = "" if not found.top else " " + " ".join(f"{t}:{lp:.4f}" for t, lp in found.top[n])
+                print(f"{token} {found.logprobs[n]:.4f} {found.entropies[n]:.4f}{others}")
+            print(f"prompt {i}: {len(p) - 1} tokens, perplexity {found.perplexity:.4f}", file=sys.stderr)
+        return 0
     cfg = SamplerConfig(temperature=a["temperature"], top_k=a["top_k"], top_p=a["top_p"],
                         repetition_penalty=a["repetition_penalty"], repetition_window=64, seed=a["seed"])
     t0 = time.time()

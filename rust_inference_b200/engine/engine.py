@@ -33,6 +33,15 @@ def resolve_dtype(dtype) -> torch.dtype:
         raise ValueError(f"dtype must be one of {sorted(_DTYPES)}, found {dtype!r}") from None
 
 
+def resolve_cache_dtype(cache_dtype):
+    """None (keys and values in the run dtype) or torch.int8, by its name too."""
+    if cache_dtype in (None, "same"):
+        return None
+    if cache_dtype in (torch.int8, "int8"):
+        return torch.int8
+    raise ValueError(f"cache_dtype must be 'same' or 'int8', found {cache_dtype!r}")
+
+
 def require_cuda(device) -> torch.device:
     device = torch.device(device)
     if device.type != "cuda":
@@ -83,7 +92,10 @@ class _PinnedRing:
 
 class Engine:
     def __init__(self, model: DecoderModel, *, max_tokens: int, max_seq_len: int | None = None,
-                 n_slots: int | None = None, use_graphs: bool = True):
+                 n_slots: int | None = None, use_graphs: bool = True, cache_dtype=None):
+        """cache_dtype: None, keys and values in the run dtype; "int8": 8-bit codes with a scale for every 16 positions of a kv
+        head (`kernels.quantized_cache`), half a bfloat16 cache's memory and reads.  Models with a layer that keeps something else
+        (a latent, normalised or convolved heads, blended values) are refused."""
         self.model = model
         self.use_graphs = use_graphs and model.graph_safe()
         self._graphs: OrderedDict = OrderedDict()       # batch size -> DecodeGraph, least recently used first
@@ -92,7 +104,7 @@ class Engine:
         self.dtype = model.dtype
         max_seq_len = resolve_max_seq_len(max_seq_len, model.spec.max_positions)
         self.cache = SequenceCache(model.cache_requests(), max_tokens=max_tokens, max_seq_len=max_seq_len,
-                                   dtype=model.dtype, device=self.device, n_slots=n_slots)
+                                   dtype=model.dtype, device=self.device, n_slots=n_slots, kv_dtype=resolve_cache_dtype(cache_dtype))
         self.max_seq_len = self.cache.max_seq_len
         model.prepare(self.max_seq_len)
         self.workspace = Workspace(self.device)
@@ -106,21 +118,21 @@ class Engine:
     @classmethod
     def from_pretrained(cls, model_dir: str, *, dtype="bfloat16", device="cuda", max_tokens: int = 8192,
                         max_seq_len: int | None = None, n_slots: int | None = None,
-                        use_graphs: bool = True) -> "Engine":
+                        use_graphs: bool = True, cache_dtype=None) -> "Engine":
         """Load a model folder (config.json + safetensors); the model class comes from
         config.json's architecture name."""
         device = require_cuda(device)
         config, spec = load_spec(model_dir)
         model = DecoderModel(spec, dtype=resolve_dtype(dtype), device=device)
         model.load(read_model_tensors(model_dir, model.declared_tensors(), spec.ignored_tensors))
-        eng = cls(model, max_tokens=max_tokens, max_seq_len=max_seq_len, n_slots=n_slots, use_graphs=use_graphs)
+        eng = cls(model, max_tokens=max_tokens, max_seq_len=max_seq_len, n_slots=n_slots, use_graphs=use_graphs, cache_dtype=cache_dtype)
         eng.config = config
         return eng
 
     @classmethod
     def from_random(cls, config, *, seed: int = 0, std: float = 0.02, norm_std: float = 0.0, dtype="bfloat16",
                     device="cuda", max_tokens: int = 8192, max_seq_len: int | None = None,
-                    n_slots: int | None = None, use_graphs: bool = True) -> "Engine":
+                    n_slots: int | None = None, use_graphs: bool = True, cache_dtype=None) -> "Engine":
         """Random weights made on the device, without a folder (benchmarks)."""
         device = require_cuda(device)
         dtype = resolve_dtype(dtype)
@@ -128,7 +140,7 @@ class Engine:
         model = DecoderModel(spec, dtype=dtype, device=device)
         model.load(random_tensors(model.declared_tensors(), seed, std=std, matrix_dtype=dtype, device=device,
                                   norm_std=norm_std))
-        eng = cls(model, max_tokens=max_tokens, max_seq_len=max_seq_len, n_slots=n_slots, use_graphs=use_graphs)
+        eng = cls(model, max_tokens=max_tokens, max_seq_len=max_seq_len, n_slots=n_slots, use_graphs=use_graphs, cache_dtype=cache_dtype)
         eng.config = config
         return eng
 

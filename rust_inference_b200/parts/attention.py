@@ -6,7 +6,7 @@ import math
 import torch
 
 from ..cache.sequence_cache import KVRequest, StateRequest
-from ..kernels import linear, ops, attention as attn_kernels
+from ..kernels import linear, ops, quantized_cache, attention as attn_kernels
 from .base import Mixer
 from .registry import register, lookup
 from .rope import RotaryEncoding
@@ -233,12 +233,18 @@ class GQAttention(Mixer):
                 out.update({nm["k_bias"]: b[q:q + kv], nm["v_bias"]: b[q + kv:q + kv + self.v_dim]})
         return out
 
+    @property
+    def quantizable(self) -> bool:
+        """Whether the layer can keep its keys and values in 8 bits: they go into the cache as projected, and rotated."""
+        return (self.conv is None and self.value_mix is None and not self.values_from_keys and self.qk_norm_eps is None
+                and hasattr(self.position, "apply_and_quantize") and self.head_dim % 2 == 0 and self.v_head_dim % 2 == 0)
+
     def prepare(self, max_positions):
         self.position.prepare(max_positions)
 
     def cache_request(self):
         keys = KVRequest(self.n_kv_heads, self.head_dim, self.window,
-                         None if self.v_head_dim == self.head_dim else self.v_head_dim)
+                         None if self.v_head_dim == self.head_dim else self.v_head_dim, quantizable=self.quantizable)
         if self.conv is None:
             return keys
         return keys, StateRequest((self.conv - 1, self.q_dim + self.kv_dim + self.v_dim), torch.float32)
@@ -277,6 +283,9 @@ class GQAttention(Mixer):
             z = ctx.buffer("conv_z", (n, self.w_qkv.n), torch.float32)
             linear.logits(x, self.w_qkv, z, ctx)                       # float32 results in both precisions
             self.forward_projected(z, 0, residual, ctx, cache_layer, writes_cache)
+            return
+        if quantized_cache.is_quantized(cache_layer) and writes_cache and self.own_kv:
+            self._forward_quantized(x, residual, ctx, cache_layer)
             return
         # a layer that has key and value projections but is scheduled to read another layer's cache leaves its own unused
         kv_width = (self.kv_dim + (0 if self.values_from_keys else self.v_dim)) if self.own_kv else 0
@@ -328,11 +337,29 @@ class GQAttention(Mixer):
                                               write_kv=writes_cache and self.own_kv, **extra)
         self._attend(qkv, gate_col, residual, ctx, cache_layer)
 
+    def _forward_quantized(self, x, residual, ctx, cache_layer):
+        """`forward` with keys and values going into a cache in 8 bits."""
+        n, width = x.shape[0], self.w_qkv.n
+        gate_col = self.q_dim + self.kv_dim + self.v_dim
+        q = ctx.buffer("q_rot", (n, self.q_dim), self.dtype)
+        sizes = dict(n_heads=self.n_heads, n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, v_head_dim=self.v_head_dim)
+        gates = None                            # the projection's rows, where gates lie behind the values
+        if width == gate_col and linear.wants_split(x, self.w_qkv):
+            acc = ctx.zeroed_buffer("qkv_acc", (n, width), torch.float32)
+            linear.accumulate_split(x, self.w_qkv, acc, ctx)
+            self.position.apply_and_quantize(acc, q, ctx, cache_layer, bias=self.b_qkv, clear=True, **sizes)
+        else:
+            gates = ctx.buffer("qkv", (n, width), self.dtype)
+            linear.project(x, self.w_qkv, gates, ctx, bias=self.b_qkv)
+            self.position.apply_and_quantize(gates, q, ctx, cache_layer, **sizes)
+        self._attend(q, gate_col, residual, ctx, cache_layer, gates)
+
     def _formed_in_attention(self, x, width, residual, ctx, cache_layer, writes_cache) -> bool:
         """A decode step whose projection is split over K: the attention's own kernel adds the bias to the sums, norms and turns the
         heads and writes the cache.  False (nothing done) where it does not take the step."""
         if (not ctx.all_single or self.extended or self.value_mix is not None or not writes_cache or self.v_head_dim != self.head_dim
-                or type(self.position) is not RotaryEncoding or not linear.wants_split(x, self.w_qkv)):
+                or type(self.position) is not RotaryEncoding or not linear.wants_split(x, self.w_qkv)
+                or quantized_cache.is_quantized(cache_layer)):
             return False                # (a position encoding of a caller's own has steps of its own)
         if getattr(ctx, "routed", False) and (self.position.partial or self.qk_norm_eps is not None or self.values_from_keys or self.out_scale != 1.0):
             return False                # not the bits of the kernels it replaces: see `Part.routes`
@@ -365,18 +392,20 @@ class GQAttention(Mixer):
             raise RuntimeError("blended values: no layer before this one has kept values of the same size in this step")
         return self.value_lambda, first[0], first[1]
 
-    def _attend(self, qkv, gate_col, residual, ctx, cache_layer):
-        """Attention over the cache, gates and the output projection; the queries are qkv's first columns."""
+    def _attend(self, qkv, gate_col, residual, ctx, cache_layer, gates=None):
+        """Attention over the cache, gates and the output projection; the queries are qkv's first columns, gates lie in it too or
+        in rows of their own."""
+        gates = qkv if gates is None else gates
         mixed = ctx.buffer("attn_out", (qkv.shape[0], self.o_dim), self.dtype)
         attn_kernels.attention(qkv, cache_layer, mixed, ctx, n_heads=self.n_heads,
                                n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, scale=self.scale,
                                window=self.window or 0, chunk=self.chunk or 0, v_head_dim=self.v_head_dim,
                                out_scale=1.0 if self.out_gate else self.out_scale, softcap=self.softcap,
                                keep_first=self.keep_first, sink=self.sinks, dist=self.dist,
-                               gate=qkv[:, gate_col:gate_col + self.n_heads] if self.head_gate else None)
+                               gate=gates[:, gate_col:gate_col + self.n_heads] if self.head_gate else None)
         if self.out_gate:
             # the gates of the projection's last columns, the mixer's factor with them (float32, one rounding)
-            ops.sigmoid_gate_(mixed, qkv, gate_col, self.out_scale)
+            ops.sigmoid_gate_(mixed, gates, gate_col, self.out_scale)
         self._project_out(mixed, residual, ctx)
 
     def _project_out(self, mixed, residual, ctx):

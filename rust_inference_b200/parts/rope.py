@@ -4,7 +4,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from ..kernels import ops
+from ..kernels import ops, quantized_cache
 from .base import PositionEncoding
 from .registry import register
 
@@ -180,6 +180,15 @@ class RotaryEncoding(PositionEncoding):
                                  n_kv_heads=n_kv_heads, head_dim=head_dim, page_size=ctx.page_size,
                                  style=self.style, write_kv=write_kv, attend=attend)
 
+    def apply_and_quantize(self, src, q_out, ctx, cache_layer, *, n_heads, n_kv_heads, head_dim, v_head_dim, bias=None, clear=False):
+        """`apply_and_store` for a cache in 8 bits: queries to q_out, keys and values into the cache as codes; from a projection
+        (`src` in the run dtype) or from the sums of one that was cut over K (`kernels.quantized_cache.write`)."""
+        if self.cos is None or self.cos.shape[0] < ctx.max_len:
+            raise RuntimeError("rope tables do not cover the step's positions; call prepare() first")
+        quantized_cache.write(src, q_out, self.cos, self.sin, cache_layer, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens,
+                              n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, v_head_dim=v_head_dim, max_new=ctx.max_new,
+                              style=self.style, rot_dims=self.rot_dims, bias=bias, clear=clear)
+
 
 @register("position", "unrotated")
 class Unrotated(PositionEncoding):
@@ -194,6 +203,11 @@ class Unrotated(PositionEncoding):
         ops.rope_cache_write(qkv, None, None, ctx.token_pos, ctx.token_seq, ctx.seq_slot, ctx.page_table, cache_layer.k,
                              cache_layer.v, n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim,
                              page_size=ctx.page_size, style=0, write_kv=True, rot_dims=0, v_head_dim=v_head_dim)
+
+    def apply_and_quantize(self, src, q_out, ctx, cache_layer, *, n_heads, n_kv_heads, head_dim, v_head_dim, bias=None, clear=False):
+        quantized_cache.write(src, q_out, None, None, cache_layer, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens,
+                              n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, v_head_dim=v_head_dim, max_new=ctx.max_new,
+                              rot_dims=0, bias=bias, clear=clear)
 
     def apply_normed_and_store(self, qkv, ctx, cache_layer, *, n_heads, n_kv_heads, head_dim, write_kv, q_weight,
                                k_weight, eps, values_from_keys=False, v_head_dim=None, value_mix=None):

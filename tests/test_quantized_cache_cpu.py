@@ -1,0 +1,54 @@
+"""What the cache in 8 bits and the scores decide on the host (no GPU)."""
+import os
+import re
+
+import pytest
+import torch
+
+from rust_inference_b200.cache.sequence_cache import KVRequest, SequenceCache
+from rust_inference_b200.cache.pager import CacheError
+from rust_inference_b200.cli import CliError, parse_args
+from rust_inference_b200.engine.engine import resolve_cache_dtype
+from rust_inference_b200.kernels import build, quantized_cache
+from rust_inference_b200.kernels.ops import KernelError
+
+
+def test_the_entry_points_arguments_are_those_of_the_sources():
+    for (module, fn), kinds in quantized_cache._SIGNATURES.items():
+        with open(os.path.join(build.CSRC, build.MODULES[module])) as f:
+            args = re.search(r"RI_API int " + fn + r"\(([^)]*)\)", f.read()).group(1).split(",")
+        found = "".join("p" if "*" in a or "cudaStream_t" in a else "l" if "long long" in a else "f" if a.split()[0] == "float" else "i"
+                        for a in args)
+        assert found == kinds, fn
+
+
+def test_cache_dtype_names():
+    assert resolve_cache_dtype(None) is None and resolve_cache_dtype("same") is None
+    assert resolve_cache_dtype("int8") is torch.int8 and resolve_cache_dtype(torch.int8) is torch.int8
+    for bad in ("int4", "float8", torch.uint8, 8):
+        with pytest.raises(ValueError):
+            resolve_cache_dtype(bad)
+
+
+def test_requests_that_are_not_kept_in_8_bits():
+    with pytest.raises(CacheError, match="8 bits"):
+        SequenceCache([KVRequest(2, 64)], max_tokens=64, max_seq_len=64, dtype=torch.float32, device="cpu", kv_dtype=torch.int8)
+    with pytest.raises(CacheError, match="8 bits"):
+        SequenceCache([(KVRequest(2, 64, quantizable=True), KVRequest(1, 40, None, 32, True))], max_tokens=64, max_seq_len=64,
+                      dtype=torch.float32, device="cpu", kv_dtype=torch.int8)
+    with pytest.raises(ValueError, match="int8"):
+        SequenceCache([], max_tokens=64, max_seq_len=64, dtype=torch.float32, device="cpu", kv_dtype=torch.float16)
+    with pytest.raises(KernelError, match="CUDA"):              # there is no path on the host
+        SequenceCache([KVRequest(2, 64, quantizable=True)], max_tokens=64, max_seq_len=64, dtype=torch.float32, device="cpu", kv_dtype=torch.int8)
+    # whether a request may be kept so is no part of what tells requests apart
+    assert KVRequest(2, 64, quantizable=True) == KVRequest(2, 64) and hash(KVRequest(2, 64, quantizable=True)) == hash(KVRequest(2, 64))
+
+
+def test_flags(tmp_path):
+    base = ["--model", str(tmp_path), "--prompt", "1,2"]
+    assert parse_args(base)["cache_dtype"] is None and parse_args(base)["score"] is None
+    a = parse_args(base + ["--cache-dtype", "int8", "--score", "5"])
+    assert a["cache_dtype"] == "int8" and a["score"] == 5
+    for bad in (["--cache-dtype", "fp8"], ["--score", "-1"], ["--score", "65"], ["--score", "x"]):
+        with pytest.raises(CliError):
+            parse_args(base + bad)

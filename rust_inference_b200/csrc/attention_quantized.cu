@@ -42,9 +42,10 @@ constexpr int PAGE = 64, BLOCK = 16, WARPS = 4, THREADS = 32 * WARPS;
 constexpr int STEP = 2 * BLOCK;                  // keys that a warp takes at a time
 constexpr int MOST_BLOCKS = 5;                   // thread blocks per SM, at most
 // What an item costs a block beside its pages (queries fetched, warps joined, the result written), in pages
-constexpr int SETUP = 2;
-// ... and what a block has at least
-constexpr int LEAST = 1;
+constexpr int SETUP = 4;
+// What a block has at least: the two pages of one turn, or as many turns as keep an item's parts to eight (64), which are added up in
+// one go (two): up to 4 pages (8).
+__device__ __forceinline__ int least_pages(int pages, int items) { return pages <= 16 * items ? 2 : (pages <= 256 * items ? 4 : 8); }
 // Parts of an item are added up eight at a time: a block that arrives last of eight adds theirs and goes on with seven others
 constexpr int GROUP = 8;
 // Weights are formed times 2^6 against a reference that follows the row's maximum only when that is 2^8 times ahead: they stay below
@@ -81,22 +82,19 @@ struct Item {
     const int* table;                            // its pages' numbers
 };
 
-__device__ __forceinline__ int units_of(const Args& a, int seq, int rows) {
-    const int n = a.cu_seqlens[seq + 1] - a.cu_seqlens[seq], start = a.seq_start[seq];
+__device__ __forceinline__ int units_of(const Args& a, int start, int n, int rows) {
     return n > 0 ? ((start + n - 1) / PAGE + 1 - first_visible_key(start, a.span) / PAGE + SETUP) * a.n_kv * ((n * a.n_rep + rows - 1) / rows) : 0;
 }
-__device__ __forceinline__ void enter(const Args& a, int seq, int rows, Item& it) {
+__device__ __forceinline__ void enter(const Args& a, int seq, int first_tok, int n, int start, int slot, int rows, Item& it) {
     it.seq = seq;
-    it.first_tok = a.cu_seqlens[seq];
-    const int n = a.cu_seqlens[seq + 1] - it.first_tok;
-    it.start = a.seq_start[seq];
+    it.first_tok = first_tok;
+    it.start = start;
     it.n_rows = n * a.n_rep;
     it.tiles = (it.n_rows + rows - 1) / rows;
-    it.first_key = first_visible_key(it.start, a.span);
-    it.last_pos = it.start + n - 1;
+    it.first_key = first_visible_key(start, a.span);
+    it.last_pos = start + n - 1;
     it.low = it.first_key / PAGE;
     it.end = n > 0 ? it.last_pos / PAGE + 1 : it.low;
-    int slot = a.seq_slot[seq];
     // checked build: a slot outside is recorded, slot 0 read in its place
     if (!RI_IN_LIMIT(slot, RI_LIMIT_SLOTS, RI_CHECK_SLOT)) slot = 0;
     it.table = a.page_table + (size_t)slot * a.max_pages;
@@ -107,7 +105,10 @@ __device__ __forceinline__ void next_item(const Args& a, int rows, Item& it) {
     it.tile = 0;
     if (++it.head < a.n_kv) return;
     it.head = 0;
-    do enter(a, it.seq + 1, rows, it); while (it.n_rows == 0);
+    do {
+        const int seq = it.seq + 1, first_tok = a.cu_seqlens[seq];
+        enter(a, seq, first_tok, a.cu_seqlens[seq + 1] - first_tok, a.seq_start[seq], a.seq_slot[seq], rows, it);
+    } while (it.n_rows == 0);
 }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -221,7 +222,7 @@ attn_quantized_kernel(const Args a) {
     static_assert(PART > 0 || ROWS * HD * 4 <= 2 * TILE, "a warp's sums fit where its values were");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int sums[THREADS + 1];
-    __shared__ int found[2];
+    __shared__ int found[6], items;
     __shared__ int last_here;
     __shared__ float4 sgroup[GROUP][ROWS];       // statistics of parts that are added up
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -229,11 +230,17 @@ attn_quantized_kernel(const Args a) {
 
     // ---- this block's run of units (lengths, slots and pages are fixed before the step) ----
     const int per = (a.n_seqs + THREADS - 1) / THREADS;
-    int mine = 0;
-    for (int s = tid * per; s < min((tid + 1) * per, a.n_seqs); ++s) mine += units_of(a, s, ROWS);
+    int mine = 0, mine_items = 0, slot = 0;
+    for (int s = tid * per; s < min((tid + 1) * per, a.n_seqs); ++s) {
+        const int n = a.cu_seqlens[s + 1] - a.cu_seqlens[s];
+        mine += units_of(a, a.seq_start[s], n, ROWS);
+        mine_items += a.n_kv * ((n * a.n_rep + ROWS - 1) / ROWS);
+        slot = a.seq_slot[s];                    // (in the cache for when it is wanted)
+    }
     sums[tid + 1] = mine;
-    if (tid == 0) sums[0] = 0;
+    if (tid == 0) sums[0] = items = 0;
     __syncthreads();
+    if (mine_items) atomicAdd(&items, mine_items);
     if (warp == 0) {                             // running sums of the 128 numbers, four per lane
         int v[4], run = 0;
 #pragma unroll
@@ -249,22 +256,31 @@ attn_quantized_kernel(const Args a) {
         for (int i = 0; i < 4; ++i) sums[4 * lane + 1 + i] = v[i] + before;
     }
     __syncthreads();
-    const int total = sums[THREADS], blocks = min((int)gridDim.x, (total + LEAST - 1) / LEAST), me = blockIdx.x;
+    const int total = sums[THREADS], me = blockIdx.x;
+    const int least = least_pages(total - SETUP * items, items), blocks = min((int)gridDim.x, (total + least - 1) / least);
     if (me >= blocks) {
         wait_for_previous_kernels();             // (who waits for this kernel waits for those before it too)
         return;
     }
-    auto run_start = [&](int b) { return (int)((long long)total * b / blocks); };
+    // the first `more` runs have one unit more than `each`
+    const int each = total / blocks, more = total % blocks;
+    auto run_start = [&](int b) { return b * each + min(b, more); };
     const int u0 = run_start(me), u1 = run_start(me + 1);
     if (sums[tid] <= u0 && u0 < sums[tid + 1]) {
-        int at = sums[tid], s = tid * per;
-        for (int n; at + (n = units_of(a, s, ROWS)) <= u0; ++s) at += n;
-        found[0] = s;
-        found[1] = at;
+        int at = sums[tid], s = tid * per, first_tok = a.cu_seqlens[s], n = a.cu_seqlens[s + 1] - first_tok, start = a.seq_start[s];
+        for (int units; at + (units = units_of(a, start, n, ROWS)) <= u0;) {
+            at += units;
+            ++s;
+            first_tok += n;
+            n = a.cu_seqlens[s + 1] - first_tok;
+            start = a.seq_start[s];
+        }
+        found[0] = s, found[1] = at, found[2] = first_tok, found[3] = n, found[4] = start;
+        found[5] = per == 1 ? slot : a.seq_slot[s];
     }
     __syncthreads();
     Item it;
-    enter(a, found[0], ROWS, it);
+    enter(a, found[0], found[2], found[3], found[4], found[5], ROWS, it);
     int page, u;                                 // the next page, and its place among the units
     {
         const int within = u0 - found[1], n = it.end - it.low + SETUP, at = within % n;
@@ -606,7 +622,7 @@ attn_quantized_kernel(const Args a) {
             store4<T>(reinterpret_cast<T*>(a.out) + (size_t)(it.first_tok + row / a.n_rep) * a.out_ld +
                       (size_t)(it.head * a.n_rep + row % a.n_rep) * HD + d, a.out_vec, v);
         };
-        auto block_of = [&](int x) { return (int)(((x + 1ll) * blocks - 1) / total); };
+        auto block_of = [&](int x) { return x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each; };
         const int first_block = block_of(item_u), parts = block_of(item_u + item_n - 1) - first_block + 1;
         // a block has two places: for an item whose pages began before its run (or with it), and for one whose began inside
         const int first_place = 2 * first_block + (run_start(first_block) < item_u ? 1 : 0);
@@ -640,24 +656,37 @@ attn_quantized_kernel(const Args a) {
             int n = parts, index = me - first_block, stride = 1;       // parts of this level, this block's among them, how far apart they lie
             for (int level = 0;; ++level) {
                 const int lead = index / GROUP * GROUP, members = min(GROUP, n - lead);
-                __threadfence();
-                __syncthreads();
+                __syncthreads();                 // all of this block's part is written
                 int* arrived = a.arrived + level * a.places + place_of(lead * stride);
                 if (tid == 0) {
+                    __threadfence();
                     last_here = atomicAdd(arrived, 1) == members - 1;
                     if (last_here) *arrived = 0;
+                    __threadfence();
                 }
                 __syncthreads();
                 if (!last_here) break;
-                __threadfence();
                 const bool done = n <= GROUP;
+                constexpr int TWO = 2;           // places that a thread reads together
+                float4 p[TWO][GROUP];
+                auto read = [&](int i0) {
+#pragma unroll
+                    for (int z = 0; z < TWO; ++z) {
+                        const int i = i0 + z * THREADS, row = i / (HD / 4), d = i % (HD / 4) * 4;
+#pragma unroll
+                        for (int x = 0; x < GROUP; ++x) {
+                            p[z][x] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (x < members && row < here)
+                                p[z][x] = __ldcg(reinterpret_cast<const float4*>(a.part + ((size_t)place_of((lead + x) * stride) * a.rows_cap + row) * HD + d));
+                        }
+                    }
+                };
                 // the parts' statistics, one per thread; what each part is weighted with, and the row's own
-                if (tid < GROUP * ROWS) {
-                    const int x = tid / ROWS, row = tid % ROWS;
-                    float4 st = make_float4(LOWEST, 0.f, 0.f, 0.f);
-                    if (x < members && row < here) st = __ldcg(a.stat + (size_t)place_of((lead + x) * stride) * a.rows_cap + row);
-                    sgroup[x][row] = st;
-                }
+                float4 st = make_float4(LOWEST, 0.f, 0.f, 0.f);
+                if (tid < GROUP * ROWS && tid / ROWS < members && tid % ROWS < here)
+                    st = __ldcg(a.stat + (size_t)place_of((lead + tid / ROWS) * stride) * a.rows_cap + tid % ROWS);
+                read(tid);
+                if (tid < GROUP * ROWS) sgroup[tid / ROWS][tid % ROWS] = st;
                 __syncthreads();
                 if (tid < here) {
                     float top = LOWEST, s = 0.f, sum = 0.f;
@@ -670,19 +699,8 @@ attn_quantized_kernel(const Args a) {
                     sml[tid] = make_float4(top, sum, s, 0.f);
                 }
                 __syncthreads();
-                constexpr int TWO = 2;           // places that a thread reads together
                 for (int i0 = tid; i0 < here * (HD / 4); i0 += TWO * THREADS) {
-                    float4 p[TWO][GROUP];
-#pragma unroll
-                    for (int z = 0; z < TWO; ++z) {
-                        const int i = i0 + z * THREADS, row = i / (HD / 4), d = i % (HD / 4) * 4;
-#pragma unroll
-                        for (int x = 0; x < GROUP; ++x) {
-                            p[z][x] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (x < members && row < here)
-                                p[z][x] = __ldcg(reinterpret_cast<const float4*>(a.part + ((size_t)place_of((lead + x) * stride) * a.rows_cap + row) * HD + d));
-                        }
-                    }
+                    if (i0 != tid) read(i0);
 #pragma unroll
                     for (int z = 0; z < TWO; ++z) {
                         const int i = i0 + z * THREADS, row = i / (HD / 4), d = i % (HD / 4) * 4;

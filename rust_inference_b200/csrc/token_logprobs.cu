@@ -13,11 +13,11 @@
 // The likeliest `top` tokens without a second pass: four neighbouring threads are a group.  With tau the top-th largest of
 // the groups' maxima, at least `top` elements are tau or more, and all of those lie in groups whose maximum is.  Those are about
 // `top` groups of 1/128 of a block's part of the row; only they are read again, out of the L2 cache, and the few elements above
-// tau, with those equal to it, are put in order by counting.  (Where blocks share a row, tau is taken from 128 maxima too, each of
-// as many groups as there are blocks.)
+// tau, with those equal to it, are put in order by counting.  (Where blocks share a row, tau is taken from 128 maxima too, each
+// of a group of every block.)
 //
-// A row belongs to one block of 512 threads, or, where the rows would leave SMs idle, to a cluster of 2, 4 or 8, which exchange
-// their sums, maxima and candidates through distributed shared memory.  What bounds many rows is memory.
+// A row belongs to one block of 512 threads, or, where the rows would leave SMs idle, to a cluster of up to 8, which read each
+// other's sums and maxima through distributed shared memory and put their candidates into the first block's.  What bounds many rows is memory.
 #include "cluster.cuh"
 
 #include <float.h>
@@ -79,10 +79,18 @@ template <> struct Piece<float> {
     static __device__ __forceinline__ void open(const uint4& v, float* f) {
         f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
     }
+    static __device__ __forceinline__ float most(const uint4& v) {             // (a NaN is left out)
+        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+    }
 };
 template <> struct Piece<__nv_bfloat16> {
     static constexpr int N = 8;
     static __device__ __forceinline__ void open(const uint4& v, float* f) { unpack8(v, f); }
+    static __device__ __forceinline__ float most(const uint4& v) {
+        const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v);
+        const float2 m = __bfloat1622float2(__hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3])));
+        return fmaxf(m.x, m.y);
+    }
 };
 
 // Larger logits first: whole numbers in their order (0 and -0 are equal, NaN before all)
@@ -91,18 +99,23 @@ __device__ __forceinline__ unsigned order(float x) {
     return x != x ? 0xffffffffu : ((u & 0x80000000u) ? ~u : u | 0x80000000u);
 }
 
+__device__ __forceinline__ float ordered(unsigned u) {                  // ... and back
+    return __uint_as_float(u == 0xffffffffu ? 0x7fffffffu : ((u & 0x80000000u) ? u ^ 0x80000000u : ~u));
+}
+
 __device__ __forceinline__ const void* peer(const void* own, int rank) {           // a place in a peer's shared memory
     uint64_t there;
     asm volatile("mapa.u64 %0, %1, %2;" : "=l"(there) : "l"(own), "r"(rank));
     return reinterpret_cast<const void*>(there);
 }
 
-struct Lists {
+struct __align__(16) Lists {
     unsigned long long found[WARPS];
+    unsigned every[GROUPS];                      // the largest of the groups' maxima in the row's blocks
     Sums sums[WARPS];
     Sums block;                                  // of this block's part of the row
     unsigned most[GROUPS];                       // the groups' maxima, in their order
-    unsigned every[GROUPS];                      // those of all the row's blocks, as many of them together as there are blocks
+    float m, log_z;                              // of the whole row; log_z NaN: no distribution
     int votes[WARPS];
     unsigned tau;
     int above_n, equal_n, groups_n;
@@ -159,6 +172,11 @@ logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, in
     if (tid == 0) s.above_n = s.equal_n = s.groups_n = 0;
     wait_for_previous_kernels();
 
+    float wanted = 0.f;                          // the target's logit, by the thread that will want it
+    if (rank == 0 && tid == THREADS - 32) {
+        const int id = targets[row];
+        if (id >= 0 && id < vocab) wanted = load1(x + id);
+    }
     Sums mine = {-FLT_MAX, 0.f, 0.f};            // (a finite reference: minus infinity less it is minus infinity)
     float most = -INFINITY;
     for (int p = p0 + tid; p < p1; p += AT_ONCE * THREADS) {
@@ -166,15 +184,17 @@ logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, in
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k)
             if (p + k * THREADS < p1) v[k] = load16(body + (size_t)(p + k * THREADS) * N);
+        float higher = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+            if (p + k * THREADS < p1) higher = fmaxf(higher, Piece<T>::most(v[k]));
+        most = fmaxf(most, higher);
+        if (higher > mine.m) raise(mine, higher);
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k) {
             if (p + k * THREADS >= p1) break;
-            float f[N], higher = -INFINITY;
+            float f[N];
             Piece<T>::open(v[k], f);
-#pragma unroll
-            for (int i = 0; i < N; ++i) higher = fmaxf(higher, f[i]);
-            most = fmaxf(most, higher);
-            if (higher > mine.m) raise(mine, higher);
 #pragma unroll
             for (int i = 0; i < N; ++i) add(mine, f[i]);
         }
@@ -211,33 +231,39 @@ logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, in
     }
     if (blocks > 1) cluster_sync();
     else __syncthreads();
-    Sums all = s.block;
-    if (blocks > 1) {
-        all = {-FLT_MAX, 0.f, 0.f};
-        for (int b = 0; b < blocks; ++b) all = joined(all, *reinterpret_cast<const Sums*>(peer(&s.block, b)));
-    }
-    // no distribution: an infinite maximum, a NaN among the sums, nothing but banned tokens
-    const bool none = !(all.m < INFINITY) || !(all.z > 0.f);
-    const float log_z = none ? __int_as_float(0x7fffffff) : logf(all.z);
-    if (rank == 0 && tid == 0) {
-        const int id = targets[row];
-        logprob[row] = id >= 0 && id < vocab ? load1(x + id) - all.m - log_z : __int_as_float(0x7fffffff);
-        entropy[row] = log_z - all.t * LN2 / all.z;
+    // ---- the last warp: the row's sums; the others: tau, the top-th largest of the groups' maxima ----
+    if (warp == WARPS - 1) {
+        Sums all = {-FLT_MAX, 0.f, 0.f};
+        if (lane < blocks) all = blocks > 1 ? *reinterpret_cast<const Sums*>(peer(&s.block, lane)) : s.block;
+#pragma unroll
+        for (int o = 1; o < MOST_BLOCKS; o <<= 1) {
+            const Sums other = {__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.z, o), __shfl_xor_sync(0xffffffffu, all.t, o)};
+            all = joined(all, other);
+        }
+        if (lane == 0) {
+            // no distribution: an infinite maximum, a NaN among the sums, nothing but banned tokens
+            const bool none = !(all.m < INFINITY) || !(all.z > 0.f);
+            s.m = all.m;
+            s.log_z = none ? __int_as_float(0x7fffffff) : logf(all.z);
+            if (rank == 0) {
+                const int id = targets[row];
+                logprob[row] = (id >= 0 && id < vocab ? wanted : __int_as_float(0x7fffffff)) - all.m - s.log_z;
+                entropy[row] = s.log_z - all.t * LN2 / all.z;
+            }
+        }
     }
     if (top == 0) {
         if (blocks > 1) cluster_sync();          // a peer may still be reading this block's sums
         return;
     }
-
-    // ---- tau: the top-th largest of the groups' maxima ----
     if (tid < GROUPS) {
-        const int per = GROUPS / blocks, at = tid % per * blocks;
-        unsigned largest = s.most[tid];
-        if (blocks > 1) {
-            const unsigned* theirs = reinterpret_cast<const unsigned*>(peer(s.most + at, tid / per));
-            largest = 0;
-            for (int i = 0; i < blocks; ++i) largest = max(largest, theirs[i]);
-        }
+        unsigned most_of[MOST_BLOCKS];           // all reads at once
+#pragma unroll
+        for (int b = 0; b < MOST_BLOCKS; ++b)
+            most_of[b] = b == 0 && blocks == 1 ? s.most[tid] : (b < blocks ? *reinterpret_cast<const unsigned*>(peer(s.most + tid, b)) : 0u);
+        unsigned largest = most_of[0];
+#pragma unroll
+        for (int b = 1; b < MOST_BLOCKS; ++b) largest = max(largest, most_of[b]);
         s.every[tid] = largest;
     }
     __syncthreads();
@@ -245,10 +271,12 @@ logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, in
         const int k = tid / 4, quarter = tid % 4 * (GROUPS / 4);
         const unsigned mine = s.every[k];
         int before = 0;
-#pragma unroll 8
-        for (int i = 0; i < GROUPS / 4; ++i) {
-            const int o = quarter + (i + 8 * (tid % 4)) % (GROUPS / 4);        // (the four in different banks)
-            before += s.every[o] > mine || (s.every[o] == mine && o < k);
+#pragma unroll
+        for (int i = 0; i < GROUPS / 4; i += 4) {
+            const int o = quarter + (i + 4 * (tid % 4)) % (GROUPS / 4);        // (the four in different banks)
+            const uint4 u = *reinterpret_cast<const uint4*>(s.every + o);
+            before += (u.x > mine || (u.x == mine && o < k)) + (u.y > mine || (u.y == mine && o + 1 < k)) +
+                      (u.z > mine || (u.z == mine && o + 2 < k)) + (u.w > mine || (u.w == mine && o + 3 < k));
         }
         before += __shfl_xor_sync(0xffffffffu, before, 1);
         before += __shfl_xor_sync(0xffffffffu, before, 2);
@@ -260,15 +288,16 @@ logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, in
     // ---- what is above it, and equal to it, in the groups that have any ----
     if (tid < GROUPS && s.most[tid] >= tau) s.group[atomicAdd(&s.groups_n, 1)] = tid;
     __syncthreads();
+    Lists& lists = blocks > 1 ? *const_cast<Lists*>(reinterpret_cast<const Lists*>(peer(&s, 0))) : s;       // the first block's
     auto look = [&](float f, int id) {
         const unsigned u = order(f);
         if (u < tau) return;
         if (u > tau) {
-            const int at = atomicAdd(&s.above_n, 1);
-            if (at < ROOM) s.above_x[at] = u, s.above_id[at] = id;
+            const int at = atomicAdd(&lists.above_n, 1);
+            if (at < ROOM) lists.above_x[at] = u, lists.above_id[at] = id;
         } else {
-            const int at = atomicAdd(&s.equal_n, 1);
-            if (at < ROOM) s.equal_id[at] = id;
+            const int at = atomicAdd(&lists.equal_n, 1);
+            if (at < ROOM) lists.equal_id[at] = id;
         }
     };
     constexpr int RUN = GROUP * N;               // neighbouring elements of a group
@@ -297,46 +326,29 @@ logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, in
     else __syncthreads();
 
     if (rank == 0) {
-        // ---- the first block brings the lists together and puts them in order ----
-        int above = s.above_n, equal = s.equal_n;
-        bool held = above <= ROOM;               // all that is above; of the equal ones as many as are wanted
-        bool ties = equal <= ROOM;
-        const int own_above = min(above, ROOM), own_equal = min(equal, ROOM);
-        int at_above = own_above, at_equal = own_equal;
-        for (int b = 1; b < blocks; ++b) {
-            const Lists& other = *reinterpret_cast<const Lists*>(peer(&s, b));
-            const int na = other.above_n, ne = other.equal_n;
-            above += na;
-            equal += ne;
-            held = held && at_above + na <= ROOM;
-            ties = ties && at_equal + ne <= ROOM;
-            if (held)
-                for (int i = tid; i < na; i += THREADS) s.above_x[at_above + i] = other.above_x[i], s.above_id[at_above + i] = other.above_id[i];
-            if (ties)
-                for (int i = tid; i < ne; i += THREADS) s.equal_id[at_equal + i] = other.equal_id[i];
-            at_above += na;
-            at_equal += ne;
-        }
-        __syncthreads();
+        // ---- the first block puts them in order ----
+        const int above = s.above_n, equal = s.equal_n;
+        const bool held = above <= ROOM, ties = equal <= ROOM;         // all that is above; all that is equal
+        const float m = s.m, log_z = s.log_z;
         int* ids = top_ids + (size_t)row * top;
         float* best = top_logprobs + (size_t)row * top;
-        auto value = [&](int id) { return load1(x + id) - all.m - log_z; };
+        const float equal_value = ordered(tau) - m - log_z;
         if (!held) {
-            one_by_one<T>(x, vocab, top, all.m, log_z, ids, best, s.found);
+            one_by_one<T>(x, vocab, top, m, log_z, ids, best, s.found);
         } else {
             for (int i = tid; i < above; i += THREADS) {
                 const unsigned u = s.above_x[i];
                 const int id = s.above_id[i];
                 int place = 0;
                 for (int o = 0; o < above; ++o) place += s.above_x[o] > u || (s.above_x[o] == u && s.above_id[o] < id);
-                if (place < top) ids[place] = id, best[place] = value(id);
+                if (place < top) ids[place] = id, best[place] = ordered(u) - m - log_z;
             }
             if (above < top && ties) {
                 for (int i = tid; i < equal; i += THREADS) {
                     const int id = s.equal_id[i];
                     int place = above;
                     for (int o = 0; o < equal; ++o) place += s.equal_id[o] < id;
-                    if (place < top) ids[place] = id, best[place] = value(id);
+                    if (place < top) ids[place] = id, best[place] = equal_value;
                 }
             } else if (above < top) {            // more of them than the list holds (banned tokens, for one): the lowest ids, in their order
                 for (int from = 0, place = above; place < top && from < vocab; from += THREADS) {
@@ -350,12 +362,12 @@ logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, in
                         if (w < warp) at += s.votes[w];
                         place += s.votes[w];
                     }
-                    if (is && at < top) ids[at] = from + tid, best[at] = value(from + tid);
+                    if (is && at < top) ids[at] = from + tid, best[at] = equal_value;
                 }
             }
         }
     }
-    if (blocks > 1) cluster_sync();              // the first block may still be reading the others' lists
+    // (the first block reads its own lists only: the others may leave)
 }
 
 }  // namespace
@@ -367,7 +379,7 @@ RI_API int ri_token_logprobs(const void* logits, int dtype, long long ld, int ro
     if (vocab <= 0 || top < 0 || top > vocab || top > MOST_TOP) return fail("token_logprobs: %d alternatives of %d tokens", top, vocab);
     // as many blocks per row as the SMs hold together (three each), and no more than have 512 pieces of a row each
     int blocks = 1;
-    while (blocks < MOST_BLOCKS && (long long)rows * blocks * 2 <= 3ll * sm_count() && vocab / (dtype == RI_F32 ? 4 : 8) >= 2 * blocks * THREADS) blocks *= 2;
+    while (blocks < MOST_BLOCKS && (long long)rows * (blocks + 1) <= 3ll * sm_count() && vocab / (dtype == RI_F32 ? 4 : 8) >= (blocks + 1) * THREADS) ++blocks;
     if ((long long)rows * blocks > 0x7fffffff) return fail("token_logprobs: %d rows are too many", rows);
     auto launch = [&](auto kernel, auto* x) {
         return launch_cluster("token_logprobs", kernel, dim3((unsigned)(rows * blocks)), THREADS, 0, blocks, stream, x, ld, vocab, targets, top,

@@ -74,7 +74,7 @@ def is_quantized(layer) -> bool:
 
 def _index(what: str, t: torch.Tensor, least: int) -> int:
     """The address of an index array of at least so many entries."""
-    if t.dtype is not torch.int32 or not t.is_cuda or t.numel() < least or not t.is_contiguous():
+    if not (t.dtype is torch.int32 and t.is_cuda and t.numel() >= least and t.is_contiguous()):
         raise KernelError(f"{what}: index arrays are contiguous int32 on the device, {least} entries or more here")
     return t.data_ptr()
 
@@ -99,26 +99,33 @@ def write(src: torch.Tensor, q_out: torch.Tensor | None, cos, sin, layer: Quanti
     n_seqs, cols = seq_slot.numel(), (n_heads + n_kv_heads) * head_dim + n_kv_heads * v_hd
     if layer.sizes != (n_kv_heads, head_dim, v_hd):
         raise KernelError(f"{what}: the layer has {layer.sizes[0]} kv heads of {layer.sizes[1:]} channels")
-    dtype = src.dtype
-    if not (src.is_cuda and src.dim() == 2 and src.is_contiguous() and src.shape[1] >= cols):
+    dtype, shape, tables = src.dtype, src.shape, page_table.shape
+    if not (src.is_cuda and len(shape) == 2 and shape[1] >= cols and src.is_contiguous()):
         raise KernelError(f"{what}: a contiguous [tokens, q | k | v columns] on the device is wanted")
-    if q_out is not None and not (q_out.is_cuda and q_out.is_contiguous() and q_out.shape == (src.shape[0], n_heads * head_dim)
-                                  and (q_out.dtype is dtype or dtype is torch.float32)):
-        raise KernelError(f"{what}: q_out must be [tokens, heads * head size]")
-    if rot and not (cos.is_cuda and sin.is_cuda and cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.dim() == 2
-                    and cos.shape[1] * 2 == rot and sin.shape == cos.shape and cos.is_contiguous() and sin.is_contiguous()):
-        raise KernelError(f"{what}: tables must be float32 [positions, rotated channels / 2]")
-    if bias is not None and not (bias.is_cuda and bias.dtype is torch.float32 and bias.is_contiguous() and bias.numel() >= cols):
-        raise KernelError(f"{what}: bias must be float32 [columns]")
-    if page_table.dim() != 2:
+    n_tokens, ld = shape
+    code = q_code = dtype_code(dtype)
+    q_at = cos_at = sin_at = bias_at = None
+    if q_out is not None:
+        if not (q_out.is_cuda and q_out.shape == (n_tokens, n_heads * head_dim) and q_out.is_contiguous()
+                and (q_out.dtype is dtype or dtype is torch.float32)):
+            raise KernelError(f"{what}: q_out must be [tokens, heads * head size]")
+        q_at, q_code = q_out.data_ptr(), dtype_code(q_out.dtype)
+    if rot:
+        if not (cos.is_cuda and sin.is_cuda and cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.is_contiguous()
+                and sin.is_contiguous() and cos.shape == sin.shape == (len(cos), rot // 2)):
+            raise KernelError(f"{what}: tables must be float32 [positions, rotated channels / 2]")
+        cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+    if bias is not None:
+        if not (bias.is_cuda and bias.dtype is torch.float32 and bias.is_contiguous() and bias.numel() >= cols):
+            raise KernelError(f"{what}: bias must be float32 [columns]")
+        bias_at = bias.data_ptr()
+    if len(tables) != 2:
         raise KernelError(f"{what}: the page table must be int32 [slots, pages]")
     _prepare("quantized_cache", "ri_quantized_write")
-    k, v, ks, vs = layer.pointers
-    _call("quantized_cache", "ri_quantized_write", src.data_ptr(), dtype_code(dtype), src.shape[1], None if bias is None else bias.data_ptr(),
-          1 if clear else 0, None if q_out is None else q_out.data_ptr(), dtype_code(dtype if q_out is None else q_out.dtype),
-          cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, _index(what, page_table, 1), page_table.shape[1],
-          _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs), _index(what, cu_seqlens, n_seqs + 1), k, v, ks, vs,
-          src.shape[0], n_seqs, max_new, n_heads, n_kv_heads, head_dim, v_hd, rot, style, _stream())
+    _call("quantized_cache", "ri_quantized_write", src.data_ptr(), code, ld, bias_at, 1 if clear else 0, q_at, q_code, cos_at, sin_at,
+          _index(what, page_table, 1), tables[1], _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs),
+          _index(what, cu_seqlens, n_seqs + 1), *layer.pointers, n_tokens, n_seqs, max_new, n_heads, n_kv_heads, head_dim, v_hd, rot, style,
+          _stream())
 
 
 def read(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, page_table: torch.Tensor, seq_slot, seq_first, seq_len, *,
@@ -131,20 +138,21 @@ def read(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, page_t
     what = "quantized_cache.read"
     n_kv, hd, v_hd = layer.sizes
     n_seqs = seq_slot.numel()
-    if not (k_out.is_cuda and v_out.is_cuda and k_out.dtype is v_out.dtype and k_out.is_contiguous() and v_out.is_contiguous()
-            and page_table.dim() == 2):
+    dtype, shape, tables = k_out.dtype, k_out.shape, page_table.shape
+    if not (k_out.is_cuda and v_out.is_cuda and dtype is v_out.dtype and k_out.is_contiguous() and v_out.is_contiguous() and len(tables) == 2):
         raise KernelError(f"{what}: outputs of one dtype, contiguous, on the device, and an int32 [slots, pages] table")
+    rows_at = None
     if cu_rows is None:
-        if k_out.shape != layer.k.shape or v_out.shape != layer.v.shape:
+        if shape != layer.k.shape or v_out.shape != layer.v.shape:
             raise KernelError(f"{what}: without cu_rows the outputs have the cache's shape")
-    elif not (k_out.dim() == 3 and k_out.shape[1:] == (n_kv, hd) and v_out.shape == (k_out.shape[0], n_kv, v_hd)):
-        raise KernelError(f"{what}: with cu_rows the outputs are [rows, kv heads, head size]")
+    else:
+        if shape != (shape[0], n_kv, hd) or v_out.shape != (shape[0], n_kv, v_hd):
+            raise KernelError(f"{what}: with cu_rows the outputs are [rows, kv heads, head size]")
+        rows_at = _index(what, cu_rows, n_seqs)
     _prepare("quantized_cache", "ri_quantized_read")
-    k, v, ks, vs = layer.pointers
-    _call("quantized_cache", "ri_quantized_read", k, v, ks, vs, k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype),
-          _index(what, page_table, 1), page_table.shape[1], _index(what, seq_slot, n_seqs), _index(what, seq_first, n_seqs),
-          _index(what, seq_len, n_seqs), None if cu_rows is None else _index(what, cu_rows, n_seqs), n_seqs, max_len, n_kv, hd, v_hd,
-          0 if seen_span is None else 1, seen_span or 0, _stream())
+    _call("quantized_cache", "ri_quantized_read", *layer.pointers, k_out.data_ptr(), v_out.data_ptr(), dtype_code(dtype),
+          _index(what, page_table, 1), tables[1], _index(what, seq_slot, n_seqs), _index(what, seq_first, n_seqs),
+          _index(what, seq_len, n_seqs), rows_at, n_seqs, max_len, n_kv, hd, v_hd, 0 if seen_span is None else 1, seen_span or 0, _stream())
     return k_out, v_out
 
 

@@ -3,7 +3,8 @@
 Each file under `csrc/` becomes one shared library with a plain C ABI, compiled the first
 time something needs it and kept beside the sources (`csrc/_build/`), so a model only
 compiles the kernels it runs: the CUDA sources by nvcc for sm_100a, the host runtime
-(`host_runtime.cpp`: cache books, step packing) by the C++ compiler.  There is no other
+(`host_runtime.cpp`: cache books, step packing) by the C++ compiler, and so is the Python
+extension through which the shortest calls go (`native_calls.cpp`).  There is no other
 implementation behind these libraries: if one cannot be built or loaded, the caller gets
 the error.
 """
@@ -47,7 +48,11 @@ MODULES = {
     "token_logprobs": "token_logprobs.cu",
     "wait_probe": "wait_probe.cu",
     "host_runtime": "host_runtime.cpp",
+    "native_calls": "native_calls.cpp",
 }
+
+# A Python extension over torch's C++ interface, imported rather than loaded with ctypes
+EXTENSIONS = {"native_calls"}
 
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
@@ -56,6 +61,22 @@ NVCC_FLAGS = [
 
 
 CXX_FLAGS = ["-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden"]
+
+
+def _extension_flags() -> tuple:
+    """(compiler flags, linker flags) of an extension over the torch and Python that run here; the versions are part of them, so
+    that another torch has it compiled again."""
+    import sysconfig
+    import torch
+    home = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    dirs = [os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"),
+            sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    lib = os.path.join(home, "lib")
+    return (["-I" + d for d in dirs] + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                                         f'-DRI_BUILT_FOR="{torch.__version__} {sys.version_info.major}.{sys.version_info.minor}"'],
+            ["-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath," + lib])
+
 
 # RI_B200_CHECK_BOUNDS=1: the checked build of the kernels (indices that reach memory through a table are
 # compared with their limits, recorded and skipped when outside: `csrc/common.cuh`).  It is compiled into
@@ -119,6 +140,8 @@ def _build_dir(checked: bool | None = None, timeline: bool | None = None) -> str
 def _source_digest(src: str, checked: bool, timeline: bool) -> str:
     h = hashlib.sha256()
     h.update(" ".join(_nvcc_flags(checked, timeline) if src.endswith(".cu") else CXX_FLAGS).encode())
+    if src in (MODULES[m] for m in EXTENSIONS):
+        h.update(" ".join(sum(_extension_flags(), [])).encode())
     headers = sorted(f for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))) if src.endswith(".cu") else []
     for name in [src] + headers:
         with open(os.path.join(CSRC, name), "rb") as f:
@@ -161,6 +184,9 @@ def build(module: str, *, force: bool = False, verbose: bool = True, checked: bo
             tmp = out + f".{os.getpid()}.tmp"
             if src.endswith(".cu"):
                 cmd = [_nvcc()] + _nvcc_flags(checked, timeline) + ["-I", CSRC, "-o", tmp, src_path]
+            elif module in EXTENSIONS:
+                flags, links = _extension_flags()
+                cmd = [_cxx()] + CXX_FLAGS + flags + ["-o", tmp, src_path] + links
             else:
                 cmd = [_cxx()] + CXX_FLAGS + ["-o", tmp, src_path]
             if verbose:
@@ -208,6 +234,29 @@ def load(module: str) -> ctypes.CDLL:
             lib.ri_last_error.restype = ctypes.c_char_p
             _loaded[module] = lib
         return lib
+
+
+_extensions: dict = {}
+
+
+def load_extension(module: str):
+    """An extension module, built first if need be.  Raises if it cannot be had."""
+    ext = _extensions.get(module)
+    if ext is None:
+        with _lock:
+            ext = _extensions.get(module)
+            if ext is None:
+                import importlib.util
+                import torch  # noqa: F401  (its libraries have to be there first)
+                path = build(module)
+                try:
+                    spec = importlib.util.spec_from_file_location("ri_" + module, path)
+                    ext = importlib.util.module_from_spec(spec)
+                    spec.loader.exec_module(ext)
+                except ImportError as e:
+                    raise KernelBuildError(f"cannot load {path}: {e}") from None
+                _extensions[module] = ext
+    return ext
 
 
 def loaded_cuda_modules() -> list[str]:

@@ -70,7 +70,29 @@ _launches = 0
 
 def launch_count() -> int:
     """How many kernel entry points have been called (each launches one kernel)."""
-    return _launches
+    return _launches + (_native_calls.launches() if _native_calls is not None else 0)
+
+
+# Entry points that are called through the extension `csrc/native_calls.cpp` (which looks at the tensors itself): its name for
+# each, with the library and the function behind it
+_NATIVE = {"write": (0, "quantized_cache", "ri_quantized_write"), "read": (1, "quantized_cache", "ri_quantized_read"),
+           "attend": (2, "attention_quantized", "ri_attention_quantized"), "logprobs": (3, "token_logprobs", "ri_token_logprobs")}
+_native_calls = None
+
+
+@functools.lru_cache(maxsize=None)
+def native(name: str):
+    """The extension's function `name`, with the entry point behind it named to it."""
+    global _native_calls
+    from .build import load_extension
+    which, module, fn = _NATIVE[name]
+    lib = load(module)
+    if _limits is not None:
+        _apply_limits(module, lib)
+    calls = load_extension("native_calls")
+    calls.bind(which, *(ctypes.cast(getattr(lib, f), c_void_p).value for f in (fn, "ri_last_error")), KernelError)
+    _native_calls = calls
+    return getattr(calls, name)
 
 
 _limits = None          # checked build: (vocabulary, slots, pages) for libraries still to be loaded
@@ -658,28 +680,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0)
     their log probabilities.  logits: float32 or bfloat16 [R, V], rows any distance apart; targets: int32 [R] (an id outside the
     vocabulary, as -1: log probability NaN).  Logits of minus infinity are tokens that cannot come; a row with a NaN, plus
     infinity or nothing else has no distribution, and its results are NaN.  Equal logits rank by their id."""
-    code = _DTYPE_CODE.get(logits.dtype)
-    if not (code is not None and logits.is_cuda and targets.is_cuda and logits.dim() == 2 and targets.dtype is torch.int32
-            and targets.is_contiguous()):
-        raise KernelError("token_logprobs: logits must be float32 or bfloat16 [rows, vocabulary], targets int32 [rows], both on the device")
-    rows, vocab = logits.shape
-    ld, step = logits.stride()
-    if targets.numel() != rows or vocab == 0 or (step != 1 and vocab != 1) or not 0 <= top <= min(vocab, TOKEN_LOGPROBS_MOST):
-        raise KernelError(f"token_logprobs: {rows} rows of {vocab} logits side by side, a target each, and 0 to {TOKEN_LOGPROBS_MOST} alternatives")
-    floats = logits if code == RI_F32 else logits.new_empty(0, dtype=torch.float32)
-    logprob, entropy = floats.new_empty(rows), floats.new_empty(rows)
-    ids = best = None
-    if top:
-        ids, best = targets.new_empty(rows, top), floats.new_empty(rows, top)
-    _prepare_logprobs()
-    _call("token_logprobs", "ri_token_logprobs", logits.data_ptr(), code, ld, rows, vocab, targets.data_ptr(), top, logprob.data_ptr(),
-          entropy.data_ptr(), ids.data_ptr() if top else None, best.data_ptr() if top else None, _stream())
-    return TokenLogprobs(logprob, entropy, ids, best)
-
-
-@functools.lru_cache(maxsize=None)
-def _prepare_logprobs() -> None:
-    load("token_logprobs").ri_token_logprobs.argtypes = [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int] + [c_void_p] * 5
+    return TokenLogprobs(*native("logprobs")(logits, targets, top, TOKEN_LOGPROBS_MOST))
 
 
 def cast(src: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

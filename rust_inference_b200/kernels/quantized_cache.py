@@ -13,35 +13,21 @@ positions of a page and kv head, [pages, kv heads, 64 / BLOCK], keys and values 
 from __future__ import annotations
 
 import functools
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_int
 
 import torch
 
 from .build import load
-from .ops import KernelError, _call, _stream, dtype_code
+from .ops import KernelError, _call, _p, _stream, native
 
 PAGE_SIZE, BLOCK = 64, 16
-
-# The entry points' arguments, one letter each, told to ctypes once: plain numbers then go through without an object for each.
-_KINDS = {"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float}
-_SIGNATURES = {
-    ("quantized_cache", "ri_quantized_write"): "piipipipppipppppppiiiiiiiiip",
-    ("quantized_cache", "ri_quantized_read"): "ppppppipippppiiiiiiip",
-    ("quantized_cache", "ri_quantized_widen"): "ppppppppipppiiiiip",
-    ("attention_quantized", "ri_attention_quantized"): "piipppppipppp" "iiiiiififplpp",
-}
-
-
-@functools.lru_cache(maxsize=None)
-def _prepare(module: str, fn: str) -> None:
-    getattr(load(module), fn).argtypes = [_KINDS[k] for k in _SIGNATURES[module, fn]]
 
 
 class QuantizedPages:
     """One layer: k, v int8 [pages, kv heads, 64, head size] (values may have a head size of their own), k_scale, v_scale
     float32 [pages, kv heads, 4], contiguous and on one device.  The tensors are looked at here, once, and stay the layer's."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "request", "sizes", "pointers", "aligned", "device")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "request", "sizes", "native", "aligned", "device")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, request=None):
         for t in (k, v, k_scale, v_scale):
@@ -56,8 +42,9 @@ class QuantizedPages:
                 raise KernelError(f"a quantized layer's scales are contiguous float32 {list(scales)}")
         self.k, self.v, self.k_scale, self.v_scale, self.request = k, v, k_scale, v_scale, request
         self.sizes = (k.shape[1], k.shape[3], v.shape[3])           # kv heads, head size, value head size
-        self.pointers = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
-        self.aligned = self.pointers[0] % 16 == 0 and self.pointers[1] % 16 == 0
+        # as the native calls take it: addresses, then sizes
+        self.native = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *self.sizes)
+        self.aligned = k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0
         self.device = k.device
 
 
@@ -93,39 +80,8 @@ def write(src: torch.Tensor, q_out: torch.Tensor | None, cos, sin, layer: Quanti
     [positions, rot_dims / 2]; rot_dims 0: nothing is rotated; style 0: pairs (i, i + rot_dims / 2), 1: pairs (2i, 2i + 1).
     src may be float32 beside a bfloat16 q_out: the sums of a product that was cut over K, with `bias` (float32 [columns]) still to
     be added, and `clear` leaves them zeroed.  q_out None: the q columns are not looked at (`cos`, `sin` then turn keys only)."""
-    what = "quantized_cache.write"
-    v_hd = head_dim if v_head_dim is None else int(v_head_dim)
-    rot = head_dim if rot_dims is None else int(rot_dims)
-    n_seqs, cols = seq_slot.numel(), (n_heads + n_kv_heads) * head_dim + n_kv_heads * v_hd
-    if layer.sizes != (n_kv_heads, head_dim, v_hd):
-        raise KernelError(f"{what}: the layer has {layer.sizes[0]} kv heads of {layer.sizes[1:]} channels")
-    dtype, shape, tables = src.dtype, src.shape, page_table.shape
-    if not (src.is_cuda and len(shape) == 2 and shape[1] >= cols and src.is_contiguous()):
-        raise KernelError(f"{what}: a contiguous [tokens, q | k | v columns] on the device is wanted")
-    n_tokens, ld = shape
-    code = q_code = dtype_code(dtype)
-    q_at = cos_at = sin_at = bias_at = None
-    if q_out is not None:
-        if not (q_out.is_cuda and q_out.shape == (n_tokens, n_heads * head_dim) and q_out.is_contiguous()
-                and (q_out.dtype is dtype or dtype is torch.float32)):
-            raise KernelError(f"{what}: q_out must be [tokens, heads * head size]")
-        q_at, q_code = q_out.data_ptr(), dtype_code(q_out.dtype)
-    if rot:
-        if not (cos.is_cuda and sin.is_cuda and cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.is_contiguous()
-                and sin.is_contiguous() and cos.shape == sin.shape == (len(cos), rot // 2)):
-            raise KernelError(f"{what}: tables must be float32 [positions, rotated channels / 2]")
-        cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
-    if bias is not None:
-        if not (bias.is_cuda and bias.dtype is torch.float32 and bias.is_contiguous() and bias.numel() >= cols):
-            raise KernelError(f"{what}: bias must be float32 [columns]")
-        bias_at = bias.data_ptr()
-    if len(tables) != 2:
-        raise KernelError(f"{what}: the page table must be int32 [slots, pages]")
-    _prepare("quantized_cache", "ri_quantized_write")
-    _call("quantized_cache", "ri_quantized_write", src.data_ptr(), code, ld, bias_at, 1 if clear else 0, q_at, q_code, cos_at, sin_at,
-          _index(what, page_table, 1), tables[1], _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs),
-          _index(what, cu_seqlens, n_seqs + 1), *layer.pointers, n_tokens, n_seqs, max_new, n_heads, n_kv_heads, head_dim, v_hd, rot, style,
-          _stream())
+    native("write")(src, q_out, cos, sin, layer.native, page_table, seq_slot, seq_start, cu_seqlens, n_heads, n_kv_heads, head_dim,
+                    head_dim if v_head_dim is None else v_head_dim, max_new, style, head_dim if rot_dims is None else rot_dims, bias, clear)
 
 
 def read(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, page_table: torch.Tensor, seq_slot, seq_first, seq_len, *,
@@ -135,24 +91,8 @@ def read(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, page_t
     the pages that hold these positions are filled (zeros elsewhere in them), the others left alone.  max_len: no sequence is
     longer.  seen_span: reading begins at the first key that a query at position seq_first[b] sees, of all keys (0), the last so many
     (> 0) or its own block of -span positions (< 0)."""
-    what = "quantized_cache.read"
-    n_kv, hd, v_hd = layer.sizes
-    n_seqs = seq_slot.numel()
-    dtype, shape, tables = k_out.dtype, k_out.shape, page_table.shape
-    if not (k_out.is_cuda and v_out.is_cuda and dtype is v_out.dtype and k_out.is_contiguous() and v_out.is_contiguous() and len(tables) == 2):
-        raise KernelError(f"{what}: outputs of one dtype, contiguous, on the device, and an int32 [slots, pages] table")
-    rows_at = None
-    if cu_rows is None:
-        if shape != layer.k.shape or v_out.shape != layer.v.shape:
-            raise KernelError(f"{what}: without cu_rows the outputs have the cache's shape")
-    else:
-        if shape != (shape[0], n_kv, hd) or v_out.shape != (shape[0], n_kv, v_hd):
-            raise KernelError(f"{what}: with cu_rows the outputs are [rows, kv heads, head size]")
-        rows_at = _index(what, cu_rows, n_seqs)
-    _prepare("quantized_cache", "ri_quantized_read")
-    _call("quantized_cache", "ri_quantized_read", *layer.pointers, k_out.data_ptr(), v_out.data_ptr(), dtype_code(dtype),
-          _index(what, page_table, 1), tables[1], _index(what, seq_slot, n_seqs), _index(what, seq_first, n_seqs),
-          _index(what, seq_len, n_seqs), rows_at, n_seqs, max_len, n_kv, hd, v_hd, 0 if seen_span is None else 1, seen_span or 0, _stream())
+    native("read")(layer.native, k_out, v_out, page_table, seq_slot, seq_first, seq_len, max_len, cu_rows, layer.k.shape[0],
+                   0 if seen_span is None else 1, seen_span or 0)
     return k_out, v_out
 
 
@@ -170,11 +110,11 @@ def widen(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, facto
     _need(factors.is_cuda and factors.dtype == torch.float32 and factors.is_contiguous() and factors.numel() >= 2 * n_seqs * n_kv, what,
           "factors must be float32 [sequences, 2, kv heads]")
     _need(page_table.dim() == 2, what, "the page table must be int32 [slots, pages]")
-    _prepare("quantized_cache", "ri_quantized_widen")
-    k, v, ks, vs = layer.pointers
-    _call("quantized_cache", "ri_quantized_widen", k, v, ks, vs, k_out.data_ptr(), v_out.data_ptr(), factors.data_ptr(),
-          _index(what, page_table, 1), page_table.shape[1], _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs),
-          _index(what, seq_len, n_seqs), n_seqs, max_len, n_kv, hd, span, _stream())
+    for t, least in ((page_table, 1), (seq_slot, n_seqs), (seq_start, n_seqs), (seq_len, n_seqs)):
+        _index(what, t, least)
+    _call("quantized_cache", "ri_quantized_widen", _p(layer.k), _p(layer.v), _p(layer.k_scale), _p(layer.v_scale), _p(k_out), _p(v_out),
+          _p(factors), _p(page_table), c_int(page_table.shape[1]), _p(seq_slot), _p(seq_start), _p(seq_len), c_int(n_seqs), c_int(max_len),
+          c_int(n_kv), c_int(hd), c_int(span), _stream())
 
 
 @functools.lru_cache(maxsize=None)
@@ -202,8 +142,7 @@ def attention(q: torch.Tensor, layer: QuantizedPages, out: torch.Tensor, page_ta
 class _Step:
     """What the calls of a step have in common: its arrays' addresses and sizes, looked at once."""
 
-    __slots__ = ("n_heads", "n_kv_heads", "head_dim", "sizes", "table", "max_pages", "slot", "start", "cu", "n_seqs", "max_new", "part",
-                 "part_size", "arrived", "kept")
+    __slots__ = ("native", "kept")
 
     def __init__(self, page_table, seq_slot, seq_start, cu_seqlens, n_heads, n_kv_heads, head_dim, max_new, part, arrived):
         what = "quantized_cache.attention"
@@ -211,15 +150,11 @@ class _Step:
               f"{n_heads} heads of {head_dim} over {n_kv_heads}, or a page table that is not [slots, pages]")
         floats, ints = attention_workspace(n_heads, n_kv_heads, head_dim, max_new)
         _need(part.is_cuda and part.dtype == torch.float32 and part.is_contiguous() and part.numel() >= floats, what, "scratch too small")
-        self.n_heads, self.n_kv_heads, self.head_dim, self.max_new = n_heads, n_kv_heads, head_dim, max_new
-        self.sizes = (n_kv_heads, head_dim, head_dim)
-        self.n_seqs = seq_slot.numel()
-        self.table, self.max_pages = _index(what, page_table, 1), page_table.shape[1]
-        self.slot, self.start = _index(what, seq_slot, self.n_seqs), _index(what, seq_start, self.n_seqs)
-        self.cu = _index(what, cu_seqlens, self.n_seqs + 1)
-        self.part, self.part_size, self.arrived = part.data_ptr(), part.numel(), _index(what, arrived, ints)
+        n_seqs = seq_slot.numel()
+        self.native = (_index(what, page_table, 1), page_table.shape[1], _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs),
+                       _index(what, cu_seqlens, n_seqs + 1), n_seqs, max_new, n_heads, n_kv_heads, head_dim, part.data_ptr(), part.numel(),
+                       _index(what, arrived, ints))
         self.kept = (page_table, seq_slot, seq_start, cu_seqlens, part, arrived)     # whose addresses these are
-        _prepare("attention_quantized", "ri_attention_quantized")
 
 
 def step_of(ctx, n_heads: int, n_kv_heads: int, head_dim: int) -> _Step:
@@ -236,18 +171,4 @@ def step_of(ctx, n_heads: int, n_kv_heads: int, head_dim: int) -> _Step:
 
 def attend_step(q, layer, out, step, scale, span, out_scale):
     """`attention` for a step that has been looked at."""
-    dtype, width = q.dtype, step.n_heads * step.head_dim
-    if not (layer.sizes == step.sizes and layer.aligned and out.dtype is dtype and (dtype is torch.bfloat16 or dtype is torch.float32)
-            and q.is_cuda and out.is_cuda and q.dim() == 2 and out.dim() == 2):
-        raise KernelError("quantized_cache.attention: queries and result must be float32 or bfloat16 [tokens, heads * head size] on the "
-                          f"device, the layer {step.n_kv_heads} kv heads of {step.head_dim}")
-    q_ld, q_step = q.stride()
-    out_ld, out_step = out.stride()
-    (rows, q_width), out_shape = q.shape, out.shape
-    if q_step != 1 or out_step != 1 or q_width < width or out_shape[0] != rows or out_shape[1] < width:
-        raise KernelError("quantized_cache.attention: rows of queries and result hold all heads side by side")
-    k, v, ks, vs = layer.pointers
-    _call("attention_quantized", "ri_attention_quantized", q.data_ptr(), 0 if dtype is torch.float32 else 1, q_ld, k, v, ks, vs, step.table,
-          step.max_pages, step.slot, step.start, step.cu, out.data_ptr(), out_ld, step.n_seqs, step.max_new, step.n_heads, step.n_kv_heads,
-          step.head_dim, scale, span, out_scale, step.part, step.part_size, step.arrived, _stream())
-    return out
+    return native("attend")(q, layer.native, out, step.native, scale, span, out_scale)

@@ -9,17 +9,41 @@ from rust_inference_b200.cache.sequence_cache import KVRequest, SequenceCache
 from rust_inference_b200.cache.pager import CacheError
 from rust_inference_b200.cli import CliError, parse_args
 from rust_inference_b200.engine.engine import resolve_cache_dtype
-from rust_inference_b200.kernels import build, quantized_cache
+from rust_inference_b200.kernels import build, ops
 from rust_inference_b200.kernels.ops import KernelError
 
 
+def _source(name):
+    with open(os.path.join(build.CSRC, name)) as f:
+        return f.read()
+
+
 def test_the_entry_points_arguments_are_those_of_the_sources():
-    for (module, fn), kinds in quantized_cache._SIGNATURES.items():
-        with open(os.path.join(build.CSRC, build.MODULES[module])) as f:
-            args = re.search(r"RI_API int " + fn + r"\(([^)]*)\)", f.read()).group(1).split(",")
-        found = "".join("p" if "*" in a or "cudaStream_t" in a else "l" if "long long" in a else "f" if a.split()[0] == "float" else "i"
-                        for a in args)
-        assert found == kinds, fn
+    """What the extension calls by address has the arguments, in kind and order, that the kernel libraries declare."""
+    def kinds(args):
+        return "".join("p" if "*" in a or "cudaStream_t" in a else "l" if "long long" in a else "f" if a.split()[0] == "float" else "i"
+                       for a in args.split(","))
+
+    for name, (_, module, fn) in ops._NATIVE.items():
+        declared = re.search(r"RI_API int " + fn + r"\(([^)]*)\)", _source(build.MODULES[module])).group(1)
+        called = re.search(r"typedef int " + name.capitalize() + r"Fn\(([^)]*)\)", _source("native_calls.cpp")).group(1)
+        assert kinds(called) == kinds(declared), fn
+
+
+def test_the_extension_refuses_what_it_cannot_take():
+    """On the host: tensors that lie there, and arguments that are no tensors, are an error with a message, not a crash."""
+    calls = build.load_extension("native_calls")
+    for fn, count in (("write", 18), ("read", 12), ("attend", 7), ("logprobs", 4), ("bind", 4)):
+        with pytest.raises((RuntimeError, TypeError)):
+            getattr(calls, fn)(*[None] * count)
+        with pytest.raises(RuntimeError):
+            getattr(calls, fn)()
+    x, t = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="on the device"):
+        calls.logprobs(x, t, 1, 64)
+    with pytest.raises((RuntimeError, TypeError)):
+        calls.logprobs(x, t, "one", 64)
+    assert calls.launches() == 0
 
 
 def test_cache_dtype_names():

@@ -34,6 +34,8 @@
 
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 using namespace ri;
 
 namespace {
@@ -760,10 +762,11 @@ int launch(Args a, long long part_floats, cudaStream_t stream) {
 // Thread blocks of a step, at most
 RI_API int ri_attention_quantized_blocks() { return MOST_BLOCKS * sm_count(); }
 
-// part: float32 [2 * blocks * min(16, n_rep * max_new) * (hd + 4)]; arrived: int32 [4 * 2 * blocks], zero, and left so.
+// part: float32 [2 * blocks * min(16, n_rep * max_new) * (hd + 4)]; arrived: int32 [4 * 2 * blocks], zero, and left so.  longest: the keys of
+// the longest sequence as far as the host knows them (what it chooses the tiles by; any number gives the same sums).
 RI_API int ri_attention_quantized(const void* q, int dtype, int q_ld, const int8_t* kc, const int8_t* vc, const float* ks, const float* vs,
                                   const int* page_table, int max_pages, const int* seq_slot, const int* seq_start, const int* cu_seqlens,
-                                  void* out, int out_ld, int n_seqs, int max_new, int n_heads, int n_kv, int hd, float scale, int span,
+                                  void* out, int out_ld, int n_seqs, int max_new, int longest, int n_heads, int n_kv, int hd, float scale, int span,
                                   float out_scale, float* part, long long part_floats, int* arrived, cudaStream_t stream) {
     if (n_seqs <= 0 || max_new <= 0) return 0;
     if (hd != 64 && hd != 128) return fail("attention_quantized: heads of %d channels (64 or 128 wanted)", hd);
@@ -791,8 +794,14 @@ RI_API int ri_attention_quantized(const void* q, int dtype, int q_ld, const int8
     a.out_scale = out_scale;
     a.part = part;
     a.arrived = arrived;
-    // tiles of 8 rows where the step has no more, else of 16
-    const int nq = rows <= 8 ? 1 : 2;
+    // A tile of 16 rows takes 1.75 times what one of 8 takes, which pays where the step has rows and keys for all of the SMs to be busy for
+    // long, 80 pages for 8 rows and more to an SM; below that half as many items to spread over the blocks cost more.  Tiles of 8 and of 16,
+    // us: 64 sequences of 1,024 keys, 32 heads over 8 of 128, 4 tokens 58.8 and 55.2 (16,384 pages), 16 tokens 182 and 165; 28 heads over 4, 3
+    // tokens (21 rows) 43.9 and 51.4; float32, 1,000 tokens over 4,096 keys 645 and 509; below: 1 sequence of 1,024 keys, 4 tokens
+    // 10.3 and 13.6; 4 sequences of 3,000, 12 heads over 2, 4 tokens in float32 15.3 and 20.9 (752 pages).
+    const long long tiles = (rows + 7) / 8, wide = (rows + 15) / 16;
+    const long long keys = span == 0 ? longest : std::min((long long)longest, (long long)max_new + (span > 0 ? span : -(long long)span));
+    const int nq = 7 * wide < 4 * tiles && (keys + PAGE - 1) / PAGE * tiles * n_seqs * n_kv > 80ll * sm_count() ? 2 : 1;
     a.rows_cap = (int)(rows < 8 * nq ? rows : 8 * nq);
     if (dtype == RI_F32 && nq == 1) return hd == 64 ? launch<64, float, 2, 1>(a, part_floats, stream) : launch<128, float, 2, 1>(a, part_floats, stream);
     if (dtype == RI_F32) return hd == 64 ? launch<64, float, 2, 2>(a, part_floats, stream) : launch<128, float, 2, 2>(a, part_floats, stream);

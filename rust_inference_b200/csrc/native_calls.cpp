@@ -191,26 +191,26 @@ PyObject* py_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ---- quantized_cache.attend_step -----------------------------------------------------------------------------------------
 // (q, layer, out, step, scale, span, out_scale); step: (page table, pages per slot, slots, starts, offsets, sequences, max_new, heads,
-//  kv heads, head size, scratch, its floats, counters)
+//  kv heads, head size, scratch, its floats, counters, the longest sequence)
 typedef int AttendFn(const void*, int, int, const int8_t*, const int8_t*, const float*, const float*, const int*, int, const int*, const int*,
-                     const int*, void*, int, int, int, int, int, int, float, int, float, float*, long long, int*, void*);
+                     const int*, void*, int, int, int, int, int, int, int, float, int, float, float*, long long, int*, void*);
 PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        const char* what = "quantized_cache.attention";
-        need(n == 7, "quantized_cache.attention: 7 arguments");
+        const char* what = "quantized_cache.attend_step";
+        need(n == 7, "quantized_cache.attend_step: 7 arguments");
         PyObject *layer = a[1], *step = a[3];
         const long long heads = item(step, 7), kv = item(step, 8), hd = item(step, 9), width = heads * hd;
         const at::Tensor &q = tensor(a[0], what), &out = tensor(a[2], what);
         const int code = code_of(q, what);
         need(item(layer, 4) == kv && item(layer, 5) == hd && item(layer, 6) == hd && (item(layer, 0) | item(layer, 1)) % 16 == 0,
-             "quantized_cache.attention: the layer has other heads, or lies off a 16-byte boundary");
+             "quantized_cache.attend_step: the layer has other heads, or lies off a 16-byte boundary");
         need(q.is_cuda() && out.is_cuda() && out.scalar_type() == q.scalar_type() && q.dim() == 2 && out.dim() == 2 && q.stride(1) == 1 &&
                  out.stride(1) == 1 && q.size(0) == out.size(0) && q.size(1) >= width && out.size(1) >= width,
-             "quantized_cache.attention: rows of queries and result hold all heads side by side, in one dtype, on the device");
+             "quantized_cache.attend_step: rows of queries and result hold all heads side by side, in one dtype, on the device");
         finish(entry<AttendFn>(ATTEND)(q.data_ptr(), code, small(q.stride(0)), address<int8_t>(item(layer, 0)), address<int8_t>(item(layer, 1)),
                                        address<float>(item(layer, 2)), address<float>(item(layer, 3)), address<int>(item(step, 0)),
                                        small(item(step, 1)), address<int>(item(step, 2)), address<int>(item(step, 3)), address<int>(item(step, 4)),
-                                       out.data_ptr(), small(out.stride(0)), small(item(step, 5)), small(item(step, 6)), small(heads), small(kv), small(hd),
+                                       out.data_ptr(), small(out.stride(0)), small(item(step, 5)), small(item(step, 6)), small(item(step, 13)), small(heads), small(kv), small(hd),
                                        (float)real(a[4]), small(number(a[5])), (float)real(a[6]), address<float>(item(step, 10)), item(step, 11),
                                        address<int>(item(step, 12)), stream()),
                ATTEND, what);

@@ -546,7 +546,9 @@ RI_API int ri_quantized_write(void* src, int src_dtype, int ld, const float* bia
     if (rot < 0 || rot % 2 || rot > hd) return fail("quantized_write: %d rotated channels of a head of %d", rot, hd);
     if (style != 0 && style != 1) return fail("quantized_write: unknown style %d", style);
     if (n_heads + 2 * n_kv > 65535) return fail("quantized_write: %d heads are too many", n_heads + 2 * n_kv);
-    // blocks of positions: so many per sequence, or, where most sequences bring far fewer tokens than the longest, counted through
+    // Blocks of positions: so many per sequence, or, where most sequences bring far fewer tokens than the longest, counted through (a warp
+    // then walks the sequences' lengths, but fewer blocks of threads find nothing to do): 16 sequences of 1 to 2,047 tokens 28.1 us by
+    // sequence, 25.9 counted through; 2 of 1 to 333 3.41 and 3.30.
     const long long each = (max_new + 2 * BLOCK - 2) / BLOCK, counted = n_tokens / BLOCK + 2ll * n_seqs;
     const bool direct = each * n_seqs <= counted;
     if ((direct ? each * n_seqs : counted) > 0x7fffffff) return fail("quantized_write: %d sequences of %d tokens are too many", n_seqs, max_new);
@@ -557,11 +559,15 @@ RI_API int ri_quantized_write(void* src, int src_dtype, int ld, const float* bia
     const int item = src_dtype == RI_F32 ? 4 : 2;
     if ((hd == 64 || hd == 128) && v_hd == hd && (rot == 0 || rot == hd) && ld * item % 16 == 0 && aligned16(src) && aligned16(q_out) &&
         aligned16(cos_t) && aligned16(sin_t) && aligned16(kc) && aligned16(vc)) {
-        // a warp takes one q head where the step would leave SMs idle otherwise, four of the same rows in a longer one (its address
-        // arithmetic and the angles' reads are then a quarter)
+        // A warp takes one q head, or two or four of the same rows (address arithmetic and the angles' reads are then shared): as few as
+        // keep the grid to what the SMs hold at once, four blocks each; two also where that keeps it to twice as much.  One, two and
+        // four, us, 32 heads over 8 of 128: 32 sequences of 1 token (384 blocks at one) 2.7, 2.8 and 3.1; 64 (768) 4.3, 3.1 and 3.8; 1,500 tokens
+        // (1,140) 8.3, 8.3 and 7.9; 2,047 (1,548) 11.7, 11.1 and 12.6; 8 times 2,047 83.6, 77.0 and 75.7.
         const int kv_blocks = (2 * n_kv + HEADS - 1) / HEADS;
-        const int q_each = (long long)runs * ((n_heads + HEADS - 1) / HEADS) > 8ll * sm_count() ? 4 : 1;
-        const int q_blocks = q_out ? (n_heads + HEADS * q_each - 1) / (HEADS * q_each) : 0;
+        const auto blocks_for = [&](int each) { return q_out ? (n_heads + HEADS * each - 1) / (HEADS * each) : 0; };
+        const auto waves = [&](int each) { return (long long)runs * (kv_blocks + blocks_for(each)) / (4.f * sm_count()); };
+        const int q_each = waves(1) <= 1.f ? 1 : (waves(2) <= 1.f || (waves(2) <= 2.f && waves(4) > 1.f) ? 2 : 4);
+        const int q_blocks = blocks_for(q_each);
         const dim3 grid((unsigned)runs, (unsigned)(kv_blocks + q_blocks));
         auto launch = [&](auto kernel) {
             return check_launch(launch_dependent(kernel, grid, dim3(64 * HEADS), 0, stream, w, kv_blocks, q_each), "quantized_write");

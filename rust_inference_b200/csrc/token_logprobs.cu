@@ -16,11 +16,13 @@
 // tau, with those equal to it, are put in order by counting.  (Where blocks share a row, tau is taken from 128 maxima too, each
 // of a group of every block.)
 //
-// A row belongs to one block of 512 threads, or, where the rows would leave SMs idle, to a cluster of up to 8, which read each
+// A row belongs to one block of 512 threads, or, where few rows are long, to a cluster of up to 8, which read each
 // other's sums and maxima through distributed shared memory and put their candidates into the first block's.  What bounds many rows is memory.
 #include "cluster.cuh"
 
 #include <float.h>
+
+#include <atomic>
 
 using namespace ri;
 
@@ -370,6 +372,32 @@ logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, in
     // (the first block reads its own lists only: the others may leave)
 }
 
+// How many clusters of so many blocks the device holds at once: they lie within groups of SMs, some of which they leave over.  Asked once.
+template <typename T>
+int clusters_held(int blocks) {
+    static std::atomic<int> known[64][MOST_BLOCKS + 1];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    n = known[dev][blocks].load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)blocks);
+        cfg.blockDim = dim3(THREADS);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)blocks;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, logprobs_kernel<T>, &cfg) != cudaSuccess || n <= 0) {
+            cudaGetLastError();
+            n = 1;
+        }
+        known[dev][blocks].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
 }  // namespace
 
 // logits [rows] of `vocab` numbers, `ld` apart; targets [rows]; top_ids, top_logprobs [rows, top] (top 0: not written)
@@ -377,9 +405,16 @@ RI_API int ri_token_logprobs(const void* logits, int dtype, long long ld, int ro
                              float* entropy, int* top_ids, float* top_logprobs, cudaStream_t stream) {
     if (rows <= 0) return 0;
     if (vocab <= 0 || top < 0 || top > vocab || top > MOST_TOP) return fail("token_logprobs: %d alternatives of %d tokens", top, vocab);
-    // as many blocks per row as the SMs hold together (three each), and no more than have 512 pieces of a row each
+    // Blocks per row: what a block does beside its part of the row, and clusters that wait for one another, have to be paid by shorter
+    // parts.  So parts of 8,192 logits or more where the blocks leave half of the SMs alone, of 28,000 or more up to as many clusters as the
+    // SMs hold at once (a cluster more costs a second round).  With 1, 2, 4 and 8, us, and the five likeliest, bfloat16:
+    //   vocabulary 128,256:  1 row 14.1, 10.1, 7.2, 6.1;  48 rows 14.4, 12.0, 11.6, 10.9;  90 rows 19.0, 17.9, 13.6, 19.3;  148 rows 17.7, 15.9, 22.2, 29.8
+    //   vocabulary 32,000:   1 row 6.5, 5.9, 5.5, 5.5;    48 rows 6.7, 7.1, 8.1, 8.5;      90 rows 7.5, 9.6, 9.2, 15.6;     148 rows 7.0, 9.6, 14.8, 23.5
+    const bool f32 = dtype == RI_F32;
     int blocks = 1;
-    while (blocks < MOST_BLOCKS && (long long)rows * (blocks + 1) <= 3ll * sm_count() && vocab / (dtype == RI_F32 ? 4 : 8) >= (blocks + 1) * THREADS) ++blocks;
+    for (int b = 2; b <= MOST_BLOCKS; ++b)
+        if ((2ll * rows * b <= sm_count() && vocab >= 8192 * b) || (vocab >= 28000 * b && rows <= (f32 ? clusters_held<float>(b) : clusters_held<__nv_bfloat16>(b))))
+            blocks = b;
     if ((long long)rows * blocks > 0x7fffffff) return fail("token_logprobs: %d rows are too many", rows);
     auto launch = [&](auto kernel, auto* x) {
         return launch_cluster("token_logprobs", kernel, dim3((unsigned)(rows * blocks)), THREADS, 0, blocks, stream, x, ld, vocab, targets, top,

@@ -13,8 +13,9 @@
   the plain form of the score
   anything else                  the generic kernel (`attention_generic`): any head size, any
                                  dtype, float32 arithmetic
-  a cache in 8 bits              the pages that a step looks at are read back into scratch in the run dtype, which the
-                                 kernels above then take (`_over_quantized`)
+  a cache in 8 bits              steps of few tokens, and those in float32, read the codes themselves (`reads_codes`); else the pages
+                                 that a step looks at go to scratch, in float16 for the tcgen05 kernel or in the run dtype for the
+                                 other kernels above (`_over_quantized`)
 
 Besides causality a mixer may limit a query's keys to the last `window` keys or to the query's own
 chunk of positions.  The tensor-core kernels take either as one signed span (`csrc/common.cuh:
@@ -135,10 +136,9 @@ def attention(qkv, cache_layer, out, ctx, *, n_heads, n_kv_heads, head_dim, scal
     result (see `ops.attention_generic`).  cache_layer: a layer in the run dtype, or one in 8 bits
     (`quantized_cache.QuantizedPages`)."""
     if type(cache_layer) is quantized_cache.QuantizedPages:
-        # steps of few rows (and all in float32) read the codes themselves
-        if ((qkv.dtype is torch.float32 or ctx.max_new * (n_heads // n_kv_heads) <= QUANTIZED_ROWS) and not (window and chunk)
-                and (head_dim == 64 or head_dim == 128) and (v_head_dim is None or v_head_dim == head_dim)
-                and not (softcap or keep_first or sink is not None or dist is not None or gate is not None)):
+        if ((head_dim == 64 or head_dim == 128) and (v_head_dim is None or v_head_dim == head_dim) and not (window and chunk)
+                and not (softcap or keep_first or sink is not None or dist is not None or gate is not None)
+                and cache_layer.aligned and reads_codes(ctx, qkv.dtype is torch.float32, n_heads, n_kv_heads)):
             return quantized_cache.attend_step(qkv, cache_layer, out, quantized_cache.step_of(ctx, n_heads, n_kv_heads, head_dim), scale,
                                                window if window else -int(chunk or 0), out_scale)
         return _over_quantized(qkv, cache_layer, out, ctx, n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, scale=scale,
@@ -238,8 +238,28 @@ def attention(qkv, cache_layer, out, ctx, *, n_heads, n_kv_heads, head_dim, scal
         gate=gate)
 
 
-# Rows (new tokens times query heads per kv head) of a sequence up to which a bfloat16 step reads the codes themselves
-QUANTIZED_ROWS = 64
+# Up to so many new tokens per sequence, or so many rows (tokens times query heads) of all sequences, a bfloat16 step reads the codes
+# themselves.  Its time is the rows' times the keys', 3.4 us per million of them (heads of 128); by way of float16 scratch it is a tile of
+# 128 tokens' walk over the keys, 15 us per thousand, and more once the tiles fill the SMs.  Measured, straight from the codes and by way of
+# scratch, us (32 heads over 8 kv heads of 128):
+#   1 sequence, 4,096 keys:    16 tokens 27 and 60, 64 tokens 43 and 61, 128 tokens 68 and 61;  30,000 keys: 64 tokens 190 and 460
+#   1 sequence, 512 keys:      16 tokens 14.0 and 13.9, 64 tokens 17.4 and 14.0
+#   8 sequences, 1,024 keys:   8 tokens 26 and 33, 16 tokens 33 and 34, 24 tokens 40 and 34;  8,000 keys: 16 tokens 116 and 204
+#   64 sequences, 1,024 keys:  16 tokens 166 and 220, 24 tokens 242 and 220
+# In float32 the other way (read back into float32 pages) is never faster: 4,096 keys, 1 sequence: 8 tokens 22 and 296, 1,000 tokens
+# 510 and 2184; 8 sequences of 1,000 tokens over 1,024 keys 1292 and 2510.
+CODES_TOKENS, CODES_ROWS = 16, 2048
+
+
+def reads_codes(ctx, f32: bool, n_heads: int, n_kv_heads: int) -> bool:
+    """Whether a step with the plain form of the score reads a cache in 8 bits directly."""
+    key = ("reads_codes", f32, n_heads, n_kv_heads)
+    answer = ctx.extras.get(key)
+    if answer is None:
+        few = ctx.max_new <= CODES_TOKENS or ctx.n_seqs * ctx.max_new * n_heads <= CODES_ROWS
+        answer = (f32 or few) and quantized_cache.attention_counts(ctx.n_seqs, ctx.page_table.shape[1], ctx.max_new, n_heads, n_kv_heads)
+        ctx.extras[key] = answer
+    return answer
 
 
 def _over_quantized(qkv, layer, out, ctx, *, window, chunk, keep_first, **forms):

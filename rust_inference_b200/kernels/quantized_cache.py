@@ -119,24 +119,15 @@ def widen(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, facto
 
 @functools.lru_cache(maxsize=None)
 def attention_workspace(n_heads: int, n_kv_heads: int, head_dim: int, max_new: int) -> tuple:
-    """(float32 numbers of scratch, int32 counters) that `attention` wants; the counters are zero when it begins, and when it ends."""
+    """(float32 numbers of scratch, int32 counters) that `attend_step` wants; the counters are zero when it begins, and when it ends."""
     blocks = int(load("attention_quantized").ri_attention_quantized_blocks())
     return 2 * blocks * min(16, max_new * (n_heads // n_kv_heads)) * (head_dim + 4), 4 * 2 * blocks
 
 
-def attention_supports(dtype: torch.dtype, head_dim: int, v_head_dim: int | None) -> bool:
-    """The sizes that `attention` takes."""
-    return dtype in (torch.float32, torch.bfloat16) and head_dim in (64, 128) and v_head_dim in (None, head_dim)
-
-
-def attention(q: torch.Tensor, layer: QuantizedPages, out: torch.Tensor, page_table: torch.Tensor, seq_slot, seq_start, cu_seqlens, *,
-              n_heads: int, n_kv_heads: int, head_dim: int, max_new: int, scale: float, part: torch.Tensor, arrived: torch.Tensor,
-              span: int = 0, out_scale: float = 1.0) -> torch.Tensor:
-    """Attention of every token of the step over its slot's cached keys, straight from the codes (csrc/attention_quantized.cu): for
-    steps of few tokens per sequence, and for float32.  q: rows whose leading n_heads * head_dim columns are the queries, rotated;
-    span: > 0 the last so many keys, < 0 the keys of the query's own block of -span positions; part, arrived: `attention_workspace`."""
-    step = _Step(page_table, seq_slot, seq_start, cu_seqlens, n_heads, n_kv_heads, head_dim, max_new, part, arrived)
-    return attend_step(q, layer, out, step, scale, span, out_scale)
+def attention_counts(n_seqs: int, pages: int, max_new: int, n_heads: int, n_kv_heads: int) -> bool:
+    """Whether `attend_step`'s units (pages of a kv head, for 8 rows) of a step over up to so many pages per sequence are counted in 31
+    bits.  (An item counts as four pages more.)"""
+    return n_seqs * (pages + 4) * n_kv_heads * ((max_new * (n_heads // n_kv_heads) + 7) // 8) < 1 << 31
 
 
 class _Step:
@@ -144,31 +135,31 @@ class _Step:
 
     __slots__ = ("native", "kept")
 
-    def __init__(self, page_table, seq_slot, seq_start, cu_seqlens, n_heads, n_kv_heads, head_dim, max_new, part, arrived):
-        what = "quantized_cache.attention"
-        _need(n_kv_heads > 0 and n_heads % n_kv_heads == 0 and attention_supports(torch.float32, head_dim, None) and page_table.dim() == 2, what,
+    def __init__(self, ctx, n_heads, n_kv_heads, head_dim):
+        what = "quantized_cache.attend_step"
+        table, n_seqs = ctx.page_table, ctx.seq_slot.numel()
+        _need(n_kv_heads > 0 and n_heads % n_kv_heads == 0 and head_dim in (64, 128) and table.dim() == 2, what,
               f"{n_heads} heads of {head_dim} over {n_kv_heads}, or a page table that is not [slots, pages]")
-        floats, ints = attention_workspace(n_heads, n_kv_heads, head_dim, max_new)
-        _need(part.is_cuda and part.dtype == torch.float32 and part.is_contiguous() and part.numel() >= floats, what, "scratch too small")
-        n_seqs = seq_slot.numel()
-        self.native = (_index(what, page_table, 1), page_table.shape[1], _index(what, seq_slot, n_seqs), _index(what, seq_start, n_seqs),
-                       _index(what, cu_seqlens, n_seqs + 1), n_seqs, max_new, n_heads, n_kv_heads, head_dim, part.data_ptr(), part.numel(),
-                       _index(what, arrived, ints))
-        self.kept = (page_table, seq_slot, seq_start, cu_seqlens, part, arrived)     # whose addresses these are
+        floats, ints = attention_workspace(n_heads, n_kv_heads, head_dim, ctx.max_new)
+        part = ctx.buffer("quantized_part", (floats,), torch.float32)
+        arrived = ctx.zeroed_buffer("quantized_arrived", (ints,), torch.int32)
+        self.native = (_index(what, table, 1), table.shape[1], _index(what, ctx.seq_slot, n_seqs), _index(what, ctx.seq_start, n_seqs),
+                       _index(what, ctx.cu_seqlens, n_seqs + 1), n_seqs, ctx.max_new, n_heads, n_kv_heads, head_dim, part.data_ptr(), part.numel(),
+                       _index(what, arrived, ints), ctx.max_len)
+        self.kept = (table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens, part, arrived)     # whose addresses these are
 
 
 def step_of(ctx, n_heads: int, n_kv_heads: int, head_dim: int) -> _Step:
-    """`attention`'s view of a step (`engine.context.StepContext`), made by the first layer that asks."""
+    """`attend_step`'s view of a step (`engine.context.StepContext`), made by the first layer that asks."""
     key = ("quantized", n_heads, n_kv_heads, head_dim)
     step = ctx.extras.get(key)
     if step is None:
-        floats, ints = attention_workspace(n_heads, n_kv_heads, head_dim, ctx.max_new)
-        step = ctx.extras[key] = _Step(ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens, n_heads, n_kv_heads, head_dim, ctx.max_new,
-                                       ctx.buffer("quantized_part", (floats,), torch.float32),
-                                       ctx.zeroed_buffer("quantized_arrived", (ints,), torch.int32))
+        step = ctx.extras[key] = _Step(ctx, n_heads, n_kv_heads, head_dim)
     return step
 
 
-def attend_step(q, layer, out, step, scale, span, out_scale):
-    """`attention` for a step that has been looked at."""
+def attend_step(q, layer: QuantizedPages, out, step: _Step, scale: float, span: int, out_scale: float) -> torch.Tensor:
+    """Attention of every token of the step over its slot's cached keys, straight from the codes (csrc/attention_quantized.cu), for heads
+    of 64 or 128.  q: float32 or bfloat16 rows whose leading columns are the queries, rotated; out: rows of q's dtype; span: > 0 the
+    last so many keys, < 0 the keys of the query's own block of -span positions, 0 all."""
     return native("attend")(q, layer.native, out, step.native, scale, span, out_scale)

@@ -76,3 +76,16 @@ def test_flags(tmp_path):
     for bad in (["--cache-dtype", "fp8"], ["--score", "-1"], ["--score", "65"], ["--score", "x"]):
         with pytest.raises(CliError):
             parse_args(base + bad)
+
+
+def test_which_steps_read_the_codes():
+    from types import SimpleNamespace
+    from rust_inference_b200.kernels import attention
+
+    def reads(n_seqs, max_new, f32=False, heads=32, kv=8, pages=64):
+        return attention.reads_codes(SimpleNamespace(n_seqs=n_seqs, max_new=max_new, page_table=torch.zeros(n_seqs, pages), extras={}), f32, heads, kv)
+
+    assert reads(1, 1) and reads(64, 1) and reads(64, 16) and reads(1, 64) and reads(1, 512, heads=4, kv=4)
+    assert not reads(64, 17) and not reads(1, 65) and not reads(8, 2048)
+    assert reads(8, 2048, f32=True) and reads(64, 2048, f32=True, pages=512)
+    assert not reads(64, 4096, f32=True, pages=2048)            # more units than 31 bits count: read back

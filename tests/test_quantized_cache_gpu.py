@@ -286,6 +286,77 @@ def test_attention(runs, n_heads, n_kv, hd, dtype, limits):
         assert (off <= 0.5 * bound).all(), float((off / bound).max())
 
 
+@pytest.mark.parametrize("runs", sorted(ATTEND))
+@pytest.mark.parametrize("n_heads, n_kv, hd, dtype", [
+    (14, 2, 64, torch.float32), (7, 1, 128, torch.bfloat16), (16, 1, 128, torch.float32), (16, 1, 64, torch.bfloat16), (40, 2, 128, torch.bfloat16)])
+def test_attention_in_wide_tiles(runs, n_heads, n_kv, hd, dtype):
+    """What the host knows of the lengths decides which tiles of rows a step is cut into, not what comes out: a step that might be long."""
+    from rust_inference_b200.kernels import quantized_cache as qc
+    step = Step(ATTEND[runs], n_kv, hd)
+    step.arrays([(s + n, 0) for s, n in ATTEND[runs]])
+    step.fill()
+    step.arrays(ATTEND[runs])
+    step.max_len = 1 << 24
+    q = torch.randn(step.n_tokens, n_heads * hd, generator=torch.Generator().manual_seed(9)).to(dtype)
+    out = torch.full((step.n_tokens, n_heads * hd), math.nan, dtype=dtype, device=DEV)
+    scale = 1.0 / math.sqrt(hd)
+    qc.attend_step(q.to(DEV), step.layer, out, qc.step_of(step.context(dtype), n_heads, n_kv, hd), scale, 0, 1.0)
+    k, v, ks, vs = step.host()
+    for b, (start, n) in enumerate(step.runs):
+        a, e = step.cu[b], step.cu[b + 1]
+        keys, vals = (plain.values(c, s, step.pages(b), start + n).double() for c, s in ((k, ks), (v, vs)))
+        unit, slip = UNITS[dtype]
+        want, bound = plain.attend(q[a:e].double().view(n, n_heads, hd), keys, vals, start, scale=scale, unit=unit, step=slip)
+        off = (out[a:e].cpu().double().view(n, n_heads, hd) - want).abs()
+        assert (off <= bound).all(), float((off / bound).max())
+
+
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("n_heads, n_kv, hd, dtype, runs", [
+    (8, 2, 64, torch.float32, [(57, 1003), (900, 700)]), (4, 1, 128, torch.float32, [(0, 1700)]),
+    (32, 8, 128, torch.bfloat16, [(1000 + 37 * i, 16 - i % 5) for i in range(12)]), (14, 2, 64, torch.bfloat16, [(2900 - i, 16) for i in range(10)]),
+    (32, 8, 128, torch.bfloat16, [(31990, 1)])])
+def test_attention_of_many_rows_and_keys(n_heads, n_kv, hd, dtype, runs, window):
+    """Steps that fill the SMs for long; some of their tokens."""
+    from rust_inference_b200.kernels import attention
+    step = Step(runs, n_kv, hd)
+    for t in (step.layer.k_scale, step.layer.v_scale):
+        t.uniform_(0.004, 0.016, generator=torch.Generator(DEV).manual_seed(3))
+    q = torch.randn(step.n_tokens, n_heads * hd, generator=torch.Generator().manual_seed(10)).to(dtype)
+    out = torch.full((step.n_tokens, n_heads * hd), math.nan, dtype=dtype, device=DEV)
+    scale = 1.0 / math.sqrt(hd)
+    attention.attention(q.to(DEV), step.layer, out, step.context(dtype), n_heads=n_heads, n_kv_heads=n_kv, head_dim=hd, scale=scale, window=window)
+    assert out.isfinite().all()
+    k, v, ks, vs = step.host()
+    unit, slip = UNITS[dtype]
+    for b, (start, n) in list(enumerate(runs))[:3]:
+        keys, vals = (plain.values(c, s, step.pages(b), start + n).double() for c, s in ((k, ks), (v, vs)))
+        for t in sorted({0, n // 3, n // 2, n - 1}):
+            row, pos = step.cu[b] + t, start + t
+            want, bound = plain.attend(q[row:row + 1].double().view(1, n_heads, hd), keys[:pos + 1], vals[:pos + 1], pos, scale=scale, unit=unit,
+                                       step=slip, window=window)
+            off = (out[row].cpu().double().view(1, n_heads, hd) - want).abs()
+            assert (off <= bound).all(), (b, t, float((off / bound).max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_over_codes_off_a_16_byte_boundary(dtype):
+    """Such a layer is read back."""
+    from rust_inference_b200.kernels import attention
+    qc = _qc()
+    step = Step([(77, 3), (10, 1)], 2, 64)
+    step.arrays([(80, 0), (11, 0)])
+    step.fill()
+    step.arrays([(77, 3), (10, 1)])
+    codes = [torch.empty(t.numel() + 1, dtype=torch.int8, device=DEV)[1:].view(t.shape).copy_(t) for t in (step.layer.k, step.layer.v)]
+    moved = qc.QuantizedPages(*codes, step.layer.k_scale, step.layer.v_scale)
+    q = torch.randn(step.n_tokens, 8 * 64, device=DEV).to(dtype)
+    got, want = torch.empty_like(q), torch.empty_like(q)
+    for layer, out in ((moved, got), (step.layer, want)):
+        attention.attention(q, layer, out, step.context(dtype), n_heads=8, n_kv_heads=2, head_dim=64, scale=0.125)
+    assert (got.float() - want.float()).abs().max() <= (2.0 ** -6 if dtype == torch.bfloat16 else 1e-4) * want.float().abs().max()
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_attention_past_what_it_does_not_see(hd, dtype):

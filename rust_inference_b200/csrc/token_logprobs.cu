@@ -154,8 +154,9 @@ __device__ void one_by_one(const T* x, int vocab, int top, float m, float log_z,
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 3)
+// PER_SM: blocks that an SM holds
+template <typename T, int PER_SM>
+__global__ void __launch_bounds__(THREADS, PER_SM)
 logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, int top, float* __restrict__ logprob, float* __restrict__ entropy,
                 int* __restrict__ top_ids, float* __restrict__ top_logprobs, int blocks) {
     constexpr int N = Piece<T>::N, AT_ONCE = 4;
@@ -181,11 +182,12 @@ logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, in
     }
     Sums mine = {-FLT_MAX, 0.f, 0.f};            // (a finite reference: minus infinity less it is minus infinity)
     float most = -INFINITY;
-    for (int p = p0 + tid; p < p1; p += AT_ONCE * THREADS) {
-        uint4 v[AT_ONCE];
+    auto get = [&](uint4 (&v)[AT_ONCE], int p) {
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k)
             if (p + k * THREADS < p1) v[k] = load16(body + (size_t)(p + k * THREADS) * N);
+    };
+    auto take = [&](const uint4 (&v)[AT_ONCE], int p) {
         float higher = -INFINITY;
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k)
@@ -199,6 +201,24 @@ logprobs_kernel(const T* logits, long long ld, int vocab, const int* targets, in
             Piece<T>::open(v[k], f);
 #pragma unroll
             for (int i = 0; i < N; ++i) add(mine, f[i]);
+        }
+    };
+    constexpr int TURN = AT_ONCE * THREADS;
+    uint4 v[AT_ONCE];
+    if (PER_SM == 2) {                           // the next pieces are on their way while these are worked on
+        uint4 w[AT_ONCE];
+        int p = p0 + tid;
+        get(v, p);
+        for (; p < p1; p += 2 * TURN) {
+            get(w, p + TURN);
+            take(v, p);
+            get(v, p + 2 * TURN);
+            take(w, p + TURN);
+        }
+    } else {
+        for (int p = p0 + tid; p < p1; p += TURN) {
+            get(v, p);
+            take(v, p);
         }
     }
     for (int i = tid; i < singles; i += THREADS) {
@@ -389,7 +409,7 @@ int clusters_held(int blocks) {
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&n, logprobs_kernel<T>, &cfg) != cudaSuccess || n <= 0) {
+        if (cudaOccupancyMaxActiveClusters(&n, logprobs_kernel<T, 2>, &cfg) != cudaSuccess || n <= 0) {
             cudaGetLastError();
             n = 1;
         }
@@ -406,22 +426,26 @@ RI_API int ri_token_logprobs(const void* logits, int dtype, long long ld, int ro
     if (rows <= 0) return 0;
     if (vocab <= 0 || top < 0 || top > vocab || top > MOST_TOP) return fail("token_logprobs: %d alternatives of %d tokens", top, vocab);
     // Blocks per row: what a block does beside its part of the row, and clusters that wait for one another, have to be paid by shorter
-    // parts.  So parts of 8,192 logits or more where the blocks leave half of the SMs alone, of 28,000 or more up to as many clusters as the
+    // parts.  So parts of 8,192 logits or more where the blocks leave half of the SMs alone, of 24,000 or more up to as many clusters as the
     // SMs hold at once (a cluster more costs a second round).  With 1, 2, 4 and 8, us, and the five likeliest, bfloat16:
-    //   vocabulary 128,256:  1 row 14.1, 10.1, 7.2, 6.1;  48 rows 14.4, 12.0, 11.6, 10.9;  90 rows 19.0, 17.9, 13.6, 19.3;  148 rows 17.7, 15.9, 22.2, 29.8
-    //   vocabulary 32,000:   1 row 6.5, 5.9, 5.5, 5.5;    48 rows 6.7, 7.1, 8.1, 8.5;      90 rows 7.5, 9.6, 9.2, 15.6;     148 rows 7.0, 9.6, 14.8, 23.5
+    //   vocabulary 128,256:  1 row 12.8, 9.4, 6.9, 6.2;  48 rows 13.2, 10.5, 10.1, 15.2;  90 rows 18.5, 14.1, 14.8, 23.4;  148 rows 15.2, 14.7, 23.2, 37.1
+    //   vocabulary 32,000:   1 row 6.1, 6.1, 5.8, 5.5;   48 rows 6.4, 7.1, 7.5, 12.6;     90 rows 7.9, 8.3, 13.3, 19.4;    148 rows 6.5, 8.7, 17.5, 30.2
     const bool f32 = dtype == RI_F32;
     int blocks = 1;
     for (int b = 2; b <= MOST_BLOCKS; ++b)
-        if ((2ll * rows * b <= sm_count() && vocab >= 8192 * b) || (vocab >= 28000 * b && rows <= (f32 ? clusters_held<float>(b) : clusters_held<__nv_bfloat16>(b))))
+        if ((2ll * rows * b <= sm_count() && vocab >= 8192 * b) || (vocab >= 24000 * b && rows <= (f32 ? clusters_held<float>(b) : clusters_held<__nv_bfloat16>(b))))
             blocks = b;
     if ((long long)rows * blocks > 0x7fffffff) return fail("token_logprobs: %d rows are too many", rows);
     auto launch = [&](auto kernel, auto* x) {
         return launch_cluster("token_logprobs", kernel, dim3((unsigned)(rows * blocks)), THREADS, 0, blocks, stream, x, ld, vocab, targets, top,
                               logprob, entropy, top_ids, top_logprobs, blocks);
     };
-    if (dtype == RI_F32) return launch(logprobs_kernel<float>, (const float*)logits);
-    if (dtype == RI_BF16) return launch(logprobs_kernel<__nv_bfloat16>, (const __nv_bfloat16*)logits);
+    // Two blocks per SM whose threads fetch while they work, or, where the rows are more than those, three that do not (their registers
+    // hold one turn), us with the five likeliest: vocabulary 151,936, float32, 61 rows 11.9 and 14.0, 148 rows 20.8 and 24.6, 300 rows 49.7 and
+    // 39.5, 2,047 rows (the likeliest) 224 and 212.
+    const bool many = rows > 2 * sm_count();
+    if (dtype == RI_F32) return many ? launch(logprobs_kernel<float, 3>, (const float*)logits) : launch(logprobs_kernel<float, 2>, (const float*)logits);
+    if (dtype == RI_BF16) return many ? launch(logprobs_kernel<__nv_bfloat16, 3>, (const __nv_bfloat16*)logits) : launch(logprobs_kernel<__nv_bfloat16, 2>, (const __nv_bfloat16*)logits);
     return fail("token_logprobs: unknown dtype %d", dtype);
 }
 

@@ -25,12 +25,13 @@
 // all blocks have the same to read.  A block's four warps take half of one of two pages each at a time, every warp with a ring of its
 // own that cp.async fills (no barrier inside a run).  An item (sequence, kv head, tile) that lies in one block is finished there;
 // one that spreads over several is written as partial sums, which the blocks that arrive last (a counter per eight parts) add up
-// in the order of the blocks, so that the result does not depend on who was last.
+// in the order of the blocks, so that the result does not depend on who was last.  Where few items are short, each gets a cluster of
+// blocks instead, which add their parts up through distributed shared memory, a third of what meeting in memory takes.
 //
 // Fragments come straight from 16-byte reads of shared memory, because the order of a contraction's terms, and which channel is which
 // row of a product, are free: lane (g, t) holds of the keys g and g + 8 the channels t HD/4 .. + HD/4, of its four keys (2t,
 // 2t + 1, 2t + 8, 2t + 9) the channels g HD/8 .. + HD/8, and of the result's rows 2t and 2t + 1 those channels again.
-#include "common.cuh"
+#include "cluster.cuh"
 
 #include <cuda_fp16.h>
 
@@ -48,6 +49,7 @@ constexpr int SETUP = 4;
 // What a block has at least: the two pages of one turn, or as many turns as keep an item's parts to eight (64), which are added up in
 // one go (two): up to 4 pages (8).
 __device__ __forceinline__ int least_pages(int pages, int items) { return pages <= 16 * items ? 2 : (pages <= 256 * items ? 4 : 8); }
+constexpr int TURNS = 4;                         // of a block, at most, where its cluster has an item of its own
 // Parts of an item are added up eight at a time: a block that arrives last of eight adds theirs and goes on with seven others
 constexpr int GROUP = 8;
 // Weights are formed times 2^6 against a reference that follows the row's maximum only when that is 2^8 times ahead: they stay below
@@ -72,6 +74,7 @@ struct Args {
     float4* stat;                                // [2 * blocks][rows_cap]: maximum, sum, unit of the sums
     int* arrived;                                // [4][2 * blocks] (8^4 parts are more than there are blocks), zero between calls
     int places;                                  // 2 * blocks
+    int cluster;                                 // blocks of a cluster, one for every item; 1: runs of units
     int rows_cap;                                // rows of a tile that any item fills
 };
 
@@ -84,8 +87,8 @@ struct Item {
     const int* table;                            // its pages' numbers
 };
 
-__device__ __forceinline__ int units_of(const Args& a, int start, int n, int rows) {
-    return n > 0 ? ((start + n - 1) / PAGE + 1 - first_visible_key(start, a.span) / PAGE + SETUP) * a.n_kv * ((n * a.n_rep + rows - 1) / rows) : 0;
+__device__ __forceinline__ int pages_of(const Args& a, int start, int n) {       // (of a sequence with new tokens)
+    return (start + n - 1) / PAGE + 1 - first_visible_key(start, a.span) / PAGE;
 }
 __device__ __forceinline__ void enter(const Args& a, int seq, int first_tok, int n, int start, int slot, int rows, Item& it) {
     it.seq = seq;
@@ -212,7 +215,8 @@ template <int HD, int NQ> constexpr int PART_BYTES = NQ == 1 ? 0 : 8 * NQ * HD *
 template <int HD, int NQ> constexpr int SMEM_BYTES = WARPS * (OWN_BYTES<HD> + PART_BYTES<HD, NQ> + 8 * NQ * 16);
 
 // NQ: tiles of 8 query rows; TERMS: float16 numbers per weight, TERMS + 1 bytes per query channel
-template <int HD, typename T, int TERMS, int NQ>
+// own: every item has a cluster of blocks of its own; else equal runs of units
+template <int HD, typename T, int TERMS, int NQ, bool own>
 __global__ void __launch_bounds__(THREADS, TERMS * NQ == 1 ? 4 : 2)
 attn_quantized_kernel(const Args a) {
     constexpr int ROWS = 8 * NQ;
@@ -224,9 +228,9 @@ attn_quantized_kernel(const Args a) {
     static_assert(PART > 0 || ROWS * HD * 4 <= 2 * TILE, "a warp's sums fit where its values were");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int sums[THREADS + 1];
-    __shared__ int found[6], items;
+    __shared__ int found[6], totals[WARPS][2];
     __shared__ int last_here;
-    __shared__ float4 sgroup[GROUP][ROWS];       // statistics of parts that are added up
+    __shared__ float4 sgroup[GROUP][ROWS];       // statistics of parts that are added up (a cluster's: each block's own first)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     let_next_kernel_start();
 
@@ -234,15 +238,31 @@ attn_quantized_kernel(const Args a) {
     const int per = (a.n_seqs + THREADS - 1) / THREADS;
     int mine = 0, mine_items = 0, slot = 0;
     for (int s = tid * per; s < min((tid + 1) * per, a.n_seqs); ++s) {
-        const int n = a.cu_seqlens[s + 1] - a.cu_seqlens[s];
-        mine += units_of(a, a.seq_start[s], n, ROWS);
-        mine_items += a.n_kv * ((n * a.n_rep + ROWS - 1) / ROWS);
+        const int n = a.cu_seqlens[s + 1] - a.cu_seqlens[s], start = a.seq_start[s];
+        const int each = a.n_kv * ((n * a.n_rep + ROWS - 1) / ROWS);
+        if (n > 0) mine += (pages_of(a, start, n) + SETUP) * each;
+        mine_items += each;
         slot = a.seq_slot[s];                    // (in the cache for when it is wanted)
     }
-    sums[tid + 1] = mine;
-    if (tid == 0) sums[0] = items = 0;
+    const int me = blockIdx.x, C = a.cluster;
+    sums[tid + 1] = own ? mine_items : mine;
+    if (tid == 0) sums[0] = 0;
+    {
+        const int units = __reduce_add_sync(0xffffffffu, mine), n = __reduce_add_sync(0xffffffffu, mine_items);
+        if (lane == 0) totals[warp][0] = units, totals[warp][1] = n;
+    }
     __syncthreads();
-    if (mine_items) atomicAdd(&items, mine_items);
+    int total = 0, items = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) total += totals[w][0], items += totals[w][1];
+    const int least = least_pages(total - SETUP * items, items), blocks = min((int)gridDim.x, (total + least - 1) / least);
+    // a cluster's item is cut into equal runs of whole turns
+    auto run_of = [&](int pages) { return max(2, ((pages + C - 1) / C + 1) & ~1); };
+    auto leave = [&]() {                         // (who waits for this kernel waits for those before it too)
+        wait_for_previous_kernels();
+        if (own) cluster_sync(), cluster_sync();
+    };
+    if (me >= (own ? items * C : blocks)) return leave();
     if (warp == 0) {                             // running sums of the 128 numbers, four per lane
         int v[4], run = 0;
 #pragma unroll
@@ -258,19 +278,14 @@ attn_quantized_kernel(const Args a) {
         for (int i = 0; i < 4; ++i) sums[4 * lane + 1 + i] = v[i] + before;
     }
     __syncthreads();
-    const int total = sums[THREADS], me = blockIdx.x;
-    const int least = least_pages(total - SETUP * items, items), blocks = min((int)gridDim.x, (total + least - 1) / least);
-    if (me >= blocks) {
-        wait_for_previous_kernels();             // (who waits for this kernel waits for those before it too)
-        return;
-    }
     // the first `more` runs have one unit more than `each`
-    const int each = total / blocks, more = total % blocks;
+    const int each = total / max(blocks, 1), more = total % max(blocks, 1);
     auto run_start = [&](int b) { return b * each + min(b, more); };
-    const int u0 = run_start(me), u1 = run_start(me + 1);
+    const int u0 = own ? me / C : run_start(me);
     if (sums[tid] <= u0 && u0 < sums[tid + 1]) {
         int at = sums[tid], s = tid * per, first_tok = a.cu_seqlens[s], n = a.cu_seqlens[s + 1] - first_tok, start = a.seq_start[s];
-        for (int units; at + (units = units_of(a, start, n, ROWS)) <= u0;) {
+        auto many = [&]() { return n > 0 ? (own ? 1 : pages_of(a, start, n) + SETUP) * a.n_kv * ((n * a.n_rep + ROWS - 1) / ROWS) : 0; };
+        for (int units; at + (units = many()) <= u0;) {
             at += units;
             ++s;
             first_tok += n;
@@ -283,18 +298,22 @@ attn_quantized_kernel(const Args a) {
     __syncthreads();
     Item it;
     enter(a, found[0], found[2], found[3], found[4], found[5], ROWS, it);
-    int page, u;                                 // the next page, and its place among the units
+    int page, u, u1;                             // the next page, and its place among the units (its number, with a cluster); the run's end
     {
-        const int within = u0 - found[1], n = it.end - it.low + SETUP, at = within % n;
+        const int within = u0 - found[1], n = own ? 1 : it.end - it.low + SETUP, at = within % n;
         it.tile = within / n % it.tiles;
         it.head = within / n / it.tiles;
-        page = it.low + max(at - SETUP, 0);
-        u = u0 + max(SETUP - at, 0);
+        if (own) {
+            const int run = run_of(it.end - it.low);
+            u = page = it.low + me % C * run;
+            u1 = min(it.end, page + run);
+        } else {
+            page = it.low + max(at - SETUP, 0);
+            u = u0 + max(SETUP - at, 0);
+            u1 = run_start(me + 1);
+        }
     }
-    if (u >= u1) {
-        wait_for_previous_kernels();
-        return;
-    }
+    if (u >= u1) return leave();
 
     // ---- half a page at a time: keys are on their way while values are worked on, values while scores are ----
     unsigned char* kt = smem + warp * OWN;
@@ -335,7 +354,7 @@ attn_quantized_kernel(const Args a) {
                 if (lane < 2) copy4(k_to + 4 * TILE + 4 * lane, a.ks + v_tile * (PAGE / BLOCK) + my_half / BLOCK + lane);
             }
             ahead_page += 2;
-            if (ahead_page >= ahead_stop && ahead_stop == ahead.end && (ahead_u += SETUP + ahead.end - ahead.low) < u1) {
+            if (!own && ahead_page >= ahead_stop && ahead_stop == ahead.end && (ahead_u += SETUP + ahead.end - ahead.low) < u1) {
                 next_item(a, ROWS, ahead);
                 ahead_page = ahead.low;
                 ahead_stop = min(ahead.end, ahead.low + (u1 - ahead_u));
@@ -358,6 +377,12 @@ attn_quantized_kernel(const Args a) {
     // a warp's sums [WARPS][ROWS][HD] and their rows' statistics [WARPS][ROWS]
     auto part_at = [&](int w) { return reinterpret_cast<float*>(smem + (PART ? WARPS * OWN + w * PART : w * OWN + 2 * TILE)); };
     float4* sml = reinterpret_cast<float4*>(smem + WARPS * (OWN + PART));
+    auto write = [&](const Item& i, int row, int d, float4 v, float sum, float s) {
+        const float inv = 1.f / sum, f = s * a.out_scale;
+        v = make_float4(v.x * inv * f, v.y * inv * f, v.z * inv * f, v.w * inv * f);
+        store4<T>(reinterpret_cast<T*>(a.out) + (size_t)(i.first_tok + row / a.n_rep) * a.out_ld + (size_t)(i.head * a.n_rep + row % a.n_rep) * HD + d,
+                  a.out_vec, v);
+    };
     while (true) {
         // ---- an item's part in this block: pages page .. stop - 1 ----
         const int stop = min(it.end, page + (u1 - u));
@@ -617,13 +642,6 @@ attn_quantized_kernel(const Args a) {
                 }
             }
         __syncthreads();
-        auto write = [&](int row, int d, float4 v, float sum, float s) {
-            const float inv = 1.f / sum, f = s * a.out_scale;
-            v = make_float4(v.x * inv * f, v.y * inv * f, v.z * inv * f, v.w * inv * f);
-            row += row0;
-            store4<T>(reinterpret_cast<T*>(a.out) + (size_t)(it.first_tok + row / a.n_rep) * a.out_ld +
-                      (size_t)(it.head * a.n_rep + row % a.n_rep) * HD + d, a.out_vec, v);
-        };
         auto block_of = [&](int x) { return x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each; };
         const int first_block = block_of(item_u), parts = block_of(item_u + item_n - 1) - first_block + 1;
         // a block has two places: for an item whose pages began before its run (or with it), and for one whose began inside
@@ -647,14 +665,17 @@ attn_quantized_kernel(const Args a) {
                 v = make_float4(fmaf(p.x, x, v.x), fmaf(p.y, x, v.y), fmaf(p.z, x, v.z), fmaf(p.w, x, v.w));
             }
             if (whole) {
-                write(row, d, v, sum, s);
+                write(it, row0 + row, d, v, sum, s);
+            } else if (own) {
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(smem) + row * HD + d) = v;       // where the first warp's keys were
+                if (d == 0) sgroup[0][row] = make_float4(top, sum, s, 0.f);
             } else {
                 const size_t at = (size_t)place_of(me - first_block) * a.rows_cap + row;
                 *reinterpret_cast<float4*>(a.part + at * HD + d) = v;
                 if (d == 0) a.stat[at] = make_float4(top, sum, s, 0.f);
             }
         }
-        if (!whole) {
+        if (!own && !whole) {
             int n = parts, index = me - first_block, stride = 1;       // parts of this level, this block's among them, how far apart they lie
             for (int level = 0;; ++level) {
                 const int lead = index / GROUP * GROUP, members = min(GROUP, n - lead);
@@ -713,7 +734,7 @@ attn_quantized_kernel(const Args a) {
                             const float w = x < members ? sgroup[x][row].w : 0.f;
                             v = make_float4(fmaf(p[z][x].x, w, v.x), fmaf(p[z][x].y, w, v.y), fmaf(p[z][x].z, w, v.z), fmaf(p[z][x].w, w, v.w));
                         }
-                        if (done) write(row, d, v, sml[row].y, sml[row].z);
+                        if (done) write(it, row0 + row, d, v, sml[row].y, sml[row].z);
                         // in the place of the first (its channels are this thread's; its statistics have been read)
                         else *reinterpret_cast<float4*>(a.part + ((size_t)place_of(lead * stride) * a.rows_cap + row) * HD + d) = v;
                     }
@@ -725,36 +746,87 @@ attn_quantized_kernel(const Args a) {
                 stride *= GROUP;
             }
         }
-        if (stop != it.end || (u += SETUP) >= u1) break;
+        if (own || stop != it.end || (u += SETUP) >= u1) break;
         __syncthreads();                         // the warps' parts have been read
         next_item(a, ROWS, it);
         page = it.low;
     }
     copies_wait<0>();
+    if (!own) return;
+
+    // ---- a cluster's parts: a warp for each row, eight lanes (four times) for their statistics, then one for each four channels ----
+    cluster_sync();
+    const int run = run_of(it.end - it.low), parts = (it.end - it.low + run - 1) / run, row0 = it.tile * ROWS, here = min(ROWS, it.n_rows - row0);
+    for (int row = me % C + parts * warp; parts > 1 && row < here; row += parts * WARPS) {
+        const int x8 = lane & 7;
+        float4 st = make_float4(LOWEST, 0.f, 0.f, 0.f), v = make_float4(0.f, 0.f, 0.f, 0.f), p[8];
+        if (x8 < parts) st = peer_float4(reinterpret_cast<const float*>(&sgroup[0][row]), x8);
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            p[x] = x < parts && 4 * lane < HD ? peer_float4(reinterpret_cast<const float*>(smem) + row * HD + 4 * lane, x) : make_float4(0.f, 0.f, 0.f, 0.f);
+        float top = st.x, s = st.z;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
+        }
+        const float f = merge_weight(st.x, top), w = f * unit_ratio(st.z, s);
+        float sum = st.y * f;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const float z = __shfl_sync(0xffffffffu, w, x);
+            v = make_float4(fmaf(p[x].x, z, v.x), fmaf(p[x].y, z, v.y), fmaf(p[x].z, z, v.z), fmaf(p[x].w, z, v.w));
+        }
+        if (4 * lane < HD) write(it, row0 + row, 4 * lane, v, sum, s);
+    }
+    cluster_sync();                              // a peer may still be reading this block's part
 }
 
 template <int HD, typename T, int TERMS, int NQ>
-int launch(Args a, long long part_floats, cudaStream_t stream) {
-    static PerDeviceOnce once;
-    static std::atomic<int> resident[64];
-    auto kernel = attn_quantized_kernel<HD, T, TERMS, NQ>;
+int launch(Args a, long long items, long long keys, long long part_floats, cudaStream_t stream) {
+    static PerDeviceOnce once, once_own;
+    static std::atomic<int> resident[64][3];
+    const auto kernel = attn_quantized_kernel<HD, T, TERMS, NQ, false>, kernel_own = attn_quantized_kernel<HD, T, TERMS, NQ, true>;
     constexpr int smem = SMEM_BYTES<HD, NQ>;
-    if (raise_dynamic_smem(kernel, smem, once, "attention_quantized")) return 1;
-    // as many blocks as the device holds at once (asked once per device)
-    int dev = 0, per_sm = 0;
+    if (raise_dynamic_smem(kernel, smem, once, "attention_quantized") || raise_dynamic_smem(kernel_own, smem, once_own, "attention_quantized")) return 1;
+    // as many blocks as the device holds at once, in clusters of eight, of four or alone (asked once per device)
+    int dev = 0;
     cudaGetDevice(&dev);
-    if (dev >= 0 && dev < 64) per_sm = resident[dev].load(std::memory_order_relaxed);
-    if (per_sm == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, THREADS, smem) != cudaSuccess || per_sm <= 0) per_sm = 1;
-        if (per_sm > MOST_BLOCKS) per_sm = MOST_BLOCKS;
-        if (dev >= 0 && dev < 64) resident[dev].store(per_sm, std::memory_order_relaxed);
-    }
-    const int blocks = per_sm * sm_count();
+    auto held = [&](int which) {
+        const int size = which == 2 ? 1 : 8 >> which;
+        int n = dev >= 0 && dev < 64 ? resident[dev][which].load(std::memory_order_relaxed) : 0;
+        if (n == 0) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)size);
+            cfg.blockDim = dim3(THREADS);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = (unsigned)size;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            const cudaError_t e = size == 1 ? cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, THREADS, smem) : cudaOccupancyMaxActiveClusters(&n, kernel_own, &cfg);
+            if (e != cudaSuccess || n <= 0) cudaGetLastError(), n = 1;
+            n = std::min(size == 1 ? n * sm_count() : n, MOST_BLOCKS * sm_count() / size);
+            if (dev >= 0 && dev < 64) resident[dev][which].store(n, std::memory_order_relaxed);
+        }
+        return n * size;
+    };
+    // A cluster for each item, of eight blocks or of four, where the device holds them all and nobody takes more than TURNS turns: else the
+    // longest of the sequences holds the others up.  With and without, us: 1 sequence of 437 keys, 14 heads over 2 of 64, 1 token 5.7 and
+    // 6.4; 32 heads over 8 of 128: 8 sequences of 4,096, 2 tokens 19.9 and 25.1; 1 of 512, 16 tokens 11.8 and 12.3; float32, 1 of 4,096 11.6 and 12.5.
+    auto fits = [&](int size) { return keys <= (long long)TURNS * 2 * PAGE * size; };
+    const int which = 8 * items <= held(0) && fits(8) ? 0 : (4 * items <= held(1) && fits(4) ? 1 : 2);
+    a.cluster = which == 2 ? 1 : 8 >> which;
+    const int blocks = which == 2 ? held(2) : a.cluster * (int)items;
     if (part_floats < 2ll * blocks * a.rows_cap * (HD + 4)) return fail("attention_quantized: scratch of %lld numbers is too small", part_floats);
     a.places = 2 * blocks;
     a.stat = reinterpret_cast<float4*>(a.part);
     a.part += (size_t)2 * blocks * a.rows_cap * 4;
-    return check_launch(launch_dependent(kernel, dim3((unsigned)blocks), dim3(THREADS), (size_t)smem, stream, a), "attention_quantized");
+    return launch_cluster("attention_quantized", which == 2 ? kernel : kernel_own, dim3((unsigned)blocks), THREADS, (size_t)smem, a.cluster, stream, a);
 }
 
 }  // namespace
@@ -803,11 +875,12 @@ RI_API int ri_attention_quantized(const void* q, int dtype, int q_ld, const int8
     const long long keys = span == 0 ? longest : std::min((long long)longest, (long long)max_new + (span > 0 ? span : -(long long)span));
     const int nq = 7 * wide < 4 * tiles && (keys + PAGE - 1) / PAGE * tiles * n_seqs * n_kv > 80ll * sm_count() ? 2 : 1;
     a.rows_cap = (int)(rows < 8 * nq ? rows : 8 * nq);
-    if (dtype == RI_F32 && nq == 1) return hd == 64 ? launch<64, float, 2, 1>(a, part_floats, stream) : launch<128, float, 2, 1>(a, part_floats, stream);
-    if (dtype == RI_F32) return hd == 64 ? launch<64, float, 2, 2>(a, part_floats, stream) : launch<128, float, 2, 2>(a, part_floats, stream);
+    const long long items = n_seqs * (nq == 1 ? tiles : wide) * n_kv;          // at most
+    if (dtype == RI_F32 && nq == 1) return hd == 64 ? launch<64, float, 2, 1>(a, items, keys, part_floats, stream) : launch<128, float, 2, 1>(a, items, keys, part_floats, stream);
+    if (dtype == RI_F32) return hd == 64 ? launch<64, float, 2, 2>(a, items, keys, part_floats, stream) : launch<128, float, 2, 2>(a, items, keys, part_floats, stream);
     if (dtype == RI_BF16 && nq == 1)
-        return hd == 64 ? launch<64, __nv_bfloat16, 1, 1>(a, part_floats, stream) : launch<128, __nv_bfloat16, 1, 1>(a, part_floats, stream);
-    if (dtype == RI_BF16) return hd == 64 ? launch<64, __nv_bfloat16, 1, 2>(a, part_floats, stream) : launch<128, __nv_bfloat16, 1, 2>(a, part_floats, stream);
+        return hd == 64 ? launch<64, __nv_bfloat16, 1, 1>(a, items, keys, part_floats, stream) : launch<128, __nv_bfloat16, 1, 1>(a, items, keys, part_floats, stream);
+    if (dtype == RI_BF16) return hd == 64 ? launch<64, __nv_bfloat16, 1, 2>(a, items, keys, part_floats, stream) : launch<128, __nv_bfloat16, 1, 2>(a, items, keys, part_floats, stream);
     return fail("attention_quantized: unknown dtype %d", dtype);
 }
 

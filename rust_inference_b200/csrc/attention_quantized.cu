@@ -49,7 +49,6 @@ constexpr int SETUP = 4;
 // What a block has at least: the two pages of one turn, or as many turns as keep an item's parts to eight (64), which are added up in
 // one go (two): up to 4 pages (8).
 __device__ __forceinline__ int least_pages(int pages, int items) { return pages <= 16 * items ? 2 : (pages <= 256 * items ? 4 : 8); }
-constexpr int TURNS = 4;                         // of a block, at most, where its cluster has an item of its own
 // Parts of an item are added up eight at a time: a block that arrives last of eight adds theirs and goes on with seven others
 constexpr int GROUP = 8;
 // Weights are formed times 2^6 against a reference that follows the row's maximum only when that is 2^8 times ahead: they stay below
@@ -815,10 +814,12 @@ int launch(Args a, long long items, long long keys, long long part_floats, cudaS
         }
         return n * size;
     };
-    // A cluster for each item, of eight blocks or of four, where the device holds them all and nobody takes more than TURNS turns: else the
-    // longest of the sequences holds the others up.  With and without, us: 1 sequence of 437 keys, 14 heads over 2 of 64, 1 token 5.7 and
-    // 6.4; 32 heads over 8 of 128: 8 sequences of 4,096, 2 tokens 19.9 and 25.1; 1 of 512, 16 tokens 11.8 and 12.3; float32, 1 of 4,096 11.6 and 12.5.
-    auto fits = [&](int size) { return keys <= (long long)TURNS * 2 * PAGE * size; };
+    // A cluster for each item, of eight blocks or of four, where the device holds them all and nobody takes more than four turns, or eight
+    // where there is one sequence (of several the longest holds the others up: with 8 sequences runs of units win once their
+    // lengths are half of the longest on average).  With and without, us, 32 heads over 8 of 128: 1 sequence of 1,024 keys 5.7 and 9.1, 4,096
+    // 8.9 and 14.1, 8,192 12.9 and 14.4, 16,384 23.0 and 17.3; 8 sequences of 4,096 17.2 and 23.4, 2,048 without 14.6; 16 of 2,048 (fours)
+    // 17.5 and 20.9; float32, 4 of 4,096 12.8 and 18.3; 14 heads over 2 of 64: 1 of 437 4.9 and 6.4, 32 of 4,096 11.9 and 17.8.
+    auto fits = [&](int size) { return keys <= (long long)(a.n_seqs == 1 ? 8 : 4) * 2 * PAGE * size; };
     const int which = 8 * items <= held(0) && fits(8) ? 0 : (4 * items <= held(1) && fits(4) ? 1 : 2);
     a.cluster = which == 2 ? 1 : 8 >> which;
     const int blocks = which == 2 ? held(2) : a.cluster * (int)items;

@@ -787,7 +787,8 @@ template <int HD, typename T, int TERMS, int NQ>
 int launch(Args a, long long items, long long keys, long long part_floats, cudaStream_t stream) {
     static PerDeviceOnce once, once_own;
     static std::atomic<int> resident[64][3];
-    const auto kernel = attn_quantized_kernel<HD, T, TERMS, NQ, false>, kernel_own = attn_quantized_kernel<HD, T, TERMS, NQ, true>;
+    // (tiles of 16 rows are for steps that do not fit clusters)
+    const auto kernel = attn_quantized_kernel<HD, T, TERMS, NQ, false>, kernel_own = attn_quantized_kernel<HD, T, TERMS, NQ, NQ == 1>;
     constexpr int smem = SMEM_BYTES<HD, NQ>;
     if (raise_dynamic_smem(kernel, smem, once, "attention_quantized") || raise_dynamic_smem(kernel_own, smem, once_own, "attention_quantized")) return 1;
     // as many blocks as the device holds at once, in clusters of eight, of four or alone (asked once per device)
@@ -820,7 +821,7 @@ int launch(Args a, long long items, long long keys, long long part_floats, cudaS
     // 8.9 and 14.1, 8,192 12.9 and 14.4, 16,384 23.0 and 17.3; 8 sequences of 4,096 17.2 and 23.4, 2,048 without 14.6; 16 of 2,048 (fours)
     // 17.5 and 20.9; float32, 4 of 4,096 12.8 and 18.3; 14 heads over 2 of 64: 1 of 437 4.9 and 6.4, 32 of 4,096 11.9 and 17.8.
     auto fits = [&](int size) { return keys <= (long long)(a.n_seqs == 1 ? 8 : 4) * 2 * PAGE * size; };
-    const int which = 8 * items <= held(0) && fits(8) ? 0 : (4 * items <= held(1) && fits(4) ? 1 : 2);
+    const int which = NQ > 1 ? 2 : (8 * items <= held(0) && fits(8) ? 0 : (4 * items <= held(1) && fits(4) ? 1 : 2));
     a.cluster = which == 2 ? 1 : 8 >> which;
     const int blocks = which == 2 ? held(2) : a.cluster * (int)items;
     if (part_floats < 2ll * blocks * a.rows_cap * (HD + 4)) return fail("attention_quantized: scratch of %lld numbers is too small", part_floats);

@@ -140,6 +140,19 @@ def test_write(runs, n_heads, n_kv, hd, v_hd, rot, style, dtype):
     _check_written(step, rows, before, q, n_heads=n_heads, rot=rot, style=style)
 
 
+@pytest.mark.parametrize("sequences", [80, 110])
+@pytest.mark.parametrize("n_heads, hd, dtype", [(30, 64, torch.bfloat16), (32, 128, torch.float32)])
+def test_write_of_many_sequences(sequences, n_heads, hd, dtype):
+    """More query heads than the SMs have warps for at once, one per warp; the last block of heads not full."""
+    runs = [((7 * i) % 45, 1 + (i % 9 == 0)) for i in range(sequences)]
+    step = Step(runs, 8, hd)
+    step.fill()
+    rows = torch.randn(step.n_tokens, (n_heads + 16) * hd, generator=torch.Generator().manual_seed(5)).to(dtype)
+    before = step.host()
+    q, _ = _write(step, rows, n_heads=n_heads, rot=hd, style=0)
+    _check_written(step, rows, before, q, n_heads=n_heads, rot=hd, style=0)
+
+
 @pytest.mark.parametrize("hd, q_dtype", [(64, torch.bfloat16), (128, torch.float32), (40, torch.bfloat16)])
 @pytest.mark.parametrize("runs", ["single", "prompts"])
 def test_write_from_sums_with_a_bias(runs, hd, q_dtype):
@@ -288,7 +301,8 @@ def test_attention(runs, n_heads, n_kv, hd, dtype, limits):
 
 @pytest.mark.parametrize("runs", sorted(ATTEND))
 @pytest.mark.parametrize("n_heads, n_kv, hd, dtype", [
-    (14, 2, 64, torch.float32), (7, 1, 128, torch.bfloat16), (16, 1, 128, torch.float32), (16, 1, 64, torch.bfloat16), (40, 2, 128, torch.bfloat16)])
+    (14, 2, 64, torch.float32), (7, 1, 128, torch.bfloat16), (16, 1, 128, torch.float32), (16, 1, 64, torch.bfloat16), (40, 2, 128, torch.bfloat16),
+    (7, 1, 64, torch.bfloat16), (4, 1, 128, torch.float32)])
 def test_attention_in_wide_tiles(runs, n_heads, n_kv, hd, dtype):
     """What the host knows of the lengths decides which tiles of rows a step is cut into, not what comes out: a step that might be long."""
     from rust_inference_b200.kernels import quantized_cache as qc

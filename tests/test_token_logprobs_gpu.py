@@ -15,8 +15,8 @@ def _ops():
     return ops
 
 
-def _check(x, targets, top):
-    got = _ops().token_logprobs(x, targets, top=top)
+def _check(x, targets, top, got=None):
+    got = _ops().token_logprobs(x, targets, top=top) if got is None else got
     rows, vocab = x.shape
     # the sum over the row in 32 bits: runs of at most vocab / 256 terms, then trees; exponentials and their arguments
     unit = (vocab / 256 + 32) * 2.0 ** -24
@@ -86,6 +86,16 @@ def test_rows_of_every_kind(vocab, dtype):
     _check(x, targets, 12)
     targets[:] = vocab
     assert _ops().token_logprobs(x, targets).logprob.isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, vocab, top", [(310, 35003, 5), (150, 50257, 3), (40, 100001, 5), (9, 70000, 0), (1, 151936, 20)])
+def test_rows_of_many_turns(rows, vocab, top, dtype):
+    """Rows that a block goes over in several turns, in clusters of several sizes, and more rows than the SMs hold two of."""
+    x, targets = _rows(rows, vocab, dtype, seed=6)
+    some = torch.randperm(rows, generator=torch.Generator().manual_seed(1))[:12].tolist()
+    found = _ops().token_logprobs(x, targets, top=top)
+    _check(x[some], targets[some], top, type(found)(*[None if f is None else f[some] for f in found]))
 
 
 def test_many_rows_and_no_rows():

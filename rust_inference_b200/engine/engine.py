@@ -235,7 +235,9 @@ class Engine:
             if decode and self.use_graphs and probe is None:
                 # one token per sequence, logits for each: the captured step of this batch size
                 dev, _, _ = self._stage(slots, tokens, wants)
-                logits = self._graph_for(len(slots)).run(dev)      # cleans up after itself if it raises
+                graph = self._graph_for(len(slots))
+                graph.expect(max(self.cache.lengths(slots)) + 1)
+                logits = graph.run(dev)                            # cleans up after itself if it raises
                 if not borrow:
                     logits = logits.clone()
             else:
@@ -300,6 +302,7 @@ class Engine:
             raise ValueError("step: a slot appears twice in one batch")
         starts = self.cache.lengths(slots)
         self.cache.reserve([(s, st + 1) for s, st in zip(slots, starts)])
+        graph.expect(max(starts) + 1)
         if graph.rows is not None:
             streams, counters = list(streams), list(counters)
         if graph.holds(slots, starts, streams, counters, seed):

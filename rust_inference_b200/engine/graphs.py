@@ -37,6 +37,7 @@ from .context import StepContext, Workspace, pack_step
 
 
 EAGER_STEPS = 2          # steps of a batch size that run on the engine's shared buffers before it gets its own
+FIRST_REACH = 1024       # keys that a captured step over a cache in 8 bits expects a sequence to have at most, to begin with
 MAX_SIZES = 8            # batch sizes (times sampler settings) an engine keeps graphs, or their beginnings, for
 HOST_RING = 4            # pinned buffers the sampled tokens of consecutive steps go to, in turn
 LOG_RING = 256           # steps whose tokens stay readable on the device (`DecodeGraph.log`)
@@ -63,6 +64,7 @@ class DecodeGraph:
         self.eager_steps = 0
         self.held = None              # [slots, lengths before the step, streams, draw counters] the static arrays describe now
         self.turn = 0                 # steps run: the host's copy of the device counter that picks the ring slots
+        self.reach = 0                # see `expect`
         self.rows = self.turn_dev = self.host_ring = self.log = self.seed_dev = None
         if sampler is not None:
             if sampler.uses_history:
@@ -114,6 +116,24 @@ class DecodeGraph:
             self.held = [list(slots), list(starts), list(streams) if streams is not None else None,
                          list(counters) if counters is not None else None, seed]
 
+    def expect(self, longest: int) -> None:
+        """The longest sequence has so many keys in the step to come.  Kernels of a cache in 8 bits choose their launches by that
+        number, as a bound that holds for a while: FIRST_REACH times a power of two.  When a sequence grows beyond it, the step is
+        captured again.  (Kernels of other caches depend on the cache's geometry only.)"""
+        if self.engine.cache.kv_dtype is None or longest <= self.reach:
+            return
+        self.reach = max(self.reach, FIRST_REACH)
+        while self.reach < longest:
+            self.reach *= 2
+        self.ctx.extras["longest"] = min(self.reach, self.engine.max_seq_len)
+        self._forget_steps()
+        self.graph = None
+
+    def _forget_steps(self) -> None:
+        """What kernels keep of the step (addresses of its scratch, their choices) is made again by the next one."""
+        for key in [k for k in self.ctx.extras if isinstance(k, tuple)]:
+            del self.ctx.extras[key]
+
     # ---- running ------------------------------------------------------------------------------
     def _step(self, logits: torch.Tensor) -> None:
         """The kernels of one step: the model, the sampler if the step holds one, the move to the next position."""
@@ -164,6 +184,7 @@ class DecodeGraph:
                 self.logits = torch.empty((self.n_seqs, self.engine.model.spec.vocab_size),
                                           dtype=torch.float32, device=self.engine.device)
                 self.ctx.workspace = self.workspace
+                self._forget_steps()
                 return self._eager(self.logits)
             torch.cuda.synchronize(self.engine.device)
             g = torch.cuda.CUDAGraph()

@@ -145,7 +145,7 @@ class _Step:
         arrived = ctx.zeroed_buffer("quantized_arrived", (ints,), torch.int32)
         self.native = (_index(what, table, 1), table.shape[1], _index(what, ctx.seq_slot, n_seqs), _index(what, ctx.seq_start, n_seqs),
                        _index(what, ctx.cu_seqlens, n_seqs + 1), n_seqs, ctx.max_new, n_heads, n_kv_heads, head_dim, part.data_ptr(), part.numel(),
-                       _index(what, arrived, ints), ctx.max_len)
+                       _index(what, arrived, ints), ctx.extras.get("longest", ctx.max_len))
         self.kept = (table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens, part, arrived)     # whose addresses these are
 
 

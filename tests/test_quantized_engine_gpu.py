@@ -80,6 +80,32 @@ def test_decoding_with_graphs_and_without(name, dtype, model_factory, monkeypatc
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_captured_step_that_is_outgrown(dtype, model_factory, monkeypatch):
+    """Captured steps choose their launches for sequences of so many keys, and are captured again when one has more: what comes out
+    stays what an engine without captured steps computes (bounds as above), before, at and after the change."""
+    from rust_inference_b200.engine import graphs
+    monkeypatch.setattr(graphs, "FIRST_REACH", 16)
+    model = model_factory("A", std=0.08)
+    toks = random_tokens(150, model.cfg["vocab_size"], seed=9)
+    engines = [_engine(model, dtype, use_graphs=g) for g in (True, False)]
+    out, reached = [], []
+    for eng in engines:
+        slot = eng.alloc_slot()
+        eng.step([slot], [toks[:5]], "none")
+        rows = []
+        for t in toks[5:]:
+            rows.append(eng.step([slot], [[t]], "last").cpu())
+            if eng.use_graphs:
+                reached.append(eng.decode_graph(1).reach)
+        out.append(torch.cat(rows))
+    assert reached[0] == 16 and reached[11] == 32 and reached[-1] == 256 and eng is not engines[0]
+    want = model.plain_logits(toks)
+    noise = rel_err(_plain_over_8_bits(model, toks, monkeypatch), want)
+    assert rel_err(out[0], out[1]) <= 2 * noise
+    assert rel_err(out[0], want[5:]) <= 3 * noise + (0 if dtype == "float32" else TOL[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_pages_that_were_used_before(dtype, model_factory):
     model = model_factory("A", std=0.08)
     toks = random_tokens(90, model.cfg["vocab_size"], seed=7)

@@ -51,7 +51,12 @@ constexpr int PAGE = 64, BLOCK = 16, WARPS = 4, THREADS = 32 * WARPS;
 constexpr int STEP = 2 * BLOCK;                  // keys that a warp takes at a time
 constexpr int MOST_BLOCKS = 5;                   // thread blocks per SM, at most
 // What an item costs a block beside its pages (queries fetched, warps joined, the result written), in pages
-constexpr int SETUP = 4;
+// (64 sequences of 128 to 2,048 keys, 32 heads over 8: 4 35.8 us, 8 35.3, 12 36.9; 1 of 30,000: 4 23.5, 8 22.7)
+constexpr int SETUP = 8;
+// Items go to blocks whole where there are no more of them than blocks and the longest has so many pages more at most than each block would
+// have of equal runs: what joining costs.  With equal runs and whole, us, 64 sequences, 32 heads over 8: 250 keys ONE_A, 1,024 ONE_B; 28 over 4:
+// 500 keys (8 pages for 3.5) ONE_C, 700 (11 for 4.8) 19.6 and 21.0.
+constexpr int JOINING = 5;
 // What a block has at least: the two pages of one turn, or as many turns as keep an item's parts to eight (64), which are added up in
 // one go (two): up to 4 pages (8).
 __device__ __forceinline__ int least_pages(int pages, int items) { return pages <= 16 * items ? 2 : (pages <= 256 * items ? 4 : 8); }
@@ -233,7 +238,7 @@ attn_quantized_kernel(const Args a) {
     static_assert(PART > 0 || ROWS * HD * 4 <= 2 * TILE, "a warp's sums fit where its values were");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int sums[THREADS + 1];
-    __shared__ int found[6], totals[WARPS][2];
+    __shared__ int found[6], totals[WARPS][3];
     __shared__ int last_here;
     __shared__ float4 sgroup[GROUP][ROWS];       // statistics of parts that are added up (a cluster's: each block's own first)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -241,26 +246,30 @@ attn_quantized_kernel(const Args a) {
 
     // ---- this block's run of units (lengths, slots and pages are fixed before the step) ----
     const int per = (a.n_seqs + THREADS - 1) / THREADS;
-    int mine = 0, mine_items = 0, slot = 0;
+    int mine = 0, mine_items = 0, longest = 0, slot = 0;
     for (int s = tid * per; s < min((tid + 1) * per, a.n_seqs); ++s) {
         const int n = a.cu_seqlens[s + 1] - a.cu_seqlens[s], start = a.seq_start[s];
-        const int each = a.n_kv * ((n * a.n_rep + ROWS - 1) / ROWS);
-        if (n > 0) mine += (pages_of(a, start, n) + SETUP) * each;
+        const int each = a.n_kv * ((n * a.n_rep + ROWS - 1) / ROWS), pages = n > 0 ? pages_of(a, start, n) : 0;
+        if (n > 0) mine += (pages + SETUP) * each;
         mine_items += each;
+        longest = max(longest, pages);
         slot = a.seq_slot[s];                    // (in the cache for when it is wanted)
     }
     const int me = blockIdx.x, C = a.cluster;
-    sums[tid + 1] = own ? mine_items : mine;
     if (tid == 0) sums[0] = 0;
     {
-        const int units = __reduce_add_sync(0xffffffffu, mine), n = __reduce_add_sync(0xffffffffu, mine_items);
-        if (lane == 0) totals[warp][0] = units, totals[warp][1] = n;
+        const int units = __reduce_add_sync(0xffffffffu, mine), n = __reduce_add_sync(0xffffffffu, mine_items), most = __reduce_max_sync(0xffffffffu, longest);
+        if (lane == 0) totals[warp][0] = units, totals[warp][1] = n, totals[warp][2] = most;
     }
     __syncthreads();
     int total = 0, items = 0;
+    longest = 0;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) total += totals[w][0], items += totals[w][1];
-    const int least = least_pages(total - SETUP * items, items), blocks = min((int)gridDim.x, (total + least - 1) / least);
+    for (int w = 0; w < WARPS; ++w) total += totals[w][0], items += totals[w][1], longest = max(longest, totals[w][2]);
+    const bool one = !own && items <= (int)gridDim.x && longest <= (total - SETUP * items) / (int)gridDim.x + JOINING;
+    const int least = least_pages(total - SETUP * items, items), blocks = one ? items : min((int)gridDim.x, (total + least - 1) / least);
+    sums[tid + 1] = own || one ? mine_items : mine;
+    __syncthreads();
     // a cluster's item is cut into equal runs of whole turns
     auto run_of = [&](int pages) { return max(2, ((pages + C - 1) / C + 1) & ~1); };
     auto leave = [&]() {                         // (who waits for this kernel waits for those before it too)
@@ -286,10 +295,10 @@ attn_quantized_kernel(const Args a) {
     // the first `more` runs have one unit more than `each`
     const int each = total / max(blocks, 1), more = total % max(blocks, 1);
     auto run_start = [&](int b) { return b * each + min(b, more); };
-    const int u0 = own ? me / C : run_start(me);
+    const int u0 = own ? me / C : (one ? me : run_start(me));
     if (sums[tid] <= u0 && u0 < sums[tid + 1]) {
         int at = sums[tid], s = tid * per, first_tok = a.cu_seqlens[s], n = a.cu_seqlens[s + 1] - first_tok, start = a.seq_start[s];
-        auto many = [&]() { return n > 0 ? (own ? 1 : pages_of(a, start, n) + SETUP) * a.n_kv * ((n * a.n_rep + ROWS - 1) / ROWS) : 0; };
+        auto many = [&]() { return n > 0 ? (own || one ? 1 : pages_of(a, start, n) + SETUP) * a.n_kv * ((n * a.n_rep + ROWS - 1) / ROWS) : 0; };
         for (int units; at + (units = many()) <= u0;) {
             at += units;
             ++s;
@@ -305,13 +314,16 @@ attn_quantized_kernel(const Args a) {
     enter(a, found[0], found[2], found[3], found[4], found[5], ROWS, it);
     int page, u, u1;                             // the next page, and its place among the units (its number, with a cluster); the run's end
     {
-        const int within = u0 - found[1], n = own ? 1 : it.end - it.low + SETUP, at = within % n;
+        const int within = u0 - found[1], n = own || one ? 1 : it.end - it.low + SETUP, at = within % n;
         it.tile = within / n % it.tiles;
         it.head = within / n / it.tiles;
         if (own) {
             const int run = run_of(it.end - it.low);
             u = page = it.low + me % C * run;
             u1 = min(it.end, page + run);
+        } else if (one) {
+            u = page = it.low;
+            u1 = it.end;
         } else {
             page = it.low + max(at - SETUP, 0);
             u = u0 + max(SETUP - at, 0);

@@ -126,8 +126,8 @@ def attention_workspace(n_heads: int, n_kv_heads: int, head_dim: int, max_new: i
 
 def attention_counts(n_seqs: int, pages: int, max_new: int, n_heads: int, n_kv_heads: int) -> bool:
     """Whether `attend_step`'s units (pages of a kv head, for 8 rows) of a step over up to so many pages per sequence are counted in 31
-    bits.  (An item counts as four pages more.)"""
-    return n_seqs * (pages + 4) * n_kv_heads * ((max_new * (n_heads // n_kv_heads) + 7) // 8) < 1 << 31
+    bits.  (An item counts as eight pages more.)"""
+    return n_seqs * (pages + 8) * n_kv_heads * ((max_new * (n_heads // n_kv_heads) + 7) // 8) < 1 << 31
 
 
 class _Step:

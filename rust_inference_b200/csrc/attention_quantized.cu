@@ -22,14 +22,14 @@
 //
 // The work.  A unit is one page (64 keys) of one kv head for a tile of 8 or 16 rows (row = token * n_rep + head of the kv head).
 // The units of a step, sequence by sequence, are cut into equal runs, one per thread block: however unequal the sequences are,
-// all blocks have the same to read.  A block's four warps take half of one of two pages each at a time, every warp with a ring of its
+// all blocks have the same to read (where that is not worth its joins, an item goes to a block whole).  A block's four warps take half of one of two pages each at a time, every warp with a ring of its
 // own that cp.async fills (no barrier inside a run).  An item (sequence, kv head, tile) that lies in one block is finished there;
 // one that spreads over several is written as partial sums, which the blocks that arrive last (a counter per eight parts) add up
 // in the order of the blocks, so that the result does not depend on who was last.  Where few items are short, each gets a cluster of
 // blocks instead, which add their parts up through distributed shared memory, a third of what meeting in memory takes.
 //
-// What it measures (32 heads over 8 of 128, bfloat16): 64 sequences of 128 to 2,048 keys 35.8 us, 4.1 TB/s of codes, 63% of what a copy
-// reaches; with the loads alone 31, without the joining of parts too 27.  2 sequences of about 30,000 keys (28 heads over 4) 24.4 us, of
+// What it measures (32 heads over 8 of 128, bfloat16): 64 sequences of 128 to 2,048 keys 35.2 us, 4.2 TB/s of codes, 64% of what a copy
+// reaches; with the loads alone 31, without the joining of parts too 27.  2 sequences of about 30,000 keys (28 heads over 4) 23.7 us, of
 // which 14 for the loads and 8 for the two rounds of joining.  1 sequence of 1,024 keys 5.6 us, 3 of them until the first keys are there.  A
 // scheduler issues in 46% of its cycles and the tensor cores are busy in 19%: what bounds the large steps is how many loads are in flight
 // beside four blocks' arithmetic per SM (a second buffer for keys 38.0 us instead of 36.4, as blocks are then fewer).
@@ -54,9 +54,9 @@ constexpr int MOST_BLOCKS = 5;                   // thread blocks per SM, at mos
 // (64 sequences of 128 to 2,048 keys, 32 heads over 8: 4 35.8 us, 8 35.3, 12 36.9; 1 of 30,000: 4 23.5, 8 22.7)
 constexpr int SETUP = 8;
 // Items go to blocks whole where there are no more of them than blocks and the longest has so many pages more at most than each block would
-// have of equal runs: what joining costs.  With equal runs and whole, us, 64 sequences, 32 heads over 8: 250 keys ONE_A, 1,024 ONE_B; 28 over 4:
-// 500 keys (8 pages for 3.5) ONE_C, 700 (11 for 4.8) 19.6 and 21.0.
-constexpr int JOINING = 5;
+// have of equal runs: what joining costs.  Equal runs and whole items, us, 64 sequences, 32 heads over 8: 250 keys 17.8 and 11.6, 1,024 33.4
+// and 29.6; 28 over 4: 500 keys (8 pages for 3.5) 17.9 and 14.5, 700 (11 for 4.8) 19.6 and 18.0, 1,024 (16 for 6.9) 22.6 and 22.9.
+constexpr int JOINING = 8;
 // What a block has at least: the two pages of one turn, or as many turns as keep an item's parts to eight (64), which are added up in
 // one go (two): up to 4 pages (8).
 __device__ __forceinline__ int least_pages(int pages, int items) { return pages <= 16 * items ? 2 : (pages <= 256 * items ? 4 : 8); }

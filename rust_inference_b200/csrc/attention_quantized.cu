@@ -9,9 +9,11 @@
 //     two signed bytes, q = 256 d1 + d0 (float32: +-127 65536, three bytes), 2^-16 (2^-24) of the row's largest
 //     number; codes times bytes add up in 32 bits without a rounding.  The codes are operands as they lie in memory;
 //   - results are sums of weights in float16 (m16n8k16, float32 sums; for float32 two float16 numbers each, the second what
-//     the first left over) times codes.  A weight times t_j over the largest t so far of the warp is rounded to 2^-12 (2^-23)
-//     relative, down to 2^-20 of the largest; the sums run in units of that t, and when a larger one comes, they are brought to
-//     it as they are to a new maximum.  A code c becomes float16 by its bits: 1024 + 128 + c has the byte c + 128 as its low one.
+//     the first left over) times codes.  A row has two references, both whole numbers so that bringing sums to a new one is
+//     exact: m, which its scores are measured from and the sum of its weights runs in, and r, the same for score_j log2 e + log2 t_j,
+//     which the products of weights and codes run in (out = 2^(r - m) times their quotient).  So w_j t_j is rounded to 2^-11 (2^-22)
+//     relative, and no finer than 2^-30 of the row's own largest such product, whatever the values of
+//     keys that the row does not see, or gives no weight to.  A code c becomes float16 by its bits: 1024 + 128 + c has the byte c + 128 as its low one.
 //     With one number per weight the products are taken of 1152 + c, one byte permutation for two codes, and a product of the same
 //     weights with -1152 follows each of them (float32 sums of that size are off by 2^-23 1152 = 1.4e-4 of a code); with two numbers
 //     1152 is taken off the codes.
@@ -40,6 +42,7 @@
 #include "cluster.cuh"
 
 #include <cuda_fp16.h>
+#include <float.h>
 
 #include <algorithm>
 
@@ -63,9 +66,12 @@ __device__ __forceinline__ int least_pages(int pages, int items) { return pages 
 // Parts of an item are added up eight at a time: a block that arrives last of eight adds theirs and goes on with seven others
 constexpr int GROUP = 8;
 // Weights are formed times 2^6 against a reference that follows the row's maximum only when that is 2^8 times ahead: they stay below
-// 2^14, which float16 holds, and sums are brought to a new reference a few times per row instead of at most steps.
+// 2^14, which float16 holds, and sums are brought to a new reference a few times per row instead of at most steps.  Weights times their
+// values' scales likewise.
 constexpr float BIAS = 6.f, AHEAD = 8.f;
-constexpr float LOWEST = -1.7e38f;               // the reference of a row without keys
+constexpr float LOWEST = -1.7e38f;               // the references of a row without keys
+// ... of products whose values are all zeros, or below 2^-120: so far below the weights' reference (results of such a size are rounded to 2^-149)
+constexpr float BELOW = 126.f;
 
 struct Args {
     const void* q;
@@ -81,7 +87,7 @@ struct Args {
     int span;
     float out_scale;
     float* part;                                 // [2 * blocks][rows_cap][HD]
-    float4* stat;                                // [2 * blocks][rows_cap]: maximum, sum, unit of the sums
+    float4* stat;                                // [2 * blocks][rows_cap]: the weights' reference, their sum, the products' reference
     int* arrived;                                // [4][2 * blocks] (8^4 parts are more than there are blocks), zero between calls
     int places;                                  // 2 * blocks
     int cluster;                                 // blocks of a cluster, one for every item; 1: runs of units
@@ -163,6 +169,14 @@ __device__ __forceinline__ float two_to(float x) {
     return y;
 }
 
+// ... of whole numbers up to 127, exactly (what it leaves of a sum that far below another is nothing)
+__device__ __forceinline__ float power(float x) { return x < -126.f ? 0.f : __int_as_float(((int)x + 127) << 23); }
+__device__ __forceinline__ float log2_of(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // the same of whole numbers, 32 terms
 __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -214,10 +228,6 @@ template <> __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16*
         p[0] = a.x, p[1] = a.y, p[2] = b.x, p[3] = b.y;
     }
 }
-
-// What several partial results of a row are weighted with: maxima m, sums l, units s of their values
-__device__ __forceinline__ float merge_weight(float m, float top) { return two_to(m - top); }
-__device__ __forceinline__ float unit_ratio(float s, float most) { return s == most ? 1.f : s / most; }      // (both 0: 1; s NaN never is the unit)
 
 template <int HD> constexpr int OWN_BYTES = 2 * STEP * HD + 16;         // a warp's keys, values, two scales of each
 // ... and what it sums up: in the place of its last values (8 rows), or beside them
@@ -394,8 +404,8 @@ attn_quantized_kernel(const Args a) {
     // a warp's sums [WARPS][ROWS][HD] and their rows' statistics [WARPS][ROWS]
     auto part_at = [&](int w) { return reinterpret_cast<float*>(smem + (PART ? WARPS * OWN + w * PART : w * OWN + 2 * TILE)); };
     float4* sml = reinterpret_cast<float4*>(smem + WARPS * (OWN + PART));
-    auto write = [&](const Item& i, int row, int d, float4 v, float sum, float s) {
-        const float inv = 1.f / sum, f = s * a.out_scale;
+    auto write = [&](const Item& i, int row, int d, float4 v, float sum, float m, float r) {
+        const float inv = 1.f / sum, f = power(r - m) * a.out_scale;
         v = make_float4(v.x * inv * f, v.y * inv * f, v.z * inv * f, v.w * inv * f);
         store4<T>(reinterpret_cast<T*>(a.out) + (size_t)(i.first_tok + row / a.n_rep) * a.out_ld + (size_t)(i.head * a.n_rep + row % a.n_rep) * HD + d,
                   a.out_vec, v);
@@ -462,10 +472,11 @@ attn_quantized_kernel(const Args a) {
             }
         }
 
-        float o[NQ][CT][4], m[NQ][2], l[NQ][2], most = 0.f, inverse = 0.f;
+        float o[NQ][CT][4], m[NQ][2], r[NQ][2], from_m[NQ][2], l[NQ][2];      // from_m: 2^(m - r)
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            m[n][0] = m[n][1] = LOWEST;
+            m[n][0] = m[n][1] = r[n][0] = r[n][1] = LOWEST;
+            from_m[n][0] = from_m[n][1] = 1.f;
             l[n][0] = l[n][1] = 0.f;
 #pragma unroll
             for (int i = 0; i < CT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
@@ -529,47 +540,40 @@ attn_quantized_kernel(const Args a) {
                             if (!(key <= pos[n][x & 1] && key >= low[n][x & 1])) s[j][n][x] = -INFINITY;
                         }
             }
-            // whether the rows' references are far behind
-            bool ahead_of[NQ];
-            float top[NQ][2];
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                ahead_of[n] = false;
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    top[n][r] = fmaxf(fmaxf(s[0][n][r], s[0][n][2 + r]), fmaxf(s[1][n][r], s[1][n][2 + r]));
-                    ahead_of[n] |= top[n][r] > m[n][r] + AHEAD;
-                }
-            }
             copies_wait<1>();
             __syncwarp();                        // the values are there
-            // a larger unit for the sums (of this warp: all lanes alike); a block that no row sees has no say
+            // (a block that no row sees has no say)
             const float v0 = edge && !(base <= last_pos && base + BLOCK > first_key) ? 0.f : scales[2];
             const float v1 = edge && !(base + BLOCK <= last_pos && base + STEP > first_key) ? 0.f : scales[3];
-            float shrink = 1.f;
-            if (fmaxf(v0, v1) > most) {
-                const float higher = fmaxf(v0, v1);
-                inverse = 1.f / higher;
-                shrink = most * inverse;
-                most = higher;
-            }
-            const float ratio[2] = {v0 == most ? 1.f : v0 * inverse, v1 == most ? 1.f : v1 * inverse};
+            const float log_v0 = log2_of(v0), log_v1 = log2_of(v1);          // a scale that is no number moves no reference
             uint32_t pb[2][TERMS][NQ][2];
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                if (__any_sync(0xffffffffu, ahead_of[n] || shrink != 1.f)) {
+                // whether the rows' references are far behind
+                float top[2], product[2];
+                bool behind = false;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const float top0 = fmaxf(s[0][n][x], s[0][n][2 + x]), top1 = fmaxf(s[1][n][x], s[1][n][2 + x]);
+                    top[x] = fmaxf(top0, top1);
+                    product[x] = fmaxf(top0 + log_v0, top1 + log_v1);
+                    behind |= top[x] > m[n][x] + AHEAD || product[x] > r[n][x] + AHEAD;
+                }
+                if (__any_sync(0xffffffffu, behind)) {
                     float alpha[2];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float& most_of = top[n][r];
-                        most_of = fmaxf(most_of, __shfl_xor_sync(0xffffffffu, most_of, 4));
-                        most_of = fmaxf(most_of, __shfl_xor_sync(0xffffffffu, most_of, 8));
-                        most_of = fmaxf(most_of, __shfl_xor_sync(0xffffffffu, most_of, 16));
-                        const float m_new = fmaxf(m[n][r], most_of);
-                        alpha[r] = two_to(m[n][r] - m_new);
-                        m[n][r] = m_new;
-                        l[n][r] *= alpha[r];
-                        alpha[r] *= shrink;
+                    for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                        for (int lanes = 4; lanes < 32; lanes <<= 1) {
+                            top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], lanes));
+                            product[x] = fmaxf(product[x], __shfl_xor_sync(0xffffffffu, product[x], lanes));
+                        }
+                        const float m_new = fmaxf(m[n][x], ceilf(top[x])), r_new = fmaxf(fmaxf(r[n][x], ceilf(product[x])), m_new - BELOW);
+                        l[n][x] *= power(m[n][x] - m_new);
+                        alpha[x] = power(r[n][x] - r_new);
+                        m[n][x] = m_new;
+                        r[n][x] = r_new;
+                        from_m[n][x] = power(m_new - r_new);
                     }
 #pragma unroll
                     for (int i = 0; i < CT; ++i) {
@@ -583,11 +587,13 @@ attn_quantized_kernel(const Args a) {
                 for (int j = 0; j < 2; ++j) {
                     float y[4];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const float ref = m[n][r] - BIAS, p0 = two_to(s[j][n][r] - ref), p1 = two_to(s[j][n][2 + r] - ref);
-                        l[n][r] += p0 + p1;
-                        y[r] = p0 * ratio[j];    // weights in units of `most`
-                        y[2 + r] = p1 * ratio[j];
+                    for (int x = 0; x < 2; ++x) {
+                        const float ref = m[n][x] - BIAS, p0 = two_to(s[j][n][x] - ref), p1 = two_to(s[j][n][2 + x] - ref);
+                        l[n][x] += p0 + p1;
+                        float f = from_m[n][x] * (j ? v1 : v0);
+                        f = f > FLT_MAX ? FLT_MAX : f;       // (beside weights of 0)
+                        y[x] = p0 * f;
+                        y[2 + x] = p1 * f;
                     }
                     if (edge) {                  // an unseen key's weight is 0 also beside a scale that is no number
 #pragma unroll
@@ -645,18 +651,18 @@ attn_quantized_kernel(const Args a) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float sum = l[n][r];
+            for (int x = 0; x < 2; ++x) {
+                float sum = l[n][x];
                 sum += __shfl_xor_sync(0xffffffffu, sum, 4);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-                const int row = 8 * n + 2 * t + r;
-                if (g == 0) sml[warp * ROWS + row] = make_float4(m[n][r], sum, most, 0.f);
+                const int row = 8 * n + 2 * t + x;
+                if (g == 0) sml[warp * ROWS + row] = make_float4(m[n][x], sum, r[n][x], 0.f);
                 if (row < here) {
                     float* to = part_at(warp) + row * HD + g * (HD / 8);
 #pragma unroll
                     for (int i = 0; i < CT; i += 2)
-                        *reinterpret_cast<float4*>(to + 2 * i) = make_float4(o[n][i][r], o[n][i][2 + r], o[n][i + 1][r], o[n][i + 1][2 + r]);
+                        *reinterpret_cast<float4*>(to + 2 * i) = make_float4(o[n][i][x], o[n][i][2 + x], o[n][i + 1][x], o[n][i + 1][2 + x]);
                 }
             }
         __syncthreads();
@@ -667,30 +673,30 @@ attn_quantized_kernel(const Args a) {
         auto place_of = [&](int part) { return part == 0 ? first_place : 2 * (first_block + part); };
         for (int i = tid; i < here * (HD / 4); i += THREADS) {
             const int row = i / (HD / 4), d = i % (HD / 4) * 4;
-            float top = LOWEST, s = 0.f, sum = 0.f;
+            float top = LOWEST, high = LOWEST, sum = 0.f;
             float4 st[WARPS], v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
                 st[w] = sml[w * ROWS + row];
                 top = fmaxf(top, st[w].x);
-                s = fmaxf(s, st[w].z);
+                high = fmaxf(high, st[w].z);
             }
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
-                const float f = merge_weight(st[w].x, top), x = f * unit_ratio(st[w].z, s);
+                const float f = power(st[w].x - top), x = power(st[w].z - high);
                 const float4 p = *reinterpret_cast<const float4*>(part_at(w) + row * HD + d);
                 sum = fmaf(st[w].y, f, sum);
                 v = make_float4(fmaf(p.x, x, v.x), fmaf(p.y, x, v.y), fmaf(p.z, x, v.z), fmaf(p.w, x, v.w));
             }
             if (whole) {
-                write(it, row0 + row, d, v, sum, s);
+                write(it, row0 + row, d, v, sum, top, high);
             } else if (own) {
                 *reinterpret_cast<float4*>(reinterpret_cast<float*>(smem) + row * HD + d) = v;       // where the first warp's keys were
-                if (d == 0) sgroup[0][row] = make_float4(top, sum, s, 0.f);
+                if (d == 0) sgroup[0][row] = make_float4(top, sum, high, 0.f);
             } else {
                 const size_t at = (size_t)place_of(me - first_block) * a.rows_cap + row;
                 *reinterpret_cast<float4*>(a.part + at * HD + d) = v;
-                if (d == 0) a.stat[at] = make_float4(top, sum, s, 0.f);
+                if (d == 0) a.stat[at] = make_float4(top, sum, high, 0.f);
             }
         }
         if (!own && !whole) {
@@ -723,21 +729,20 @@ attn_quantized_kernel(const Args a) {
                     }
                 };
                 // the parts' statistics, one per thread; what each part is weighted with, and the row's own
-                float4 st = make_float4(LOWEST, 0.f, 0.f, 0.f);
+                float4 st = make_float4(LOWEST, 0.f, LOWEST, 0.f);
                 if (tid < GROUP * ROWS && tid / ROWS < members && tid % ROWS < here)
                     st = __ldcg(a.stat + (size_t)place_of((lead + tid / ROWS) * stride) * a.rows_cap + tid % ROWS);
                 read(tid);
                 if (tid < GROUP * ROWS) sgroup[tid / ROWS][tid % ROWS] = st;
                 __syncthreads();
                 if (tid < here) {
-                    float top = LOWEST, s = 0.f, sum = 0.f;
-                    for (int x = 0; x < members; ++x) top = fmaxf(top, sgroup[x][tid].x), s = fmaxf(s, sgroup[x][tid].z);
+                    float top = LOWEST, high = LOWEST, sum = 0.f;
+                    for (int x = 0; x < members; ++x) top = fmaxf(top, sgroup[x][tid].x), high = fmaxf(high, sgroup[x][tid].z);
                     for (int x = 0; x < members; ++x) {
-                        const float f = merge_weight(sgroup[x][tid].x, top);
-                        sum = fmaf(sgroup[x][tid].y, f, sum);
-                        sgroup[x][tid].w = f * unit_ratio(sgroup[x][tid].z, s);
+                        sum = fmaf(sgroup[x][tid].y, power(sgroup[x][tid].x - top), sum);
+                        sgroup[x][tid].w = power(sgroup[x][tid].z - high);
                     }
-                    sml[tid] = make_float4(top, sum, s, 0.f);
+                    sml[tid] = make_float4(top, sum, high, 0.f);
                 }
                 __syncthreads();
                 for (int i0 = tid; i0 < here * (HD / 4); i0 += TWO * THREADS) {
@@ -752,7 +757,7 @@ attn_quantized_kernel(const Args a) {
                             const float w = x < members ? sgroup[x][row].w : 0.f;
                             v = make_float4(fmaf(p[z][x].x, w, v.x), fmaf(p[z][x].y, w, v.y), fmaf(p[z][x].z, w, v.z), fmaf(p[z][x].w, w, v.w));
                         }
-                        if (done) write(it, row0 + row, d, v, sml[row].y, sml[row].z);
+                        if (done) write(it, row0 + row, d, v, sml[row].y, sml[row].x, sml[row].z);
                         // in the place of the first (its channels are this thread's; its statistics have been read)
                         else *reinterpret_cast<float4*>(a.part + ((size_t)place_of(lead * stride) * a.rows_cap + row) * HD + d) = v;
                     }
@@ -777,19 +782,19 @@ attn_quantized_kernel(const Args a) {
     const int run = run_of(it.end - it.low), parts = (it.end - it.low + run - 1) / run, row0 = it.tile * ROWS, here = min(ROWS, it.n_rows - row0);
     for (int row = me % C + parts * warp; parts > 1 && row < here; row += parts * WARPS) {
         const int x8 = lane & 7;
-        float4 st = make_float4(LOWEST, 0.f, 0.f, 0.f), v = make_float4(0.f, 0.f, 0.f, 0.f), p[8];
+        float4 st = make_float4(LOWEST, 0.f, LOWEST, 0.f), v = make_float4(0.f, 0.f, 0.f, 0.f), p[8];
         if (x8 < parts) st = peer_float4(reinterpret_cast<const float*>(&sgroup[0][row]), x8);
 #pragma unroll
         for (int x = 0; x < 8; ++x)
             p[x] = x < parts && 4 * lane < HD ? peer_float4(reinterpret_cast<const float*>(smem) + row * HD + 4 * lane, x) : make_float4(0.f, 0.f, 0.f, 0.f);
-        float top = st.x, s = st.z;
+        float top = st.x, high = st.z;
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
+            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
         }
-        const float f = merge_weight(st.x, top), w = f * unit_ratio(st.z, s);
-        float sum = st.y * f;
+        const float w = power(st.z - high);
+        float sum = st.y * power(st.x - top);
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
 #pragma unroll
@@ -797,7 +802,7 @@ attn_quantized_kernel(const Args a) {
             const float z = __shfl_sync(0xffffffffu, w, x);
             v = make_float4(fmaf(p[x].x, z, v.x), fmaf(p[x].y, z, v.y), fmaf(p[x].z, z, v.z), fmaf(p[x].w, z, v.w));
         }
-        if (4 * lane < HD) write(it, row0 + row, 4 * lane, v, sum, s);
+        if (4 * lane < HD) write(it, row0 + row, 4 * lane, v, sum, top, high);
     }
     cluster_sync();                              // a peer may still be reading this block's part
 }

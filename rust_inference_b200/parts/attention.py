@@ -13,6 +13,17 @@ from .rope import RotaryEncoding
 from .spec import TensorSpec, PartSpec
 
 
+def _quantizes(position) -> bool:
+    """Whether a position encoding has a way into a cache in 8 bits that is as much its own as its way into another: a class that
+    changes what it does to heads, and does not say what that is here, is not passed by."""
+    places = [vars(position)] + [vars(c) for c in type(position).__mro__]
+
+    def place(name):
+        return next((i for i, names in enumerate(places) if name in names), len(places))
+
+    return place("apply_and_quantize") <= min(place("apply_and_store"), place("apply_and_store_from_accumulators"), len(places) - 1)
+
+
 @register("mixer", "gqa_attention")
 class GQAttention(Mixer):
     """q, k, v projections with optional biases (attention.rs:66-76), the position encoding
@@ -235,9 +246,10 @@ class GQAttention(Mixer):
 
     @property
     def quantizable(self) -> bool:
-        """Whether the layer can keep its keys and values in 8 bits: they go into the cache as projected, and rotated."""
+        """Whether the layer can keep its keys and values in 8 bits: they go into the cache as projected, and as the position
+        encoding turns them."""
         return (self.conv is None and self.value_mix is None and not self.values_from_keys and self.qk_norm_eps is None
-                and hasattr(self.position, "apply_and_quantize") and self.head_dim % 2 == 0 and self.v_head_dim % 2 == 0)
+                and _quantizes(self.position) and self.head_dim % 2 == 0 and self.v_head_dim % 2 == 0)
 
     def prepare(self, max_positions):
         self.position.prepare(max_positions)

@@ -126,13 +126,7 @@ class DecodeGraph:
         while self.reach < longest:
             self.reach *= 2
         self.ctx.extras["longest"] = min(self.reach, self.engine.max_seq_len)
-        self._forget_steps()
         self.graph = None
-
-    def _forget_steps(self) -> None:
-        """What kernels keep of the step (addresses of its scratch, their choices) is made again by the next one."""
-        for key in [k for k in self.ctx.extras if isinstance(k, tuple)]:
-            del self.ctx.extras[key]
 
     # ---- running ------------------------------------------------------------------------------
     def _step(self, logits: torch.Tensor) -> None:
@@ -184,7 +178,6 @@ class DecodeGraph:
                 self.logits = torch.empty((self.n_seqs, self.engine.model.spec.vocab_size),
                                           dtype=torch.float32, device=self.engine.device)
                 self.ctx.workspace = self.workspace
-                self._forget_steps()
                 return self._eager(self.logits)
             torch.cuda.synchronize(self.engine.device)
             g = torch.cuda.CUDAGraph()

@@ -253,13 +253,8 @@ CODES_TOKENS, CODES_ROWS = 16, 2048
 
 def reads_codes(ctx, f32: bool, n_heads: int, n_kv_heads: int) -> bool:
     """Whether a step with the plain form of the score reads a cache in 8 bits directly."""
-    key = ("reads_codes", f32, n_heads, n_kv_heads)
-    answer = ctx.extras.get(key)
-    if answer is None:
-        few = ctx.max_new <= CODES_TOKENS or ctx.n_seqs * ctx.max_new * n_heads <= CODES_ROWS
-        answer = (f32 or few) and quantized_cache.attention_counts(ctx.n_seqs, ctx.page_table.shape[1], ctx.max_new, n_heads, n_kv_heads)
-        ctx.extras[key] = answer
-    return answer
+    few = ctx.max_new <= CODES_TOKENS or ctx.n_seqs * ctx.max_new * n_heads <= CODES_ROWS
+    return (f32 or few) and quantized_cache.attention_counts(ctx.n_seqs, ctx.page_table.shape[1], ctx.max_new, n_heads, n_kv_heads)
 
 
 def _over_quantized(qkv, layer, out, ctx, *, window, chunk, keep_first, **forms):

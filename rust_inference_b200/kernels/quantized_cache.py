@@ -133,27 +133,40 @@ def attention_counts(n_seqs: int, pages: int, max_new: int, n_heads: int, n_kv_h
 class _Step:
     """What the calls of a step have in common: its arrays' addresses and sizes, looked at once."""
 
-    __slots__ = ("native", "kept")
+    __slots__ = ("native", "kept", "max_new", "longest")
 
     def __init__(self, ctx, n_heads, n_kv_heads, head_dim):
         what = "quantized_cache.attend_step"
         table, n_seqs = ctx.page_table, ctx.seq_slot.numel()
         _need(n_kv_heads > 0 and n_heads % n_kv_heads == 0 and head_dim in (64, 128) and table.dim() == 2, what,
               f"{n_heads} heads of {head_dim} over {n_kv_heads}, or a page table that is not [slots, pages]")
+        self.max_new, self.longest = ctx.max_new, _longest(ctx)
         floats, ints = attention_workspace(n_heads, n_kv_heads, head_dim, ctx.max_new)
         part = ctx.buffer("quantized_part", (floats,), torch.float32)
         arrived = ctx.zeroed_buffer("quantized_arrived", (ints,), torch.int32)
         self.native = (_index(what, table, 1), table.shape[1], _index(what, ctx.seq_slot, n_seqs), _index(what, ctx.seq_start, n_seqs),
                        _index(what, ctx.cu_seqlens, n_seqs + 1), n_seqs, ctx.max_new, n_heads, n_kv_heads, head_dim, part.data_ptr(), part.numel(),
-                       _index(what, arrived, ints), ctx.extras.get("longest", ctx.max_len))
-        self.kept = (table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens, part, arrived)     # whose addresses these are
+                       _index(what, arrived, ints), self.longest)
+        self.kept = (table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens, ctx.workspace, part, arrived)     # whose addresses these are
+
+    def stands(self, ctx) -> bool:
+        """Whether the step still has the arrays, the scratch and the sizes that were looked at."""
+        kept = self.kept
+        return (kept[2] is ctx.seq_start and kept[3] is ctx.cu_seqlens and kept[1] is ctx.seq_slot and kept[0] is ctx.page_table
+                and kept[4] is ctx.workspace and self.max_new == ctx.max_new and self.longest == _longest(ctx))
+
+
+def _longest(ctx) -> int:
+    """The keys of the step's longest sequence, as far as the host knows them (a captured step has a bound of its own)."""
+    return ctx.extras.get("longest", ctx.max_len)
 
 
 def step_of(ctx, n_heads: int, n_kv_heads: int, head_dim: int) -> _Step:
-    """`attend_step`'s view of a step (`engine.context.StepContext`), made by the first layer that asks."""
+    """`attend_step`'s view of a step (`engine.context.StepContext`), made by the first layer that asks, and again if the step has
+    been given other arrays, scratch or sizes since."""
     key = ("quantized", n_heads, n_kv_heads, head_dim)
     step = ctx.extras.get(key)
-    if step is None:
+    if step is None or not step.stands(ctx):
         step = ctx.extras[key] = _Step(ctx, n_heads, n_kv_heads, head_dim)
     return step
 

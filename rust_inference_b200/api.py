@@ -63,10 +63,13 @@ class Model:
     def memory(self) -> dict:
         """Bytes the model holds on the device and what a decode step has to read of them: the weights
         (every declared tensor once), the weights a step reads (the embedding table only when it is also
-        the head), the cache as allocated, and the cache bytes one position of one sequence adds."""
+        the head), the cache as allocated, the cache bytes one position of one sequence adds and, over a cache in
+        8 bits, the most that a step may add for keys and values of a layer that it brings to another type
+        (`kernels.attention.scratch_pages`: for prompts the pages of their positions)."""
         eng = self.engine
         item = 4 if eng.dtype.itemsize == 4 else 2
-        per_position = 0
+        per_position = scratch = 0
+
         def flat(entry):
             if isinstance(entry, tuple):
                 for sub in entry:
@@ -82,8 +85,10 @@ class Model:
                         per_position += req.n_kv_heads * (req.head_dim + values) * item
                     else:                        # a byte per number, and a block's two scales shared by its positions
                         per_position += req.n_kv_heads * (req.head_dim + values + 2 * 4 / 16)
+                        scratch = max(scratch, eng.cache.n_pages * eng.cache.page_size * req.n_kv_heads * (req.head_dim + values) * item)
         return {"weight_bytes": eng.model.weight_bytes(), "weight_bytes_per_step": eng.model.weight_bytes(False),
-                "cache_bytes": eng.cache.bytes(), "cache_bytes_per_position": int(per_position)}
+                "cache_bytes": eng.cache.bytes(), "cache_bytes_per_position": int(per_position),
+                "cache_scratch_bytes": scratch}
 
     def state_dict(self) -> dict:
         """name -> tensor for every tensor of the model, under the weight file's names, as held on the

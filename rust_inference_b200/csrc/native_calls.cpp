@@ -155,13 +155,13 @@ PyObject* py_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---- quantized_cache.read ------------------------------------------------------------------------------------------------
-// (layer, k_out, v_out, page_table, seq_slot, seq_first, seq_len, max_len, cu_rows or None, pages, seen, span); pages: the layer's
+// (layer, k_out, v_out, page_table, seq_slot, seq_first, seq_len, max_len, cu_rows or None, pages, seen, span, out_pages); pages: the layer's
 typedef int ReadFn(const int8_t*, const int8_t*, const float*, const float*, void*, void*, int, const int*, int, const int*, const int*, const int*,
-                   const int*, int, int, int, int, int, int, int, void*);
+                   const int*, int, int, int, int, int, int, int, int, void*);
 PyObject* py_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const char* what = "quantized_cache.read";
-        need(n == 12, "quantized_cache.read: 12 arguments");
+        need(n == 13, "quantized_cache.read: 13 arguments");
         PyObject* layer = a[0];
         const long long kv = item(layer, 4), hd = item(layer, 5), v_hd = item(layer, 6), pages = number(a[9]);
         const at::Tensor &k = tensor(a[1], what), &v = tensor(a[2], what), &table = tensor(a[3], what);
@@ -172,9 +172,10 @@ PyObject* py_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const long long seqs = tensor(a[4], what).numel();
         const int* rows = nullptr;
         if (a[8] == Py_None) {
-            const int64_t ks[4] = {pages, kv, 64, hd}, vs[4] = {pages, kv, 64, v_hd};
+            const long long own = number(a[12]), out_pages = own > 0 ? seqs * own : pages;
+            const int64_t ks[4] = {out_pages, kv, 64, hd}, vs[4] = {out_pages, kv, 64, v_hd};
             need(k.sizes() == at::IntArrayRef(ks, 4) && v.sizes() == at::IntArrayRef(vs, 4),
-                 "quantized_cache.read: without cu_rows the outputs have the cache's shape");
+                 "quantized_cache.read: without cu_rows the outputs have the cache's shape, or so many pages for each sequence");
         } else {
             need(k.dim() == 3 && v.dim() == 3 && k.size(1) == kv && k.size(2) == hd && v.size(0) == k.size(0) && v.size(1) == kv && v.size(2) == v_hd,
                  "quantized_cache.read: with cu_rows the outputs are [rows, kv heads, head size]");
@@ -183,7 +184,7 @@ PyObject* py_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
         finish(entry<ReadFn>(READ)(address<int8_t>(item(layer, 0)), address<int8_t>(item(layer, 1)), address<float>(item(layer, 2)),
                                    address<float>(item(layer, 3)), k.data_ptr(), v.data_ptr(), code, index(a[3], 1, what), small(table.size(1)),
                                    index(a[4], seqs, what), index(a[5], seqs, what), index(a[6], seqs, what), rows, small(seqs), small(number(a[7])),
-                                   small(kv), small(hd), small(v_hd), small(number(a[10])), small(number(a[11])), stream()),
+                                   small(kv), small(hd), small(v_hd), small(number(a[10])), small(number(a[11])), small(number(a[12])), stream()),
                READ, what);
         Py_RETURN_NONE;
     });

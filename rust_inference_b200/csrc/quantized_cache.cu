@@ -498,8 +498,10 @@ __global__ void __launch_bounds__(32 * ONE_WARPS) write_one_kernel(Written w) {
 }
 
 // Reading back: a block of threads takes a page of one kv head, keys and values, as many codes per thread and turn as make sixteen
-// bytes of values (a warp then writes whole sectors).  What bounds it is memory: 31,999 positions of 8 heads of 128 to bfloat16 36.2 us,
-// 5.4 TB/s, 83% of what a copy reaches.
+// bytes of values (a warp then writes whole sectors).  What bounds it is memory: 31,999 positions of 8 heads of 128 to bfloat16 36.8 us,
+// 5.4 TB/s, 82% of what a copy reaches.  (Registers for 6 blocks per SM in bfloat16 and 7 in float32: with 8 in bfloat16 seven prompts of up
+// to 2,047 tokens take 21.5 us with their writing instead of 20.7; with 6 in float32 8 sequences of 500 to 4,000 41.9 instead of 41.0.)
+// ROWS: to rows of a sequence's own (cu_rows); else to pages.
 constexpr int READERS = 256;
 struct Read {
     const int8_t *kc, *vc;
@@ -507,13 +509,15 @@ struct Read {
     void *k_out, *v_out;
     const int *page_table, *seq_slot, *seq_first, *seq_len, *cu_rows;   // cu_rows null: out has the cache's pages
     int max_pages, n_kv, hd, v_hd, pages;                              // pages: of a sequence, at most
+    int out_pages;                                                     // 0: a page goes where it lies; else sequence b's i-th to b * out_pages + i
     int seen, span;                                                    // seen: from the first key that position seq_first sees (span)
 };
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool ROWS>
 __device__ __forceinline__ void read_tile(const Read& r, const int8_t* codes, const float* scales, T* out, int size, int head, int page,
-                                          int base, int first, int len, int seq) {
+                                          int out_page, int base, int first, int len, int row_of_0) {
     const size_t tile = (size_t)page * r.n_kv + head;
+    T* const own = out + ((size_t)out_page * r.n_kv + head) * PAGE * size;             // (pages)
     codes += tile * PAGE * size;
     scales += tile * PER_PAGE;
     constexpr int PER = VEC ? 16 / sizeof(T) : 1, AT_ONCE = VEC ? 4 : 1;             // codes that make sixteen bytes of values; pieces at once
@@ -532,13 +536,10 @@ __device__ __forceinline__ void read_tile(const Read& r, const int8_t* codes, co
             const int e = e0 + k * READERS * PER;
             if (e >= PAGE * size) break;
             const int row = e / size, d = e % size, pos = base + row;
-            T* to = out + tile * PAGE * size + e;
-            if (r.cu_rows != nullptr) {
-                if (pos < first || pos >= len) continue;
-                to = out + ((size_t)(r.cu_rows[seq] + pos - first) * r.n_kv + head) * size + d;
-            }
-            const float s = scales[row / BLOCK];
             const bool there = pos >= first && pos < len;    // the rest of a page reads as zeros
+            if (ROWS && !there) continue;
+            T* const to = ROWS ? out + ((ptrdiff_t)(row_of_0 + pos) * r.n_kv + head) * size + d : own + e;
+            const float s = scales[row / BLOCK];
             __align__(16) float v[8];
 #pragma unroll
             for (int i = 0; i < PER; ++i) v[i] = there ? s * (float)(int8_t)((i < 4 ? c[k].x : c[k].y) >> (8 * (i & 3))) : 0.f;
@@ -549,20 +550,22 @@ __device__ __forceinline__ void read_tile(const Read& r, const int8_t* codes, co
     }
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(READERS) read_kernel(Read r) {
+template <typename T, bool VEC, bool ROWS>
+__global__ void __launch_bounds__(READERS, sizeof(T) == 2 ? 6 : 7) read_kernel(Read r) {
     let_next_kernel_start();
     const int seq = blockIdx.x / r.pages, head = blockIdx.y;
     const int first = r.seen ? first_visible_key(r.seq_first[seq], r.span) : r.seq_first[seq], len = r.seq_len[seq];
     const int index = first / PAGE + (int)(blockIdx.x % r.pages), base = index * PAGE;
+    const int row_of_0 = ROWS ? r.cu_rows[seq] - first : 0;            // the row of position 0, if it had one
     wait_for_previous_kernels();
     if (base >= len) return;
     const int slot = r.seq_slot[seq];
     if (!RI_BLOCK_IN_LIMIT(slot, RI_LIMIT_SLOTS, RI_CHECK_SLOT) || !RI_BLOCK_IN_RANGE(index, r.max_pages, RI_CHECK_PAGE_INDEX)) return;
     const int page = r.page_table[(size_t)slot * r.max_pages + index];
     if (!RI_BLOCK_IN_LIMIT(page, RI_LIMIT_PAGES, RI_CHECK_PAGE)) return;
-    read_tile<T, VEC>(r, r.kc, r.ks, reinterpret_cast<T*>(r.k_out), r.hd, head, page, base, first, len, seq);
-    read_tile<T, VEC>(r, r.vc, r.vs, reinterpret_cast<T*>(r.v_out), r.v_hd, head, page, base, first, len, seq);
+    const int out_page = r.out_pages ? seq * r.out_pages + index : page;
+    read_tile<T, VEC, ROWS>(r, r.kc, r.ks, reinterpret_cast<T*>(r.k_out), r.hd, head, page, out_page, base, first, len, row_of_0);
+    read_tile<T, VEC, ROWS>(r, r.vc, r.vs, reinterpret_cast<T*>(r.v_out), r.v_hd, head, page, out_page, base, first, len, row_of_0);
 }
 
 // A cache's pages for the prompts' attention (attention_tcgen05.cu): as float16 numbers over a power of two of their own per
@@ -577,6 +580,7 @@ struct Widen {
     float* factors;              // [sequences][2][kv heads]
     const int *page_table, *seq_slot, *seq_start, *seq_len;
     int max_pages, n_kv, pages, span;
+    int out_pages;               // as in Read
 };
 constexpr int WIDENERS = 256;
 
@@ -601,7 +605,7 @@ __global__ void __launch_bounds__(WIDENERS) widen_kernel(Widen w) {
     const int* pages = w.page_table + (size_t)slot * w.max_pages;
     const int page = pages[index];
     if (!RI_BLOCK_IN_LIMIT(page, RI_LIMIT_PAGES, RI_CHECK_PAGE)) return;
-    const size_t tile = (size_t)page * w.n_kv + head;
+    const size_t tile = (size_t)page * w.n_kv + head, out_tile = w.out_pages ? ((size_t)seq * w.out_pages + index) * w.n_kv + head : tile;
     constexpr int TURNS = PAGE * HD / 8 / WIDENERS;
     uint2 k[TURNS], v[TURNS];
 #pragma unroll
@@ -644,25 +648,28 @@ __global__ void __launch_bounds__(WIDENERS) widen_kernel(Widen w) {
     for (int i = 0; i < TURNS; ++i) {
         const int e = tid + i * WIDENERS, row = e / (HD / 8);
         const bool there = index * PAGE + row < len;
-        reinterpret_cast<uint4*>(w.k_out + tile * PAGE * HD)[e] = widened(k[i], scales[0][row / BLOCK], there);
-        reinterpret_cast<uint4*>(w.v_out + tile * PAGE * HD)[e] = widened(v[i], scales[1][row / BLOCK], there);
+        reinterpret_cast<uint4*>(w.k_out + out_tile * PAGE * HD)[e] = widened(k[i], scales[0][row / BLOCK], there);
+        reinterpret_cast<uint4*>(w.v_out + out_tile * PAGE * HD)[e] = widened(v[i], scales[1][row / BLOCK], there);
     }
 }
 
 }  // namespace
 
-// The pages that a step's queries see (all keys, or a span of them: first_visible_key) as float16 numbers, of the cache's shape, and
-// float32 factors [n_seqs][2][n_kv] that keys and values are to be multiplied by.  Heads of 64 or 128; max_len: no sequence is longer.
+// The pages that a step's queries see (all keys, or a span of them: first_visible_key) as float16 numbers, and
+// float32 factors [n_seqs][2][n_kv] that keys and values are to be multiplied by.  out_pages 0: the outputs have the cache's shape; else
+// they are [n_seqs * out_pages, ...], and a sequence's i-th page is that one's own (max_len / 64 rounded up or more).  Heads of
+// 64 or 128; max_len: no sequence is longer.
 RI_API int ri_quantized_widen(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, void* k_out, void* v_out, float* factors,
                               const int* page_table, int max_pages, const int* seq_slot, const int* seq_start, const int* seq_len,
-                              int n_seqs, int max_len, int n_kv, int hd, int span, cudaStream_t stream) {
+                              int n_seqs, int max_len, int n_kv, int hd, int span, int out_pages, cudaStream_t stream) {
     if (n_seqs <= 0 || max_len <= 0) return 0;
     if (hd != 64 && hd != 128) return fail("quantized_widen: heads of %d channels (64 or 128 wanted)", hd);
     if (n_kv > 65535) return fail("quantized_widen: %d kv heads are too many", n_kv);
     if (!aligned16(kc) || !aligned16(vc) || !aligned16(k_out) || !aligned16(v_out)) return fail("quantized_widen: pages must lie on 16-byte boundaries");
     const int pages = (max_len + PAGE - 1) / PAGE;
     if ((long long)pages * n_seqs > 0x7fffffff) return fail("quantized_widen: %d sequences of %d positions are too many", n_seqs, max_len);
-    const Widen w = {kc, vc, ks, vs, (__half*)k_out, (__half*)v_out, factors, page_table, seq_slot, seq_start, seq_len, max_pages, n_kv, pages, span};
+    if (out_pages < 0 || (out_pages > 0 && out_pages < pages)) return fail("quantized_widen: %d pages for %d positions", out_pages, max_len);
+    const Widen w = {kc, vc, ks, vs, (__half*)k_out, (__half*)v_out, factors, page_table, seq_slot, seq_start, seq_len, max_pages, n_kv, pages, span, out_pages};
     const dim3 grid((unsigned)(pages * n_seqs), (unsigned)n_kv);
     auto launch = [&](auto kernel) { return check_launch(launch_dependent(kernel, grid, dim3(WIDENERS), 0, stream, w), "quantized_widen"); };
     return hd == 64 ? launch(widen_kernel<64>) : launch(widen_kernel<128>);
@@ -727,21 +734,25 @@ RI_API int ri_quantized_write(void* src, int src_dtype, int ld, const float* bia
 }
 
 // Values of the positions seq_first..seq_len - 1 of every sequence (seen: from the first key that a query at seq_first sees within
-// `span`, see first_visible_key).  cu_rows null: k_out, v_out have the cache's shape and get whole pages (zeros elsewhere in them); else they are [rows, kv heads, head size] and sequence b's rows begin at cu_rows[b].
+// `span`, see first_visible_key).  cu_rows null: k_out, v_out get whole pages (zeros elsewhere in them), out_pages as in
+// ri_quantized_widen; else they are [rows, kv heads, head size] and sequence b's rows begin at cu_rows[b].
 // max_len: no sequence is longer.
 RI_API int ri_quantized_read(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, void* k_out, void* v_out, int dtype,
                              const int* page_table, int max_pages, const int* seq_slot, const int* seq_first, const int* seq_len,
-                             const int* cu_rows, int n_seqs, int max_len, int n_kv, int hd, int v_hd, int seen, int span, cudaStream_t stream) {
+                             const int* cu_rows, int n_seqs, int max_len, int n_kv, int hd, int v_hd, int seen, int span, int out_pages, cudaStream_t stream) {
     if (n_seqs <= 0 || max_len <= 0) return 0;
     if (n_kv > 65535) return fail("quantized_read: %d kv heads are too many", n_kv);
     const int pages = (max_len + PAGE - 1) / PAGE;
     if ((long long)pages * n_seqs > 0x7fffffff) return fail("quantized_read: %d sequences of %d positions are too many", n_seqs, max_len);
-    const Read r = {kc, vc, ks, vs, k_out, v_out, page_table, seq_slot, seq_first, seq_len, cu_rows, max_pages, n_kv, hd, v_hd, pages, seen, span};
+    if (out_pages < 0 || (out_pages > 0 && out_pages < pages)) return fail("quantized_read: %d pages for %d positions", out_pages, max_len);
+    const Read r = {kc, vc, ks, vs, k_out, v_out, page_table, seq_slot, seq_first, seq_len, cu_rows, max_pages, n_kv, hd, v_hd, pages, out_pages, seen, span};
     const dim3 grid((unsigned)(pages * n_seqs), (unsigned)n_kv);
     const bool vec = hd % 8 == 0 && v_hd % 8 == 0 && aligned16(kc) && aligned16(vc) && aligned16(k_out) && aligned16(v_out);
     auto launch = [&](auto kernel) { return check_launch(launch_dependent(kernel, grid, dim3(READERS), 0, stream, r), "quantized_read"); };
-    if (dtype == RI_F32) return vec ? launch(read_kernel<float, true>) : launch(read_kernel<float, false>);
-    if (dtype == RI_BF16) return vec ? launch(read_kernel<__nv_bfloat16, true>) : launch(read_kernel<__nv_bfloat16, false>);
+    auto form = [&](auto rows_kernel, auto pages_kernel) { return cu_rows != nullptr ? launch(rows_kernel) : launch(pages_kernel); };
+    using B = __nv_bfloat16;
+    if (dtype == RI_F32) return vec ? form(read_kernel<float, true, true>, read_kernel<float, true, false>) : form(read_kernel<float, false, true>, read_kernel<float, false, false>);
+    if (dtype == RI_BF16) return vec ? form(read_kernel<B, true, true>, read_kernel<B, true, false>) : form(read_kernel<B, false, true>, read_kernel<B, false, false>);
     return fail("quantized_read: unknown dtype %d", dtype);
 }
 

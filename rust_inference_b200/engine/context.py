@@ -48,6 +48,14 @@ class Workspace:
             self._flat[key] = flat
         return flat[:n].view(*shape)
 
+    def counting(self, n: int) -> torch.Tensor:
+        """int32 0 .. n - 1, which nobody writes to."""
+        key = ("counting", torch.int32)
+        flat = self._flat.get(key)
+        if flat is None or flat.numel() < n:
+            flat = self._flat[key] = torch.arange(n, dtype=torch.int32, device=self.device)
+        return flat[:n]
+
     def rezero(self) -> None:
         for (name, _), flat in self._flat.items():
             if isinstance(name, str) and name.startswith("zeroed:"):

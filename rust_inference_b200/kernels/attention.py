@@ -23,6 +23,7 @@ first_visible_key`); both at once go to the generic kernel.
 """
 from __future__ import annotations
 
+import copy
 import functools
 import os
 from typing import NamedTuple
@@ -266,20 +267,35 @@ def _over_quantized(qkv, layer, out, ctx, *, window, chunk, keep_first, **forms)
         from . import attention_tc
         if attention_tc.supports(hd, ctx.page_size, heads, kv, qkv.shape[1], out.shape[1]):
             span = window if window else -int(chunk or 0)
-            k = ctx.buffer("widened_k", layer.k.shape, torch.float16)
-            v = ctx.buffer("widened_v", layer.v.shape, torch.float16)
+            pages, own, there = scratch_pages(ctx, layer.k.shape[0], ctx.max_len)
+            k = ctx.buffer("widened_k", (pages, *layer.k.shape[1:]), torch.float16)
+            v = ctx.buffer("widened_v", (pages, *layer.v.shape[1:]), torch.float16)
             factors = ctx.buffer("widened_factors", (ctx.n_seqs, 2, kv), torch.float32)
-            quantized_cache.widen(layer, k, v, factors, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.seq_len, max_len=ctx.max_len, span=span)
-            return attention_tc.prefill_half(qkv, k, v, factors, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.cu_seqlens, out,
+            quantized_cache.widen(layer, k, v, factors, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.seq_len, max_len=ctx.max_len, span=span,
+                                  out_pages=own)
+            return attention_tc.prefill_half(qkv, k, v, factors, there.page_table, there.seq_slot, ctx.seq_start, ctx.cu_seqlens, out,
                                              n_seqs=ctx.n_seqs, max_new=ctx.max_new, n_heads=heads, n_kv_heads=kv, head_dim=hd,
                                              page_size=ctx.page_size, scale=forms["scale"], window=span, out_scale=forms["out_scale"])
-    k = ctx.buffer("readback_k", layer.k.shape, qkv.dtype)
-    v = ctx.buffer("readback_v", layer.v.shape, qkv.dtype)
     # (a captured step may run with longer sequences than it was captured with)
     longest = ctx.page_table.shape[1] * ctx.page_size if ctx.all_single else ctx.max_len
+    pages, own, there = scratch_pages(ctx, layer.k.shape[0], longest)
+    k = ctx.buffer("readback_k", (pages, *layer.k.shape[1:]), qkv.dtype)
+    v = ctx.buffer("readback_v", (pages, *layer.v.shape[1:]), qkv.dtype)
     quantized_cache.read(layer, k, v, ctx.page_table, ctx.seq_slot, ctx.seq_start, ctx.seq_len, max_len=longest,
-                         seen_span=0 if keep_first else (window if window else -int(chunk or 0)))
-    return attention(qkv, _Pages(k, v), out, ctx, window=window, chunk=chunk, keep_first=keep_first, **forms)
+                         seen_span=0 if keep_first else (window if window else -int(chunk or 0)), out_pages=own)
+    return attention(qkv, _Pages(k, v), out, there, window=window, chunk=chunk, keep_first=keep_first, **forms)
+
+
+def scratch_pages(ctx, pool: int, longest: int) -> tuple:
+    """Where a step's keys and values go that are brought to another type: (scratch pages, of each sequence its own so many or 0,
+    the step with the table of them).  As many as the longest sequence has for each, or the pool's own pages where those are fewer."""
+    own = -(-longest // ctx.page_size)
+    if ctx.n_seqs * own >= pool:
+        return pool, 0, ctx
+    numbers = ctx.workspace.counting(ctx.n_seqs * own)
+    there = copy.copy(ctx)
+    there.page_table, there.seq_slot = numbers.view(ctx.n_seqs, own), numbers[:ctx.n_seqs]
+    return ctx.n_seqs * own, own, there
 
 
 class _Pages(NamedTuple):

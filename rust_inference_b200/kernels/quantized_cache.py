@@ -85,28 +85,30 @@ def write(src: torch.Tensor, q_out: torch.Tensor | None, cos, sin, layer: Quanti
 
 
 def read(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, page_table: torch.Tensor, seq_slot, seq_first, seq_len, *,
-         max_len: int, cu_rows: torch.Tensor | None = None, seen_span: int | None = None) -> tuple:
+         max_len: int, cu_rows: torch.Tensor | None = None, seen_span: int | None = None, out_pages: int = 0) -> tuple:
     """The values of the positions seq_first[b] .. seq_len[b] - 1 of every sequence b, in float32 or bfloat16.  With cu_rows, k_out
     and v_out are [rows, kv heads, head size] and sequence b's rows begin at cu_rows[b]; without, they have the cache's shape and
-    the pages that hold these positions are filled (zeros elsewhere in them), the others left alone.  max_len: no sequence is
-    longer.  seen_span: reading begins at the first key that a query at position seq_first[b] sees, of all keys (0), the last so many
+    the pages that hold these positions are filled (zeros elsewhere in them), the others left alone; with out_pages they are
+    [sequences * out_pages, kv heads, 64, head size] instead, and a sequence's i-th page is the i-th of its own.  max_len: no
+    sequence is longer.  seen_span: reading begins at the first key that a query at position seq_first[b] sees, of all keys (0), the last so many
     (> 0) or its own block of -span positions (< 0)."""
     native("read")(layer.native, k_out, v_out, page_table, seq_slot, seq_first, seq_len, max_len, cu_rows, layer.k.shape[0],
-                   0 if seen_span is None else 1, seen_span or 0)
+                   0 if seen_span is None else 1, seen_span or 0, out_pages)
     return k_out, v_out
 
 
 def widen(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, factors: torch.Tensor, page_table: torch.Tensor, seq_slot,
-          seq_start, seq_len, *, max_len: int, span: int = 0) -> None:
+          seq_start, seq_len, *, max_len: int, span: int = 0, out_pages: int = 0) -> None:
     """The pages that a step's queries see as float16 numbers for `attention_tc.prefill_half`: k_out, v_out float16 of the cache's
-    shape, and factors float32 [sequences, 2, kv heads] that keys and values are to be multiplied by.  What is outside a sequence's
+    shape (or with out_pages for each sequence, as for `read`), and factors float32 [sequences, 2, kv heads] that keys and values are to be multiplied by.  What is outside a sequence's
     seen blocks is 0; a block that is no number is that in its keys."""
     what = "quantized_cache.widen"
     n_kv, hd, v_hd = layer.sizes
     n_seqs = seq_slot.numel()
     _need(layer.aligned and v_hd == hd and hd in (64, 128), what, "heads of 64 or 128 channels, keys and values alike")
     _need(k_out.is_cuda and v_out.is_cuda and k_out.dtype == v_out.dtype == torch.float16 and k_out.is_contiguous() and v_out.is_contiguous()
-          and k_out.shape == layer.k.shape and v_out.shape == layer.v.shape, what, "outputs must be float16 of the cache's shape")
+          and k_out.shape == v_out.shape == (n_seqs * out_pages if out_pages else layer.k.shape[0], *layer.k.shape[1:]), what,
+          "outputs must be float16 of the cache's shape, or so many pages for each sequence")
     _need(factors.is_cuda and factors.dtype == torch.float32 and factors.is_contiguous() and factors.numel() >= 2 * n_seqs * n_kv, what,
           "factors must be float32 [sequences, 2, kv heads]")
     _need(page_table.dim() == 2, what, "the page table must be int32 [slots, pages]")
@@ -114,7 +116,7 @@ def widen(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, facto
         _index(what, t, least)
     _call("quantized_cache", "ri_quantized_widen", _p(layer.k), _p(layer.v), _p(layer.k_scale), _p(layer.v_scale), _p(k_out), _p(v_out),
           _p(factors), _p(page_table), c_int(page_table.shape[1]), _p(seq_slot), _p(seq_start), _p(seq_len), c_int(n_seqs), c_int(max_len),
-          c_int(n_kv), c_int(hd), c_int(span), _stream())
+          c_int(n_kv), c_int(hd), c_int(span), c_int(out_pages), _stream())
 
 
 @functools.lru_cache(maxsize=None)

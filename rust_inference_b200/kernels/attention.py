@@ -139,7 +139,8 @@ def attention(qkv, cache_layer, out, ctx, *, n_heads, n_kv_heads, head_dim, scal
     if type(cache_layer) is quantized_cache.QuantizedPages:
         if ((head_dim == 64 or head_dim == 128) and (v_head_dim is None or v_head_dim == head_dim) and not (window and chunk)
                 and not (softcap or keep_first or sink is not None or dist is not None or gate is not None)
-                and cache_layer.aligned and reads_codes(ctx, qkv.dtype is torch.float32, n_heads, n_kv_heads)):
+                and cache_layer.aligned and reads_codes(ctx, qkv.dtype is torch.float32, n_heads, n_kv_heads, head_dim,
+                                                        window if window else -int(chunk or 0))):
             return quantized_cache.attend_step(qkv, cache_layer, out, quantized_cache.step_of(ctx, n_heads, n_kv_heads, head_dim), scale,
                                                window if window else -int(chunk or 0), out_scale)
         return _over_quantized(qkv, cache_layer, out, ctx, n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, scale=scale,
@@ -239,8 +240,8 @@ def attention(qkv, cache_layer, out, ctx, *, n_heads, n_kv_heads, head_dim, scal
         gate=gate)
 
 
-# Up to so many new tokens per sequence, or so many rows (tokens times query heads) of all sequences, a bfloat16 step reads the codes
-# themselves.  Its time is the rows' times the keys', 3.4 us per million of them (heads of 128); by way of float16 scratch it is a tile of
+# Up to so many new tokens per sequence, or, where the host does not know each sequence's, so many rows (tokens times query heads) of all
+# sequences, a bfloat16 step reads the codes themselves.  Its time is the rows' times the keys', 3.4 us per million of them (heads of 128); by way of float16 scratch it is a tile of
 # 128 tokens' walk over the keys, 15 us per thousand, and more once the tiles fill the SMs.  Measured, straight from the codes and by way of
 # scratch, us (32 heads over 8 kv heads of 128):
 #   1 sequence, 4,096 keys:    16 tokens 27 and 60, 64 tokens 43 and 61, 128 tokens 68 and 61;  30,000 keys: 64 tokens 190 and 460
@@ -250,12 +251,48 @@ def attention(qkv, cache_layer, out, ctx, *, n_heads, n_kv_heads, head_dim, scal
 # In float32 the other way (read back into float32 pages) is never faster: 4,096 keys, 1 sequence: 8 tokens 22 and 296, 1,000 tokens
 # 510 and 2184; 8 sequences of 1,000 tokens over 1,024 keys 1292 and 2510.
 CODES_TOKENS, CODES_ROWS = 16, 2048
+# Steps in which sequences bring different numbers of tokens are judged by the time that either way takes, us: straight from the codes
+# CODES_UNIT for every page of an item (8 rows of a kv head), its set-up counted as 8 pages; by way of scratch SCRATCH_KEY for every key of a
+# head's tile of 128 tokens, or TILE_KEY for every key of the longest where there are few tiles, and the copy's bytes.  Measured, straight
+# from the codes and by way of scratch, us (32 heads over 8 of 128):
+#   63 sequences of 2,000 keys with 1 token and 1 prompt:  17 tokens 71 and 387, 500 tokens 118 and 423, 1,500 345 and 504, 2,500 746 and 593
+#   8 of 2,000 with 1 token and 8 prompts of 40            35 and 61
+#   15 of 8,000 with 1 token and a prompt of 2,000         513 and 459
+#   63 of 2,000 with 1 token and 1,000 tokens behind 29,000  2775 and 1330
+#   7 prompts of 300  171 and 34;  100 tokens behind 30,000  286 and 435
+# (28 heads over 4 of 128, 14 over 2 of 64 likewise: 37 and 284, 20 and 119 for the first of them.)
+CODES_UNIT = {64: 1.0e-3, 128: 1.5e-3}
+SCRATCH_KEY, TILE_KEY, COPY_BYTE, CODES_CALL, SCRATCH_CALL = 6.0e-5, 1.5e-2, 1.0 / 6.0e6, 5.0, 8.0
 
 
-def reads_codes(ctx, f32: bool, n_heads: int, n_kv_heads: int) -> bool:
+def reads_codes(ctx, f32: bool, n_heads: int, n_kv_heads: int, head_dim: int = 128, span: int = 0) -> bool:
     """Whether a step with the plain form of the score reads a cache in 8 bits directly."""
-    few = ctx.max_new <= CODES_TOKENS or ctx.n_seqs * ctx.max_new * n_heads <= CODES_ROWS
-    return (f32 or few) and quantized_cache.attention_counts(ctx.n_seqs, ctx.page_table.shape[1], ctx.max_new, n_heads, n_kv_heads)
+    counts = getattr(ctx, "host_counts", None)
+    few = f32 or ctx.max_new <= CODES_TOKENS
+    if not few and counts is None:
+        few = ctx.n_seqs * ctx.max_new * n_heads <= CODES_ROWS
+    elif not few:
+        key = ("reads_codes", n_heads, n_kv_heads, head_dim, span)
+        held = ctx.extras.get(key)
+        if held is None or held[0] is not counts or held[1] is not ctx.host_starts:
+            held = ctx.extras[key] = (counts, ctx.host_starts, codes_are_faster(ctx.host_starts, counts, n_heads, n_kv_heads, head_dim, span))
+        few = held[2]
+    return few and quantized_cache.attention_counts(ctx.n_seqs, ctx.page_table.shape[1], ctx.max_new, n_heads, n_kv_heads)
+
+
+def codes_are_faster(starts, counts, n_heads: int, n_kv_heads: int, head_dim: int, span: int = 0) -> bool:
+    """`reads_codes` for a bfloat16 step of sequences with so many keys before it and so many new tokens."""
+    units = tile_keys = copied = longest = 0
+    rep = n_heads // n_kv_heads
+    for start, n in zip(starts, counts):
+        keys = start + n if span == 0 else min(start + n, n + abs(span))
+        units += -(-n * rep // 8) * (-(-keys // 64) + 8)
+        tile_keys += -(-n // 128) * keys
+        copied += keys
+        longest = max(longest, keys)
+    codes = CODES_CALL + CODES_UNIT[head_dim] * n_kv_heads * units
+    scratch = SCRATCH_CALL + max(TILE_KEY * longest, SCRATCH_KEY * n_heads * tile_keys) + COPY_BYTE * 6 * head_dim * n_kv_heads * copied
+    return codes <= scratch
 
 
 def _over_quantized(qkv, layer, out, ctx, *, window, chunk, keep_first, **forms):

@@ -52,7 +52,7 @@ def test_a_models_prompt_takes_scratch_for_its_own_pages(model_factory):
     lib = Model.load(model.folder, cache_dtype="int8", max_tokens_in_cache=1 << 20)
     eng = lib.engine
     slot = eng.alloc_slot()
-    eng.step([slot], [random_tokens(600, model.cfg["vocab_size"], seed=1)], "last")
+    eng.step([slot], [random_tokens(1000, model.cfg["vocab_size"], seed=1)], "last")
     layer = eng.cache.layer(0)
     taken = {name: flat.numel() * flat.element_size() for (name, _), flat in eng.workspace._flat.items() if "widened" in name or "readback" in name}
     assert 0 < sum(taken.values()) < layer.k.numel() // 100

@@ -807,8 +807,9 @@ attn_quantized_kernel(const Args a) {
     cluster_sync();                              // a peer may still be reading this block's part
 }
 
+// form, if asked for: which kernel it would be, clusters of eight, of four or runs of units (0, 1, 2), times 4 and NQ; nothing is launched
 template <int HD, typename T, int TERMS, int NQ>
-int launch(Args a, long long items, long long keys, long long part_floats, cudaStream_t stream) {
+int launch(Args a, long long items, long long keys, long long part_floats, int* form, cudaStream_t stream) {
     static PerDeviceOnce once, once_own;
     static std::atomic<int> resident[64][3];
     // (tiles of 16 rows are for steps that do not fit clusters)
@@ -846,6 +847,10 @@ int launch(Args a, long long items, long long keys, long long part_floats, cudaS
     // 17.5 and 20.9; float32, 4 of 4,096 12.8 and 18.3; 14 heads over 2 of 64: 1 of 437 4.9 and 6.4, 32 of 4,096 11.9 and 17.8.
     auto fits = [&](int size) { return keys <= (long long)(a.n_seqs == 1 ? 8 : 4) * 2 * PAGE * size; };
     const int which = NQ > 1 ? 2 : (8 * items <= held(0) && fits(8) ? 0 : (4 * items <= held(1) && fits(4) ? 1 : 2));
+    if (form != nullptr) {
+        *form = 4 * which + NQ;
+        return 0;
+    }
     a.cluster = which == 2 ? 1 : 8 >> which;
     const int blocks = which == 2 ? held(2) : a.cluster * (int)items;
     if (part_floats < 2ll * blocks * a.rows_cap * (HD + 4)) return fail("attention_quantized: scratch of %lld numbers is too small", part_floats);
@@ -855,7 +860,37 @@ int launch(Args a, long long items, long long keys, long long part_floats, cudaS
     return launch_cluster("attention_quantized", which == 2 ? kernel : kernel_own, dim3((unsigned)blocks), THREADS, (size_t)smem, a.cluster, stream, a);
 }
 
+// a.n_seqs, n_rep, n_kv and span are set; longest: the keys of the longest sequence
+int choose(Args a, int dtype, int max_new, int longest, int hd, long long part_floats, int* form, cudaStream_t stream) {
+    const long long rows = (long long)max_new * a.n_rep;
+    // A tile of 16 rows takes 1.75 times what one of 8 takes, which pays where the step has rows and keys for all of the SMs to be busy for
+    // long, 80 pages for 8 rows and more to an SM; below that half as many items to spread over the blocks cost more.  Tiles of 8 and of 16,
+    // us: 64 sequences of 1,024 keys, 32 heads over 8 of 128, 4 tokens 58.8 and 55.2 (16,384 pages), 16 tokens 182 and 165; 28 heads over 4, 3
+    // tokens (21 rows) 43.9 and 51.4; float32, 1,000 tokens over 4,096 keys 645 and 509; below: 1 sequence of 1,024 keys, 4 tokens
+    // 10.3 and 13.6; 4 sequences of 3,000, 12 heads over 2, 4 tokens in float32 15.3 and 20.9 (752 pages).
+    const long long tiles = (rows + 7) / 8, wide = (rows + 15) / 16;
+    const long long keys = a.span == 0 ? longest : std::min((long long)longest, (long long)max_new + (a.span > 0 ? a.span : -(long long)a.span));
+    const int nq = 7 * wide < 4 * tiles && (keys + PAGE - 1) / PAGE * tiles * a.n_seqs * a.n_kv > 80ll * sm_count() ? 2 : 1;
+    a.rows_cap = (int)(rows < 8 * nq ? rows : 8 * nq);
+    const long long items = a.n_seqs * (nq == 1 ? tiles : wide) * a.n_kv;        // at most
+    using B = __nv_bfloat16;
+    if (dtype == RI_F32 && nq == 1) return hd == 64 ? launch<64, float, 2, 1>(a, items, keys, part_floats, form, stream) : launch<128, float, 2, 1>(a, items, keys, part_floats, form, stream);
+    if (dtype == RI_F32) return hd == 64 ? launch<64, float, 2, 2>(a, items, keys, part_floats, form, stream) : launch<128, float, 2, 2>(a, items, keys, part_floats, form, stream);
+    if (dtype == RI_BF16 && nq == 1) return hd == 64 ? launch<64, B, 1, 1>(a, items, keys, part_floats, form, stream) : launch<128, B, 1, 1>(a, items, keys, part_floats, form, stream);
+    if (dtype == RI_BF16) return hd == 64 ? launch<64, B, 1, 2>(a, items, keys, part_floats, form, stream) : launch<128, B, 1, 2>(a, items, keys, part_floats, form, stream);
+    return fail("attention_quantized: unknown dtype %d", dtype);
+}
+
 }  // namespace
+
+// Which kernel `ri_attention_quantized` launches for such a step, as a number; -1 for one that it does not take
+RI_API int ri_attention_quantized_form(int dtype, int n_seqs, int max_new, int longest, int n_heads, int n_kv, int hd, int span) {
+    if (n_seqs <= 0 || max_new <= 0 || (hd != 64 && hd != 128) || n_kv <= 0 || n_heads % n_kv) return -1;
+    Args a = {};
+    a.n_seqs = n_seqs, a.n_rep = n_heads / n_kv, a.n_kv = n_kv, a.span = span;
+    int form = -1;
+    return choose(a, dtype, max_new, longest, hd, 0, &form, nullptr) ? -1 : form;
+}
 
 // Thread blocks of a step, at most
 RI_API int ri_attention_quantized_blocks() { return MOST_BLOCKS * sm_count(); }
@@ -892,22 +927,7 @@ RI_API int ri_attention_quantized(const void* q, int dtype, int q_ld, const int8
     a.out_scale = out_scale;
     a.part = part;
     a.arrived = arrived;
-    // A tile of 16 rows takes 1.75 times what one of 8 takes, which pays where the step has rows and keys for all of the SMs to be busy for
-    // long, 80 pages for 8 rows and more to an SM; below that half as many items to spread over the blocks cost more.  Tiles of 8 and of 16,
-    // us: 64 sequences of 1,024 keys, 32 heads over 8 of 128, 4 tokens 58.8 and 55.2 (16,384 pages), 16 tokens 182 and 165; 28 heads over 4, 3
-    // tokens (21 rows) 43.9 and 51.4; float32, 1,000 tokens over 4,096 keys 645 and 509; below: 1 sequence of 1,024 keys, 4 tokens
-    // 10.3 and 13.6; 4 sequences of 3,000, 12 heads over 2, 4 tokens in float32 15.3 and 20.9 (752 pages).
-    const long long tiles = (rows + 7) / 8, wide = (rows + 15) / 16;
-    const long long keys = span == 0 ? longest : std::min((long long)longest, (long long)max_new + (span > 0 ? span : -(long long)span));
-    const int nq = 7 * wide < 4 * tiles && (keys + PAGE - 1) / PAGE * tiles * n_seqs * n_kv > 80ll * sm_count() ? 2 : 1;
-    a.rows_cap = (int)(rows < 8 * nq ? rows : 8 * nq);
-    const long long items = n_seqs * (nq == 1 ? tiles : wide) * n_kv;          // at most
-    if (dtype == RI_F32 && nq == 1) return hd == 64 ? launch<64, float, 2, 1>(a, items, keys, part_floats, stream) : launch<128, float, 2, 1>(a, items, keys, part_floats, stream);
-    if (dtype == RI_F32) return hd == 64 ? launch<64, float, 2, 2>(a, items, keys, part_floats, stream) : launch<128, float, 2, 2>(a, items, keys, part_floats, stream);
-    if (dtype == RI_BF16 && nq == 1)
-        return hd == 64 ? launch<64, __nv_bfloat16, 1, 1>(a, items, keys, part_floats, stream) : launch<128, __nv_bfloat16, 1, 1>(a, items, keys, part_floats, stream);
-    if (dtype == RI_BF16) return hd == 64 ? launch<64, __nv_bfloat16, 1, 2>(a, items, keys, part_floats, stream) : launch<128, __nv_bfloat16, 1, 2>(a, items, keys, part_floats, stream);
-    return fail("attention_quantized: unknown dtype %d", dtype);
+    return choose(a, dtype, max_new, longest, hd, part_floats, nullptr, stream);
 }
 
 RI_DEFINE_LAST_ERROR()

@@ -32,7 +32,7 @@ import weakref
 import numpy as np
 import torch
 
-from ..kernels import ops
+from ..kernels import ops, quantized_cache
 from .context import StepContext, Workspace, pack_step
 
 
@@ -65,6 +65,8 @@ class DecodeGraph:
         self.held = None              # [slots, lengths before the step, streams, draw counters] the static arrays describe now
         self.turn = 0                 # steps run: the host's copy of the device counter that picks the ring slots
         self.reach = 0                # see `expect`
+        self.forms = None             # the kernels over a cache in 8 bits that the capture holds
+        self.outgrown = False         # ... and that the step to come would not choose
         self.rows = self.turn_dev = self.host_ring = self.log = self.seed_dev = None
         if sampler is not None:
             if sampler.uses_history:
@@ -118,15 +120,17 @@ class DecodeGraph:
 
     def expect(self, longest: int) -> None:
         """The longest sequence has so many keys in the step to come.  Kernels of a cache in 8 bits choose their launches by that
-        number, as a bound that holds for a while: FIRST_REACH times a power of two.  When a sequence grows beyond it, the step is
-        captured again.  (Kernels of other caches depend on the cache's geometry only.)"""
-        if self.engine.cache.kv_dtype is None or longest <= self.reach:
+        number, as a bound that holds for a while: FIRST_REACH times a power of two, until a sequence grows beyond it or all are
+        down to a quarter of it.  Where the choice changes with it, the step is captured again.  (Kernels of other caches depend on
+        the cache's geometry only.)"""
+        if self.engine.cache.kv_dtype is None or self.reach // 4 < longest <= self.reach or longest <= self.reach == FIRST_REACH:
             return
-        self.reach = max(self.reach, FIRST_REACH)
+        self.reach = FIRST_REACH
         while self.reach < longest:
             self.reach *= 2
         self.ctx.extras["longest"] = min(self.reach, self.engine.max_seq_len)
-        self.graph = None
+        if self.graph is not None:
+            self.outgrown = quantized_cache.step_forms(self.ctx, self.ctx.extras["longest"]) != self.forms
 
     # ---- running ------------------------------------------------------------------------------
     def _step(self, logits: torch.Tensor) -> None:
@@ -164,7 +168,7 @@ class DecodeGraph:
         return out
 
     def _launch(self) -> torch.Tensor:
-        if self.graph is None:
+        if self.graph is None or self.outgrown:
             self.eager_steps += 1
             if self.eager_steps <= EAGER_STEPS:
                 # kernel by kernel, on the engine's shared scratch (the first time this also compiles
@@ -189,7 +193,9 @@ class DecodeGraph:
             finally:
                 if collecting:
                     gc.enable()
-            self.graph = g
+            self.graph, self.outgrown = g, False
+            if self.engine.cache.kv_dtype is not None:
+                self.forms = quantized_cache.step_forms(self.ctx, self.ctx.extras["longest"])
         self.graph.replay()
         return self.logits
 

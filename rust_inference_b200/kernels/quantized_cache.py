@@ -18,7 +18,7 @@ from ctypes import c_int
 import torch
 
 from .build import load
-from .ops import KernelError, _call, _p, _stream, native
+from .ops import RI_BF16, RI_F32, KernelError, _call, _p, _stream, native
 
 PAGE_SIZE, BLOCK = 64, 16
 
@@ -135,7 +135,7 @@ def attention_counts(n_seqs: int, pages: int, max_new: int, n_heads: int, n_kv_h
 class _Step:
     """What the calls of a step have in common: its arrays' addresses and sizes, looked at once."""
 
-    __slots__ = ("native", "kept", "max_new", "longest")
+    __slots__ = ("native", "kept", "max_new", "longest", "calls")
 
     def __init__(self, ctx, n_heads, n_kv_heads, head_dim):
         what = "quantized_cache.attend_step"
@@ -143,6 +143,7 @@ class _Step:
         _need(n_kv_heads > 0 and n_heads % n_kv_heads == 0 and head_dim in (64, 128) and table.dim() == 2, what,
               f"{n_heads} heads of {head_dim} over {n_kv_heads}, or a page table that is not [slots, pages]")
         self.max_new, self.longest = ctx.max_new, _longest(ctx)
+        self.calls = set()                                      # (span, dtype) of the layers' calls
         floats, ints = attention_workspace(n_heads, n_kv_heads, head_dim, ctx.max_new)
         part = ctx.buffer("quantized_part", (floats,), torch.float32)
         arrived = ctx.zeroed_buffer("quantized_arrived", (ints,), torch.int32)
@@ -177,4 +178,13 @@ def attend_step(q, layer: QuantizedPages, out, step: _Step, scale: float, span: 
     """Attention of every token of the step over its slot's cached keys, straight from the codes (csrc/attention_quantized.cu), for heads
     of 64 or 128.  q: float32 or bfloat16 rows whose leading columns are the queries, rotated; out: rows of q's dtype; span: > 0 the
     last so many keys, < 0 the keys of the query's own block of -span positions, 0 all."""
+    step.calls.add((span, q.dtype))
     return native("attend")(q, layer.native, out, step.native, scale, span, out_scale)
+
+
+def step_forms(ctx, longest: int) -> dict:
+    """Which kernels the calls of a step so far would launch if its longest sequence had so many keys."""
+    form = load("attention_quantized").ri_attention_quantized_form
+    return {(key, call): form(*(c_int(v) for v in (RI_F32 if call[1] is torch.float32 else RI_BF16, step.kept[1].numel(), step.max_new, longest,
+                                                   *key[1:], call[0])))
+            for key, step in ctx.extras.items() if type(step) is _Step for call in step.calls}

@@ -21,8 +21,11 @@ class TokenScores:
 
     @property
     def perplexity(self) -> float:
-        """e to the mean of the negative log probabilities."""
-        return math.exp(-sum(self.logprobs) / len(self.logprobs))
+        """e to the mean of the negative log probabilities (infinite beyond what a float holds)."""
+        try:
+            return math.exp(-sum(self.logprobs) / len(self.logprobs))
+        except OverflowError:
+            return math.inf
 
 
 class Model:

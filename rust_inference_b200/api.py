@@ -145,6 +145,8 @@ class Model:
             raise ValueError("score: a text of at least two tokens")
         eng = self.engine
         vocab = eng.model.spec.vocab_size
+        if not 0 <= top <= min(ops.TOKEN_LOGPROBS_MOST, vocab):
+            raise ValueError(f"score: 0 to {min(ops.TOKEN_LOGPROBS_MOST, vocab)} alternatives, found {top}")
         if not 0 <= tokens[-1] < vocab:
             raise ValueError(f"score: a token id outside [0, {vocab}): {tokens[-1]}")
         piece = max(1, SCORE_LOGITS // vocab)

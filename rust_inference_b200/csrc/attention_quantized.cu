@@ -885,7 +885,7 @@ int choose(Args a, int dtype, int max_new, int longest, int hd, long long part_f
 
 // Which kernel `ri_attention_quantized` launches for such a step, as a number; -1 for one that it does not take
 RI_API int ri_attention_quantized_form(int dtype, int n_seqs, int max_new, int longest, int n_heads, int n_kv, int hd, int span) {
-    if (n_seqs <= 0 || max_new <= 0 || (hd != 64 && hd != 128) || n_kv <= 0 || n_heads % n_kv) return -1;
+    if (n_seqs <= 0 || max_new <= 0 || (hd != 64 && hd != 128) || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv) return -1;
     Args a = {};
     a.n_seqs = n_seqs, a.n_rep = n_heads / n_kv, a.n_kv = n_kv, a.span = span;
     int form = -1;
@@ -903,7 +903,7 @@ RI_API int ri_attention_quantized(const void* q, int dtype, int q_ld, const int8
                                   float out_scale, float* part, long long part_floats, int* arrived, cudaStream_t stream) {
     if (n_seqs <= 0 || max_new <= 0) return 0;
     if (hd != 64 && hd != 128) return fail("attention_quantized: heads of %d channels (64 or 128 wanted)", hd);
-    if (n_kv <= 0 || n_heads % n_kv) return fail("attention_quantized: %d heads over %d kv heads", n_heads, n_kv);
+    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv) return fail("attention_quantized: %d heads over %d kv heads", n_heads, n_kv);
     if ((uintptr_t)kc % 16 || (uintptr_t)vc % 16 || (uintptr_t)part % 16) return fail("attention_quantized: codes and scratch must lie on 16-byte boundaries");
     const long long rows = (long long)max_new * (n_heads / n_kv);
     if ((long long)n_seqs * (max_pages + SETUP) * n_kv * ((rows + 7) / 8) > 0x7fffffff || rows > 0x7fffffff)

@@ -116,6 +116,7 @@ PyObject* py_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const long long heads = number(a[9]), kv = number(a[10]), hd = number(a[11]), v_hd = number(a[12]), rot = number(a[15]);
         PyObject* layer = a[4];
         if (item(layer, 4) != kv || item(layer, 5) != hd || item(layer, 6) != v_hd) refuse("quantized_cache.write: the layer has other heads");
+        need(heads >= 0, "quantized_cache.write: a negative number of heads");
         const long long cols = (heads + kv) * hd + kv * v_hd;
         const at::Tensor& src = tensor(a[0], what);
         need(src.is_cuda() && src.dim() == 2 && src.is_contiguous() && src.size(1) >= cols,

@@ -686,7 +686,7 @@ RI_API int ri_quantized_write(void* src, int src_dtype, int ld, const float* bia
     if (hd <= 0 || v_hd <= 0 || hd % 2 || v_hd % 2) return fail("quantized_write: heads of %d and %d channels (even numbers wanted)", hd, v_hd);
     if (rot < 0 || rot % 2 || rot > hd) return fail("quantized_write: %d rotated channels of a head of %d", rot, hd);
     if (style != 0 && style != 1) return fail("quantized_write: unknown style %d", style);
-    if (n_heads + 2 * n_kv > 65535) return fail("quantized_write: %d heads are too many", n_heads + 2 * n_kv);
+    if (n_heads < 0 || n_kv <= 0 || n_heads + 2ll * n_kv > 65535) return fail("quantized_write: %d heads and %d kv heads", n_heads, n_kv);
     // Blocks of positions: so many per sequence, or, where most sequences bring far fewer tokens than the longest, counted through (a warp
     // then walks the sequences' lengths, but fewer blocks of threads find nothing to do): 16 sequences of 1 to 2,047 tokens 28.1 us by
     // sequence, 25.9 counted through; 2 of 1 to 333 3.41 and 3.30.

@@ -140,7 +140,7 @@ class _Step:
     def __init__(self, ctx, n_heads, n_kv_heads, head_dim):
         what = "quantized_cache.attend_step"
         table, n_seqs = ctx.page_table, ctx.seq_slot.numel()
-        _need(n_kv_heads > 0 and n_heads % n_kv_heads == 0 and head_dim in (64, 128) and table.dim() == 2, what,
+        _need(n_kv_heads > 0 and n_heads > 0 and n_heads % n_kv_heads == 0 and head_dim in (64, 128) and table.dim() == 2, what,
               f"{n_heads} heads of {head_dim} over {n_kv_heads}, or a page table that is not [slots, pages]")
         self.max_new, self.longest = ctx.max_new, _longest(ctx)
         self.calls = set()                                      # (span, dtype) of the layers' calls

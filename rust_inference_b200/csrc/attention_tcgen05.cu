@@ -44,14 +44,18 @@
 // scale has 11 significant bits, not 8.  A row's query is brought to [2^14, 2^15) by a power of two and made float16 in place, where
 // the copy put it, by the thread that has the row's softmax (a bfloat16 number is exact in float16 down to 2^-28 of the row's
 // largest); the powers go into the scale of the row's scores and into the factor on its result.  P is float16 too, times 2^6:
-// up to 2^14 between two moves of the maximum, 2^-12 of a weight down to 2^-20 of the largest.  (2,048 tokens of 28 heads of 128 over
+// up to 2^14 between two moves of the maximum, 2^-11 of a weight, and no finer than 2^-31 of the largest.  (2,048 tokens of 28 heads of 128 over
 // 4, results against 64 bits: 4.1e-3 of their size by way of bfloat16 pages, 1.7e-3 this way, which is bfloat16's own rounding.)
+// A kv head of a sequence whose scales are too far apart for float16 has its pages in bfloat16 (factor -1): its queries stay as they
+// are, its weights become bfloat16 numbers, and the products are told so.
 //
 // All mbarrier waits are bounded; on a timeout the kernel records a code in the host-visible
 // status word and winds down.
 #include "tcgen05_common.cuh"
 
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 using namespace ri;
 using namespace ri::tc;
@@ -127,7 +131,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     constexpr int V_BUFS = LATENT ? 1 : 2;
     constexpr int S_COL = 0, O_COL = 2 * BN;             // two score buffers, then the output accumulator
     constexpr int TMEM_COLS = 256;
-    constexpr uint32_t TYPES = HALF ? 0u : (1u << 7) | (1u << 10);      // both operands float16, or both bfloat16
+    constexpr uint32_t BF16_TYPES = (1u << 7) | (1u << 10), TYPES = HALF ? 0u : BF16_TYPES;      // both operands float16, or both bfloat16
     constexpr uint32_t IDESC_S = (1u << 4) | TYPES | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
     constexpr uint32_t IDESC_PV = (1u << 4) | TYPES | (1u << 16) | ((uint32_t)(V_ATOMS * 64 >> 3) << 17) |
                                   ((uint32_t)(BM >> 4) << 24);
@@ -140,6 +144,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     struct Sync {
         uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full, pv_done;
         uint64_t q_half;
+        volatile int in_bf16;        // HALF: the sequence's kv head is kept in bfloat16, and so are queries and weights
         uint32_t tmem_base_slot;
         volatile int abort_flag;
     };
@@ -270,8 +275,13 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         {                                                        // the whole warp goes through, one lane issues
             const uint32_t leader = elect_one();
             bool ok;
-            if constexpr (HALF) ok = mbar_wait_warp(smem_u32(&sy.q_half), 0);
-            else ok = mbar_wait_warp(smem_u32(&q_full), 0);
+            uint32_t types = 0u;
+            if constexpr (HALF) {
+                ok = mbar_wait_warp(smem_u32(&sy.q_half), 0) && mbar_wait_warp(smem_u32(&q_full), 0);
+                types = __shfl_sync(0xffffffffu, sy.in_bf16 ? BF16_TYPES : 0u, 0);
+            } else {
+                ok = mbar_wait_warp(smem_u32(&q_full), 0);
+            }
             if (!ok) { if (lane == 0) report(status, ST_ATTN_MMA); abort_flag = 1; }
             // The descriptors are built once, and a page's MMAs add constants to their address field (shared memory
             // ends below 256 KiB, so the 14-bit field never carries).
@@ -290,7 +300,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks)
                     umma_by(leader, s_acc, q_desc + (uint64_t)(((ks / 4) * BM * 128 + (ks % 4) * 32) >> 4),
-                            kd + (uint64_t)(((ks / 4) * BN * 128 + (ks % 4) * 32) >> 4), IDESC_S, ks > 0);
+                            kd + (uint64_t)(((ks / 4) * BN * 128 + (ks % 4) * 32) >> 4), IDESC_S | types, ks > 0);
                 umma_commit_by(leader, k_empty0 + 8u * kb);
                 umma_commit_by(leader, s_full0 + 8u * kb);
                 return true;
@@ -309,7 +319,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 for (int ks = 0; ks < BN / 16; ++ks)
                     // P of page j lies, two bf16 to a column, over the first half of the score buffer it came from
                     umma_ts(leader, tmem_base + O_COL, tmem_base + S_COL + pb * BN + ks * 8, vd + (uint64_t)(ks * 16 * 128 >> 4),
-                            IDESC_PV, j > 0 || ks > 0);
+                            IDESC_PV | types, j > 0 || ks > 0);
                 if constexpr (LATENT == 2)
 #pragma unroll
                     for (int ks = 0; ks < BN / 16; ++ks)
@@ -329,14 +339,18 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         float m_used = -INFINITY, l = 0.f;
         bool ok = true;
         float row_scale = scale_log2;
+        bool in_bf16 = false;
         if constexpr (HALF) {
             // the row's queries as float16 numbers, sixteen bytes at a time, each eight rows' in different banks
             wait_for_previous_kernels();                      // the factors come from the kernel before
+            const float k_factor = factors[(size_t)(2 * b) * n_kv_heads + kvh];
+            in_bf16 = k_factor < 0.f;
+            if (lane == 0) sy.in_bf16 = in_bf16;              // (all four warps the same)
             if (!mbar_wait(smem_u32(&q_full), 0) || abort_flag) {
                 if (lane == 0) { report(status, ST_ATTN_SOFTMAX); abort_flag = 1; }
                 ok = false;
             }
-            if (ok) {
+            if (ok && !in_bf16) {
                 uint4* const mine = reinterpret_cast<uint4*>(smem_raw + (q_smem - raw)) + r * 8;
                 float top = 0.f;
 #pragma unroll
@@ -348,7 +362,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
                 const int e = max((int)(__float_as_uint(top) >> 23) - 127, -112);
                 const float up = __uint_as_float((uint32_t)(127 + 14 - min(e, 127)) << 23);
-                row_scale = scale_log2 * (factors[(size_t)(2 * b) * n_kv_heads + kvh] * __uint_as_float((uint32_t)max(127 - 14 + e, 1) << 23));
+                row_scale = scale_log2 * (k_factor * __uint_as_float((uint32_t)max(127 - 14 + e, 1) << 23));
 #pragma unroll
                 for (int i = 0; i < ATOMS * 8; ++i) {
                     uint4& at = mine[(i / 8) * BM * 8 + ((i + r) & 7)];
@@ -364,6 +378,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sy.q_half));
         }
+        auto pages = [&](auto half) {            // weights in float16, or in bfloat16
         for (int j = 0; j < n_pages && ok; ++j) {
             if (!mbar_wait(smem_u32(&s_full[j & 1]), (uint32_t)((j >> 1) & 1)) || abort_flag) {
                 if (lane == 0) { report(status, ST_ATTN_SOFTMAX); abort_flag = 1; }
@@ -422,7 +437,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 const float2 e = __ffma2_rn(make_float2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), scale2, shift2);
                 const float2 p = make_float2(fast_exp2(e.x), fast_exp2(e.y));
                 sum2 = __fadd2_rn(sum2, p);
-                pk[c >> 1] = HALF ? pack2_half(p.x, p.y) : pack2(p.x, p.y);
+                pk[c >> 1] = decltype(half)::value ? pack2_half(p.x, p.y) : pack2(p.x, p.y);
             }
             const float sum = sum2.x + sum2.y;
             if (j > 0) {
@@ -473,6 +488,9 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&p_full));
         }
+        };
+        if (HALF && !in_bf16) pages(std::bool_constant<HALF>{});
+        else pages(std::false_type{});
         if (ok) {
             if (!mbar_wait(smem_u32(&pv_done), (uint32_t)((n_pages - 1) & 1))) {
                 if (lane == 0) { report(status, ST_ATTN_SOFTMAX); abort_flag = 1; }

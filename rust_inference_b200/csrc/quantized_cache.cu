@@ -573,6 +573,9 @@ __global__ void __launch_bounds__(READERS, sizeof(T) == 2 ? 6 : 7) read_kernel(R
 // a page of one kv head and finds that scale for itself (four numbers a page).  What a sequence does not see, before its first
 // seen block and behind its end, is 0.  A block that is no number is that in its keys, whose scores a row that does not see them
 // leaves out, and 0 in its values, which every row's sum runs over.
+// Float16 has no finer numbers than 2^-32 of the largest scale, and the attention no finer weights than 2^-31 of a row's largest: with
+// scales more than 2^12 apart the small ones, of rows that may not see the large ones, would be rounded by those.  Such a sequence's kv
+// head gets bfloat16 numbers, which have the same 8 bits everywhere, and the factors -1 and 1, which say so.
 struct Widen {
     const int8_t *kc, *vc;
     const float *ks, *vs;
@@ -589,9 +592,11 @@ __device__ __forceinline__ float power_above(float scale) {            // 2^e wi
     return scale > 0.f ? __uint_as_float((uint32_t)(127 + max(e, -126)) << 23) : 1.f;
 }
 
+constexpr unsigned APART = 12u << 23;              // as far apart as float16 numbers serve, as the bits of powers of two
+
 template <int HD>
 __global__ void __launch_bounds__(WIDENERS) widen_kernel(Widen w) {
-    __shared__ float scratch[33];
+    __shared__ uint4 found[WIDENERS / 32];          // the largest and the smallest scale of a warp's blocks, of keys and of values, by their bits
     __shared__ float scales[2][PER_PAGE];
     let_next_kernel_start();
     const int seq = blockIdx.x / w.pages, head = blockIdx.y, tid = threadIdx.x;
@@ -613,15 +618,26 @@ __global__ void __launch_bounds__(WIDENERS) widen_kernel(Widen w) {
         k[i] = reinterpret_cast<const uint2*>(w.kc + tile * PAGE * HD)[tid + i * WIDENERS];
         v[i] = reinterpret_cast<const uint2*>(w.vc + tile * PAGE * HD)[tid + i * WIDENERS];
     }
-    float k_top = 0.f, v_top = 0.f;                 // (fmaxf leaves out what is no number)
+    uint4 range = make_uint4(0u, ~0u, 0u, ~0u);     // (positive numbers are in the order of their bits; zeros and what is no number are left out)
     for (int b = first + tid; b <= last; b += WIDENERS) {
         const int p = pages[b / PER_PAGE];
         if (!RI_IN_LIMIT(p, RI_LIMIT_PAGES, RI_CHECK_PAGE)) continue;
         const size_t at = ((size_t)p * w.n_kv + head) * PER_PAGE + b % PER_PAGE;
-        k_top = fmaxf(k_top, w.ks[at]);
-        v_top = fmaxf(v_top, w.vs[at]);
+        const float ks = w.ks[at], vs = w.vs[at];
+        if (ks > 0.f) range.x = max(range.x, __float_as_uint(ks)), range.y = min(range.y, __float_as_uint(ks));
+        if (vs > 0.f) range.z = max(range.z, __float_as_uint(vs)), range.w = min(range.w, __float_as_uint(vs));
     }
-    const float k_unit = power_above(block_max(k_top, scratch)), v_unit = power_above(block_max(v_top, scratch));
+    range = make_uint4(__reduce_max_sync(0xffffffffu, range.x), __reduce_min_sync(0xffffffffu, range.y), __reduce_max_sync(0xffffffffu, range.z),
+                       __reduce_min_sync(0xffffffffu, range.w));
+    if (tid % 32 == 0) found[tid / 32] = range;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WIDENERS / 32; ++i) {
+        const uint4 f = found[i];
+        range = make_uint4(max(range.x, f.x), min(range.y, f.y), max(range.z, f.z), min(range.w, f.w));
+    }
+    const bool apart = (range.x != 0u && range.x - range.y > APART) || (range.z != 0u && range.z - range.w > APART);
+    const float k_unit = apart ? 1.f : power_above(__uint_as_float(range.x)), v_unit = apart ? 1.f : power_above(__uint_as_float(range.z));
     if (tid < PER_PAGE) {
         const int b = index * PER_PAGE + tid;
         const bool seen = b >= first && b <= last;
@@ -630,7 +646,7 @@ __global__ void __launch_bounds__(WIDENERS) widen_kernel(Widen w) {
         scales[1][tid] = vs != vs ? 0.f : vs / v_unit;
     }
     if (index == first / PER_PAGE && tid == 0) {
-        w.factors[(size_t)(2 * seq) * w.n_kv + head] = k_unit;
+        w.factors[(size_t)(2 * seq) * w.n_kv + head] = apart ? -1.f : k_unit;
         w.factors[(size_t)(2 * seq + 1) * w.n_kv + head] = v_unit;
     }
     __syncthreads();
@@ -640,7 +656,9 @@ __global__ void __launch_bounds__(WIDENERS) widen_kernel(Widen w) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t two = (i < 2 ? c.x : c.y) >> (16 * (i & 1));
-            h[i] = there ? __floats2half2_rn(s * (float)(int8_t)two, s * (float)(int8_t)(two >> 8)) : __floats2half2_rn(0.f, 0.f);
+            const float x = there ? s * (float)(int8_t)two : 0.f, y = there ? s * (float)(int8_t)(two >> 8) : 0.f;
+            if (apart) reinterpret_cast<__nv_bfloat162*>(h)[i] = __floats2bfloat162_rn(x, y);
+            else h[i] = __floats2half2_rn(x, y);
         }
         return o;
     };
@@ -656,7 +674,7 @@ __global__ void __launch_bounds__(WIDENERS) widen_kernel(Widen w) {
 }  // namespace
 
 // The pages that a step's queries see (all keys, or a span of them: first_visible_key) as float16 numbers, and
-// float32 factors [n_seqs][2][n_kv] that keys and values are to be multiplied by.  out_pages 0: the outputs have the cache's shape; else
+// float32 factors [n_seqs][2][n_kv] that keys and values are to be multiplied by (keys' -1: bfloat16 numbers, as they are).  out_pages 0: the outputs have the cache's shape; else
 // they are [n_seqs * out_pages, ...], and a sequence's i-th page is that one's own (max_len / 64 rounded up or more).  Heads of
 // 64 or 128; max_len: no sequence is longer.
 RI_API int ri_quantized_widen(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, void* k_out, void* v_out, float* factors,

@@ -46,3 +46,30 @@ def attend_codes(q, keys, values, start, *, scale, window=0, chunk=0, float32):
             out[t, h] = w @ c
             bound[t, h] = slip * size + sums + (2.0 ** -22 if float32 else 2.0 ** -8) * out[t, h].abs()
     return out, bound
+
+
+def attend_pages(q, keys, values, start, *, scale, window=0, chunk=0, apart):
+    """The same for bfloat16 prompts, whose keys and values go by way of 16-bit pages: float16 numbers, 2^-11 relative and no finer than
+    2^-32 of the sequence's largest scale, and weights to 2^-11, no finer than 2^-31 of the row's largest; or, where scales lie
+    `apart`, all three to bfloat16's 2^-8."""
+    (kc, ks), (vc, vs) = keys, values
+    n, heads, hd = q.shape
+    rep = heads // kc.shape[1]
+    unit, page_floor, weight_floor = (2.0 ** -8, 0.0, 0.0) if apart else (2.0 ** -11, 2.0 ** -32, 2.0 ** -31)
+    out, bound = torch.zeros(n, heads, hd, dtype=torch.float64), torch.zeros(n, heads, hd, dtype=torch.float64)
+    for t in range(n):
+        pos = start + t
+        low = max(0, pos - window + 1) if window else 0
+        low = max(low, pos - pos % chunk) if chunk else low
+        for h in range(heads):
+            k = kc[low:pos + 1, h // rep] * ks[low:pos + 1, h // rep, None]
+            v = vc[low:pos + 1, h // rep] * vs[low:pos + 1, h // rep, None]
+            row = q[t, h]
+            score = k @ row * scale
+            p = torch.softmax(score, dim=0)
+            off = ((k.abs() @ row.abs()) * (1.01 * unit) + row.abs().sum() * page_floor * float(ks[:, h // rep].max())) * scale + score.abs() * 2.0 ** -20
+            slip = 2 * math.expm1(float(off.max())) + 2.05 * unit + (len(p) + 32) * 2.0 ** -23
+            out[t, h] = p @ v
+            bound[t, h] = (slip * (p @ v.abs()) + weight_floor * float(p.max()) * v.abs().sum(dim=0) + page_floor * float(vs[:, h // rep].max())
+                           + 2.0 ** -8 * out[t, h].abs())
+    return out, bound

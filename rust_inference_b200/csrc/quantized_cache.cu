@@ -726,14 +726,15 @@ RI_API int ri_quantized_write(void* src, int src_dtype, int ld, const float* bia
             if (src_dtype == RI_F32 && q_dtype == RI_BF16) return hd == 64 ? launch(write_one_kernel<float, B, 64>) : launch(write_one_kernel<float, B, 128>);
             if (src_dtype == RI_BF16 && q_dtype == RI_BF16) return hd == 64 ? launch(write_one_kernel<B, B, 64>) : launch(write_one_kernel<B, B, 128>);
         }
-        // A warp takes one q head, or two or four of the same rows (address arithmetic and the angles' reads are then shared): as few as
-        // keep the grid to what the SMs hold at once, four blocks each; two also where that keeps it to twice as much.  One, two and
-        // four, us, 32 heads over 8 of 128: 32 sequences of 1 token (384 blocks at one) 2.7, 2.8 and 3.1; 64 (768) 4.3, 3.1 and 3.8; 1,500 tokens
-        // (1,140) 8.3, 8.3 and 7.9; 2,047 (1,548) 11.7, 11.1 and 12.6; 8 times 2,047 83.6, 77.0 and 75.7.
+        // A warp takes one q head, or two or four of the same rows (address arithmetic and the angles' reads are then shared): one while the
+        // SMs hold the grid at once, four blocks each; two up to twice as much.  One, two and four, us (steps of one token are not here):
+        //   32 heads over 8 of 128:  16 sequences of 2 tokens (384 blocks at one) 2.3, 2.5, 2.9;  32 (768) 3.1, 2.8, 3.5;  64 (1,536) 5.2, 4.7, 4.7;
+        //     2,047 tokens (1,548) 12.6, 12.0, 13.6;  3 times 1,000 (2,304) 17.6, 16.7, 16.7;  8 times 2,047 (12,384) 83.5, 76.7, 75.5
+        //   28 over 4:  64 sequences of 5 (1,152) 4.7, 4.2, 4.7;  2,047 tokens (1,161) 9.3, 9.3, 9.8;  8 times 2,047 (9,288) 61.5, 56.0, 54.7
         const int kv_blocks = (2 * n_kv + HEADS - 1) / HEADS;
         const auto blocks_for = [&](int each) { return q_out ? (n_heads + HEADS * each - 1) / (HEADS * each) : 0; };
         const auto waves = [&](int each) { return (long long)runs * (kv_blocks + blocks_for(each)) / (4.f * sm_count()); };
-        const int q_each = waves(1) <= 1.f ? 1 : (waves(2) <= 1.f || (waves(2) <= 2.f && waves(4) > 1.f) ? 2 : 4);
+        const int q_each = waves(1) <= 1.f ? 1 : (waves(2) <= 2.f ? 2 : 4);
         const int q_blocks = blocks_for(q_each);
         const dim3 grid((unsigned)runs, (unsigned)(kv_blocks + q_blocks));
         auto launch = [&](auto kernel) {

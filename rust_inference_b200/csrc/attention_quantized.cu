@@ -30,11 +30,12 @@
 // in the order of the blocks, so that the result does not depend on who was last.  Where few items are short, each gets a cluster of
 // blocks instead, which add their parts up through distributed shared memory, a third of what meeting in memory takes.
 //
-// What it measures (32 heads over 8 of 128, bfloat16): 64 sequences of 128 to 2,048 keys 35.2 us, 4.2 TB/s of codes, 64% of what a copy
-// reaches; with the loads alone 31, without the joining of parts too 27.  2 sequences of about 30,000 keys (28 heads over 4) 23.7 us, of
-// which 14 for the loads and 8 for the two rounds of joining.  1 sequence of 1,024 keys 5.6 us, 3 of them until the first keys are there.  A
+// What it measures (32 heads over 8 of 128, bfloat16): 64 sequences of 128 to 2,048 keys 34.8 us, 4.3 TB/s of codes, 65% of what a copy
+// reaches; with the loads alone 31, without the joining of parts too 27.  2 sequences of about 30,000 keys (28 heads over 4) 22.7 us, of
+// which 14 for the loads and 8 for the two rounds of joining.  1 sequence of 1,024 keys 5.7 us, 3 of them until the first keys are there.  A
 // scheduler issues in 46% of its cycles and the tensor cores are busy in 19%: what bounds the large steps is how many loads are in flight
-// beside four blocks' arithmetic per SM (a second buffer for keys 38.0 us instead of 36.4, as blocks are then fewer).
+// beside four blocks' arithmetic per SM (a second buffer for keys and values 38.0 us instead of 36.4, as blocks are then fewer; one for keys
+// alone would leave four, and is not measured).
 //
 // Fragments come straight from 16-byte reads of shared memory, because the order of a contraction's terms, and which channel is which
 // row of a product, are free: lane (g, t) holds of the keys g and g + 8 the channels t HD/4 .. + HD/4, of its four keys (2t,

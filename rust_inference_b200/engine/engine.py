@@ -94,7 +94,8 @@ class Engine:
     def __init__(self, model: DecoderModel, *, max_tokens: int, max_seq_len: int | None = None,
                  n_slots: int | None = None, use_graphs: bool = True, cache_dtype=None):
         """cache_dtype: None, keys and values in the run dtype; "int8": 8-bit codes with a scale for every 16 positions of a kv
-        head (`kernels.quantized_cache`), half a bfloat16 cache's memory and reads.  Models with a layer that keeps something else
+        head (`kernels.quantized_cache`), half a bfloat16 cache's memory and, with heads of 64 or 128 and the plain form of the score,
+        half its reads.  Models with a layer that keeps something else
         (a latent, normalised or convolved heads, blended values) are refused."""
         self.model = model
         self.use_graphs = use_graphs and model.graph_safe()

@@ -84,8 +84,8 @@ def prefill(qkv: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, page_
 def prefill_half(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, factors: torch.Tensor, page_table, seq_slot, seq_start, cu_seqlens,
                  out: torch.Tensor, *, n_seqs: int, max_new: int, n_heads: int, n_kv_heads: int, head_dim: int, page_size: int, scale: float,
                  window: int = 0, out_scale: float = 1.0) -> torch.Tensor:
-    """`prefill` over pages of float16 numbers that are to be multiplied by a factor per sequence and kv head
-    (`quantized_cache.widen`); q and out are bfloat16."""
+    """`prefill` over pages of float16 numbers that are to be multiplied by a factor per sequence and kv head, or of bfloat16 ones in
+    their place where the keys' factor is -1 (`quantized_cache.widen`); q and out are bfloat16."""
     _need_cuda(q, k, v, factors, page_table, seq_slot, seq_start, cu_seqlens, out)
     _need(q.dtype == torch.bfloat16 and k.dtype == v.dtype == torch.float16 and out.dtype == torch.bfloat16 and q.is_contiguous()
           and k.is_contiguous() and v.is_contiguous() and out.is_contiguous() and v.shape == k.shape and out.shape[1] >= n_heads * head_dim

@@ -100,7 +100,8 @@ def read(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, page_t
 def widen(layer: QuantizedPages, k_out: torch.Tensor, v_out: torch.Tensor, factors: torch.Tensor, page_table: torch.Tensor, seq_slot,
           seq_start, seq_len, *, max_len: int, span: int = 0, out_pages: int = 0) -> None:
     """The pages that a step's queries see as float16 numbers for `attention_tc.prefill_half`: k_out, v_out float16 of the cache's
-    shape (or with out_pages for each sequence, as for `read`), and factors float32 [sequences, 2, kv heads] that keys and values are to be multiplied by.  What is outside a sequence's
+    shape (or with out_pages for each sequence, as for `read`), and factors float32 [sequences, 2, kv heads] that keys and values are to be multiplied by; where scales
+    lie too far apart for float16, the pages hold bfloat16 numbers instead and the keys' factor is -1.  What is outside a sequence's
     seen blocks is 0; a block that is no number is that in its keys."""
     what = "quantized_cache.widen"
     n_kv, hd, v_hd = layer.sizes

@@ -1,0 +1,61 @@
+// Microscaled numbers: 32 consecutive numbers of a row share a power of two, 2^e, whose exponent is kept as the byte e + 127, and each
+// is kept as the nearest number of a small type times 2^e (ties to the even one): four bits, +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}, or eight
+// (e4m3, up to 448).  e is the smallest exponent, -127 at least, for which nothing in the block exceeds the type's largest number times 2^e.
+// A block with an infinity or a NaN among its numbers has the byte 255 and stands for 32 NaNs.
+//
+// A matrix [n, k] of such numbers is held with k rounded up to whole `SPAN`s of 128, zeros behind a row's end: codes [n, span count * 128]
+// of a byte each, or of half a byte (number 2i in the low half of byte i), and exponents in the order in which the tensor cores' scale
+// registers take them: one piece of 512 bytes for every 128 rows and span, the exponent of row r and the span's block j (0..3) at
+// (r % 32) * 16 + r % 128 / 32 * 4 + j.  Pieces lie [row / 128][span].
+#pragma once
+
+#include "common.cuh"
+
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+
+namespace ri {
+namespace mx {
+
+constexpr int BLOCK = 32;              // numbers that share an exponent
+constexpr int SPAN = 128;              // numbers of a row that one step of a product takes
+constexpr int PIECE = 512;             // bytes of exponents of 128 rows and one span
+
+__host__ __device__ __forceinline__ int spans(int k) { return (k + SPAN - 1) / SPAN; }
+__device__ __forceinline__ size_t exponent_at(int row, int block, int n_spans) {
+    return ((size_t)(row >> 7) * n_spans + (block >> 2)) * PIECE + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+}
+
+// The exponent byte of a block whose largest magnitude has these bits (a float's, so that a NaN's are larger than any number's).  The
+// largest number of the type is 1.5 * 2^2 or 1.75 * 2^8.
+template <int BITS>
+__device__ __forceinline__ uint32_t exponent_byte(uint32_t largest) {
+    constexpr uint32_t MOST = BITS == 4 ? 0x400000u : 0x600000u, UP = BITS == 4 ? 2u : 8u;
+    const uint32_t e = largest >> 23;
+    if (e == 255u) return 255u;
+    const uint32_t want = e + ((largest & 0x7fffffu) > MOST ? 1u : 0u);
+    return e == 0u || want < UP ? 0u : want - UP;       // (a subnormal number is far below 2^-127 times the type's largest)
+}
+// 2^-e, which brings a block's numbers to the type (0 for the byte 255, whose codes say nothing)
+__device__ __forceinline__ float to_type(uint32_t byte) { return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23); }
+// 2^e
+__device__ __forceinline__ float from_type(uint32_t byte) {
+    return byte == 255u ? __uint_as_float(0x7fc00000u) : byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+}
+
+// The codes of eight numbers (already times 2^-e): a word of four bits each, two words of eight.
+__device__ __forceinline__ uint32_t four_bits(const float* y) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(y[2 * i], y[2 * i + 1]), __NV_E2M1, cudaRoundNearest) << (8 * i);
+    return w;
+}
+__device__ __forceinline__ uint32_t eight_bits(const float* y) {       // of four numbers
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3) |
+           (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+}
+__device__ __forceinline__ uint8_t eight_bits_of_one(float y) { return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3); }
+
+}  // namespace mx
+}  // namespace ri

@@ -17,6 +17,7 @@ class Workspace:
         self.device = torch.device(device)
         self._flat: dict = {}
         self._views: dict = {}        # (name, dtype) -> (shape, view): what was asked for last
+        self._rows: dict = {}         # name -> (codes, exponents, {(n, k): Rows over them})
 
     def get(self, name: str, shape, dtype: torch.dtype) -> torch.Tensor:
         key = (name, dtype)
@@ -47,6 +48,19 @@ class Workspace:
             flat = torch.zeros(max(n, 1), dtype=dtype, device=self.device)
             self._flat[key] = flat
         return flat[:n].view(*shape)
+
+    def rows(self, name: str, n: int, k: int):
+        """A buffer for rows [n, k] in microscaled 8 bits (`kernels.microscaled.Rows`), kept like the others."""
+        codes, exponents, made = self._rows.get(name, (None, None, None))
+        if made is not None and (n, k) in made:
+            return made[n, k]
+        from ..kernels.microscaled import Rows
+        a, b = (self.get(name + part, (size,), torch.uint8) for part, size in zip((":codes", ":exponents"), Rows.sizes(n, k)))
+        if made is None or a.data_ptr() != codes.data_ptr() or b.data_ptr() != exponents.data_ptr() or len(made) >= 256:
+            made = {}
+        made[n, k] = Rows(n, k, codes=a, exponents=b)
+        self._rows[name] = (a, b, made)
+        return made[n, k]
 
     def counting(self, n: int) -> torch.Tensor:
         """int32 0 .. n - 1, which nobody writes to."""

@@ -46,6 +46,8 @@ MODULES = {
     "quantized_cache": "quantized_cache.cu",
     "attention_quantized": "attention_quantized.cu",
     "token_logprobs": "token_logprobs.cu",
+    "microscaled": "microscaled.cu",
+    "gemm_microscaled": "gemm_microscaled.cu",
     "wait_probe": "wait_probe.cu",
     "host_runtime": "host_runtime.cpp",
     "native_calls": "native_calls.cpp",

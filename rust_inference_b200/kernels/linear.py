@@ -6,12 +6,14 @@ Which kernel runs is decided here, by dtype and shape:
             whole 16-byte pieces and sums not short (`_in_parts`), else the FFMA kernel (`gemm_simt`);
   bfloat16  the tcgen05 kernel (`gemm_tcgen05`) when the shape meets its alignment rule,
             else the FFMA kernel on bf16 operands.  Either way accumulation is float32.
+A matrix held in microscaled 4 bits (`microscaled.Matrix`) has kernels of its own (`gemm_microscaled`), for either dtype: x is then
+rows in 8 bits (`microscaled.Rows`), or plain rows that are brought to them, and what a product stores may be such rows too.
 """
 from __future__ import annotations
 
 import torch
 
-from . import ops, tcgen05
+from . import microscaled, ops, tcgen05
 from .attention import _sm_count
 
 
@@ -27,8 +29,12 @@ class Weight:
         self.tc = None
 
 
+def is_microscaled(w) -> bool:
+    return type(w) is microscaled.Matrix
+
+
 def _use_tensor_cores(x: torch.Tensor, w: Weight) -> bool:
-    if x.dtype != torch.bfloat16:
+    if is_microscaled(w) or x.dtype != torch.bfloat16:
         return False
     return tcgen05.supports(x, w)
 
@@ -63,6 +69,8 @@ on_tensor_cores = _use_tensor_cores      # for callers that choose their path by
 
 def project(x, w: Weight, out, ctx, bias=None):
     """out<run dtype> = x W^T + bias."""
+    if is_microscaled(w):
+        return microscaled.product(x, w, out, ctx, bias=bias)
     if _use_tensor_cores(x, w):
         return tcgen05.gemm(x, w, out, ops.EPI_STORE, ctx, bias=bias)
     return _plain(x, w, out, ops.EPI_STORE, ctx=ctx, bias=bias)
@@ -70,6 +78,10 @@ def project(x, w: Weight, out, ctx, bias=None):
 
 def logits(x, w: Weight, out, ctx, silu_cols=None):
     """out<float32> = x W^T; with silu_cols (float32 [1] on the device) the first so many columns through silu."""
+    if is_microscaled(w):
+        if silu_cols is not None:
+            raise ops.KernelError("a product with some columns through silu has no form for weights in 4 bits")
+        return microscaled.product(x, w, out, ctx)
     if silu_cols is not None:
         if _use_tensor_cores(x, w):
             return tcgen05.gemm(x, w, out, ops.EPI_SILU_F32, ctx, silu_cols=silu_cols)
@@ -81,6 +93,8 @@ def logits(x, w: Weight, out, ctx, silu_cols=None):
 
 def into_residual(x, w: Weight, residual, ctx):
     """residual<float32> += x W^T."""
+    if is_microscaled(w):
+        return microscaled.product(x, w, residual, ctx, add=True)
     if _use_tensor_cores(x, w):
         return tcgen05.gemm(x, w, residual, ops.EPI_RESIDUAL, ctx)
     return _plain(x, w, residual, ops.EPI_RESIDUAL, ctx=ctx)
@@ -90,6 +104,8 @@ def gated(x, w_gate: Weight, w_up: Weight, out, ctx, form=None):
     """out<run dtype> = silu(x Wg^T) * (x Wu^T); with `form` (`ops.gate_form`: float32 [5] on the device: alpha,
     limit, shift, cubic, mult) out = mult g' sigmoid(alpha g' (1 + cubic g'^2)) (u' + shift), g' = min(x Wg^T, limit),
     u' = clamp(x Wu^T, -limit, limit)."""
+    if is_microscaled(w_gate):
+        return microscaled.product(x, w_gate, out, ctx, w2=w_up, form=form)
     if _use_tensor_cores(x, w_gate):
         return tcgen05.gemm(x, w_gate, out, ops.EPI_SILU_MUL, ctx, w2=w_up, gate_form=form)
     return _plain(x, w_gate, out, ops.EPI_SILU_MUL, w_up, ctx=ctx, gate_form=form)
@@ -98,6 +114,8 @@ def gated(x, w_gate: Weight, w_up: Weight, out, ctx, form=None):
 def activated(x, w: Weight, out, ctx, form):
     """out<run dtype> = act(x W^T), an activation with its four constants `form` (float32 on the device: `ops.xielu`'s
     two learned numbers through `ops.whole_act_form`, or `ops.RELU_SQUARED_FORM`), applied to the float32 accumulators in the product's epilogue."""
+    if is_microscaled(w):
+        return microscaled.product(x, w, out, ctx, act=form)
     if _use_tensor_cores(x, w):
         return tcgen05.gemm(x, w, out, ops.EPI_ACT, ctx, act_form=form)
     return _plain(x, w, out, ops.EPI_ACT, ctx=ctx, act_form=form)

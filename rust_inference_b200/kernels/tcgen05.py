@@ -32,6 +32,10 @@ STATUS_TEXT = {
     34: "experts: a TMA load did not land before the CTA had to leave",
     41: "float32 product: the reading warps waited too long for a free stage",
     42: "float32 product: the MMA issuer waited too long for operands or for its accumulator",
+    51: "microscaled product: the TMA producer waited too long for a free stage",
+    52: "microscaled product: the MMA issuer waited too long for a copy or for its accumulator",
+    53: "microscaled product: the epilogue waited too long for the accumulator",
+    54: "microscaled product: a copy did not land before the CTA had to leave",
     43: "float32 product: the adding warps waited too long for the accumulator",
 }
 

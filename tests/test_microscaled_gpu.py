@@ -1,0 +1,240 @@
+"""Weights in microscaled 4 bits, rows in 8 and their products against 64-bit arithmetic.
+
+Tolerances.  What is held is exact: the nearest numbers, ties to even, bit for bit; float32 and bfloat16 hold them.  A norm is formed in
+64 bits and rounded once to 24 before it is rounded to 4 bits of mantissa, so a result is as near to the exact norm y as the nearest number,
+but for 2^-22 |y|.  A product's terms are exact (4 + 2 bits of mantissa, powers of two); the tensor cores add 32 of them, aligned, to a
+float32 sum, K / 32 times, each time off by at most a unit in the last place (2^-23) of what has been added up in magnitude, and a handful
+of pieces of K and a bias join the same way: (K / 32 + 16) 2^-23 sum |x w|, and half a step of the result's type."""
+import math
+
+import pytest
+import torch
+
+import plain_microscaled as plain
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def spread(n, k, seed, dtype=torch.float32, wide=6.0):
+    """Numbers whose blocks lie powers of two apart."""
+    g = gen(seed)
+    x = torch.randn(n, k, generator=g) * torch.exp2(wide * torch.randn(n, -(-k // 32), generator=g).repeat_interleave(32, 1)[:, :k])
+    return x.to(dtype)
+
+
+def context(dtype=torch.bfloat16):
+    from rust_inference_b200.engine.context import StepContext, Workspace
+    i = torch.zeros(2, dtype=torch.int32, device=DEV)
+    return StepContext(n_tokens=1, n_seqs=1, token_ids=i, token_pos=i, token_seq=i, seq_slot=i, seq_start=i, seq_len=i, cu_seqlens=i, logit_rows=i,
+                       n_logit_rows=0, max_new=1, max_len=1, all_single=True, page_table=i[None], page_size=64, dtype=dtype, device=i.device,
+                       workspace=Workspace(i.device))
+
+
+def check_status():
+    from rust_inference_b200.kernels import tcgen05
+    torch.cuda.synchronize()
+    tcgen05.check_status()
+
+
+SIZES = [(1, 1), (1, 31), (2, 32), (3, 33), (5, 127), (129, 128), (31, 129), (300, 1000), (257, 4096), (130, 2052)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,k", SIZES)
+def test_held_numbers_are_the_nearest(n, k, dtype):
+    from rust_inference_b200.kernels import microscaled
+    x = spread(n, k, 1000 * n + k, dtype)
+    for held, numbers in ((microscaled.Matrix.of(x.to(DEV)), plain.FOUR), (microscaled.quantize(x.to(DEV)), plain.EIGHT)):
+        want = plain.nearest(x, numbers)
+        for out in (torch.float32, torch.bfloat16):
+            got = microscaled.values(held, out)
+            assert got.dtype == out and torch.equal(got.double().cpu(), want)
+
+
+def test_ties_borders_and_numbers_that_are_none():
+    from rust_inference_b200.kernels import microscaled
+    rows = []
+    for numbers in (plain.FOUR, plain.EIGHT):
+        t = torch.tensor(numbers, dtype=torch.float64)
+        mid = (t[1:] + t[:-1]) / 2
+        for e in (0.0, -20.0, 50.0, -100.0):
+            for v in (t, mid, mid * (1 + 2.0 ** -20), mid * (1 - 2.0 ** -20)):
+                for part in (v * 2.0 ** e).split(31):
+                    row = torch.zeros(32, dtype=torch.float64)
+                    row[0] = numbers[-1] * 2.0 ** e                      # the type's largest: the power of two is 2^e
+                    row[1:1 + len(part)] = part
+                    rows += [row, -row]
+        for top in (numbers[-1] * (1 + 2.0 ** -23), numbers[-1], numbers[-1] * (1 - 2.0 ** -23)):
+            row = torch.full((32,), 0.3, dtype=torch.float64)
+            row[7] = top
+            rows.append(row)
+    rows += [torch.zeros(32).double(), torch.full((32,), 1e-45).double(), torch.full((32,), 2.0 ** -126).double(), torch.full((32,), 3.4e38).double(),
+             torch.arange(32).double() * 1e-40, torch.arange(32).double() * 2.0 ** -128]
+    for bad in (math.inf, -math.inf, math.nan):
+        row = torch.arange(32).double()
+        row[5] = bad
+        rows.append(row)
+    x = torch.stack(rows).float()
+    for held, numbers in ((microscaled.Matrix.of(x.to(DEV)), plain.FOUR), (microscaled.quantize(x.to(DEV)), plain.EIGHT)):
+        want, got = plain.nearest(x, numbers).float(), microscaled.values(held, torch.float32).cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+def test_rows_apart_and_off_a_boundary():
+    from rust_inference_b200.kernels import microscaled
+    for dtype in (torch.float32, torch.bfloat16):
+        wide = spread(70, 401, 3, dtype).to(DEV)
+        for x in (wide[:, :256], wide[:, 1:257], wide[3:, 100:399], wide[::2, :64], wide.t()):
+            want4, want8 = plain.nearest(x.cpu(), plain.FOUR), plain.nearest(x.cpu(), plain.EIGHT)
+            assert torch.equal(microscaled.values(microscaled.Matrix.of(x)).double().cpu(), want4)
+            if x.stride(1) == 1:
+                assert torch.equal(microscaled.values(microscaled.quantize(x)).double().cpu(), want8)
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (3, 63), (130, 257), (256, 384)])
+def test_matrix_from_a_files_codes(n, k):
+    from rust_inference_b200.kernels import microscaled
+    x = spread(n, k, 5)
+    want = plain.nearest(x, plain.FOUR)
+    codes, exponents = plain.codes_of(want, k)
+    if k % 2:
+        codes[:, -1] |= 0x70                                # what lies behind a row's end says nothing
+    m = microscaled.Matrix.of_codes(codes.to(DEV), exponents.to(DEV), k)
+    assert torch.equal(microscaled.values(m).double().cpu(), want)
+    other = microscaled.Matrix.of(want.float().to(DEV))    # the same rule on the same numbers (3.2 becomes 3, which is 6 times half as much)
+    assert torch.equal(m.exponents, other.exponents) and torch.equal(m.codes, other.codes)
+
+
+@pytest.mark.parametrize("branch", [None, torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,k", [(1, 1), (1, 31), (2, 896), (9, 1333), (3, 4096), (5, 8960), (2, 18944), (700, 260)])
+def test_norm(n, k, branch):
+    from rust_inference_b200.kernels import microscaled
+    g = gen(n * k)
+    x = 3 * torch.randn(n, k, generator=g) + 0.5
+    b = None if branch is None else torch.randn(n, k, generator=g).to(branch)
+    w = 1 + 0.2 * torch.randn(k, generator=g)
+    want_total, y = plain.rmsnorm(x, b, w, 1e-5)
+    near = plain.nearest(y, plain.EIGHT)
+    rows = microscaled.Rows(n, k)
+    for total in ("none", "other", "same"):
+        xd = x.to(DEV)
+        to = {"none": None, "other": torch.full_like(xd, math.nan), "same": xd}[total]
+        microscaled.rmsnorm(xd, w.to(DEV), 1e-5, rows, branch=None if b is None else b.to(DEV), total=to)
+        if to is not None:
+            assert torch.equal(to.cpu(), want_total)
+        got = microscaled.values(rows).double().cpu()
+        assert ((got - y).abs() <= (near - y).abs() + 2.0 ** -22 * y.abs()).all()
+
+
+def exact_product(x, w):
+    """x W^T and the sum of its terms' magnitudes, 64 bits."""
+    x, w = plain.nearest(x, plain.EIGHT).to(DEV), plain.nearest(w, plain.FOUR).to(DEV)
+    return x @ w.t(), x.abs() @ w.abs().t()
+
+
+def bound(k, mass, y, dtype):
+    return (k / 32 + 16) * 2.0 ** -23 * mass + HALF_STEP[dtype] * y.abs()
+
+
+PRODUCTS = [(1, 1, 1), (1, 128, 128), (2, 130, 64), (1, 896, 896), (7, 1000, 1333), (8, 3584, 3584), (16, 257, 2048), (17, 640, 384), (33, 129, 4097),
+            (64, 2560, 2048), (61, 300, 8960), (100, 129, 640), (127, 1152, 896), (128, 256, 512), (129, 200, 300), (200, 5000, 256), (333, 2560, 2048),
+            (1000, 640, 1536), (3, 40000, 160), (5, 128, 18944)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_product(m, n, k, dtype):
+    from rust_inference_b200.kernels import linear, microscaled
+    ctx = context(dtype)
+    x, w = spread(m, k, 11 * m + k, dtype, 1.0), spread(n, k, 13 * n + k, wide=1.0)
+    b = torch.randn(n, generator=gen(n)).to(DEV)
+    y, mass = exact_product(x, w)
+    held = microscaled.Matrix.of(w.to(DEV))
+    xd = x.to(DEV)
+    for bias in (None, b):
+        out = torch.full((m, n), math.nan, dtype=dtype, device=DEV)
+        linear.project(xd, held, out, ctx, bias=bias)
+        want = y if bias is None else y + bias.double()
+        assert ((out.double() - want).abs() <= bound(k, mass + (0 if bias is None else bias.double().abs()), want, dtype)).all()
+    start = torch.randn(m, n, generator=gen(m)).to(DEV)
+    out = start.clone()
+    linear.into_residual(microscaled.quantize(xd), held, out, ctx)
+    want = y + start.double()
+    assert ((out.double() - want).abs() <= bound(k, mass + start.double().abs(), want, torch.float32)).all()
+    again = start.clone()
+    linear.into_residual(xd, held, again, ctx)
+    assert torch.equal(out, again)
+    check_status()
+
+
+@pytest.mark.parametrize("form", [None, "bounded"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 4864, 896), (8, 1000, 1333), (9, 18944, 256), (16, 300, 2048), (31, 640, 640), (64, 1100, 512), (100, 256, 2048),
+                                   (128, 700, 300), (129, 200, 300), (333, 1500, 640), (700, 129, 1000)])
+def test_gated_and_into_eight_bits(m, n, k, form):
+    from rust_inference_b200.kernels import linear, microscaled, ops
+    ctx = context()
+    x = spread(m, k, 3 * m + k, wide=0.5)
+    wg, wu = (spread(n, k, s + n + k, wide=0.5) / math.sqrt(k) for s in (1, 2))
+    f = None if form is None else ops.gate_form(alpha=1.702, limit=1.5, shift=1.0, device=DEV)
+    g, gm = exact_product(x, wg)
+    u, um = exact_product(x, wu)
+    want = plain.gate(g, u, f)
+    # gate and up are off by so much, and the gate's slope is 1.1 at most in size (alpha = 1.702: 1.1 too); a few units in the last place of float32 beside it
+    eg, eu = ((k / 32 + 16) * 2.0 ** -23 * v for v in (gm, um))
+    up = u.abs() + 1 if f is not None else u.abs()
+    off = 1.2 * eg * (up + eu) + g.abs() * eu + 2.0 ** -20 * (g.abs() * up)
+    held = [microscaled.Matrix.of(w.to(DEV)) for w in (wg, wu)]
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.full((m, n), math.nan, dtype=dtype, device=DEV)
+        linear.gated(x.to(DEV), *held, out, ctx, form=f)
+        assert ((out.double() - want).abs() <= off + HALF_STEP[dtype] * want.abs() * 1.01).all()
+    rows = microscaled.Rows(m, n)
+    rows.codes.fill_(255)
+    linear.gated(x.to(DEV), *held, rows, ctx, form=f)
+    got = microscaled.values(rows).double()
+    # a block's step follows its largest number: half a step is 2^-4 of a number, or 2^-10 times 2^e, which is at most the block's largest / 224
+    near = plain.nearest(want.cpu(), plain.EIGHT).to(DEV)
+    wide = torch.nn.functional.pad(want.abs() + off, (0, -n % 32)).view(m, -1, 32).amax(dim=2, keepdim=True).expand(-1, -1, 32).reshape(m, -1)[:, :n]
+    assert ((got - want).abs() <= torch.maximum(2.0 ** -4 * want.abs(), 2.0 ** -10 * wide / 224) + off * 1.1).all()
+    assert float((got != near).double().mean()) < 0.01
+    # behind a row's end there are zeros, for the next product
+    if n % 128:
+        assert not rows.codes.view(m, -1)[:, n:].any()
+    # and the next product reads them as they lie
+    wd = spread(200, n, 9, wide=0.5)
+    down = microscaled.Matrix.of(wd.to(DEV))
+    out = torch.empty(m, 200, dtype=torch.float32, device=DEV)
+    linear.project(rows, down, out, ctx)
+    w8 = plain.nearest(wd, plain.FOUR).to(DEV)
+    y, mass = got @ w8.t(), got.abs() @ w8.abs().t()
+    assert ((out.double() - y).abs() <= bound(n, mass, y, torch.float32)).all()
+    check_status()
+
+
+@pytest.mark.parametrize("m", [1, 9, 130, 600])
+def test_activated(m):
+    from rust_inference_b200.kernels import linear, microscaled, ops
+    ctx = context()
+    x, w = spread(m, 500, m, wide=0.5), spread(390, 500, 77, wide=0.5) / 20
+    form = torch.tensor(ops.RELU_SQUARED_FORM, dtype=torch.float32, device=DEV)
+    y, mass = exact_product(x, w)
+    want = y.clamp(min=0) ** 2
+    off = (500 / 32 + 16) * 2.0 ** -23 * mass
+    off = 2 * off * (y.abs() + off) + 2.0 ** -21 * want
+    held = microscaled.Matrix.of(w.to(DEV))
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.full((m, 390), math.nan, dtype=dtype, device=DEV)
+        linear.activated(x.to(DEV), held, out, ctx, form)
+        assert ((out.double() - want).abs() <= off + HALF_STEP[dtype] * want * 1.01).all()
+    rows = microscaled.Rows(m, 390)
+    linear.activated(x.to(DEV), held, rows, ctx, form)
+    got = microscaled.values(rows).double()
+    assert float((got != plain.nearest(want.cpu(), plain.EIGHT).to(DEV)).double().mean()) < 0.01
+    check_status()

@@ -399,6 +399,284 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 }
 
 // ---------------------------------------------------------------------------------------------
+// Many tokens, on pairs of SMs (tcgen05 cta_group::2).  A tile is 256 tokens x 256 rows of W: 256 features, or the gate rows of 128 and the up
+// rows of the same.  Each CTA of the pair holds 128 of the tokens (its half of A and of the accumulator) and 128 of the rows of W (its half of
+// B, which the tensor cores of both read), and the exponents of its tokens and of all the rows of W.  The first CTA issues the MMAs.
+//
+// Two accumulators of 256 columns would leave tensor memory no room for exponents, so the second begins 32 columns before the first ends: an
+// epilogue reads the columns that both use first, and says so, and then the MMAs of the next tile may begin.
+// ---------------------------------------------------------------------------------------------
+constexpr int PAIR_TOK = 2 * ROWS, PAIR_ROWS = 2 * ROWS;
+constexpr int PAIR_EXP = 3 * PIECE;                    // exponents of a stage: 128 tokens, 256 rows of W
+constexpr int PAIR_STAGE = 2 * TILE + PAIR_EXP;
+constexpr int SECOND_ACC = 224, PAIR_EXP_COL = 480;    // columns: accumulators [0, 256) and [224, 480), two sets of exponents behind them
+
+__device__ __forceinline__ uint32_t in_first_cta(uint32_t local_addr) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(local_addr));
+    return a;
+}
+// A tile into this CTA's shared memory whose arrival is counted by a barrier of the pair's first CTA.
+__device__ __forceinline__ void load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t leader, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+        ::"r"(bar), "h"((uint16_t)3), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    tmem_ld16(taddr, r);
+    tmem_ld16(taddr + 16, r + 16);
+}
+
+// 32 features of a token, from feature f on, as this thread has computed them.
+template <int OUT>
+__device__ __forceinline__ void store_run(const Result& r, int t, int f, int n_feat, bool aligned, const float* v) {
+    if (OUT == OUT_ROWS) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) top = max(top, f + j < n_feat ? __float_as_uint(v[j]) & 0x7fffffffu : 0u);
+        const uint32_t byte = exponent_byte<8>(top);
+        const float by = to_type(byte);
+        uint4 c[2];
+        uint32_t* w = reinterpret_cast<uint32_t*>(c);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = f + 4 * q + j < n_feat ? v[4 * q + j] * by : 0.f;
+            w[q] = eight_bits(y);
+        }
+        uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(r.out) + (size_t)t * r.n_spans * SPAN + f);
+        to[0] = c[0];
+        to[1] = c[1];
+        r.exponents[exponent_at(t, f >> 5, r.n_spans)] = (uint8_t)byte;
+        return;
+    }
+    const size_t at = (size_t)t * n_feat + f;
+    if (aligned && f + 32 <= n_feat) {
+        if (OUT == OUT_BF16) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(r.out) + at)[q] = pack8(v + 8 * q);
+        } else {
+            float* to = reinterpret_cast<float*>(r.out) + at;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                if (OUT == OUT_ADD)
+                    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to + 4 * q), "f"(v[4 * q]), "f"(v[4 * q + 1]),
+                                 "f"(v[4 * q + 2]), "f"(v[4 * q + 3]) : "memory");
+                else
+                    reinterpret_cast<float4*>(to)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+        if (f + j < n_feat) {
+            if (OUT == OUT_BF16) reinterpret_cast<__nv_bfloat16*>(r.out)[at + j] = __float2bfloat16_rn(v[j]);
+            else if (OUT == OUT_F32) reinterpret_cast<float*>(r.out)[at + j] = v[j];
+            else atomicAdd(reinterpret_cast<float*>(r.out) + at + j, v[j]);
+        }
+}
+
+template <bool DUAL, int OUT>
+__global__ void __launch_bounds__(THREADS, 1)
+mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const __grid_constant__ CUtensorMap map_x,
+               const __grid_constant__ CUtensorMap map_we, const __grid_constant__ CUtensorMap map_we2, const __grid_constant__ CUtensorMap map_xe,
+               const float* __restrict__ constants, int act, Result res, int n_tok, int n_feat, int n_spans, int stages, int* status) {
+    constexpr int FEATS = DUAL ? PAIR_ROWS / 2 : PAIR_ROWS;    // features of a tile
+    constexpr uint32_t IDESC = instruction(PAIR_TOK, PAIR_ROWS, 0, 5);
+    constexpr uint32_t CTA_TX = TILE + W_COPIED + PAIR_EXP;    // bytes of a stage that a CTA's copies count
+
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[MAX_STAGES];     // used in the first CTA only
+    __shared__ __align__(8) uint64_t empty_bar[MAX_STAGES];
+    __shared__ __align__(8) uint64_t acc_full[2];
+    __shared__ __align__(8) uint64_t next_bar;                 // first CTA: the epilogues have read the columns that the next tile writes too
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ volatile int abort_flag;
+
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t exp_base = smem_base + (uint32_t)stages * 2 * TILE;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();                      // 0: issues the MMAs
+    const int pair = (int)blockIdx.x >> 1, n_pairs = (int)gridDim.x >> 1;
+    const int n_tok_tiles = (n_tok + PAIR_TOK - 1) / PAIR_TOK, n_feat_tiles = (n_feat + FEATS - 1) / FEATS;
+    const int total_tiles = n_tok_tiles * n_feat_tiles;
+    const int my_tiles = (pair < total_tiles) ? (total_tiles - 1 - pair) / n_pairs + 1 : 0;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&empty_bar[s]), 1);
+        }
+        for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&acc_full[i]), 1);
+        mbar_init(smem_u32(&next_bar), 8);                     // one arrival per epilogue warp of the pair
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    cluster_sync();                                        // the partner's barriers stand before anything arrives there
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_base_slot;
+    const uint32_t full0 = smem_u32(&full_bar[0]), empty0 = smem_u32(&empty_bar[0]);
+    const uint32_t full0_first = in_first_cta(full0);
+    let_next_kernel_start();
+
+    // token tiles vary fastest, so that pairs which run together share the rows of W in L2
+    auto tile_coords = [&](int i, int& f0, int& t0) {
+        const int item = pair + i * n_pairs;
+        t0 = (item % n_tok_tiles) * PAIR_TOK;
+        f0 = (item / n_tok_tiles) * FEATS;
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0, s = 0;
+            uint32_t ph = 0;
+            bool alive = true;
+            wait_for_previous_kernels();                         // the rows come from the kernel before
+            const CUtensorMap* my_w = (DUAL && rank == 1) ? &map_w2 : &map_w;
+            const CUtensorMap* second_we = DUAL ? &map_we2 : &map_we;
+            const int w_off = DUAL ? 0 : rank * ROWS;
+            for (int i = 0; i < my_tiles && alive; ++i) {
+                int f0, t0;
+                tile_coords(i, f0, t0);
+                if (abort_flag) break;
+                // pieces of exponents: a row of a map each (beyond the last one: zeros)
+                const int xe = (t0 / ROWS + rank) * n_spans, we = (f0 / ROWS) * n_spans, we2 = DUAL ? we : we + n_spans;
+                for (int j = 0; j < n_spans; ++j, ++it) {
+                    if (!mbar_wait(empty0 + 8u * s, ph ^ 1u)) {
+                        if (!abort_flag) report(status, ST_PRODUCER_TIMEOUT);
+                        abort_flag = 1;
+                        alive = false;
+                        break;
+                    }
+                    const uint32_t stage = smem_base + (uint32_t)s * 2 * TILE, ex = exp_base + (uint32_t)s * PAIR_EXP, bar = full0_first + 8u * s;
+                    if (rank == 0) mbar_expect_tx(full0 + 8u * s, 2 * CTA_TX);                 // both CTAs' bytes
+                    load_2d_pair(stage, &map_x, bar, j * SPAN, t0 + rank * ROWS);
+                    load_2d_pair(stage + TILE, my_w, bar, j * SPAN, f0 + w_off);
+                    load_2d_pair(ex, &map_xe, bar, 0, xe + j);
+                    load_2d_pair(ex + PIECE, &map_we, bar, 0, we + j);
+                    load_2d_pair(ex + 2 * PIECE, second_we, bar, 0, we2 + j);
+                    if (++s == stages) { s = 0; ph ^= 1u; }
+                }
+            }
+            // Do not leave while a copy into this CTA's shared memory may still be in flight: a stage whose `empty` barrier has completed
+            // again was read by the MMAs, so its copies had landed.
+            for (int j = 0; j < stages && it > 0; ++j) {
+                if (!mbar_wait(empty0 + 8u * s, ph ^ 1u)) {
+                    report(status, ST_DRAIN_TIMEOUT);
+                    break;
+                }
+                if (++s == stages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {                                         // the whole warp goes through, one lane issues
+            const uint32_t leader = elect_one();
+            int s = 0;
+            uint32_t ph = 0;
+            bool alive = true;
+            const uint64_t desc_x0 = make_smem_desc(smem_base), desc_e0 = piece_desc(exp_base);
+            for (int i = 0; i < my_tiles && alive; ++i) {
+                // the columns that the tile before shares have been read, and with them all of the one before that
+                if (i > 0 && !mbar_wait_warp(smem_u32(&next_bar), (uint32_t)(i - 1) & 1u)) {
+                    if (lane == 0) report(status, ST_MMA_TIMEOUT);
+                    abort_flag = 1;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t acc = tmem_base + (uint32_t)((i & 1) * SECOND_ACC);
+                for (int j = 0; j < n_spans; ++j) {
+                    if (!mbar_wait_warp(full0 + 8u * s, ph)) {
+                        if (lane == 0) report(status, ST_MMA_TIMEOUT);
+                        abort_flag = 1;
+                        alive = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t ex = tmem_base + (uint32_t)(PAIR_EXP_COL + (j & 1) * 16);
+                    const uint64_t e = desc_e0 + (uint64_t)((uint32_t)s * (PAIR_EXP >> 4));
+#pragma unroll
+                    for (int m = 0; m < 3; ++m) exponents_to_tmem<1>(leader, ex + 4 * m, e + (uint64_t)(m * (PIECE >> 4)));
+                    const uint64_t x = desc_x0 + (uint64_t)((uint32_t)s * (2 * TILE >> 4)), w = x + (TILE >> 4);
+#pragma unroll
+                    for (int b = 0; b < SPAN / BLOCK; ++b)
+                        mx_mma<1>(leader, acc, x + 2 * b, w + 2 * b, of_block(IDESC, b), ex, ex + 4, j > 0 || b > 0);
+                    commit_pair(leader, empty0 + 8u * s);                // frees the stage in both CTAs
+                    if (++s == stages) { s = 0; ph ^= 1u; }
+                }
+                commit_pair(leader, smem_u32(&acc_full[i & 1]));
+            }
+        }
+    } else {
+        // a thread has a token, and 32 of its features at a time
+        const int lane_base = (warp & 3) * 32;
+        const uint32_t next_first = in_first_cta(smem_u32(&next_bar));
+        wait_for_previous_kernels();
+        const Epilogue e = load_epilogue<DUAL>(constants, act);
+        const bool aligned = OUT == OUT_BF16 ? n_feat % 8 == 0 : n_feat % 4 == 0;
+        for (int i = 0; i < my_tiles; ++i) {
+            int f0, t0;
+            tile_coords(i, f0, t0);
+            const bool landed = mbar_wait(smem_u32(&acc_full[i & 1]), (uint32_t)(i >> 1) & 1u);
+            if (!landed) {
+                if (lane == 0) report(status, ST_EPILOGUE_TIMEOUT);
+                abort_flag = 1;
+            }
+            tc_fence_after();
+            __syncwarp();
+            if (__any_sync(0xffffffffu, !landed || abort_flag)) break;
+            const int t = t0 + rank * ROWS + lane_base + lane;
+            const uint32_t trow = tmem_base + ((uint32_t)lane_base << 16) + (uint32_t)((i & 1) * SECOND_ACC);
+            constexpr int RUNS = FEATS / 32;
+#pragma unroll 1
+            for (int n = 0; n < RUNS; ++n) {
+                // the first accumulator shares its last columns, the second its first
+                const int c = ((i & 1) ? n : RUNS - 1 - n) * 32, f = f0 + c;
+                float v[32], u[DUAL ? 32 : 1];
+                tmem_ld32(trow + c, reinterpret_cast<uint32_t*>(v));
+                if (DUAL) tmem_ld32(trow + ROWS + c, reinterpret_cast<uint32_t*>(u));
+                tmem_wait_ld();
+                if (n == 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_cluster(next_first);
+                }
+                if (f >= (OUT == OUT_ROWS ? res.n_spans * SPAN : n_feat) || t >= n_tok) continue;
+                const bool biased = !DUAL && !e.act && OUT != OUT_ADD && e.constants != nullptr;
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    v[j] = result<DUAL, OUT>(v[j], DUAL ? u[j] : 0.f, biased && f + j < n_feat ? e.constants[f + j] : 0.f, e);
+                store_run<OUT>(res, t, f, n_feat, aligned, v);
+            }
+        }
+    }
+
+    // nothing of the pair's tensor or shared memory is freed while the partner may still use it
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
 // Codes as a tensor map with a box of a span and `box_rows` rows, 128-byte swizzle, zeros outside: of 8 bits, or of 4 that are spread.
@@ -416,8 +694,28 @@ int encode_codes(CUtensorMap* map, const void* ptr, long long rows, int n_spans,
     return 0;
 }
 
+// Exponents as a tensor map whose rows are pieces.
+int encode_pieces(CUtensorMap* map, const void* ptr, long long pieces) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail("gemm_microscaled: cuTensorMapEncodeTiled is not available from the driver");
+    if ((uintptr_t)ptr % 16) return fail("gemm_microscaled: exponents must begin on a 16-byte boundary");
+    cuuint64_t dims[2] = {PIECE / 4, (cuuint64_t)pieces};
+    cuuint64_t strides[1] = {PIECE};
+    cuuint32_t box[2] = {PIECE / 4, 1};
+    cuuint32_t elem[2] = {1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail("gemm_microscaled: cuTensorMapEncodeTiled failed for exponents (code %d)", (int)r);
+    return 0;
+}
+
+// The tensor maps that a matrix or rows keep: of the codes, and of the exponents.
+struct Maps {
+    CUtensorMap codes, exponents;
+};
+
 struct Call {
-    const CUtensorMap *w, *w2, *x;
+    const Maps *w, *w2, *x;
     const uint8_t *w_exp, *w2_exp, *x_exp;
     const float* constants;
     int act;
@@ -429,12 +727,21 @@ struct Call {
 
 int columns(int need) { return need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512; }
 
-// How the first kernel cuts a product: tokens of a tile and CTAs of a cluster.
+// How a product is cut: on pairs of SMs, or into tiles of tn tokens with K over the CTAs of a cluster.
 struct Plan {
+    bool pairs;
     int tn, cluster;
 };
+int g_pair_tokens = 256;         // products of at least so many tokens run on pairs of SMs
+
 Plan plan(int n_tok, int n_feat, int n_spans) {
     Plan p;
+    p.pairs = n_tok >= g_pair_tokens;
+    if (p.pairs) {
+        p.tn = ROWS;
+        p.cluster = 1;
+        return p;
+    }
     p.tn = n_tok >= TOKENS_MOST ? TOKENS_MOST : (n_tok + 15) / 16 * 16;
     p.cluster = 1;
     const long long tiles = (long long)((n_feat + ROWS - 1) / ROWS);
@@ -469,26 +776,58 @@ int launch_feature(const Call& c) {
     // CTAs that wait for others of their cluster must not wait for tensor memory that CTAs of another cluster hold, which may wait likewise:
     // shared memory in proportion to their columns keeps all that an SM takes in within its 512 columns.
     if (p.cluster > 1 && smem < (size_t)cols * 456) smem = (size_t)cols * 456 < SMEM_LIMIT ? (size_t)cols * 456 : SMEM_LIMIT;
-    return launch_cluster("gemm_microscaled", kernel, dim3((unsigned)ctas), THREADS, smem, p.cluster, c.stream, *c.w, *c.w2, *c.x, c.w_exp, c.w2_exp, c.x_exp,
+    return launch_cluster("gemm_microscaled", kernel, dim3((unsigned)ctas), THREADS, smem, p.cluster, c.stream, c.w->codes, c.w2->codes, c.x->codes, c.w_exp, c.w2_exp, c.x_exp,
                           c.constants, c.act, c.res, c.n_tok, c.n_feat, c.n_spans, p.cluster, stages, p.tn, buffers, cols, c.status);
+}
+
+template <bool DUAL, int OUT>
+int launch_pair(const Call& c) {
+    constexpr int FEATS = DUAL ? PAIR_ROWS / 2 : PAIR_ROWS;
+    const long long tiles = (long long)((c.n_tok + PAIR_TOK - 1) / PAIR_TOK) * ((c.n_feat + FEATS - 1) / FEATS);
+    if (tiles > 0x7fffffffLL) return fail("gemm_microscaled: %lld tiles exceed the index range", tiles);
+    auto kernel = mx_pair_kernel<DUAL, OUT>;
+    static PerDeviceOnce configured;
+    if (int rc = raise_dynamic_smem(kernel, SMEM_LIMIT, configured, "gemm_microscaled")) return rc;
+    constexpr int STAGES = (SMEM_LIMIT - 1024) / PAIR_STAGE;
+    static_assert(STAGES <= MAX_STAGES && STAGES >= 2, "a ring of stages");
+    long long pairs = sm_count() / 2;
+    if (pairs > tiles) pairs = tiles;
+    return launch_cluster("gemm_microscaled (pairs of SMs)", kernel, dim3((unsigned)(2 * pairs)), THREADS, (size_t)STAGES * PAIR_STAGE + 1024, 2, c.stream,
+                          c.w->codes, c.w2->codes, c.x->codes, c.w->exponents, c.w2->exponents, c.x->exponents, c.constants, c.act, c.res, c.n_tok, c.n_feat,
+                          c.n_spans, STAGES, c.status);
+}
+
+template <bool DUAL, int OUT>
+int launch(const Call& c) {
+    return plan(c.n_tok, c.n_feat, c.n_spans).pairs ? launch_pair<DUAL, OUT>(c) : launch_feature<DUAL, OUT>(c);
 }
 
 }  // namespace
 
-// The tensor map of codes [rows, spans * 128] of `bits` (4 or 8) bits, into the 128 bytes at `map_out` (64-byte aligned).  box_rows: 128 for
-// a matrix, `ri_mx_box` for rows.
-RI_API int ri_mx_encode(void* map_out, const void* ptr, long long rows, int n_spans, int bits, int box_rows) {
-    if ((uintptr_t)map_out % 64) return fail("gemm_microscaled: tensor map storage must be 64-byte aligned");
+// The tensor maps of codes [rows, spans * 128] of `bits` (4 or 8) bits and of their exponents, into the 256 bytes at `maps_out` (64-byte
+// aligned).  box_rows: 128 for a matrix, `ri_mx_box` for rows.
+RI_API int ri_mx_encode(void* maps_out, const void* codes, const void* exponents, long long rows, int n_spans, int bits, int box_rows) {
+    if ((uintptr_t)maps_out % 64) return fail("gemm_microscaled: tensor map storage must be 64-byte aligned");
     if (rows <= 0 || n_spans <= 0 || (bits != 4 && bits != 8) || box_rows < 8 || box_rows > 256)
         return fail("gemm_microscaled: no map of [%lld, %d] in %d bits with boxes of %d rows", rows, n_spans, bits, box_rows);
-    return encode_codes(reinterpret_cast<CUtensorMap*>(map_out), ptr, rows, n_spans, bits, box_rows);
+    const long long pieces = (rows + ROWS - 1) / ROWS * n_spans;
+    if (pieces > 0x7fffffffLL) return fail("gemm_microscaled: %lld pieces of exponents exceed the index range", pieces);
+    Maps* maps = reinterpret_cast<Maps*>(maps_out);
+    if (int rc = encode_codes(&maps->codes, codes, rows, n_spans, bits, box_rows)) return rc;
+    return encode_pieces(&maps->exponents, exponents, pieces);
+}
+
+// Products of at least so many tokens run on pairs of SMs (for comparisons and tests).
+RI_API int ri_mx_set_pairs(int tokens) {
+    g_pair_tokens = tokens;
+    return 0;
 }
 
 // Rows of the box of a product's X.
 RI_API int ri_mx_box(int n_tok, int n_feat, int n_spans) { return plan(n_tok, n_feat, n_spans).tn; }
 
 // `kind`: what is written (`Out`); `dual`: gated, with the second matrix; `act`: `constants` are an activation's.  out_exp, out_spans: with rows in 8 bits.
-RI_API int ri_mx_gemm(const void* map_w, const void* map_w2, const void* map_x, const void* w_exp, const void* w2_exp, const void* x_exp,
+RI_API int ri_mx_gemm(const void* maps_w, const void* maps_w2, const void* maps_x, const void* w_exp, const void* w2_exp, const void* x_exp,
                       const float* constants, int dual, int act, int kind, void* out, void* out_exp, int out_spans, int n_tok, int n_feat, int n_spans,
                       int* status, cudaStream_t stream) {
     if (n_tok <= 0 || n_feat <= 0) return 0;
@@ -496,9 +835,9 @@ RI_API int ri_mx_gemm(const void* map_w, const void* map_w2, const void* map_x, 
     if (kind < OUT_BF16 || kind > OUT_ADD || (dual && act) || (kind == OUT_ADD && (dual || act || constants != nullptr)) || (act && constants == nullptr))
         return fail("gemm_microscaled: no epilogue %d (gated %d, activated %d)", kind, dual, act);
     Call c;
-    c.w = reinterpret_cast<const CUtensorMap*>(map_w);
-    c.w2 = reinterpret_cast<const CUtensorMap*>(dual ? map_w2 : map_w);
-    c.x = reinterpret_cast<const CUtensorMap*>(map_x);
+    c.w = reinterpret_cast<const Maps*>(maps_w);
+    c.w2 = reinterpret_cast<const Maps*>(dual ? maps_w2 : maps_w);
+    c.x = reinterpret_cast<const Maps*>(maps_x);
     c.w_exp = (const uint8_t*)w_exp;
     c.w2_exp = (const uint8_t*)w2_exp;
     c.x_exp = (const uint8_t*)x_exp;
@@ -512,16 +851,16 @@ RI_API int ri_mx_gemm(const void* map_w, const void* map_w2, const void* map_x, 
     c.stream = stream;
     if (dual) {
         switch (kind) {
-            case OUT_BF16: return launch_feature<true, OUT_BF16>(c);
-            case OUT_F32: return launch_feature<true, OUT_F32>(c);
-            default: return launch_feature<true, OUT_ROWS>(c);
+            case OUT_BF16: return launch<true, OUT_BF16>(c);
+            case OUT_F32: return launch<true, OUT_F32>(c);
+            default: return launch<true, OUT_ROWS>(c);
         }
     }
     switch (kind) {
-        case OUT_BF16: return launch_feature<false, OUT_BF16>(c);
-        case OUT_F32: return launch_feature<false, OUT_F32>(c);
-        case OUT_ROWS: return launch_feature<false, OUT_ROWS>(c);
-        default: return launch_feature<false, OUT_ADD>(c);
+        case OUT_BF16: return launch<false, OUT_BF16>(c);
+        case OUT_F32: return launch<false, OUT_F32>(c);
+        case OUT_ROWS: return launch<false, OUT_ROWS>(c);
+        default: return launch<false, OUT_ADD>(c);
     }
 }
 

@@ -40,9 +40,9 @@ def _here(what: str, *tensors) -> None:
             raise KernelError(f"{what}: a tensor that is not on the current CUDA device; this library has no CPU path")
 
 
-def _encode(codes: torch.Tensor, rows: int, spans: int, bits: int, box: int) -> torch.Tensor:
-    m = torch.empty(128, dtype=torch.uint8)           # CPU allocations are 64-byte aligned
-    _call("gemm_microscaled", "ri_mx_encode", c_void_p(m.data_ptr()), _p(codes), c_longlong(rows), c_int(spans), c_int(bits), c_int(box))
+def _encode(codes: torch.Tensor, exponents: torch.Tensor, rows: int, spans: int, bits: int, box: int) -> torch.Tensor:
+    m = torch.empty(256, dtype=torch.uint8)           # CPU allocations are 64-byte aligned
+    _call("gemm_microscaled", "ri_mx_encode", c_void_p(m.data_ptr()), _p(codes), _p(exponents), c_longlong(rows), c_int(spans), c_int(bits), c_int(box))
     ops._launches -= 1                                # encoding a map launches nothing
     return m
 
@@ -104,7 +104,7 @@ class Matrix:
 
     def map(self) -> torch.Tensor:
         if self._map is None:
-            self._map = _encode(self.codes, self.n, self.spans, 4, 128)
+            self._map = _encode(self.codes, self.exponents, self.n, self.spans, 4, 128)
         return self._map
 
 
@@ -137,7 +137,7 @@ class Rows:
     def map(self, box: int) -> torch.Tensor:
         m = self._maps.get(box)
         if m is None:
-            m = self._maps[box] = _encode(self.codes, self.n, self.spans, 8, box)
+            m = self._maps[box] = _encode(self.codes, self.exponents, self.n, self.spans, 8, box)
         return m
 
 

@@ -33,7 +33,7 @@ constexpr int ROWS = 128;                          // rows of W or of X in a til
 constexpr int TILE = ROWS * SPAN;                  // its bytes, a byte a number
 constexpr int W_COPIED = TILE / 2;                 // what a copy of 4-bit codes counts
 constexpr int MAX_STAGES = 12;
-constexpr int THREADS = 192;
+constexpr int THREADS = 192, FEW_THREADS = 320;    // of the kernel on pairs, of the one for few tokens
 constexpr int SMEM_LIMIT = 225 * 1024;
 constexpr int CLUSTER_MOST = 8;
 constexpr int TOKENS_MOST = 128;                   // of a tile of the first kernel
@@ -72,10 +72,47 @@ __device__ __forceinline__ void mx_mma(uint32_t leader, uint32_t d, uint64_t a, 
             "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
             ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(exp_a), "r"(exp_b), "r"((uint32_t)accumulate), "r"(leader) : "memory");
 }
-// A piece of exponents into this CTA's shared memory.
-__device__ __forceinline__ void load_piece(uint32_t dst, const uint8_t* src, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"((uint32_t)PIECE), "r"(bar) : "memory");
+// Copies, for a warp that stays together: every lane calls, the one whose `leader` is set issues (in a branch that one lane takes, each took
+// 120 clocks to issue, and these products wait for little else).
+__device__ __forceinline__ void expect_by(uint32_t leader, uint32_t bar, uint32_t bytes) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
+                 ::"r"(bar), "r"(bytes), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void load_2d_by(uint32_t leader, uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(leader) : "memory");
+}
+// A ring's position: the stage, its barrier's parity, and what a look at that barrier, taken a step before, has shown.  (A wait that begins
+// when its turn has come costs a step some 60 clocks, also where the barrier has long completed.)
+struct Ring {
+    uint32_t bars;               // the stages' barriers
+    int s;
+    uint32_t parity;
+    bool seen;
+    __device__ __forceinline__ uint32_t bar() const { return bars + 8u * (uint32_t)s; }
+    __device__ __forceinline__ bool wait() const { return seen || mbar_wait_warp(bar(), parity); }      // bounded; the same answer for the warp
+    // looks at the next stage's barrier before what is issued between the two calls
+    __device__ __forceinline__ bool look(int stages) const {
+        const bool wraps = s + 1 == stages;
+        uint32_t ok;                       // (test_wait: try_wait would stay for a while)
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(wraps ? bars : bar() + 8u), "r"(wraps ? parity ^ 1u : parity) : "memory");
+        return ok != 0;
+    }
+    __device__ __forceinline__ void next(int stages, bool looked) {
+        if (++s == stages) {
+            s = 0;
+            parity ^= 1u;
+        }
+        seen = __all_sync(0xffffffffu, looked);
+    }
+};
+// a piece of exponents into this CTA's shared memory
+__device__ __forceinline__ void load_piece_by(uint32_t leader, uint32_t dst, const uint8_t* src, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}"
+                 ::"r"(dst), "l"(src), "r"((uint32_t)PIECE), "r"(bar), "r"(leader) : "memory");
 }
 
 // The epilogues' arithmetic.  `constants`: the bias [features], or an activation's or a gate's constants, or null.  Fast exponentials where
@@ -114,28 +151,42 @@ struct Result {
     uint8_t* exponents;
     int n_spans;
 };
-// One number of token t and feature f of the first kernel, whose warp has 32 features that begin at a multiple of 32.
-template <int OUT>
-__device__ __forceinline__ void store_lane(const Result& r, int t, int f, int n_feat, float v) {
+// What N tokens (t(0), t(1), ...; those that `good` says) have at feature f of the first kernel, whose warp has 32 features that begin at a
+// multiple of 32.  The tokens' chains of instructions are independent and without branches, so that they run side by side.
+template <int OUT, int N, typename T, typename G>
+__device__ __forceinline__ void store_lanes(const Result& r, T t, G good, int f, int n_feat, const float* v) {
     if (OUT == OUT_ROWS) {
-        if (f >= n_feat) v = 0.f;
-        const uint32_t byte = exponent_byte<8>(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
-        reinterpret_cast<uint8_t*>(r.out)[(size_t)t * r.n_spans * SPAN + f] = eight_bits_of_one(v * to_type(byte));
-        if ((f & 31) == 0) r.exponents[exponent_at(t, f >> 5, r.n_spans)] = (uint8_t)byte;
+        uint32_t byte[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) byte[j] = exponent_byte<8>(__reduce_max_sync(0xffffffffu, f < n_feat ? __float_as_uint(v[j]) & 0x7fffffffu : 0u));
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint8_t code = eight_bits_of_one(f < n_feat ? v[j] * to_type(byte[j]) : 0.f);
+            if (good(j)) reinterpret_cast<uint8_t*>(r.out)[(size_t)t(j) * r.n_spans * SPAN + f] = code;
+        }
+        if ((f & 31) == 0) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (good(j)) r.exponents[exponent_at(t(j), f >> 5, r.n_spans)] = (uint8_t)byte[j];
+        }
     } else if (f < n_feat) {
-        const size_t at = (size_t)t * n_feat + f;
-        if (OUT == OUT_BF16) reinterpret_cast<__nv_bfloat16*>(r.out)[at] = __float2bfloat16_rn(v);
-        else if (OUT == OUT_F32) reinterpret_cast<float*>(r.out)[at] = v;
-        else atomicAdd(reinterpret_cast<float*>(r.out) + at, v);         // one add per number: no order to depend on
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const size_t at = (size_t)t(j) * n_feat + f;
+            if (!good(j)) continue;
+            if (OUT == OUT_BF16) reinterpret_cast<__nv_bfloat16*>(r.out)[at] = __float2bfloat16_rn(v[j]);
+            else if (OUT == OUT_F32) reinterpret_cast<float*>(r.out)[at] = v[j];
+            else atomicAdd(reinterpret_cast<float*>(r.out) + at, v[j]);         // one add per number: no order to depend on
+        }
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Few tokens.  A persistent grid of tiles of 128 features x tn tokens, or clusters of CTAs that share a tile's K.  Warp 0 issues the copies,
-// warp 1 allocates tensor memory and issues the MMAs, warps 2-5 run the epilogue.
+// Few tokens.  Tiles of 128 features x tn tokens, for a persistent grid of CTAs, or each for a cluster whose CTAs share its K.  Warp 0 issues the copies, warp 1 allocates tensor memory and issues the MMAs,
+// warps 2-9 run the epilogue, two for each quarter of tensor memory's lanes, which take turns at 16 tokens.
 // ---------------------------------------------------------------------------------------------
 template <bool DUAL, int OUT>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(FEW_THREADS, 1)
 mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const __grid_constant__ CUtensorMap map_x,
                   const uint8_t* __restrict__ w_exp, const uint8_t* __restrict__ w2_exp, const uint8_t* x_exp, const float* __restrict__ constants, int act,
                   Result res, int n_tok, int n_feat, int n_spans, int cluster, int stages, int tn, int buffers, int tmem_cols, int* status) {
@@ -157,11 +208,14 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t exp_base = smem_base + (uint32_t)stages * tile_bytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;      // epilogue warps: the TMEM lanes that a warp may read, and which of the two it is
     const bool clustered = cluster > 1;
     const int rank = clustered ? (int)cluster_rank() : 0;
     const int n_tok_tiles = (n_tok + tn - 1) / tn, n_feat_tiles = (n_feat + ROWS - 1) / ROWS;
     const int total_tiles = n_tok_tiles * n_feat_tiles;
-    const int my_tiles = clustered ? 1 : ((int)blockIdx.x < total_tiles) ? (total_tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+    // a cluster has one tile, a CTA without one its share of them
+    const int first = (int)blockIdx.x / cluster;
+    const int my_tiles = clustered ? 1 : (first < total_tiles) ? (total_tiles - 1 - first) / (int)gridDim.x + 1 : 0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
@@ -170,7 +224,7 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&acc_full[i]), 1);
-            mbar_init(smem_u32(&acc_empty[i]), 4);
+            mbar_init(smem_u32(&acc_empty[i]), 8);             // one arrival per epilogue warp
         }
         abort_flag = any_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -188,46 +242,39 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     let_next_kernel_start();
 
     // token tiles vary fastest, so that CTAs which run together share a tile of W in L2
-    auto tile_coords = [&](int i, int& f0, int& t0, int& begin, int& count) {
-        if (clustered) {
-            f0 = ((int)blockIdx.x / cluster) * ROWS;
-            t0 = 0;
-            begin = n_spans * rank / cluster;
-            count = n_spans * (rank + 1) / cluster - begin;                // >= 1: cluster <= n_spans
-            return;
-        }
-        const int tile = (int)blockIdx.x + i * (int)gridDim.x;
+    auto tile_coords = [&](int i, int& f0, int& t0) {
+        const int tile = first + i * (int)gridDim.x;
         f0 = (tile / n_tok_tiles) * ROWS;
         t0 = (tile % n_tok_tiles) * tn;
-        begin = 0;
-        count = n_spans;
     };
+    const int begin = n_spans * rank / cluster, count = n_spans * (rank + 1) / cluster - begin;       // spans of this CTA: cluster <= n_spans
 
     if (warp == 0) {
-        if (lane == 0) {
-            int it = 0, s = 0;               // spans issued; ring position and pass parity, carried along
-            uint32_t ph = 0;
+        {                                                        // the whole warp goes through, one lane issues
+            const uint32_t leader = elect_one();
+            int it = 0;                      // spans issued
+            Ring ring{empty0, 0, 1u, true};  // (a barrier's phase before its first counts as completed)
             bool waited = false, alive = true;
             for (int i = 0; i < my_tiles && alive; ++i) {
-                int f0, t0, begin, count;
-                tile_coords(i, f0, t0, begin, count);
+                int f0, t0;
+                tile_coords(i, f0, t0);
                 if (abort_flag) break;
-                // pieces of exponents of this tile's rows; a tile's tokens lie within one piece (tn = 128, or a single tile of fewer)
+                // pieces of exponents of this tile's rows (a tile's tokens are all or the first of one: tn is 128, or there is one tile)
                 const uint8_t* we = w_exp + ((size_t)(f0 / ROWS) * n_spans + begin) * PIECE;
                 const uint8_t* we2 = DUAL ? w2_exp + ((size_t)(f0 / ROWS) * n_spans + begin) * PIECE : nullptr;
                 const uint8_t* xe = x_exp + ((size_t)(t0 / ROWS) * n_spans + begin) * PIECE;
                 auto load_w = [&](int at, int j) {
                     const uint32_t bar = full0 + 8u * (uint32_t)at, stage = smem_base + (uint32_t)at * tile_bytes, ex = exp_base + (uint32_t)at * EXP_BYTES;
-                    mbar_expect_tx(bar, stage_tx);
-                    tma_load_2d(stage, &map_w, bar, (begin + j) * SPAN, f0);
-                    if (DUAL) tma_load_2d(stage + TILE, &map_w2, bar, (begin + j) * SPAN, f0);
-                    load_piece(ex, we + (size_t)j * PIECE, bar);
-                    if (DUAL) load_piece(ex + PIECE, we2 + (size_t)j * PIECE, bar);
+                    expect_by(leader, bar, stage_tx);
+                    load_2d_by(leader, stage, &map_w, bar, (begin + j) * SPAN, f0);
+                    if (DUAL) load_2d_by(leader, stage + TILE, &map_w2, bar, (begin + j) * SPAN, f0);
+                    load_piece_by(leader, ex, we + (size_t)j * PIECE, bar);
+                    if (DUAL) load_piece_by(leader, ex + PIECE, we2 + (size_t)j * PIECE, bar);
                 };
                 auto load_x = [&](int at, int j) {
-                    const uint32_t bar = full0 + 8u * (uint32_t)at, stage = smem_base + (uint32_t)at * tile_bytes, ex = exp_base + (uint32_t)at * EXP_BYTES;
-                    tma_load_2d(stage + MATS * TILE, &map_x, bar, (begin + j) * SPAN, t0);
-                    load_piece(ex + MATS * PIECE, xe + (size_t)j * PIECE, bar);
+                    const uint32_t bar = full0 + 8u * (uint32_t)at;
+                    load_2d_by(leader, smem_base + (uint32_t)at * tile_bytes + MATS * TILE, &map_x, bar, (begin + j) * SPAN, t0);
+                    load_piece_by(leader, exp_base + (uint32_t)at * EXP_BYTES + MATS * PIECE, xe + (size_t)j * PIECE, bar);
                 };
                 int j = 0;
                 if (!waited) {
@@ -238,37 +285,37 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
                     waited = true;
                     for (j = 0; j < ahead; ++j) load_x(j, j);
                     it = ahead;
-                    if (ahead == stages) ph = 1; else s = ahead;
+                    if (ahead == stages) ring = Ring{empty0, 0, 0u, false}; else ring.s = ahead;
                 }
                 for (; j < count; ++j, ++it) {
-                    if (!mbar_wait(empty0 + 8u * s, ph ^ 1u)) {
-                        if (!abort_flag) report(status, ST_PRODUCER_TIMEOUT);
+                    if (!ring.wait()) {
+                        if (lane == 0 && !abort_flag) report(status, ST_PRODUCER_TIMEOUT);
                         abort_flag = 1;
                         alive = false;
                         break;
                     }
-                    load_w(s, j);
-                    load_x(s, j);
-                    if (++s == stages) { s = 0; ph ^= 1u; }
+                    const bool looked = ring.look(stages);
+                    load_w(ring.s, j);
+                    load_x(ring.s, j);
+                    ring.next(stages, looked);
                 }
             }
             // do not leave, or hand the ring to the cluster, while a copy into it may still be in flight
             for (int j = max(0, it - stages); j < it; ++j)
-                if (!mbar_wait(full0 + 8u * (uint32_t)(j % stages), (uint32_t)(j / stages) & 1u)) {
-                    report(status, ST_DRAIN_TIMEOUT);
+                if (!mbar_wait_warp(full0 + 8u * (uint32_t)(j % stages), (uint32_t)(j / stages) & 1u)) {
+                    if (lane == 0) report(status, ST_DRAIN_TIMEOUT);
                     abort_flag = 1;
                     break;
                 }
         }
     } else if (warp == 1) {
         const uint32_t leader = elect_one();                     // the whole warp goes through, one lane issues
-        int s = 0;
-        uint32_t ph = 0;
+        Ring ring{full0, 0, 0u, false};
         bool alive = true;
         const uint64_t desc_w0 = make_smem_desc(smem_base), desc_e0 = piece_desc(exp_base);
         for (int i = 0; i < my_tiles && alive; ++i) {
-            int f0, t0, begin, count;
-            tile_coords(i, f0, t0, begin, count);
+            int f0, t0;
+            tile_coords(i, f0, t0);
             const int buf = buffers == 2 ? i & 1 : 0, round = buffers == 2 ? i >> 1 : i;
             if (!mbar_wait_warp(smem_u32(&acc_empty[buf]), (uint32_t)(round & 1) ^ 1u)) {
                 if (lane == 0) report(status, ST_MMA_TIMEOUT);
@@ -278,36 +325,36 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
             tc_fence_after();
             const uint32_t acc = tmem_base + (uint32_t)(buf * acc_cols);
             for (int j = 0; j < count; ++j) {
-                if (!mbar_wait_warp(full0 + 8u * s, ph)) {
+                if (!ring.wait()) {
                     if (lane == 0) report(status, ST_MMA_TIMEOUT);
                     abort_flag = 1;
                     alive = false;
                     break;
                 }
                 tc_fence_after();
+                const bool looked = ring.look(stages);
                 // exponents go to one of two sets of columns behind the accumulators, while the MMAs before still read the other
                 const uint32_t ex = tmem_base + (uint32_t)(buffers * acc_cols + (j & 1) * (MATS + 1) * 4);
-                const uint64_t e = desc_e0 + (uint64_t)((uint32_t)s * (EXP_BYTES >> 4));
+                const uint64_t e = desc_e0 + (uint64_t)((uint32_t)ring.s * (EXP_BYTES >> 4));
 #pragma unroll
                 for (int m = 0; m <= MATS; ++m) exponents_to_tmem<0>(leader, ex + 4 * m, e + (uint64_t)(m * (PIECE >> 4)));
-                const uint64_t w = desc_w0 + (uint64_t)((uint32_t)s * (tile_bytes >> 4)), x = w + (uint64_t)(MATS * (TILE >> 4));
+                const uint64_t w = desc_w0 + (uint64_t)((uint32_t)ring.s * (tile_bytes >> 4)), x = w + (uint64_t)(MATS * (TILE >> 4));
 #pragma unroll
                 for (int b = 0; b < SPAN / BLOCK; ++b) {
                     mx_mma<0>(leader, acc, w + 2 * b, x + 2 * b, of_block(idesc, b), ex, ex + 4 * MATS, j > 0 || b > 0);
                     if (DUAL) mx_mma<0>(leader, acc + tn, w + (TILE >> 4) + 2 * b, x + 2 * b, of_block(idesc, b), ex + 4, ex + 4 * MATS, j > 0 || b > 0);
                 }
-                umma_commit_by(leader, empty0 + 8u * s);
-                if (++s == stages) { s = 0; ph ^= 1u; }
+                umma_commit_by(leader, empty0 + 8u * (uint32_t)ring.s);
+                ring.next(stages, looked);
             }
             umma_commit_by(leader, smem_u32(&acc_full[buf]));
         }
     } else {
         wait_for_previous_kernels();          // `out` may still be read or written by the kernel before
-        const int lane_base = (warp & 3) * 32;                 // the TMEM lanes this warp may read
         const Epilogue e = load_epilogue<DUAL>(constants, act);
         for (int i = 0; i < my_tiles; ++i) {
-            int f0, t0, begin, count;
-            tile_coords(i, f0, t0, begin, count);
+            int f0, t0;
+            tile_coords(i, f0, t0);
             const int buf = buffers == 2 ? i & 1 : 0, round = buffers == 2 ? i >> 1 : i;
             const bool landed = mbar_wait(smem_u32(&acc_full[buf]), (uint32_t)(round & 1));
             if (!landed) {
@@ -317,21 +364,21 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
             tc_fence_after();
             __syncwarp();
             if (__any_sync(0xffffffffu, !landed || abort_flag)) break;
-            if (clustered) break;                                  // the pieces of K meet below
-            const int f = f0 + lane_base + lane;
+            if (clustered) break;                                  // the pieces meet below
+            const int f = f0 + quarter * 32 + lane;
             const float b = (!DUAL && !e.act && OUT != OUT_ADD && e.constants != nullptr && f < n_feat) ? e.constants[f] : 0.f;
-            const uint32_t trow = tmem_base + ((uint32_t)lane_base << 16) + (uint32_t)(buf * acc_cols);
+            const uint32_t trow = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * acc_cols);
 #pragma unroll 1
-            for (int c0 = 0; c0 < tn; c0 += 16) {
+            for (int c0 = half * 16; c0 < tn; c0 += 32) {
                 if (t0 + c0 >= n_tok) break;
                 uint32_t v[16], u[16];
                 tmem_ld16(trow + c0, v);
                 if (DUAL) tmem_ld16(trow + tn + c0, u);
                 tmem_wait_ld();
+                float r[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (t0 + c0 + j < n_tok)
-                        store_lane<OUT>(res, t0 + c0 + j, f, n_feat, result<DUAL, OUT>(__uint_as_float(v[j]), DUAL ? __uint_as_float(u[j]) : 0.f, b, e));
+                for (int j = 0; j < 16; ++j) r[j] = result<DUAL, OUT>(__uint_as_float(v[j]), DUAL ? __uint_as_float(u[j]) : 0.f, b, e);
+                store_lanes<OUT, 16>(res, [&](int j) { return t0 + c0 + j; }, [&](int j) { return t0 + c0 + j < n_tok; }, f, n_feat, r);
             }
             tc_fence_before();
             __syncwarp();
@@ -340,13 +387,16 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     }
 
     if (clustered) {
-        // Token c is finished by the CTA of rank c % cluster: everybody sends it its sums of that token, into `recv`
+        // Token c of the tile is finished by the CTA of rank c % cluster: everybody sends it its sums of that token, into `recv`
         // [rank of the sender][c / cluster][(gate, up)][128], which lies where the ring was, and it adds them in the order of the ranks.
         // A CTA that gave up says so before; then none of the cluster writes.
         constexpr int SENT = MATS * ROWS;                          // floats per token
-        const int held = (n_tok + cluster - 1) / cluster;
+        const int held = (tn + cluster - 1) / cluster;
+        int f0, t0;
+        tile_coords(0, f0, t0);
+        const int tokens = min(tn, n_tok - t0);
         float* recv = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)));
-        const int fl = (warp & 3) * 32 + lane;
+        const int fl = quarter * 32 + lane;
         __syncwarp();
         cluster_wait();                                            // the peers run
         if (abort_flag && lane == 0) set_in_all(&any_failed, cluster);
@@ -354,10 +404,10 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         cluster_sync();                                            // nobody's ring is in use any more
         const bool failed = any_failed != 0;
         if (warp >= 2 && !failed) {
-            const uint32_t trow = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+            const uint32_t trow = tmem_base + ((uint32_t)(quarter * 32) << 16);
             const float* mine = recv + (size_t)rank * held * SENT + fl;
 #pragma unroll 1
-            for (int c0 = 0; c0 < n_tok; c0 += 16) {
+            for (int c0 = half * 16; c0 < tokens; c0 += 32) {
                 uint32_t v[16], u[16];
                 tmem_ld16(trow + c0, v);
                 if (DUAL) tmem_ld16(trow + tn + c0, u);
@@ -365,27 +415,38 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
                 int to = c0 % cluster, at = (c0 / cluster) * SENT;
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    if (c0 + j >= n_tok) break;
-                    store_peer_float(mine + at, (uint32_t)to, __uint_as_float(v[j]));
-                    if (DUAL) store_peer_float(mine + at + ROWS, (uint32_t)to, __uint_as_float(u[j]));
+                    if (c0 + j < tokens) {
+                        store_peer_float(mine + at, (uint32_t)to, __uint_as_float(v[j]));
+                        if (DUAL) store_peer_float(mine + at + ROWS, (uint32_t)to, __uint_as_float(u[j]));
+                    }
                     if (++to == cluster) { to = 0; at += SENT; }
                 }
             }
         }
         __syncwarp();
         cluster_sync();                                            // everything sent has arrived
-        const int f = ((int)blockIdx.x / cluster) * ROWS + fl;
+        const int f = f0 + fl;
         if (warp >= 2 && !failed) {
             const Epilogue e = load_epilogue<DUAL>(constants, act);
             const float b = (!DUAL && !e.act && OUT != OUT_ADD && e.constants != nullptr && f < n_feat) ? e.constants[f] : 0.f;
-            for (int i = 0, c = rank; c < n_tok; ++i, c += cluster) {
+            constexpr int TOGETHER = 4;
+            for (int i = half * TOGETHER; rank + i * cluster < tokens; i += 2 * TOGETHER) {
+                const int c = rank + i * cluster, n = min(TOGETHER, (tokens - c + cluster - 1) / cluster);      // tokens c, c + cluster, ...
+                float a[TOGETHER] = {}, u[TOGETHER] = {};
                 const float* from = recv + (size_t)i * SENT + fl;
-                float a = 0.f, u = 0.f;
+#pragma unroll 4
                 for (int p = 0; p < cluster; ++p, from += (size_t)held * SENT) {
-                    a += from[0];
-                    if (DUAL) u += from[ROWS];
+#pragma unroll
+                    for (int j = 0; j < TOGETHER; ++j) {
+                        if (j < n) {
+                            a[j] += from[j * SENT];
+                            if (DUAL) u[j] += from[j * SENT + ROWS];
+                        }
+                    }
                 }
-                store_lane<OUT>(res, c, f, n_feat, result<DUAL, OUT>(a, u, b, e));
+#pragma unroll
+                for (int j = 0; j < TOGETHER; ++j) a[j] = result<DUAL, OUT>(a[j], u[j], b, e);
+                store_lanes<OUT, TOGETHER>(res, [&](int j) { return t0 + c + j * cluster; }, [&](int j) { return j < n; }, f, n_feat, a);
             }
         }
     }
@@ -417,10 +478,11 @@ __device__ __forceinline__ uint32_t in_first_cta(uint32_t local_addr) {
     return a;
 }
 // A tile into this CTA's shared memory whose arrival is counted by a barrier of the pair's first CTA.
-__device__ __forceinline__ void load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y) {
+__device__ __forceinline__ void load_2d_pair(uint32_t leader, uint32_t dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y) : "memory");
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+        ::"r"(dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(leader) : "memory");
 }
 __device__ __forceinline__ void commit_pair(uint32_t leader, uint32_t bar) {
     asm volatile(
@@ -543,9 +605,10 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     };
 
     if (warp == 0) {
-        if (lane == 0) {
-            int it = 0, s = 0;
-            uint32_t ph = 0;
+        {                                                        // the whole warp goes through, one lane issues
+            const uint32_t leader = elect_one();
+            int it = 0;
+            Ring ring{empty0, 0, 1u, true};
             bool alive = true;
             wait_for_previous_kernels();                         // the rows come from the kernel before
             const CUtensorMap* my_w = (DUAL && rank == 1) ? &map_w2 : &map_w;
@@ -558,37 +621,37 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 // pieces of exponents: a row of a map each (beyond the last one: zeros)
                 const int xe = (t0 / ROWS + rank) * n_spans, we = (f0 / ROWS) * n_spans, we2 = DUAL ? we : we + n_spans;
                 for (int j = 0; j < n_spans; ++j, ++it) {
-                    if (!mbar_wait(empty0 + 8u * s, ph ^ 1u)) {
-                        if (!abort_flag) report(status, ST_PRODUCER_TIMEOUT);
+                    if (!ring.wait()) {
+                        if (lane == 0 && !abort_flag) report(status, ST_PRODUCER_TIMEOUT);
                         abort_flag = 1;
                         alive = false;
                         break;
                     }
-                    const uint32_t stage = smem_base + (uint32_t)s * 2 * TILE, ex = exp_base + (uint32_t)s * PAIR_EXP, bar = full0_first + 8u * s;
-                    if (rank == 0) mbar_expect_tx(full0 + 8u * s, 2 * CTA_TX);                 // both CTAs' bytes
-                    load_2d_pair(stage, &map_x, bar, j * SPAN, t0 + rank * ROWS);
-                    load_2d_pair(stage + TILE, my_w, bar, j * SPAN, f0 + w_off);
-                    load_2d_pair(ex, &map_xe, bar, 0, xe + j);
-                    load_2d_pair(ex + PIECE, &map_we, bar, 0, we + j);
-                    load_2d_pair(ex + 2 * PIECE, second_we, bar, 0, we2 + j);
-                    if (++s == stages) { s = 0; ph ^= 1u; }
+                    const bool looked = ring.look(stages);
+                    const uint32_t stage = smem_base + (uint32_t)ring.s * 2 * TILE, ex = exp_base + (uint32_t)ring.s * PAIR_EXP, bar = full0_first + 8u * (uint32_t)ring.s;
+                    if (rank == 0) expect_by(leader, full0 + 8u * (uint32_t)ring.s, 2 * CTA_TX);                 // both CTAs' bytes
+                    load_2d_pair(leader, stage, &map_x, bar, j * SPAN, t0 + rank * ROWS);
+                    load_2d_pair(leader, stage + TILE, my_w, bar, j * SPAN, f0 + w_off);
+                    load_2d_pair(leader, ex, &map_xe, bar, 0, xe + j);
+                    load_2d_pair(leader, ex + PIECE, &map_we, bar, 0, we + j);
+                    load_2d_pair(leader, ex + 2 * PIECE, second_we, bar, 0, we2 + j);
+                    ring.next(stages, looked);
                 }
             }
             // Do not leave while a copy into this CTA's shared memory may still be in flight: a stage whose `empty` barrier has completed
             // again was read by the MMAs, so its copies had landed.
             for (int j = 0; j < stages && it > 0; ++j) {
-                if (!mbar_wait(empty0 + 8u * s, ph ^ 1u)) {
-                    report(status, ST_DRAIN_TIMEOUT);
+                if (!ring.wait()) {
+                    if (lane == 0) report(status, ST_DRAIN_TIMEOUT);
                     break;
                 }
-                if (++s == stages) { s = 0; ph ^= 1u; }
+                ring.next(stages, false);
             }
         }
     } else if (warp == 1) {
         if (rank == 0) {                                         // the whole warp goes through, one lane issues
             const uint32_t leader = elect_one();
-            int s = 0;
-            uint32_t ph = 0;
+            Ring ring{full0, 0, 0u, false};
             bool alive = true;
             const uint64_t desc_x0 = make_smem_desc(smem_base), desc_e0 = piece_desc(exp_base);
             for (int i = 0; i < my_tiles && alive; ++i) {
@@ -601,23 +664,24 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 tc_fence_after();
                 const uint32_t acc = tmem_base + (uint32_t)((i & 1) * SECOND_ACC);
                 for (int j = 0; j < n_spans; ++j) {
-                    if (!mbar_wait_warp(full0 + 8u * s, ph)) {
+                    if (!ring.wait()) {
                         if (lane == 0) report(status, ST_MMA_TIMEOUT);
                         abort_flag = 1;
                         alive = false;
                         break;
                     }
                     tc_fence_after();
+                    const bool looked = ring.look(stages);
                     const uint32_t ex = tmem_base + (uint32_t)(PAIR_EXP_COL + (j & 1) * 16);
-                    const uint64_t e = desc_e0 + (uint64_t)((uint32_t)s * (PAIR_EXP >> 4));
+                    const uint64_t e = desc_e0 + (uint64_t)((uint32_t)ring.s * (PAIR_EXP >> 4));
 #pragma unroll
                     for (int m = 0; m < 3; ++m) exponents_to_tmem<1>(leader, ex + 4 * m, e + (uint64_t)(m * (PIECE >> 4)));
-                    const uint64_t x = desc_x0 + (uint64_t)((uint32_t)s * (2 * TILE >> 4)), w = x + (TILE >> 4);
+                    const uint64_t x = desc_x0 + (uint64_t)((uint32_t)ring.s * (2 * TILE >> 4)), w = x + (TILE >> 4);
 #pragma unroll
                     for (int b = 0; b < SPAN / BLOCK; ++b)
                         mx_mma<1>(leader, acc, x + 2 * b, w + 2 * b, of_block(IDESC, b), ex, ex + 4, j > 0 || b > 0);
-                    commit_pair(leader, empty0 + 8u * s);                // frees the stage in both CTAs
-                    if (++s == stages) { s = 0; ph ^= 1u; }
+                    commit_pair(leader, empty0 + 8u * (uint32_t)ring.s); // frees the stage in both CTAs
+                    ring.next(stages, looked);
                 }
                 commit_pair(leader, smem_u32(&acc_full[i & 1]));
             }
@@ -734,7 +798,8 @@ struct Plan {
 };
 int g_pair_tokens = 256;         // products of at least so many tokens run on pairs of SMs
 
-Plan plan(int n_tok, int n_feat, int n_spans) {
+int g_cluster = 0, g_per_sm = 0;
+Plan plan(int n_tok, int n_feat, int n_spans, bool dual) {
     Plan p;
     p.pairs = n_tok >= g_pair_tokens;
     if (p.pairs) {
@@ -743,41 +808,42 @@ Plan plan(int n_tok, int n_feat, int n_spans) {
         return p;
     }
     p.tn = n_tok >= TOKENS_MOST ? TOKENS_MOST : (n_tok + 15) / 16 * 16;
+    const long long tiles = (long long)((n_feat + ROWS - 1) / ROWS) * ((n_tok + p.tn - 1) / p.tn);
     p.cluster = 1;
-    const long long tiles = (long long)((n_feat + ROWS - 1) / ROWS);
-    if (n_tok <= TOKENS_MOST)
-        while (p.cluster < CLUSTER_MOST && tiles * (p.cluster + 1) <= sm_count() && n_spans >= 2 * (p.cluster + 1)) ++p.cluster;
+    while (p.cluster < CLUSTER_MOST && tiles * (p.cluster + 1) <= 2 * sm_count() - 20 && n_spans >= 2 * (p.cluster + 1)) ++p.cluster;
+    if (g_cluster) p.cluster = g_cluster < n_spans ? g_cluster : n_spans;
     return p;
 }
 
 template <bool DUAL, int OUT>
 int launch_feature(const Call& c) {
-    constexpr int MATS = DUAL ? 2 : 1;
-    const Plan p = plan(c.n_tok, c.n_feat, c.n_spans);
+    const Plan p = plan(c.n_tok, c.n_feat, c.n_spans, DUAL);
     const long long tiles = (long long)((c.n_tok + p.tn - 1) / p.tn) * ((c.n_feat + ROWS - 1) / ROWS);
     if (tiles > 0x7fffffffLL / CLUSTER_MOST) return fail("gemm_microscaled: %lld tiles exceed the index range", tiles);
     auto kernel = mx_feature_kernel<DUAL, OUT>;
     static PerDeviceOnce configured;
     if (int rc = raise_dynamic_smem(kernel, SMEM_LIMIT, configured, "gemm_microscaled")) return rc;
+    constexpr int MATS = DUAL ? 2 : 1;
     const int stage = MATS * TILE + p.tn * SPAN + (MATS + 1) * PIECE;
-    const int recv = p.cluster > 1 ? p.cluster * ((c.n_tok + p.cluster - 1) / p.cluster) * MATS * ROWS * 4 : 0;
-    const int most = (c.n_spans + p.cluster - 1) / p.cluster;            // spans of a tile
-    int stages = (SMEM_LIMIT - 1024) / stage;
+    const int recv = p.cluster > 1 ? p.cluster * ((p.tn + p.cluster - 1) / p.cluster) * MATS * ROWS * 4 : 0;
+    const int most = (c.n_spans + p.cluster - 1) / p.cluster;            // spans of a CTA
+    int stages = ((g_per_sm == 1 ? SMEM_LIMIT : g_per_sm == 3 ? 150 * 1024 : g_per_sm == 4 ? 185 * 1024 : 112 * 1024) - 1024) / stage;
     if (stages > MAX_STAGES) stages = MAX_STAGES;
     if (p.cluster > 1 && stages > most) stages = most;
     const size_t ring = (size_t)stages * stage;
     size_t smem = (ring > (size_t)recv ? ring : (size_t)recv) + 1024;
     long long ctas = p.cluster > 1 ? tiles * p.cluster : tiles;
-    if (p.cluster == 1 && ctas > sm_count()) ctas = sm_count();
-    const int exps = 2 * (MATS + 1) * 4;
+    constexpr int EXP_COLS = 2 * (MATS + 1) * 4;
+    const int per_sm = smem <= 113 * 1024 && 2 * columns(MATS * p.tn + EXP_COLS) <= 512 ? 2 : 1;
+    if (p.cluster == 1 && ctas > per_sm * sm_count()) ctas = per_sm * sm_count();
     int buffers = (p.cluster > 1 || ctas == tiles) ? 1 : 2;
-    if (buffers * MATS * p.tn + exps > 512) buffers = 1;
-    const int cols = columns(buffers * MATS * p.tn + exps);
+    if (per_sm * columns(buffers * MATS * p.tn + EXP_COLS) > 512) buffers = 1;
+    const int cols = columns(buffers * MATS * p.tn + EXP_COLS);
     // CTAs that wait for others of their cluster must not wait for tensor memory that CTAs of another cluster hold, which may wait likewise:
     // shared memory in proportion to their columns keeps all that an SM takes in within its 512 columns.
     if (p.cluster > 1 && smem < (size_t)cols * 456) smem = (size_t)cols * 456 < SMEM_LIMIT ? (size_t)cols * 456 : SMEM_LIMIT;
-    return launch_cluster("gemm_microscaled", kernel, dim3((unsigned)ctas), THREADS, smem, p.cluster, c.stream, c.w->codes, c.w2->codes, c.x->codes, c.w_exp, c.w2_exp, c.x_exp,
-                          c.constants, c.act, c.res, c.n_tok, c.n_feat, c.n_spans, p.cluster, stages, p.tn, buffers, cols, c.status);
+    return launch_cluster("gemm_microscaled", kernel, dim3((unsigned)ctas), FEW_THREADS, smem, p.cluster, c.stream, c.w->codes, c.w2->codes, c.x->codes, c.w_exp,
+                          c.w2_exp, c.x_exp, c.constants, c.act, c.res, c.n_tok, c.n_feat, c.n_spans, p.cluster, stages, p.tn, buffers, cols, c.status);
 }
 
 template <bool DUAL, int OUT>
@@ -799,7 +865,7 @@ int launch_pair(const Call& c) {
 
 template <bool DUAL, int OUT>
 int launch(const Call& c) {
-    return plan(c.n_tok, c.n_feat, c.n_spans).pairs ? launch_pair<DUAL, OUT>(c) : launch_feature<DUAL, OUT>(c);
+    return plan(c.n_tok, c.n_feat, c.n_spans, DUAL).pairs ? launch_pair<DUAL, OUT>(c) : launch_feature<DUAL, OUT>(c);
 }
 
 }  // namespace
@@ -818,13 +884,17 @@ RI_API int ri_mx_encode(void* maps_out, const void* codes, const void* exponents
 }
 
 // Products of at least so many tokens run on pairs of SMs (for comparisons and tests).
+RI_API int ri_mx_set_plan(int cluster, int per_sm) {
+    g_cluster = cluster; g_per_sm = per_sm;
+    return 0;
+}
 RI_API int ri_mx_set_pairs(int tokens) {
     g_pair_tokens = tokens;
     return 0;
 }
 
 // Rows of the box of a product's X.
-RI_API int ri_mx_box(int n_tok, int n_feat, int n_spans) { return plan(n_tok, n_feat, n_spans).tn; }
+RI_API int ri_mx_box(int n_tok, int n_feat, int n_spans, int dual) { return plan(n_tok, n_feat, n_spans, dual != 0).tn; }
 
 // `kind`: what is written (`Out`); `dual`: gated, with the second matrix; `act`: `constants` are an activation's.  out_exp, out_spans: with rows in 8 bits.
 RI_API int ri_mx_gemm(const void* maps_w, const void* maps_w2, const void* maps_x, const void* w_exp, const void* w2_exp, const void* x_exp,

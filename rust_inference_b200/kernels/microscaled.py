@@ -220,7 +220,7 @@ def product(x, w: Matrix, out, ctx, *, w2: Matrix | None = None, bias=None, form
     _need(to is not rows.codes, "microscaled.product: rows cannot be their own product")
     _here(what, rows.codes, w.codes, w2.codes if w2 is not None else None, to, constants)
     from .tcgen05 import status_word
-    box = load("gemm_microscaled").ri_mx_box(c_int(n_tok), c_int(w.n), c_int(w.spans))
+    box = load("gemm_microscaled").ri_mx_box(c_int(n_tok), c_int(w.n), c_int(w.spans), c_int(1 if w2 is not None else 0))
     _call("gemm_microscaled", "ri_mx_gemm", c_void_p(w.map().data_ptr()), c_void_p(w2.map().data_ptr() if w2 is not None else 0),
           c_void_p(rows.map(box).data_ptr()), _p(w.exponents), _p(w2.exponents if w2 is not None else None), _p(rows.exponents), _p(constants),
           c_int(1 if w2 is not None else 0), c_int(1 if act is not None else 0), c_int(kind), _p(to), _p(to_exp), c_int(to_spans), c_int(n_tok), c_int(w.n),

@@ -33,7 +33,7 @@ constexpr int ROWS = 128;                          // rows of W or of X in a til
 constexpr int TILE = ROWS * SPAN;                  // its bytes, a byte a number
 constexpr int W_COPIED = TILE / 2;                 // what a copy of 4-bit codes counts
 constexpr int MAX_STAGES = 12;
-constexpr int THREADS = 192, FEW_THREADS = 320;    // of the kernel on pairs, of the one for few tokens
+constexpr int THREADS = 320;
 constexpr int SMEM_LIMIT = 225 * 1024;
 constexpr int CLUSTER_MOST = 8;
 constexpr int TOKENS_MOST = 128;                   // of a tile of the first kernel
@@ -137,11 +137,19 @@ __device__ __forceinline__ float gated_quick(float g, float u, const GateForm& f
     u = fmaxf(fminf(u, f.limit), -f.limit) + f.shift;
     return __fdividef(g, 1.f + __expf(-f.alpha * g * fmaf(f.cubic * g, g, 1.f))) * u * f.mult;
 }
+// `act_quick_f32` (common.cuh) without branches: a warp whose accumulators lie on both sides of zero would go through one after the other
+// (256 features of a token took 7 us, 1.5 so)
+__device__ __forceinline__ float act_chosen(float z, const ActForm& f) {
+    const float series = z * z * fmaf(z, fmaf(z, fmaf(z, 1.f / 120.f, 1.f / 24.f), 1.f / 6.f), 0.5f);
+    const float t = z > -0.25f ? series : __expf(z) - 1.f - z;
+    const float curved = z > 0.f ? f.ap * z * z : f.an == 0.f ? 0.f : f.an * t;
+    return fmaf(f.lin, z, curved);
+}
 template <bool DUAL, int OUT>
 __device__ __forceinline__ float result(float a, float u, float bias, const Epilogue& e) {
     if (OUT == OUT_ADD) return a;
     if (DUAL) return OUT == OUT_F32 ? gated_f32(a, u, e.gf) : gated_quick(a, u, e.gf);
-    if (e.act) return OUT == OUT_F32 ? act_f32(a, e.af) : act_quick_f32(a, e.af);
+    if (e.act) return OUT == OUT_F32 ? act_f32(a, e.af) : act_chosen(a, e.af);
     return a + bias;
 }
 
@@ -182,11 +190,11 @@ __device__ __forceinline__ void store_lanes(const Result& r, T t, G good, int f,
 }
 
 // ---------------------------------------------------------------------------------------------
-// Few tokens.  Tiles of 128 features x tn tokens, for a persistent grid of CTAs, or each for a cluster whose CTAs share its K.  Warp 0 issues the copies, warp 1 allocates tensor memory and issues the MMAs,
+// Few tokens.  Tiles of 128 features x tn tokens, for a persistent grid of CTAs, or (not gated) each for a cluster whose CTAs share its K.  Warp 0 issues the copies, warp 1 allocates tensor memory and issues the MMAs,
 // warps 2-9 run the epilogue, two for each quarter of tensor memory's lanes, which take turns at 16 tokens.
 // ---------------------------------------------------------------------------------------------
 template <bool DUAL, int OUT>
-__global__ void __launch_bounds__(FEW_THREADS, 1)
+__global__ void __launch_bounds__(THREADS, 1)
 mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const __grid_constant__ CUtensorMap map_x,
                   const uint8_t* __restrict__ w_exp, const uint8_t* __restrict__ w2_exp, const uint8_t* x_exp, const float* __restrict__ constants, int act,
                   Result res, int n_tok, int n_feat, int n_spans, int cluster, int stages, int tn, int buffers, int tmem_cols, int* status) {
@@ -209,7 +217,7 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     const uint32_t exp_base = smem_base + (uint32_t)stages * tile_bytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int quarter = warp & 3, half = (warp - 2) >> 2;      // epilogue warps: the TMEM lanes that a warp may read, and which of the two it is
-    const bool clustered = cluster > 1;
+    const bool clustered = !DUAL && cluster > 1;
     const int rank = clustered ? (int)cluster_rank() : 0;
     const int n_tok_tiles = (n_tok + tn - 1) / tn, n_feat_tiles = (n_feat + ROWS - 1) / ROWS;
     const int total_tiles = n_tok_tiles * n_feat_tiles;
@@ -386,11 +394,10 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         }
     }
 
-    if (clustered) {
+    if constexpr (!DUAL) if (clustered) {
         // Token c of the tile is finished by the CTA of rank c % cluster: everybody sends it its sums of that token, into `recv`
-        // [rank of the sender][c / cluster][(gate, up)][128], which lies where the ring was, and it adds them in the order of the ranks.
+        // [rank of the sender][c / cluster][128], which lies where the ring was, and it adds them in the order of the ranks.
         // A CTA that gave up says so before; then none of the cluster writes.
-        constexpr int SENT = MATS * ROWS;                          // floats per token
         const int held = (tn + cluster - 1) / cluster;
         int f0, t0;
         tile_coords(0, f0, t0);
@@ -405,21 +412,17 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         const bool failed = any_failed != 0;
         if (warp >= 2 && !failed) {
             const uint32_t trow = tmem_base + ((uint32_t)(quarter * 32) << 16);
-            const float* mine = recv + (size_t)rank * held * SENT + fl;
+            const float* mine = recv + (size_t)rank * held * ROWS + fl;
 #pragma unroll 1
             for (int c0 = half * 16; c0 < tokens; c0 += 32) {
-                uint32_t v[16], u[16];
+                uint32_t v[16];
                 tmem_ld16(trow + c0, v);
-                if (DUAL) tmem_ld16(trow + tn + c0, u);
                 tmem_wait_ld();
-                int to = c0 % cluster, at = (c0 / cluster) * SENT;
+                int to = c0 % cluster, at = (c0 / cluster) * ROWS;
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    if (c0 + j < tokens) {
-                        store_peer_float(mine + at, (uint32_t)to, __uint_as_float(v[j]));
-                        if (DUAL) store_peer_float(mine + at + ROWS, (uint32_t)to, __uint_as_float(u[j]));
-                    }
-                    if (++to == cluster) { to = 0; at += SENT; }
+                    if (c0 + j < tokens) store_peer_float(mine + at, (uint32_t)to, __uint_as_float(v[j]));
+                    if (++to == cluster) { to = 0; at += ROWS; }
                 }
             }
         }
@@ -427,25 +430,22 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         cluster_sync();                                            // everything sent has arrived
         const int f = f0 + fl;
         if (warp >= 2 && !failed) {
-            const Epilogue e = load_epilogue<DUAL>(constants, act);
-            const float b = (!DUAL && !e.act && OUT != OUT_ADD && e.constants != nullptr && f < n_feat) ? e.constants[f] : 0.f;
+            const Epilogue e = load_epilogue<false>(constants, act);
+            const float b = (!e.act && OUT != OUT_ADD && e.constants != nullptr && f < n_feat) ? e.constants[f] : 0.f;
             constexpr int TOGETHER = 4;
             for (int i = half * TOGETHER; rank + i * cluster < tokens; i += 2 * TOGETHER) {
                 const int c = rank + i * cluster, n = min(TOGETHER, (tokens - c + cluster - 1) / cluster);      // tokens c, c + cluster, ...
-                float a[TOGETHER] = {}, u[TOGETHER] = {};
-                const float* from = recv + (size_t)i * SENT + fl;
+                float a[TOGETHER] = {};
+                const float* from = recv + (size_t)i * ROWS + fl;
 #pragma unroll 4
-                for (int p = 0; p < cluster; ++p, from += (size_t)held * SENT) {
+                for (int p = 0; p < cluster; ++p, from += (size_t)held * ROWS) {
 #pragma unroll
                     for (int j = 0; j < TOGETHER; ++j) {
-                        if (j < n) {
-                            a[j] += from[j * SENT];
-                            if (DUAL) u[j] += from[j * SENT + ROWS];
-                        }
+                        if (j < n) a[j] += from[j * ROWS];
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < TOGETHER; ++j) a[j] = result<DUAL, OUT>(a[j], u[j], b, e);
+                for (int j = 0; j < TOGETHER; ++j) a[j] = result<false, OUT>(a[j], 0.f, b, e);
                 store_lanes<OUT, TOGETHER>(res, [&](int j) { return t0 + c + j * cluster; }, [&](int j) { return j < n; }, f, n_feat, a);
             }
         }
@@ -581,7 +581,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             mbar_init(smem_u32(&empty_bar[s]), 1);
         }
         for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&acc_full[i]), 1);
-        mbar_init(smem_u32(&next_bar), 8);                     // one arrival per epilogue warp of the pair
+        mbar_init(smem_u32(&next_bar), 16);                    // one arrival per epilogue warp of the pair
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -687,8 +687,8 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             }
         }
     } else {
-        // a thread has a token, and 32 of its features at a time
-        const int lane_base = (warp & 3) * 32;
+        // a thread has a token, and 32 of its features at a time; two warps share a quarter of the tokens and take turns at the runs
+        const int lane_base = (warp & 3) * 32, half = (warp - 2) >> 2;
         const uint32_t next_first = in_first_cta(smem_u32(&next_bar));
         wait_for_previous_kernels();
         const Epilogue e = load_epilogue<DUAL>(constants, act);
@@ -708,23 +708,26 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             const uint32_t trow = tmem_base + ((uint32_t)lane_base << 16) + (uint32_t)((i & 1) * SECOND_ACC);
             constexpr int RUNS = FEATS / 32;
 #pragma unroll 1
-            for (int n = 0; n < RUNS; ++n) {
-                // the first accumulator shares its last columns, the second its first
+            for (int n = half; n < RUNS; n += 2) {
+                // the first accumulator shares its last columns, the second its first: those are read in the first turn
                 const int c = ((i & 1) ? n : RUNS - 1 - n) * 32, f = f0 + c;
                 float v[32], u[DUAL ? 32 : 1];
                 tmem_ld32(trow + c, reinterpret_cast<uint32_t*>(v));
                 if (DUAL) tmem_ld32(trow + ROWS + c, reinterpret_cast<uint32_t*>(u));
                 tmem_wait_ld();
-                if (n == 0) {
+                if (n == half) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) arrive_cluster(next_first);
                 }
                 if (f >= (OUT == OUT_ROWS ? res.n_spans * SPAN : n_feat) || t >= n_tok) continue;
-                const bool biased = !DUAL && !e.act && OUT != OUT_ADD && e.constants != nullptr;
+                if (DUAL || e.act) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    v[j] = result<DUAL, OUT>(v[j], DUAL ? u[j] : 0.f, biased && f + j < n_feat ? e.constants[f + j] : 0.f, e);
+                    for (int j = 0; j < 32; ++j) v[j] = result<DUAL, OUT>(v[j], DUAL ? u[j] : 0.f, 0.f, e);
+                } else if (OUT != OUT_ADD && e.constants != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] += f + j < n_feat ? e.constants[f + j] : 0.f;
+                }
                 store_run<OUT>(res, t, f, n_feat, aligned, v);
             }
         }
@@ -791,27 +794,60 @@ struct Call {
 
 int columns(int need) { return need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512; }
 
-// How a product is cut: on pairs of SMs, or into tiles of tn tokens with K over the CTAs of a cluster.
+// How a product is cut: on pairs of SMs, or into tiles of tn tokens with K over the CTAs of a cluster, one or two CTAs to an SM.
 struct Plan {
     bool pairs;
-    int tn, cluster;
+    int tn, cluster, per_sm;
 };
-int g_pair_tokens = 256;         // products of at least so many tokens run on pairs of SMs
+int g_pair_tokens = 0;           // > 0: products of at least so many tokens run on pairs of SMs, others do not (tests)
 
-int g_cluster = 0, g_per_sm = 0;
+// What a product takes, in units of 10 ns, from measurements of the products of models 896 to 4,096 wide (weights from memory), good to a tenth
+// where no other product of the rule is near (tn: tokens of the tile):
+//   first kernel, not cut   a round of tiles: 12.5 + 0.066 tn a span, and 100 beside the next one's; once 190 + 1.85 tn
+//   cut over clusters       the same for the spans of a CTA; once 320 + 2.2 tn, and the codes at 6 TB/s
+//   pairs                   a round of tiles: 36 a span, and 100; once 700 (stores of 256 tokens that nothing runs beside)
+// So a product of [3584, 3584] (us, first kernel / pairs) with 256 tokens takes 10.1 / 15.5, 1,024: 17.8 / 18.6, 2,048: 30.0 / 28.3, and of
+// [3584, 18944] 24.4 / 50, 66.7 / 55.2 and 128 / 108; of [2048, 2048] with 64 tokens, not cut / in clusters of four, 5.3 / 5.7, of [3584, 3584]
+// 7.5 / 7.1, of [3584, 18944] 30 / 13.1.
 Plan plan(int n_tok, int n_feat, int n_spans, bool dual) {
     Plan p;
-    p.pairs = n_tok >= g_pair_tokens;
-    if (p.pairs) {
-        p.tn = ROWS;
-        p.cluster = 1;
-        return p;
-    }
     p.tn = n_tok >= TOKENS_MOST ? TOKENS_MOST : (n_tok + 15) / 16 * 16;
-    const long long tiles = (long long)((n_feat + ROWS - 1) / ROWS) * ((n_tok + p.tn - 1) / p.tn);
-    p.cluster = 1;
-    while (p.cluster < CLUSTER_MOST && tiles * (p.cluster + 1) <= 2 * sm_count() - 20 && n_spans >= 2 * (p.cluster + 1)) ++p.cluster;
-    if (g_cluster) p.cluster = g_cluster < n_spans ? g_cluster : n_spans;
+    p.cluster = p.per_sm = 1;
+    const long long sms = sm_count(), feat_tiles = (n_feat + ROWS - 1) / ROWS, tiles = feat_tiles * ((n_tok + p.tn - 1) / p.tn);
+    if (dual) {
+        // Gated products fill the ring with two matrices, and a cluster's exchange costs them what it saves.  On pairs a tile has twice the
+        // tokens and reads them once for both matrices: beyond 128 tokens always (200 tokens, 148 tiles 45.0 / 29.3 us), from 72 where a
+        // round is enough (96 tokens, 38 tiles 11.7 / 9.6, 70 tiles 14.3 / 12.0; 86 tiles, two rounds, 16.4 / 18.7).
+        p.pairs = n_tok > TOKENS_MOST || (n_tok >= 72 && 2 * feat_tiles <= sms);
+    } else {
+        const double span = 12.5 + 0.066 * p.tn, rounds = (double)((tiles + sms - 1) / sms);
+        const double meet = 320 + 2.2 * p.tn + (double)n_feat * n_spans * (SPAN / 2) / 6e4;
+        double best = rounds * (span * n_spans + 100) + 90 + 1.85 * p.tn;
+        for (int c = 2; c <= CLUSTER_MOST && c <= n_spans; ++c) {
+            // Clusters of whole SMs lie within groups of SMs, and those of the next kernel come in while these leave: large ones find their place
+            // late where they are many (16 clusters of 7: 12.2 us, of 4: 7.1).
+            if (tiles * c > (c > 4 ? sms * 2 / 3 : blocks_alone((const void*)mx_feature_kernel<false, OUT_F32>, THREADS, SMEM_LIMIT, c))) continue;
+            const double cost = span * ((n_spans + c - 1) / c) + meet;
+            if (cost < best) {
+                best = cost;
+                p.cluster = c;
+            }
+        }
+        // Up to 16 tokens, whose stages are small, twice the CTAs keep more copies in flight where each still has a long piece of K
+        // (8 tokens, us, one CTA per SM / two: [3584, 18944] 11.6 / 10.9, [4096, 14336] 10.4 / 10.0, [6144, 4096] 7.3 / 6.9).
+        if (n_tok <= 16 && n_spans / p.cluster >= 14) {
+            const long long most = 2 * (sms - 10) / tiles;
+            const int c = (int)(most < CLUSTER_MOST ? most : CLUSTER_MOST);
+            if (c > p.cluster) {
+                p.cluster = c;
+                p.per_sm = 2;
+            }
+        }
+        const long long pair_tiles = (long long)((n_tok + PAIR_TOK - 1) / PAIR_TOK) * ((n_feat + PAIR_ROWS - 1) / PAIR_ROWS), pairs = sms / 2;
+        p.pairs = n_tok > TOKENS_MOST && ((pair_tiles + pairs - 1) / pairs) * (36.0 * n_spans + 100) + 700 < best;
+    }
+    if (g_pair_tokens > 0) p.pairs = n_tok >= g_pair_tokens;
+    if (p.pairs) p.tn = ROWS;
     return p;
 }
 
@@ -825,24 +861,27 @@ int launch_feature(const Call& c) {
     if (int rc = raise_dynamic_smem(kernel, SMEM_LIMIT, configured, "gemm_microscaled")) return rc;
     constexpr int MATS = DUAL ? 2 : 1;
     const int stage = MATS * TILE + p.tn * SPAN + (MATS + 1) * PIECE;
-    const int recv = p.cluster > 1 ? p.cluster * ((p.tn + p.cluster - 1) / p.cluster) * MATS * ROWS * 4 : 0;
+    const int recv = p.cluster > 1 ? p.cluster * ((p.tn + p.cluster - 1) / p.cluster) * ROWS * 4 : 0;
     const int most = (c.n_spans + p.cluster - 1) / p.cluster;            // spans of a CTA
-    int stages = ((g_per_sm == 1 ? SMEM_LIMIT : g_per_sm == 3 ? 150 * 1024 : g_per_sm == 4 ? 185 * 1024 : 112 * 1024) - 1024) / stage;
+    // A ring fills the SM, also where a next kernel's could begin in half of it: what is on its way from memory is what these products wait for
+    // (8 tokens, a gated product of [18944, 3584]: 102 KB of codes on their way 16.2 us, 51 KB 19.6).
+    int stages = ((p.per_sm == 2 ? SMEM_LIMIT / 2 : SMEM_LIMIT) - 1024) / stage;
     if (stages > MAX_STAGES) stages = MAX_STAGES;
     if (p.cluster > 1 && stages > most) stages = most;
     const size_t ring = (size_t)stages * stage;
     size_t smem = (ring > (size_t)recv ? ring : (size_t)recv) + 1024;
-    long long ctas = p.cluster > 1 ? tiles * p.cluster : tiles;
+    long long ctas = tiles * p.cluster;
+    if (p.cluster == 1 && ctas > sm_count()) ctas = sm_count();
+    // two accumulators, so that a tile's epilogue runs beside the next one's MMAs, where a CTA has several tiles and the columns suffice
     constexpr int EXP_COLS = 2 * (MATS + 1) * 4;
-    const int per_sm = smem <= 113 * 1024 && 2 * columns(MATS * p.tn + EXP_COLS) <= 512 ? 2 : 1;
-    if (p.cluster == 1 && ctas > per_sm * sm_count()) ctas = per_sm * sm_count();
-    int buffers = (p.cluster > 1 || ctas == tiles) ? 1 : 2;
-    if (per_sm * columns(buffers * MATS * p.tn + EXP_COLS) > 512) buffers = 1;
-    const int cols = columns(buffers * MATS * p.tn + EXP_COLS);
+    const int one = MATS * p.tn + EXP_COLS, two = one + MATS * p.tn;
+    const int buffers = (p.cluster == 1 && ctas < tiles && two <= 512) ? 2 : 1;
+    const int need = buffers == 2 ? two : one, cols = columns(need);
+    if (need > 512 || stages < 1 || smem > (size_t)SMEM_LIMIT) return fail("gemm_microscaled: %d columns of tensor memory, %lld bytes of shared memory", need, (long long)smem);
     // CTAs that wait for others of their cluster must not wait for tensor memory that CTAs of another cluster hold, which may wait likewise:
     // shared memory in proportion to their columns keeps all that an SM takes in within its 512 columns.
     if (p.cluster > 1 && smem < (size_t)cols * 456) smem = (size_t)cols * 456 < SMEM_LIMIT ? (size_t)cols * 456 : SMEM_LIMIT;
-    return launch_cluster("gemm_microscaled", kernel, dim3((unsigned)ctas), FEW_THREADS, smem, p.cluster, c.stream, c.w->codes, c.w2->codes, c.x->codes, c.w_exp,
+    return launch_cluster("gemm_microscaled", kernel, dim3((unsigned)ctas), THREADS, smem, p.cluster, c.stream, c.w->codes, c.w2->codes, c.x->codes, c.w_exp,
                           c.w2_exp, c.x_exp, c.constants, c.act, c.res, c.n_tok, c.n_feat, c.n_spans, p.cluster, stages, p.tn, buffers, cols, c.status);
 }
 
@@ -883,11 +922,7 @@ RI_API int ri_mx_encode(void* maps_out, const void* codes, const void* exponents
     return encode_pieces(&maps->exponents, exponents, pieces);
 }
 
-// Products of at least so many tokens run on pairs of SMs (for comparisons and tests).
-RI_API int ri_mx_set_plan(int cluster, int per_sm) {
-    g_cluster = cluster; g_per_sm = per_sm;
-    return 0;
-}
+// tokens > 0: products of at least so many tokens run on pairs of SMs, others do not; 0: as planned (for comparisons and tests).
 RI_API int ri_mx_set_pairs(int tokens) {
     g_pair_tokens = tokens;
     return 0;

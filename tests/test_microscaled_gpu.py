@@ -145,7 +145,7 @@ def bound(k, mass, y, dtype):
 
 PRODUCTS = [(1, 1, 1), (1, 128, 128), (2, 130, 64), (1, 896, 896), (7, 1000, 1333), (8, 3584, 3584), (16, 257, 2048), (17, 640, 384), (33, 129, 4097),
             (64, 2560, 2048), (61, 300, 8960), (100, 129, 640), (127, 1152, 896), (128, 256, 512), (129, 200, 300), (200, 5000, 256), (333, 2560, 2048),
-            (1000, 640, 1536), (3, 40000, 160), (5, 128, 18944)]
+            (1000, 640, 1536), (3, 40000, 160), (5, 128, 18944), (130, 41000, 200)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -176,7 +176,7 @@ def test_product(m, n, k, dtype):
 
 @pytest.mark.parametrize("form", [None, "bounded"])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 4864, 896), (8, 1000, 1333), (9, 18944, 256), (16, 300, 2048), (31, 640, 640), (64, 1100, 512), (100, 256, 2048),
-                                   (128, 700, 300), (129, 200, 300), (333, 1500, 640), (700, 129, 1000)])
+                                   (128, 700, 300), (129, 200, 300), (333, 1500, 640), (700, 129, 1000), (200, 20000, 130), (128, 25000, 129)])
 def test_gated_and_into_eight_bits(m, n, k, form):
     from rust_inference_b200.kernels import linear, microscaled, ops
     ctx = context()

@@ -776,12 +776,30 @@ int encode_pieces(CUtensorMap* map, const void* ptr, long long pieces) {
     return 0;
 }
 
-// The tensor maps that a matrix or rows keep: of the codes, and of the exponents.
+// The tensor maps that a matrix or rows keep: of the codes, with boxes of so many rows, and of the exponents.
 struct Maps {
     CUtensorMap codes, exponents;
 };
+static_assert(sizeof(Maps) == sizeof(Held::maps[0]), "a pair of maps");
+int maps_of(Held* h, int box_rows, const Maps** found) {
+    const int i = box_rows / 16 - 1;
+    Maps* m = reinterpret_cast<Maps*>(h->maps[i]);
+    if (!(h->made.load(std::memory_order_acquire) >> i & 1u)) {
+        if (int rc = encode_codes(&m->codes, h->codes, h->n, h->n_spans, h->bits, box_rows)) return rc;
+        if (int rc = encode_pieces(&m->exponents, h->exponents, (long long)(h->n + ROWS - 1) / ROWS * h->n_spans)) return rc;
+        h->made.fetch_or(1u << i, std::memory_order_release);
+    }
+    *found = m;
+    return 0;
+}
 
+// How a product is cut: on pairs of SMs, or into tiles of tn tokens with K over the CTAs of a cluster, one or two CTAs to an SM.
+struct Plan {
+    bool pairs;
+    int tn, cluster, per_sm;
+};
 struct Call {
+    Plan plan;
     const Maps *w, *w2, *x;
     const uint8_t *w_exp, *w2_exp, *x_exp;
     const float* constants;
@@ -794,11 +812,6 @@ struct Call {
 
 int columns(int need) { return need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512; }
 
-// How a product is cut: on pairs of SMs, or into tiles of tn tokens with K over the CTAs of a cluster, one or two CTAs to an SM.
-struct Plan {
-    bool pairs;
-    int tn, cluster, per_sm;
-};
 int g_pair_tokens = 0;           // > 0: products of at least so many tokens run on pairs of SMs, others do not (tests)
 
 // What a product takes, in units of 10 ns, from measurements of the products of models 896 to 4,096 wide (weights from memory), good to a tenth
@@ -853,7 +866,7 @@ Plan plan(int n_tok, int n_feat, int n_spans, bool dual) {
 
 template <bool DUAL, int OUT>
 int launch_feature(const Call& c) {
-    const Plan p = plan(c.n_tok, c.n_feat, c.n_spans, DUAL);
+    const Plan& p = c.plan;
     const long long tiles = (long long)((c.n_tok + p.tn - 1) / p.tn) * ((c.n_feat + ROWS - 1) / ROWS);
     if (tiles > 0x7fffffffLL / CLUSTER_MOST) return fail("gemm_microscaled: %lld tiles exceed the index range", tiles);
     auto kernel = mx_feature_kernel<DUAL, OUT>;
@@ -904,23 +917,10 @@ int launch_pair(const Call& c) {
 
 template <bool DUAL, int OUT>
 int launch(const Call& c) {
-    return plan(c.n_tok, c.n_feat, c.n_spans, DUAL).pairs ? launch_pair<DUAL, OUT>(c) : launch_feature<DUAL, OUT>(c);
+    return c.plan.pairs ? launch_pair<DUAL, OUT>(c) : launch_feature<DUAL, OUT>(c);
 }
 
 }  // namespace
-
-// The tensor maps of codes [rows, spans * 128] of `bits` (4 or 8) bits and of their exponents, into the 256 bytes at `maps_out` (64-byte
-// aligned).  box_rows: 128 for a matrix, `ri_mx_box` for rows.
-RI_API int ri_mx_encode(void* maps_out, const void* codes, const void* exponents, long long rows, int n_spans, int bits, int box_rows) {
-    if ((uintptr_t)maps_out % 64) return fail("gemm_microscaled: tensor map storage must be 64-byte aligned");
-    if (rows <= 0 || n_spans <= 0 || (bits != 4 && bits != 8) || box_rows < 8 || box_rows > 256)
-        return fail("gemm_microscaled: no map of [%lld, %d] in %d bits with boxes of %d rows", rows, n_spans, bits, box_rows);
-    const long long pieces = (rows + ROWS - 1) / ROWS * n_spans;
-    if (pieces > 0x7fffffffLL) return fail("gemm_microscaled: %lld pieces of exponents exceed the index range", pieces);
-    Maps* maps = reinterpret_cast<Maps*>(maps_out);
-    if (int rc = encode_codes(&maps->codes, codes, rows, n_spans, bits, box_rows)) return rc;
-    return encode_pieces(&maps->exponents, exponents, pieces);
-}
 
 // tokens > 0: products of at least so many tokens run on pairs of SMs, others do not; 0: as planned (for comparisons and tests).
 RI_API int ri_mx_set_pairs(int tokens) {
@@ -928,45 +928,46 @@ RI_API int ri_mx_set_pairs(int tokens) {
     return 0;
 }
 
-// Rows of the box of a product's X.
-RI_API int ri_mx_box(int n_tok, int n_feat, int n_spans, int dual) { return plan(n_tok, n_feat, n_spans, dual != 0).tn; }
-
-// `kind`: what is written (`Out`); `dual`: gated, with the second matrix; `act`: `constants` are an activation's.  out_exp, out_spans: with rows in 8 bits.
-RI_API int ri_mx_gemm(const void* maps_w, const void* maps_w2, const void* maps_x, const void* w_exp, const void* w2_exp, const void* x_exp,
-                      const float* constants, int dual, int act, int kind, void* out, void* out_exp, int out_spans, int n_tok, int n_feat, int n_spans,
-                      int* status, cudaStream_t stream) {
-    if (n_tok <= 0 || n_feat <= 0) return 0;
-    if (n_spans <= 0) return fail("gemm_microscaled: rows without numbers");
-    if (kind < OUT_BF16 || kind > OUT_ADD || (dual && act) || (kind == OUT_ADD && (dual || act || constants != nullptr)) || (act && constants == nullptr))
-        return fail("gemm_microscaled: no epilogue %d (gated %d, activated %d)", kind, dual, act);
+// out = X W^T with an epilogue: a bias or nothing (`constants` float32 [features] or null); `act`: an activation's four constants; w2 not null:
+// the gate's five constants, or null for silu; `add`: added to out.  x, w, w2 and, where the result is rows in 8 bits, out_held are `Held`s; otherwise
+// `out` is [out_rows, out_cols] of `out_dtype`.  `status` is a host-visible int that receives a code if a wait ran out.
+RI_API int ri_mx_product(void* x_held, void* w_held, void* w2_held, const float* constants, long long n_constants, int act, int add, void* out,
+                         int out_dtype, long long out_rows, long long out_cols, void* out_held, int* status, cudaStream_t stream) {
+    Held *x = (Held*)x_held, *w = (Held*)w_held, *w2 = (Held*)w2_held, *to = (Held*)out_held;
+    int device = -1;
+    if (cudaGetDevice(&device) != cudaSuccess || x->device != device || w->device != device || (w2 && w2->device != device) || (to && to->device != device))
+        return fail("gemm_microscaled: rows and matrices lie on the current device");
+    if (x->bits != 8 || w->bits != 4 || x->k != w->k || (w2 && (w2->bits != 4 || w2->n != w->n || w2->k != w->k)))
+        return fail("gemm_microscaled: rows [%d, %d] in %d bits and a matrix [%d, %d] in %d", x->n, x->k, x->bits, w->n, w->k, w->bits);
+    if (to ? (to->bits != 8 || to->n != x->n || to->k != w->n) : (out_rows != x->n || out_cols != w->n))
+        return fail("gemm_microscaled: the result is [%d, %d]", x->n, w->n);
+    if (to && (to->codes == x->codes || to->exponents == x->exponents)) return fail("gemm_microscaled: rows cannot be their own product");
+    if (add && (to || out_dtype != RI_F32)) return fail("gemm_microscaled: sums are added to float32 numbers");
+    if ((act != 0) + (add != 0) + (w2 != nullptr) > 1 || (add && constants)) return fail("gemm_microscaled: a bias, an activation, a gate and an addition are not combined");
+    if ((act && !constants) || (constants && n_constants != (act ? 4 : w2 ? 5 : w->n)))
+        return fail("gemm_microscaled: %lld constants of an epilogue", n_constants);
+    const Plan p = plan(x->n, w->n, w->n_spans, w2 != nullptr);
     Call c;
-    c.w = reinterpret_cast<const Maps*>(maps_w);
-    c.w2 = reinterpret_cast<const Maps*>(dual ? maps_w2 : maps_w);
-    c.x = reinterpret_cast<const Maps*>(maps_x);
-    c.w_exp = (const uint8_t*)w_exp;
-    c.w2_exp = (const uint8_t*)w2_exp;
-    c.x_exp = (const uint8_t*)x_exp;
+    c.plan = p;
+    if (maps_of(x, p.tn, &c.x) || maps_of(w, ROWS, &c.w) || maps_of(w2 ? w2 : w, ROWS, &c.w2)) return 1;
+    c.x_exp = x->exponents;
+    c.w_exp = w->exponents;
+    c.w2_exp = w2 ? w2->exponents : nullptr;
     c.constants = constants;
     c.act = act;
-    c.res = Result{out, (uint8_t*)out_exp, out_spans};
-    c.n_tok = n_tok;
-    c.n_feat = n_feat;
-    c.n_spans = n_spans;
+    c.res = to ? Result{to->codes, to->exponents, to->n_spans} : Result{out, nullptr, 0};
+    c.n_tok = x->n;
+    c.n_feat = w->n;
+    c.n_spans = w->n_spans;
     c.status = status;
     c.stream = stream;
-    if (dual) {
-        switch (kind) {
-            case OUT_BF16: return launch<true, OUT_BF16>(c);
-            case OUT_F32: return launch<true, OUT_F32>(c);
-            default: return launch<true, OUT_ROWS>(c);
-        }
+    if (w2) {
+        if (to) return launch<true, OUT_ROWS>(c);
+        return out_dtype == RI_BF16 ? launch<true, OUT_BF16>(c) : launch<true, OUT_F32>(c);
     }
-    switch (kind) {
-        case OUT_BF16: return launch<false, OUT_BF16>(c);
-        case OUT_F32: return launch<false, OUT_F32>(c);
-        case OUT_ROWS: return launch<false, OUT_ROWS>(c);
-        default: return launch<false, OUT_ADD>(c);
-    }
+    if (to) return launch<false, OUT_ROWS>(c);
+    if (add) return launch<false, OUT_ADD>(c);
+    return out_dtype == RI_BF16 ? launch<false, OUT_BF16>(c) : launch<false, OUT_F32>(c);
 }
 
 RI_DEFINE_LAST_ERROR()

@@ -198,11 +198,11 @@ int blocks_for(uint32_t groups) {
     return (int)(want < most ? want : most);
 }
 
-int sizes(const char* what, long long n, long long k, uint32_t* groups) {
-    if (n < 0 || k < 0 || n > 0x7fffffffLL || k > 0x7fffffffLL - SPAN) return fail("%s: [%lld, %lld] numbers", what, n, k);
-    const long long g = n * spans((int)k) * (SPAN / 8);
-    if (g > 0x7fffffffLL) return fail("%s: [%lld, %lld] numbers are more than are counted in 31 bits of eight", what, n, k);
-    *groups = (uint32_t)g;
+// Groups of eight numbers of what is held, which must lie on the current device.
+int groups_of(const char* what, const Held* h, uint32_t* groups) {
+    int device = -1;
+    if (cudaGetDevice(&device) != cudaSuccess || device != h->device) return fail("%s: what is held lies on device %d, the current one is %d", what, h->device, device);
+    *groups = (uint32_t)((long long)h->n * h->n_spans * (SPAN / 8));
     return 0;
 }
 
@@ -242,38 +242,59 @@ int norm(const float* x, const void* branch, const float* weight, float* total, 
 
 }  // namespace
 
-// x [n, k] (rows `ld` numbers apart) to codes of `bits` (4 or 8) bits and their exponents.
-RI_API int ri_mx_hold(const void* x, int dtype, int bits, long long n, long long k, long long ld, void* codes, void* exponents, cudaStream_t stream) {
-    uint32_t groups;
-    if (bits != 4 && bits != 8) return fail("mx_hold: numbers of 4 or 8 bits, not %d", bits);
-    if (int rc = sizes("mx_hold", n, k, &groups)) return rc;
-    if (ld < k) return fail("mx_hold: rows of %lld numbers lie %lld apart", k, ld);
-    if (groups == 0) return 0;
-    if (dtype == RI_BF16) return bits == 4 ? hold<__nv_bfloat16, 4>(x, (int)n, (int)k, ld, codes, exponents, groups, stream)
-                                           : hold<__nv_bfloat16, 8>(x, (int)n, (int)k, ld, codes, exponents, groups, stream);
-    return bits == 4 ? hold<float, 4>(x, (int)n, (int)k, ld, codes, exponents, groups, stream)
-                     : hold<float, 8>(x, (int)n, (int)k, ld, codes, exponents, groups, stream);
+// Bytes of a `Held`, 64-byte aligned.
+RI_API long long ri_mx_held_bytes() { return (long long)sizeof(Held); }
+
+// A `Held` at `at`: [n, k] numbers of `bits` bits (4: a matrix, 8: rows) over these buffers of the device `device`.
+RI_API int ri_mx_make(void* at, void* codes, void* exponents, long long n, long long k, int bits, int device) {
+    if ((uintptr_t)at % 64) return fail("mx_make: 64-byte aligned memory is wanted");
+    if (n <= 0 || k <= 0 || k > 0x7fffffffLL - SPAN || (bits != 4 && bits != 8)) return fail("mx_make: no [%lld, %lld] numbers of %d bits", n, k, bits);
+    if (n * spans((int)k) > 0x7fffffffLL / (SPAN / 8)) return fail("mx_make: [%lld, %lld] numbers are more than 2^31 eights", n, k);
+    if ((uintptr_t)codes % 32 || (uintptr_t)exponents % 32) return fail("mx_make: buffers must begin on a 32-byte boundary");
+    Held* h = new (at) Held;
+    h->codes = (uint8_t*)codes;
+    h->exponents = (uint8_t*)exponents;
+    h->n = (int)n;
+    h->k = (int)k;
+    h->n_spans = spans((int)k);
+    h->bits = bits;
+    h->device = device;
+    h->made.store(0);
+    return 0;
 }
 
-// The numbers [n, k] that codes of `bits` bits stand for.
-RI_API int ri_mx_values(const void* codes, const void* exponents, int dtype, int bits, long long n, long long k, void* out, cudaStream_t stream) {
+// x [n, k] (rows `ld` numbers apart) to what is held.
+RI_API int ri_mx_hold(const void* x, int dtype, long long n, long long k, long long ld, void* held, cudaStream_t stream) {
+    const Held* h = (const Held*)held;
     uint32_t groups;
-    if (bits != 4 && bits != 8) return fail("mx_values: numbers of 4 or 8 bits, not %d", bits);
-    if (int rc = sizes("mx_values", n, k, &groups)) return rc;
-    if (groups == 0) return 0;
-    if (dtype == RI_BF16) return bits == 4 ? values<__nv_bfloat16, 4>(codes, exponents, (int)k, out, groups, stream)
-                                           : values<__nv_bfloat16, 8>(codes, exponents, (int)k, out, groups, stream);
-    return bits == 4 ? values<float, 4>(codes, exponents, (int)k, out, groups, stream) : values<float, 8>(codes, exponents, (int)k, out, groups, stream);
+    if (n != h->n || k != h->k || ld < k) return fail("mx_hold: [%lld, %lld] numbers, rows %lld apart, do not go into [%d, %d]", n, k, ld, h->n, h->k);
+    if (int rc = groups_of("mx_hold", h, &groups)) return rc;
+    if (dtype == RI_BF16) return h->bits == 4 ? hold<__nv_bfloat16, 4>(x, h->n, h->k, ld, h->codes, h->exponents, groups, stream)
+                                              : hold<__nv_bfloat16, 8>(x, h->n, h->k, ld, h->codes, h->exponents, groups, stream);
+    return h->bits == 4 ? hold<float, 4>(x, h->n, h->k, ld, h->codes, h->exponents, groups, stream)
+                        : hold<float, 8>(x, h->n, h->k, ld, h->codes, h->exponents, groups, stream);
 }
 
-// total = stream + branch (branch null: the stream itself; total null: not kept; it may be the stream), and the norm of it times `weight` in 8 bits.
+// out [n, k]: the numbers that are held.
+RI_API int ri_mx_values(const void* held, int dtype, long long n, long long k, void* out, cudaStream_t stream) {
+    const Held* h = (const Held*)held;
+    uint32_t groups;
+    if (n != h->n || k != h->k) return fail("mx_values: [%d, %d] numbers do not go into [%lld, %lld]", h->n, h->k, n, k);
+    if (int rc = groups_of("mx_values", h, &groups)) return rc;
+    if (dtype == RI_BF16) return h->bits == 4 ? values<__nv_bfloat16, 4>(h->codes, h->exponents, h->k, out, groups, stream)
+                                              : values<__nv_bfloat16, 8>(h->codes, h->exponents, h->k, out, groups, stream);
+    return h->bits == 4 ? values<float, 4>(h->codes, h->exponents, h->k, out, groups, stream) : values<float, 8>(h->codes, h->exponents, h->k, out, groups, stream);
+}
+
+// total = stream + branch (branch null: the stream itself; total null: not kept; it may be the stream), [n, k], and the norm of it times `weight` in 8 bits.
 RI_API int ri_mx_rmsnorm(const float* x, const void* branch, int branch_dtype, const float* weight, float* total, long long n, long long k, double eps,
-                         void* codes, void* exponents, cudaStream_t stream) {
+                         void* held, cudaStream_t stream) {
+    const Held* h = (const Held*)held;
     uint32_t groups;
-    if (int rc = sizes("mx_rmsnorm", n, k, &groups)) return rc;
-    if (groups == 0) return 0;
-    return branch_dtype == RI_BF16 ? norm<__nv_bfloat16>(x, branch, weight, total, (int)n, (int)k, eps, codes, exponents, stream)
-                                   : norm<float>(x, branch, weight, total, (int)n, (int)k, eps, codes, exponents, stream);
+    if (n != h->n || k != h->k || h->bits != 8) return fail("mx_rmsnorm: a norm of [%lld, %lld] does not go into [%d, %d] of %d bits", n, k, h->n, h->k, h->bits);
+    if (int rc = groups_of("mx_rmsnorm", h, &groups)) return rc;
+    return branch_dtype == RI_BF16 ? norm<__nv_bfloat16>(x, branch, weight, total, h->n, h->k, eps, h->codes, h->exponents, stream)
+                                   : norm<float>(x, branch, weight, total, h->n, h->k, eps, h->codes, h->exponents, stream);
 }
 
 RI_DEFINE_LAST_ERROR()

@@ -14,12 +14,23 @@
 #include <cuda_fp4.h>
 #include <cuda_fp8.h>
 
+#include <new>
+
 namespace ri {
 namespace mx {
 
 constexpr int BLOCK = 32;              // numbers that share an exponent
 constexpr int SPAN = 128;              // numbers of a row that one step of a product takes
 constexpr int PIECE = 512;             // bytes of exponents of 128 rows and one span
+
+// A matrix or rows as the entry points take them: host memory of the caller's, made by `ri_mx_make` once, beside the device's buffers.  The
+// products' tensor maps are encoded when they are first wanted, a pair (codes, exponents) for every 16 rows of a box.
+struct Held {
+    uint8_t *codes, *exponents;
+    int n, k, n_spans, bits, device;
+    std::atomic<uint32_t> made;            // which of the maps are there
+    alignas(64) unsigned char maps[8][256];
+};
 
 __host__ __device__ __forceinline__ int spans(int k) { return (k + SPAN - 1) / SPAN; }
 __device__ __forceinline__ size_t exponent_at(int row, int block, int n_spans) {

@@ -3,7 +3,7 @@
 // for twenty to thirty arguments that are looked at and converted one by one in Python; from here it is 3.1 to 3.8 us (6.4), of
 // which the launch is 2.7.
 //
-// The functions take their arguments by position (kernels/quantized_cache.py and kernels/ops.py have the interfaces and their
+// The functions take their arguments by position (kernels/quantized_cache.py, kernels/microscaled.py and kernels/ops.py have the interfaces and their
 // documentation).  `bind` names the entry points, by address, and the exception class that refusals and failed launches raise.
 #include <Python.h>
 
@@ -24,8 +24,8 @@ struct Bound {
     void* fn = nullptr;
     const char* (*last_error)() = nullptr;
 };
-Bound bound[4];
-enum { WRITE = 0, READ = 1, ATTEND = 2, LOGPROBS = 3 };
+enum { WRITE = 0, READ = 1, ATTEND = 2, LOGPROBS = 3, MX_HOLD = 4, MX_VALUES = 5, MX_NORM = 6, MX_PRODUCT = 7, ENTRIES = 8 };
+Bound bound[ENTRIES];
 
 struct Refused {                                 // thrown with a message for `error_class`
     std::string what;
@@ -276,12 +276,110 @@ PyObject* py_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// ---- microscaled ---------------------------------------------------------------------------------------------------------
+// What is held comes as the address of its description in host memory (`Held`, microscaled.cuh); its library looks at that.
+bool here(const at::Tensor& t) { return t.is_cuda() && t.get_device() == c10::cuda::current_device(); }
+const at::Tensor& rows(PyObject* o, const char* what) {                 // numbers of a row lie side by side
+    const at::Tensor& t = tensor(o, what);
+    if (!here(t) || t.dim() != 2 || (t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1)))
+        refuse(std::string(what) + ": rows [n, k] on the current device, their numbers side by side, are wanted");
+    return t;
+}
+const at::Tensor& dense(PyObject* o, const char* what) {
+    const at::Tensor& t = tensor(o, what);
+    if (!here(t) || t.dim() != 2 || !t.is_contiguous()) refuse(std::string(what) + ": a contiguous [n, k] on the current device is wanted");
+    return t;
+}
+typedef int MxHoldFn(const void*, int, long long, long long, long long, void*, void*);
+void mx_hold(const at::Tensor& x, void* held, const char* what) {
+    finish(entry<MxHoldFn>(MX_HOLD)(x.data_ptr(), code_of(x, what), x.size(0), x.size(1), x.size(0) > 1 ? x.stride(0) : x.size(1), held, stream()), MX_HOLD, what);
+}
+// (x, held)
+PyObject* py_mx_hold(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n == 2, "microscaled: 2 arguments");
+        mx_hold(rows(a[0], "microscaled"), address<void>(number(a[1])), "microscaled");
+        Py_RETURN_NONE;
+    });
+}
+// (held, out)
+typedef int MxValuesFn(const void*, int, long long, long long, void*, void*);
+PyObject* py_mx_values(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const char* what = "microscaled.values";
+        need(n == 2, "microscaled.values: 2 arguments");
+        const at::Tensor& out = dense(a[1], what);
+        finish(entry<MxValuesFn>(MX_VALUES)(address<void>(number(a[0])), code_of(out, what), out.size(0), out.size(1), out.data_ptr(), stream()), MX_VALUES, what);
+        Py_RETURN_NONE;
+    });
+}
+// (x, branch or None, weight, total or None, eps, held)
+typedef int MxNormFn(const float*, const void*, int, const float*, float*, long long, long long, double, void*, void*);
+PyObject* py_mx_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const char* what = "microscaled.rmsnorm";
+        need(n == 6, "microscaled.rmsnorm: 6 arguments");
+        const at::Tensor &x = dense(a[0], what), &weight = tensor(a[2], what);
+        need(x.scalar_type() == at::kFloat, "microscaled.rmsnorm: x must be float32");
+        need(here(weight) && weight.scalar_type() == at::kFloat && weight.is_contiguous() && weight.numel() == x.size(1), "microscaled.rmsnorm: weight must be float32 [k]");
+        const void* branch = nullptr;
+        int branch_code = 0;
+        if (a[1] != Py_None) {
+            const at::Tensor& b = dense(a[1], what);
+            need(b.sizes() == x.sizes(), "microscaled.rmsnorm: a branch as x is wanted");
+            branch = b.data_ptr();
+            branch_code = code_of(b, what);
+        }
+        float* total = nullptr;
+        if (a[3] != Py_None) {
+            const at::Tensor& t = dense(a[3], what);
+            need(t.scalar_type() == at::kFloat && t.sizes() == x.sizes(), "microscaled.rmsnorm: total must be float32, as x");
+            total = t.data_ptr<float>();
+        }
+        finish(entry<MxNormFn>(MX_NORM)(x.data_ptr<float>(), branch, branch_code, weight.data_ptr<float>(), total, x.size(0), x.size(1), real(a[4]),
+                                        address<void>(number(a[5])), stream()), MX_NORM, what);
+        Py_RETURN_NONE;
+    });
+}
+// (plain rows or None, held rows, matrix, second matrix or 0, constants or None, act, add, out or None, held result or 0, status word)
+typedef int MxProductFn(void*, void*, void*, const float*, long long, int, int, void*, int, long long, long long, void*, int*, void*);
+PyObject* py_mx_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const char* what = "microscaled.product";
+        need(n == 10, "microscaled.product: 10 arguments");
+        void* held = address<void>(number(a[1]));
+        const float* constants = nullptr;
+        long long n_constants = 0;
+        if (a[4] != Py_None) {
+            const at::Tensor& t = tensor(a[4], what);
+            need(here(t) && t.scalar_type() == at::kFloat && t.is_contiguous(), "microscaled.product: a bias or an activation's constants are contiguous float32 on the current device");
+            constants = t.data_ptr<float>();
+            n_constants = t.numel();
+        }
+        void* out = nullptr;
+        int out_code = 0;
+        long long out_rows = 0, out_cols = 0;
+        if (a[7] != Py_None) {
+            const at::Tensor& o = dense(a[7], what);
+            out = o.data_ptr();
+            out_code = code_of(o, what);
+            out_rows = o.size(0);
+            out_cols = o.size(1);
+        }
+        if (a[0] != Py_None) mx_hold(rows(a[0], what), held, what);
+        finish(entry<MxProductFn>(MX_PRODUCT)(held, address<void>(number(a[2])), address<void>(number(a[3])), constants, n_constants, (int)number(a[5]),
+                                              (int)number(a[6]), out, out_code, out_rows, out_cols, address<void>(number(a[8])), address<int>(number(a[9])),
+                                              stream()), MX_PRODUCT, what);
+        Py_RETURN_NONE;
+    });
+}
+
 // (which, address of the entry point, address of its library's ri_last_error, exception class)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         need(n == 4, "bind: 4 arguments");
         const long long which = number(a[0]);
-        need(which >= 0 && which < 4, "bind: no such entry point");
+        need(which >= 0 && which < ENTRIES, "bind: no such entry point");
         bound[which].fn = address<void>(number(a[1]));
         bound[which].last_error = reinterpret_cast<const char* (*)()>(static_cast<intptr_t>(number(a[2])));
         Py_INCREF(a[3]);
@@ -296,6 +394,8 @@ template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)> PyMethodDef m
     return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
 }
 PyMethodDef methods[] = {method<py_write>("write"), method<py_read>("read"), method<py_attend>("attend"), method<py_logprobs>("logprobs"),
+                         method<py_mx_hold>("mx_hold"), method<py_mx_values>("mx_values"), method<py_mx_rmsnorm>("mx_rmsnorm"),
+                         method<py_mx_product>("mx_product"),
                          method<py_bind>("bind"), method<py_launches>("launches"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "ri_native_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

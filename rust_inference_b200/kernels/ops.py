@@ -76,7 +76,9 @@ def launch_count() -> int:
 # Entry points that are called through the extension `csrc/native_calls.cpp` (which looks at the tensors itself): its name for
 # each, with the library and the function behind it
 _NATIVE = {"write": (0, "quantized_cache", "ri_quantized_write"), "read": (1, "quantized_cache", "ri_quantized_read"),
-           "attend": (2, "attention_quantized", "ri_attention_quantized"), "logprobs": (3, "token_logprobs", "ri_token_logprobs")}
+           "attend": (2, "attention_quantized", "ri_attention_quantized"), "logprobs": (3, "token_logprobs", "ri_token_logprobs"),
+           "mx_hold": (4, "microscaled", "ri_mx_hold"), "mx_values": (5, "microscaled", "ri_mx_values"),
+           "mx_rmsnorm": (6, "microscaled", "ri_mx_rmsnorm"), "mx_product": (7, "gemm_microscaled", "ri_mx_product")}
 _native_calls = None
 
 

@@ -15,144 +15,232 @@ namespace {
 
 constexpr int THREADS = 256;
 
-// Eight numbers of a row of k, from column c on; zeros behind its end.  WHOLE: rows are whole 16-byte pieces that begin on a 16-byte boundary.
-// (Volatile reads: rows may come from the kernel before, and these stay behind the wait for it.)
-template <typename T, bool WHOLE>
-__device__ __forceinline__ void load8(const T* row, int c, int k, float* v) {
-    if (WHOLE && c < k) {
-        if (sizeof(T) == 2) {
-            const float4 raw = load_written(reinterpret_cast<const float*>(row + c));
-            unpack8(*reinterpret_cast<const uint4*>(&raw), v);
-        } else {
-            const float4 a = load_written(reinterpret_cast<const float*>(row + c)), b = load_written(reinterpret_cast<const float*>(row + c) + 4);
+// Eight consecutive numbers of a row.  WHOLE: rows are whole eights that begin on a 16-byte boundary.  (Reads that stay behind the wait for the
+// kernel before, which may have written them.)
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+    float v[8];
+    // from column c on of a row of k; zeros behind its end
+    template <bool WHOLE> __device__ __forceinline__ void load(const float* row, int c, int k) {
+        if (WHOLE && c < k) {
+            const float4 a = load_written(row + c), b = load_written(row + c + 4);
             v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
             v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = !WHOLE && c + i < k ? const_cast<const volatile float*>(row)[c + i] : 0.f;
         }
-        return;
     }
+    // the largest magnitude, as a float's bits (a NaN's are larger than any number's)
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t t = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < k ? to_f32<T>(const_cast<const volatile T*>(row)[c + i]) : 0.f;
-}
-template <> __device__ __forceinline__ void load8<__nv_bfloat16, false>(const __nv_bfloat16* row, int c, int k, float* v) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const unsigned short raw = c + i < k ? reinterpret_cast<const volatile unsigned short*>(row)[c + i] : (unsigned short)0;
-        v[i] = __uint_as_float((uint32_t)raw << 16);
+        for (int i = 0; i < 8; ++i) t = max(t, __float_as_uint(v[i]) & 0x7fffffffu);
+        return t;
     }
-}
-
-// Eight numbers of one thread, whose block four neighbouring threads hold, to codes and exponent.
-template <int BITS>
-__device__ __forceinline__ void store8(const float* v, int row, int c, int n_spans, uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents) {
-    uint32_t top = 0;
+    __device__ __forceinline__ void scaled(uint32_t byte, float* y) const {          // times 2^-e
+        const float f = to_type(byte);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    const uint32_t four = 0xfu << (threadIdx.x & 28);        // a row's threads come in whole fours, not in whole warps
-    top = max(top, __shfl_xor_sync(four, top, 1));
-    top = max(top, __shfl_xor_sync(four, top, 2));
-    const uint32_t byte = exponent_byte<BITS>(top);
-    const float f = to_type(byte);
-    float y[8];
+        for (int i = 0; i < 8; ++i) y[i] = v[i] * f;
+    }
+};
+template <> struct Eight<__nv_bfloat16> {
+    uint32_t w[4];
+    template <bool WHOLE> __device__ __forceinline__ void load(const __nv_bfloat16* row, int c, int k) {
+        if (WHOLE && c < k) {
+            const float4 a = load_written(reinterpret_cast<const float*>(row + c));
+            w[0] = __float_as_uint(a.x); w[1] = __float_as_uint(a.y); w[2] = __float_as_uint(a.z); w[3] = __float_as_uint(a.w);
+        } else {
+            const volatile uint16_t* at = reinterpret_cast<const volatile uint16_t*>(row);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = v[i] * f;
-    const size_t at = (size_t)row * n_spans * SPAN + c;
-    if (BITS == 4) {
-        *reinterpret_cast<uint32_t*>(codes + at / 2) = four_bits(y);
-    } else {
-        *reinterpret_cast<uint2*>(codes + at) = make_uint2(eight_bits(y), eight_bits(y + 4));
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t lo = !WHOLE && c + 2 * i < k ? at[c + 2 * i] : 0u, hi = !WHOLE && c + 2 * i + 1 < k ? at[c + 2 * i + 1] : 0u;
+                w[i] = lo | hi << 16;
+            }
+        }
     }
-    if ((c & 31) == 0) exponents[exponent_at(row, c >> 5, n_spans)] = (uint8_t)byte;
-}
-
-template <typename T, int BITS, bool WHOLE>
-__global__ void __launch_bounds__(THREADS) hold_kernel(const T* x, int k, long long ld, int n_spans, uint32_t groups, uint8_t* codes, uint8_t* exponents) {
-    let_next_kernel_start();
-    wait_for_previous_kernels();
-    const uint32_t per_row = n_spans * (SPAN / 8);
-    for (uint32_t g = blockIdx.x * THREADS + threadIdx.x; g < groups; g += gridDim.x * THREADS) {
-        const int row = (int)(g / per_row), c = (int)(g - (uint32_t)row * per_row) * 8;
-        float v[8];
-        load8<T, WHOLE>(x + (size_t)row * ld, c, k, v);
-        store8<BITS>(v, row, c, n_spans, codes, exponents);
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t t = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t = __vmaxu2(t, w[i] & 0x7fff7fffu);
+        return max(t << 16, t & 0xffff0000u);
     }
-}
-
-template <typename T, int BITS, bool WHOLE>
-__global__ void __launch_bounds__(THREADS) values_kernel(const uint8_t* codes, const uint8_t* exponents, int k, int n_spans, uint32_t groups, T* out) {
-    let_next_kernel_start();
-    wait_for_previous_kernels();
-    const uint32_t per_row = n_spans * (SPAN / 8);
-    for (uint32_t g = blockIdx.x * THREADS + threadIdx.x; g < groups; g += gridDim.x * THREADS) {
-        const int row = (int)(g / per_row), c = (int)(g - (uint32_t)row * per_row) * 8;
-        if (c >= k) continue;
-        const size_t at = (size_t)row * n_spans * SPAN + c;
-        const volatile uint32_t* from = reinterpret_cast<const volatile uint32_t*>(codes + (BITS == 4 ? at / 2 : at));
-        uint32_t w[2];
-        w[0] = from[0];
-        if (BITS == 8) w[1] = from[1];
-        const float f = from_type(const_cast<const volatile uint8_t*>(exponents)[exponent_at(row, c >> 5, n_spans)]);
-        float v[8];
+    __device__ __forceinline__ void scaled(uint32_t byte, float* y) const {          // (a product that is no normal number any more is 0 in either type)
+        const __nv_bfloat162 f = to_type_bf162(byte);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const __half2_raw h = BITS == 4 ? __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(w[0] >> (8 * i)), __NV_E2M1)
-                                            : __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
-            const float2 p = __half22float2(__half2(h));
-            v[2 * i] = p.x * f;
-            v[2 * i + 1] = p.y * f;
+            const uint32_t p = as_word(__hmul2(as_bf162(w[i]), f));
+            y[2 * i] = __uint_as_float(p << 16);
+            y[2 * i + 1] = __uint_as_float(p & 0xffff0000u);
         }
-        T* to = out + (size_t)row * k + c;
-        if (WHOLE) {
-            if (sizeof(T) == 2) {
-                *reinterpret_cast<uint4*>(to) = pack8(v);
-            } else {
-                reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
-            }
-        } else {
-            for (int i = 0; i < 8 && c + i < k; ++i) to[i] = from_f32<T>(v[i]);
+    }
+    __device__ __forceinline__ void add_to(float* v) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] += __uint_as_float(w[i] << 16);
+            v[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+
+// The largest of a block's four threads.
+__device__ __forceinline__ uint32_t block_top(uint32_t top) {
+    const uint32_t four = 0xfu << (threadIdx.x & 28);        // a row's threads come in whole fours, not in whole warps
+    top = max(top, __shfl_xor_sync(four, top, 1));
+    return max(top, __shfl_xor_sync(four, top, 2));
+}
+
+// A warp takes a part of a row, GROUPS times 256 numbers, whose reads are on their way together: four where there is much to do, else one.
+template <typename T, int BITS, bool WHOLE, int GROUPS>
+__global__ void __launch_bounds__(THREADS) hold_kernel(const T* x, int n, int k, long long ld, int n_spans, uint32_t parts, uint32_t items, uint8_t* codes,
+                                                       uint8_t* exponents) {
+    let_next_kernel_start();
+    wait_for_previous_kernels();
+    const int lane = threadIdx.x & 31;
+    for (uint32_t it = (blockIdx.x * THREADS + threadIdx.x) >> 5; it < items; it += gridDim.x * (THREADS / 32)) {
+        const int row = (int)(it / parts), c0 = (int)(it - (uint32_t)row * parts) * (GROUPS * 256) + lane * 8, width = n_spans * SPAN;
+        if (row >= n) {                            // of a matrix's last 128 rows those that are none
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i)
+                if ((lane & 3) == 0 && c0 + i * 256 < width) exponents[exponent_at(row, (c0 + i * 256) >> 5, n_spans)] = 0;
+            continue;
+        }
+        const T* from = x + (size_t)row * ld;
+        Eight<T> v[GROUPS];
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) v[i].template load<WHOLE>(from, c0 + i * 256, k);
+        uint8_t* to = codes + (size_t)row * n_spans * (SPAN * BITS / 8) + c0 * BITS / 8;
+        uint8_t* exp_to = exponents + exponent_at(row, c0 >> 5, n_spans);           // (256 numbers further on: two pieces)
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            if (c0 + i * 256 >= width) break;
+            const uint32_t byte = exponent_byte<BITS>(block_top(v[i].top()));
+            float y[8];
+            v[i].scaled(byte, y);
+            if (BITS == 4) *reinterpret_cast<uint32_t*>(to + i * 128) = four_bits(y);
+            else *reinterpret_cast<uint2*>(to + i * 256) = make_uint2(eight_bits(y), eight_bits(y + 4));
+            if ((lane & 3) == 0) exp_to[i * 2 * PIECE] = (uint8_t)byte;
         }
     }
 }
 
-// A block of threads per row.  Sum of squares, root and factors are in 64 bits: the result is rounded to four bits of mantissa, and what
-// lies next to the middle of two numbers should fall as the formula says, not as a sum's last bits do.  (The arithmetic hides behind the
-// memory's: see the figures in front of the launch.)  HELD: so many groups of eight per thread stay in registers between the two passes;
-// longer rows are read again.
+// The same for reading back, a thread 16 bytes of the result at a time.
+template <typename T> struct Sixteen { static constexpr int N = 16 / sizeof(T); };
+
+template <typename T, int BITS, bool WHOLE, int GROUPS>
+__global__ void __launch_bounds__(THREADS) values_kernel(const uint8_t* codes, const uint8_t* exponents, int k, int n_spans, uint32_t parts, uint32_t items, T* out) {
+    constexpr int N = Sixteen<T>::N, BYTES = N * BITS / 8;          // numbers of a thread, and bytes of their codes: 2, 4 or 8
+    let_next_kernel_start();
+    wait_for_previous_kernels();
+    const int lane = threadIdx.x & 31;
+    for (uint32_t it = (blockIdx.x * THREADS + threadIdx.x) >> 5; it < items; it += gridDim.x * (THREADS / 32)) {
+        const int row = (int)(it / parts), c0 = (int)(it - (uint32_t)row * parts) * (GROUPS * 32 * N) + lane * N;
+        const volatile uint8_t* at = codes + (size_t)row * n_spans * (SPAN * BITS / 8) + c0 * BITS / 8;
+        const volatile uint8_t* exp_at = exponents + exponent_at(row, c0 >> 5, n_spans);      // (32 N numbers further on: one or two pieces)
+        T* to = out + (size_t)row * k + c0;
+        uint32_t w[GROUPS][2], byte[GROUPS];
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            if (c0 + i * 32 * N >= k) break;
+            const volatile uint8_t* from = at + i * 32 * BYTES;
+            if (BYTES == 2) w[i][0] = *reinterpret_cast<const volatile uint16_t*>(from);
+            else w[i][0] = *reinterpret_cast<const volatile uint32_t*>(from);
+            if (BYTES == 8) w[i][1] = *reinterpret_cast<const volatile uint32_t*>(from + 4);
+            byte[i] = exp_at[i * (N / 4) * PIECE];
+        }
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const int c = c0 + i * 32 * N;
+            if (c >= k) break;
+            __nv_bfloat162 v[N / 2];
+#pragma unroll
+            for (int q = 0; q < N / 2; ++q)
+                v[q] = BITS == 4 ? four_to_bf162((w[i][0] >> (8 * q) & 0xffu) * 0x1001u) : eight_to_bf162(__byte_perm(w[i][q >> 1], 0, q & 1 ? 0x4342 : 0x4140));
+            uint4 r;
+            uint32_t* p = reinterpret_cast<uint32_t*>(&r);
+            if (sizeof(T) == 2) {
+                const __nv_bfloat162 f = from_type_bf162(byte[i]);
+#pragma unroll
+                for (int q = 0; q < N / 2; ++q) p[q] = as_word(__hmul2(v[q], f));
+            } else {
+                const float f = from_type(byte[i]);
+#pragma unroll
+                for (int q = 0; q < N / 2; ++q) {
+                    p[2 * q] = __float_as_uint(__low2float(v[q]) * f);
+                    p[2 * q + 1] = __float_as_uint(__high2float(v[q]) * f);
+                }
+            }
+            T* dst = to + i * 32 * N;
+            if (WHOLE) {
+                *reinterpret_cast<uint4*>(dst) = r;
+            } else {
+#pragma unroll
+                for (int q = 0; q < N; ++q)
+                    if (c + q < k) {
+                        if (sizeof(T) == 2) reinterpret_cast<uint16_t*>(dst)[q] = (uint16_t)(p[q >> 1] >> (16 * (q & 1)));
+                        else reinterpret_cast<uint32_t*>(dst)[q] = p[q];
+                    }
+            }
+        }
+    }
+}
+
+// A double as the float towards zero, its last bit set where that is not the double: rounded again to fewer bits it becomes what the double
+// would.  0 below 2^-126.
+__device__ __forceinline__ uint32_t to_odd(double y) {
+    const uint32_t hi = (uint32_t)__double2hiint(y), lo = (uint32_t)__double2loint(y), mag = hi & 0x7fffffffu;
+    const uint32_t bits = (mag - (896u << 20)) << 3 | lo >> 29 | ((lo & 0x1fffffffu) != 0u ? 1u : 0u);
+    const uint32_t fine = mag < (897u << 20) ? 0u : mag >= (1151u << 20) ? (mag > 0x7ff00000u || (mag == 0x7ff00000u && lo != 0u) ? 0x7fc00000u : 0x7f800000u) : bits;
+    return fine | (hi & 0x80000000u);
+}
+
+// A block of threads per row.  Sum of squares, root and factors are in 64 bits, up to the rounding to 8: what lies next to the middle of two numbers
+// falls as the formula says, not as a sum's last bits do.  That costs two conversions and three operations in 64 bits a number, beside the
+// memory's time (2,047 rows of 4,096 with a branch: see below).  HELD: so many groups of eight per thread stay in registers between the two
+// passes; longer rows are read again.
 template <typename B, int HELD, bool WHOLE>
 __global__ void rmsnorm_kernel(const float* stream, const B* branch, const float* __restrict__ weight, float* total, int k, int n_spans, double eps,
                                uint8_t* codes, uint8_t* exponents) {
     __shared__ double sums[33];
     let_next_kernel_start();
-    wait_for_previous_kernels();
     const int row = blockIdx.x, tid = threadIdx.x, threads = blockDim.x, groups = n_spans * (SPAN / 8);
     const float* x = stream + (size_t)row * k;
     const B* add = branch == nullptr ? nullptr : branch + (size_t)row * k;
-    float held[HELD][8];
-    auto read = [&](int g, float* v) {
-        load8<float, WHOLE>(x, g * 8, k, v);
+    wait_for_previous_kernels();
+    Eight<float> held[HELD];
+    auto read = [&](int g, Eight<float>& v) {
+        v.template load<WHOLE>(x, g * 8, k);
         if (add != nullptr) {
-            float b[8];
-            load8<B, WHOLE>(add, g * 8, k, b);
+            Eight<B> b;
+            b.template load<WHOLE>(add, g * 8, k);
+            if constexpr (sizeof(B) == 2) {
+                b.add_to(v.v);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += b[i];
+                for (int i = 0; i < 8; ++i) v.v[i] += b.v[i];
+            }
         }
     };
-    double sum = 0.0;
-    auto square = [&](const float* v) {
+    double sum = 0.0, more = 0.0;
+    auto square = [&](const Eight<float>& v) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fma((double)v[i], (double)v[i], sum);
+        for (int i = 0; i < 8; i += 2) {
+            sum = fma((double)v.v[i], (double)v.v[i], sum);
+            more = fma((double)v.v[i + 1], (double)v.v[i + 1], more);
+        }
     };
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
-        if (tid + h * threads < groups) {
-            read(tid + h * threads, held[h]);
-            square(held[h]);
-        }
+        if (tid + h * threads < groups) read(tid + h * threads, held[h]);
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+        if (tid + h * threads < groups) square(held[h]);
     for (int g = tid + HELD * threads; g < groups; g += threads) {
-        float v[8];
+        Eight<float> v;
         read(g, v);
         square(v);
     }
+    sum += more;
     const int lane = tid & 31, warp = tid >> 5;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -162,74 +250,113 @@ __global__ void rmsnorm_kernel(const float* stream, const B* branch, const float
         double s = lane < threads / 32 ? sums[lane] : 0.0;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) sums[32] = 1.0 / sqrt(s / (double)k + eps);
+        if (lane == 0) sums[32] = rsqrt(s / (double)k + eps);
     }
     __syncthreads();
     const double r = sums[32];
-    auto finish = [&](int g, float* v) {
+    auto finish = [&](int g, const Eight<float>& v) {
         const int c = g * 8;
         if (total != nullptr) {
             float* to = total + (size_t)row * k + c;
             if (WHOLE) {
                 if (c < k) {
-                    reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                    reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
+                    reinterpret_cast<float4*>(to)[0] = make_float4(v.v[0], v.v[1], v.v[2], v.v[3]);
+                    reinterpret_cast<float4*>(to)[1] = make_float4(v.v[4], v.v[5], v.v[6], v.v[7]);
                 }
             } else {
-                for (int i = 0; i < 8 && c + i < k; ++i) to[i] = v[i];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (c + i < k) to[i] = v.v[i];
             }
         }
+        float w[8];
+        if (WHOLE && c < k) {
+            const float4 a = *reinterpret_cast<const float4*>(weight + c), b = *reinterpret_cast<const float4*>(weight + c + 4);
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+            w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < k ? (float)((double)v[i] * r * (double)weight[c + i]) : 0.f;
-        store8<8>(v, row, c, n_spans, codes, exponents);
+            for (int i = 0; i < 8; ++i) w[i] = !WHOLE && c + i < k ? weight[c + i] : 0.f;
+        }
+        Eight<float> y;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y.v[i] = __uint_as_float(to_odd((double)v.v[i] * r * (double)w[i]));
+        const uint32_t byte = exponent_byte<8>(block_top(y.top()));
+        float z[8];
+        y.scaled(byte, z);
+        *reinterpret_cast<uint2*>(codes + (size_t)row * n_spans * SPAN + c) = make_uint2(eight_bits(z), eight_bits(z + 4));
+        if ((c & 31) == 0) exponents[exponent_at(row, c >> 5, n_spans)] = (uint8_t)byte;
     };
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
         if (tid + h * threads < groups) finish(tid + h * threads, held[h]);
     for (int g = tid + HELD * threads; g < groups; g += threads) {
-        float v[8];
+        Eight<float> v;
         read(g, v);
         finish(g, v);
     }
 }
 
-int blocks_for(uint32_t groups) {
-    const long long want = ((long long)groups + THREADS - 1) / THREADS, most = 16LL * sm_count();
+// Blocks of threads for so many parts of rows, a warp each; where there are many, a few a warp.
+int blocks_for(long long items) {
+    const long long want = (items + THREADS / 32 - 1) / (THREADS / 32), most = 1LL << 30;
     return (int)(want < most ? want : most);
 }
 
-// Groups of eight numbers of what is held, which must lie on the current device.
-int groups_of(const char* what, const Held* h, uint32_t* groups) {
+// What is held must lie on the current device.
+int on_device(const char* what, const Held* h) {
     int device = -1;
     if (cudaGetDevice(&device) != cudaSuccess || device != h->device) return fail("%s: what is held lies on device %d, the current one is %d", what, h->device, device);
-    *groups = (uint32_t)((long long)h->n * h->n_spans * (SPAN / 8));
     return 0;
 }
 
-template <typename T, int BITS>
-int hold(const void* x, int n, int k, long long ld, void* codes, void* exponents, uint32_t groups, cudaStream_t stream) {
-    const bool whole = k % 8 == 0 && (ld * (long long)sizeof(T)) % 16 == 0 && (uintptr_t)x % 16 == 0;
-    const dim3 grid((unsigned)blocks_for(groups));
-    uint8_t *c = (uint8_t*)codes, *e = (uint8_t*)exponents;
-    const T* from = (const T*)x;
-    return check_launch(whole ? launch_dependent(hold_kernel<T, BITS, true>, grid, dim3(THREADS), 0, stream, from, k, ld, spans(k), groups, c, e)
-                              : launch_dependent(hold_kernel<T, BITS, false>, grid, dim3(THREADS), 0, stream, from, k, ld, spans(k), groups, c, e), "mx_hold");
+// Launches GROUPS = 4 where its warps are at least as many as the device holds at a time, else 1.
+template <typename F1, typename F4>
+int by_size(int rows, int width, int of_warp, F1 one, F4 four) {
+    const uint32_t parts = (width + 4 * of_warp - 1) / (4 * of_warp);
+    if ((long long)rows * parts >= 64LL * sm_count()) return four(parts, (uint32_t)rows * parts);
+    const uint32_t small = (width + of_warp - 1) / of_warp;
+    return one(small, (uint32_t)rows * small);
 }
 
-template <typename T, int BITS>
-int values(const void* codes, const void* exponents, int k, void* out, uint32_t groups, cudaStream_t stream) {
-    const bool whole = k % 8 == 0 && (uintptr_t)out % 16 == 0;
-    const dim3 grid((unsigned)blocks_for(groups));
-    const uint8_t *c = (const uint8_t*)codes, *e = (const uint8_t*)exponents;
-    T* to = (T*)out;
-    return check_launch(whole ? launch_dependent(values_kernel<T, BITS, true>, grid, dim3(THREADS), 0, stream, c, e, k, spans(k), groups, to)
-                              : launch_dependent(values_kernel<T, BITS, false>, grid, dim3(THREADS), 0, stream, c, e, k, spans(k), groups, to), "mx_values");
+template <typename T, int BITS, bool WHOLE>
+int hold(const T* x, long long ld, const Held* h, cudaStream_t stream) {
+    // (a matrix's exponents are all written, in whole pieces; those of rows behind the last one have no effect on a product but must be numbers)
+    const int rows = BITS == 4 ? (h->n + 127) & ~127 : h->n;
+    auto go = [&](auto kernel, uint32_t parts, uint32_t items) {
+        return check_launch(launch_dependent(kernel, dim3((unsigned)blocks_for(items)), dim3(THREADS), 0, stream, x, h->n, h->k, ld, h->n_spans, parts, items, h->codes,
+                                             h->exponents), "mx_hold");
+    };
+    return by_size(rows, h->n_spans * SPAN, 256, [&](uint32_t p, uint32_t i) { return go(hold_kernel<T, BITS, WHOLE, 1>, p, i); },
+                   [&](uint32_t p, uint32_t i) { return go(hold_kernel<T, BITS, WHOLE, 4>, p, i); });
+}
+template <typename T>
+int hold(const T* x, long long ld, const Held* h, cudaStream_t stream) {
+    const bool whole = h->k % 8 == 0 && (ld * (long long)sizeof(T)) % 16 == 0 && (uintptr_t)x % 16 == 0;
+    if (h->bits == 4) return whole ? hold<T, 4, true>(x, ld, h, stream) : hold<T, 4, false>(x, ld, h, stream);
+    return whole ? hold<T, 8, true>(x, ld, h, stream) : hold<T, 8, false>(x, ld, h, stream);
+}
+
+template <typename T, int BITS, bool WHOLE>
+int values(const Held* h, T* out, cudaStream_t stream) {
+    auto go = [&](auto kernel, uint32_t parts, uint32_t items) {
+        return check_launch(launch_dependent(kernel, dim3((unsigned)blocks_for(items)), dim3(THREADS), 0, stream, h->codes, h->exponents, h->k, h->n_spans, parts, items, out),
+                            "mx_values");
+    };
+    return by_size(h->n, h->k, 32 * Sixteen<T>::N, [&](uint32_t p, uint32_t i) { return go(values_kernel<T, BITS, WHOLE, 1>, p, i); },
+                   [&](uint32_t p, uint32_t i) { return go(values_kernel<T, BITS, WHOLE, 4>, p, i); });
+}
+template <typename T>
+int values(const Held* h, T* out, cudaStream_t stream) {
+    const bool whole = h->k % Sixteen<T>::N == 0 && (uintptr_t)out % 16 == 0;
+    if (h->bits == 4) return whole ? values<T, 4, true>(h, out, stream) : values<T, 4, false>(h, out, stream);
+    return whole ? values<T, 8, true>(h, out, stream) : values<T, 8, false>(h, out, stream);
 }
 
 template <typename B>
 int norm(const float* x, const void* branch, const float* weight, float* total, int n, int k, double eps, void* codes, void* exponents, cudaStream_t stream) {
     const int groups = spans(k) * (SPAN / 8);
-    const bool whole = k % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)branch % 16 == 0 && (uintptr_t)total % 16 == 0;
+    const bool whole = k % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)branch % 16 == 0 && (uintptr_t)total % 16 == 0 && (uintptr_t)weight % 16 == 0;
     constexpr int HELD = 2;
     int threads = ((groups + HELD - 1) / HELD + 31) / 32 * 32;
     if (threads > 512) threads = 512;
@@ -249,7 +376,7 @@ RI_API long long ri_mx_held_bytes() { return (long long)sizeof(Held); }
 RI_API int ri_mx_make(void* at, void* codes, void* exponents, long long n, long long k, int bits, int device) {
     if ((uintptr_t)at % 64) return fail("mx_make: 64-byte aligned memory is wanted");
     if (n <= 0 || k <= 0 || k > 0x7fffffffLL - SPAN || (bits != 4 && bits != 8)) return fail("mx_make: no [%lld, %lld] numbers of %d bits", n, k, bits);
-    if (n * spans((int)k) > 0x7fffffffLL / (SPAN / 8)) return fail("mx_make: [%lld, %lld] numbers are more than 2^31 eights", n, k);
+    if ((n + 127) * spans((int)k) > 0x7fffffffLL / (SPAN / 8)) return fail("mx_make: [%lld, %lld] numbers are more than 2^31 eights", n, k);
     if ((uintptr_t)codes % 32 || (uintptr_t)exponents % 32) return fail("mx_make: buffers must begin on a 32-byte boundary");
     Held* h = new (at) Held;
     h->codes = (uint8_t*)codes;
@@ -266,33 +393,25 @@ RI_API int ri_mx_make(void* at, void* codes, void* exponents, long long n, long 
 // x [n, k] (rows `ld` numbers apart) to what is held.
 RI_API int ri_mx_hold(const void* x, int dtype, long long n, long long k, long long ld, void* held, cudaStream_t stream) {
     const Held* h = (const Held*)held;
-    uint32_t groups;
     if (n != h->n || k != h->k || ld < k) return fail("mx_hold: [%lld, %lld] numbers, rows %lld apart, do not go into [%d, %d]", n, k, ld, h->n, h->k);
-    if (int rc = groups_of("mx_hold", h, &groups)) return rc;
-    if (dtype == RI_BF16) return h->bits == 4 ? hold<__nv_bfloat16, 4>(x, h->n, h->k, ld, h->codes, h->exponents, groups, stream)
-                                              : hold<__nv_bfloat16, 8>(x, h->n, h->k, ld, h->codes, h->exponents, groups, stream);
-    return h->bits == 4 ? hold<float, 4>(x, h->n, h->k, ld, h->codes, h->exponents, groups, stream)
-                        : hold<float, 8>(x, h->n, h->k, ld, h->codes, h->exponents, groups, stream);
+    if (int rc = on_device("mx_hold", h)) return rc;
+    return dtype == RI_BF16 ? hold((const __nv_bfloat16*)x, ld, h, stream) : hold((const float*)x, ld, h, stream);
 }
 
 // out [n, k]: the numbers that are held.
 RI_API int ri_mx_values(const void* held, int dtype, long long n, long long k, void* out, cudaStream_t stream) {
     const Held* h = (const Held*)held;
-    uint32_t groups;
     if (n != h->n || k != h->k) return fail("mx_values: [%d, %d] numbers do not go into [%lld, %lld]", h->n, h->k, n, k);
-    if (int rc = groups_of("mx_values", h, &groups)) return rc;
-    if (dtype == RI_BF16) return h->bits == 4 ? values<__nv_bfloat16, 4>(h->codes, h->exponents, h->k, out, groups, stream)
-                                              : values<__nv_bfloat16, 8>(h->codes, h->exponents, h->k, out, groups, stream);
-    return h->bits == 4 ? values<float, 4>(h->codes, h->exponents, h->k, out, groups, stream) : values<float, 8>(h->codes, h->exponents, h->k, out, groups, stream);
+    if (int rc = on_device("mx_values", h)) return rc;
+    return dtype == RI_BF16 ? values(h, (__nv_bfloat16*)out, stream) : values(h, (float*)out, stream);
 }
 
 // total = stream + branch (branch null: the stream itself; total null: not kept; it may be the stream), [n, k], and the norm of it times `weight` in 8 bits.
 RI_API int ri_mx_rmsnorm(const float* x, const void* branch, int branch_dtype, const float* weight, float* total, long long n, long long k, double eps,
                          void* held, cudaStream_t stream) {
     const Held* h = (const Held*)held;
-    uint32_t groups;
     if (n != h->n || k != h->k || h->bits != 8) return fail("mx_rmsnorm: a norm of [%lld, %lld] does not go into [%d, %d] of %d bits", n, k, h->n, h->k, h->bits);
-    if (int rc = groups_of("mx_rmsnorm", h, &groups)) return rc;
+    if (int rc = on_device("mx_rmsnorm", h)) return rc;
     return branch_dtype == RI_BF16 ? norm<__nv_bfloat16>(x, branch, weight, total, h->n, h->k, eps, h->codes, h->exponents, stream)
                                    : norm<float>(x, branch, weight, total, h->n, h->k, eps, h->codes, h->exponents, stream);
 }

@@ -54,7 +54,7 @@ __device__ __forceinline__ float from_type(uint32_t byte) {
     return byte == 255u ? __uint_as_float(0x7fc00000u) : byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
 }
 
-// The codes of eight numbers (already times 2^-e): a word of four bits each, two words of eight.
+// The codes of eight numbers (already times 2^-e): a word of four bits each.
 __device__ __forceinline__ uint32_t four_bits(const float* y) {
     uint32_t w = 0;
 #pragma unroll
@@ -65,6 +65,21 @@ __device__ __forceinline__ uint32_t four_bits(const float* y) {
 __device__ __forceinline__ uint32_t eight_bits(const float* y) {       // of four numbers
     return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3) |
            (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+}
+// Two codes, in the low halves of a word's halves, as bfloat16 numbers: exponent and mantissa in place, times the difference of the
+// exponents' biases.  (Only shifts and products, whose rate conversions do not have.)
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+__device__ __forceinline__ uint32_t as_word(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ __nv_bfloat162 eight_to_bf162(uint32_t w) { return __hmul2(as_bf162((w & 0x00800080u) << 8 | (w & 0x007f007fu) << 4), as_bf162(0x7b807b80u)); }
+__device__ __forceinline__ __nv_bfloat162 four_to_bf162(uint32_t w) { return __hmul2(as_bf162((w & 0x00080008u) << 12 | (w & 0x00070007u) << 6), as_bf162(0x7e807e80u)); }
+// 2^e and 2^-e
+__device__ __forceinline__ __nv_bfloat162 from_type_bf162(uint32_t byte) {
+    const uint32_t h = byte == 255u ? 0x7fc0u : byte == 0u ? 0x0040u : byte << 7;
+    return as_bf162(h | h << 16);
+}
+__device__ __forceinline__ __nv_bfloat162 to_type_bf162(uint32_t byte) {
+    const uint32_t h = byte == 255u ? 0u : (254u - byte) << 7;
+    return as_bf162(h | h << 16);
 }
 __device__ __forceinline__ uint8_t eight_bits_of_one(float y) { return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3); }
 

@@ -294,6 +294,35 @@ typedef int MxHoldFn(const void*, int, long long, long long, long long, void*, v
 void mx_hold(const at::Tensor& x, void* held, const char* what) {
     finish(entry<MxHoldFn>(MX_HOLD)(x.data_ptr(), code_of(x, what), x.size(0), x.size(1), x.size(0) > 1 ? x.stride(0) : x.size(1), held, stream()), MX_HOLD, what);
 }
+// (matrix) -> (codes, exponents, description): 4 bits.  `make` and `held_bytes`: addresses of ri_mx_make and the bytes of a description.
+typedef int MxMakeFn(void*, void*, void*, long long, long long, int, int);
+PyObject* py_mx_matrix(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const char* what = "microscaled.Matrix";
+        need(n == 3, "microscaled.Matrix: 3 arguments");
+        const at::Tensor& x = rows(a[0], what);
+        const int64_t N = x.size(0), spans = (x.size(1) + 127) / 128;
+        need(N > 0 && spans > 0, "microscaled.Matrix: a matrix of at least one number is wanted");
+        code_of(x, what);
+        const auto bytes = x.options().dtype(at::kByte).layout(at::kStrided).requires_grad(false);
+        const at::Tensor made[3] = {at::empty({N, spans * 64}, bytes), at::empty({(N + 127) / 128, spans, 512}, bytes),
+                                    at::empty({number(a[2])}, bytes.device(at::kCPU))};
+        if (address<MxMakeFn>(number(a[1]))(made[2].data_ptr(), made[0].data_ptr(), made[1].data_ptr(), N, x.size(1), 4, x.get_device()) != 0)
+            refuse(std::string(what) + ": " + bound[MX_HOLD].last_error());
+        mx_hold(x, made[2].data_ptr(), what);
+        PyObject* out = PyTuple_New(3);
+        if (out == nullptr) throw Raised{};
+        for (int i = 0; i < 3; ++i) {
+            PyObject* o = THPVariable_Wrap(made[i]);
+            if (o == nullptr) {
+                Py_DECREF(out);
+                throw Raised{};
+            }
+            PyTuple_SET_ITEM(out, i, o);
+        }
+        return out;
+    });
+}
 // (x, held)
 PyObject* py_mx_hold(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
@@ -394,7 +423,7 @@ template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)> PyMethodDef m
     return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
 }
 PyMethodDef methods[] = {method<py_write>("write"), method<py_read>("read"), method<py_attend>("attend"), method<py_logprobs>("logprobs"),
-                         method<py_mx_hold>("mx_hold"), method<py_mx_values>("mx_values"), method<py_mx_rmsnorm>("mx_rmsnorm"),
+                         method<py_mx_hold>("mx_hold"), method<py_mx_matrix>("mx_matrix"), method<py_mx_values>("mx_values"), method<py_mx_rmsnorm>("mx_rmsnorm"),
                          method<py_mx_product>("mx_product"),
                          method<py_bind>("bind"), method<py_launches>("launches"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "ri_native_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -15,7 +15,7 @@ A block that holds an infinity or a NaN stands for 32 NaNs.
 from __future__ import annotations
 
 import functools
-from ctypes import c_int, c_longlong, c_void_p
+from ctypes import c_int, c_longlong, c_void_p, cast
 
 import torch
 
@@ -45,6 +45,14 @@ def _describe(codes: torch.Tensor, exponents: torch.Tensor, n: int, k: int, bits
     return at
 
 
+@functools.lru_cache(maxsize=None)
+def _maker():
+    native("mx_hold")                                            # names the entry points that it takes
+    from .build import load_extension
+    fn, make, size = load_extension("native_calls").mx_matrix, cast(load("microscaled").ri_mx_make, c_void_p).value, _held_bytes()
+    return lambda t: fn(t, make, size)
+
+
 class Matrix:
     """A weight matrix [n, k] in 4 bits, for the products of `kernels.linear`."""
 
@@ -64,8 +72,10 @@ class Matrix:
         ops._need_cuda(t)
         if (t.stride(1) != 1 and t.shape[1] > 1) or t.stride(0) < t.shape[1]:
             t = t.contiguous()
-        m = cls._empty(*t.shape, t.device)
-        native("mx_hold")(t, m.native)
+        m = cls.__new__(cls)
+        m.codes, m.exponents, m._described = _maker()(t)
+        m.n, m.k = t.shape
+        m.spans, m.device, m.native = _spans(m.k), t.device, m._described.data_ptr()
         return m
 
     @classmethod

@@ -39,29 +39,31 @@ class Model:
     @classmethod
     def load(cls, path: str, max_seq_len: int | None = None, *, dtype: str = "bfloat16",
              device: str = "cuda", max_tokens_in_cache: int | None = None, n_slots: int | None = None,
-             cache_dtype: str | None = None) -> "Model":
+             cache_dtype: str | None = None, weights_dtype: str | None = None) -> "Model":
         """path: a folder with config.json and model.safetensors (or shards with an index).
         max_seq_len overrides the model's context length, as `--max-seq-len` does in the
         reference (model.rs:142-144): it caps the cache and the rotary table.
         max_tokens_in_cache: positions all live sequences may hold together (default: 8 sequences
         of max_seq_len, at most 65,536 positions).
-        cache_dtype: "int8" keeps keys and values in 8 bits (see `Engine`); default: in `dtype`."""
+        cache_dtype: "int8" keeps keys and values in 8 bits (see `Engine`); default: in `dtype`.
+        weights_dtype: "mxfp4" holds the matrices of attention projections and dense feed-forwards in microscaled 4 bits (see
+        `kernels.microscaled`), whatever the file holds them in; default: in `dtype`.  Decoders that route to experts are refused."""
         from .config.registry import load_spec
         seq = resolve_max_seq_len(max_seq_len, load_spec(path)[1].max_positions)
         if max_tokens_in_cache is None:
             max_tokens_in_cache = min(8 * seq, max(seq, 65536))
         return cls(Engine.from_pretrained(path, dtype=dtype, device=device, max_tokens=max_tokens_in_cache,
-                                          max_seq_len=seq, n_slots=n_slots, cache_dtype=cache_dtype))
+                                          max_seq_len=seq, n_slots=n_slots, cache_dtype=cache_dtype, weights_dtype=weights_dtype))
 
     @classmethod
     def random(cls, config, *, seed: int = 0, std: float = 0.02, norm_std: float = 0.0, dtype: str = "bfloat16",
                device: str = "cuda", max_seq_len: int | None = None, max_tokens_in_cache: int = 65536,
-               n_slots: int | None = None, cache_dtype: str | None = None) -> "Model":
+               n_slots: int | None = None, cache_dtype: str | None = None, weights_dtype: str | None = None) -> "Model":
         """A model with random weights made on the device from a typed config and a seed: matrices and
         biases N(0, std), norm weights 1 + N(0, norm_std)."""
         return cls(Engine.from_random(config, seed=seed, std=std, norm_std=norm_std, dtype=dtype, device=device,
                                       max_tokens=max_tokens_in_cache, max_seq_len=max_seq_len, n_slots=n_slots,
-                                      cache_dtype=cache_dtype))
+                                      cache_dtype=cache_dtype, weights_dtype=weights_dtype))
 
     def memory(self) -> dict:
         """Bytes the model holds on the device and what a decode step has to read of them: the weights
@@ -96,7 +98,7 @@ class Model:
     def state_dict(self) -> dict:
         """name -> tensor for every tensor of the model, under the weight file's names, as held on the
         device (matrices in the run dtype, norm weights and biases float32; packed matrices as views
-        of their parts).  Handing these to a plain implementation gives it the very numbers the
+        of their parts; matrices in 4 bits as the numbers that they stand for).  Handing these to a plain implementation gives it the very numbers the
         engine computes with, without a folder on disk."""
         return self.engine.model.state_dict()
 

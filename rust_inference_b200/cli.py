@@ -19,6 +19,7 @@ Added for a library that takes token ids and may run without a checkpoint:
                                             generated tokens, seconds, tokens per second, bytes copied, the model's
                                             bytes on the device
   --cache-dtype int8                        keys and values in 8 bits instead of the run dtype
+  --weights-dtype mxfp4                     matrices of attention projections and dense feed-forwards in microscaled 4 bits
   --score K                                 instead of generating: for every token of a prompt but the first one line with its
                                             id, its log probability, the entropy of its distribution and the K likeliest
                                             tokens; per prompt the perplexity on standard error
@@ -56,6 +57,7 @@ Options:
   --stop-ids         Stop token ids (default: the model's eos ids)
   --dtype            bfloat16 (default) or float32
   --cache-dtype      same (default: as --dtype) or int8: keys and values in 8 bits
+  --weights-dtype    same (default: as --dtype) or mxfp4: projections and dense feed-forwards in microscaled 4 bits
   --score            Score the prompts instead of generating; the number of alternatives to print per token
   --slots            Sequences live at once (default: as many as the cache holds)
   --print-logits-topk  Print the K largest logits after each prompt
@@ -82,7 +84,7 @@ def parse_args(argv: list) -> dict:
     a = {"model": None, "prompts": [], "max_tokens": 512, "temperature": 0.8, "top_k": 40, "top_p": 0.95,
          "repetition_penalty": 1.1, "seed": 12345, "max_seq_len": None, "stop_ids": None,
          "dtype": "bfloat16", "help": False, "random_config": None, "weights_seed": 0, "random_prompts": None,
-         "slots": None, "cache_dtype": None, "score": None, "logits_topk": 0, "layer_stats": False, "bench": False}
+         "slots": None, "cache_dtype": None, "weights_dtype": None, "score": None, "logits_topk": 0, "layer_stats": False, "bench": False}
     i = 0
 
     def value(flag):
@@ -136,6 +138,10 @@ def parse_args(argv: list) -> dict:
             a["cache_dtype"] = value("--cache-dtype")
             if a["cache_dtype"] not in ("same", "int8"):
                 raise CliError(f"Invalid --cache-dtype: {a['cache_dtype']!r}")
+        elif arg == "--weights-dtype":
+            a["weights_dtype"] = value("--weights-dtype")
+            if a["weights_dtype"] not in ("same", "mxfp4"):
+                raise CliError(f"Invalid --weights-dtype: {a['weights_dtype']!r}")
         elif arg == "--score":
             a["score"] = number("--score", int)
             if not 0 <= a["score"] <= 64:
@@ -206,9 +212,10 @@ def main(argv=None) -> int:
             with open(a["random_config"], encoding="utf-8") as f:
                 config = config_from_dict(json.load(f))
             model = Model.random(config, seed=a["weights_seed"], dtype=a["dtype"], max_seq_len=a["max_seq_len"],
-                                 n_slots=a["slots"], cache_dtype=a["cache_dtype"])
+                                 n_slots=a["slots"], cache_dtype=a["cache_dtype"], weights_dtype=a["weights_dtype"])
         else:
-            model = Model.load(a["model"], a["max_seq_len"], dtype=a["dtype"], n_slots=a["slots"], cache_dtype=a["cache_dtype"])
+            model = Model.load(a["model"], a["max_seq_len"], dtype=a["dtype"], n_slots=a["slots"], cache_dtype=a["cache_dtype"],
+                               weights_dtype=a["weights_dtype"])
     except Exception as e:                          # main.rs:257-263
         print(f"Failed to load model: {e}", file=sys.stderr)
         return 1

@@ -199,7 +199,7 @@ __device__ __forceinline__ uint32_t to_odd(double y) {
 // memory's time (2,047 rows of 4,096 with a branch: see below).  HELD: so many groups of eight per thread stay in registers between the two
 // passes; longer rows are read again.
 template <typename B, int HELD, bool WHOLE>
-__global__ void rmsnorm_kernel(const float* stream, const B* branch, const float* __restrict__ weight, float* total, int k, int n_spans, double eps,
+__global__ void __launch_bounds__(HELD == 1 ? 1024 : 512) rmsnorm_kernel(const float* stream, const B* branch, const float* __restrict__ weight, float* total, int k, int n_spans, double eps,
                                uint8_t* codes, uint8_t* exponents) {
     __shared__ double sums[33];
     let_next_kernel_start();
@@ -353,18 +353,24 @@ int values(const Held* h, T* out, cudaStream_t stream) {
     return whole ? values<T, 8, true>(h, out, stream) : values<T, 8, false>(h, out, stream);
 }
 
-template <typename B>
-int norm(const float* x, const void* branch, const float* weight, float* total, int n, int k, double eps, void* codes, void* exponents, cudaStream_t stream) {
-    const int groups = spans(k) * (SPAN / 8);
-    const bool whole = k % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)branch % 16 == 0 && (uintptr_t)total % 16 == 0 && (uintptr_t)weight % 16 == 0;
-    constexpr int HELD = 2;
+template <typename B, int HELD>
+int norm(const float* x, const B* branch, const float* weight, float* total, const Held* h, double eps, int most, cudaStream_t stream) {
+    const int groups = h->n_spans * (SPAN / 8);
+    const bool whole = h->k % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)branch % 16 == 0 && (uintptr_t)total % 16 == 0 && (uintptr_t)weight % 16 == 0;
     int threads = ((groups + HELD - 1) / HELD + 31) / 32 * 32;
-    if (threads > 512) threads = 512;
-    uint8_t *c = (uint8_t*)codes, *e = (uint8_t*)exponents;
-    const B* b = (const B*)branch;
-    return check_launch(whole ? launch_dependent(rmsnorm_kernel<B, HELD, true>, dim3((unsigned)n), dim3(threads), 0, stream, x, b, weight, total, k, spans(k), eps, c, e)
-                              : launch_dependent(rmsnorm_kernel<B, HELD, false>, dim3((unsigned)n), dim3(threads), 0, stream, x, b, weight, total, k, spans(k), eps, c, e),
-                        "mx_rmsnorm");
+    if (threads > most) threads = most;
+    auto go = [&](auto kernel) {
+        return check_launch(launch_dependent(kernel, dim3((unsigned)h->n), dim3(threads), 0, stream, x, branch, weight, total, h->k, h->n_spans, eps, h->codes, h->exponents),
+                            "mx_rmsnorm");
+    };
+    return whole ? go(rmsnorm_kernel<B, HELD, true>) : go(rmsnorm_kernel<B, HELD, false>);
+}
+// Few rows are as fast as one of them, which many threads with one group each have sooner (8 rows of 3,584: one group 3.3 us, two 4.2; 148 of
+// 4,096 3.8 / 4.9); many are as fast as the SMs' instructions, of which two groups a thread take fewer (2,047 of 4,096: 26.2 / 23.9).
+template <typename B>
+int norm(const float* x, const void* branch, const float* weight, float* total, const Held* h, double eps, cudaStream_t stream) {
+    return h->n <= 2 * sm_count() ? norm<B, 1>(x, (const B*)branch, weight, total, h, eps, 1024, stream)
+                                  : norm<B, 2>(x, (const B*)branch, weight, total, h, eps, 512, stream);
 }
 
 }  // namespace
@@ -412,8 +418,8 @@ RI_API int ri_mx_rmsnorm(const float* x, const void* branch, int branch_dtype, c
     const Held* h = (const Held*)held;
     if (n != h->n || k != h->k || h->bits != 8) return fail("mx_rmsnorm: a norm of [%lld, %lld] does not go into [%d, %d] of %d bits", n, k, h->n, h->k, h->bits);
     if (int rc = on_device("mx_rmsnorm", h)) return rc;
-    return branch_dtype == RI_BF16 ? norm<__nv_bfloat16>(x, branch, weight, total, h->n, h->k, eps, h->codes, h->exponents, stream)
-                                   : norm<float>(x, branch, weight, total, h->n, h->k, eps, h->codes, h->exponents, stream);
+    return branch_dtype == RI_BF16 ? norm<__nv_bfloat16>(x, branch, weight, total, h, eps, stream)
+                                   : norm<float>(x, branch, weight, total, h, eps, stream);
 }
 
 RI_DEFINE_LAST_ERROR()

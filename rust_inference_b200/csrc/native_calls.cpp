@@ -290,9 +290,9 @@ const at::Tensor& dense(PyObject* o, const char* what) {
     if (!here(t) || t.dim() != 2 || !t.is_contiguous()) refuse(std::string(what) + ": a contiguous [n, k] on the current device is wanted");
     return t;
 }
-typedef int MxHoldFn(const void*, int, long long, long long, long long, void*, void*);
+typedef int Mx_holdFn(const void*, int, long long, long long, long long, void*, void*);
 void mx_hold(const at::Tensor& x, void* held, const char* what) {
-    finish(entry<MxHoldFn>(MX_HOLD)(x.data_ptr(), code_of(x, what), x.size(0), x.size(1), x.size(0) > 1 ? x.stride(0) : x.size(1), held, stream()), MX_HOLD, what);
+    finish(entry<Mx_holdFn>(MX_HOLD)(x.data_ptr(), code_of(x, what), x.size(0), x.size(1), x.size(0) > 1 ? x.stride(0) : x.size(1), held, stream()), MX_HOLD, what);
 }
 // (matrix) -> (codes, exponents, description): 4 bits.  `make` and `held_bytes`: addresses of ri_mx_make and the bytes of a description.
 typedef int MxMakeFn(void*, void*, void*, long long, long long, int, int);
@@ -332,18 +332,18 @@ PyObject* py_mx_hold(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 // (held, out)
-typedef int MxValuesFn(const void*, int, long long, long long, void*, void*);
+typedef int Mx_valuesFn(const void*, int, long long, long long, void*, void*);
 PyObject* py_mx_values(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const char* what = "microscaled.values";
         need(n == 2, "microscaled.values: 2 arguments");
         const at::Tensor& out = dense(a[1], what);
-        finish(entry<MxValuesFn>(MX_VALUES)(address<void>(number(a[0])), code_of(out, what), out.size(0), out.size(1), out.data_ptr(), stream()), MX_VALUES, what);
+        finish(entry<Mx_valuesFn>(MX_VALUES)(address<void>(number(a[0])), code_of(out, what), out.size(0), out.size(1), out.data_ptr(), stream()), MX_VALUES, what);
         Py_RETURN_NONE;
     });
 }
 // (x, branch or None, weight, total or None, eps, held)
-typedef int MxNormFn(const float*, const void*, int, const float*, float*, long long, long long, double, void*, void*);
+typedef int Mx_rmsnormFn(const float*, const void*, int, const float*, float*, long long, long long, double, void*, void*);
 PyObject* py_mx_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const char* what = "microscaled.rmsnorm";
@@ -365,13 +365,13 @@ PyObject* py_mx_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
             need(t.scalar_type() == at::kFloat && t.sizes() == x.sizes(), "microscaled.rmsnorm: total must be float32, as x");
             total = t.data_ptr<float>();
         }
-        finish(entry<MxNormFn>(MX_NORM)(x.data_ptr<float>(), branch, branch_code, weight.data_ptr<float>(), total, x.size(0), x.size(1), real(a[4]),
+        finish(entry<Mx_rmsnormFn>(MX_NORM)(x.data_ptr<float>(), branch, branch_code, weight.data_ptr<float>(), total, x.size(0), x.size(1), real(a[4]),
                                         address<void>(number(a[5])), stream()), MX_NORM, what);
         Py_RETURN_NONE;
     });
 }
 // (plain rows or None, held rows, matrix, second matrix or 0, constants or None, act, add, out or None, held result or 0, status word)
-typedef int MxProductFn(void*, void*, void*, const float*, long long, int, int, void*, int, long long, long long, void*, int*, void*);
+typedef int Mx_productFn(void*, void*, void*, const float*, long long, int, int, void*, int, long long, long long, void*, int*, void*);
 PyObject* py_mx_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const char* what = "microscaled.product";
@@ -396,7 +396,7 @@ PyObject* py_mx_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
             out_cols = o.size(1);
         }
         if (a[0] != Py_None) mx_hold(rows(a[0], what), held, what);
-        finish(entry<MxProductFn>(MX_PRODUCT)(held, address<void>(number(a[2])), address<void>(number(a[3])), constants, n_constants, (int)number(a[5]),
+        finish(entry<Mx_productFn>(MX_PRODUCT)(held, address<void>(number(a[2])), address<void>(number(a[3])), constants, n_constants, (int)number(a[5]),
                                               (int)number(a[6]), out, out_code, out_rows, out_cols, address<void>(number(a[8])), address<int>(number(a[9])),
                                               stream()), MX_PRODUCT, what);
         Py_RETURN_NONE;

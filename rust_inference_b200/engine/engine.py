@@ -42,6 +42,15 @@ def resolve_cache_dtype(cache_dtype):
     raise ValueError(f"cache_dtype must be 'same' or 'int8', found {cache_dtype!r}")
 
 
+def resolve_weights_dtype(weights_dtype):
+    """None (matrices in the run dtype) or "mxfp4"."""
+    if weights_dtype in (None, "same"):
+        return None
+    if weights_dtype == "mxfp4":
+        return "mxfp4"
+    raise ValueError(f"weights_dtype must be 'same' or 'mxfp4', found {weights_dtype!r}")
+
+
 def require_cuda(device) -> torch.device:
     device = torch.device(device)
     if device.type != "cuda":
@@ -119,12 +128,13 @@ class Engine:
     @classmethod
     def from_pretrained(cls, model_dir: str, *, dtype="bfloat16", device="cuda", max_tokens: int = 8192,
                         max_seq_len: int | None = None, n_slots: int | None = None,
-                        use_graphs: bool = True, cache_dtype=None) -> "Engine":
+                        use_graphs: bool = True, cache_dtype=None, weights_dtype=None) -> "Engine":
         """Load a model folder (config.json + safetensors); the model class comes from
-        config.json's architecture name."""
+        config.json's architecture name.  weights_dtype: "mxfp4" holds matrices in 4 bits (see `DecoderModel`)."""
+        weights_dtype = resolve_weights_dtype(weights_dtype)
         device = require_cuda(device)
         config, spec = load_spec(model_dir)
-        model = DecoderModel(spec, dtype=resolve_dtype(dtype), device=device)
+        model = DecoderModel(spec, dtype=resolve_dtype(dtype), device=device, weights_dtype=weights_dtype)
         model.load(read_model_tensors(model_dir, model.declared_tensors(), spec.ignored_tensors))
         eng = cls(model, max_tokens=max_tokens, max_seq_len=max_seq_len, n_slots=n_slots, use_graphs=use_graphs, cache_dtype=cache_dtype)
         eng.config = config
@@ -133,12 +143,13 @@ class Engine:
     @classmethod
     def from_random(cls, config, *, seed: int = 0, std: float = 0.02, norm_std: float = 0.0, dtype="bfloat16",
                     device="cuda", max_tokens: int = 8192, max_seq_len: int | None = None,
-                    n_slots: int | None = None, use_graphs: bool = True, cache_dtype=None) -> "Engine":
+                    n_slots: int | None = None, use_graphs: bool = True, cache_dtype=None, weights_dtype=None) -> "Engine":
         """Random weights made on the device, without a folder (benchmarks)."""
+        weights_dtype = resolve_weights_dtype(weights_dtype)
         device = require_cuda(device)
         dtype = resolve_dtype(dtype)
         spec = get_architecture(config.architecture).build_spec(config)
-        model = DecoderModel(spec, dtype=dtype, device=device)
+        model = DecoderModel(spec, dtype=dtype, device=device, weights_dtype=weights_dtype)
         model.load(random_tensors(model.declared_tensors(), seed, std=std, matrix_dtype=dtype, device=device,
                                   norm_std=norm_std))
         eng = cls(model, max_tokens=max_tokens, max_seq_len=max_seq_len, n_slots=n_slots, use_graphs=use_graphs, cache_dtype=cache_dtype)
@@ -157,7 +168,7 @@ class Engine:
         synchronisation point: a device-to-host read of the step's result); in the checked build
         (RI_B200_CHECK_BOUNDS=1) also if a kernel met an index outside its table."""
         from ..kernels import tcgen05
-        if self.dtype == torch.bfloat16:
+        if self.dtype == torch.bfloat16 or getattr(getattr(self, "model", None), "weights_dtype", None) is not None:
             tcgen05.check_status()
         tcgen05.check_f32_status()
         from ..kernels import ops

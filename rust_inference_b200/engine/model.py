@@ -75,7 +75,9 @@ class LayerProbe:
 
 
 class DecoderModel:
-    def __init__(self, spec: ModelSpec, *, dtype: torch.dtype, device):
+    def __init__(self, spec: ModelSpec, *, dtype: torch.dtype, device, weights_dtype: str | None = None):
+        """weights_dtype: None, matrices in the run dtype; "mxfp4": those of the parts that can, the attention's projections and the dense
+        feed-forwards, in microscaled 4 bits (`kernels.microscaled`), the others, embedding, head and vectors as without."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"run dtype must be float32 or bfloat16, not {dtype}")
         self.spec = spec
@@ -91,6 +93,9 @@ class DecoderModel:
         self.stream_parts = [_build("stream", ps, **kw) for ps in spec.stream_parts]
 
         self.routed = any(part.routes for layer in self.layers for part in layer.parts.values())
+        self.weights_dtype = weights_dtype
+        if weights_dtype is not None:
+            self._hold_microscaled()
 
         # the schedule: who writes which cache layer
         seen = set()
@@ -113,6 +118,19 @@ class DecoderModel:
                 raise ValueError(f"schedule names stream part {entry.before[0]}, the model has {len(self.stream_parts)}")
             self.schedule.append((entry.layer, entry.cache, writes))
             self._before.append(entry.before)
+
+    def _hold_microscaled(self) -> None:
+        if self.weights_dtype != "mxfp4":
+            raise ValueError(f"weights_dtype must be 'same' or 'mxfp4', found {self.weights_dtype!r}")
+        if self.routed:
+            # a router chooses between scores that may nearly tie, so that such a decoder's sums do not depend on a step's size; those of
+            # products in 4 bits are cut by it, and most of its weights are its experts', which stay as they are
+            raise ValueError("weights in 4 bits are for decoders that do not route tokens to experts")
+        takers = [part for layer in self.layers for part in layer.parts.values() if part.holds_microscaled]
+        if not takers:
+            raise ValueError("the model has no attention projections or dense feed-forwards whose weights could be held in 4 bits")
+        for part in takers:
+            part.weights_dtype = self.weights_dtype
 
     # ---- tensors -----------------------------------------------------------
     def _named_parts(self):
@@ -143,8 +161,10 @@ class DecoderModel:
             return ops.cast(t, dtype)
         return t.to(dtype)
 
-    def _place(self, t: torch.Tensor, ts: TensorSpec) -> torch.Tensor:
+    def _place(self, t: torch.Tensor, ts: TensorSpec, part=None) -> torch.Tensor:
         if ts.role == "matrix":
+            if part is not None and part.weights_dtype is not None:         # rounded once, from what is stored
+                return self._to(t, t.dtype if t.dtype in (torch.float32, torch.bfloat16) else torch.float32)
             return self._to(t, self.dtype)
         if ts.role == "vector":
             return self._to(t, torch.float32)
@@ -168,9 +188,9 @@ class DecoderModel:
             ts = declared[name]
             if tuple(t.shape) != tuple(ts.shape):
                 raise ValueError(f"{name}: expected shape {list(ts.shape)}, found {list(t.shape)}")
-            placed = self._place(t, ts)
-            got.add(name)
             part, local = owners[name]
+            placed = self._place(t, ts, part)
+            got.add(name)
             bucket = pending.setdefault(id(part), (part, {}))[1]
             bucket[local] = placed
             if len(bucket) == counts[id(part)]:
@@ -217,6 +237,7 @@ class DecoderModel:
         is held in (the embedding table only counts when it is also the head, or when asked)."""
         total = 0
         item = 4 if self.dtype == torch.float32 else 2
+        held = {prefix + local for prefix, part in self._named_parts() if part.weights_dtype is not None for local in part.tensor_specs()}
         skip = set()
         if not include_embedding and not self.head.wants_tie:
             skip = {self._embedding_spec.prefix + local for local in self.embedding.tensor_specs()}
@@ -225,6 +246,9 @@ class DecoderModel:
             for d in ts.shape:
                 n *= d
             if name in skip:
+                continue
+            if name in held and ts.role == "matrix":
+                total += ts.shape[0] * -(-ts.shape[1] // 128) * (64 + 4)       # 128 numbers: half a byte each, four exponents
                 continue
             total += n * (item if ts.role == "matrix" else 4)
         return total

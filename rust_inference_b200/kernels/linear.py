@@ -33,6 +33,11 @@ def is_microscaled(w) -> bool:
     return type(w) is microscaled.Matrix
 
 
+def plain(w, dtype: torch.dtype) -> torch.Tensor:
+    """The matrix [out, in] itself, or the numbers that one in 4 bits stands for, in the run dtype."""
+    return microscaled.values(w, dtype) if is_microscaled(w) else w.t
+
+
 def _use_tensor_cores(x: torch.Tensor, w: Weight) -> bool:
     if is_microscaled(w) or x.dtype != torch.bfloat16:
         return False
@@ -125,6 +130,9 @@ def accumulate_split(x, w: Weight, acc, ctx) -> bool:
     """acc<float32> += x W^T with K split over enough CTAs to fill the GPU, if the tensor-core
     kernel takes the shape (returns False otherwise and does nothing).  For small steps whose
     output has too few tiles to keep every SM streaming weights."""
+    if is_microscaled(w):
+        microscaled.product(x, w, acc, ctx, add=True)
+        return True
     if not _use_tensor_cores(x, w):
         return False
     tcgen05.gemm(x, w, acc, ops.EPI_RESIDUAL, ctx)
@@ -137,8 +145,11 @@ def accumulate_split(x, w: Weight, acc, ctx) -> bool:
 SPLIT_MAX_TOKENS = 256
 
 
-def wants_split(x, w: Weight) -> bool:
-    """True for a small step whose projection would otherwise leave most SMs idle."""
+def wants_split(x, w: Weight, dtype: torch.dtype | None = None) -> bool:
+    """True for a small step whose projection would otherwise leave most SMs idle.  (`dtype`: the run dtype, for x in 8 bits and a
+    matrix in 4, whose sums go to the accumulators in small steps likewise, for the kernels that take them from there.)"""
+    if is_microscaled(w):
+        return dtype is torch.bfloat16 and x.shape[0] <= SPLIT_MAX_TOKENS
     if not _use_tensor_cores(x, w) or x.shape[0] > SPLIT_MAX_TOKENS:
         return False
     return tcgen05.pick_split(x.shape[0], w.n, w.k) > 1

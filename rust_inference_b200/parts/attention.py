@@ -32,6 +32,8 @@ class GQAttention(Mixer):
     kv head h / (heads / kv heads) (:37, :96), and the output projection without bias added
     onto the residual stream (:123, transformer.rs:38-39)."""
 
+    holds_microscaled = True
+
     # Beyond the dense decoder's form, as parameters: values of a head size of their own (`v_head_dim`),
     # a score scale other than 1/sqrt(head_dim) (`scale`), keys limited to the query's own block of
     # `chunk` positions counted from the start of the sequence, a factor on the mixer's result
@@ -184,7 +186,7 @@ class GQAttention(Mixer):
             rows = sum(m.shape[0] for m in mats)
             if rows % 8:                               # rows of zeros keep a token's row a multiple of 16 bytes, which the
                 mats.append(torch.zeros(-rows % 8, mats[0].shape[1], dtype=mats[0].dtype, device=mats[0].device))   # tensor-core kernels want
-        self.w_qkv = linear.Weight(torch.cat(mats, dim=0))
+        self.w_qkv = self.weight(torch.cat(mats, dim=0))
         if self.sink:
             self.sinks = tensors[nm["sink"]].contiguous()
         if self.fixed_sink is not None:
@@ -207,12 +209,12 @@ class GQAttention(Mixer):
             self.b_qkv = torch.cat(biases, dim=0).contiguous()
             if self.b_qkv.numel() < self.w_qkv.n:      # the gates' rows, and the rows of zeros after them
                 self.b_qkv = torch.cat([self.b_qkv, self.b_qkv.new_zeros(self.w_qkv.n - self.b_qkv.numel())]).contiguous()
-        self.w_o = linear.Weight(tensors[nm["o"]])
+        self.w_o = self.weight(tensors[nm["o"]])
 
     def get_tensors(self):
         q, kv, nm = self.q_dim, self.kv_dim, self.names
-        w = self.w_qkv.t
-        out = {nm["q"]: w[:q], nm["o"]: self.w_o.t}
+        w = linear.plain(self.w_qkv, self.dtype)
+        out = {nm["q"]: w[:q], nm["o"]: linear.plain(self.w_o, self.dtype)}
         at = q
         if self.own_kv:
             out[nm["k"]] = w[q:q + kv]
@@ -309,7 +311,7 @@ class GQAttention(Mixer):
         if self._formed_in_attention(x, width, residual, ctx, cache_layer, writes_cache):
             return
         from_acc = getattr(self.position, "apply_and_store_from_accumulators", None) if usual else None
-        if from_acc is not None and linear.wants_split(x, self.w_qkv):
+        if from_acc is not None and linear.wants_split(x, self.w_qkv, self.dtype):
             # a small step: the projection is split over K into float32 accumulators, and the
             # position encoding adds the bias, rotates and stores from there
             acc = ctx.zeroed_buffer("qkv_acc", (n, width), torch.float32)
@@ -318,7 +320,7 @@ class GQAttention(Mixer):
             from_acc(acc, self.b_qkv, qkv, ctx, cache_layer, n_heads=self.n_heads, n_kv_heads=self.n_kv_heads,
                      head_dim=self.head_dim, write_kv=writes_cache)
         elif (special and not self.values_from_keys and not self.head_gate and not self.out_gate and writes_cache and self.own_kv
-              and linear.wants_split(x, self.w_qkv) and hasattr(self.position, "apply_normed_and_store_from_accumulators")):
+              and linear.wants_split(x, self.w_qkv, self.dtype) and hasattr(self.position, "apply_normed_and_store_from_accumulators")):
             # the same for heads that are normed, or whose values are blended
             acc = ctx.zeroed_buffer("qkv_acc", (n, width), torch.float32)
             linear.accumulate_split(x, self.w_qkv, acc, ctx)
@@ -356,7 +358,7 @@ class GQAttention(Mixer):
         q = ctx.buffer("q_rot", (n, self.q_dim), self.dtype)
         sizes = dict(n_heads=self.n_heads, n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, v_head_dim=self.v_head_dim)
         gates = None                            # the projection's rows, where gates lie behind the values
-        if width == gate_col and linear.wants_split(x, self.w_qkv):
+        if width == gate_col and linear.wants_split(x, self.w_qkv, self.dtype):
             acc = ctx.zeroed_buffer("qkv_acc", (n, width), torch.float32)
             linear.accumulate_split(x, self.w_qkv, acc, ctx)
             self.position.apply_and_quantize(acc, q, ctx, cache_layer, bias=self.b_qkv, clear=True, **sizes)
@@ -370,7 +372,7 @@ class GQAttention(Mixer):
         """A decode step whose projection is split over K: the attention's own kernel adds the bias to the sums, norms and turns the
         heads and writes the cache.  False (nothing done) where it does not take the step."""
         if (not ctx.all_single or self.extended or self.value_mix is not None or not writes_cache or self.v_head_dim != self.head_dim
-                or type(self.position) is not RotaryEncoding or not linear.wants_split(x, self.w_qkv)
+                or type(self.position) is not RotaryEncoding or not linear.wants_split(x, self.w_qkv, self.dtype)
                 or quantized_cache.is_quantized(cache_layer)):
             return False                # (a position encoding of a caller's own has steps of its own)
         if getattr(ctx, "routed", False) and (self.position.partial or self.qk_norm_eps is not None or self.values_from_keys or self.out_scale != 1.0):

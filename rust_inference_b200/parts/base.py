@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import torch
 
+from ..kernels import linear, microscaled
 from .spec import TensorSpec
 
 
@@ -25,19 +26,38 @@ class Part:
     # before it becomes another choice, so a decoder with such a part keeps its products' sums and its heads' roundings as they are
     # for any number of tokens (`StepContext.routed`).
     routes = False
+    # True if the part's matrices may be held in microscaled 4 bits (`kernels.microscaled`): it makes its products by `kernels.linear`
+    # from what `weight` gives it, and reads its input by nothing else.
+    holds_microscaled = False
+    weights_dtype = None                         # None: matrices in the run dtype; "mxfp4": in 4 bits (set before the tensors arrive)
 
     def __init__(self, *, hidden_size: int, dtype: torch.dtype, device):
         self.hidden_size = hidden_size
         self.dtype = dtype
         self.device = torch.device(device)
 
+    def weight(self, t: torch.Tensor):
+        """A matrix as the part's products take it."""
+        if self.weights_dtype is None:
+            return linear.Weight(t)
+        return microscaled.Matrix.of(t)
+
+    @property
+    def takes_rows(self) -> bool:
+        """Whether the part's input may come as rows in 8 bits."""
+        return self.weights_dtype is not None
+
+    def scratch(self, ctx, name: str, n: int, k: int):
+        """Scratch for rows [n, k] that only products of this part read: in 8 bits where its matrices are in 4."""
+        return ctx.buffer(name, (n, k), self.dtype) if self.weights_dtype is None else ctx.workspace.rows(name + "_rows", n, k)
+
     def tensor_specs(self) -> dict:
         """Local tensor name -> TensorSpec."""
         return {}
 
     def set_tensors(self, tensors: dict) -> None:
-        """Receives the declared tensors: matrices in the run dtype, vectors float32,
-        tables int32, all on the device."""
+        """Receives the declared tensors: matrices in the run dtype (float32 or bfloat16, as they are stored, where the part holds
+        them in 4 bits), vectors float32, tables int32, all on the device."""
         if tensors:
             raise NotImplementedError
 
@@ -54,6 +74,8 @@ class Part:
 
 
 class Norm(Part):
+    makes_rows = False        # True: `out` may be `microscaled.Rows` (without `rows`)
+
     def forward(self, x: torch.Tensor, out: torch.Tensor, rows: torch.Tensor | None = None) -> torch.Tensor:
         """x float32 [*, hidden] -> out (run dtype) [R, hidden]; `rows` picks input rows."""
         raise NotImplementedError
@@ -170,6 +192,14 @@ class Arrangement:
     def cache_request(self, mixer_request):
         """What the layer needs of the cache, given what its mixer asks for (None: it has none or asks for nothing)."""
         return mixer_request
+
+    @staticmethod
+    def normed_buffer(residual: torch.Tensor, ctx, norm, reader):
+        """Scratch for what `norm` makes of the stream and `reader` alone reads: rows in 8 bits where both sides deal in them."""
+        n, k = residual.shape
+        if getattr(norm, "makes_rows", False) and getattr(reader, "takes_rows", False):
+            return ctx.workspace.rows("normed_rows", n, k)
+        return ctx.buffer("normed", (n, k), ctx.dtype)
 
     def forward(self, residual: torch.Tensor, ctx, cache_layer, writes_cache: bool) -> None:
         raise NotImplementedError

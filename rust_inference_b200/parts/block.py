@@ -17,11 +17,12 @@ class PreNorm(Arrangement):
     ROLES = {"mixer": "mixer", "feed_forward": "feed_forward", "mixer_norm": "norm", "feed_forward_norm": "norm"}
 
     def forward(self, residual, ctx, cache_layer, writes_cache):
-        normed = ctx.buffer("normed", (residual.shape[0], residual.shape[1]), ctx.dtype)
+        normed = self.normed_buffer(residual, ctx, self.mixer_norm, self.mixer)
         self.mixer_norm.forward(residual, normed)
         self.mixer.forward(normed, residual, ctx, cache_layer, writes_cache)
         if self.feed_forward is None:
             return
+        normed = self.normed_buffer(residual, ctx, self.feed_forward_norm, self.feed_forward)
         self.feed_forward_norm.forward(residual, normed)
         self.feed_forward.forward(normed, residual, ctx)
 

@@ -14,6 +14,7 @@ from .spec import TensorSpec
 
 @register("feed_forward", "swiglu")
 class SwiGLU(FeedForward):
+    holds_microscaled = True
     def __init__(self, *, intermediate_size: int, hidden_size: int, dtype, device):
         super().__init__(hidden_size=hidden_size, dtype=dtype, device=device)
         self.intermediate_size = intermediate_size
@@ -28,15 +29,15 @@ class SwiGLU(FeedForward):
         }
 
     def set_tensors(self, tensors):
-        self.w_gate = linear.Weight(tensors["gate_proj.weight"])
-        self.w_up = linear.Weight(tensors["up_proj.weight"])
-        self.w_down = linear.Weight(tensors["down_proj.weight"])
+        self.w_gate = self.weight(tensors["gate_proj.weight"])
+        self.w_up = self.weight(tensors["up_proj.weight"])
+        self.w_down = self.weight(tensors["down_proj.weight"])
 
     def get_tensors(self):
-        return {"gate_proj.weight": self.w_gate.t, "up_proj.weight": self.w_up.t, "down_proj.weight": self.w_down.t}
+        return {"gate_proj.weight": linear.plain(self.w_gate, self.dtype), "up_proj.weight": linear.plain(self.w_up, self.dtype), "down_proj.weight": linear.plain(self.w_down, self.dtype)}
 
     def forward(self, x, residual, ctx):
-        act = ctx.buffer("ffn_act", (x.shape[0], self.intermediate_size), self.dtype)
+        act = self.scratch(ctx, "ffn_act", x.shape[0], self.intermediate_size)
         # gate and up in one pass over x, SiLU-gate in the epilogue (mlp.rs:35-43)
         linear.gated(x, self.w_gate, self.w_up, act, ctx)
         # down projection added onto the residual stream (mlp.rs:45, transformer.rs:47)
@@ -48,6 +49,8 @@ class BoundedGLU(FeedForward):
     """y = g * sigmoid(alpha * g) * (u + shift) with g = min(W_gate x, limit) and u = clamp(W_up x, -limit, limit);
     out = W_down y.  The activation is the gated epilogue of the gate / up contraction with these three
     constants (float32 arithmetic on the accumulators).  `names`: gate, up, down below the part's prefix."""
+
+    holds_microscaled = True
 
     _NAMES = {"gate": "gate_proj.weight", "up": "up_proj.weight", "down": "down_proj.weight"}
 
@@ -70,16 +73,16 @@ class BoundedGLU(FeedForward):
 
     def set_tensors(self, tensors):
         nm = self.names
-        self.w_gate = linear.Weight(tensors[nm["gate"]])
-        self.w_up = linear.Weight(tensors[nm["up"]])
-        self.w_down = linear.Weight(tensors[nm["down"]])
+        self.w_gate = self.weight(tensors[nm["gate"]])
+        self.w_up = self.weight(tensors[nm["up"]])
+        self.w_down = self.weight(tensors[nm["down"]])
 
     def get_tensors(self):
         nm = self.names
-        return {nm["gate"]: self.w_gate.t, nm["up"]: self.w_up.t, nm["down"]: self.w_down.t}
+        return {nm["gate"]: linear.plain(self.w_gate, self.dtype), nm["up"]: linear.plain(self.w_up, self.dtype), nm["down"]: linear.plain(self.w_down, self.dtype)}
 
     def forward(self, x, residual, ctx):
-        act = ctx.buffer("ffn_act", (x.shape[0], self.intermediate_size), self.dtype)
+        act = self.scratch(ctx, "ffn_act", x.shape[0], self.intermediate_size)
         linear.gated(x, self.w_gate, self.w_up, act, ctx, form=self.form)
         linear.into_residual(act, self.w_down, residual, ctx)
 
@@ -90,6 +93,8 @@ class GatedDense(FeedForward):
     (0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))), computed as z sigmoid(2 sqrt(2/pi) z (1 + 0.044715 z^2))).
     The activation and the factor are the gated epilogue of the gate / up contraction (float32 arithmetic on the
     accumulators).  `names`: gate, up, down below the part's prefix."""
+
+    holds_microscaled = True
 
     _NAMES = {"gate": "gate_proj.weight", "up": "up_proj.weight", "down": "down_proj.weight"}
     ACTIVATIONS = {"silu": (1.0, 0.0), "gelu_tanh": (ops.GELU_TANH_ALPHA, ops.GELU_TANH_CUBIC)}
@@ -111,16 +116,16 @@ class GatedDense(FeedForward):
 
     def set_tensors(self, tensors):
         nm = self.names
-        self.w_gate = linear.Weight(tensors[nm["gate"]])
-        self.w_up = linear.Weight(tensors[nm["up"]])
-        self.w_down = linear.Weight(tensors[nm["down"]])
+        self.w_gate = self.weight(tensors[nm["gate"]])
+        self.w_up = self.weight(tensors[nm["up"]])
+        self.w_down = self.weight(tensors[nm["down"]])
 
     def get_tensors(self):
         nm = self.names
-        return {nm["gate"]: self.w_gate.t, nm["up"]: self.w_up.t, nm["down"]: self.w_down.t}
+        return {nm["gate"]: linear.plain(self.w_gate, self.dtype), nm["up"]: linear.plain(self.w_up, self.dtype), nm["down"]: linear.plain(self.w_down, self.dtype)}
 
     def forward(self, x, residual, ctx):
-        act = ctx.buffer("ffn_act", (x.shape[0], self.intermediate_size), self.dtype)
+        act = self.scratch(ctx, "ffn_act", x.shape[0], self.intermediate_size)
         linear.gated(x, self.w_gate, self.w_up, act, ctx, form=self.form)
         linear.into_residual(act, self.w_down, residual, ctx)
 
@@ -131,6 +136,8 @@ class DenseActivation(FeedForward):
     act(z) = softplus(p) z^2 + z / 2 for z > 0 and (1/2 + softplus(q)) (e^z - 1 - z) + z / 2 otherwise, applied to
     the up projection's float32 accumulators in that product's epilogue; p and q are read on the device.  "relu_squared":
     act(z) = max(z, 0)^2 in the same epilogue, without a tensor of its own.  `names`: up, down, act below the prefix."""
+
+    holds_microscaled = True
 
     _NAMES = {"up": "up_proj.weight", "down": "down_proj.weight", "act": "act"}
     ACTIVATIONS = ("xielu", "relu_squared")
@@ -153,7 +160,7 @@ class DenseActivation(FeedForward):
 
     def set_tensors(self, tensors):
         nm = self.names
-        self.w_up, self.w_down = linear.Weight(tensors[nm["up"]]), linear.Weight(tensors[nm["down"]])
+        self.w_up, self.w_down = self.weight(tensors[nm["up"]]), self.weight(tensors[nm["down"]])
         if self.activation == "xielu":
             self.act = ops.whole_act_form(tensors[nm["act"]]).contiguous()
         else:
@@ -161,12 +168,12 @@ class DenseActivation(FeedForward):
 
     def get_tensors(self):
         nm = self.names
-        out = {nm["up"]: self.w_up.t, nm["down"]: self.w_down.t}
+        out = {nm["up"]: linear.plain(self.w_up, self.dtype), nm["down"]: linear.plain(self.w_down, self.dtype)}
         if self.activation == "xielu":
             out[nm["act"]] = self.act[:2]
         return out
 
     def forward(self, x, residual, ctx):
-        act = ctx.buffer("ffn_act", (x.shape[0], self.intermediate_size), self.dtype)
+        act = self.scratch(ctx, "ffn_act", x.shape[0], self.intermediate_size)
         linear.activated(x, self.w_up, act, ctx, self.act)
         linear.into_residual(act, self.w_down, residual, ctx)

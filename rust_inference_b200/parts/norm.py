@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import torch
 
-from ..kernels import ops
+from ..kernels import microscaled, ops
 from .base import Norm
 from .registry import register
 from .spec import TensorSpec
@@ -37,7 +37,11 @@ class RMSNorm(Norm):
     def get_tensors(self):
         return {self.weight_name: self.weight}
 
+    makes_rows = True
+
     def forward(self, x, out, rows=None):
+        if type(out) is microscaled.Rows:
+            return microscaled.rmsnorm(x, self.factor, self.eps, out)
         return ops.rmsnorm(x, self.factor, self.eps, out, rows)
 
     def forward_times(self, factor: float, x, out, rows=None):

@@ -39,6 +39,7 @@ constexpr int CLUSTER_MOST = 8;
 constexpr int TOKENS_MOST = 128;                   // of a tile of the first kernel
 
 enum Status { ST_PRODUCER_TIMEOUT = 51, ST_MMA_TIMEOUT = 52, ST_EPILOGUE_TIMEOUT = 53, ST_DRAIN_TIMEOUT = 54 };
+constexpr int NEEDS_ROWS = 2;                       // a product's answer to plain rows that have to be in 8 bits before
 enum Out { OUT_BF16 = 0, OUT_F32 = 1, OUT_ROWS = 2, OUT_ADD = 3 };
 
 // Instruction descriptor of kind mxf8f6f4: the exponents' byte of A (bits 29, 30) and of B (4, 5) to be set per instruction, types of A and B
@@ -189,19 +190,81 @@ __device__ __forceinline__ void store_lanes(const Result& r, T t, G good, int f,
     }
 }
 
+// Plain rows that a kernel for few tokens brings to 8 bits itself: up to PLAIN_MOST of them, whose spans all have a stage of the ring.  The epilogue's
+// warps, which have nothing else to do then, read them and write codes and exponents as TMA would have brought them.  (A product of [3584, 3584], us,
+// rows that are in 8 bits, plain ones, plain ones by a kernel before: 1 token 5.2 / 5.3 / 6.4, 4 tokens 5.4 / 5.7 / 5.9, 8 tokens 5.5 / 6.2 / 5.9.)
+constexpr int PLAIN_MOST = 4;
+struct PlainRows {
+    const void* at;              // null: rows in 8 bits come by TMA
+    int f32, k;
+    long long ld;
+};
+
+// The CTA's spans, `count` from `begin` on, by 256 threads: eight numbers of a row each, so that sixteen threads have a span of a row, and four a
+// block; four reads of a thread are on their way together.
+template <typename T>
+__device__ __forceinline__ void write_plain(const PlainRows& x, int n_tok, int begin, int count, uint32_t tiles, uint32_t tile_bytes, uint32_t pieces,
+                                            uint32_t piece_bytes, int thread) {
+    const int items = count * n_tok * 16, chunk = thread & 15;
+    for (int i0 = thread; i0 < items + 15; i0 += 4 * 256) {           // (whole quads go round together: items is a multiple of 16)
+        float v[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = (i0 + i * 256) >> 4, span = q / n_tok, row = q - span * n_tok, c = (begin + span) * SPAN + chunk * 8;
+            const bool there = span < count && c < x.k;
+            if (sizeof(T) == 2) {
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (there) {
+                    const float4 f = load_written(reinterpret_cast<const float*>(reinterpret_cast<const T*>(x.at) + (size_t)row * x.ld + c));
+                    w = *reinterpret_cast<const uint4*>(&f);
+                }
+                unpack8(w, v[i]);
+            } else {
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+                if (there) {
+                    const float* at = reinterpret_cast<const float*>(x.at) + (size_t)row * x.ld + c;
+                    a = load_written(at);
+                    b = load_written(at + 4);
+                }
+                v[i][0] = a.x; v[i][1] = a.y; v[i][2] = a.z; v[i][3] = a.w;
+                v[i][4] = b.x; v[i][5] = b.y; v[i][6] = b.z; v[i][7] = b.w;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = (i0 + i * 256) >> 4, span = q / n_tok, row = q - span * n_tok;
+            if (span >= count) break;
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+            const uint32_t four = 0xfu << (threadIdx.x & 28);
+            top = max(top, __shfl_xor_sync(four, top, 1));
+            top = max(top, __shfl_xor_sync(four, top, 2));
+            const uint32_t byte = exponent_byte<8>(top);
+            const float f = to_type(byte);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] *= f;
+            const uint32_t at = tiles + (uint32_t)span * tile_bytes + row * SPAN + (((chunk >> 1) ^ (row & 7)) << 4) + (chunk & 1) * 8;
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(eight_bits(v[i])), "r"(eight_bits(v[i] + 4)) : "memory");
+            if ((chunk & 3) == 0)
+                asm volatile("st.shared.b8 [%0], %1;" ::"r"(pieces + (uint32_t)span * piece_bytes + row * 16 + (chunk >> 2)), "r"(byte) : "memory");
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------
 // Few tokens.  Tiles of 128 features x tn tokens, for a persistent grid of CTAs, or (not gated) each for a cluster whose CTAs share its K.  Warp 0 issues the copies, warp 1 allocates tensor memory and issues the MMAs,
 // warps 2-9 run the epilogue, two for each quarter of tensor memory's lanes, which take turns at 16 tokens.
 // ---------------------------------------------------------------------------------------------
 template <bool DUAL, int OUT>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS, DUAL ? 1 : 2)
 mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const __grid_constant__ CUtensorMap map_x,
-                  const uint8_t* __restrict__ w_exp, const uint8_t* __restrict__ w2_exp, const uint8_t* x_exp, const float* __restrict__ constants, int act,
-                  Result res, int n_tok, int n_feat, int n_spans, int cluster, int stages, int tn, int buffers, int tmem_cols, int* status) {
+                  const uint8_t* __restrict__ w_exp, const uint8_t* __restrict__ w2_exp, const uint8_t* x_exp, const PlainRows plain, const float* __restrict__ constants, int act,
+                  Result res, int n_tok, int n_feat, int n_spans, int cluster, int stages, int tn, int buffers, int tmem_cols, int recv_at, int* status) {
     constexpr int MATS = DUAL ? 2 : 1;
     const uint32_t tile_bytes = MATS * TILE + tn * SPAN;                          // of a stage's codes
     constexpr uint32_t EXP_BYTES = (MATS + 1) * PIECE;                            // of its exponents
-    const uint32_t stage_tx = (uint32_t)(MATS * (W_COPIED + PIECE) + tn * SPAN + PIECE);
+    const uint32_t stage_tx = (uint32_t)(MATS * (W_COPIED + PIECE) + (plain.at == nullptr ? tn * SPAN + PIECE : 0));
     const int acc_cols = MATS * tn;
     const uint32_t idesc = instruction(ROWS, tn, 5, 0);
 
@@ -227,7 +290,7 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
-            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&full_bar[s]), plain.at == nullptr ? 1 : 9);         // the copies', and the writing warps'
             mbar_init(smem_u32(&empty_bar[s]), 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -280,6 +343,7 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
                     if (DUAL) load_piece_by(leader, ex + PIECE, we2 + (size_t)j * PIECE, bar);
                 };
                 auto load_x = [&](int at, int j) {
+                    if (plain.at != nullptr) return;
                     const uint32_t bar = full0 + 8u * (uint32_t)at;
                     load_2d_by(leader, smem_base + (uint32_t)at * tile_bytes + MATS * TILE, &map_x, bar, (begin + j) * SPAN, t0);
                     load_piece_by(leader, exp_base + (uint32_t)at * EXP_BYTES + MATS * PIECE, xe + (size_t)j * PIECE, bar);
@@ -308,6 +372,7 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
                     ring.next(stages, looked);
                 }
             }
+            RI_PHASE_LATEST(1);
             // do not leave, or hand the ring to the cluster, while a copy into it may still be in flight
             for (int j = max(0, it - stages); j < it; ++j)
                 if (!mbar_wait_warp(full0 + 8u * (uint32_t)(j % stages), (uint32_t)(j / stages) & 1u)) {
@@ -359,6 +424,14 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         }
     } else {
         wait_for_previous_kernels();          // `out` may still be read or written by the kernel before
+        if (plain.at != nullptr) {                                // (a CTA has one tile then, and count <= stages)
+            const uint32_t tiles = smem_base + MATS * TILE, pieces = exp_base + MATS * PIECE;
+            if (plain.f32) write_plain<float>(plain, n_tok, begin, count, tiles, tile_bytes, pieces, EXP_BYTES, (int)threadIdx.x - 64);
+            else write_plain<__nv_bfloat16>(plain, n_tok, begin, count, tiles, tile_bytes, pieces, EXP_BYTES, (int)threadIdx.x - 64);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");           // for the tensor cores' reads
+            __syncwarp();
+            if (lane < count) mbar_arrive(full0 + 8u * (uint32_t)lane);
+        }
         const Epilogue e = load_epilogue<DUAL>(constants, act);
         for (int i = 0; i < my_tiles; ++i) {
             int f0, t0;
@@ -394,23 +467,24 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         }
     }
 
+    RI_PHASE_LATEST(2);
     if constexpr (!DUAL) if (clustered) {
         // Token c of the tile is finished by the CTA of rank c % cluster: everybody sends it its sums of that token, into `recv`
-        // [rank of the sender][c / cluster][128], which lies where the ring was, and it adds them in the order of the ranks.
+        // [rank of the sender][c / cluster][128], and it adds them in the order of the ranks.  `recv` lies behind the ring, where both are in
+        // the shared memory that there is (`recv_at`), else where the ring was, once nobody's is in use any more.
         // A CTA that gave up says so before; then none of the cluster writes.
         const int held = (tn + cluster - 1) / cluster;
         int f0, t0;
         tile_coords(0, f0, t0);
         const int tokens = min(tn, n_tok - t0);
-        float* recv = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)));
+        float* recv = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)) + recv_at);
         const int fl = quarter * 32 + lane;
         __syncwarp();
         cluster_wait();                                            // the peers run
         if (abort_flag && lane == 0) set_in_all(&any_failed, cluster);
         __syncwarp();
-        cluster_sync();                                            // nobody's ring is in use any more
-        const bool failed = any_failed != 0;
-        if (warp >= 2 && !failed) {
+        if (recv_at == 0) cluster_sync();                          // nobody's ring is in use any more
+        if (warp >= 2 && !abort_flag) {
             const uint32_t trow = tmem_base + ((uint32_t)(quarter * 32) << 16);
             const float* mine = recv + (size_t)rank * held * ROWS + fl;
 #pragma unroll 1
@@ -428,6 +502,7 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         }
         __syncwarp();
         cluster_sync();                                            // everything sent has arrived
+        const bool failed = any_failed != 0;
         const int f = f0 + fl;
         if (warp >= 2 && !failed) {
             const Epilogue e = load_epilogue<false>(constants, act);
@@ -453,6 +528,7 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 
     tc_fence_before();
     __syncthreads();
+    RI_PHASE_LATEST(5);
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)tmem_cols) : "memory");
@@ -802,6 +878,7 @@ struct Call {
     Plan plan;
     const Maps *w, *w2, *x;
     const uint8_t *w_exp, *w2_exp, *x_exp;
+    PlainRows plain;
     const float* constants;
     int act;
     Result res;
@@ -882,9 +959,13 @@ int launch_feature(const Call& c) {
     if (stages > MAX_STAGES) stages = MAX_STAGES;
     if (p.cluster > 1 && stages > most) stages = most;
     const size_t ring = (size_t)stages * stage;
-    size_t smem = (ring > (size_t)recv ? ring : (size_t)recv) + 1024;
+    // what a cluster's CTAs send each other has a place of its own where it is small (a meeting point fewer), else the ring's
+    const bool apart = p.cluster > 1 && recv <= 32 * 1024 && ring + recv + 1024 <= (size_t)(p.per_sm == 2 ? SMEM_LIMIT / 2 : SMEM_LIMIT);
+    const int recv_at = apart ? (int)ring : 0;
+    size_t smem = (apart ? ring + recv : ring > (size_t)recv ? ring : (size_t)recv) + 1024;
     long long ctas = tiles * p.cluster;
     if (p.cluster == 1 && ctas > sm_count()) ctas = sm_count();
+    if (c.plain.at != nullptr && (stages < most || ctas < tiles)) return NEEDS_ROWS;
     // two accumulators, so that a tile's epilogue runs beside the next one's MMAs, where a CTA has several tiles and the columns suffice
     constexpr int EXP_COLS = 2 * (MATS + 1) * 4;
     const int one = MATS * p.tn + EXP_COLS, two = one + MATS * p.tn;
@@ -895,7 +976,7 @@ int launch_feature(const Call& c) {
     // shared memory in proportion to their columns keeps all that an SM takes in within its 512 columns.
     if (p.cluster > 1 && smem < (size_t)cols * 456) smem = (size_t)cols * 456 < SMEM_LIMIT ? (size_t)cols * 456 : SMEM_LIMIT;
     return launch_cluster("gemm_microscaled", kernel, dim3((unsigned)ctas), THREADS, smem, p.cluster, c.stream, c.w->codes, c.w2->codes, c.x->codes, c.w_exp,
-                          c.w2_exp, c.x_exp, c.constants, c.act, c.res, c.n_tok, c.n_feat, c.n_spans, p.cluster, stages, p.tn, buffers, cols, c.status);
+                          c.w2_exp, c.x_exp, c.plain, c.constants, c.act, c.res, c.n_tok, c.n_feat, c.n_spans, p.cluster, stages, p.tn, buffers, cols, recv_at, c.status);
 }
 
 template <bool DUAL, int OUT>
@@ -930,33 +1011,41 @@ RI_API int ri_mx_set_pairs(int tokens) {
 
 // out = X W^T with an epilogue: a bias or nothing (`constants` float32 [features] or null); `act`: an activation's four constants; w2 not null:
 // the gate's five constants, or null for silu; `add`: added to out.  x, w, w2 and, where the result is rows in 8 bits, out_held are `Held`s; otherwise
-// `out` is [out_rows, out_cols] of `out_dtype`.  `status` is a host-visible int that receives a code if a wait ran out.
-RI_API int ri_mx_product(void* x_held, void* w_held, void* w2_held, const float* constants, long long n_constants, int act, int add, void* out,
-                         int out_dtype, long long out_rows, long long out_cols, void* out_held, int* status, cudaStream_t stream) {
+// `out` is [out_rows, out_cols] of `out_dtype`.  X is what x holds, or, with `x_plain` not null, the plain rows
+// [x->n, x->k] there, `x_ld` numbers apart; the answer is 2, and nothing is done, where they have to be brought to x first.
+// `status` is a host-visible int that receives a code if a wait ran out.
+RI_API int ri_mx_product(void* x_held, const void* x_plain, int x_dtype, long long x_rows, long long x_cols, long long x_ld, void* w_held, void* w2_held, const float* constants,
+                         long long n_constants, int act, int add, void* out, int out_dtype, long long out_rows, long long out_cols, void* out_held,
+                         int* status, cudaStream_t stream) {
     Held *x = (Held*)x_held, *w = (Held*)w_held, *w2 = (Held*)w2_held, *to = (Held*)out_held;
+    const long long n_tok = x->n;
     int device = -1;
     if (cudaGetDevice(&device) != cudaSuccess || x->device != device || w->device != device || (w2 && w2->device != device) || (to && to->device != device))
         return fail("gemm_microscaled: rows and matrices lie on the current device");
-    if (x->bits != 8 || w->bits != 4 || x->k != w->k || (w2 && (w2->bits != 4 || w2->n != w->n || w2->k != w->k)))
-        return fail("gemm_microscaled: rows [%d, %d] in %d bits and a matrix [%d, %d] in %d", x->n, x->k, x->bits, w->n, w->k, w->bits);
-    if (to ? (to->bits != 8 || to->n != x->n || to->k != w->n) : (out_rows != x->n || out_cols != w->n))
-        return fail("gemm_microscaled: the result is [%d, %d]", x->n, w->n);
+    if (x->bits != 8 || x->k != w->k || w->bits != 4 || (w2 && (w2->bits != 4 || w2->n != w->n || w2->k != w->k)))
+        return fail("gemm_microscaled: rows and a matrix [%d, %d], or two matrices, that do not go together", w->n, w->k);
+    if (x_plain && (x_rows != x->n || x_cols != x->k || x_ld < x->k)) return fail("gemm_microscaled: plain rows [%lld, %lld] for [%d, %d]", x_rows, x_cols, x->n, x->k);
+    if (to ? (to->bits != 8 || to->n != n_tok || to->k != w->n) : (out_rows != n_tok || out_cols != w->n))
+        return fail("gemm_microscaled: the result is [%lld, %d]", n_tok, w->n);
     if (to && (to->codes == x->codes || to->exponents == x->exponents)) return fail("gemm_microscaled: rows cannot be their own product");
     if (add && (to || out_dtype != RI_F32)) return fail("gemm_microscaled: sums are added to float32 numbers");
     if ((act != 0) + (add != 0) + (w2 != nullptr) > 1 || (add && constants)) return fail("gemm_microscaled: a bias, an activation, a gate and an addition are not combined");
     if ((act && !constants) || (constants && n_constants != (act ? 4 : w2 ? 5 : w->n)))
         return fail("gemm_microscaled: %lld constants of an epilogue", n_constants);
-    const Plan p = plan(x->n, w->n, w->n_spans, w2 != nullptr);
+    // plain rows are read in whole eights on 16-byte boundaries
+    if (x_plain && (n_tok > PLAIN_MOST || x->k % 8 || (uintptr_t)x_plain % 16 || x_ld * (x_dtype == RI_BF16 ? 2 : 4) % 16)) return NEEDS_ROWS;
+    const Plan p = plan((int)n_tok, w->n, w->n_spans, w2 != nullptr);
     Call c;
     c.plan = p;
     if (maps_of(x, p.tn, &c.x) || maps_of(w, ROWS, &c.w) || maps_of(w2 ? w2 : w, ROWS, &c.w2)) return 1;
     c.x_exp = x->exponents;
+    c.plain = PlainRows{x_plain, x_dtype != RI_BF16, w->k, x_ld};
     c.w_exp = w->exponents;
     c.w2_exp = w2 ? w2->exponents : nullptr;
     c.constants = constants;
     c.act = act;
     c.res = to ? Result{to->codes, to->exponents, to->n_spans} : Result{out, nullptr, 0};
-    c.n_tok = x->n;
+    c.n_tok = (int)n_tok;
     c.n_feat = w->n;
     c.n_spans = w->n_spans;
     c.status = status;

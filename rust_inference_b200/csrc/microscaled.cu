@@ -94,7 +94,7 @@ __device__ __forceinline__ uint32_t block_top(uint32_t top) {
 template <typename T, int BITS, bool WHOLE, int GROUPS>
 __global__ void __launch_bounds__(THREADS) hold_kernel(const T* x, int n, int k, long long ld, int n_spans, uint32_t parts, uint32_t items, uint8_t* codes,
                                                        uint8_t* exponents) {
-    let_next_kernel_start();
+    if (BITS == 8) let_next_kernel_start();                 // (a matrix: see `settle`)
     wait_for_previous_kernels();
     const int lane = threadIdx.x & 31;
     for (uint32_t it = (blockIdx.x * THREADS + threadIdx.x) >> 5; it < items; it += gridDim.x * (THREADS / 32)) {
@@ -201,12 +201,25 @@ __device__ __forceinline__ uint32_t to_odd(double y) {
 template <typename B, int HELD, bool WHOLE>
 __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512) rmsnorm_kernel(const float* stream, const B* branch, const float* __restrict__ weight, float* total, int k, int n_spans, double eps,
                                uint8_t* codes, uint8_t* exponents) {
-    __shared__ double sums[33];
+    __shared__ double sums[32];
     let_next_kernel_start();
     const int row = blockIdx.x, tid = threadIdx.x, threads = blockDim.x, groups = n_spans * (SPAN / 8);
     const float* x = stream + (size_t)row * k;
     const B* add = branch == nullptr ? nullptr : branch + (size_t)row * k;
+    auto weights = [&](int g, float* w) {
+        const int c = g * 8;
+        if (WHOLE && c < k) {
+            const float4 a = *reinterpret_cast<const float4*>(weight + c), b = *reinterpret_cast<const float4*>(weight + c + 4);
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+            w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = !WHOLE && c + i < k ? weight[c + i] : 0.f;
+        }
+    };
     wait_for_previous_kernels();
+    float ahead[8];
+    if (HELD == 1) weights(tid, ahead);                      // on their way beside the row
     Eight<float> held[HELD];
     auto read = [&](int g, Eight<float>& v) {
         v.template load<WHOLE>(x, g * 8, k);
@@ -241,20 +254,16 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512) rmsnorm_kernel(const f
         square(v);
     }
     sum += more;
-    const int lane = tid & 31, warp = tid >> 5;
+    const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) sums[warp] = sum;
     __syncthreads();
-    if (warp == 0) {
-        double s = lane < threads / 32 ? sums[lane] : 0.0;
+    double s = lane < warps ? sums[lane] : 0.0;                   // every warp adds the warps' sums, in the same order
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) sums[32] = rsqrt(s / (double)k + eps);
-    }
-    __syncthreads();
-    const double r = sums[32];
-    auto finish = [&](int g, const Eight<float>& v) {
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const double r = rsqrt(s / (double)k + eps);
+    auto finish = [&](int g, const Eight<float>& v, const float* w) {
         const int c = g * 8;
         if (total != nullptr) {
             float* to = total + (size_t)row * k + c;
@@ -269,15 +278,6 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512) rmsnorm_kernel(const f
                     if (c + i < k) to[i] = v.v[i];
             }
         }
-        float w[8];
-        if (WHOLE && c < k) {
-            const float4 a = *reinterpret_cast<const float4*>(weight + c), b = *reinterpret_cast<const float4*>(weight + c + 4);
-            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-            w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = !WHOLE && c + i < k ? weight[c + i] : 0.f;
-        }
         Eight<float> y;
 #pragma unroll
         for (int i = 0; i < 8; ++i) y.v[i] = __uint_as_float(to_odd((double)v.v[i] * r * (double)w[i]));
@@ -289,11 +289,17 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512) rmsnorm_kernel(const f
     };
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
-        if (tid + h * threads < groups) finish(tid + h * threads, held[h]);
+        if (tid + h * threads < groups) {
+            float w[8];
+            if (HELD > 1) weights(tid + h * threads, w);
+            finish(tid + h * threads, held[h], HELD > 1 ? w : ahead);
+        }
     for (int g = tid + HELD * threads; g < groups; g += threads) {
         Eight<float> v;
+        float w[8];
         read(g, v);
-        finish(g, v);
+        weights(g, w);
+        finish(g, v, w);
     }
 }
 
@@ -330,10 +336,18 @@ int hold(const T* x, long long ld, const Held* h, cudaStream_t stream) {
     return by_size(rows, h->n_spans * SPAN, 256, [&](uint32_t p, uint32_t i) { return go(hold_kernel<T, BITS, WHOLE, 1>, p, i); },
                    [&](uint32_t p, uint32_t i) { return go(hold_kernel<T, BITS, WHOLE, 4>, p, i); });
 }
+// Products read their matrices before they wait for the kernel before them.  So the kernel that makes one lets none begin early, and a kernel that
+// nothing may overlap follows it, whose end everything behind it waits for.
+__global__ void settle_kernel() {}
+
 template <typename T>
 int hold(const T* x, long long ld, const Held* h, cudaStream_t stream) {
     const bool whole = h->k % 8 == 0 && (ld * (long long)sizeof(T)) % 16 == 0 && (uintptr_t)x % 16 == 0;
-    if (h->bits == 4) return whole ? hold<T, 4, true>(x, ld, h, stream) : hold<T, 4, false>(x, ld, h, stream);
+    if (h->bits == 4) {
+        if (int rc = whole ? hold<T, 4, true>(x, ld, h, stream) : hold<T, 4, false>(x, ld, h, stream)) return rc;
+        settle_kernel<<<1, 1, 0, stream>>>();
+        return check_launch("mx_hold");
+    }
     return whole ? hold<T, 8, true>(x, ld, h, stream) : hold<T, 8, false>(x, ld, h, stream);
 }
 
@@ -402,6 +416,12 @@ RI_API int ri_mx_hold(const void* x, int dtype, long long n, long long k, long l
     if (n != h->n || k != h->k || ld < k) return fail("mx_hold: [%lld, %lld] numbers, rows %lld apart, do not go into [%d, %d]", n, k, ld, h->n, h->k);
     if (int rc = on_device("mx_hold", h)) return rc;
     return dtype == RI_BF16 ? hold((const __nv_bfloat16*)x, ld, h, stream) : hold((const float*)x, ld, h, stream);
+}
+
+// After a matrix has been written by something else than `ri_mx_hold`: see `settle_kernel`.
+RI_API int ri_mx_settle(cudaStream_t stream) {
+    settle_kernel<<<1, 1, 0, stream>>>();
+    return check_launch("mx_settle");
 }
 
 // out [n, k]: the numbers that are held.

@@ -370,8 +370,10 @@ PyObject* py_mx_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Py_RETURN_NONE;
     });
 }
-// (plain rows or None, held rows, matrix, second matrix or 0, constants or None, act, add, out or None, held result or 0, status word)
-typedef int Mx_productFn(void*, void*, void*, const float*, long long, int, int, void*, int, long long, long long, void*, int*, void*);
+// (plain rows or None, held rows (scratch, where there are plain ones), matrix, second matrix or 0, constants or None, act, add, out or None,
+//  held result or 0, status word).  A few plain rows go to the product as they are, others by way of the scratch: 2 is its answer to those.
+typedef int Mx_productFn(void*, const void*, int, long long, long long, long long, void*, void*, const float*, long long, int, int, void*, int, long long,
+                         long long, void*, int*, void*);
 PyObject* py_mx_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const char* what = "microscaled.product";
@@ -395,10 +397,20 @@ PyObject* py_mx_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
             out_rows = o.size(0);
             out_cols = o.size(1);
         }
-        if (a[0] != Py_None) mx_hold(rows(a[0], what), held, what);
-        finish(entry<Mx_productFn>(MX_PRODUCT)(held, address<void>(number(a[2])), address<void>(number(a[3])), constants, n_constants, (int)number(a[5]),
-                                              (int)number(a[6]), out, out_code, out_rows, out_cols, address<void>(number(a[8])), address<int>(number(a[9])),
-                                              stream()), MX_PRODUCT, what);
+        const at::Tensor* x = a[0] == Py_None ? nullptr : &rows(a[0], what);
+        const int x_code = x ? code_of(*x, what) : 0;
+        auto call = [&](bool plain) {
+            return entry<Mx_productFn>(MX_PRODUCT)(held, plain ? x->data_ptr() : nullptr, x_code, plain ? x->size(0) : 0, plain ? x->size(1) : 0,
+                                                   plain ? (x->size(0) > 1 ? x->stride(0) : x->size(1)) : 0, address<void>(number(a[2])),
+                                                   address<void>(number(a[3])), constants, n_constants, (int)number(a[5]), (int)number(a[6]), out, out_code,
+                                                   out_rows, out_cols, address<void>(number(a[8])), address<int>(number(a[9])), stream());
+        };
+        int rc = call(x != nullptr);
+        if (rc == 2) {
+            mx_hold(*x, held, what);
+            rc = call(false);
+        }
+        finish(rc, MX_PRODUCT, what);
         Py_RETURN_NONE;
     });
 }

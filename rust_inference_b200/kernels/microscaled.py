@@ -21,7 +21,7 @@ import torch
 
 from . import ops
 from .build import load
-from .ops import _call, _need, _p, native
+from .ops import _call, _need, _p, _stream, native
 
 BLOCK, SPAN, PIECE = 32, 128, 512
 
@@ -102,6 +102,7 @@ class Matrix:
         wide = torch.zeros(m.exponents.shape[0] * 128, spans * 4, dtype=torch.uint8, device=codes.device)
         wide[:n, :exponents.shape[1]] = exponents
         m.exponents.copy_(wide.view(-1, 4, 32, spans, 4).permute(0, 3, 2, 1, 4).reshape(-1, spans, PIECE))
+        _call("microscaled", "ri_mx_settle", _stream())
         return m
 
     @property

@@ -334,11 +334,12 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
                 const uint8_t* we = w_exp + ((size_t)(f0 / ROWS) * n_spans + begin) * PIECE;
                 const uint8_t* we2 = DUAL ? w2_exp + ((size_t)(f0 / ROWS) * n_spans + begin) * PIECE : nullptr;
                 const uint8_t* xe = x_exp + ((size_t)(t0 / ROWS) * n_spans + begin) * PIECE;
+                const int w_row = ((f0 / ROWS) * n_spans + begin) * ROWS;        // the map's, of the tile of the first span
                 auto load_w = [&](int at, int j) {
                     const uint32_t bar = full0 + 8u * (uint32_t)at, stage = smem_base + (uint32_t)at * tile_bytes, ex = exp_base + (uint32_t)at * EXP_BYTES;
                     expect_by(leader, bar, stage_tx);
-                    load_2d_by(leader, stage, &map_w, bar, (begin + j) * SPAN, f0);
-                    if (DUAL) load_2d_by(leader, stage + TILE, &map_w2, bar, (begin + j) * SPAN, f0);
+                    load_2d_by(leader, stage, &map_w, bar, 0, w_row + j * ROWS);
+                    if (DUAL) load_2d_by(leader, stage + TILE, &map_w2, bar, 0, w_row + j * ROWS);
                     load_piece_by(leader, ex, we + (size_t)j * PIECE, bar);
                     if (DUAL) load_piece_by(leader, ex + PIECE, we2 + (size_t)j * PIECE, bar);
                 };
@@ -695,6 +696,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 tile_coords(i, f0, t0);
                 if (abort_flag) break;
                 // pieces of exponents: a row of a map each (beyond the last one: zeros)
+                const int w_row = ((f0 + w_off) / ROWS) * n_spans * ROWS;        // the map's, of this CTA's tile of the first span (beyond the last one: zeros)
                 const int xe = (t0 / ROWS + rank) * n_spans, we = (f0 / ROWS) * n_spans, we2 = DUAL ? we : we + n_spans;
                 for (int j = 0; j < n_spans; ++j, ++it) {
                     if (!ring.wait()) {
@@ -707,7 +709,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                     const uint32_t stage = smem_base + (uint32_t)ring.s * 2 * TILE, ex = exp_base + (uint32_t)ring.s * PAIR_EXP, bar = full0_first + 8u * (uint32_t)ring.s;
                     if (rank == 0) expect_by(leader, full0 + 8u * (uint32_t)ring.s, 2 * CTA_TX);                 // both CTAs' bytes
                     load_2d_pair(leader, stage, &map_x, bar, j * SPAN, t0 + rank * ROWS);
-                    load_2d_pair(leader, stage + TILE, my_w, bar, j * SPAN, f0 + w_off);
+                    load_2d_pair(leader, stage + TILE, my_w, bar, 0, w_row + j * ROWS);
                     load_2d_pair(leader, ex, &map_xe, bar, 0, xe + j);
                     load_2d_pair(leader, ex + PIECE, &map_we, bar, 0, we + j);
                     load_2d_pair(leader, ex + 2 * PIECE, second_we, bar, 0, we2 + j);
@@ -827,8 +829,9 @@ int encode_codes(CUtensorMap* map, const void* ptr, long long rows, int n_spans,
     EncodeTiledFn fn = encode_fn();
     if (!fn) return fail("gemm_microscaled: cuTensorMapEncodeTiled is not available from the driver");
     if ((uintptr_t)ptr % 32) return fail("gemm_microscaled: codes must begin on a 32-byte boundary");
-    cuuint64_t dims[2] = {(cuuint64_t)n_spans * SPAN, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)n_spans * SPAN * bits / 8};
+    // (a matrix's tiles lie one after the other: rows of a span, 128 for each of them)
+    cuuint64_t dims[2] = {(cuuint64_t)(bits == 4 ? 1 : n_spans) * SPAN, bits == 4 ? (cuuint64_t)((rows + ROWS - 1) / ROWS) * n_spans * ROWS : (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)dims[0] * bits / 8};
     cuuint32_t box[2] = {(cuuint32_t)SPAN, (cuuint32_t)box_rows};
     cuuint32_t elem[2] = {1, 1};
     CUresult r = fn(map, bits == 4 ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box,

@@ -99,25 +99,28 @@ __global__ void __launch_bounds__(THREADS) hold_kernel(const T* x, int n, int k,
     const int lane = threadIdx.x & 31;
     for (uint32_t it = (blockIdx.x * THREADS + threadIdx.x) >> 5; it < items; it += gridDim.x * (THREADS / 32)) {
         const int row = (int)(it / parts), c0 = (int)(it - (uint32_t)row * parts) * (GROUPS * 256) + lane * 8, width = n_spans * SPAN;
-        if (row >= n) {                            // of a matrix's last 128 rows those that are none
+        uint8_t* to = codes + code_at<BITS>(row, c0, n_spans);                       // (256 numbers further on: two tiles, or 256 bytes)
+        uint8_t* exp_to = exponents + exponent_at(row, c0 >> 5, n_spans);           // (two pieces)
+        if (BITS == 4 && row >= n) {               // of a matrix's last 128 rows those that are none
 #pragma unroll
-            for (int i = 0; i < GROUPS; ++i)
-                if ((lane & 3) == 0 && c0 + i * 256 < width) exponents[exponent_at(row, (c0 + i * 256) >> 5, n_spans)] = 0;
+            for (int i = 0; i < GROUPS; ++i) {
+                if (c0 + i * 256 >= width) break;
+                *reinterpret_cast<uint32_t*>(to + i * 2 * 128 * (SPAN / 2)) = 0u;
+                if ((lane & 3) == 0) exp_to[i * 2 * PIECE] = 0;
+            }
             continue;
         }
         const T* from = x + (size_t)row * ld;
         Eight<T> v[GROUPS];
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) v[i].template load<WHOLE>(from, c0 + i * 256, k);
-        uint8_t* to = codes + (size_t)row * n_spans * (SPAN * BITS / 8) + c0 * BITS / 8;
-        uint8_t* exp_to = exponents + exponent_at(row, c0 >> 5, n_spans);           // (256 numbers further on: two pieces)
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
             if (c0 + i * 256 >= width) break;
             const uint32_t byte = exponent_byte<BITS>(block_top(v[i].top()));
             float y[8];
             v[i].scaled(byte, y);
-            if (BITS == 4) *reinterpret_cast<uint32_t*>(to + i * 128) = four_bits(y);
+            if (BITS == 4) *reinterpret_cast<uint32_t*>(to + i * 2 * 128 * (SPAN / 2)) = four_bits(y);
             else *reinterpret_cast<uint2*>(to + i * 256) = make_uint2(eight_bits(y), eight_bits(y + 4));
             if ((lane & 3) == 0) exp_to[i * 2 * PIECE] = (uint8_t)byte;
         }
@@ -135,14 +138,14 @@ __global__ void __launch_bounds__(THREADS) values_kernel(const uint8_t* codes, c
     const int lane = threadIdx.x & 31;
     for (uint32_t it = (blockIdx.x * THREADS + threadIdx.x) >> 5; it < items; it += gridDim.x * (THREADS / 32)) {
         const int row = (int)(it / parts), c0 = (int)(it - (uint32_t)row * parts) * (GROUPS * 32 * N) + lane * N;
-        const volatile uint8_t* at = codes + (size_t)row * n_spans * (SPAN * BITS / 8) + c0 * BITS / 8;
+        const volatile uint8_t* at = codes + code_at<BITS>(row, c0, n_spans);
         const volatile uint8_t* exp_at = exponents + exponent_at(row, c0 >> 5, n_spans);      // (32 N numbers further on: one or two pieces)
         T* to = out + (size_t)row * k + c0;
         uint32_t w[GROUPS][2], byte[GROUPS];
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
             if (c0 + i * 32 * N >= k) break;
-            const volatile uint8_t* from = at + i * 32 * BYTES;
+            const volatile uint8_t* from = at + (BITS == 4 ? i * (N / 4) * 128 * (SPAN / 2) : i * 32 * BYTES);
             if (BYTES == 2) w[i][0] = *reinterpret_cast<const volatile uint16_t*>(from);
             else w[i][0] = *reinterpret_cast<const volatile uint32_t*>(from);
             if (BYTES == 8) w[i][1] = *reinterpret_cast<const volatile uint32_t*>(from + 4);
@@ -327,7 +330,7 @@ int by_size(int rows, int width, int of_warp, F1 one, F4 four) {
 
 template <typename T, int BITS, bool WHOLE>
 int hold(const T* x, long long ld, const Held* h, cudaStream_t stream) {
-    // (a matrix's exponents are all written, in whole pieces; those of rows behind the last one have no effect on a product but must be numbers)
+    // (a matrix is written in whole tiles: rows behind the last one have no effect on a product, and are zeros)
     const int rows = BITS == 4 ? (h->n + 127) & ~127 : h->n;
     auto go = [&](auto kernel, uint32_t parts, uint32_t items) {
         return check_launch(launch_dependent(kernel, dim3((unsigned)blocks_for(items)), dim3(THREADS), 0, stream, x, h->n, h->k, ld, h->n_spans, parts, items, h->codes,
@@ -396,7 +399,7 @@ RI_API long long ri_mx_held_bytes() { return (long long)sizeof(Held); }
 RI_API int ri_mx_make(void* at, void* codes, void* exponents, long long n, long long k, int bits, int device) {
     if ((uintptr_t)at % 64) return fail("mx_make: 64-byte aligned memory is wanted");
     if (n <= 0 || k <= 0 || k > 0x7fffffffLL - SPAN || (bits != 4 && bits != 8)) return fail("mx_make: no [%lld, %lld] numbers of %d bits", n, k, bits);
-    if ((n + 127) * spans((int)k) > 0x7fffffffLL / (SPAN / 8)) return fail("mx_make: [%lld, %lld] numbers are more than 2^31 eights", n, k);
+    if ((n + 127) / 128 * 128 * spans((int)k) > 0x7fffffffLL / (SPAN / 8)) return fail("mx_make: [%lld, %lld] numbers are more than 2^31 eights", n, k);
     if ((uintptr_t)codes % 32 || (uintptr_t)exponents % 32) return fail("mx_make: buffers must begin on a 32-byte boundary");
     Held* h = new (at) Held;
     h->codes = (uint8_t*)codes;

@@ -3,10 +3,11 @@
 // (e4m3, up to 448).  e is the smallest exponent, -127 at least, for which nothing in the block exceeds the type's largest number times 2^e.
 // A block with an infinity or a NaN among its numbers has the byte 255 and stands for 32 NaNs.
 //
-// A matrix [n, k] of such numbers is held with k rounded up to whole `SPAN`s of 128, zeros behind a row's end: codes [n, span count * 128]
-// of a byte each, or of half a byte (number 2i in the low half of byte i), and exponents in the order in which the tensor cores' scale
-// registers take them: one piece of 512 bytes for every 128 rows and span, the exponent of row r and the span's block j (0..3) at
-// (r % 32) * 16 + r % 128 / 32 * 4 + j.  Pieces lie [row / 128][span].
+// [n, k] such numbers are held with k rounded up to whole `SPAN`s of 128, zeros behind a row's end.  Rows in 8 bits: codes [n, span count * 128].
+// A matrix in 4 bits, whose n is rounded up to whole 128s too, lies as the products read it, a tile of 128 rows and a span, 8 KB, after the other,
+// [row / 128][span][128][64 bytes], number 2i in the low half of byte i (in rows as long as the matrix's, a tile would be 128 pieces of 64 bytes that
+// lie far apart: see the products' figures).  Exponents lie in the order in which the tensor cores' scale registers take them: one piece of 512
+// bytes for every 128 rows and span, [row / 128][span], the exponent of row r and the span's block j (0..3) at (r % 32) * 16 + r % 128 / 32 * 4 + j.
 #pragma once
 
 #include "common.cuh"
@@ -35,6 +36,13 @@ struct Held {
 __host__ __device__ __forceinline__ int spans(int k) { return (k + SPAN - 1) / SPAN; }
 __device__ __forceinline__ size_t exponent_at(int row, int block, int n_spans) {
     return ((size_t)(row >> 7) * n_spans + (block >> 2)) * PIECE + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+}
+
+// The byte of the code of row `row` and column c.
+template <int BITS>
+__device__ __forceinline__ size_t code_at(int row, int c, int n_spans) {
+    if (BITS == 8) return (size_t)row * n_spans * SPAN + c;
+    return (((size_t)(row >> 7) * n_spans + (c >> 7)) * 128 + (row & 127)) * (SPAN / 2) + (c & 127) / 2;
 }
 
 // The exponent byte of a block whose largest magnitude has these bits (a float's, so that a NaN's are larger than any number's).  The

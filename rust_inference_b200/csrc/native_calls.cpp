@@ -305,7 +305,7 @@ PyObject* py_mx_matrix(PyObject*, PyObject* const* a, Py_ssize_t n) {
         need(N > 0 && spans > 0, "microscaled.Matrix: a matrix of at least one number is wanted");
         code_of(x, what);
         const auto bytes = x.options().dtype(at::kByte).layout(at::kStrided).requires_grad(false);
-        const at::Tensor made[3] = {at::empty({N, spans * 64}, bytes), at::empty({(N + 127) / 128, spans, 512}, bytes),
+        const at::Tensor made[3] = {at::empty({(N + 127) / 128, spans, 128, 64}, bytes), at::empty({(N + 127) / 128, spans, 512}, bytes),
                                     at::empty({number(a[2])}, bytes.device(at::kCPU))};
         if (address<MxMakeFn>(number(a[1]))(made[2].data_ptr(), made[0].data_ptr(), made[1].data_ptr(), N, x.size(1), 4, x.get_device()) != 0)
             refuse(std::string(what) + ": " + bound[MX_HOLD].last_error());

@@ -81,8 +81,8 @@ class Matrix:
     @classmethod
     def _empty(cls, n, k, device) -> "Matrix":
         spans = _spans(k)
-        # exponents of rows behind the last one, in its piece of 128, are read beside it and have no effect: zeros, so that they are numbers
-        return cls(n, k, torch.empty(n, spans * SPAN // 2, dtype=torch.uint8, device=device),
+        # rows behind the last one, in its tile of 128, are read beside it and have no effect
+        return cls(n, k, torch.zeros(-(-n // 128), spans, 128, SPAN // 2, dtype=torch.uint8, device=device),
                    torch.zeros(-(-n // 128), spans, PIECE, dtype=torch.uint8, device=device))
 
     @classmethod
@@ -94,12 +94,13 @@ class Matrix:
               and tuple(exponents.shape) == (n, -(-k // BLOCK)), "microscaled.Matrix: codes uint8 [n, ceil(k / 2)] and exponents uint8 [n, ceil(k / 32)] are wanted")
         ops._need_cuda(codes, exponents)
         m = cls._empty(n, k, codes.device)
-        m.codes.zero_()
-        m.codes[:, :codes.shape[1]] = codes
+        spans, tiles = m.spans, m.exponents.shape[0]
+        wide = torch.zeros(tiles * 128, spans * 64, dtype=torch.uint8, device=codes.device)
+        wide[:n, :codes.shape[1]] = codes
         if k % 2:
-            m.codes[:, k // 2] &= 15
-        spans = m.spans
-        wide = torch.zeros(m.exponents.shape[0] * 128, spans * 4, dtype=torch.uint8, device=codes.device)
+            wide[:, k // 2] &= 15
+        m.codes.copy_(wide.view(tiles, 128, spans, 64).transpose(1, 2))
+        wide = torch.zeros(tiles * 128, spans * 4, dtype=torch.uint8, device=codes.device)
         wide[:n, :exponents.shape[1]] = exponents
         m.exponents.copy_(wide.view(-1, 4, 32, spans, 4).permute(0, 3, 2, 1, 4).reshape(-1, spans, PIECE))
         _call("microscaled", "ri_mx_settle", _stream())

@@ -197,18 +197,18 @@ __device__ __forceinline__ uint32_t to_odd(double y) {
     return fine | (hi & 0x80000000u);
 }
 
-// A block of threads per row.  Sum of squares, root and factors are in 64 bits, up to the rounding to 8: what lies next to the middle of two numbers
-// falls as the formula says, not as a sum's last bits do.  That costs two conversions and three operations in 64 bits a number, beside the
-// memory's time (2,047 rows of 4,096 with a branch: see below).  HELD: so many groups of eight per thread stay in registers between the two
+// A block of threads per row.  Results are what the formula in 64 bits, rounded once, gives: what lies next to the middle of two numbers falls as the
+// formula says, not as a sum's last bits do.  The sum of squares and its root are in 64 bits; factors too, but only where 32 leave it open.  HELD: so many groups of eight per thread stay in registers between the two
 // passes; longer rows are read again.
 template <typename B, int HELD, bool WHOLE>
-__global__ void __launch_bounds__(HELD == 1 ? 1024 : 512) rmsnorm_kernel(const float* stream, const B* branch, const float* __restrict__ weight, float* total, int k, int n_spans, double eps,
-                               uint8_t* codes, uint8_t* exponents) {
+__global__ void __launch_bounds__(HELD == 1 ? 1024 : 512, HELD == 1 ? 1 : 2) rmsnorm_kernel(const float* stream, const B* branch, const float* __restrict__ weight, float* total, int k,
+                                                                                            int n_spans, double inverse, double eps, uint8_t* codes,
+                                                                                            uint8_t* exponents) {
     __shared__ double sums[32];
+    constexpr uint32_t NEAR = 4;
     let_next_kernel_start();
-    const int row = blockIdx.x, tid = threadIdx.x, threads = blockDim.x, groups = n_spans * (SPAN / 8);
-    const float* x = stream + (size_t)row * k;
-    const B* add = branch == nullptr ? nullptr : branch + (size_t)row * k;
+    const int tid = threadIdx.x, threads = blockDim.x, groups = n_spans * (SPAN / 8);
+    const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
     auto weights = [&](int g, float* w) {
         const int c = g * 8;
         if (WHOLE && c < k) {
@@ -220,21 +220,22 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512) rmsnorm_kernel(const f
             for (int i = 0; i < 8; ++i) w[i] = !WHOLE && c + i < k ? weight[c + i] : 0.f;
         }
     };
-    wait_for_previous_kernels();
-    float ahead[8];
-    if (HELD == 1) weights(tid, ahead);                      // on their way beside the row
-    Eight<float> held[HELD];
-    auto read = [&](int g, Eight<float>& v) {
-        v.template load<WHOLE>(x, g * 8, k);
-        if (add != nullptr) {
-            Eight<B> b;
-            b.template load<WHOLE>(add, g * 8, k);
-            if constexpr (sizeof(B) == 2) {
-                b.add_to(v.v);
-            } else {
+    auto join = [&](Eight<float>& v, const Eight<B>& b) {
+        if constexpr (sizeof(B) == 2) {
+            b.add_to(v.v);
+        } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v.v[i] += b.v[i];
-            }
+            for (int i = 0; i < 8; ++i) v.v[i] += b.v[i];
+        }
+    };
+    wait_for_previous_kernels();
+    const int row = blockIdx.x;
+    auto read = [&](int g, Eight<float>& v) {
+        v.template load<WHOLE>(stream + (size_t)row * k, g * 8, k);
+        if (branch != nullptr) {
+            Eight<B> b;
+            b.template load<WHOLE>(branch + (size_t)row * k, g * 8, k);
+            join(v, b);
         }
     };
     double sum = 0.0, more = 0.0;
@@ -245,19 +246,23 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512) rmsnorm_kernel(const f
             more = fma((double)v.v[i + 1], (double)v.v[i + 1], more);
         }
     };
+    Eight<float> held[HELD];
+    float w[HELD][8];
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
         if (tid + h * threads < groups) read(tid + h * threads, held[h]);
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
-        if (tid + h * threads < groups) square(held[h]);
+        if (tid + h * threads < groups) {
+            weights(tid + h * threads, w[h]);
+            square(held[h]);
+        }
     for (int g = tid + HELD * threads; g < groups; g += threads) {
         Eight<float> v;
         read(g, v);
         square(v);
     }
     sum += more;
-    const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) sums[warp] = sum;
@@ -265,8 +270,9 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512) rmsnorm_kernel(const f
     double s = lane < warps ? sums[lane] : 0.0;                   // every warp adds the warps' sums, in the same order
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const double r = rsqrt(s / (double)k + eps);
-    auto finish = [&](int g, const Eight<float>& v, const float* w) {
+    const double r = rsqrt(s * inverse + eps);
+    const float r32 = (float)r;
+    auto finish = [&](int g, const Eight<float>& v, const float* by) {
         const int c = g * 8;
         if (total != nullptr) {
             float* to = total + (size_t)row * k + c;
@@ -282,27 +288,46 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512) rmsnorm_kernel(const f
             }
         }
         Eight<float> y;
+        auto exact = [&] {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y.v[i] = __uint_as_float(to_odd((double)v.v[i] * r * (double)w[i]));
-        const uint32_t byte = exponent_byte<8>(block_top(y.top()));
+            for (int i = 0; i < 8; ++i) y.v[i] = __uint_as_float(to_odd((double)v.v[i] * r * (double)by[i]));
+        };
+        // In 32 bits first, which is off by three units in the last place at most: that decides, but next to where the exponent or a code changes
+        // (one block in 10^5, and one eight in 700, most of these for numbers below the type's 2^-6).
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y.v[i] = v.v[i] * r32 * by[i];
+        uint32_t top = block_top(y.top()), byte = exponent_byte<8>(top);
         float z[8];
-        y.scaled(byte, z);
+        if (top != 0u && ((top & 0x7fffffu) - (0x600000u - NEAR) <= 2u * NEAR || (top >> 23) - 16u > 222u)) {  // (the same for a block's four threads)
+            exact();
+            byte = exponent_byte<8>(block_top(y.top()));
+            y.scaled(byte, z);
+        } else {
+            y.scaled(byte, z);
+            uint32_t apart = 0xffffffffu;                 // from the middle of two codes, in units in the last place, plus NEAR
+            float least = 1.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                apart = min(apart, (__float_as_uint(z[i]) + 0x80000u + NEAR) & 0xfffffu);
+                least = fminf(least, fabsf(z[i]));
+            }
+            if (apart <= 2u * NEAR || least < 0x1p-6f) {
+                exact();
+                y.scaled(byte, z);
+            }
+        }
         *reinterpret_cast<uint2*>(codes + (size_t)row * n_spans * SPAN + c) = make_uint2(eight_bits(z), eight_bits(z + 4));
         if ((c & 31) == 0) exponents[exponent_at(row, c >> 5, n_spans)] = (uint8_t)byte;
     };
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
-        if (tid + h * threads < groups) {
-            float w[8];
-            if (HELD > 1) weights(tid + h * threads, w);
-            finish(tid + h * threads, held[h], HELD > 1 ? w : ahead);
-        }
+        if (tid + h * threads < groups) finish(tid + h * threads, held[h], w[h]);
     for (int g = tid + HELD * threads; g < groups; g += threads) {
         Eight<float> v;
-        float w[8];
+        float by[8];
         read(g, v);
-        weights(g, w);
-        finish(g, v, w);
+        weights(g, by);
+        finish(g, v, by);
     }
 }
 
@@ -377,13 +402,14 @@ int norm(const float* x, const B* branch, const float* weight, float* total, con
     int threads = ((groups + HELD - 1) / HELD + 31) / 32 * 32;
     if (threads > most) threads = most;
     auto go = [&](auto kernel) {
-        return check_launch(launch_dependent(kernel, dim3((unsigned)h->n), dim3(threads), 0, stream, x, branch, weight, total, h->k, h->n_spans, eps, h->codes, h->exponents),
-                            "mx_rmsnorm");
+        return check_launch(launch_dependent(kernel, dim3((unsigned)h->n), dim3(threads), 0, stream, x, branch, weight, total, h->k, h->n_spans, 1.0 / h->k, eps, h->codes,
+                                             h->exponents), "mx_rmsnorm");
     };
     return whole ? go(rmsnorm_kernel<B, HELD, true>) : go(rmsnorm_kernel<B, HELD, false>);
 }
-// Few rows are as fast as one of them, which many threads with one group each have sooner (8 rows of 3,584: one group 3.3 us, two 4.2; 148 of
-// 4,096 3.8 / 4.9); many are as fast as the SMs' instructions, of which two groups a thread take fewer (2,047 of 4,096: 26.2 / 23.9).
+// Few rows are as fast as one of them, which many threads with one group each have sooner (8 rows of 3,584: one group 2.9 us, two 3.2; 148 of
+// 4,096 3.3 / 3.7); many are as fast as the SMs' instructions, of which two groups a thread take fewer (2,047 of 4,096: 25.8 / 22.7, with a branch
+// 4.1 TB/s).
 template <typename B>
 int norm(const float* x, const void* branch, const float* weight, float* total, const Held* h, double eps, cudaStream_t stream) {
     return h->n <= 2 * sm_count() ? norm<B, 1>(x, (const B*)branch, weight, total, h, eps, 1024, stream)

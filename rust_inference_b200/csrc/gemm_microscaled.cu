@@ -770,7 +770,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         const uint32_t next_first = in_first_cta(smem_u32(&next_bar));
         wait_for_previous_kernels();
         const Epilogue e = load_epilogue<DUAL>(constants, act);
-        const bool aligned = OUT == OUT_BF16 ? n_feat % 8 == 0 : n_feat % 4 == 0;
+        const bool aligned = (OUT == OUT_BF16 ? n_feat % 8 == 0 : n_feat % 4 == 0) && (reinterpret_cast<uintptr_t>(res.out) & 15) == 0;
         for (int i = 0; i < my_tiles; ++i) {
             int f0, t0;
             tile_coords(i, f0, t0);
@@ -917,9 +917,10 @@ Plan plan(int n_tok, int n_feat, int n_spans, bool dual) {
         const double meet = 320 + 2.2 * p.tn + (double)n_feat * n_spans * (SPAN / 2) / 6e4;
         double best = rounds * (span * n_spans + 100) + 90 + 1.85 * p.tn;
         for (int c = 2; c <= CLUSTER_MOST && c <= n_spans; ++c) {
-            // Clusters of whole SMs lie within groups of SMs, and those of the next kernel come in while these leave: large ones find their place
-            // late where they are many (16 clusters of 7: 12.2 us, of 4: 7.1).
-            if (tiles * c > (c > 4 ? sms * 2 / 3 : blocks_alone((const void*)mx_feature_kernel<false, OUT_F32>, THREADS, SMEM_LIMIT, c))) continue;
+            // Clusters of whole SMs lie within groups of SMs, which leaves some over, and those of the next kernel come in while these leave: where
+            // there are many, the last find their place late (36 clusters of 4, 9.9 us instead of 6.1), large ones sooner (16 of 7, 12.2 instead
+            // of 7.1).
+            if (tiles * c > (c > 4 ? sms * 2 / 3 : sms - 20)) continue;
             const double cost = span * ((n_spans + c - 1) / c) + meet;
             if (cost < best) {
                 best = cost;

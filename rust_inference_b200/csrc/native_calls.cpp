@@ -290,6 +290,20 @@ const at::Tensor& dense(PyObject* o, const char* what) {
     if (!here(t) || t.dim() != 2 || !t.is_contiguous()) refuse(std::string(what) + ": a contiguous [n, k] on the current device is wanted");
     return t;
 }
+// Whether two tensors' numbers lie in the same memory, in part at least.
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+    auto ends = [](const at::Tensor& t, uintptr_t& from, uintptr_t& to) {
+        long long last = 0;
+        for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+        from = reinterpret_cast<uintptr_t>(t.data_ptr());
+        to = from + static_cast<uintptr_t>(last + 1) * t.element_size();
+    };
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    uintptr_t a0, a1, b0, b1;
+    ends(a, a0, a1);
+    ends(b, b0, b1);
+    return a0 < b1 && b0 < a1;
+}
 typedef int Mx_holdFn(const void*, int, long long, long long, long long, void*, void*);
 void mx_hold(const at::Tensor& x, void* held, const char* what) {
     finish(entry<Mx_holdFn>(MX_HOLD)(x.data_ptr(), code_of(x, what), x.size(0), x.size(1), x.size(0) > 1 ? x.stride(0) : x.size(1), held, stream()), MX_HOLD, what);
@@ -363,6 +377,13 @@ PyObject* py_mx_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (a[3] != Py_None) {
             const at::Tensor& t = dense(a[3], what);
             need(t.scalar_type() == at::kFloat && t.sizes() == x.sizes(), "microscaled.rmsnorm: total must be float32, as x");
+            for (PyObject* o : {a[0], a[1]}) {
+                if (o == Py_None) continue;
+                const at::Tensor& other = tensor(o, what);
+                need(!overlap(t, other) || (t.data_ptr() == other.data_ptr() && t.scalar_type() == other.scalar_type()),
+                     "microscaled.rmsnorm: total is x or the branch itself, or lies apart from them");
+            }
+            need(!overlap(t, weight), "microscaled.rmsnorm: total lies apart from the weight");
             total = t.data_ptr<float>();
         }
         finish(entry<Mx_rmsnormFn>(MX_NORM)(x.data_ptr<float>(), branch, branch_code, weight.data_ptr<float>(), total, x.size(0), x.size(1), real(a[4]),
@@ -399,6 +420,7 @@ PyObject* py_mx_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }
         const at::Tensor* x = a[0] == Py_None ? nullptr : &rows(a[0], what);
         const int x_code = x ? code_of(*x, what) : 0;
+        if (x && out) need(!overlap(*x, tensor(a[7], what)), "microscaled.product: the result lies apart from the rows");
         auto call = [&](bool plain) {
             return entry<Mx_productFn>(MX_PRODUCT)(held, plain ? x->data_ptr() : nullptr, x_code, plain ? x->size(0) : 0, plain ? x->size(1) : 0,
                                                    plain ? (x->size(0) > 1 ? x->stride(0) : x->size(1)) : 0, address<void>(number(a[2])),

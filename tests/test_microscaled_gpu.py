@@ -238,3 +238,204 @@ def test_activated(m):
     got = microscaled.values(rows).double()
     assert float((got != plain.nearest(want.cpu(), plain.EIGHT).to(DEV)).double().mean()) < 0.01
     check_status()
+
+
+@pytest.mark.parametrize("m", [3, 130, 600])
+def test_numbers_that_are_none_stay_where_they_are(m):
+    """A NaN or an infinity makes its token's results, or its feature's, NaN, and no others."""
+    from rust_inference_b200.kernels import linear, microscaled
+    ctx = context(torch.float32)
+    x, w = spread(m, 300, 1, wide=0.5), spread(260, 300, 2, wide=0.5)
+    x[1, 7], x[2, 299], w[5, 0], w[259, 100] = math.nan, math.inf, -math.inf, math.nan
+    out = torch.zeros(m, 260, dtype=torch.float32, device=DEV)
+    linear.project(x.to(DEV), microscaled.Matrix.of(w.to(DEV)), out, ctx)
+    bad = torch.zeros(m, 260, dtype=torch.bool)
+    bad[1:3] = True
+    bad[:, [5, 259]] = True
+    assert torch.equal(torch.isnan(out).cpu(), bad) and torch.isfinite(out.cpu()[~bad]).all()
+    y, mass = exact_product(x.nan_to_num(0, 0, 0), w.nan_to_num(0, 0, 0))
+    good = ~bad.to(DEV)
+    assert ((out.double() - y).abs() <= bound(300, mass, y, torch.float32))[good].all()
+    rows = microscaled.Rows(m, 260)
+    linear.gated(x.to(DEV), microscaled.Matrix.of(w.to(DEV)), microscaled.Matrix.of(w.to(DEV)), rows, ctx)
+    got = microscaled.values(rows).cpu()
+    blocks = torch.zeros(m, 260, dtype=torch.bool)
+    blocks[1:3] = True
+    blocks[:, 0:32] = True
+    blocks[:, 256:260] = True
+    assert torch.equal(torch.isnan(got), blocks)
+    check_status()
+
+
+@pytest.mark.parametrize("up", [-120, -60, 0, 60, 110])
+def test_far_powers_of_two(up):
+    """Powers of two far apart cancel in the product, also where each alone is near float32's ends."""
+    from rust_inference_b200.kernels import linear, microscaled
+    ctx = context(torch.float32)
+    x, w = spread(5, 256, 3, wide=0.5), spread(130, 256, 4, wide=0.5)
+    out = torch.empty(5, 130, dtype=torch.float32, device=DEV)
+    linear.project((x * 2.0 ** up).to(DEV), microscaled.Matrix.of((w * 2.0 ** -up).to(DEV)), out, ctx)
+    y, mass = exact_product(x * 2.0 ** up, w * 2.0 ** -up)
+    assert ((out.double() - y).abs() <= bound(256, mass, y, torch.float32)).all()
+
+
+def test_results_off_a_boundary_and_in_wider_memory():
+    """Results that begin off a 16-byte boundary; what lies before and behind them stays."""
+    from rust_inference_b200.kernels import linear, microscaled
+    for m in (2, 40, 300, 1000):
+        x, w = spread(m, 256, 5, wide=0.5), spread(256, 256, 6, wide=0.5)
+        y, mass = exact_product(x, w)
+        held, xd = microscaled.Matrix.of(w.to(DEV)), x.to(DEV)
+        for dtype in (torch.bfloat16, torch.float32):
+            ctx = context(dtype)
+            room = torch.full((m * 256 + 9,), 7.0, dtype=dtype, device=DEV)
+            out = room[1:1 + m * 256].view(m, 256)
+            linear.project(xd, held, out, ctx)
+            assert ((out.double() - y).abs() <= bound(256, mass, y, dtype)).all()
+            if dtype is torch.float32:
+                linear.into_residual(xd, held, out, ctx)
+                assert ((out.double() - 2 * y).abs() <= bound(256, 2 * mass, 2 * y, dtype)).all()
+            assert float(room[0]) == 7.0 and (room[1 + m * 256:] == 7.0).all()
+    # plain rows off a boundary, and rows apart
+    w = spread(70, 64, 8, wide=0.5)
+    held = microscaled.Matrix.of(w.to(DEV))
+    wide = spread(3, 200, 9, wide=0.5).to(DEV)
+    for x in (wide[:, :64], wide[:, 3:67], wide[:, 8:72], wide[:1, 1:65], wide[::2, :64]):
+        out = torch.empty(x.shape[0], 70, dtype=torch.float32, device=DEV)
+        linear.project(x, held, out, context(torch.float32))
+        y, mass = exact_product(x.cpu(), w)
+        assert ((out.double() - y).abs() <= bound(64, mass, y, torch.float32)).all()
+    check_status()
+
+
+def test_no_tokens():
+    from rust_inference_b200.kernels import linear, microscaled
+    held = microscaled.Matrix.of(torch.ones(5, 40, device=DEV))
+    out = torch.empty(0, 5, dtype=torch.bfloat16, device=DEV)
+    assert linear.project(torch.empty(0, 40, dtype=torch.bfloat16, device=DEV), held, out, context()) is out
+
+
+@pytest.mark.parametrize("m", [1, 8, 40, 200, 700])
+def test_a_run_of_them_captured_and_again(m):
+    """What a decoder's feed-forward does with them, the stream on its way through: against 64 bits, the same bits every time, captured, replayed over
+    other inputs, and on another stream."""
+    from rust_inference_b200.kernels import linear, microscaled
+    ctx = context()
+    k, inner = 640, 1100
+    weight = (1 + 0.1 * torch.randn(k, generator=gen(1))).to(DEV)
+    wg, wu, wd = spread(inner, k, 2, wide=0.3) / 12, spread(inner, k, 3, wide=0.3) / 12, spread(k, inner, 4, wide=0.3) / 16
+    g, u, d = (microscaled.Matrix.of(w.to(DEV)) for w in (wg, wu, wd))
+    normed, act = microscaled.Rows(m, k), microscaled.Rows(m, inner)
+    stream, branch = torch.empty(m, k, device=DEV), torch.empty(m, k, dtype=torch.bfloat16, device=DEV)
+    total = torch.empty(m, k, device=DEV)
+
+    def step():
+        microscaled.rmsnorm(stream, weight, 1e-6, normed, branch=branch, total=total)
+        linear.gated(normed, g, u, act, ctx)
+        linear.into_residual(act, d, total, ctx)
+
+    def fill(seed):
+        stream.copy_(2 * torch.randn(m, k, generator=gen(seed)))
+        branch.copy_(torch.randn(m, k, generator=gen(seed + 1)))
+
+    def want():
+        t, y = plain.rmsnorm(stream, branch, weight, 1e-6)
+        h = plain.nearest(y, plain.EIGHT)
+        w4 = [plain.nearest(w, plain.FOUR) for w in (wg, wu, wd)]
+        a = plain.gate(h @ w4[0].t(), h @ w4[1].t())
+        a8 = plain.nearest(a, plain.EIGHT)
+        off = (a - a8).abs() @ w4[2].abs().t()
+        return t.double() + a8 @ w4[2].t(), off
+
+    fill(10)
+    step()
+    first = total.clone()
+    y, off = want()
+    # a number of the gate's next to the middle of two falls to the other side now and then: a step instead of none, one of a thousand at most
+    assert ((first.double().cpu() - y).abs() <= 0.25 * off + 1e-4 * y.abs() + 1e-5).all()
+    for _ in range(3):
+        step()
+        assert torch.equal(total, first)
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(other):
+        step()
+    torch.cuda.current_stream().wait_stream(other)
+    assert torch.equal(total, first)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step()
+    for seed in (20, 10, 30):
+        fill(seed)
+        graph.replay()
+        replayed = total.clone()
+        step()
+        assert torch.equal(replayed, total)
+        if seed == 10:
+            assert torch.equal(replayed, first)
+    check_status()
+
+
+def test_a_matrix_is_read_right_behind_its_making():
+    """Products begin their reads of a matrix before the kernel before them has ended: not before the matrix is there."""
+    from rust_inference_b200.kernels import linear, microscaled
+    ctx = context()
+    x = microscaled.quantize(spread(2, 4096, 1, wide=0.5).to(DEV))
+    ws = [spread(4096, 4096, 40 + i, torch.bfloat16, wide=0.5).to(DEV) for i in range(2)]
+    want = []
+    for w in ws:
+        m = microscaled.Matrix.of(w)
+        torch.cuda.synchronize()
+        want.append(linear.project(x, m, torch.empty(2, 4096, dtype=torch.float32, device=DEV), ctx))
+    for turn in range(20):
+        m = microscaled.Matrix.of(ws[turn % 2])                    # (in the memory of the one before)
+        out = linear.project(x, m, torch.empty(2, 4096, dtype=torch.float32, device=DEV), ctx)
+        assert torch.equal(out, want[turn % 2])
+        del m
+
+
+def test_refusals():
+    from rust_inference_b200.kernels import linear, microscaled, ops
+    KE = ops.KernelError
+    ctx = context()
+    w = microscaled.Matrix.of(torch.ones(40, 64, device=DEV))
+    x = torch.ones(3, 64, dtype=torch.bfloat16, device=DEV)
+    out = torch.empty(3, 40, dtype=torch.bfloat16, device=DEV)
+    f32 = torch.empty(3, 40, device=DEV)
+    rows = microscaled.quantize(x)
+    bad = [
+        lambda: linear.project(x[:, :63], w, out, ctx), lambda: linear.project(x, w, out[:2], ctx), lambda: linear.project(x, w, out.t(), ctx),
+        lambda: linear.project(x.half(), w, out, ctx), lambda: linear.project(x, w, out.half(), ctx), lambda: linear.project(x.cpu(), w, out, ctx),
+        lambda: linear.project(x, w, out, ctx, bias=torch.ones(39, device=DEV)), lambda: linear.project(x, w, out, ctx, bias=torch.ones(40, device=DEV).half()),
+        lambda: linear.into_residual(x, w, out, ctx), lambda: linear.into_residual(x, w, microscaled.Rows(3, 40), ctx),
+        lambda: linear.gated(x, w, microscaled.Matrix.of(torch.ones(41, 64, device=DEV)), out, ctx),
+        lambda: linear.gated(x, w, torch.ones(40, 64, device=DEV), out, ctx), lambda: linear.logits(x, w, f32, ctx, silu_cols=torch.ones(1, device=DEV)),
+        lambda: linear.project(rows, microscaled.Matrix.of(torch.ones(64, 64, device=DEV)), rows, ctx),
+        lambda: linear.project(rows, w, microscaled.Rows(3, 41), ctx), lambda: microscaled.quantize(x, microscaled.Rows(4, 64)),
+        lambda: microscaled.product(x, w, out, ctx, bias=torch.ones(40, device=DEV), add=True), lambda: microscaled.product(x, w, out, ctx, form=torch.ones(5, device=DEV)),
+        lambda: microscaled.Matrix.of(torch.ones(0, 4, device=DEV)), lambda: microscaled.Matrix.of(torch.ones(4, device=DEV)),
+        lambda: microscaled.Matrix.of(torch.ones(4, 4, dtype=torch.float16, device=DEV)), lambda: microscaled.Rows(0, 4), lambda: microscaled.Rows(4, 0),
+        lambda: microscaled.Rows(4, 64, codes=torch.zeros(4, dtype=torch.uint8, device=DEV)),
+        lambda: microscaled.Rows(1, 64, codes=torch.zeros(129, dtype=torch.uint8, device=DEV)[1:]),
+        lambda: microscaled.rmsnorm(x, torch.ones(64, device=DEV), 1e-5, rows), lambda: microscaled.rmsnorm(x.float(), torch.ones(63, device=DEV), 1e-5, rows),
+        lambda: microscaled.rmsnorm(x.float(), torch.ones(64, device=DEV), 1e-5, microscaled.Rows(2, 64)),
+        lambda: microscaled.rmsnorm(x.float(), torch.ones(64, device=DEV), 1e-5, rows, branch=x[:2]),
+        lambda: microscaled.rmsnorm(x.float(), torch.ones(64, device=DEV), 1e-5, rows, total=torch.empty(3, 64, dtype=torch.bfloat16, device=DEV)),
+        lambda: microscaled.values(rows, torch.float16), lambda: microscaled.values(w, torch.float32, out=torch.empty(64, 40, device=DEV)),
+        lambda: microscaled.Matrix.of_codes(torch.zeros(4, 5, dtype=torch.uint8, device=DEV), torch.zeros(4, 1, dtype=torch.uint8, device=DEV), 12),
+        lambda: microscaled.Matrix.of_codes(torch.zeros(4, 6, dtype=torch.uint8, device=DEV), torch.zeros(4, 2, dtype=torch.uint8, device=DEV), 12),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(KE):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    # memory that a call reads and writes at different places
+    room = torch.zeros(4 * 64 + 64, device=DEV)
+    stream = room[:3 * 64].view(3, 64)
+    with pytest.raises(KE, match="apart"):
+        microscaled.rmsnorm(stream, torch.ones(64, device=DEV), 1e-5, rows, total=room[64:4 * 64].view(3, 64))
+    square = microscaled.Matrix.of(torch.ones(64, 64, device=DEV))
+    with pytest.raises(KE, match="apart"):
+        linear.project(x, square, x, ctx)
+    check_status()

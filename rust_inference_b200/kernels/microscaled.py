@@ -93,6 +93,7 @@ class Matrix:
         _need(codes.dtype == torch.uint8 and exponents.dtype == torch.uint8 and n > 0 and k > 0 and tuple(codes.shape) == (n, -(-k // 2))
               and tuple(exponents.shape) == (n, -(-k // BLOCK)), "microscaled.Matrix: codes uint8 [n, ceil(k / 2)] and exponents uint8 [n, ceil(k / 32)] are wanted")
         ops._need_cuda(codes, exponents)
+        _need(codes.device.index == torch.cuda.current_device() and exponents.device == codes.device, "microscaled.Matrix: codes and exponents lie on the current device")
         m = cls._empty(n, k, codes.device)
         spans, tiles = m.spans, m.exponents.shape[0]
         wide = torch.zeros(tiles * 128, spans * 64, dtype=torch.uint8, device=codes.device)

@@ -439,3 +439,32 @@ def test_refusals():
     with pytest.raises(KE, match="apart"):
         linear.project(x, square, x, ctx)
     check_status()
+
+
+def test_a_files_codes_on_another_device_than_the_current_one(monkeypatch):
+    from rust_inference_b200.kernels import microscaled, ops
+    codes, exponents = torch.zeros(4, 6, dtype=torch.uint8, device=DEV), torch.zeros(4, 1, dtype=torch.uint8, device=DEV)
+    microscaled.Matrix.of_codes(codes, exponents, 12)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    with pytest.raises(ops.KernelError, match="current device"):
+        microscaled.Matrix.of_codes(codes, exponents, 12)
+
+
+@pytest.mark.parametrize("n,k", [(896, 896), (2048, 2048), (3584, 3584), (1152, 904), (200, 8)])
+def test_a_few_plain_rows_are_what_rows_in_eight_bits_are(n, k):
+    """However a product comes by its rows, its results are the same to the bit."""
+    from rust_inference_b200.kernels import linear, microscaled
+    ctx = context()
+    held = microscaled.Matrix.of(spread(n, k, n + k, wide=1.0).to(DEV))
+    for m in range(1, 10):
+        for dtype in (torch.bfloat16, torch.float32):
+            x = spread(m, k + 8, 3 * m + k, dtype, 2.0).to(DEV)[:, :k]
+            out, again = (torch.full((m, n), math.nan, device=DEV) for _ in range(2))
+            linear.logits(x, held, out, ctx)
+            linear.logits(microscaled.quantize(x), held, again, ctx)
+            assert torch.equal(out, again)
+            rows, from_rows = microscaled.Rows(m, n), microscaled.Rows(m, n)
+            linear.gated(x, held, held, rows, ctx)
+            linear.gated(microscaled.quantize(x), held, held, from_rows, ctx)
+            assert torch.equal(microscaled.values(rows), microscaled.values(from_rows))
+    check_status()

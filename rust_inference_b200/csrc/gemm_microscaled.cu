@@ -154,6 +154,18 @@ __device__ __forceinline__ float result(float a, float u, float bias, const Epil
     return a + bias;
 }
 
+// So many of a warp's 32 rows of accumulators from one column on.
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t* r) {
+    if (N == 4)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr) : "memory");
+    else if (N == 8)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+    else
+        tmem_ld16(taddr, r);
+}
+
 // What a product writes: plain numbers [tokens, features], or rows in 8 bits with `spans` spans and their exponents.
 struct Result {
     void* out;
@@ -190,10 +202,11 @@ __device__ __forceinline__ void store_lanes(const Result& r, T t, G good, int f,
     }
 }
 
-// Plain rows that a kernel for few tokens brings to 8 bits itself: up to PLAIN_MOST of them, whose spans all have a stage of the ring.  The epilogue's
-// warps, which have nothing else to do then, read them and write codes and exponents as TMA would have brought them.  (A product of [3584, 3584], us,
-// rows that are in 8 bits, plain ones, plain ones by a kernel before: 1 token 5.2 / 5.3 / 6.4, 4 tokens 5.4 / 5.7 / 5.9, 8 tokens 5.5 / 6.2 / 5.9.)
-constexpr int PLAIN_MOST = 4;
+// Plain rows that a kernel for few tokens brings to 8 bits itself: those whose spans all have a stage of the ring, up to 4 of them, and up to
+// PLAIN_MOST where K is not cut or a CTA has no more than 32 spans of all rows together.  The epilogue's warps, which have nothing else to do then, read
+// them and write codes and exponents as TMA would have brought them.  (us, plain rows / by a kernel before: [3584, 3584], 7 spans a CTA, 1 token
+// 5.1 / 6.4, 4 tokens 5.5 / 5.9, 8 tokens 6.0 / 5.75; [2048, 2048], 4 spans, 8 tokens 4.5 / 4.95; [896, 896], uncut, 8 tokens 4.05 / 4.2.)
+constexpr int PLAIN_MOST = 8;
 struct PlainRows {
     const void* at;              // null: rows in 8 bits come by TMA
     int f32, k;
@@ -206,11 +219,12 @@ template <typename T>
 __device__ __forceinline__ void write_plain(const PlainRows& x, int n_tok, int begin, int count, uint32_t tiles, uint32_t tile_bytes, uint32_t pieces,
                                             uint32_t piece_bytes, int thread) {
     const int items = count * n_tok * 16, chunk = thread & 15;
+    const uint32_t of_row = 0xffffu / (uint32_t)n_tok + 1;          // (exact: numbers below 2^10 by at most 16)
     for (int i0 = thread; i0 < items + 15; i0 += 4 * 256) {           // (whole quads go round together: items is a multiple of 16)
         float v[4][8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int q = (i0 + i * 256) >> 4, span = q / n_tok, row = q - span * n_tok, c = (begin + span) * SPAN + chunk * 8;
+            const int q = (i0 + i * 256) >> 4, span = (int)((uint32_t)q * of_row >> 16), row = q - span * n_tok, c = (begin + span) * SPAN + chunk * 8;
             const bool there = span < count && c < x.k;
             if (sizeof(T) == 2) {
                 uint4 w = make_uint4(0u, 0u, 0u, 0u);
@@ -232,7 +246,7 @@ __device__ __forceinline__ void write_plain(const PlainRows& x, int n_tok, int b
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int q = (i0 + i * 256) >> 4, span = q / n_tok, row = q - span * n_tok;
+            const int q = (i0 + i * 256) >> 4, span = (int)((uint32_t)q * of_row >> 16), row = q - span * n_tok;
             if (span >= count) break;
             uint32_t top = 0;
 #pragma unroll
@@ -254,9 +268,9 @@ __device__ __forceinline__ void write_plain(const PlainRows& x, int n_tok, int b
 
 // ---------------------------------------------------------------------------------------------
 // Few tokens.  Tiles of 128 features x tn tokens, for a persistent grid of CTAs, or (not gated) each for a cluster whose CTAs share its K.  Warp 0 issues the copies, warp 1 allocates tensor memory and issues the MMAs,
-// warps 2-9 run the epilogue, two for each quarter of tensor memory's lanes, which take turns at 16 tokens.
+// warps 2-9 run the epilogue, two for each quarter of tensor memory's lanes, which take turns at TURN tokens.
 // ---------------------------------------------------------------------------------------------
-template <bool DUAL, int OUT>
+template <bool DUAL, int OUT, int TURN>
 __global__ void __launch_bounds__(THREADS, DUAL ? 1 : 2)
 mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const __grid_constant__ CUtensorMap map_x,
                   const uint8_t* __restrict__ w_exp, const uint8_t* __restrict__ w2_exp, const uint8_t* x_exp, const PlainRows plain, const float* __restrict__ constants, int act,
@@ -451,16 +465,16 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
             const float b = (!DUAL && !e.act && OUT != OUT_ADD && e.constants != nullptr && f < n_feat) ? e.constants[f] : 0.f;
             const uint32_t trow = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * acc_cols);
 #pragma unroll 1
-            for (int c0 = half * 16; c0 < tn; c0 += 32) {
+            for (int c0 = half * TURN; c0 < tn; c0 += 2 * TURN) {
                 if (t0 + c0 >= n_tok) break;
-                uint32_t v[16], u[16];
-                tmem_ld16(trow + c0, v);
-                if (DUAL) tmem_ld16(trow + tn + c0, u);
+                uint32_t v[TURN], u[TURN];
+                tmem_load<TURN>(trow + c0, v);
+                if (DUAL) tmem_load<TURN>(trow + tn + c0, u);
                 tmem_wait_ld();
-                float r[16];
+                float r[TURN];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) r[j] = result<DUAL, OUT>(__uint_as_float(v[j]), DUAL ? __uint_as_float(u[j]) : 0.f, b, e);
-                store_lanes<OUT, 16>(res, [&](int j) { return t0 + c0 + j; }, [&](int j) { return t0 + c0 + j < n_tok; }, f, n_feat, r);
+                for (int j = 0; j < TURN; ++j) r[j] = result<DUAL, OUT>(__uint_as_float(v[j]), DUAL ? __uint_as_float(u[j]) : 0.f, b, e);
+                store_lanes<OUT, TURN>(res, [&](int j) { return t0 + c0 + j; }, [&](int j) { return t0 + c0 + j < n_tok; }, f, n_feat, r);
             }
             tc_fence_before();
             __syncwarp();
@@ -489,13 +503,13 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
             const uint32_t trow = tmem_base + ((uint32_t)(quarter * 32) << 16);
             const float* mine = recv + (size_t)rank * held * ROWS + fl;
 #pragma unroll 1
-            for (int c0 = half * 16; c0 < tokens; c0 += 32) {
-                uint32_t v[16];
-                tmem_ld16(trow + c0, v);
+            for (int c0 = half * TURN; c0 < tokens; c0 += 2 * TURN) {
+                uint32_t v[TURN];
+                tmem_load<TURN>(trow + c0, v);
                 tmem_wait_ld();
                 int to = c0 % cluster, at = (c0 / cluster) * ROWS;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
+                for (int j = 0; j < TURN; ++j) {
                     if (c0 + j < tokens) store_peer_float(mine + at, (uint32_t)to, __uint_as_float(v[j]));
                     if (++to == cluster) { to = 0; at += ROWS; }
                 }
@@ -945,12 +959,12 @@ Plan plan(int n_tok, int n_feat, int n_spans, bool dual) {
     return p;
 }
 
-template <bool DUAL, int OUT>
+template <bool DUAL, int OUT, int TURN>
 int launch_feature(const Call& c) {
     const Plan& p = c.plan;
     const long long tiles = (long long)((c.n_tok + p.tn - 1) / p.tn) * ((c.n_feat + ROWS - 1) / ROWS);
     if (tiles > 0x7fffffffLL / CLUSTER_MOST) return fail("gemm_microscaled: %lld tiles exceed the index range", tiles);
-    auto kernel = mx_feature_kernel<DUAL, OUT>;
+    auto kernel = mx_feature_kernel<DUAL, OUT, TURN>;
     static PerDeviceOnce configured;
     if (int rc = raise_dynamic_smem(kernel, SMEM_LIMIT, configured, "gemm_microscaled")) return rc;
     constexpr int MATS = DUAL ? 2 : 1;
@@ -969,7 +983,7 @@ int launch_feature(const Call& c) {
     size_t smem = (apart ? ring + recv : ring > (size_t)recv ? ring : (size_t)recv) + 1024;
     long long ctas = tiles * p.cluster;
     if (p.cluster == 1 && ctas > sm_count()) ctas = sm_count();
-    if (c.plain.at != nullptr && (stages < most || ctas < tiles)) return NEEDS_ROWS;
+    if (c.plain.at != nullptr && (stages < most || ctas < tiles || (c.n_tok > 4 && p.cluster > 1 && most * c.n_tok > 32))) return NEEDS_ROWS;
     // two accumulators, so that a tile's epilogue runs beside the next one's MMAs, where a CTA has several tiles and the columns suffice
     constexpr int EXP_COLS = 2 * (MATS + 1) * 4;
     const int one = MATS * p.tn + EXP_COLS, two = one + MATS * p.tn;
@@ -1002,7 +1016,11 @@ int launch_pair(const Call& c) {
 
 template <bool DUAL, int OUT>
 int launch(const Call& c) {
-    return c.plan.pairs ? launch_pair<DUAL, OUT>(c) : launch_feature<DUAL, OUT>(c);
+    if (c.plan.pairs) return launch_pair<DUAL, OUT>(c);
+    // Up to 16 tokens a turn of the epilogue takes 8, of gated products 4, since a turn costs as much for tokens that are not there; beyond that 16
+    // (us, turns of 16 / 8 / 4: gated [18944, 3584] 1 token 15.8 / 14.7 / 14.3, 16 tokens 16.0 / 15.0 / 15.2, 61 19.4 / 19.7 / 19.8; [1152, 896] 1
+    // token 3.25 / 3.0 / 3.0, 61 4.0 / 4.0 / 4.2).
+    return c.n_tok <= 16 ? launch_feature<DUAL, OUT, DUAL ? 4 : 8>(c) : launch_feature<DUAL, OUT, 16>(c);
 }
 
 }  // namespace

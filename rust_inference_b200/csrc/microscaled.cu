@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512, HELD == 1 ? 1 : 2) rms
             for (int i = 0; i < 8; ++i) v.v[i] += b.v[i];
         }
     };
+    if (HELD == 1 && blockIdx.x == 0 && tid * 8 < k) asm volatile("prefetch.global.L2 [%0];" ::"l"(weight + tid * 8));   // (while the kernel before ends)
     wait_for_previous_kernels();
     const int row = blockIdx.x;
     auto read = [&](int g, Eight<float>& v) {
@@ -267,9 +268,10 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512, HELD == 1 ? 1 : 2) rms
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) sums[warp] = sum;
     __syncthreads();
-    double s = lane < warps ? sums[lane] : 0.0;                   // every warp adds the warps' sums, in the same order
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    // every warp adds the warps' sums, in the same order: lanes that are apart by the power of two that holds them have the same
+    const int over = warps <= 1 ? 1 : 2 << (31 - __clz(warps - 1)), at = lane & (over - 1);
+    double s = at < warps ? sums[at] : 0.0;
+    for (int o = over >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     const double r = rsqrt(s * inverse + eps);
     const float r32 = (float)r;
     auto finish = [&](int g, const Eight<float>& v, const float* by) {

@@ -214,16 +214,16 @@ struct PlainRows {
 };
 
 // The CTA's spans, `count` from `begin` on, by 256 threads: eight numbers of a row each, so that sixteen threads have a span of a row, and four a
-// block; four reads of a thread are on their way together.
+// block; two reads of a thread are on their way together.
 template <typename T>
 __device__ __forceinline__ void write_plain(const PlainRows& x, int n_tok, int begin, int count, uint32_t tiles, uint32_t tile_bytes, uint32_t pieces,
                                             uint32_t piece_bytes, int thread) {
     const int items = count * n_tok * 16, chunk = thread & 15;
     const uint32_t of_row = 0xffffu / (uint32_t)n_tok + 1;          // (exact: numbers below 2^10 by at most 16)
-    for (int i0 = thread; i0 < items + 15; i0 += 4 * 256) {           // (whole quads go round together: items is a multiple of 16)
-        float v[4][8];
+    for (int i0 = thread; i0 < items + 15; i0 += 2 * 256) {           // (whole quads go round together: items is a multiple of 16)
+        float v[2][8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             const int q = (i0 + i * 256) >> 4, span = (int)((uint32_t)q * of_row >> 16), row = q - span * n_tok, c = (begin + span) * SPAN + chunk * 8;
             const bool there = span < count && c < x.k;
             if (sizeof(T) == 2) {
@@ -245,7 +245,7 @@ __device__ __forceinline__ void write_plain(const PlainRows& x, int n_tok, int b
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             const int q = (i0 + i * 256) >> 4, span = (int)((uint32_t)q * of_row >> 16), row = q - span * n_tok;
             if (span >= count) break;
             uint32_t top = 0;
@@ -1016,7 +1016,7 @@ int launch_pair(const Call& c) {
 
 template <bool DUAL, int OUT>
 int launch(const Call& c) {
-    if (c.plan.pairs) return launch_pair<DUAL, OUT>(c);
+    if (c.plan.pairs) return c.plain.at != nullptr ? NEEDS_ROWS : launch_pair<DUAL, OUT>(c);
     // Up to 16 tokens a turn of the epilogue takes 8, of gated products 4, since a turn costs as much for tokens that are not there; beyond that 16
     // (us, turns of 16 / 8 / 4: gated [18944, 3584] 1 token 15.8 / 14.7 / 14.3, 16 tokens 16.0 / 15.0 / 15.2, 61 19.4 / 19.7 / 19.8; [1152, 896] 1
     // token 3.25 / 3.0 / 3.0, 61 4.0 / 4.0 / 4.2).

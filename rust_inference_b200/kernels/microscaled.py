@@ -199,3 +199,8 @@ def product(x, w: Matrix, out, ctx, *, w2: Matrix | None = None, bias=None, form
 def _status_address() -> int:
     from .tcgen05 import status_word
     return status_word().data_ptr()
+
+
+def set_pairs(tokens: int = 0) -> None:
+    """Products of at least so many tokens run on pairs of SMs, others do not; 0: whichever takes less time (for tests and comparisons)."""
+    load("gemm_microscaled").ri_mx_set_pairs(c_int(tokens))

@@ -468,3 +468,25 @@ def test_a_few_plain_rows_are_what_rows_in_eight_bits_are(n, k):
             linear.gated(microscaled.quantize(x), held, held, from_rows, ctx)
             assert torch.equal(microscaled.values(rows), microscaled.values(from_rows))
     check_status()
+
+
+@pytest.fixture(params=["pairs of SMs", "single SMs"])
+def one_kernel(request):
+    from rust_inference_b200.kernels import microscaled
+    microscaled.set_pairs(1 if request.param == "pairs of SMs" else 1 << 30)
+    yield
+    microscaled.set_pairs()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (2, 130, 64), (61, 300, 8960), (129, 200, 300), (200, 5000, 256), (257, 385, 129), (333, 2560, 2048), (1000, 640, 1536),
+                                   (130, 41000, 200), (513, 20100, 136)])
+def test_either_kernel_takes_every_product(one_kernel, m, n, k):
+    for dtype in (torch.bfloat16, torch.float32):
+        test_product(m, n, k, dtype)
+    if n < 10000:
+        test_gated_and_into_eight_bits(m, n, k, "bounded")
+
+
+@pytest.mark.parametrize("m", [1, 130, 600])
+def test_either_kernel_applies_every_activation(one_kernel, m):
+    test_activated(m)

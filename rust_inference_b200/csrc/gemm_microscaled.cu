@@ -138,6 +138,8 @@ __device__ __forceinline__ float gated_quick(float g, float u, const GateForm& f
     u = fmaxf(fminf(u, f.limit), -f.limit) + f.shift;
     return __fdividef(g, 1.f + __expf(-f.alpha * g * fmaf(f.cubic * g, g, 1.f))) * u * f.mult;
 }
+// the same with the constants of silu
+__device__ __forceinline__ float silu_quick(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 // `act_quick_f32` (common.cuh) without branches: a warp whose accumulators lie on both sides of zero would go through one after the other
 // (256 features of a token took 7 us, 1.5 so)
 __device__ __forceinline__ float act_chosen(float z, const ActForm& f) {
@@ -589,13 +591,34 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
     tmem_ld16(taddr + 16, r + 16);
 }
 
-// 32 features of a token, from feature f on, as this thread has computed them.
+// 32 features of a token each, from feature f on, as the 32 threads of a warp have computed them for tokens t.. of which `tokens` are there: pieces of
+// 16 bytes change places in the warp's 2 KB of shared memory, so that neighbouring threads write neighbouring pieces.
+constexpr int EXCHANGE = 2048;
+__device__ __forceinline__ uint32_t piece_at(uint32_t room, int token, int piece, int pieces) {
+    return room + (uint32_t)(token * pieces + (piece ^ (token * pieces / 8 & (pieces - 1)))) * 16u;
+}
+template <int PIECES>
+__device__ __forceinline__ void exchange(uint32_t room, int lane, uint4* c) {
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece_at(room, lane, q, PIECES)), "r"(c[q].x), "r"(c[q].y), "r"(c[q].z), "r"(c[q].w) : "memory");
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(c[q].x), "=r"(c[q].y), "=r"(c[q].z), "=r"(c[q].w)
+                     : "r"(piece_at(room, q * (32 / PIECES) + lane / PIECES, lane % PIECES, PIECES)) : "memory");
+}
 template <int OUT>
-__device__ __forceinline__ void store_run(const Result& r, int t, int f, int n_feat, bool aligned, const float* v) {
+__device__ __forceinline__ void store_run(const Result& r, int t, int tokens, int f, int n_feat, bool aligned, uint32_t room, int lane, float* v) {
     if (OUT == OUT_ROWS) {
+        if (f + 32 > n_feat) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = f + j < n_feat ? v[j] : 0.f;
+        }
         uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) top = max(top, f + j < n_feat ? __float_as_uint(v[j]) & 0x7fffffffu : 0u);
+        for (int j = 0; j < 32; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
         const uint32_t byte = exponent_byte<8>(top);
         const float by = to_type(byte);
         uint4 c[2];
@@ -604,33 +627,51 @@ __device__ __forceinline__ void store_run(const Result& r, int t, int f, int n_f
         for (int q = 0; q < 8; ++q) {
             float y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = f + 4 * q + j < n_feat ? v[4 * q + j] * by : 0.f;
+            for (int j = 0; j < 4; ++j) y[j] = v[4 * q + j] * by;
             w[q] = eight_bits(y);
         }
-        uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(r.out) + (size_t)t * r.n_spans * SPAN + f);
-        to[0] = c[0];
-        to[1] = c[1];
-        r.exponents[exponent_at(t, f >> 5, r.n_spans)] = (uint8_t)byte;
+        exchange<2>(room, lane, c);
+        uint8_t* to = reinterpret_cast<uint8_t*>(r.out) + (size_t)(t + lane / 2) * r.n_spans * SPAN + f + lane % 2 * 16;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            if (q * 16 + lane / 2 < tokens) *reinterpret_cast<uint4*>(to + (size_t)(q * 16) * r.n_spans * SPAN) = c[q];
+        if (lane < tokens) r.exponents[exponent_at(t + lane, f >> 5, r.n_spans)] = (uint8_t)byte;
         return;
     }
-    const size_t at = (size_t)t * n_feat + f;
     if (aligned && f + 32 <= n_feat) {
         if (OUT == OUT_BF16) {
+            uint4 c[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(r.out) + at)[q] = pack8(v + 8 * q);
+            for (int q = 0; q < 4; ++q) c[q] = pack8(v + 8 * q);
+            exchange<4>(room, lane, c);
+            __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(r.out) + (size_t)(t + lane / 4) * n_feat + f + lane % 4 * 8;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (q * 8 + lane / 4 < tokens) *reinterpret_cast<uint4*>(to + (size_t)(q * 8) * n_feat) = c[q];
         } else {
-            float* to = reinterpret_cast<float*>(r.out) + at;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                if (OUT == OUT_ADD)
-                    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to + 4 * q), "f"(v[4 * q]), "f"(v[4 * q + 1]),
-                                 "f"(v[4 * q + 2]), "f"(v[4 * q + 3]) : "memory");
-                else
-                    reinterpret_cast<float4*>(to)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            for (int h = 0; h < 2; ++h) {                                             // sixteen features at a time
+                uint4 c[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) c[q] = *reinterpret_cast<uint4*>(v + 16 * h + 4 * q);
+                exchange<4>(room, lane, c);
+                float* to = reinterpret_cast<float*>(r.out) + (size_t)(t + lane / 4) * n_feat + f + 16 * h + lane % 4 * 4;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (q * 8 + lane / 4 < tokens) {
+                        float* at = to + (size_t)(q * 8) * n_feat;
+                        if (OUT == OUT_ADD)
+                            asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(__uint_as_float(c[q].x)),
+                                         "f"(__uint_as_float(c[q].y)), "f"(__uint_as_float(c[q].z)), "f"(__uint_as_float(c[q].w)) : "memory");
+                        else
+                            *reinterpret_cast<uint4*>(at) = c[q];
+                    }
             }
         }
         return;
     }
+    if (lane >= tokens) return;
+    const size_t at = (size_t)(t + lane) * n_feat + f;
 #pragma unroll
     for (int j = 0; j < 32; ++j)
         if (f + j < n_feat) {
@@ -747,13 +788,6 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             bool alive = true;
             const uint64_t desc_x0 = make_smem_desc(smem_base), desc_e0 = piece_desc(exp_base);
             for (int i = 0; i < my_tiles && alive; ++i) {
-                // the columns that the tile before shares have been read, and with them all of the one before that
-                if (i > 0 && !mbar_wait_warp(smem_u32(&next_bar), (uint32_t)(i - 1) & 1u)) {
-                    if (lane == 0) report(status, ST_MMA_TIMEOUT);
-                    abort_flag = 1;
-                    break;
-                }
-                tc_fence_after();
                 const uint32_t acc = tmem_base + (uint32_t)((i & 1) * SECOND_ACC);
                 for (int j = 0; j < n_spans; ++j) {
                     if (!ring.wait()) {
@@ -768,6 +802,16 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                     const uint64_t e = desc_e0 + (uint64_t)((uint32_t)ring.s * (PAIR_EXP >> 4));
 #pragma unroll
                     for (int m = 0; m < 3; ++m) exponents_to_tmem<1>(leader, ex + 4 * m, e + (uint64_t)(m * (PIECE >> 4)));
+                    if (j == 0 && i > 0) {
+                        // the columns that the tile before shares have been read, and with them all of the one before that
+                        if (!mbar_wait_warp(smem_u32(&next_bar), (uint32_t)(i - 1) & 1u)) {
+                            if (lane == 0) report(status, ST_MMA_TIMEOUT);
+                            abort_flag = 1;
+                            alive = false;
+                            break;
+                        }
+                        tc_fence_after();
+                    }
                     const uint64_t x = desc_x0 + (uint64_t)((uint32_t)ring.s * (2 * TILE >> 4)), w = x + (TILE >> 4);
 #pragma unroll
                     for (int b = 0; b < SPAN / BLOCK; ++b)
@@ -784,6 +828,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         const uint32_t next_first = in_first_cta(smem_u32(&next_bar));
         wait_for_previous_kernels();
         const Epilogue e = load_epilogue<DUAL>(constants, act);
+        const uint32_t room = exp_base + (uint32_t)stages * PAIR_EXP + (uint32_t)(warp - 2) * EXCHANGE;
         const bool aligned = (OUT == OUT_BF16 ? n_feat % 8 == 0 : n_feat % 4 == 0) && (reinterpret_cast<uintptr_t>(res.out) & 15) == 0;
         for (int i = 0; i < my_tiles; ++i) {
             int f0, t0;
@@ -796,7 +841,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             tc_fence_after();
             __syncwarp();
             if (__any_sync(0xffffffffu, !landed || abort_flag)) break;
-            const int t = t0 + rank * ROWS + lane_base + lane;
+            const int t = t0 + rank * ROWS + lane_base;                // the warp's first token
             const uint32_t trow = tmem_base + ((uint32_t)lane_base << 16) + (uint32_t)((i & 1) * SECOND_ACC);
             constexpr int RUNS = FEATS / 32;
 #pragma unroll 1
@@ -804,23 +849,31 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 // the first accumulator shares its last columns, the second its first: those are read in the first turn
                 const int c = ((i & 1) ? n : RUNS - 1 - n) * 32, f = f0 + c;
                 float v[32], u[DUAL ? 32 : 1];
-                tmem_ld32(trow + c, reinterpret_cast<uint32_t*>(v));
-                if (DUAL) tmem_ld32(trow + ROWS + c, reinterpret_cast<uint32_t*>(u));
-                tmem_wait_ld();
+                if (!DUAL || (i & 1)) tmem_ld32(trow + c, reinterpret_cast<uint32_t*>(v));
+                else tmem_ld32(trow + ROWS + c, reinterpret_cast<uint32_t*>(u));
                 if (n == half) {
+                    tmem_wait_ld();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) arrive_cluster(next_first);
                 }
-                if (f >= (OUT == OUT_ROWS ? res.n_spans * SPAN : n_feat) || t >= n_tok) continue;
-                if (DUAL || e.act) {
+                if (DUAL) {
+                    if (i & 1) tmem_ld32(trow + ROWS + c, reinterpret_cast<uint32_t*>(u));
+                    else tmem_ld32(trow + c, reinterpret_cast<uint32_t*>(v));
+                }
+                tmem_wait_ld();
+                if (f >= (OUT == OUT_ROWS ? res.n_spans * SPAN : n_feat) || t >= n_tok) continue;           // (of no thread's, or of all)
+                if (DUAL && OUT != OUT_F32 && e.constants == nullptr) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = silu_quick(v[j], u[DUAL ? j : 0]);
+                } else if (DUAL || e.act) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = result<DUAL, OUT>(v[j], DUAL ? u[j] : 0.f, 0.f, e);
                 } else if (OUT != OUT_ADD && e.constants != nullptr) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] += f + j < n_feat ? e.constants[f + j] : 0.f;
                 }
-                store_run<OUT>(res, t, f, n_feat, aligned, v);
+                store_run<OUT>(res, t, n_tok - t, f, n_feat, aligned, room, lane, v);
             }
         }
     }
@@ -912,9 +965,9 @@ int g_pair_tokens = 0;           // > 0: products of at least so many tokens run
 // where no other product of the rule is near (tn: tokens of the tile):
 //   first kernel, not cut   a round of tiles: 12.5 + 0.066 tn a span, and 100 beside the next one's; once 190 + 1.85 tn
 //   cut over clusters       the same for the spans of a CTA; once 320 + 2.2 tn, and the codes at 6 TB/s
-//   pairs                   a round of tiles: 36 a span, and 100; once 700 (stores of 256 tokens that nothing runs beside)
-// So a product of [3584, 3584] (us, first kernel / pairs) with 256 tokens takes 10.1 / 15.5, 1,024: 17.8 / 18.6, 2,048: 30.0 / 28.3, and of
-// [3584, 18944] 24.4 / 50, 66.7 / 55.2 and 128 / 108; of [2048, 2048] with 64 tokens, not cut / in clusters of four, 5.3 / 5.7, of [3584, 3584]
+//   pairs                   a round of tiles: 34 a span, and 90; once 560 (stores of 256 tokens that nothing runs beside)
+// So a product of [3584, 3584] (us, first kernel / pairs) with 256 tokens takes 11.9 / 15.5, 1,024: 18.7 / 16.9, 2,048: 31.9 / 27.4, and of
+// [3584, 18944] 25.1 / 49.4, 70.5 / 54.1 and 133 / 106; of [2048, 2048] with 64 tokens, not cut / in clusters of four, 5.3 / 5.7, of [3584, 3584]
 // 7.5 / 7.1, of [3584, 18944] 30 / 13.1.
 Plan plan(int n_tok, int n_feat, int n_spans, bool dual) {
     Plan p;
@@ -923,9 +976,9 @@ Plan plan(int n_tok, int n_feat, int n_spans, bool dual) {
     const long long sms = sm_count(), feat_tiles = (n_feat + ROWS - 1) / ROWS, tiles = feat_tiles * ((n_tok + p.tn - 1) / p.tn);
     if (dual) {
         // Gated products fill the ring with two matrices, and a cluster's exchange costs them what it saves.  On pairs a tile has twice the
-        // tokens and reads them once for both matrices: beyond 128 tokens always (200 tokens, 148 tiles 45.0 / 29.3 us), from 72 where a
-        // round is enough (96 tokens, 38 tiles 11.7 / 9.6, 70 tiles 14.3 / 12.0; 86 tiles, two rounds, 16.4 / 18.7).
-        p.pairs = n_tok > TOKENS_MOST || (n_tok >= 72 && 2 * feat_tiles <= sms);
+        // tokens and reads them once for both matrices: beyond 128 tokens always (160 tokens, 148 tiles 43.9 / 26.6 us), from 56 where a
+        // round is enough (56 tokens, 38 tiles 8.7 / 8.0, 70 tiles 10.75 / 10.75; 96 tokens 11.5 / 8.1, 13.7 / 10.4; 86 tiles, two rounds, 16.1 / 16.7).
+        p.pairs = n_tok > TOKENS_MOST || (n_tok >= 56 && 2 * feat_tiles <= sms);
     } else {
         const double span = 12.5 + 0.066 * p.tn, rounds = (double)((tiles + sms - 1) / sms);
         const double meet = 320 + 2.2 * p.tn + (double)n_feat * n_spans * (SPAN / 2) / 6e4;
@@ -952,7 +1005,7 @@ Plan plan(int n_tok, int n_feat, int n_spans, bool dual) {
             }
         }
         const long long pair_tiles = (long long)((n_tok + PAIR_TOK - 1) / PAIR_TOK) * ((n_feat + PAIR_ROWS - 1) / PAIR_ROWS), pairs = sms / 2;
-        p.pairs = n_tok > TOKENS_MOST && ((pair_tiles + pairs - 1) / pairs) * (36.0 * n_spans + 100) + 700 < best;
+        p.pairs = n_tok > TOKENS_MOST && ((pair_tiles + pairs - 1) / pairs) * (34.0 * n_spans + 90) + 560 < best;
     }
     if (g_pair_tokens > 0) p.pairs = n_tok >= g_pair_tokens;
     if (p.pairs) p.tn = ROWS;
@@ -1005,11 +1058,11 @@ int launch_pair(const Call& c) {
     auto kernel = mx_pair_kernel<DUAL, OUT>;
     static PerDeviceOnce configured;
     if (int rc = raise_dynamic_smem(kernel, SMEM_LIMIT, configured, "gemm_microscaled")) return rc;
-    constexpr int STAGES = (SMEM_LIMIT - 1024) / PAIR_STAGE;
+    constexpr int ROOM = 8 * EXCHANGE, STAGES = (SMEM_LIMIT - 1024 - ROOM) / PAIR_STAGE;
     static_assert(STAGES <= MAX_STAGES && STAGES >= 2, "a ring of stages");
     long long pairs = sm_count() / 2;
     if (pairs > tiles) pairs = tiles;
-    return launch_cluster("gemm_microscaled (pairs of SMs)", kernel, dim3((unsigned)(2 * pairs)), THREADS, (size_t)STAGES * PAIR_STAGE + 1024, 2, c.stream,
+    return launch_cluster("gemm_microscaled (pairs of SMs)", kernel, dim3((unsigned)(2 * pairs)), THREADS, (size_t)STAGES * PAIR_STAGE + ROOM + 1024, 2, c.stream,
                           c.w->codes, c.w2->codes, c.x->codes, c.w->exponents, c.w2->exponents, c.x->exponents, c.constants, c.act, c.res, c.n_tok, c.n_feat,
                           c.n_spans, STAGES, c.status);
 }

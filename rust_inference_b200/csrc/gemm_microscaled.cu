@@ -269,8 +269,12 @@ __device__ __forceinline__ void write_plain(const PlainRows& x, int n_tok, int b
 }
 
 // ---------------------------------------------------------------------------------------------
-// Few tokens.  Tiles of 128 features x tn tokens, for a persistent grid of CTAs, or (not gated) each for a cluster whose CTAs share its K.  Warp 0 issues the copies, warp 1 allocates tensor memory and issues the MMAs,
-// warps 2-9 run the epilogue, two for each quarter of tensor memory's lanes, which take turns at TURN tokens.
+// Few tokens.  Tiles of 128 features x tn tokens, for a persistent grid of CTAs, or (not gated) each for a cluster whose CTAs share its K.  Warp 0
+// issues the copies, warp 1 allocates tensor memory and issues the MMAs, warps 2-9 run the epilogue, two for each quarter of tensor memory's
+// lanes, which take turns at TURN tokens.
+// What bounds it: the weights' way from memory, where there are enough of them (8 tokens: two matrices [18944, 3584], 72 MB, 14.6 us, 4.9 TB/s; between
+// the kernels of a step 12.7 with one token, since the first ring of weights goes out before the wait); else trips: the rows' 1 us after the wait, the last
+// span's MMAs and the epilogue 0.5, the cluster's meeting 1.2 ([4608, 3584] 6.0 us, [3584, 3584] 5.5, [3584, 18944] 10.6, [896, 896] 3.0).
 // ---------------------------------------------------------------------------------------------
 template <bool DUAL, int OUT, int TURN>
 __global__ void __launch_bounds__(THREADS, DUAL ? 1 : 2)
@@ -559,6 +563,11 @@ mx_feature_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 //
 // Two accumulators of 256 columns would leave tensor memory no room for exponents, so the second begins 32 columns before the first ends: an
 // epilogue reads the columns that both use first, and says so, and then the MMAs of the next tile may begin.
+//
+// What bounds it: the clock, which falls to 1.6 GHz under these MMAs, and at it the tensor cores, which are busy for 75 to 87% of the time; the way from
+// L2 (8.6 TB/s; without the copies of X an eighth less time), the turn of the accumulators at a tile's end (7% at 28 spans a tile), the epilogue's
+// instructions and stores (4 and 3%).  2,048 tokens: gated [18944, 3584] 184 us, 3.0 PFLOP/s, with one kernel for the two matrices and the rows in 8 bits
+// that the next product reads; [3584, 18944] onto the stream 100 us, 2.8 PFLOP/s.
 // ---------------------------------------------------------------------------------------------
 constexpr int PAIR_TOK = 2 * ROWS, PAIR_ROWS = 2 * ROWS;
 constexpr int PAIR_EXP = 3 * PIECE;                    // exponents of a stage: 128 tokens, 256 rows of W

@@ -974,6 +974,9 @@ int g_pair_tokens = 0;           // > 0: products of at least so many tokens run
 // where no other product of the rule is near (tn: tokens of the tile):
 //   first kernel, not cut   a round of tiles: 12.5 + 0.066 tn a span, and 100 beside the next one's; once 190 + 1.85 tn
 //   cut over clusters       the same for the spans of a CTA; once 320 + 2.2 tn, and the codes at 6 TB/s
+//   either, up to 16 tokens 60 more where a CTA's spans are more than its ring holds, but less than two of it: the last are asked for when the rows have
+//                           come, and nothing hides their wait ([1536, 1536], 12 spans, ring of 11, 1 token: uncut 4.25 us, clusters of 8 3.5, plain rows
+//                           5.2 / 3.75; [4608, 3584], 28 spans: uncut 6.0, clusters of 3 6.0, and a decode step of 8 sequences 5% slower with them)
 //   pairs                   a round of tiles: 34 a span, and 90; once 560 (stores of 256 tokens that nothing runs beside)
 // So a product of [3584, 3584] (us, first kernel / pairs) with 256 tokens takes 11.9 / 15.5, 1,024: 18.7 / 16.9, 2,048: 31.9 / 27.4, and of
 // [3584, 18944] 25.1 / 49.4, 70.5 / 54.1 and 133 / 106; of [2048, 2048] with 64 tokens, not cut / in clusters of four, 5.3 / 5.7, of [3584, 3584]
@@ -991,13 +994,15 @@ Plan plan(int n_tok, int n_feat, int n_spans, bool dual) {
     } else {
         const double span = 12.5 + 0.066 * p.tn, rounds = (double)((tiles + sms - 1) / sms);
         const double meet = 320 + 2.2 * p.tn + (double)n_feat * n_spans * (SPAN / 2) / 6e4;
-        double best = rounds * (span * n_spans + 100) + 90 + 1.85 * p.tn;
+        const int ring = (SMEM_LIMIT - 1024) / (TILE + p.tn * SPAN + 2 * PIECE);
+        auto late = [&](int count) { return p.tn <= 16 && count > ring && count < 2 * ring ? 60 : 0; };
+        double best = rounds * (span * n_spans + 100) + 90 + 1.85 * p.tn + late(n_spans);
         for (int c = 2; c <= CLUSTER_MOST && c <= n_spans; ++c) {
             // Clusters of whole SMs lie within groups of SMs, which leaves some over, and those of the next kernel come in while these leave: where
             // there are many, the last find their place late (36 clusters of 4, 9.9 us instead of 6.1), large ones sooner (16 of 7, 12.2 instead
             // of 7.1).
             if (tiles * c > (c > 4 ? sms * 2 / 3 : sms - 20)) continue;
-            const double cost = span * ((n_spans + c - 1) / c) + meet;
+            const double cost = span * ((n_spans + c - 1) / c) + meet + late((n_spans + c - 1) / c);
             if (cost < best) {
                 best = cost;
                 p.cluster = c;

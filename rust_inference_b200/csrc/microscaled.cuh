@@ -6,7 +6,7 @@
 // [n, k] such numbers are held with k rounded up to whole `SPAN`s of 128, zeros behind a row's end.  Rows in 8 bits: codes [n, span count * 128].
 // A matrix in 4 bits, whose n is rounded up to whole 128s too, lies as the products read it, a tile of 128 rows and a span, 8 KB, after the other,
 // [row / 128][span][128][64 bytes], number 2i in the low half of byte i (in rows as long as the matrix's, a tile would be 128 pieces of 64 bytes that
-// lie far apart: see the products' figures).  Exponents lie in the order in which the tensor cores' scale registers take them: one piece of 512
+// lie far apart: two large matrices for 8 tokens 2 to 3% slower).  Exponents lie in the order in which the tensor cores' scale registers take them: one piece of 512
 // bytes for every 128 rows and span, [row / 128][span], the exponent of row r and the span's block j (0..3) at (r % 32) * 16 + r % 128 / 32 * 4 + j.
 #pragma once
 

@@ -490,3 +490,90 @@ def test_either_kernel_takes_every_product(one_kernel, m, n, k):
 @pytest.mark.parametrize("m", [1, 130, 600])
 def test_either_kernel_applies_every_activation(one_kernel, m):
     test_activated(m)
+
+
+def test_two_streams_at_once():
+    """Products of either kernel and a plain bfloat16 one, side by side on two streams: results as alone."""
+    from rust_inference_b200.kernels import linear, microscaled
+    sides = []
+    for s, (m, hidden, inner) in enumerate(((8, 2048, 5632), (300, 1536, 4096))):
+        ctx = context()
+        ws = [spread(n, k, 7 * s + n + k, torch.bfloat16, 0.3).to(DEV) / math.sqrt(k) for n, k in ((hidden, hidden), (inner, hidden), (inner, hidden), (hidden, inner))]
+        held, weight = [microscaled.Matrix.of(w) for w in ws], linear.Weight(ws[0])
+        x = spread(m, hidden, s, torch.bfloat16, 0.3).to(DEV)
+        act, outs = microscaled.Rows(m, inner), [torch.empty(m, hidden, dtype=d, device=DEV) for d in (torch.bfloat16, torch.float32, torch.bfloat16)]
+
+        def run(ctx=ctx, x=x, held=held, weight=weight, act=act, outs=outs):
+            linear.project(x, held[0], outs[0], ctx)
+            linear.gated(outs[0], held[1], held[2], act, ctx)
+            linear.logits(act, held[3], outs[1], ctx)
+            linear.project(x, weight, outs[2], ctx)
+        sides.append((run, outs))
+    alone = []
+    for run, outs in sides:
+        run()
+        alone.append([o.clone() for o in outs])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sides]
+    for _ in range(20):
+        for _ in range(5):
+            for (run, _), stream in zip(sides, streams):
+                with torch.cuda.stream(stream):
+                    run()
+        torch.cuda.synchronize()
+        for (_, outs), want in zip(sides, alone):
+            for o, w in zip(outs[:2], want):
+                assert torch.equal(o, w)
+            assert ((outs[2] - want[2]).abs() <= 2.0 ** -6 * want[2].abs() + 2.0 ** -6).all()       # (its pieces of K may meet in any order)
+    check_status()
+
+
+def test_more_numbers_than_31_bits_count():
+    from rust_inference_b200.kernels import linear, microscaled
+    ctx = context()
+    n, k, m = 40000, 96, 60000
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(m, k, generator=g, device=DEV)
+    w = microscaled.Matrix.of(torch.randn(n, k, generator=g, device=DEV))
+    out = torch.empty(m, n, dtype=torch.bfloat16, device=DEV)
+    last = torch.empty(77, n, dtype=torch.bfloat16, device=DEV)
+    linear.project(x[-77:], w, last, ctx)
+    for pairs in (1, 1 << 30):
+        microscaled.set_pairs(pairs)
+        try:
+            out[-77:] = math.nan
+            linear.project(x, w, out, ctx)
+        finally:
+            microscaled.set_pairs()
+        # either sum is off by (96 / 32 + 16) 2^-23 of what is added up (about 60, 200 at most); then a step of the result's type
+        assert ((out[-77:].float() - last.float()).abs() <= 2.0 ** -7 * last.float().abs() + 2 * 19 * 2.0 ** -23 * 200).all()
+    # rows in 8 bits of them, and read back
+    rows = microscaled.quantize(out)
+    assert torch.equal(microscaled.values(rows, torch.bfloat16)[-77:], microscaled.values(microscaled.quantize(out[-77:]), torch.bfloat16))
+    del out
+    other = microscaled.Rows(m, n)
+    linear.gated(x, w, w, other, ctx)
+    few = microscaled.Rows(77, n)
+    linear.gated(x[-77:], w, w, few, ctx)
+    a, b = microscaled.values(other, torch.bfloat16)[-77:].float(), microscaled.values(few, torch.bfloat16).float()
+    # a code apart (2^-3 of a number, or 2^-9 times 2^e, which is at most the block's largest / 224), and twice that where e is one apart
+    wide = b.abs().view(77, -1, 32).amax(dim=2, keepdim=True).expand(-1, -1, 32).reshape(77, n)
+    assert ((a - b).abs() <= 2.0 ** -3 * b.abs() + 2.0 ** -8 * wide / 224).all() and float((a != b).float().mean()) < 1e-3
+    del other, rows
+    # a matrix of as many, and a norm of as many
+    wide = torch.randn(m, n, dtype=torch.bfloat16, generator=g, device=DEV)
+    held = microscaled.Matrix.of(wide)
+    assert torch.equal(microscaled.values(held, torch.bfloat16)[-77:], microscaled.values(microscaled.Matrix.of(wide[-77:]), torch.bfloat16))
+    y = torch.randn(3, n, generator=g, device=DEV)
+    got = torch.empty(3, m, device=DEV)
+    linear.logits(y, held, got, ctx)
+    y8, w4 = microscaled.values(microscaled.quantize(y)).double(), microscaled.values(microscaled.Matrix.of(wide[-128:])).double()
+    want, mass = y8 @ w4.t(), y8.abs() @ w4.abs().t()
+    assert ((got[:, -128:].double() - want).abs() <= bound(n, mass, want, torch.float32)).all()
+    del held
+    stream = wide.float()
+    rows = microscaled.rmsnorm(stream, torch.ones(n, device=DEV), 1e-6, microscaled.Rows(m, n), branch=wide, total=stream)
+    again = microscaled.rmsnorm(wide[-77:].float() * 2, torch.ones(n, device=DEV), 1e-6, microscaled.Rows(77, n))
+    assert torch.equal(microscaled.values(rows, torch.bfloat16)[-77:], microscaled.values(again, torch.bfloat16))
+    assert torch.equal(stream[-77:], wide[-77:].float() * 2)
+    check_status()

@@ -345,15 +345,18 @@ PyObject* py_mx_hold(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Py_RETURN_NONE;
     });
 }
-// (held, out)
+// (held, out), or (held, None, bfloat16 or float32, n, k) for a new tensor
 typedef int Mx_valuesFn(const void*, int, long long, long long, void*, void*);
 PyObject* py_mx_values(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const char* what = "microscaled.values";
-        need(n == 2, "microscaled.values: 2 arguments");
-        const at::Tensor& out = dense(a[1], what);
+        need(n == 2 || n == 5, "microscaled.values: 2 or 5 arguments");
+        const bool made = n == 5 && a[1] == Py_None;
+        const at::Tensor out = made ? at::empty({number(a[3]), number(a[4])}, at::TensorOptions().device(at::kCUDA, c10::cuda::current_device())
+                                                                                  .dtype(number(a[2]) ? at::kBFloat16 : at::kFloat))
+                                    : dense(a[1], what);
         finish(entry<Mx_valuesFn>(MX_VALUES)(address<void>(number(a[0])), code_of(out, what), out.size(0), out.size(1), out.data_ptr(), stream()), MX_VALUES, what);
-        Py_RETURN_NONE;
+        return THPVariable_Wrap(out);
     });
 }
 // (x, branch or None, weight, total or None, eps, held)

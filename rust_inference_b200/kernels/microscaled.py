@@ -21,7 +21,7 @@ import torch
 
 from . import ops
 from .build import load
-from .ops import _call, _need, _p, _stream, native
+from .ops import KernelError, _call, _need, _p, _stream, native
 
 BLOCK, SPAN, PIECE = 32, 128, 512
 
@@ -67,15 +67,16 @@ class Matrix:
     @classmethod
     def of(cls, t: torch.Tensor) -> "Matrix":
         """The matrix nearest to t [n, k], float32 or bfloat16, whose rows may lie apart."""
-        _need(t.dim() == 2 and t.shape[0] > 0 and t.shape[1] > 0 and t.dtype in (torch.float32, torch.bfloat16),
+        n, k = t.shape if t.dim() == 2 else (0, 0)
+        _need(n > 0 and k > 0 and t.dtype in (torch.float32, torch.bfloat16),
               "microscaled.Matrix: a matrix [n, k] of at least one number, float32 or bfloat16, is wanted")
         ops._need_cuda(t)
-        if (t.stride(1) != 1 and t.shape[1] > 1) or t.stride(0) < t.shape[1]:
+        if not t.is_contiguous() and ((t.stride(1) != 1 and k > 1) or t.stride(0) < k):
             t = t.contiguous()
         m = cls.__new__(cls)
         m.codes, m.exponents, m._described = _maker()(t)
-        m.n, m.k = t.shape
-        m.spans, m.device, m.native = _spans(m.k), t.device, m._described.data_ptr()
+        m.n, m.k = n, k
+        m.spans, m.device, m.native = _spans(k), t.device, m._described.data_ptr()
         return m
 
     @classmethod
@@ -161,7 +162,8 @@ def values(held, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = 
     """The numbers [n, k] that a `Matrix` or `Rows` stands for, in float32 or bfloat16 (which hold them exactly, but for results that
     the type has no room for)."""
     if out is None:
-        out = torch.empty(held.n, held.k, dtype=dtype, device=held.device)
+        _need(dtype in (torch.float32, torch.bfloat16), "microscaled.values: float32 or bfloat16 is wanted")
+        return native("mx_values")(held.native, None, dtype is torch.bfloat16, held.n, held.k)
     _need(out.dtype is dtype, "microscaled.values: out is of the dtype asked for")
     native("mx_values")(held.native, out)
     return out
@@ -180,18 +182,22 @@ def product(x, w: Matrix, out, ctx, *, w2: Matrix | None = None, bias=None, form
     """out = x W^T + bias; with `act` an activation of it (`ops.whole_act_form`); with w2 the gated form of x W^T and x W2^T (`form`:
     `ops.gate_form`, None: silu); with `add` out<float32> += x W^T.  x: `Rows`, or plain rows, which are brought to 8 bits in the step's
     scratch; out: plain rows, or (not with `add`) `Rows`."""
-    _need(type(w) is Matrix and (w2 is None or type(w2) is Matrix), "microscaled.product: matrices in 4 bits are wanted")
-    plain = type(x) is not Rows
-    if plain and (x.dim() != 2 or x.shape[0] == 0):
-        _need(x.dim() == 2 and x.shape[1] == w.k and tuple(out.shape) == (0, w.n), "microscaled.product: rows [tokens, k] and a result [tokens, features] are wanted")
-        return out
-    _need((bias is not None) + (act is not None) + (w2 is not None) + add <= 1 and (form is None or w2 is not None),
-          "microscaled.product: a bias, an activation, a gate and an addition are not combined")
+    if type(w) is not Matrix or (w2 is not None and type(w2) is not Matrix):
+        raise KernelError("microscaled.product: matrices in 4 bits are wanted")
+    if type(x) is Rows:
+        rows, x = x, None
+    else:
+        shape = x.shape
+        if len(shape) != 2 or shape[0] == 0:
+            _need(len(shape) == 2 and shape[1] == w.k and tuple(out.shape) == (0, w.n), "microscaled.product: rows [tokens, k] and a result [tokens, features] are wanted")
+            return out
+        rows = ctx.workspace.rows("mx_rows", shape[0], w.k)
+    if (bias is not None) + (act is not None) + (w2 is not None) + add > 1 or (form is not None and w2 is None):
+        raise KernelError("microscaled.product: a bias, an activation, a gate and an addition are not combined")
     constants = bias if bias is not None else ops.whole_act_form(act) if act is not None else ops.whole_gate_form(form) if form is not None else None
-    rows = ctx.workspace.rows("mx_rows", x.shape[0], w.k) if plain else x
     held = type(out) is Rows
-    native("mx_product")(x if plain else None, rows.native, w.native, 0 if w2 is None else w2.native, constants, act is not None, add,
-                         None if held else out, out.native if held else 0, _status_address())
+    native("mx_product")(x, rows.native, w.native, 0 if w2 is None else w2.native, constants, act is not None, add, None if held else out,
+                         out.native if held else 0, _status_address())
     return out
 
 

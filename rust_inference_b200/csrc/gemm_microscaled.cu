@@ -205,10 +205,11 @@ __device__ __forceinline__ void store_lanes(const Result& r, T t, G good, int f,
 }
 
 // Plain rows that a kernel for few tokens brings to 8 bits itself: those whose spans all have a stage of the ring, up to 4 of them, and up to
-// PLAIN_MOST where K is not cut or a CTA has no more than 32 spans of all rows together.  The epilogue's warps, which have nothing else to do then, read
-// them and write codes and exponents as TMA would have brought them.  (us, plain rows / by a kernel before: [3584, 3584], 7 spans a CTA, 1 token
-// 5.1 / 6.4, 4 tokens 5.5 / 5.9, 8 tokens 6.0 / 5.75; [2048, 2048], 4 spans, 8 tokens 4.5 / 4.95; [896, 896], uncut, 8 tokens 4.05 / 4.2.)
-constexpr int PLAIN_MOST = 8;
+// PLAIN_MOST where a CTA has no more than 32 spans of all rows together (64 where K is not cut).  The epilogue's warps, which have nothing else to do
+// then, read them and write codes and exponents as TMA would have brought them.  (us, plain rows / by a kernel before: [3584, 3584], 7 spans a CTA,
+// 1 token 5.1 / 6.4, 4 tokens 5.5 / 5.9, 8 tokens 6.0 / 5.75; [1536, 1536], 2 spans, 16 tokens 4.4 / 5.0; [896, 896], 7 spans, uncut, 8 tokens
+// 4.05 / 4.2, 16 tokens 5.2 / 4.4.)
+constexpr int PLAIN_MOST = 16;
 struct PlainRows {
     const void* at;              // null: rows in 8 bits come by TMA
     int f32, k;
@@ -1050,7 +1051,7 @@ int launch_feature(const Call& c) {
     size_t smem = (apart ? ring + recv : ring > (size_t)recv ? ring : (size_t)recv) + 1024;
     long long ctas = tiles * p.cluster;
     if (p.cluster == 1 && ctas > sm_count()) ctas = sm_count();
-    if (c.plain.at != nullptr && (stages < most || ctas < tiles || (c.n_tok > 4 && p.cluster > 1 && most * c.n_tok > 32))) return NEEDS_ROWS;
+    if (c.plain.at != nullptr && (stages < most || ctas < tiles || (c.n_tok > 4 && most * c.n_tok > (p.cluster > 1 ? 32 : 64)))) return NEEDS_ROWS;
     // two accumulators, so that a tile's epilogue runs beside the next one's MMAs, where a CTA has several tiles and the columns suffice
     constexpr int EXP_COLS = 2 * (MATS + 1) * 4;
     const int one = MATS * p.tn + EXP_COLS, two = one + MATS * p.tn;

@@ -24,15 +24,15 @@ template <> struct Sized<2> { using type = uint16_t; };
 template <typename T> struct Eight;
 template <> struct alignas(16) Eight<float> {
     float v[8];
-    // from column c on of a row of k; zeros behind its end
-    template <bool WHOLE> __device__ __forceinline__ void load(const float* row, int c, int k) {
-        if (WHOLE && c < k) {
+    // from column c on of a row of k, in whole eights on 16-byte boundaries; zeros behind its end
+    __device__ __forceinline__ void load(const float* row, int c, int k) {
+        if (c < k) {
             const float4 a = load_written(row + c), b = load_written(row + c + 4);
             v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
             v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = !WHOLE && c + i < k ? const_cast<const volatile float*>(row)[c + i] : 0.f;
+            for (int i = 0; i < 8; ++i) v[i] = 0.f;
         }
     }
     // the largest magnitude, as a float's bits (a NaN's are larger than any number's)
@@ -50,17 +50,13 @@ template <> struct alignas(16) Eight<float> {
 };
 template <> struct alignas(16) Eight<__nv_bfloat16> {
     uint32_t w[4];
-    template <bool WHOLE> __device__ __forceinline__ void load(const __nv_bfloat16* row, int c, int k) {
-        if (WHOLE && c < k) {
+    __device__ __forceinline__ void load(const __nv_bfloat16* row, int c, int k) {
+        if (c < k) {
             const float4 a = load_written(reinterpret_cast<const float*>(row + c));
             w[0] = __float_as_uint(a.x); w[1] = __float_as_uint(a.y); w[2] = __float_as_uint(a.z); w[3] = __float_as_uint(a.w);
         } else {
-            const volatile uint16_t* at = reinterpret_cast<const volatile uint16_t*>(row);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t lo = !WHOLE && c + 2 * i < k ? at[c + 2 * i] : 0u, hi = !WHOLE && c + 2 * i + 1 < k ? at[c + 2 * i + 1] : 0u;
-                w[i] = lo | hi << 16;
-            }
+            for (int i = 0; i < 4; ++i) w[i] = 0u;
         }
     }
     __device__ __forceinline__ uint32_t top() const {
@@ -94,12 +90,29 @@ __device__ __forceinline__ uint32_t block_top(uint32_t top) {
     return max(top, __shfl_xor_sync(four, top, 2));
 }
 
+// Rows that are no whole eights on 16-byte boundaries: a warp reads (and writes) 32 neighbouring numbers at a time, eight times, and they change places
+// in its part of shared memory, `room`, so that each thread has eight in a row.  ([3584, 18945] bfloat16 to 4 bits 71 -> 51 us and back 193 -> 40;
+// the norm of 2,047 rows of 4,097 56 -> 34 us.)
+template <typename T> using Bits = typename Sized<sizeof(T)>::type;
+template <typename T>
+__device__ __forceinline__ void read_apart(const T* row, int c, int k, Bits<T>* raw) {                // c: the first of this thread's numbers
+#pragma unroll
+    for (int q = 0; q < 8; ++q) raw[q] = c + q * 32 < k ? reinterpret_cast<const volatile Bits<T>*>(row)[c + q * 32] : (Bits<T>)0;
+}
+template <typename T>
+__device__ __forceinline__ void gather(Bits<T>* room, int lane, const Bits<T>* raw, Eight<T>& v) {
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 8; ++q) room[q * 32 + lane] = raw[q];
+    __syncwarp();
+    v = *reinterpret_cast<const Eight<T>*>(room + lane * 8);
+}
+
 // A warp takes a part of a row, GROUPS times 256 numbers, whose reads are on their way together: four where there is much to do, else one.
 template <typename T, int BITS, bool WHOLE, int GROUPS>
 __global__ void __launch_bounds__(THREADS) hold_kernel(const T* x, int n, int k, long long ld, int n_spans, uint32_t parts, uint32_t items, uint8_t* codes,
                                                        uint8_t* exponents) {
-    using Bits = typename Sized<sizeof(T)>::type;
-    __shared__ alignas(32) Bits room[WHOLE ? 1 : THREADS / 32][256];
+    __shared__ alignas(16) Bits<T> room[WHOLE ? 1 : THREADS / 32][256];
     if (BITS == 8) let_next_kernel_start();                 // (a matrix: see `settle`)
     wait_for_previous_kernels();
     const int lane = threadIdx.x & 31;
@@ -120,26 +133,13 @@ __global__ void __launch_bounds__(THREADS) hold_kernel(const T* x, int n, int k,
         Eight<T> v[GROUPS];
         if (WHOLE) {
 #pragma unroll
-            for (int i = 0; i < GROUPS; ++i) v[i].template load<true>(from, c0 + i * 256, k);
+            for (int i = 0; i < GROUPS; ++i) v[i].load(from, c0 + i * 256, k);
         } else {
-            // one number of 32 neighbouring ones at a time, which change places in shared memory ([3584, 18945] bfloat16 71 -> 51 us, float32 121 -> 60)
-            Bits raw[GROUPS][8];
-            const int first = c0 - lane * 8 + lane;
+            Bits<T> raw[GROUPS][8];
 #pragma unroll
-            for (int i = 0; i < GROUPS; ++i)
+            for (int i = 0; i < GROUPS; ++i) read_apart(from, c0 - lane * 7 + i * 256, k, raw[i]);
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const int c = first + i * 256 + q * 32;
-                    raw[i][q] = c < k ? reinterpret_cast<const volatile Bits*>(from)[c] : (Bits)0;
-                }
-#pragma unroll
-            for (int i = 0; i < GROUPS; ++i) {
-                __syncwarp();
-#pragma unroll
-                for (int q = 0; q < 8; ++q) room[threadIdx.x >> 5][q * 32 + lane] = raw[i][q];
-                __syncwarp();
-                v[i] = *reinterpret_cast<const Eight<T>*>(&room[threadIdx.x >> 5][lane * 8]);
-            }
+            for (int i = 0; i < GROUPS; ++i) gather(room[threadIdx.x >> 5], lane, raw[i], v[i]);
         }
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
@@ -160,8 +160,7 @@ template <typename T> struct Sixteen { static constexpr int N = 16 / sizeof(T); 
 template <typename T, int BITS, bool WHOLE, int GROUPS>
 __global__ void __launch_bounds__(THREADS) values_kernel(const uint8_t* codes, const uint8_t* exponents, int k, int n_spans, uint32_t parts, uint32_t items, T* out) {
     constexpr int N = Sixteen<T>::N, BYTES = N * BITS / 8;          // numbers of a thread, and bytes of their codes: 2, 4 or 8
-    using Bits = typename Sized<sizeof(T)>::type;
-    __shared__ alignas(16) Bits room[WHOLE ? 1 : THREADS / 32][32 * N];
+    __shared__ alignas(16) Bits<T> room[WHOLE ? 1 : THREADS / 32][32 * N];
     let_next_kernel_start();
     wait_for_previous_kernels();
     const int lane = threadIdx.x & 31;
@@ -205,11 +204,11 @@ __global__ void __launch_bounds__(THREADS) values_kernel(const uint8_t* codes, c
             T* dst = to + i * 32 * N;
             if (WHOLE) {
                 *reinterpret_cast<uint4*>(dst) = r;
-            } else {                                  // (as the reads of numbers that lie so: bfloat16 193 -> 40 us)
+            } else {
                 __syncwarp();
                 *reinterpret_cast<uint4*>(&room[threadIdx.x >> 5][lane * N]) = r;
                 __syncwarp();
-                Bits* line = reinterpret_cast<Bits*>(dst) - lane * N;
+                Bits<T>* line = reinterpret_cast<Bits<T>*>(dst) - lane * N;
 #pragma unroll
                 for (int q = 0; q < N; ++q)
                     if (c - lane * N + q * 32 + lane < k) line[q * 32 + lane] = room[threadIdx.x >> 5][q * 32 + lane];
@@ -235,19 +234,32 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512, HELD == 1 ? 1 : 2) rms
                                                                                             int n_spans, double inverse, double eps, uint8_t* codes,
                                                                                             uint8_t* exponents) {
     __shared__ double sums[32];
+    __shared__ alignas(16) uint32_t rooms[WHOLE ? 1 : HELD == 1 ? 32 : 16][256];
     constexpr uint32_t NEAR = 4;
     let_next_kernel_start();
     const int tid = threadIdx.x, threads = blockDim.x, groups = n_spans * (SPAN / 8);
     const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
+    uint32_t* room = rooms[WHOLE ? 0 : warp];
+    // the groups of a row that a thread has; where they change places, those that its warp has
+    auto there = [&](int g) { return (WHOLE ? g : g - lane) < groups; };
     auto weights = [&](int g, float* w) {
         const int c = g * 8;
-        if (WHOLE && c < k) {
-            const float4 a = *reinterpret_cast<const float4*>(weight + c), b = *reinterpret_cast<const float4*>(weight + c + 4);
-            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-            w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-        } else {
+        if (WHOLE) {
+            if (c < k) {
+                const float4 a = *reinterpret_cast<const float4*>(weight + c), b = *reinterpret_cast<const float4*>(weight + c + 4);
+                w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+                w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = !WHOLE && c + i < k ? weight[c + i] : 0.f;
+                for (int i = 0; i < 8; ++i) w[i] = 0.f;
+            }
+        } else {
+            uint32_t raw[8];
+            Eight<float> e;
+            read_apart(weight, c - lane * 7, k, raw);
+            gather(room, lane, raw, e);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = e.v[i];
         }
     };
     auto join = [&](Eight<float>& v, const Eight<B>& b) {
@@ -262,12 +274,19 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512, HELD == 1 ? 1 : 2) rms
     wait_for_previous_kernels();
     const int row = blockIdx.x;
     auto read = [&](int g, Eight<float>& v) {
-        v.template load<WHOLE>(stream + (size_t)row * k, g * 8, k);
-        if (branch != nullptr) {
-            Eight<B> b;
-            b.template load<WHOLE>(branch + (size_t)row * k, g * 8, k);
-            join(v, b);
+        Eight<B> b;
+        if (WHOLE) {
+            v.load(stream + (size_t)row * k, g * 8, k);
+            if (branch != nullptr) b.load(branch + (size_t)row * k, g * 8, k);
+        } else {
+            uint32_t raw[8];
+            Bits<B> more[8];
+            read_apart(stream + (size_t)row * k, g * 8 - lane * 7, k, raw);
+            if (branch != nullptr) read_apart(branch + (size_t)row * k, g * 8 - lane * 7, k, more);
+            gather(room, lane, raw, v);
+            if (branch != nullptr) gather(reinterpret_cast<Bits<B>*>(room), lane, more, b);
         }
+        if (branch != nullptr) join(v, b);
     };
     double sum = 0.0, more = 0.0;
     auto square = [&](const Eight<float>& v) {
@@ -281,14 +300,14 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512, HELD == 1 ? 1 : 2) rms
     float w[HELD][8];
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
-        if (tid + h * threads < groups) read(tid + h * threads, held[h]);
+        if (there(tid + h * threads)) read(tid + h * threads, held[h]);
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
-        if (tid + h * threads < groups) {
+        if (there(tid + h * threads)) {
             weights(tid + h * threads, w[h]);
             square(held[h]);
         }
-    for (int g = tid + HELD * threads; g < groups; g += threads) {
+    for (int g = tid + HELD * threads; there(g); g += threads) {
         Eight<float> v;
         read(g, v);
         square(v);
@@ -314,9 +333,12 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512, HELD == 1 ? 1 : 2) rms
                     reinterpret_cast<float4*>(to)[1] = make_float4(v.v[4], v.v[5], v.v[6], v.v[7]);
                 }
             } else {
+                __syncwarp();
+                *reinterpret_cast<Eight<float>*>(room + lane * 8) = v;
+                __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (c + i < k) to[i] = v.v[i];
+                for (int q = 0; q < 8; ++q)
+                    if (c - lane * 7 + q * 32 < k) to[q * 32 - lane * 7] = __uint_as_float(room[q * 32 + lane]);
             }
         }
         Eight<float> y;
@@ -348,13 +370,14 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512, HELD == 1 ? 1 : 2) rms
                 y.scaled(byte, z);
             }
         }
+        if (!WHOLE && g >= groups) return;
         *reinterpret_cast<uint2*>(codes + (size_t)row * n_spans * SPAN + c) = make_uint2(eight_bits(z), eight_bits(z + 4));
         if ((c & 31) == 0) exponents[exponent_at(row, c >> 5, n_spans)] = (uint8_t)byte;
     };
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
-        if (tid + h * threads < groups) finish(tid + h * threads, held[h], w[h]);
-    for (int g = tid + HELD * threads; g < groups; g += threads) {
+        if (there(tid + h * threads)) finish(tid + h * threads, held[h], w[h]);
+    for (int g = tid + HELD * threads; there(g); g += threads) {
         Eight<float> v;
         float by[8];
         read(g, v);

@@ -577,3 +577,30 @@ def test_more_numbers_than_31_bits_count():
     assert torch.equal(microscaled.values(rows, torch.bfloat16)[-77:], microscaled.values(again, torch.bfloat16))
     assert torch.equal(stream[-77:], wide[-77:].float() * 2)
     check_status()
+
+
+@pytest.mark.parametrize("n,k", [(2, 8191), (3, 8321), (2, 20001), (400, 129), (400, 4099), (310, 9003)])
+def test_norm_of_odd_rows_longer_than_a_block_holds(n, k):
+    """Rows off every boundary, the second part of which is read again; nothing behind the last row is written."""
+    from rust_inference_b200.kernels import microscaled
+    for branch in (None, torch.bfloat16, torch.float32):
+        test_norm(n, k, branch)
+    g = gen(n + k)
+    room = torch.full((n * k + 64,), 7.0, device=DEV)
+    stream = room[1:n * k + 1].view(n, k)                      # 4 bytes off a boundary
+    x, b, w = torch.randn(n, k, generator=g), torch.randn(n, k, generator=g).bfloat16(), 1 + 0.1 * torch.randn(k, generator=g)
+    stream.copy_(x)
+    a, e = microscaled.Rows.sizes(n, k)
+    codes, exponents = torch.full((a + 64,), 9, dtype=torch.uint8, device=DEV), torch.full((e + 64,), 9, dtype=torch.uint8, device=DEV)
+    rows = microscaled.Rows(n, k, codes=codes, exponents=exponents)
+    microscaled.rmsnorm(stream, w.to(DEV), 1e-5, rows, branch=b.to(DEV), total=stream)
+    want, y = plain.rmsnorm(x, b, w, 1e-5)
+    assert torch.equal(stream.cpu(), want) and room[0] == 7.0 and (room[n * k + 1:] == 7.0).all() and (codes[a:] == 9).all() and (exponents[e:] == 9).all()
+    near = plain.nearest(y, plain.EIGHT)
+    assert ((microscaled.values(rows).double().cpu() - y).abs() <= (near - y).abs() + 2.0 ** -22 * y.abs()).all()
+    # the same memory for holding and reading back
+    held = microscaled.quantize(stream, rows)
+    out = torch.full((n * k + 64,), 5.0, device=DEV)
+    microscaled.values(held, torch.float32, out=out[3:n * k + 3].view(n, k))
+    assert torch.equal(out[3:n * k + 3].view(n, k).double().cpu(), plain.nearest(want, plain.EIGHT)) and (out[:3] == 5.0).all() and (out[n * k + 3:] == 5.0).all()
+    assert (codes[a:] == 9).all() and (exponents[e:] == 9).all()

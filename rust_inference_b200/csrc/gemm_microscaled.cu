@@ -608,12 +608,16 @@ __device__ __forceinline__ uint32_t piece_at(uint32_t room, int token, int piece
     return room + (uint32_t)(token * pieces + (piece ^ (token * pieces / 8 & (pieces - 1)))) * 16u;
 }
 template <int PIECES>
-__device__ __forceinline__ void exchange(uint32_t room, int lane, uint4* c) {
+__device__ __forceinline__ void spread(uint32_t room, int lane, const uint4* c) {
     __syncwarp();
 #pragma unroll
     for (int q = 0; q < PIECES; ++q)
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece_at(room, lane, q, PIECES)), "r"(c[q].x), "r"(c[q].y), "r"(c[q].z), "r"(c[q].w) : "memory");
     __syncwarp();
+}
+template <int PIECES>
+__device__ __forceinline__ void exchange(uint32_t room, int lane, uint4* c) {
+    spread<PIECES>(room, lane, c);
 #pragma unroll
     for (int q = 0; q < PIECES; ++q)
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(c[q].x), "=r"(c[q].y), "=r"(c[q].z), "=r"(c[q].w)
@@ -680,15 +684,37 @@ __device__ __forceinline__ void store_run(const Result& r, int t, int tokens, in
         }
         return;
     }
-    if (lane >= tokens) return;
-    const size_t at = (size_t)(t + lane) * n_feat + f;
+    // rows off a 16-byte boundary, or the last features: a number at a time, those of neighbouring features together (2,048 tokens of [4606, 3584],
+    // float32 sums: 157 -> 35 us)
+    if constexpr (OUT == OUT_BF16) {
+        uint4 c[4];
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-        if (f + j < n_feat) {
-            if (OUT == OUT_BF16) reinterpret_cast<__nv_bfloat16*>(r.out)[at + j] = __float2bfloat16_rn(v[j]);
-            else if (OUT == OUT_F32) reinterpret_cast<float*>(r.out)[at + j] = v[j];
-            else atomicAdd(reinterpret_cast<float*>(r.out) + at + j, v[j]);
+        for (int q = 0; q < 4; ++q) c[q] = pack8(v + 8 * q);
+        spread<4>(room, lane, c);
+        uint16_t* to = reinterpret_cast<uint16_t*>(r.out) + (size_t)t * n_feat + f + lane;
+#pragma unroll 8
+        for (int row = 0; row < 32; ++row) {
+            uint16_t y;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(piece_at(room, row, lane / 8, 4) + lane % 8 * 2) : "memory");
+            if (row < tokens && f + lane < n_feat) to[(size_t)row * n_feat] = y;
         }
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {                                                 // sixteen features of two tokens
+            spread<4>(room, lane, reinterpret_cast<const uint4*>(v + 16 * h));
+            const int at = f + 16 * h + lane % 16;
+            float* to = reinterpret_cast<float*>(r.out) + (size_t)(t + lane / 16) * n_feat + at;
+#pragma unroll 8
+            for (int row = lane / 16; row < 32; row += 2, to += (size_t)2 * n_feat) {
+                float y;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(piece_at(room, row, lane % 16 / 4, 4) + lane % 4 * 4) : "memory");
+                if (row < tokens && at < n_feat) {
+                    if (OUT == OUT_ADD) atomicAdd(to, y);
+                    else *to = y;
+                }
+            }
+        }
+    }
 }
 
 template <bool DUAL, int OUT>
@@ -858,7 +884,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             for (int n = half; n < RUNS; n += 2) {
                 // the first accumulator shares its last columns, the second its first: those are read in the first turn
                 const int c = ((i & 1) ? n : RUNS - 1 - n) * 32, f = f0 + c;
-                float v[32], u[DUAL ? 32 : 1];
+                alignas(16) float v[32], u[DUAL ? 32 : 1];
                 if (!DUAL || (i & 1)) tmem_ld32(trow + c, reinterpret_cast<uint32_t*>(v));
                 else tmem_ld32(trow + ROWS + c, reinterpret_cast<uint32_t*>(u));
                 if (n == half) {

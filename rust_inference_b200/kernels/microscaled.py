@@ -196,9 +196,15 @@ def product(x, w: Matrix, out, ctx, *, w2: Matrix | None = None, bias=None, form
         raise KernelError("microscaled.product: a bias, an activation, a gate and an addition are not combined")
     constants = bias if bias is not None else ops.whole_act_form(act) if act is not None else ops.whole_gate_form(form) if form is not None else None
     held = type(out) is Rows
-    native("mx_product")(x, rows.native, w.native, 0 if w2 is None else w2.native, constants, act is not None, add, None if held else out,
+    _product()(x, rows.native, w.native, 0 if w2 is None else w2.native, constants, act is not None, add, None if held else out,
                          out.native if held else 0, _status_address())
     return out
+
+
+@functools.lru_cache(maxsize=None)
+def _product():
+    native("mx_hold")                                            # brings plain rows to 8 bits where the product does not
+    return native("mx_product")
 
 
 @functools.lru_cache(maxsize=None)

@@ -604,3 +604,19 @@ def test_norm_of_odd_rows_longer_than_a_block_holds(n, k):
     microscaled.values(held, torch.float32, out=out[3:n * k + 3].view(n, k))
     assert torch.equal(out[3:n * k + 3].view(n, k).double().cpu(), plain.nearest(want, plain.EIGHT)) and (out[:3] == 5.0).all() and (out[n * k + 3:] == 5.0).all()
     assert (codes[a:] == 9).all() and (exponents[e:] == 9).all()
+
+
+@pytest.mark.parametrize("call", ["linear.project(torch.ones(20, 64, dtype=torch.bfloat16, device='cuda'), w, torch.empty(20, 8, dtype=torch.bfloat16, device='cuda'), ctx)",
+                                  "microscaled.values(w)", "microscaled.quantize(torch.ones(3, 7, device='cuda'))",
+                                  "microscaled.rmsnorm(torch.ones(2, 64, device='cuda'), torch.ones(64, device='cuda'), 1e-6, microscaled.Rows(2, 64))"])
+def test_each_call_as_a_process_first_one(call):
+    """A matrix from a file's codes, and then any of the others: nothing has to have been called before."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = ("import sys; sys.path[:0] = [%r, %r]\nimport torch\nfrom test_microscaled_gpu import context\n"
+            "from rust_inference_b200.kernels import linear, microscaled\nctx = context()\n"
+            "w = microscaled.Matrix.of_codes(torch.full((8, 32), 34, dtype=torch.uint8, device='cuda'), torch.full((8, 2), 127, dtype=torch.uint8, device='cuda'), 64)\n"
+            "%s\ntorch.cuda.synchronize()\n" % (os.path.dirname(here), here, call))
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)

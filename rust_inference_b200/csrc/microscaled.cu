@@ -5,7 +5,7 @@
 //   ri_mx_rmsnorm  total = stream + branch;  rows in 8 bits of  total / sqrt(mean(total^2) + eps) * weight
 //
 // All are bound by memory: [3584, 18944] from bfloat16 to 4 bits 36.5 us (4.7 TB/s), back 31.9 (5.4); the norm of 2,047 rows of 4,096 with a bfloat16
-// branch and the total 22.6 us (4.1; reading, one sum, writing, 3.5 rounds of blocks), of one row of 896 1.5, of 8 of 3,584 2.9: trips.
+// branch and the total 21.9 us (4.2; reading, one sum, writing, 3.5 rounds of blocks), of one row of 896 1.5, of 8 of 3,584 2.9: trips.
 // A thread has eight consecutive numbers of a row (16 or 32 bytes in, 4 or 8 out), four neighbouring threads a block, whose largest magnitude two
 // exchanges find.
 #include "microscaled.cuh"

@@ -117,6 +117,19 @@ __device__ __forceinline__ GateForm load_gate_form(const float* p) {
     return f;
 }
 
+// A gate's clamps: the smaller and the larger of two numbers, and a NaN where one of them is (fminf and fmaxf give the other one, so that a NaN would
+// come out of a bounded gate as an ordinary number).
+__device__ __forceinline__ float at_most(float x, float limit) {
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(limit));
+    return y;
+}
+__device__ __forceinline__ float at_least(float x, float limit) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(limit));
+    return y;
+}
+
 // An activation of one argument (epilogue 4 of the contractions, and a kernel of its own):
 //   act(z) = a_p z^2 + l z for z > 0,   a_n (e^z - 1 - z) + l z otherwise.
 // Four floats {p, q, l, fixed} in device memory.  fixed = 0: a learned form, a_p = softplus(p), a_n = 1/2 + softplus(q)
@@ -157,8 +170,8 @@ __device__ __forceinline__ float silu_f32(float x) {
 
 // The gated activation with accurate exponentials (the 32-bit path); alpha 1 without limit and shift is silu_f32(g) * u.
 __device__ __forceinline__ float gated_f32(float g, float u, const GateForm& f) {
-    g = fminf(g, f.limit);
-    u = fmaxf(fminf(u, f.limit), -f.limit) + f.shift;
+    g = at_most(g, f.limit);
+    u = at_least(at_most(u, f.limit), -f.limit) + f.shift;
     if (f.alpha == 1.f && f.cubic == 0.f) return silu_f32(g) * u * f.mult;
     const float z = f.alpha * g * fmaf(f.cubic * g, g, 1.f), e = expf(-fabsf(z));
     const float sig = (z >= 0.f ? 1.f : e) / (1.f + e);

@@ -134,8 +134,8 @@ __device__ __forceinline__ Epilogue load_epilogue(const float* constants, int ac
     return e;
 }
 __device__ __forceinline__ float gated_quick(float g, float u, const GateForm& f) {
-    g = fminf(g, f.limit);
-    u = fmaxf(fminf(u, f.limit), -f.limit) + f.shift;
+    g = at_most(g, f.limit);
+    u = at_least(at_most(u, f.limit), -f.limit) + f.shift;
     return __fdividef(g, 1.f + __expf(-f.alpha * g * fmaf(f.cubic * g, g, 1.f))) * u * f.mult;
 }
 // the same with the constants of silu

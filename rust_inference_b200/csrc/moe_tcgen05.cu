@@ -38,8 +38,8 @@ enum Status { ST_PRODUCER_TIMEOUT = 31, ST_MMA_TIMEOUT = 32, ST_EPILOGUE_TIMEOUT
 // The gate of the gated form (`GateForm`, common.cuh; without constants SiLU(g) * u, bit for bit), with the hardware's
 // fast exponential and division: the result is rounded to bf16 right away.
 __device__ __forceinline__ float gated_to_bf16(float g, float u, const GateForm& f) {
-    g = fminf(g, f.limit);
-    u = fmaxf(fminf(u, f.limit), -f.limit) + f.shift;
+    g = at_most(g, f.limit);
+    u = at_least(at_most(u, f.limit), -f.limit) + f.shift;
     return __fdividef(g, 1.f + __expf(-f.alpha * g * fmaf(f.cubic * g, g, 1.f))) * u * f.mult;
 }
 

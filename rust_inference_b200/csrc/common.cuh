@@ -173,7 +173,7 @@ __device__ __forceinline__ float gated_f32(float g, float u, const GateForm& f) 
     g = at_most(g, f.limit);
     u = at_least(at_most(u, f.limit), -f.limit) + f.shift;
     if (f.alpha == 1.f && f.cubic == 0.f) return silu_f32(g) * u * f.mult;
-    const float z = f.alpha * g * fmaf(f.cubic * g, g, 1.f), e = expf(-fabsf(z));
+    const float z = f.alpha * g * (f.cubic == 0.f ? 1.f : fmaf(f.cubic * g, g, 1.f)), e = expf(-fabsf(z));      // (0 times an infinite gate is none)
     const float sig = (z >= 0.f ? 1.f : e) / (1.f + e);
     return g * sig * u * f.mult;
 }

@@ -136,7 +136,8 @@ __device__ __forceinline__ Epilogue load_epilogue(const float* constants, int ac
 __device__ __forceinline__ float gated_quick(float g, float u, const GateForm& f) {
     g = at_most(g, f.limit);
     u = at_least(at_most(u, f.limit), -f.limit) + f.shift;
-    return __fdividef(g, 1.f + __expf(-f.alpha * g * fmaf(f.cubic * g, g, 1.f))) * u * f.mult;
+    const float inner = f.cubic == 0.f ? 1.f : fmaf(f.cubic * g, g, 1.f);          // (0 times an infinite gate is none)
+    return __fdividef(g, 1.f + __expf(-f.alpha * g * inner)) * u * f.mult;
 }
 // the same with the constants of silu
 __device__ __forceinline__ float silu_quick(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }

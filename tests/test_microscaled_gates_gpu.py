@@ -80,3 +80,26 @@ def test_a_nan_in_either_factor_of_a_plain_gate(m, form):
         linear.gated(x.to(DEV, dtype), *(linear.Weight(w.to(DEV, dtype)) for w in (wg, wu)), out, context(dtype), form=form_of(form))
         assert torch.equal(torch.isnan(out).cpu(), bad)
     check_status()
+
+
+@pytest.mark.parametrize("form", ["silu", "gelu", "steep"])
+@pytest.mark.parametrize("m", [2, 130, 300])
+def test_an_infinite_gate(one_kernel, m, form):
+    """Sums beyond float32's numbers: an infinite gate times a factor is infinite, whichever kernel computes it and whatever it writes."""
+    from rust_inference_b200.kernels import linear, microscaled, ops
+    k, n = 64, 160
+    x = torch.ones(m, k)
+    x[1] = 2.0 ** 100
+    wg, wu = torch.ones(n, k), torch.ones(n, k) * 2.0 ** -90
+    wg[40] = 2.0 ** 100                                    # token 1: 64 2^200
+    f = ops.gate_form(alpha=1.702, device=DEV) if form == "steep" else form_of(form)
+    held = [microscaled.Matrix.of(w.to(DEV)) for w in (wg, wu)]
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.zeros(m, n, dtype=dtype, device=DEV)
+        linear.gated(x.to(DEV), *held, out, context(dtype), form=f)
+        assert float(out[1, 40]) == INF and torch.isfinite(out[0]).all() and torch.isfinite(out[1, :40]).all() and torch.isfinite(out[1, 41:]).all()
+    rows = microscaled.Rows(m, n)
+    linear.gated(x.to(DEV), *held, rows, context(), form=f)
+    got = torch.isnan(microscaled.values(rows)).cpu()
+    assert got[1, 32:64].all() and not got[0].any() and not got[1, :32].any() and not got[1, 64:].any()
+    check_status()

@@ -217,13 +217,12 @@ __global__ void __launch_bounds__(THREADS) values_kernel(const uint8_t* codes, c
     }
 }
 
-// A double as the float towards zero, its last bit set where that is not the double: rounded again to fewer bits it becomes what the double
-// would.  0 below 2^-126.
+// A double as the float towards zero, its last bit set where that is not the double: rounded again to fewer bits it becomes what the double would.
 __device__ __forceinline__ uint32_t to_odd(double y) {
-    const uint32_t hi = (uint32_t)__double2hiint(y), lo = (uint32_t)__double2loint(y), mag = hi & 0x7fffffffu;
-    const uint32_t bits = (mag - (896u << 20)) << 3 | lo >> 29 | ((lo & 0x1fffffffu) != 0u ? 1u : 0u);
-    const uint32_t fine = mag < (897u << 20) ? 0u : mag >= (1151u << 20) ? (mag > 0x7ff00000u || (mag == 0x7ff00000u && lo != 0u) ? 0x7fc00000u : 0x7f800000u) : bits;
-    return fine | (hi & 0x80000000u);
+    const float f = __double2float_rz(y);
+    const uint32_t bits = __float_as_uint(f);
+    if (fabs(y) >= 0x1p128) return (bits & 0x80000000u) | 0x7f800000u;
+    return bits | ((double)f != y ? 1u : 0u);            // (a NaN too)
 }
 
 // A block of threads per row.  Results are what the formula in 64 bits, rounded once, gives: what lies next to the middle of two numbers falls as the
@@ -324,6 +323,7 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512, HELD == 1 ? 1 : 2) rms
     for (int o = over >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     const double r = rsqrt(s * inverse + eps);
     const float r32 = (float)r;
+    const bool fine = r32 >= 0x1p-126f;
     auto finish = [&](int g, const Eight<float>& v, const float* by) {
         const int c = g * 8;
         if (total != nullptr) {
@@ -348,12 +348,18 @@ __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512, HELD == 1 ? 1 : 2) rms
             for (int i = 0; i < 8; ++i) y.v[i] = __uint_as_float(to_odd((double)v.v[i] * r * (double)by[i]));
         };
         // In 32 bits first, which is off by three units in the last place at most: that decides, but next to where the exponent or a code changes
-        // (one block in 10^5, and one eight in 700, most of these for numbers below the type's 2^-6).
+        // (one block in 10^5, and one eight in 700, most of these for numbers below the type's 2^-6), and where a factor may be no normal number: with an
+        // inverse root or a weight out of the ordinary, and in blocks of nothing above 2^-47 (numbers from the type's 2^-6 on are 2^-15 of the largest at
+        // least, so that v r32 is 2^-62 over a weight below 2^64).
+        float heavy = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y.v[i] = v.v[i] * r32 * by[i];
-        uint32_t top = block_top(y.top()), byte = exponent_byte<8>(top);
+        for (int i = 0; i < 8; ++i) {
+            y.v[i] = v.v[i] * r32 * by[i];
+            heavy = fmaxf(heavy, fabsf(by[i]));
+        }
+        uint32_t top = block_top(fine && heavy < 0x1p64f ? y.top() : 0x7f800000u), byte = exponent_byte<8>(top);
         float z[8];
-        if (top != 0u && ((top & 0x7fffffu) - (0x600000u - NEAR) <= 2u * NEAR || (top >> 23) - 16u > 222u)) {  // (the same for a block's four threads)
+        if ((top & 0x7fffffu) - (0x600000u - NEAR) <= 2u * NEAR || (top >> 23) - 80u > 158u) {  // (the same for a block's four threads)
             exact();
             byte = exponent_byte<8>(block_top(y.top()));
             y.scaled(byte, z);

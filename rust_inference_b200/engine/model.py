@@ -7,10 +7,22 @@ architecture: which parts a layer has and in which order layers run comes from t
 """
 from __future__ import annotations
 
+import contextlib
+import functools
+
 import torch
 
 from ..parts.registry import lookup
 from ..parts.spec import ModelSpec, TensorSpec
+
+
+def _on_its_device(method):
+    """With the model's device as the current one, which is where kernels run: a model may lie on another."""
+    @functools.wraps(method)
+    def call(self, *args, **kw):
+        with torch.cuda.device(self.device) if self.device.type == "cuda" else contextlib.nullcontext():
+            return method(self, *args, **kw)
+    return call
 
 
 def _build(category: str, part_spec, *, hidden_size, dtype, device):
@@ -172,6 +184,7 @@ class DecoderModel:
             return t.to(device=self.device, dtype=torch.int32).contiguous()
         raise ValueError(f"unknown tensor role {ts.role!r}")
 
+    @_on_its_device
     def load(self, named_tensors) -> None:
         """Takes (name, tensor) pairs covering `declared_tensors()` and hands each part its own."""
         declared = self.declared_tensors()
@@ -205,6 +218,7 @@ class DecoderModel:
                 raise ValueError("the head is tied to the embedding, which has no table to share")
             self.head.tie(table)                          # the same storage, no copy
 
+    @_on_its_device
     def state_dict(self) -> dict:
         """Every tensor of the model under the name the weight file gives it, as the model holds it
         on the device (matrices in the run dtype, vectors float32): what the parts packed together

@@ -1136,6 +1136,12 @@ RI_API int ri_mx_product(void* x_held, const void* x_plain, int x_dtype, long lo
                          int* status, cudaStream_t stream) {
     Held *x = (Held*)x_held, *w = (Held*)w_held, *w2 = (Held*)w2_held, *to = (Held*)out_held;
     const long long n_tok = x->n;
+    // (other CTAs read their rows and matrices while the first ones write)
+    const long long out_bytes = out ? out_rows * out_cols * item_bytes(out_dtype) : 0, plain_bytes = x_plain ? ((x_rows - 1) * x_ld + x_cols) * item_bytes(x_dtype) : 0;
+    auto from_result = [&](const Held* h) { return h == nullptr || (to ? apart(h, to) : apart(h, out, out_bytes)); };
+    auto from_result_bytes = [&](const void* p, long long bytes) { return to ? apart(to, p, bytes) : apart(out, out_bytes, p, bytes); };
+    if (!from_result(x) || !from_result(w) || !from_result(w2) || !from_result_bytes(x_plain, plain_bytes) || !from_result_bytes(constants, 4 * n_constants))
+        return fail("gemm_microscaled: the result must lie apart from the rows, the matrices and the constants");
     int device = -1;
     if (cudaGetDevice(&device) != cudaSuccess || x->device != device || w->device != device || (w2 && w2->device != device) || (to && to->device != device))
         return fail("gemm_microscaled: rows and matrices lie on the current device");
@@ -1144,7 +1150,6 @@ RI_API int ri_mx_product(void* x_held, const void* x_plain, int x_dtype, long lo
     if (x_plain && (x_rows != x->n || x_cols != x->k || x_ld < x->k)) return fail("gemm_microscaled: plain rows [%lld, %lld] for [%d, %d]", x_rows, x_cols, x->n, x->k);
     if (to ? (to->bits != 8 || to->n != n_tok || to->k != w->n) : (out_rows != n_tok || out_cols != w->n))
         return fail("gemm_microscaled: the result is [%lld, %d]", n_tok, w->n);
-    if (to && (to->codes == x->codes || to->exponents == x->exponents)) return fail("gemm_microscaled: rows cannot be their own product");
     if (add && (to || out_dtype != RI_F32)) return fail("gemm_microscaled: sums are added to float32 numbers");
     if ((act != 0) + (add != 0) + (w2 != nullptr) > 1 || (add && constants)) return fail("gemm_microscaled: a bias, an activation, a gate and an addition are not combined");
     if ((act && !constants) || (constants && n_constants != (act ? 4 : w2 ? 5 : w->n)))

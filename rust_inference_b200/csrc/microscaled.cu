@@ -489,6 +489,7 @@ RI_API int ri_mx_make(void* at, void* codes, void* exponents, long long n, long 
     if (n <= 0 || k <= 0 || k > 0x7fffffffLL - SPAN || (bits != 4 && bits != 8)) return fail("mx_make: no [%lld, %lld] numbers of %d bits", n, k, bits);
     if ((n + 127) / 128 * 128 * spans((int)k) > 0x7fffffffLL / (SPAN / 8)) return fail("mx_make: [%lld, %lld] numbers are more than 2^31 eights", n, k);
     if ((uintptr_t)codes % 32 || (uintptr_t)exponents % 32) return fail("mx_make: buffers must begin on a 32-byte boundary");
+    if (!apart(codes, code_bytes(n, spans((int)k), bits), exponents, exponent_bytes(n, spans((int)k)))) return fail("mx_make: codes and exponents must lie apart");
     Held* h = new (at) Held;
     h->codes = (uint8_t*)codes;
     h->exponents = (uint8_t*)exponents;
@@ -505,6 +506,7 @@ RI_API int ri_mx_make(void* at, void* codes, void* exponents, long long n, long 
 RI_API int ri_mx_hold(const void* x, int dtype, long long n, long long k, long long ld, void* held, cudaStream_t stream) {
     const Held* h = (const Held*)held;
     if (n != h->n || k != h->k || ld < k) return fail("mx_hold: [%lld, %lld] numbers, rows %lld apart, do not go into [%d, %d]", n, k, ld, h->n, h->k);
+    if (!apart(h, x, ((n - 1) * ld + k) * item_bytes(dtype))) return fail("mx_hold: the numbers must lie apart from what holds them");
     if (int rc = on_device("mx_hold", h)) return rc;
     return dtype == RI_BF16 ? hold((const __nv_bfloat16*)x, ld, h, stream) : hold((const float*)x, ld, h, stream);
 }
@@ -519,6 +521,7 @@ RI_API int ri_mx_settle(cudaStream_t stream) {
 RI_API int ri_mx_values(const void* held, int dtype, long long n, long long k, void* out, cudaStream_t stream) {
     const Held* h = (const Held*)held;
     if (n != h->n || k != h->k) return fail("mx_values: [%d, %d] numbers do not go into [%lld, %lld]", h->n, h->k, n, k);
+    if (!apart(h, out, n * k * item_bytes(dtype))) return fail("mx_values: the numbers must lie apart from what holds them");
     if (int rc = on_device("mx_values", h)) return rc;
     return dtype == RI_BF16 ? values(h, (__nv_bfloat16*)out, stream) : values(h, (float*)out, stream);
 }
@@ -528,6 +531,8 @@ RI_API int ri_mx_rmsnorm(const float* x, const void* branch, int branch_dtype, c
                          void* held, cudaStream_t stream) {
     const Held* h = (const Held*)held;
     if (n != h->n || k != h->k || h->bits != 8) return fail("mx_rmsnorm: a norm of [%lld, %lld] does not go into [%d, %d] of %d bits", n, k, h->n, h->k, h->bits);
+    if (!apart(h, x, n * k * 4) || !apart(h, branch, n * k * item_bytes(branch_dtype)) || !apart(h, weight, k * 4) || !apart(h, total, n * k * 4))
+        return fail("mx_rmsnorm: the rows in 8 bits must lie apart from what is read and from the total");
     if (int rc = on_device("mx_rmsnorm", h)) return rc;
     return branch_dtype == RI_BF16 ? norm<__nv_bfloat16>(x, branch, weight, total, h, eps, stream)
                                    : norm<float>(x, branch, weight, total, h, eps, stream);

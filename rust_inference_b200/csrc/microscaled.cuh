@@ -34,6 +34,21 @@ struct Held {
 };
 
 __host__ __device__ __forceinline__ int spans(int k) { return (k + SPAN - 1) / SPAN; }
+
+// Whether two pieces of memory (or none, where one is null) have no byte in common.
+inline bool apart(const void* a, long long a_bytes, const void* b, long long b_bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a == nullptr || b == nullptr || x + (uintptr_t)a_bytes <= y || y + (uintptr_t)b_bytes <= x;
+}
+inline long long code_bytes(long long n, int n_spans, int bits) { return (bits == 4 ? (n + 127) / 128 * 128 * (SPAN / 2) : n * SPAN) * n_spans; }
+inline long long exponent_bytes(long long n, int n_spans) { return (n + 127) / 128 * n_spans * PIECE; }
+inline bool apart(const Held* h, const void* p, long long bytes) {
+    return apart(h->codes, code_bytes(h->n, h->n_spans, h->bits), p, bytes) && apart(h->exponents, exponent_bytes(h->n, h->n_spans), p, bytes);
+}
+inline bool apart(const Held* a, const Held* b) {
+    return apart(a, b->codes, code_bytes(b->n, b->n_spans, b->bits)) && apart(a, b->exponents, exponent_bytes(b->n, b->n_spans));
+}
+inline long long item_bytes(int dtype) { return dtype == RI_BF16 ? 2 : 4; }
 __device__ __forceinline__ size_t exponent_at(int row, int block, int n_spans) {
     return ((size_t)(row >> 7) * n_spans + (block >> 2)) * PIECE + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }

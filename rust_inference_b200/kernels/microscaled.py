@@ -53,7 +53,21 @@ def _maker():
     return lambda t: fn(t, make, size)
 
 
-class Matrix:
+class _NotPlain(KernelError, AttributeError):
+    pass
+
+
+class _Held:
+    """What matrices and rows have in common: they are no tensors, and a kernel that would take them for one refuses them."""
+
+    __slots__ = ()
+
+    def __getattr__(self, name):
+        raise _NotPlain(f"microscaled.{type(self).__name__} has no {name!r}: it is multiplied by the products of `kernels.linear` with matrices in 4 bits, "
+                        "not given to operators that take tensors (`microscaled.values` makes one of it)")
+
+
+class Matrix(_Held):
     """A weight matrix [n, k] in 4 bits, for the products of `kernels.linear`."""
 
     __slots__ = ("n", "k", "spans", "codes", "exponents", "device", "_described", "native")
@@ -90,7 +104,7 @@ class Matrix:
     def of_codes(cls, codes: torch.Tensor, exponents: torch.Tensor, k: int) -> "Matrix":
         """From codes uint8 [n, ceil(k / 2)], number 2i in the low half of byte i (the sign, then the place among 0, 0.5, 1, 1.5, 2, 3, 4, 6),
         and exponents plus 127, uint8 [n, ceil(k / 32)] (255: NaN)."""
-        n = codes.shape[0]
+        n = codes.shape[0] if codes.dim() == 2 else 0
         _need(codes.dtype == torch.uint8 and exponents.dtype == torch.uint8 and n > 0 and k > 0 and tuple(codes.shape) == (n, -(-k // 2))
               and tuple(exponents.shape) == (n, -(-k // BLOCK)), "microscaled.Matrix: codes uint8 [n, ceil(k / 2)] and exponents uint8 [n, ceil(k / 32)] are wanted")
         ops._need_cuda(codes, exponents)
@@ -116,7 +130,7 @@ class Matrix:
         return self.codes.numel() + self.exponents.numel()
 
 
-class Rows:
+class Rows(_Held):
     """Room for rows [n, k] in 8 bits, which a norm, a product or `quantize` fills and products read.  `codes` and `exponents`: buffers of
     the caller's own, uint8 and of `Rows.sizes(n, k)` bytes at least."""
 
@@ -161,6 +175,7 @@ def quantize(x: torch.Tensor, out: Rows | None = None) -> Rows:
 def values(held, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """The numbers [n, k] that a `Matrix` or `Rows` stands for, in float32 or bfloat16 (which hold them exactly, but for results that
     the type has no room for)."""
+    _need(type(held) is Matrix or type(held) is Rows, "microscaled.values: a Matrix or Rows are wanted")
     if out is None:
         _need(dtype in (torch.float32, torch.bfloat16), "microscaled.values: float32 or bfloat16 is wanted")
         return native("mx_values")(held.native, None, dtype is torch.bfloat16, held.n, held.k)

@@ -103,3 +103,65 @@ def test_an_infinite_gate(one_kernel, m, form):
     got = torch.isnan(microscaled.values(rows)).cpu()
     assert got[1, 32:64].all() and not got[0].any() and not got[1, :32].any() and not got[1, 64:].any()
     check_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 640), (16, 130, 333), (100, 256, 512), (300, 390, 1000)])
+def test_a_gelu_gate_with_a_factor(one_kernel, m, n, k):
+    """Every constant of a gate but the limit: out = mult g sigmoid(alpha g (1 + cubic g^2)) u."""
+    from rust_inference_b200.kernels import linear, microscaled
+    x, wg, wu = spread(m, k, 3 * m + k, wide=0.5), spread(n, k, n + k, wide=0.5) * 2 / math.sqrt(k), spread(n, k, n + k + 1, wide=0.5) / math.sqrt(k)
+    f = form_of("gelu")
+    g, gm = exact_product(x, wg)
+    u, um = exact_product(x, wu)
+    want = plain.gate(g, u, f)
+    eg, eu = ((k / 32 + 16) * 2.0 ** -23 * v for v in (gm, um))
+    # the slope of the gate is below 1.13, half of that here; the exponential's argument a has three roundings and its result 2 + 1.2 |a| units in the
+    # last place, which a term that it leaves counts: (1.2 + 2) |a| + 2, and 6 for the division and the products
+    a = (f[0] * g * (1 + f[3] * g * g)).abs()
+    off = 0.6 * eg * (u.abs() + eu) + 0.5 * g.abs() * eu + (4 * a.clamp(max=120) + 16) * 2.0 ** -23 * want.abs() + 1e-30
+    held = [microscaled.Matrix.of(w.to(DEV)) for w in (wg, wu)]
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.full((m, n), math.nan, dtype=dtype, device=DEV)
+        linear.gated(x.to(DEV), *held, out, context(dtype), form=f)
+        assert ((out.double() - want).abs() <= off + HALF_STEP[dtype] * want.abs() * 1.01).all()
+    rows = microscaled.Rows(m, n)
+    linear.gated(x.to(DEV), *held, rows, context(), form=f)
+    assert rows_near(microscaled.values(rows).double(), want, off)
+    check_status()
+
+
+@pytest.mark.parametrize("learned", [(0.3, -0.7), (-2.0, 1.5), None])
+@pytest.mark.parametrize("m", [1, 16, 130, 300])
+def test_an_activation_on_both_sides_of_its_pieces(one_kernel, m, learned):
+    """act(z) = a_p z^2 + l z above zero, a_n (e^z - 1 - z) + l z below, with a_p = softplus(p), a_n = 1/2 + softplus(q), l = 1/2 (None: the square of
+    relu), for z from -20 to 20, most of them near zero."""
+    from rust_inference_b200.kernels import linear, microscaled, ops
+    k, n = 500, 390
+    x, w = spread(m, k, m, wide=0.5), spread(n, k, 78, wide=0.7) / 40
+    if learned is None:
+        form, ap, an, lin = torch.tensor(ops.RELU_SQUARED_FORM, device=DEV), 1.0, 0.0, 0.0
+    else:
+        p, q = (float(torch.tensor(v)) for v in learned)
+        form, ap, an, lin = torch.tensor(learned, device=DEV), math.log1p(math.exp(p)), 0.5 + math.log1p(math.exp(q)), 0.5
+    z, mass = exact_product(x, w)
+    below = z < 0
+    if m > 1:
+        assert (z > 1).any() and (z < -1).any() and (z.abs() < 0.25).any() and ((z < -0.25) & (z > -1)).any()
+    t = torch.expm1(z.clamp(max=0)) - z.clamp(max=0)
+    curved = torch.where(below, an * t, ap * z * z)
+    want = curved + lin * z
+    dz = (k / 32 + 16) * 2.0 ** -23 * mass
+    slope = torch.where(below, torch.full_like(z, an + lin), 2 * ap * (z.abs() + dz) + lin) + an + lin
+    # constants off by 2^-22 (softplus), four roundings of each term; where the result is rounded to 8 or 16 bits, e^z - 1 - z from five terms above -1/4
+    # (2e-5 of it) and as a difference below: its terms are at most 1 + |z|, off by 2^-22 of that
+    off = slope * dz + 2.0 ** -21 * (curved.abs() + (lin * z).abs()) + 2.0 ** -22 * an * z.abs() * below
+    quick = off + an * (2e-5 * t + torch.where(z < -0.2, 2.0 ** -21 * (1 + z.abs()), 0.0 * z)) * below
+    held = microscaled.Matrix.of(w.to(DEV))
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.full((m, n), math.nan, dtype=dtype, device=DEV)
+        linear.activated(x.to(DEV), held, out, context(dtype), form)
+        assert ((out.double() - want).abs() <= (off if dtype is torch.float32 else quick) + HALF_STEP[dtype] * want.abs() * 1.01).all()
+    rows = microscaled.Rows(m, n)
+    linear.activated(x.to(DEV), held, rows, context(), form)
+    assert rows_near(microscaled.values(rows).double(), want, quick)
+    check_status()

@@ -41,6 +41,8 @@ class RMSNorm(Norm):
 
     def forward(self, x, out, rows=None):
         if type(out) is microscaled.Rows:
+            if rows is not None:
+                raise ops.KernelError("a norm into rows in 8 bits takes every row of its input, not a choice of them")
             return microscaled.rmsnorm(x, self.factor, self.eps, out)
         return ops.rmsnorm(x, self.factor, self.eps, out, rows)
 

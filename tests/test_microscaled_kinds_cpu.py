@@ -39,6 +39,15 @@ def test_operators_that_want_the_other_kind():
             call()
 
 
+def test_a_norm_of_chosen_rows():
+    """As many rows as there are, in another order: not the rows in 8 bits of all of them."""
+    from rust_inference_b200.parts.norm import RMSNorm
+    norm = RMSNorm(eps=1e-5, hidden_size=64, dtype=torch.bfloat16, device="cpu")
+    norm.set_tensors({"weight": torch.ones(64)})
+    with pytest.raises(KernelError, match="choice"):
+        norm.forward(torch.ones(3, 64), made(microscaled.Rows, 3, 64), rows=torch.tensor([2, 1, 0], dtype=torch.int32))
+
+
 def test_codes_of_other_shapes():
     codes, exponents = torch.zeros(4, 6, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8)
     for c, e in ((codes[0, 0], exponents), (codes[0], exponents), (codes[None], exponents), (codes, exponents[0]), (codes.int(), exponents), (codes[:0], exponents[:0])):

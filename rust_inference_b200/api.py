@@ -47,7 +47,9 @@ class Model:
         of max_seq_len, at most 65,536 positions).
         cache_dtype: "int8" keeps keys and values in 8 bits (see `Engine`); default: in `dtype`.
         weights_dtype: "mxfp4" holds the matrices of attention projections and dense feed-forwards in microscaled 4 bits (see
-        `kernels.microscaled`), whatever the file holds them in; default: in `dtype`.  Decoders that route to experts are refused."""
+        `kernels.microscaled`), whatever the file holds them in; default: in `dtype`.  Their products read activations rounded to
+        microscaled 8 bits (a number is off by 2^-4 of itself at most), whatever `dtype` is.  Decoders that route to experts are refused; small
+        models, whose steps are chains of short kernels, may take longer for a token than without."""
         from .config.registry import load_spec
         seq = resolve_max_seq_len(max_seq_len, load_spec(path)[1].max_positions)
         if max_tokens_in_cache is None:

@@ -19,7 +19,8 @@ Added for a library that takes token ids and may run without a checkpoint:
                                             generated tokens, seconds, tokens per second, bytes copied, the model's
                                             bytes on the device
   --cache-dtype int8                        keys and values in 8 bits instead of the run dtype
-  --weights-dtype mxfp4                     matrices of attention projections and dense feed-forwards in microscaled 4 bits
+  --weights-dtype mxfp4                     matrices of attention projections and dense feed-forwards in microscaled 4 bits, and what
+                                            they multiply in 8
   --score K                                 instead of generating: for every token of a prompt but the first one line with its
                                             id, its log probability, the entropy of its distribution and the K likeliest
                                             tokens; per prompt the perplexity on standard error
@@ -57,7 +58,7 @@ Options:
   --stop-ids         Stop token ids (default: the model's eos ids)
   --dtype            bfloat16 (default) or float32
   --cache-dtype      same (default: as --dtype) or int8: keys and values in 8 bits
-  --weights-dtype    same (default: as --dtype) or mxfp4: projections and dense feed-forwards in microscaled 4 bits
+  --weights-dtype    same (default: as --dtype) or mxfp4: projections and dense feed-forwards in microscaled 4 bits, what they multiply in 8
   --score            Score the prompts instead of generating; the number of alternatives to print per token
   --slots            Sequences live at once (default: as many as the cache holds)
   --print-logits-topk  Print the K largest logits after each prompt

@@ -5,7 +5,7 @@
 //   ri_mx_rmsnorm  total = stream + branch;  rows in 8 bits of  total / sqrt(mean(total^2) + eps) * weight
 //
 // All are bound by memory: [3584, 18944] from bfloat16 to 4 bits 36.5 us (4.7 TB/s), back 31.9 (5.4); the norm of 2,047 rows of 4,096 with a bfloat16
-// branch and the total 21.9 us (4.2; reading, one sum, writing, 3.5 rounds of blocks), of one row of 896 1.5, of 8 of 3,584 2.9: trips.
+// branch and the total 22 us (4.1; reading, one sum, writing, 3.5 rounds of blocks), without them 17.0, of one row of 896 1.5, of 8 of 3,584 2.4: trips.
 // A thread has eight consecutive numbers of a row (16 or 32 bytes in, 4 or 8 out), four neighbouring threads a block, whose largest magnitude two
 // exchanges find.
 #include "microscaled.cuh"
@@ -227,7 +227,9 @@ __device__ __forceinline__ uint32_t to_odd(double y) {
 
 // A block of threads per row.  Results are what the formula in 64 bits, rounded once, gives: what lies next to the middle of two numbers falls as the
 // formula says, not as a sum's last bits do.  The sum of squares and its root are in 64 bits; factors too, but only where 32 leave it open (32 bits
-// throughout: 2,047 rows of 4,096 without a branch 16.5 -> 14.9 us, few rows 0.1 to 0.4 less).  HELD: so many groups of eight per thread stay in
+// throughout: 2,047 rows of 4,096 without a branch 17.0 -> 14.8 us, with branch and total 22.1 -> 21.4; 8 of 3,584 2.4 -> 2.0, of which the sum and its root are
+// 0.15 and the factors 0.2; one of 896 1.5 -> 1.35.  Beside that the exchanges that find a block's largest are 0.1 to 0.2.  Into bfloat16 the same rows take
+// 12.4, 1.5 and 1.1).  HELD: so many groups of eight per thread stay in
 // registers between the two passes; longer rows are read again.
 template <typename B, int HELD, bool WHOLE>
 __global__ void __launch_bounds__(HELD == 1 ? 1024 : 512, HELD == 1 ? 1 : 2) rmsnorm_kernel(const float* stream, const B* branch, const float* __restrict__ weight, float* total, int k,
@@ -469,9 +471,9 @@ int norm(const float* x, const B* branch, const float* weight, float* total, con
     };
     return whole ? go(rmsnorm_kernel<B, HELD, true>) : go(rmsnorm_kernel<B, HELD, false>);
 }
-// Few rows are as fast as one of them, which many threads with one group each have sooner (8 rows of 3,584: one group 2.9 us, two 3.2; 148 of
-// 4,096 3.3 / 3.7); many are as fast as the SMs' instructions, of which two groups a thread take fewer (2,047 of 4,096: 25.8 / 22.7, with a branch
-// 4.1 TB/s).
+// Few rows are as fast as one of them, which many threads with one group each have sooner (us, one group / two: 8 rows of 3,584 2.4 / 2.7, 148 of
+// 4,096 2.6 / 3.25, 296 of them 4.0 / 4.4); many are as fast as the SMs' instructions, of which two groups a thread take fewer (330 of 4,096 5.7 / 5.55,
+// 600 8.1 / 7.5, 2,047 20.8 / 17.0, with branch and total 25.6 / 22.1).
 template <typename B>
 int norm(const float* x, const void* branch, const float* weight, float* total, const Held* h, double eps, cudaStream_t stream) {
     return h->n <= 2 * sm_count() ? norm<B, 1>(x, (const B*)branch, weight, total, h, eps, 1024, stream)

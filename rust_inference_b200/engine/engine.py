@@ -130,7 +130,8 @@ class Engine:
                         max_seq_len: int | None = None, n_slots: int | None = None,
                         use_graphs: bool = True, cache_dtype=None, weights_dtype=None) -> "Engine":
         """Load a model folder (config.json + safetensors); the model class comes from
-        config.json's architecture name.  weights_dtype: "mxfp4" holds matrices in 4 bits (see `DecoderModel`)."""
+        config.json's architecture name.  weights_dtype: "mxfp4" holds matrices in 4 bits, and rounds what they multiply to 8 (see
+        `DecoderModel`)."""
         weights_dtype = resolve_weights_dtype(weights_dtype)
         device = require_cuda(device)
         config, spec = load_spec(model_dir)

@@ -89,7 +89,8 @@ class LayerProbe:
 class DecoderModel:
     def __init__(self, spec: ModelSpec, *, dtype: torch.dtype, device, weights_dtype: str | None = None):
         """weights_dtype: None, matrices in the run dtype; "mxfp4": those of the parts that can, the attention's projections and the dense
-        feed-forwards, in microscaled 4 bits (`kernels.microscaled`), the others, embedding, head and vectors as without."""
+        feed-forwards, in microscaled 4 bits (`kernels.microscaled`), which multiply activations rounded to microscaled 8 bits, the others,
+        embedding, head and vectors as without."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"run dtype must be float32 or bfloat16, not {dtype}")
         self.spec = spec

@@ -3,7 +3,7 @@
 32 consecutive numbers of a row share a power of two, the smallest for which none of them exceeds the type's largest number times it, and
 each is kept as the nearest number of the type times that power, ties to the even one: in a matrix (`Matrix`) 4 bits, +-{0, 0.5, 1, 1.5, 2, 3,
 4, 6}, in rows of activations (`Rows`) 8, with four bits of exponent and three of mantissa, up to 448.  csrc/microscaled.cuh has the layout.
-A block that holds an infinity or a NaN stands for 32 NaNs.
+A block that holds an infinity or a NaN stands for 32 NaNs.  Whatever a product with a `Matrix` reads is in 8 bits then, in a float32 run too.
 
     w = microscaled.Matrix.of(t)                                  # [n, k] float32 or bfloat16, once, when a model is loaded
     w = microscaled.Matrix.of_codes(codes, exponents, k)          # from a file that holds such numbers already

@@ -82,6 +82,57 @@ def test_a_nan_in_either_factor_of_a_plain_gate(m, form):
     check_status()
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("m", [8, 700])
+def test_a_nan_in_either_factor_of_a_wide_plain_gate(m, form):
+    """In bfloat16, one token tile and many (on pairs of SMs too)."""
+    from rust_inference_b200.kernels import linear, tcgen05
+    k, n = 256, 1024
+    x, wg, wu = (spread(r, k, s, torch.bfloat16, 0.3).to(DEV) / math.sqrt(16) for r, s in ((m, 1), (n, 2), (n, 3)))
+    wg[5, 0], wu[1000, 3] = math.nan, math.nan
+    bad = torch.zeros(m, n, dtype=torch.bool, device=DEV)
+    bad[:, [5, 1000]] = True
+    for always in (False, True):
+        tcgen05.set_pairs(1, always=True) if always else tcgen05.set_pairs(0)
+        try:
+            out = torch.zeros(m, n, dtype=torch.bfloat16, device=DEV)
+            linear.gated(x, linear.Weight(wg), linear.Weight(wu), out, context(), form=form_of(form))
+        finally:
+            tcgen05.set_pairs()
+        assert torch.equal(torch.isnan(out), bad)
+    check_status()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_a_nan_in_either_factor_of_the_experts_gates(form):
+    """The experts' products, on the tensor cores (bfloat16) and without them."""
+    from rust_inference_b200.kernels import ops, tcgen05
+    experts, n, k, tokens = 3, 40, 64, 30
+    x = spread(tokens, k, 1, wide=0.3).to(DEV)
+    wg, wu = ((spread(experts * n, k, s, wide=0.3) / 8).view(experts, n, k).to(DEV) for s in (2, 3))
+    wg[1, 5, 0], wu[2, 33, 3] = math.nan, math.nan
+    ids = (torch.arange(tokens, dtype=torch.int32, device=DEV) % experts)[:, None].contiguous()
+    bad = torch.zeros(tokens, n, dtype=torch.bool, device=DEV)                      # by token
+    bad[1::3, 5] = True
+    bad[2::3, 33] = True
+    for dtype, cores in ((torch.float32, False), (torch.bfloat16, False), (torch.bfloat16, True)):
+        rows = tcgen05.GROUPED_TILE_ROWS if cores else ops.moe_tile_rows()
+        offsets, order, tiles, n_tiles, place = (torch.zeros(c, dtype=torch.int32, device=DEV)
+                                                 for c in (experts + 1, tokens, 2 * (-(-tokens // rows) + experts), 1, tokens))
+        ops.moe_arrange(ids, tokens, experts, rows, offsets, order, tiles, n_tiles, place)
+        out = torch.zeros(tokens, n, dtype=dtype, device=DEV)
+        mats = [w.to(dtype).contiguous() for w in (wg, wu)]
+        if cores:
+            xs = x.to(dtype)[order.long()].contiguous()
+            tcgen05.grouped_gemm(xs, *mats, out, offsets, tiles, n_tiles, n_pairs=tokens, gate_form=form_of(form))
+            got = torch.isnan(out)[place.long()]
+        else:
+            ops.moe_grouped_simt(x.to(dtype), *mats, out, offsets, order, tiles, n_tiles, n_pairs=tokens, top=1, gate_form=form_of(form))
+            got = torch.isnan(out)
+        assert torch.equal(got, bad)
+    check_status()
+
+
 @pytest.mark.parametrize("form", ["silu", "gelu", "steep"])
 @pytest.mark.parametrize("m", [2, 130, 300])
 def test_an_infinite_gate(one_kernel, m, form):
